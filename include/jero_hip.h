@@ -296,6 +296,83 @@ int jero_hip_gqa_attention(float *out_dev, const float *q_dev, const void *k_dev
                            int n_heads_q, int n_heads_kv, int head_dim, int64_t seq_len, float scale,
                            void *workspace_dev, size_t workspace_bytes, void *stream);
 
+/* ---- latent attention over a paged cache ----
+ * The attention of models whose cache holds one latent vector a token, shared by all heads
+ * (mla_absorbed_attention_f32, called from the DeepSeek2 recipe's sublayer,
+ * src/qwen_deepseek.rs:1099-1197, over the latent arena of src/kv.rs:413-455).  A position's cache
+ * row is [c | kp]: its normalised latent c[rank] and the rotated key part kp[rope_dim] all heads
+ * share.  Head h's key and value of position j are
+ *   k_j = [W_uk[h] c_j | kp_j],  v_j = W_uv[h] c_j     (W_uk[h]: nope_dim x rank, W_uv[h]: v_dim x rank)
+ * and a query [qn | qp] attends causally: out = sum_j softmax_j(scale * q . k_j) v_j over j <= its
+ * position, qp rotated to that position.  The rotation turns pairs (2i, 2i + 1) by
+ * position * rope_theta^(-2i / rope_dim), the angle computed in 64 bits.
+ *
+ * The cache is a pool of blocks of block_size positions; a sequence's table row names the block of
+ * each run of block_size positions, so a contiguous cache is one block per sequence.  A call's
+ * tokens are its last positions: sequence s has lens[s] positions with this call's tokens among
+ * them, and its tokens are rows starts[s] .. starts[s + 1] - 1 of x / q / out (starts NULL: row s,
+ * one token each, and n_tokens = n_seqs).  lens, starts and the table are read on the device, so a
+ * captured graph follows them from replay to replay.
+ *   - Token rows from starts[n_seqs] on belong to no sequence: they are not read, their outputs not
+ *     written.
+ *   - A position below 0 (a sequence with more tokens than positions) is not stored and attends to
+ *     nothing; a token that attends to nothing gets zeros.
+ *   - Positions from max_len on are neither stored nor attended to.
+ *   - A block id outside [0, n_blocks) is never followed: its positions are not stored, and masked.
+ * Two tokens of one call must not share a slot of the pool.  Sums are f32; with f32 activations the
+ * products carry 22 bits of each f32 factor (two f16 parts), with f16 activations intermediate
+ * queries, expanded keys and values, and softmax numerators are rounded to f16. */
+typedef struct jero_latent_cache {
+  void *rows_dev;            /* [n_blocks][block_size][rank + rope_dim] of kv_dtype, 16-byte aligned */
+  const int32_t *table_dev;  /* [n_seqs][table_stride] block ids */
+  const int32_t *lens_dev;   /* [n_seqs] */
+  const int32_t *starts_dev; /* [n_seqs + 1], not decreasing, or NULL */
+  int64_t n_blocks, table_stride, n_seqs;
+  int64_t max_len; /* at least 1, at most table_stride * block_size and JERO_MAX_LATENT_POSITIONS */
+  int block_size;  /* a power of two up to 2^20 */
+  int kv_dtype;    /* JERO_KV_F32 or JERO_KV_F16 */
+  int rank;        /* a multiple of 8 up to 512 */
+  int rope_dim;    /* a multiple of 8 up to 64 */
+} jero_latent_cache;
+#define JERO_MAX_LATENT_POSITIONS 4194304
+
+/* Stores the rows of n_tokens tokens: x_dev row t (x_stride elements apart, of act_dtype JERO_F32 or
+ * JERO_F16) is [xc | xp] as the down projection leaves it, and the cache row of its position becomes
+ * [RMSNorm(xc) * norm | rotated xp], rounded once to kv_dtype.  norm_dev: f32 [rank] (NULL: xc is
+ * stored as it is); eps the norm's; rope_theta 0: xp is stored as it is. */
+int jero_hip_mla_append(const jero_latent_cache *cache, int act_dtype, const void *x_dev, int64_t x_stride,
+                        int64_t n_tokens, const float *norm_dev, float eps, float rope_theta, void *stream);
+
+/* The absorbed form, for single tokens (or a few a sequence): q' = q_n W_uk attends to the latent
+ * rows themselves, and W_uv is applied to the attended latent.  q_dev: [n_tokens][n_heads][nope_dim
+ * + rope_dim] of act_dtype, rows q_stride elements apart, before the rotation (rope_theta 0: already
+ * rotated); out_dev: [n_tokens][n_heads][v_dim] of act_dtype, rows out_stride apart; k_b_dev:
+ * [n_heads][rank][nope_dim] f16, W_uk transposed; v_b_dev: [n_heads][v_dim][rank] f16.  nope_dim and
+ * v_dim multiples of 8 up to 256, strides multiples of 8, all 16-byte aligned; f16 activations need
+ * an f16 cache (CapabilityMismatch otherwise).  out may not overlap the inputs.  Workspace:
+ * jero_hip_mla_absorbed_workspace_bytes(...) bytes, 256-byte aligned (NULL: library-owned, calls must
+ * not overlap on one device). */
+size_t jero_hip_mla_absorbed_workspace_bytes(const jero_latent_cache *cache, int64_t n_tokens, int n_heads);
+int jero_hip_mla_absorbed_attention(const jero_latent_cache *cache, int act_dtype, const void *q_dev, int64_t q_stride,
+                                    int64_t n_tokens, int n_heads, int nope_dim, int v_dim, const void *k_b_dev,
+                                    const void *v_b_dev, float scale, float rope_theta, void *out_dev,
+                                    int64_t out_stride, void *workspace_dev, size_t workspace_bytes, void *stream);
+
+/* The expanded form, for prompts and chunks of them: keys and values of every position are made
+ * from the latent rows once, into the workspace, and each head attends in nope_dim + rope_dim.  As
+ * the absorbed form, with kv_b_dev: [n_heads][nope_dim + v_dim][rank] f16, a head's W_uk rows before
+ * its W_uv rows (nope_dim + rope_dim up to 256).  total_len: at least the sum of the lengths (each
+ * up to max_len); a sequence whose rows do not fit within total_len after those before it is treated
+ * as empty.  The keys and values of as many heads as the workspace holds are made at a time: it must
+ * hold one head's, jero_hip_mla_prefill_workspace_bytes(..., 1, ...), and the entry point's n_heads gives what
+ * holds them all up to 1 GiB. */
+size_t jero_hip_mla_prefill_workspace_bytes(const jero_latent_cache *cache, int act_dtype, int n_heads, int nope_dim,
+                                            int v_dim, int64_t total_len);
+int jero_hip_mla_prefill_attention(const jero_latent_cache *cache, int act_dtype, const void *q_dev, int64_t q_stride,
+                                   int64_t n_tokens, int n_heads, int nope_dim, int v_dim, const void *kv_b_dev,
+                                   int64_t total_len, float scale, float rope_theta, void *out_dev, int64_t out_stride,
+                                   void *workspace_dev, size_t workspace_bytes, void *stream);
+
 /* ---- routed experts ----
  * dispatch_qwen3_moe_ffn (src/qwen_deepseek.rs:847-951) from router logits, with
  * select_top_k_experts(logits, top_k, normalize = true) (src/gemma.rs:362-442) and

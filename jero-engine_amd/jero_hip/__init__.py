@@ -75,6 +75,13 @@ _SIGS = {
     "jero_hip_repack_gemm": (_I32, [_I32, _P, _SZ, _I64, _I64, _P, _SZ, C.POINTER(C.c_int), _P]),
     "jero_hip_repack_experts": (_I32, [_I32, _P, _SZ, _I64, _I64, _I64, _P, C.POINTER(C.c_int), _P]),
     "jero_hip_gqa_attention": (_I32, [_P, _P, _P, _P, _I32, _I32, _I32, _I32, _I64, _F, _P, _SZ, _P]),
+    "jero_hip_mla_append": (_I32, [_P, _I32, _P, _I64, _I64, _P, _F, _F, _P]),
+    "jero_hip_mla_absorbed_workspace_bytes": (_SZ, [_P, _I64, _I32]),
+    "jero_hip_mla_absorbed_attention": (_I32, [_P, _I32, _P, _I64, _I64, _I32, _I32, _I32, _P, _P, _F, _F, _P, _I64, _P,
+                                               _SZ, _P]),
+    "jero_hip_mla_prefill_workspace_bytes": (_SZ, [_P, _I32, _I32, _I32, _I32, _I64]),
+    "jero_hip_mla_prefill_attention": (_I32, [_P, _I32, _P, _I64, _I64, _I32, _I32, _I32, _P, _I64, _F, _F, _P, _I64, _P,
+                                              _SZ, _P]),
     "jero_hip_moe_ffn": (_I32, [_P, _P, _I64, _I64, _I32, _I32, _P, _SZ, _I32, _P, _SZ, _I32, _P, _SZ, _I64, _I64,
                                 _P, _P, _P, _P, _SZ, _P]),
     "jero_hip_moe_workspace_bytes": (_SZ, [_I64, _I64, _I32, _I64, _I64]),
@@ -494,6 +501,145 @@ def gqa_causal_attention_f32(out, q, k, v, n_heads_q, n_heads_kv, head_dim, seq_
     ws_n = workspace.numel() * workspace.element_size() if workspace is not None else 0
     check(lib().jero_hip_gqa_attention(_ptr(out), _ptr(q), _ptr(k), _ptr(v), kv_dtype, n_heads_q, n_heads_kv,
                                        head_dim, seq_len, scale, ws_p, ws_n, _stream(stream)))
+    return out
+
+
+class HipLatentCache(C.Structure):
+    """jero_latent_cache."""
+    _fields_ = [("rows_dev", C.c_void_p), ("table_dev", C.c_void_p), ("lens_dev", C.c_void_p), ("starts_dev", C.c_void_p),
+                ("n_blocks", C.c_int64), ("table_stride", C.c_int64), ("n_seqs", C.c_int64), ("max_len", C.c_int64),
+                ("block_size", C.c_int), ("kv_dtype", C.c_int), ("rank", C.c_int), ("rope_dim", C.c_int)]
+
+
+def _latent_check(cond, status, message):
+    if not cond:
+        raise K3Error(status, message)
+
+
+class LatentCache:
+    """A paged pool of latent rows (jero_latent_cache): ``rows`` [n_blocks, block_size, rank + rope_dim] f32 or
+    f16, ``table`` [n_seqs, blocks] int32 block ids, ``lens`` [n_seqs] int32 positions of each sequence with the
+    call's tokens among them, ``starts`` [n_seqs + 1] int32 first token row of each sequence (None: one token
+    each).  Device tensors, held and read as they are when a call runs; max_len (default: all a table row
+    holds) bounds the positions looked at.  The latent arena of src/kv.rs:413-455."""
+
+    def __init__(self, rows, table, lens, rank, starts=None, max_len=None):
+        import torch
+        held = [("rows", rows), ("table", table), ("lens", lens)] + ([("starts", starts)] if starts is not None else [])
+        for name, t in held:
+            _latent_check(t.is_cuda and t.device == rows.device, 21, f"LatentCache: {name} must be on the cache's GPU")
+            _latent_check(t.is_contiguous(), 21, f"LatentCache: {name} must be contiguous")
+            _latent_check(name == "rows" or t.dtype == torch.int32, 21, f"LatentCache: {name} must be int32")
+        _latent_check(rows.dtype in (torch.float32, torch.float16), 10, "LatentCache: rows must be float32 or float16")
+        _latent_check(rows.dim() == 3 and table.dim() == 2 and lens.dim() == 1, 14,
+                      "LatentCache: rows [blocks, block_size, width], table [seqs, blocks], lens [seqs]")
+        _latent_check(table.shape[0] == lens.shape[0], 14, "LatentCache: table and lens differ in sequences")
+        _latent_check(starts is None or starts.shape == (lens.shape[0] + 1,), 14, "LatentCache: starts must be [seqs + 1]")
+        _latent_check(0 < rank < rows.shape[2], 14, "LatentCache: rank must be below the rows' width")
+        self.rows, self.table, self.lens, self.starts, self.rank = rows, table, lens, starts, rank
+        if max_len is None:
+            max_len = table.shape[1] * rows.shape[1]
+        self.c = HipLatentCache(rows.data_ptr(), table.data_ptr(), lens.data_ptr(),
+                                starts.data_ptr() if starts is not None else None, rows.shape[0], table.shape[1],
+                                lens.shape[0], max_len, rows.shape[1], KV_F16 if rows.dtype == torch.float16 else KV_F32,
+                                rank, rows.shape[2] - rank)
+        self.ref = C.byref(self.c)
+
+
+def _latent_act(t, cache, what):
+    """act_dtype of a device tensor whose last dimensions are packed."""
+    import torch
+    _latent_check(t.is_cuda and t.device == cache.rows.device, 21, f"{what} must be on the cache's GPU")
+    if t.dtype == torch.float32:
+        return F32
+    _latent_check(t.dtype == torch.float16, 10, f"{what} must be float32 or float16")
+    return F16
+
+
+def _latent_stream(cache, stream):
+    """The stream's handle; a call runs on the current device, which has to be the cache's."""
+    if stream is None:
+        import torch
+        _latent_check(cache.rows.device.index == torch.cuda.current_device(), 21,
+                      "the cache must be on the current device")
+    else:
+        _latent_check(stream.device == cache.rows.device, 21, "the stream must be of the cache's device")
+    return _stream(stream)
+
+
+def mla_append(cache, x, norm, eps, rope_theta, stream=None):
+    """Stores the tokens' rows in the cache (jero_hip_mla_append): x [tokens, rank + rope_dim] f32 or f16 (rows
+    may be apart), its latent part RMS-normalised with the f32 weights ``norm`` (None: stored as it is), its key
+    part rotated to the token's position (rope_theta 0: stored as it is)."""
+    import torch
+    act = _latent_act(x, cache, "mla_append: x")
+    _latent_check(x.dim() == 2 and x.shape[1] == cache.rows.shape[2] and x.stride(1) == 1, 14,
+                  "mla_append: x must be [tokens, rank + rope_dim] with packed rows")
+    if norm is not None:
+        _latent_check(norm.dtype == torch.float32 and norm.device == x.device and norm.is_contiguous()
+                      and norm.numel() == cache.rank, 14, "mla_append: norm must be rank packed float32 values")
+    check(lib().jero_hip_mla_append(cache.ref, act, x.data_ptr(), x.stride(0) if x.shape[0] > 1 else x.shape[1],
+                                    x.shape[0], _ptr(norm), eps, rope_theta, _latent_stream(cache, stream)))
+
+
+def _latent_args(what, out, q, cache, weights, v_dim):
+    import torch
+    act = _latent_act(q, cache, f"{what}: q")
+    _latent_check(out.dtype == q.dtype and out.device == q.device, 21, f"{what}: out and q differ in type or device")
+    _latent_check(q.dim() == 3 and out.dim() == 3 and out.shape[:2] == q.shape[:2] and out.shape[2] == v_dim, 14,
+                  f"{what}: q must be [tokens, heads, nope + rope], out [tokens, heads, v]")
+    for t in (q, out):
+        _latent_check(t.stride(2) == 1 and t.stride(1) == t.shape[2], 21, f"{what}: a token's heads must be packed")
+    for w in weights:
+        _latent_check(w.dtype == torch.float16 and w.device == q.device and w.is_contiguous(), 21,
+                      f"{what}: weights must be packed float16 on the cache's GPU")
+    T, H, D = q.shape
+    return act, T, H, q.stride(0) if T > 1 else H * D, out.stride(0) if T > 1 else H * v_dim
+
+
+def _latent_workspace(workspace, need, like):
+    if workspace is None:
+        import torch
+        workspace = torch.empty(need, dtype=torch.uint8, device=like.device)
+    else:
+        _latent_check(workspace.device == like.device and workspace.is_contiguous(), 21,
+                      "workspace must be packed, on the cache's GPU")
+    return workspace, workspace.numel() * workspace.element_size()
+
+
+def mla_absorbed_attention(out, q, cache, k_b, v_b, scale, rope_theta, workspace=None, stream=None):
+    """Latent attention of single tokens, or a few a sequence, over the cache's rows as they are
+    (mla_absorbed_attention_f32, src/qwen_deepseek.rs:1099-1197; jero_hip_mla_absorbed_attention).  q [tokens,
+    heads, nope + rope_dim] f32 or f16 before the rotation; out [tokens, heads, v] of its type; k_b [heads, rank,
+    nope] and v_b [heads, v, rank] f16.  The rows of q and out may be apart.  The tokens' own rows have been
+    appended."""
+    what = "mla_absorbed_attention"
+    _latent_check(k_b.dim() == 3 and v_b.dim() == 3, 14, f"{what}: k_b must be [heads, rank, nope], v_b [heads, v, rank]")
+    act, T, H, qs, os_ = _latent_args(what, out, q, cache, (k_b, v_b), v_b.shape[1])
+    N = q.shape[2] - cache.c.rope_dim
+    _latent_check(tuple(k_b.shape) == (H, cache.rank, N) and tuple(v_b.shape) == (H, v_b.shape[1], cache.rank), 14,
+                  f"{what}: k_b must be [heads, rank, nope], v_b [heads, v, rank]")
+    L, s = lib(), _latent_stream(cache, stream)
+    ws, n = _latent_workspace(workspace, L.jero_hip_mla_absorbed_workspace_bytes(cache.ref, T, H), q)
+    check(L.jero_hip_mla_absorbed_attention(cache.ref, act, q.data_ptr(), qs, T, H, N, v_b.shape[1], k_b.data_ptr(),
+                                            v_b.data_ptr(), scale, rope_theta, out.data_ptr(), os_, ws.data_ptr(), n, s))
+    return out
+
+
+def mla_prefill_attention(out, q, cache, kv_b, total_len, scale, rope_theta, workspace=None, stream=None):
+    """Latent attention of prompts, or chunks of them, over keys and values made from the cache's rows
+    (jero_hip_mla_prefill_attention).  As mla_absorbed_attention, with kv_b [heads, nope + v, rank] f16 and
+    total_len at least the sum of the sequences' lengths."""
+    what = "mla_prefill_attention"
+    _latent_check(kv_b.dim() == 3 and out.dim() == 3, 14, f"{what}: kv_b must be [heads, nope + v, rank]")
+    V = out.shape[2]
+    act, T, H, qs, os_ = _latent_args(what, out, q, cache, (kv_b,), V)
+    N = q.shape[2] - cache.c.rope_dim
+    _latent_check(tuple(kv_b.shape) == (H, N + V, cache.rank), 14, f"{what}: kv_b must be [heads, nope + v, rank]")
+    L, s = lib(), _latent_stream(cache, stream)
+    ws, n = _latent_workspace(workspace, L.jero_hip_mla_prefill_workspace_bytes(cache.ref, act, H, N, V, total_len), q)
+    check(L.jero_hip_mla_prefill_attention(cache.ref, act, q.data_ptr(), qs, T, H, N, V, kv_b.data_ptr(), total_len,
+                                           scale, rope_theta, out.data_ptr(), os_, ws.data_ptr(), n, s))
     return out
 
 

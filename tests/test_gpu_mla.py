@@ -1,0 +1,434 @@
+"""Latent attention on the GPU: append, the absorbed and the expanded form against the 64-bit oracle.
+
+Pool rows that no sequence owns, and those past a length, hold NaN unless a test says otherwise, so
+a row read where it must not be shows in the output."""
+import numpy as np
+import pytest
+import torch
+
+import jero_hip as J
+from mla_oracle import EPS, THETA, Problem, off
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [("f32", "f16"), ("f16", "f16"), ("f32", "f32")]
+BIG = dict(rank=512, rope=64, nope=128, v=128)
+FORMS = ["absorbed", "expanded"]
+
+# lens, new, heads, block, widths: each edge of the tiles (16, 32, 64 positions; 16, 32, 64, 128 query rows),
+# pages that end inside one, sequences of one token and of none
+CASES = [
+    ([1], [1], 1, 16, {}),
+    ([2], [2], 3, 1, dict(rank=8, rope=8, nope=8, v=8)),
+    ([15, 16, 17], [1, 1, 1], 5, 4, {}),
+    ([31, 32, 33, 34], [1, 3, 0, 2], 4, 16, dict(rank=72, rope=24, nope=40, v=56)),
+    ([63, 64, 65], [1, 1, 1], 8, 64, dict(rank=128, rope=32, nope=64, v=64)),
+    ([127, 128, 129, 1], [2, 1, 1, 1], 20, 32, dict(rank=128, rope=32, nope=64, v=64)),
+    ([200, 5, 77], [1, 1, 1], 17, 16, BIG),
+    ([1000], [1], 65, 64, BIG),
+    ([515, 40], [1, 4], 128, 16, BIG),
+    ([300], [2], 33, 256, dict(rank=328, rope=40, nope=104, v=88)),
+    ([130, 131], [1, 1], 2, 8, dict(rank=512, rope=64, nope=256, v=256)),
+    ([90, 64], [1, 1], 3, 16, dict(rank=256, rope=64, nope=192, v=192)),
+]
+PROMPTS = [
+    ([130], [130], 2, 16, {}),
+    ([64, 65, 129], [64, 65, 129], 3, 32, dict(rank=128, rope=32, nope=64, v=64)),
+    ([300, 20, 257], [17, 20, 200], 2, 16, BIG),
+    ([97, 256], [31, 128], 3, 4, dict(rank=72, rope=24, nope=40, v=56)),
+    ([140], [140], 1, 64, dict(rank=256, rope=64, nope=192, v=256)),
+]
+
+
+def ids(case):
+    return "-".join(str(x) for x in case[0]) + f"_h{case[2]}_b{case[3]}_r{case[4].get('rank', 64)}"
+
+
+def problem(case, act="f32", kv="f16", **kw):
+    lens, new, heads, block, dims = case
+    return Problem(sum(lens) + heads, lens, new, heads=heads, block=block, act=act, kv=kv, **dims, **kw)
+
+
+def one_each(p):
+    return p.new == [1] * len(p.new)
+
+
+@pytest.mark.parametrize("act,kv", TYPES)
+@pytest.mark.parametrize("case", CASES + PROMPTS, ids=ids)
+@pytest.mark.parametrize("form", FORMS)
+def test_against_the_oracle(dev, form, case, act, kv):
+    print(f"mla {form} {act} {kv} {case}", flush=True)
+    if form == "expanded" and case[4].get("nope", 0) + case[4].get("rope", 0) > 256:
+        pytest.skip("refused: nope + rope above 256")
+    p = problem(case, act, kv, pad_rows=2)
+    p.device(dev)
+    ref = p.attention()
+    print("  off by", p.check(p.run(form), ref, form), flush=True)
+    if form == "absorbed" and one_each(p):  # a decode step: no starts
+        q = Problem(sum(case[0]) + case[2], *case[:2], heads=case[2], block=case[3], act=act, kv=kv, **case[4])
+        q.device(dev, starts=False)
+        q.check(q.run(form), what="without starts")
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_rows_that_attend_to_nothing_get_zeros(dev, form):
+    """An empty sequence, a sequence with more tokens than positions, and a sequence without tokens."""
+    p = Problem(5, [0, 3, 7, 40], [1, 5, 0, 2], heads=6, pad_rows=3).device(dev)
+    out = p.run(form)
+    p.check(out, what=form)
+    assert (out[0] == 0).all() and (out[1:3] == 0).all() and (out[3] != 0).any()
+
+
+@pytest.mark.parametrize("act,kv", TYPES)
+@pytest.mark.parametrize("form", FORMS)
+def test_bad_blocks_are_masked(dev, form, act, kv):
+    """Ids outside the pool are not followed: their positions are masked, all of them leave zeros."""
+    p = Problem(6, [100, 64, 20], [1, 2, 1], heads=5, act=act, kv=kv)
+    p.table[0, 2] = p.n_blocks
+    p.table[0, 4] = -1
+    p.table[1, 0] = 2 ** 31 - 1
+    p.table[2, :] = -(2 ** 31)
+    p.device(dev)
+    out = p.run(form)
+    p.check(out, what=form)
+    assert (out[3] == 0).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_positions_from_max_len_on_are_not_attended_to(dev, form):
+    p = Problem(7, [100, 30, 64], [3, 1, 1], heads=3, max_len=64).device(dev)
+    p.check(p.run(form), what=form)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_masked_places_may_hold_anything(dev, form):
+    """The rows past each length and the blocks of others hold infinities, or the type's lowest value."""
+    for rest in (np.inf, -np.inf, np.finfo(np.float16).min):
+        p = Problem(8, [50, 17, 129], [2, 1, 1], heads=4, rest=rest).device(dev)
+        p.check(p.run(form), what=f"{form} {rest}")
+
+
+@pytest.mark.parametrize("act,kv", TYPES)
+@pytest.mark.parametrize("form", FORMS)
+def test_peaked_scores(dev, form, act, kv):
+    """Queries 40 times as long: one position takes nearly all of a row, the rest underflow."""
+    p = Problem(9, [70, 200], [2, 1], heads=4, act=act, kv=kv, gain=60.0).device(dev)
+    p.check(p.run(form), what=form)
+
+
+def test_long_queries_and_far_positions(dev):
+    """Absorbed queries past f16's range (their scores are brought back by the scale), and the rotation at a
+    position where 32-bit angles are off by 1e-3."""
+    p = Problem(10, [40], [1], heads=4)
+    p.q *= np.float32(3e4)
+    p.scale = float(np.float32(p.scale / 3e4))
+    p.device(dev)
+    p.check(p.run("absorbed"), what="long queries")
+    far = Problem(11, [20001], [1], heads=2, block=256, rank=64, rope=64, max_len=20001).device(dev)
+    far.check(far.run("absorbed"), what="far position")
+    far.check(far.run("expanded"), what="far position")
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_rotated_queries(dev, form):
+    """rope_theta 0: the queries come rotated."""
+    p = Problem(12, [33, 80], [2, 1], heads=3).device(dev)
+    p.check(p.run(form, theta=0.0), p.attention(theta=0.0), form)
+    p.check(p.run(form, theta=5e5), p.attention(theta=5e5), form)
+
+
+@pytest.mark.parametrize("act", ["f32", "f16"])
+@pytest.mark.parametrize("form", FORMS)
+def test_strided_rows(dev, form, act):
+    """q and out as columns of wider rows: the columns beside out stay as they were."""
+    p = Problem(13, [33, 80], [5, 1], heads=3, act=act).device(dev)
+    D, V = p.H * (p.N + p.P), p.H * p.V
+    wide = torch.full((p.T, D + 24), float("nan"), dtype=p.d["q"].dtype, device=dev)
+    wide[:, 16:16 + D] = p.d["q"].view(p.T, D)
+    dst = torch.full((p.T, V + 16), 7.0, dtype=p.d["q"].dtype, device=dev)
+    q = wide[:, 16:16 + D].unflatten(1, (p.H, p.N + p.P))
+    out = p.run(form, out=dst[:, 8:8 + V].unflatten(1, (p.H, p.V)), q=q)
+    p.check(out, what=form)
+    assert (dst[:, :8] == 7).all() and (dst[:, 8 + V:] == 7).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_workspaces(dev, form):
+    """A caller's workspace, the library's own, and for the expanded form one that holds a single head's."""
+    p = Problem(14, [70, 131], [6, 1], heads=5, rank=128, rope=32, nope=64, v=64).device(dev)
+    ref = p.attention()
+    want = p.run(form)
+    p.check(want, ref, form)
+    L = J.lib()
+    if form == "absorbed":
+        need = L.jero_hip_mla_absorbed_workspace_bytes(p.cache.ref, p.T, p.H)
+    else:
+        need = L.jero_hip_mla_prefill_workspace_bytes(p.cache.ref, J.F32, 2, p.N, p.V, p.total())
+    ws = torch.full((need + 256,), 255, dtype=torch.uint8, device=dev)  # NaNs
+    got = p.run(form, workspace=ws[:need])
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and (ws[need:] == 255).all()
+    with pytest.raises(J.K3Error) as ei:
+        p.run(form, workspace=ws[:256])
+    assert ei.value.variant == "TensorBoundsError"
+    out = torch.zeros_like(want)
+    q, d = p.d["q"], p.d
+    if form == "absorbed":
+        J.check(L.jero_hip_mla_absorbed_attention(p.cache.ref, J.F32, q.data_ptr(), q.stride(0), p.T, p.H, p.N, p.V,
+                                                  d["k_b"].data_ptr(), d["v_b"].data_ptr(), p.scale, THETA,
+                                                  out.data_ptr(), out.stride(0), None, 0, J._stream()))
+    else:
+        J.check(L.jero_hip_mla_prefill_attention(p.cache.ref, J.F32, q.data_ptr(), q.stride(0), p.T, p.H, p.N, p.V,
+                                                 d["kv_b"].data_ptr(), p.total(), p.scale, THETA, out.data_ptr(),
+                                                 out.stride(0), None, 0, J._stream()))
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+def test_sequences_past_total_len_are_empty(dev):
+    p = Problem(15, [40, 100, 30], [2, 3, 1], heads=3).device(dev)
+    out = p.run("expanded", total=75)  # the second does not fit behind the first, the third does
+    want = p.run("expanded")
+    torch.cuda.synchronize()
+    assert torch.equal(out[:2], want[:2]) and (out[2:5] == 0).all() and torch.equal(out[5], want[5])
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_same_calls_give_the_same_bits(dev, form):
+    p = Problem(16, [700, 90], [3, 1], heads=20, **BIG).device(dev)
+    a, b = p.run(form), p.run(form)
+    torch.cuda.synchronize()
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_a_captured_call_follows_lengths_and_tables(dev, form):
+    """Replayed as the sequences grow and as a block moves, each replay against an eager call, with eager work
+    in between."""
+    p = Problem(17, [90, 33], [1, 1], heads=4, max_len=128, block=16)
+    for s, n in enumerate(p.lens):  # blocks for what will be appended
+        p.table[s, :8] = np.arange(8) + 8 * s
+    g = np.random.default_rng(1)
+    p.n_blocks = 17
+    p.rows = g.standard_normal((17, 16, p.R + p.P)).astype(np.float16)
+    p.device(dev)
+    out = torch.zeros((p.T, p.H, p.V), device=dev)
+    L = J.lib()
+    need = max(L.jero_hip_mla_absorbed_workspace_bytes(p.cache.ref, p.T, p.H),
+               L.jero_hip_mla_prefill_workspace_bytes(p.cache.ref, J.F32, p.H, p.N, p.V, 256))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    kw = {} if form == "absorbed" else dict(total=256)
+    s = torch.cuda.Stream(dev)
+    with torch.cuda.stream(s):
+        p.run(form, out=out, workspace=ws, **kw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        J.mla_append(p.cache, p.d["x"], p.d["norm"], EPS, THETA)
+        p.run(form, out=out, workspace=ws, **kw)
+    for step in range(5):
+        p.lens = [91 + step, 34 + 17 * step]
+        p.d["lens"].copy_(torch.tensor(p.lens, dtype=torch.int32))
+        if step == 3:  # the first sequence's block 2 moves to the spare one
+            p.d["rows"][16] = p.d["rows"][int(p.table[0, 2])]
+            p.table[0, 2] = 16
+            p.d["table"].copy_(torch.from_numpy(p.table))
+        p.d["x"].copy_(torch.from_numpy(g.standard_normal(p.x.shape).astype(np.float32)))
+        p.q = g.standard_normal(p.q.shape).astype(np.float32)
+        p.d["q"].copy_(torch.from_numpy(p.q))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        p.rows = p.d["rows"].cpu().numpy()
+        p.check(out, what=f"{form} step {step}")
+        eager = p.run(form, **kw)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, out)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_two_streams_at_once(dev, form):
+    """Two calls that overlap, each with a workspace of its own."""
+    ps = [Problem(18 + i, [400 + 50 * i], [1 + i], heads=8, rank=128, rope=32, nope=64, v=64).device(dev) for i in range(2)]
+    want = [p.run(form).clone() for p in ps]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(dev) for _ in ps]
+    for _ in range(5):
+        got = []
+        for p, s in zip(ps, streams):
+            with torch.cuda.stream(s):
+                got.append(p.run(form))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    s = streams[0]
+    out = ps[0].run(form, stream=s)
+    s.synchronize()
+    assert torch.equal(out, want[0])
+
+
+# ---------------------------------------------------------------- append
+
+
+def check_rows(p, rows, before, ref, hit):
+    got = rows.float().cpu().numpy().astype(np.float64)
+    old = before.astype(np.float64)
+    assert np.array_equal(got[~hit], old[~hit], equal_nan=True), "rows of no token were written"
+    half = 2.0 ** -11 if p.kv == "f16" else 2.0 ** -24
+    # the stored value's half step; the f32 arithmetic before it: the mean of squares (rank sums), its root and
+    # quotient and two products for the latent, two products and a sum of the pair's length for the key part
+    slack = 2.0 ** -24 * (6 + np.sqrt(p.R))
+    pair = np.abs(ref[hit])
+    k = pair[:, p.R:].reshape(len(pair), -1, 2)
+    pair[:, p.R:] = np.repeat(np.sqrt((k ** 2).sum(-1)), 2, -1)
+    far = half * np.abs(ref[hit]) + slack * pair + (2.0 ** -25 if p.kv == "f16" else 0)
+    assert (np.abs(got[hit] - ref[hit]) <= far).all()
+
+
+APPENDS = [
+    ([1], [1], 16, {}), ([5, 17, 64], [5, 1, 33], 16, {}), ([300, 2, 0], [300, 2, 0], 64, BIG),
+    ([20, 3], [4, 3], 1, dict(rank=8, rope=8)), ([100, 50], [100, 7], 32, dict(rank=328, rope=24)),
+    ([16, 33], [2, 5], 8, dict(rank=504, rope=56)),
+]
+
+
+@pytest.mark.parametrize("act,kv", TYPES + [("f16", "f32")])
+@pytest.mark.parametrize("case", APPENDS, ids=lambda c: f"{c[0]}_{c[2]}")
+def test_append(dev, case, act, kv):
+    lens, new, block, dims = case
+    print(f"mla_append {act} {kv} {case}", flush=True)
+    p = Problem(21, lens, new, block=block, act=act, kv=kv, pad_rows=2, **dims).device(dev)
+    J.mla_append(p.cache, p.d["x"], p.d["norm"], EPS, THETA)
+    check_rows(p, p.d["rows"], p.rows, *p.appended())
+    p.device(dev)
+    J.mla_append(p.cache, p.d["x"], None, 0.0, 0.0)  # stored as they are
+    check_rows(p, p.d["rows"], p.rows, *p.appended(theta=0, norm=False))
+
+
+@pytest.mark.parametrize("act", ["f32", "f16"])
+@pytest.mark.parametrize("before", [1, 3, 8])
+def test_append_columns_of_wider_rows(dev, act, before):
+    """x at any offset and stride of its elements."""
+    p = Problem(22, [40, 9], [13, 9], act=act).device(dev)
+    wide = torch.full((p.T, before + p.R + p.P + 5), float("nan"), dtype=p.d["x"].dtype, device=dev)
+    wide[:, before:before + p.R + p.P] = p.d["x"]
+    J.mla_append(p.cache, wide[:, before:before + p.R + p.P], p.d["norm"], EPS, THETA)
+    check_rows(p, p.d["rows"], p.rows, *p.appended())
+
+
+def test_append_leaves_out_what_has_no_slot(dev):
+    """Positions below 0 and from max_len on, and blocks outside the pool."""
+    p = Problem(23, [3, 70, 40], [6, 20, 40], max_len=60, rest=0.5)
+    p.table[2, 1] = p.n_blocks + 5
+    p.table[1, 3] = -1
+    p.device(dev)
+    J.mla_append(p.cache, p.d["x"], p.d["norm"], EPS, THETA)
+    check_rows(p, p.d["rows"], p.rows, *p.appended())
+
+
+def test_append_far_and_zero_rows(dev):
+    """A row of zeros stays zeros (eps), and the rotation holds at the longest context."""
+    p = Problem(24, [131072], [2], block=1 << 17, rank=16, rope=64, rest=0.0)
+    p.x[0, :16] = 0
+    p.device(dev)
+    J.mla_append(p.cache, p.d["x"], p.d["norm"], EPS, THETA)
+    check_rows(p, p.d["rows"], p.rows, *p.appended())
+
+
+def test_slots_past_32_bits(dev):
+    """A pool of more than 4 GiB: rows whose element and byte offsets do not fit 32 bits are written and read."""
+    R, P, bs = 512, 64, 1 << 16
+    n = 60  # 60 * 65536 * 576 = 2.26e9 elements, 4.5e9 bytes
+    rows = torch.empty((n, bs, R + P), dtype=torch.float16, device=dev)
+    table = torch.tensor([[n - 1]], dtype=torch.int32, device=dev)
+    p = Problem(25, [80], [80], block=1 << 16, heads=2, **BIG)
+    low = Problem(25, [80], [80], block=1 << 16, heads=2, **BIG).device(dev)
+    p.d = dict(low.d, rows=rows, table=table)
+    rows[n - 1, :80] = low.d["rows"][int(low.table[0, 0]), :80]
+    p.cache = J.LatentCache(rows, table, low.d["lens"], R, starts=low.d["starts"], max_len=80)
+    for form in FORMS:
+        a, b = p.run(form), low.run(form)
+        torch.cuda.synchronize()
+        assert torch.equal(a, b)
+    J.mla_append(p.cache, p.d["x"], p.d["norm"], EPS, THETA)
+    J.mla_append(low.cache, low.d["x"], low.d["norm"], EPS, THETA)
+    assert torch.equal(rows[n - 1, :80], low.d["rows"][int(low.table[0, 0]), :80])
+
+
+# ---------------------------------------------------------------- together
+
+
+@pytest.mark.parametrize("act,kv", TYPES)
+def test_a_prompt_and_its_decode_steps(dev, act, kv):
+    """As a model's layer runs them: prompts appended and attended to in the expanded form, then tokens one at
+    a time in the absorbed form; every step against the oracle over the rows the cache then holds, and the last
+    tokens' outputs against the expanded form of the same queries."""
+    p = Problem(30, [37, 60], [37, 60], heads=6, act=act, kv=kv, rank=128, rope=32, nope=64, v=64, max_len=96)
+    g = np.random.default_rng(2)
+    p.table[:] = np.random.default_rng(3).permutation(12).reshape(2, 6)
+    p.n_blocks = 12
+    p.rows = np.full((12, 16, 160), np.nan, p.rows.dtype)
+    p.device(dev)
+    J.mla_append(p.cache, p.d["x"], p.d["norm"], EPS, THETA)
+    ref, hit = p.appended()
+    check_rows(p, p.d["rows"], p.rows, ref, hit)
+    p.rows = p.d["rows"].cpu().numpy()
+    p.check(p.run("expanded"), what="prompt")
+    for step in range(3):
+        p.lens = [n + 1 for n in p.lens]
+        p.new, p.T = [1, 1], 2
+        p.starts = np.array([0, 1, 2], np.int32)
+        p.x = (g.standard_normal((2, 160)) * 1.7).astype(p.x.dtype)
+        p.q = (g.standard_normal((2, 6, 96)) * 1.5).astype(p.q.dtype)
+        p.device(dev, starts=False)
+        J.mla_append(p.cache, p.d["x"], p.d["norm"], EPS, THETA)
+        p.rows = p.d["rows"].cpu().numpy()
+        a = p.run("absorbed")
+        p.check(a, what=f"step {step}")
+        p.cache = J.LatentCache(p.d["rows"], p.d["table"], p.d["lens"], p.R, starts=torch.from_numpy(p.starts).to(dev),
+                                max_len=p.max_len)
+        b = p.run("expanded")
+        p.check(b, what=f"step {step}")
+        exact, bounds = p.attention()
+        assert off(a.double().cpu().numpy(), b.double().cpu().numpy(), 2 * bounds)[0] <= 1
+
+
+def test_refusals_of_the_python_front_end(dev):
+    p = Problem(31, [20], [2]).device(dev)
+    d, c = p.d, p.cache
+    out = torch.zeros((2, 4, 40), device=dev)
+
+    def refused(variant, fn):
+        with pytest.raises(J.K3Error) as ei:
+            fn()
+        assert ei.value.variant == variant
+
+    A = lambda **k: J.mla_absorbed_attention(k.get("out", out), k.get("q", d["q"]), c, k.get("k_b", d["k_b"]),  # noqa: E731
+                                             k.get("v_b", d["v_b"]), 0.1, k.get("theta", THETA))
+    E = lambda **k: J.mla_prefill_attention(k.get("out", out), k.get("q", d["q"]), c, k.get("kv_b", d["kv_b"]),  # noqa: E731
+                                            k.get("total", 20), 0.1, THETA)
+    for call in (A, E):
+        refused("InvalidArgument", lambda: call(out=out.half()))
+        refused("InvalidArgument", lambda: call(q=d["q"].cpu()))
+        refused("CapabilityMismatch", lambda: call(q=d["q"].double(), out=out.double()))
+        refused("TensorBoundsError", lambda: call(out=out[:1]))
+        refused("InvalidArgument", lambda: call(q=d["q"].transpose(1, 2).contiguous().transpose(1, 2)))
+        refused("TensorBoundsError", lambda: call(q=d["q"][:0], out=out[:0]))
+    refused("InvalidArgument", lambda: A(k_b=d["k_b"].float()))
+    refused("TensorBoundsError", lambda: A(k_b=d["k_b"][:3]))
+    refused("TensorBoundsError", lambda: A(v_b=d["v_b"][:, :, :56].contiguous()))
+    refused("InvalidArgument", lambda: A(theta=-1.0))
+    refused("TensorBoundsError", lambda: E(kv_b=d["kv_b"][:, :70].contiguous()))
+    refused("TensorBoundsError", lambda: E(total=0))
+    refused("TensorBoundsError", lambda: J.mla_append(c, d["x"][:, :79], d["norm"], EPS, THETA))
+    refused("TensorBoundsError", lambda: J.mla_append(c, d["x"], d["norm"][:60], EPS, THETA))
+    refused("InvalidArgument", lambda: J.mla_append(c, d["x"].cpu(), d["norm"], EPS, THETA))
+    refused("InvalidArgument", lambda: J.mla_append(c, d["x"], d["norm"], -1.0, THETA))
+    T = torch
+    for kw, variant in ((dict(rows=d["rows"].double()), "CapabilityMismatch"), (dict(table=d["table"].long()), "InvalidArgument"),
+                        (dict(lens=d["lens"].cpu()), "InvalidArgument"), (dict(rank=80), "TensorBoundsError"),
+                        (dict(starts=T.zeros(3, dtype=T.int32, device=dev)), "TensorBoundsError"),
+                        (dict(table=d["table"][:, :1].expand(-1, 4)), "InvalidArgument")):
+        a = dict(rows=d["rows"], table=d["table"], lens=d["lens"], rank=64)
+        a.update(kw)
+        refused(variant, lambda: J.LatentCache(**a))
