@@ -47,103 +47,714 @@ __global__ void __launch_bounds__(256) mla_append_kernel(LatentCache c, const X*
 }
 
 // ---------------------------------------------------------------- absorbed attention
+//
+// Three launches.  mla_absorb_kernel makes the absorbed queries q' = [q_n W_uk | rotated q_p] and the
+// plan; mla_attend_kernel reads every cache row once for up to 64 heads, with a running maximum and
+// sum, and leaves one partial row per (run of tiles, token, head); mla_values_kernel merges a token's
+// partials and applies W_uv.
+//
+// The plan cuts the tiles of all tokens, one after the other, into equal runs, one per workgroup and
+// group of heads, so that ragged lengths fill the chip: with splits of equal length per token, 32
+// sequences of 900 to 6000 positions leave half the workgroups short.  Run w of token t writes partial
+// w + t: along the runs either w or t grows, so the number names the pair.
 
-// q'[t][h] = [ q_n W_uk[h] | rotated q_p ] in f32, one workgroup per (token, head).
+typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef short s4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kMlaRuns = 256;  // workgroups of the attend kernel: one per CU, its tiles fill the LDS
+
+struct MlaPlan {
+  int* prefix;  // [T + 1] tiles before each token
+  int* seq;     // [T] sequence, -1 for a row of none
+  int* end;     // [T] positions attended to
+};
+
+// Sequence and position of token t by one thread (mla_locate is a wave's).
+__device__ __forceinline__ bool mla_locate_thread(const LatentCache& c, int t, int& seq, int& pos) {
+  if (!c.starts) {
+    seq = t;
+    pos = c.lens[t] - 1;
+    return true;
+  }
+  int lo = 0, hi = c.n_seqs + 1;  // starts below lo are <= t, those from hi on are not
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (c.starts[mid] <= t) lo = mid + 1;
+    else hi = mid;
+  }
+  seq = lo - 1;
+  if (seq < 0 || seq >= c.n_seqs) return false;
+  pos = int(int64_t(c.lens[seq]) - c.starts[seq + 1] + t);
+  return true;
+}
+
+__device__ __forceinline__ f4_t mfma(h8_t a, h8_t b, f4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// x as two f16 parts, hi + lo = x to 22 bits.
+__device__ __forceinline__ void split2(float x, _Float16& hi, _Float16& lo) {
+  hi = _Float16(x);
+  lo = _Float16(x - float(hi));
+}
+
 template <typename X>
+__device__ __forceinline__ void load8(const X* p, float (&v)[8]);
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+template <>
+__device__ __forceinline__ void load8<_Float16>(const _Float16* p, float (&v)[8]) {
+  const h8_t a = *reinterpret_cast<const h8_t*>(p);
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] = float(a[e]);
+}
+
+// Grid (tiles of 64 latent columns, then one for the key part, then one for the plan; heads; tokens by
+// 64).  A wave holds 16 rows of W_uk^T in registers and takes the tokens 16 at a time: one read of the
+// weights for 64 tokens, which is all this kernel costs for a few.  f32 queries go in as two f16 parts.
+template <typename X, int NT>
 __global__ void __launch_bounds__(256) mla_absorb_kernel(LatentCache c, const X* __restrict__ q, int64_t q_stride,
                                                          int nope, const _Float16* __restrict__ k_b, MlaRope rope,
-                                                         float* __restrict__ qa) {
-  const int t = blockIdx.x, h = blockIdx.y, nh = gridDim.y;
-  int seq, pos;
-  if (!mla_locate(c, t, threadIdx.x & 63, seq, pos)) return;
-  const X* qr = q + t * q_stride + int64_t(h) * (nope + c.rope);
-  float* o = qa + (int64_t(t) * nh + h) * c.width;
-  for (int r = threadIdx.x; r < c.rank; r += 256) {
+                                                         float* __restrict__ qa, MlaPlan plan, int tile) {
+  const int h = blockIdx.y, nh = gridDim.y, t0 = blockIdx.z * 64;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int nr = (c.rank + 63) / 64;
+  const int64_t qh = int64_t(h) * (nope + c.rope);
+  if (int(blockIdx.x) < nr) {
+    const int g = lane >> 4, col = lane & 15;
+    const int r0 = blockIdx.x * 64 + wv * 16;
+    if (r0 >= c.rank) return;
+    const int r = min(r0 + col, c.rank - 1);
     const _Float16* w = k_b + (int64_t(h) * c.rank + r) * nope;
-    float s = 0.f;
-    for (int n = 0; n < nope; n++) s += float(qr[n]) * float(w[n]);
-    o[r] = s;
+    h8_t b[NT];
+#pragma unroll
+    for (int i = 0; i < NT; i++) b[i] = *reinterpret_cast<const h8_t*>(w + min(32 * i + 8 * g, nope - 8));
+    for (int t = t0; t < min(t0 + 64, c.n_tokens); t += 16) {
+      const X* qr = q + min(t + col, c.n_tokens - 1) * q_stride + qh;
+      f4_t hi = {0.f, 0.f, 0.f, 0.f}, lo = hi;
+#pragma unroll
+      for (int i = 0; i < NT; i++) {
+        float v[8];
+        load8<X>(qr + min(32 * i + 8 * g, nope - 8), v);
+        h8_t ah, al;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          _Float16 x, y;
+          split2(32 * i + 8 * g < nope ? v[e] : 0.f, x, y);
+          ah[e] = x, al[e] = y;
+        }
+        hi = mfma(ah, b[i], hi);
+        if (sizeof(X) == 4) lo = mfma(al, b[i], lo);
+      }
+      if (r0 + col < c.rank)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (t + 4 * g + e < c.n_tokens) qa[(int64_t(t + 4 * g + e) * nh + h) * c.width + r0 + col] = hi[e] + lo[e];
+    }
+    return;
   }
-  if (int(threadIdx.x) < c.rope / 2) {
-    const int i = threadIdx.x;
-    const float a = float(qr[nope + 2 * i]), b = float(qr[nope + 2 * i + 1]);
-    const float2 cs = rope.on ? mla_cos_sin(rope, i, pos) : make_float2(1.f, 0.f);
-    o[c.rank + 2 * i] = a * cs.x - b * cs.y;
-    o[c.rank + 2 * i + 1] = a * cs.y + b * cs.x;
+  if (int(blockIdx.x) == nr) {  // the key part
+    __shared__ int s_pos[64];
+    if (tid < 64) {
+      int seq, pos = -1;
+      if (t0 + tid < c.n_tokens && !mla_locate_thread(c, t0 + tid, seq, pos)) pos = -1;
+      s_pos[tid] = pos;
+    }
+    __syncthreads();
+    const int pairs = c.rope / 2, n = min(64, c.n_tokens - t0) * pairs;
+    for (int k = tid; k < n; k += 256) {
+      const int t = k / pairs, i = k % pairs;
+      const X* qr = q + (t0 + t) * q_stride + qh + nope + 2 * i;
+      const float x = float(qr[0]), y = float(qr[1]);
+      const float2 cs = rope.on ? mla_cos_sin(rope, i, s_pos[t]) : make_float2(1.f, 0.f);
+      float* o = qa + (int64_t(t0 + t) * nh + h) * c.width + c.rank + 2 * i;
+      o[0] = x * cs.x - y * cs.y;
+      o[1] = x * cs.y + y * cs.x;
+    }
+    return;
+  }
+  if (h || t0) return;
+  // the plan: 256 tokens at a time, a scan of their tiles
+  __shared__ int s_scan[4];
+  int base = 0;
+  for (int first = 0; first < c.n_tokens; first += 256) {
+    const int t = first + tid;
+    int seq = -1, pos = -1, end = 0;
+    if (t < c.n_tokens) {
+      if (!mla_locate_thread(c, t, seq, pos)) seq = -1, pos = -1;
+      end = pos < 0 ? 0 : min(int(min(int64_t(pos) + 1, int64_t(c.max_len))), c.max_len);
+    }
+    const int mine = (end + tile - 1) / tile;
+    int sum = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int v = __shfl_up(sum, off, 64);
+      if (lane >= off) sum += v;
+    }
+    if (lane == 63) s_scan[wv] = sum;
+    __syncthreads();
+    int before = base;
+    for (int w = 0; w < wv; w++) before += s_scan[w];
+    const int all = s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
+    if (t < c.n_tokens) {
+      plan.prefix[t] = before + sum - mine;
+      plan.seq[t] = seq;
+      plan.end[t] = end;
+    }
+    base += all;
+    __syncthreads();
+  }
+  if (tid == 0) plan.prefix[c.n_tokens] = base;
+}
+
+// Tiles of a run: the plan's tiles over the runs, at least `least` each.
+__device__ __forceinline__ int mla_per_run(int tiles, int runs, int least) { return max((tiles + runs - 1) / runs, least); }
+
+// The last token whose prefix is not behind tile x, 64 candidates at a time.
+__device__ __forceinline__ int mla_token_of(const int* prefix, int n, int x, int lane) {
+  int lo = 0, len = n;  // the answer is in [lo, lo + len)
+  while (len > 1) {
+    const int step = (len + 63) / 64;
+    const int i = lo + lane * step;
+    const bool below = i < lo + len && prefix[i] <= x;
+    const int k = max(__popcll(__ballot(below)) - 1, 0);
+    const int at = lo + k * step;
+    len = min(step, lo + len - at);
+    lo = at;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ float max_over_groups(float v) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+  v = fmaxf(v, __shfl_xor(v, 16, kWave));
+  return fmaxf(v, __shfl_xor(v, 32, kWave));
+}
+__device__ __forceinline__ float sum_over_groups(float v) {
+  v += __shfl_xor(v, 16, kWave);
+  return v + __shfl_xor(v, 32, kWave);
+}
+
+// 16 bytes a lane straight from global memory to LDS, lane l's to base + 16 l: the loads in flight take no
+// registers.  The compiler does not know of these loads; dma_wait waits for the wave's own, and a barrier
+// then shows them to the others.
+__device__ __forceinline__ void dma_row(const void* row, uint32_t lane_bytes, uint32_t lds) {  // uniform row
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(lane_bytes), "s"(row)
+               : "memory");
+}
+__device__ __forceinline__ void dma_lanes(const void* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
+}
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+typedef __attribute__((address_space(3))) s4_t lds_s4;
+
+// Shape of the attend kernel: HG waves of 16 heads by KS waves of WR positions, RT + PT the padded widths,
+// KV the cache's type.  LDS holds a step's rows in f16: the latents RPI rows to 1024 bytes, with 16 bytes
+// after each 1024 so that 16 rows fall on all banks (RPI > 1: the rows of one 1024 swap their 16-byte chunks
+// by their number instead), then the key parts, whose chunks are swapped the same way.  An f16 cache is
+// loaded straight into one of two such buffers; an f32 cache into a raw buffer, from which each wave turns
+// its rows into a buffer of their upper and one of their lower parts.
+template <int RT, int PT, int HG, int KS, int WR, typename KV>
+struct AttendShape {
+  static constexpr bool kWide = sizeof(KV) == 4;
+  static constexpr int kWaves = HG * KS;
+  static constexpr int kTile = WR * KS;  // positions a step
+  static constexpr int kRows = kTile / kWaves;  // rows a wave loads
+  static constexpr int RPI = 512 / RT;
+  static constexpr int kLat = kTile / RPI * 1040;
+  static constexpr int kBuf = kLat + kTile * PT * 2;
+  static constexpr int kRaw = kWide ? kTile * (RT + PT) * 4 : 0;
+  static constexpr int kMerge = KS > 1 ? HG * (KS - 1) * 16 * (RT + 4) * 4 : 0;  // over the buffers
+  static constexpr int kLds = 2 * kBuf + kRaw > kMerge ? 2 * kBuf + kRaw : kMerge;
+  static_assert(kTile <= 64 && kRows % RPI == 0 && kLds <= 160 * 1024, "tile shape");
+  // byte of 16-byte chunk k (of the latent, or the key part) of row r
+  __device__ static __forceinline__ int lat(int r, int k) {
+    return r / RPI * 1040 + (r % RPI) * (RT * 2) + 16 * (k ^ ((r % RPI) * (16 / RPI)));
+  }
+  __device__ static __forceinline__ int key(int r, int k) {
+    constexpr int N = PT / 8;
+    return kLat + r * (PT * 2) + 16 * (k ^ ((r / (16 / N)) & (N - 1)));
+  }
+};
+
+// One run of tiles for HG x 16 heads.  Scores S^T[position][head] = K q'^T: A the cache rows from LDS, B
+// the absorbed queries, held in registers for a token; the result has a head per lane column and positions
+// 4g + e (g = lane / 16) of each 16, which is the B layout of the product O^T[r][head] += C^T p if 32 positions
+// are taken in the order 4g .. 4g + 3, 16 + 4g .. 16 + 4g + 3: numerators never leave the lane, and C^T comes
+// from the same LDS rows by transposing reads.  The accumulators (RT x 16 heads a wave) stay in registers;
+// they are rescaled only where the maximum grew by more than 2^8 (numerators stay below 256, far from f16's
+// end).  The next step's rows are on their way to LDS during this step's products.
+template <int RT, int PT, int HG, int KS, int WR, typename KV, bool TWO>
+__global__ void __launch_bounds__(64 * HG * KS, 1)
+    mla_attend_kernel(LatentCache c, const float* __restrict__ qa, int nh, float scale, MlaPlan plan, int runs, int least,
+                      float* __restrict__ part_o, float2* __restrict__ part_ml) {
+  using S = AttendShape<RT, PT, HG, KS, WR, KV>;
+  constexpr bool WIDE = S::kWide;
+  constexpr int KT = (RT + PT) / 32, DT = RT / 16, RW = S::kRows, RPI = S::RPI, TR = S::kTile;
+  constexpr int NT = WR / 16;  // 16-position tiles a wave
+  constexpr uint64_t FULL = ~0ull >> (64 - TR);
+  __shared__ __attribute__((aligned(16))) uint8_t s_raw[S::kLds];
+  const uint32_t lds0 = uint32_t(uintptr_t((lds_u8*)s_raw));
+
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, col = lane & 15;
+  const int hgw = wv % HG, kp = wv / HG;  // the wave's heads and positions
+  // runs of the same tiles for different heads sit on one XCD (blocks go round the 8)
+  const int groups = (nh + 16 * HG - 1) / (16 * HG);
+  const int b8 = blockIdx.x >> 3;
+  const int run = (b8 / groups) * 8 + (blockIdx.x & 7), h0 = (b8 % groups) * (16 * HG) + hgw * 16;
+  const int tiles = plan.prefix[c.n_tokens];
+  const int per = mla_per_run(tiles, runs, least);
+  int x = run * per;
+  const int x_end = min(x + per, tiles);
+  if (x >= x_end) return;
+  const int head = min(h0 + col, nh - 1);
+
+  for (int t = mla_token_of(plan.prefix, c.n_tokens, x, lane); x < x_end; t++) {
+    const int first = plan.prefix[t], last = min(plan.prefix[t + 1], x_end);
+    if (last <= x) continue;  // a token without positions
+    const int seq = plan.seq[t], end = plan.end[t];
+    const int32_t* table = c.table + seq * c.table_stride;
+
+    // lane r looks up row r of the step at p0: its block
+    auto look = [&](int p0) {
+      const int p = p0 + min(lane, TR - 1);
+      return uint32_t(p < end ? table[p >> c.shift] : -1);
+    };
+    // loads the wave's rows of that step into buffer buf; returns which rows of the step there are
+    auto fetch = [&](int p0, uint32_t blk, int buf) {
+      const int p = p0 + min(lane, TR - 1);
+      const bool ok = blk < c.n_blocks;
+      // a row that is not there reads the pool's first and is cleared once it has come
+      const int64_t at = ok ? ((int64_t(blk) << c.shift) + (p & ((1 << c.shift) - 1))) * c.width * int(sizeof(KV)) : 0;
+      const uint8_t* rows = static_cast<const uint8_t*>(c.rows);
+      constexpr int CB = 8 * int(sizeof(KV));            // bytes of 8 values
+      constexpr int LB = RT * int(sizeof(KV));           // bytes of a row's latent
+      if constexpr (!WIDE) {
+        const uint32_t dst = lds0 + buf * S::kBuf;
+#pragma unroll
+        for (int i = 0; i < RW / RPI; i++) {
+          const int r = wv * RW + i * RPI;
+          const uint32_t to = dst + r / RPI * 1040;
+          if constexpr (RPI == 1) {
+            const uint32_t lo = __builtin_amdgcn_readlane(int(uint32_t(at)), r), hi = __builtin_amdgcn_readlane(int(at >> 32), r);
+            dma_row(rows + ((int64_t(hi) << 32) | lo), min(16 * lane, 2 * c.rank - 16), to);
+          } else {
+            constexpr int L = 64 / RPI;
+            const int rr = lane / L, k = (lane % L) ^ (rr * (16 / RPI));
+            const int64_t o = __shfl(at, r + rr, kWave);
+            dma_lanes(rows + o + min(16 * k, 2 * c.rank - 16), to);
+          }
+        }
+      } else {
+        // the raw rows of a wave follow each other, latents then key parts
+        const uint32_t dst = lds0 + 2 * S::kBuf + wv * RW * LB;
+#pragma unroll
+        for (int i = 0; i < RW * LB / 1024; i++) {
+          const int b = i * 1024 + 16 * lane;  // byte of the wave's latents
+          const int64_t o = __shfl(at, wv * RW + b / LB, kWave);
+          dma_lanes(rows + o + min(b % LB, 4 * c.rank - 16), dst + i * 1024);
+        }
+      }
+      constexpr int KB = PT * int(sizeof(KV));  // bytes of a row's key part
+#pragma unroll
+      for (int i = 0; i < (RW * KB + 1023) / 1024; i++) {
+        const int b = i * 1024 + 16 * lane;
+        const int r = wv * RW + b / KB;
+        const int64_t o = __shfl(at, min(r, TR - 1), kWave);
+        const int sw = WIDE ? 0 : 16 * ((r / (16 / (PT / 8))) & (PT / 8 - 1));
+        const uint32_t to = WIDE ? lds0 + 2 * S::kBuf + TR * LB + wv * RW * KB + i * 1024
+                                 : lds0 + buf * S::kBuf + S::kLat + wv * RW * KB + i * 1024;
+        if ((RW * KB) % 1024 == 0 || b < RW * KB)
+          dma_lanes(rows + o + c.rank * int(sizeof(KV)) + min((b % KB) ^ sw, (c.rope / 8) * CB - 16), to);
+      }
+      return __ballot(ok && lane < TR);
+    };
+    // clears the wave's rows that are not there
+    auto clear = [&](uint64_t mask, int buf) {
+      for (int r = wv * RW; r < wv * RW + RW; r++)
+        if (!((mask >> r) & 1)) {
+          uint8_t* p = s_raw + buf * S::kBuf;
+          const u32x4 z = {0u, 0u, 0u, 0u};
+          if (lane < RT / 8) *reinterpret_cast<u32x4*>(p + S::lat(r, lane)) = z;
+          if (lane < PT / 8) *reinterpret_cast<u32x4*>(p + S::key(r, lane)) = z;
+        }
+    };
+    // an f32 cache: the wave's raw rows to their upper and lower parts
+    auto convert = [&](uint64_t mask) {
+      auto part = [&](const uint8_t* src, int row, int dst) {
+        const bool on = (mask >> row) & 1;
+        float v[8];
+        load8<float>(reinterpret_cast<const float*>(src), v);
+        h8_t hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          _Float16 a, b;
+          split2(on ? v[e] : 0.f, a, b);
+          hi[e] = a, lo[e] = b;
+        }
+        *reinterpret_cast<h8_t*>(s_raw + dst) = hi;
+        *reinterpret_cast<h8_t*>(s_raw + S::kBuf + dst) = lo;
+      };
+      const uint8_t* raw = s_raw + 2 * S::kBuf;
+#pragma unroll 4
+      for (int i = 0; i < RW * RT / 512; i++) {
+        const int b = i * 64 + lane, r = wv * RW + b / (RT / 8), k = b % (RT / 8);
+        part(raw + (r * RT + 8 * k) * 4, r, S::lat(r, k));
+      }
+      for (int b = lane; b < RW * PT / 8; b += 64) {
+        const int r = wv * RW + b / (PT / 8), k = b % (PT / 8);
+        part(raw + (TR * RT + r * PT + 8 * k) * 4, r, S::key(r, k));
+      }
+    };
+
+    const int p0 = (x - first) * TR;
+    const int steps = last - x;
+    uint32_t blk = look(p0);
+    __syncthreads();  // the buffers are free of the token before
+    uint64_t next = fetch(p0, blk, 0);
+    blk = look(p0 + TR);
+
+    // the absorbed queries of the wave's heads: B operands, each head brought near 1 by a power of two so that
+    // its parts stay within f16's range, which goes into the score's factor
+    h8_t qh[KT], ql[TWO ? KT : 1];
+    float factor;
+    {
+      const float* qr = qa + (int64_t(t) * nh + head) * c.width;
+      float mx = 0.f;
+      for (int k = 8 * g; k < c.width; k += 32) {
+        float v[8];
+        load8<float>(qr + k, v);
+#pragma unroll
+        for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[e]));
+      }
+      mx = max_over_groups(mx);
+      int ex = 0;
+      if (mx > 0.f && mx < INFINITY) ex = ilogbf(mx);
+      factor = ldexpf(scale * 1.44269504088896341f, ex);
+#pragma unroll
+      for (int i = 0; i < KT; i++) {
+        const int k = 32 * i + 8 * g;
+        const bool on = k < RT ? k < c.rank : k - RT < c.rope;
+        float v[8];
+        load8<float>(qr + (on ? (k < RT ? k : c.rank + k - RT) : 0), v);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          _Float16 a, b;
+          split2(on ? ldexpf(v[e], -ex) : 0.f, a, b);
+          qh[i][e] = a;
+          if (TWO) ql[i][e] = b;
+        }
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // few rows in flight: registers
+      }
+    }
+    f4_t o[DT];
+#pragma unroll
+    for (int i = 0; i < DT; i++) o[i] = f4_t{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+
+    for (int i = 0; i < steps; i++) {
+      const uint64_t here = next;
+      const int buf = WIDE ? 0 : i & 1;
+      dma_wait();
+      if constexpr (WIDE) {
+        __syncthreads();  // the parts of the step before have been read
+        convert(here);
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the raw rows have been read
+      } else {
+        if (here != FULL) clear(here, buf);
+      }
+      if constexpr (!WIDE) __syncthreads();
+      if (i + 1 < steps) {
+        next = fetch(p0 + (i + 1) * TR, blk, buf ^ 1);
+        blk = look(p0 + (i + 2) * TR);
+      }
+      if constexpr (WIDE) __syncthreads();
+      const uint8_t* kv = s_raw + buf * S::kBuf;
+      // scores
+      f4_t sa[NT], sb[NT];
+#pragma unroll
+      for (int j = 0; j < NT; j++) sa[j] = sb[j] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KT; k++) {
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+          const int r = kp * WR + 16 * j + col;
+          const int at = k < RT / 32 ? S::lat(r, 4 * k + g) : S::key(r, 4 * k + g - RT / 8);
+          const h8_t a = *reinterpret_cast<const h8_t*>(kv + at);
+          sa[j] = mfma(a, qh[k], sa[j]);
+          if constexpr (TWO) sb[j] = mfma(a, ql[k], sb[j]);
+          if constexpr (WIDE) sb[j] = mfma(*reinterpret_cast<const h8_t*>(kv + S::kBuf + at), qh[k], sb[j]);
+        }
+      }
+      float sc[4 * NT], mx = -INFINITY;
+      const uint64_t own = here >> (kp * WR);
+#pragma unroll
+      for (int j = 0; j < NT; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) sc[4 * j + e] = (sa[j][e] + sb[j][e]) * factor;
+      if (here != FULL) {
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (!((own >> (16 * j + 4 * g + e)) & 1)) sc[4 * j + e] = -INFINITY;
+      }
+#pragma unroll
+      for (int e = 0; e < 4 * NT; e++) mx = fmaxf(mx, sc[e]);
+      mx = max_over_groups(mx);
+      if (__any(mx > m + 8.f)) {
+        const float mn = fmaxf(m, mx);
+        const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        l *= a;
+        m = mn;
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[d] *= a;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+      _Float16 ph[4 * NT], pl[4 * NT];
+#pragma unroll
+      for (int e = 0; e < 4 * NT; e++) {
+        const float p = __builtin_amdgcn_exp2f(sc[e] - ref);
+        l += p;
+        split2(p, ph[e], pl[e]);
+      }
+      // O^T += C^T p.  Lane l of a transposing read names 4 values of row 4g + col / 4 and gets column col of
+      // the 4 rows.
+      const int vr = kp * WR + 4 * g + (col >> 2), vc = (col & 3) >> 1, vb = 8 * (col & 1);
+      auto tr = [&](int d, int j, int plane) {
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_s4*)(kv + plane * S::kBuf + S::lat(vr + 16 * j, 2 * d + vc) + vb));
+      };
+      if constexpr (NT == 1) {
+        const h4_t bh = {ph[0], ph[1], ph[2], ph[3]}, bl = {pl[0], pl[1], pl[2], pl[3]};
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+          const h4_t v = __builtin_bit_cast(h4_t, tr(d, 0, 0));
+          o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(v, bh, o[d], 0, 0, 0);
+          if constexpr (TWO) o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(v, bl, o[d], 0, 0, 0);
+          if constexpr (WIDE)
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(h4_t, tr(d, 0, 1)), bh, o[d], 0, 0, 0);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NT; j += 2) {
+          h8_t bh, bl;
+#pragma unroll
+          for (int e = 0; e < 8; e++) bh[e] = ph[4 * j + e], bl[e] = pl[4 * j + e];
+          auto both = [&](int d, int plane) {
+            return __builtin_bit_cast(h8_t, __builtin_shufflevector(tr(d, j, plane), tr(d, j + 1, plane), 0, 1, 2, 3, 4, 5, 6, 7));
+          };
+#pragma unroll
+          for (int d = 0; d < DT; d++) {
+            const h8_t v = both(d, 0);
+            o[d] = mfma(v, bh, o[d]);
+            if constexpr (TWO) o[d] = mfma(v, bl, o[d]);
+            if constexpr (WIDE) o[d] = mfma(both(d, 1), bh, o[d]);
+          }
+        }
+      }
+    }
+    l = sum_over_groups(l);
+
+    // waves of the same heads merge through LDS, over the buffers
+    const int64_t slot = run + t;
+    if constexpr (KS > 1) {
+      float* const s_o = reinterpret_cast<float*>(s_raw);
+      constexpr int W = RT + 4;
+      __syncthreads();
+      if (kp) {
+        float* w = s_o + ((kp - 1) * HG + hgw) * 16 * W + col * W;
+#pragma unroll
+        for (int d = 0; d < DT; d++) *reinterpret_cast<f4_t*>(w + 16 * d + 4 * g) = o[d];
+        if (g == 0) w[RT] = m, w[RT + 1] = l;
+      }
+      __syncthreads();
+      if (kp == 0) {
+        float mt = m;
+#pragma unroll
+        for (int k = 0; k < KS - 1; k++) mt = fmaxf(mt, s_o[(k * HG + hgw) * 16 * W + col * W + RT]);
+        const float ref = mt == -INFINITY ? 0.f : mt;
+        const float a = __builtin_amdgcn_exp2f(m - ref);
+        l *= a;
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[d] *= a;
+#pragma unroll
+        for (int k = 0; k < KS - 1; k++) {
+          const float* w = s_o + (k * HG + hgw) * 16 * W + col * W;
+          const float b = __builtin_amdgcn_exp2f(w[RT] - ref);
+          l += b * w[RT + 1];
+#pragma unroll
+          for (int d = 0; d < DT; d++) o[d] += b * *reinterpret_cast<const f4_t*>(w + 16 * d + 4 * g);
+        }
+        m = mt;
+      }
+    }
+    if (kp == 0 && h0 + col < nh) {
+      float* po = part_o + (slot * nh + head) * c.rank;
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+        if (16 * d + 4 * g < c.rank) *reinterpret_cast<f4_t*>(po + 16 * d + 4 * g) = o[d];
+      if (g == 0) part_ml[slot * nh + head] = make_float2(m, l);
+    }
+    x = last;
   }
 }
 
-// The attended latent o[t][h][rank] in f32, one workgroup per (token, head), one pass: each wave takes
-// every fourth position with a running maximum and sum, and the four merge at the end.
-template <typename KV>
-__global__ void __launch_bounds__(256) mla_attend_kernel(LatentCache c, const float* __restrict__ qa, float scale,
-                                                         float* __restrict__ o) {
-  constexpr int DL = (kMlaMaxRank + kMlaMaxRope) / kWave;
-  constexpr int RL = kMlaMaxRank / kWave;
-  __shared__ float s_o[4][kMlaMaxRank];
-  __shared__ float s_m[4], s_l[4];
-  const int t = blockIdx.x, h = blockIdx.y, nh = gridDim.y;
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  int seq, pos;
-  if (!mla_locate(c, t, lane, seq, pos)) return;
-  const float* qr = qa + (int64_t(t) * nh + h) * c.width;
-  float q[DL], acc[RL];
-#pragma unroll
-  for (int i = 0; i < DL; i++) q[i] = lane + 64 * i < c.width ? qr[lane + 64 * i] * scale : 0.f;
-#pragma unroll
-  for (int i = 0; i < RL; i++) acc[i] = 0.f;
-  float m = -INFINITY, l = 0.f;
-  const int end = min(pos + 1, c.max_len);
-  for (int j = wv; j < end; j += 4) {
-    const int64_t at = mla_row(c, seq, j);
-    if (at < 0) continue;
-    const KV* row = static_cast<const KV*>(c.rows) + at;
-    float k[DL], s = 0.f;
-#pragma unroll
-    for (int i = 0; i < DL; i++) {
-      k[i] = lane + 64 * i < c.width ? float(row[lane + 64 * i]) : 0.f;
-      s += q[i] * k[i];
-    }
-    s = wave_sum_dpp(s);
-    const float mn = fmaxf(m, s);
-    const float a = mn == m ? 1.f : expf(m - mn), p = expf(s - mn);
-    l = l * a + p;
-    m = mn;
-#pragma unroll
-    for (int i = 0; i < RL; i++) acc[i] = acc[i] * a + p * k[i];
-  }
-#pragma unroll
-  for (int i = 0; i < RL; i++) s_o[wv][lane + 64 * i] = acc[i];
-  if (lane == 0) s_m[wv] = m, s_l[wv] = l;
-  __syncthreads();
-  for (int r = threadIdx.x; r < c.rank; r += 256) {
-    float M = -INFINITY;
-    for (int w = 0; w < 4; w++) M = s_l[w] > 0.f ? fmaxf(M, s_m[w]) : M;
-    float num = 0.f, den = 0.f;
-    for (int w = 0; w < 4; w++) {
-      if (!(s_l[w] != 0.f)) continue;  // no position of its own
-      const float e = expf(s_m[w] - M);
-      num += e * s_o[w][r];
-      den += e * s_l[w];
-    }
-    o[(int64_t(t) * nh + h) * c.rank + r] = den != 0.f ? num / den : 0.f;
-  }
-}
-
-// out[t][h][v] = o[t][h] . W_uv[h][v], one workgroup per (token, head).
-template <typename X>
-__global__ void __launch_bounds__(256) mla_values_kernel(LatentCache c, const float* __restrict__ o,
-                                                         const _Float16* __restrict__ v_b, int v_dim,
+// out[t][h] = W_uv[h] o[t][h], o the merged partials: one workgroup of 8 waves per head and 16 tokens.  The
+// weights' rows (16 of them a wave, its MFMA operand) are on their way while the partials are merged into LDS.
+// With few tokens the waves share a token's partials, else each wave takes tokens of its own.
+template <typename X, int RT>
+__global__ void __launch_bounds__(512) mla_values_kernel(LatentCache c, const float* __restrict__ part_o,
+                                                         const float2* __restrict__ part_ml, MlaPlan plan, int runs,
+                                                         int least, const _Float16* __restrict__ v_b, int v_dim,
                                                          X* __restrict__ out, int64_t out_stride) {
-  const int t = blockIdx.x, h = blockIdx.y, nh = gridDim.y;
-  int seq, pos;
-  if (!mla_locate(c, t, threadIdx.x & 63, seq, pos)) return;
-  const float* a = o + (int64_t(t) * nh + h) * c.rank;
-  for (int v = threadIdx.x; v < v_dim; v += 256) {
-    const _Float16* w = v_b + (int64_t(h) * v_dim + v) * c.rank;
-    float s = 0.f;
-    for (int r = 0; r < c.rank; r++) s += a[r] * float(w[r]);
-    out[t * out_stride + int64_t(h) * v_dim + v] = X(s);
+  constexpr int KT = RT / 32, P = RT + 8, NW = 8, U = 8;
+  __shared__ __attribute__((aligned(16))) _Float16 s_hi[16][P], s_lo[16][P];
+  __shared__ float s_acc[NW][RT];
+  __shared__ float s_m[NW], s_l[NW];
+  const int h = blockIdx.x, nh = gridDim.x, t0 = blockIdx.y * 16;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int g = lane >> 4, col = lane & 15;
+  const int vt = (v_dim + 15) / 16;
+  h8_t b[KT];
+  auto weights = [&](int tile) {
+    const _Float16* w = v_b + (int64_t(h) * v_dim + min(16 * tile + col, v_dim - 1)) * c.rank;
+#pragma unroll
+    for (int i = 0; i < KT; i++) b[i] = *reinterpret_cast<const h8_t*>(w + min(32 * i + 8 * g, c.rank - 8));
+  };
+  weights(min(wv, vt - 1));
+  const int nt = min(16, c.n_tokens - t0);
+  const int per = mla_per_run(plan.prefix[c.n_tokens], runs, least);
+  const int r0 = min(8 * lane, c.rank - 8);
+
+  // partials w0, w0 + by, ... below w1 of token t, of which lane l holds elements 8l ..: sum, maximum, total
+  float acc[8], m, l;
+  auto merge = [&](int t, int w0, int w1, int by) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) acc[e] = 0.f;
+    m = -INFINITY, l = 0.f;
+    for (int w = w0; w < w1; w += by * U) {
+      float4 lo[U], hi[U];
+      float2 ml[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int64_t at = int64_t(min(w + u * by, w1 - 1) + t) * nh + h;
+        const float* p = part_o + at * c.rank + r0;
+        lo[u] = *reinterpret_cast<const float4*>(p);
+        hi[u] = *reinterpret_cast<const float4*>(p + 4);
+        ml[u] = part_ml[at];
+      }
+      float mn = m;
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (w + u * by < w1) mn = fmaxf(mn, ml[u].x);
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      const float a = __builtin_amdgcn_exp2f(m - ref);
+      l *= a;
+#pragma unroll
+      for (int e = 0; e < 8; e++) acc[e] *= a;
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        if (w + u * by >= w1) continue;
+        const float f = __builtin_amdgcn_exp2f(ml[u].x - ref);
+        l += f * ml[u].y;
+        acc[0] += f * lo[u].x, acc[1] += f * lo[u].y, acc[2] += f * lo[u].z, acc[3] += f * lo[u].w;
+        acc[4] += f * hi[u].x, acc[5] += f * hi[u].y, acc[6] += f * hi[u].z, acc[7] += f * hi[u].w;
+      }
+      m = mn;
+    }
+  };
+  auto keep = [&](int row, float sum) {
+    const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+    if (8 * lane < RT) {
+      h8_t hi, lo;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        _Float16 x, y;
+        split2(8 * lane < c.rank ? acc[e] * inv : 0.f, x, y);
+        hi[e] = x, lo[e] = y;
+      }
+      *reinterpret_cast<h8_t*>(&s_hi[row][8 * lane]) = hi;
+      *reinterpret_cast<h8_t*>(&s_lo[row][8 * lane]) = lo;
+    }
+  };
+  auto range = [&](int t, int& w0, int& w1) {
+    const int a = plan.prefix[t], e = plan.prefix[t + 1];
+    w0 = a / per;
+    w1 = e > a ? (e - 1) / per + 1 : w0;
+  };
+  int w0, w1;
+  if (nt > 2) {
+    for (int i = wv; i < 16; i += NW) {
+      m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; e++) acc[e] = 0.f;
+      if (i < nt) {
+        range(t0 + i, w0, w1);
+        merge(t0 + i, w0, w1, 1);
+      }
+      keep(i, l);
+    }
+  } else {
+    for (int i = 0; i < nt; i++) {
+      range(t0 + i, w0, w1);
+      merge(t0 + i, w0 + wv, w1, NW);
+      if (8 * lane < RT) {
+        reinterpret_cast<float4*>(&s_acc[wv][8 * lane])[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        reinterpret_cast<float4*>(&s_acc[wv][8 * lane])[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      }
+      if (lane == 0) s_m[wv] = m, s_l[wv] = l;
+      __syncthreads();
+      if (wv == 0) {
+        float mt = -INFINITY, sum = 0.f;
+        for (int w = 0; w < NW; w++) mt = fmaxf(mt, s_m[w]);
+        const float ref = mt == -INFINITY ? 0.f : mt;
+#pragma unroll
+        for (int e = 0; e < 8; e++) acc[e] = 0.f;
+        for (int w = 0; w < NW; w++) {
+          const float f = __builtin_amdgcn_exp2f(s_m[w] - ref);
+          sum += f * s_l[w];
+#pragma unroll
+          for (int e = 0; e < 8; e++) acc[e] += f * s_acc[w][min(8 * lane, RT - 8) + e];
+        }
+        keep(i, sum);
+      }
+      __syncthreads();
+    }
+    if (wv >= nt)  // the rows of no token
+      for (int i = wv; i < 16; i += NW) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) acc[e] = 0.f;
+        keep(i, 1.f);
+      }
+    if (wv < nt)
+      for (int i = wv + NW; i < 16; i += NW) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) acc[e] = 0.f;
+        keep(i, 1.f);
+      }
+  }
+  __syncthreads();
+  for (int tile = wv; tile < vt; tile += NW) {
+    if (tile != wv) weights(tile);
+    f4_t hi = {0.f, 0.f, 0.f, 0.f}, lo = hi;
+#pragma unroll
+    for (int i = 0; i < KT; i++) {
+      hi = mfma(*reinterpret_cast<const h8_t*>(&s_hi[col][32 * i + 8 * g]), b[i], hi);
+      lo = mfma(*reinterpret_cast<const h8_t*>(&s_lo[col][32 * i + 8 * g]), b[i], lo);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int t = t0 + 4 * g + e, v = 16 * tile + col;
+      if (t < c.n_tokens && v < v_dim && plan.seq[t] >= 0) out[t * out_stride + int64_t(h) * v_dim + v] = X(hi[e] + lo[e]);
+    }
   }
 }
 
@@ -283,9 +894,60 @@ extern "C" int jero_hip_mla_append(const jero_latent_cache* cache, int act_dtype
   return check_launch("mla_append");
 }
 
+namespace jero {
+
+// Where the parts of the absorbed form's workspace are.
+struct AbsorbedSpace {
+  size_t part_o, part_ml, plan, bytes;
+};
+
+static AbsorbedSpace absorbed_space(const jero_latent_cache* c, int64_t n_tokens, int n_heads) {
+  auto up = [](size_t n) { return (n + 255) & ~size_t(255); };
+  const size_t rows = size_t(n_tokens) * n_heads, parts = (size_t(n_tokens) + kMlaRuns) * n_heads;
+  AbsorbedSpace s;
+  s.part_o = up(rows * (size_t(c->rank) + c->rope_dim) * 4);
+  s.part_ml = s.part_o + up(parts * c->rank * 4);
+  s.plan = s.part_ml + up(parts * 8);
+  s.bytes = s.plan + up((3 * size_t(n_tokens) + 1) * 4);
+  return s;
+}
+
+template <int RT, int PT, int HG, int KS, int WR, typename KV, bool TWO>
+static void launch_attend(const LatentCache& c, const float* qa, int nh, float scale, const MlaPlan& plan, int runs,
+                          int least, float* part_o, float2* part_ml, hipStream_t s) {
+  const int groups = (nh + 16 * HG - 1) / (16 * HG);
+  hipLaunchKernelGGL((mla_attend_kernel<RT, PT, HG, KS, WR, KV, TWO>), dim3(unsigned(runs) * groups), dim3(64 * HG * KS),
+                     0, s, c, qa, nh, scale, plan, runs, least, part_o, part_ml);
+}
+
+// Positions a step: an f16 cache's two buffers hold 64, an f32 cache's parts and raw rows 32.
+constexpr int attend_tile(bool f32_kv) { return f32_kv ? 32 : 64; }
+// Heads a workgroup: 16 by each of its 1, 2 or 4 waves' worth; with fewer than 4 the others share the positions.
+static int attend_heads(int nh) { return nh <= 16 ? 16 : nh <= 32 ? 32 : 64; }
+
+template <int RT, int PT, typename KV, bool TWO>
+static void launch_attend_heads(const LatentCache& c, const float* qa, int nh, float scale, const MlaPlan& plan, int runs,
+                                int least, float* part_o, float2* part_ml, hipStream_t s) {
+  constexpr int T = attend_tile(sizeof(KV) == 4);
+  if (attend_heads(nh) == 16) launch_attend<RT, PT, 1, 2, T / 2, KV, TWO>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
+  else if (attend_heads(nh) == 32)
+    launch_attend<RT, PT, 2, 2, T / 2, KV, TWO>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
+  else launch_attend<RT, PT, 4, 1, T, KV, TWO>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
+}
+
+template <int RT, int PT>
+static void launch_attend_types(bool f32_act, bool f32_kv, const LatentCache& c, const float* qa, int nh, float scale,
+                                const MlaPlan& plan, int runs, int least, float* part_o, float2* part_ml, hipStream_t s) {
+  if (f32_kv) launch_attend_heads<RT, PT, float, true>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
+  else if (f32_act) launch_attend_heads<RT, PT, _Float16, true>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
+  else launch_attend_heads<RT, PT, _Float16, false>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
+}
+
+}  // namespace jero
+
 extern "C" size_t jero_hip_mla_absorbed_workspace_bytes(const jero_latent_cache* cache, int64_t n_tokens, int n_heads) {
-  if (!cache || n_tokens < 1 || n_heads < 1) return 0;
-  return size_t(n_tokens) * n_heads * (2 * size_t(cache->rank) + cache->rope_dim) * sizeof(float);
+  if (!cache || n_tokens < 1 || n_heads < 1 || cache->rank < 1 || cache->rope_dim < 1) return 0;
+  return absorbed_space(cache, n_tokens, n_heads).bytes;
 }
 
 extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, int act_dtype, const void* q_dev,
@@ -299,33 +961,61 @@ extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, i
   if (rc) return rc;
   MlaRope rope;
   if ((rc = mla_rope_of(rope_theta, cache->rope_dim, &rope))) return rc;
+  const AbsorbedSpace sp = absorbed_space(cache, n_tokens, n_heads);
   void* ws = workspace_dev;
-  if ((rc = absorbed_workspace(jero_hip_mla_absorbed_workspace_bytes(cache, n_tokens, n_heads), &ws, workspace_bytes,
-                               kName)))
-    return rc;
+  if ((rc = absorbed_workspace(sp.bytes, &ws, workspace_bytes, kName))) return rc;
   const LatentCache c = mla_cache_of(cache, n_tokens);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  float* qa = static_cast<float*>(ws);
-  float* o = qa + n_tokens * n_heads * c.width;
-  const dim3 grid{unsigned(n_tokens), unsigned(n_heads), 1};
+  uint8_t* const w = static_cast<uint8_t*>(ws);
+  float *qa = reinterpret_cast<float*>(w), *part_o = reinterpret_cast<float*>(w + sp.part_o);
+  float2* part_ml = reinterpret_cast<float2*>(w + sp.part_ml);
+  MlaPlan plan;
+  plan.prefix = reinterpret_cast<int*>(w + sp.plan);
+  plan.seq = plan.prefix + n_tokens + 1;
+  plan.end = plan.seq + n_tokens;
   const _Float16 *kb = static_cast<const _Float16*>(k_b_dev), *vb = static_cast<const _Float16*>(v_b_dev);
-  if (act_dtype == JERO_F32)
-    hipLaunchKernelGGL((mla_absorb_kernel<float>), grid, dim3(256), 0, s, c, static_cast<const float*>(q_dev), q_stride,
-                       nope_dim, kb, rope, qa);
-  else
-    hipLaunchKernelGGL((mla_absorb_kernel<_Float16>), grid, dim3(256), 0, s, c, static_cast<const _Float16*>(q_dev),
-                       q_stride, nope_dim, kb, rope, qa);
+  const bool f32 = act_dtype == JERO_F32;
+  const int tile = attend_tile(cache->kv_dtype == JERO_KV_F32);
+  const int groups = (n_heads + attend_heads(n_heads) - 1) / attend_heads(n_heads);
+  const int runs = groups >= kMlaRuns / 8 ? 8 : kMlaRuns / groups / 8 * 8, least = 1;
+
+  const dim3 ga{unsigned((c.rank + 63) / 64 + 2), unsigned(n_heads), unsigned((n_tokens + 63) / 64)};
+#define JERO_ABSORB(X, NT)                                                                                           \
+  hipLaunchKernelGGL((mla_absorb_kernel<X, NT>), ga, dim3(256), 0, s, c, static_cast<const X*>(q_dev), q_stride, nope_dim, \
+                     kb, rope, qa, plan, tile)
+  if (nope_dim <= 128) {
+    if (f32) JERO_ABSORB(float, 4);
+    else JERO_ABSORB(_Float16, 4);
+  } else {
+    if (f32) JERO_ABSORB(float, 8);
+    else JERO_ABSORB(_Float16, 8);
+  }
+#undef JERO_ABSORB
   if ((rc = check_launch("mla absorb"))) return rc;
-  if (cache->kv_dtype == JERO_KV_F16)
-    hipLaunchKernelGGL((mla_attend_kernel<_Float16>), grid, dim3(256), 0, s, c, qa, scale, o);
+
+  const bool wide = cache->kv_dtype == JERO_KV_F32;
+  if (c.rank <= 128 && c.rope <= 32)
+    launch_attend_types<128, 32>(f32, wide, c, qa, n_heads, scale, plan, runs, least, part_o, part_ml, s);
+  else if (c.rank <= 256)
+    launch_attend_types<256, 64>(f32, wide, c, qa, n_heads, scale, plan, runs, least, part_o, part_ml, s);
   else
-    hipLaunchKernelGGL((mla_attend_kernel<float>), grid, dim3(256), 0, s, c, qa, scale, o);
+    launch_attend_types<512, 64>(f32, wide, c, qa, n_heads, scale, plan, runs, least, part_o, part_ml, s);
   if ((rc = check_launch("mla attend"))) return rc;
-  if (act_dtype == JERO_F32)
-    hipLaunchKernelGGL((mla_values_kernel<float>), grid, dim3(256), 0, s, c, o, vb, v_dim, static_cast<float*>(out_dev),
-                       out_stride);
-  else
-    hipLaunchKernelGGL((mla_values_kernel<_Float16>), grid, dim3(256), 0, s, c, o, vb, v_dim,
-                       static_cast<_Float16*>(out_dev), out_stride);
+
+  const dim3 gv{unsigned(n_heads), unsigned((n_tokens + 15) / 16), 1};
+#define JERO_VALUES(X, RT)                                                                                              \
+  hipLaunchKernelGGL((mla_values_kernel<X, RT>), gv, dim3(512), 0, s, c, part_o, part_ml, plan, runs, least, vb, v_dim, \
+                     static_cast<X*>(out_dev), out_stride)
+  if (c.rank <= 128) {
+    if (f32) JERO_VALUES(float, 128);
+    else JERO_VALUES(_Float16, 128);
+  } else if (c.rank <= 256) {
+    if (f32) JERO_VALUES(float, 256);
+    else JERO_VALUES(_Float16, 256);
+  } else {
+    if (f32) JERO_VALUES(float, 512);
+    else JERO_VALUES(_Float16, 512);
+  }
+#undef JERO_VALUES
   return check_launch("mla values");
 }
