@@ -230,9 +230,13 @@ __device__ __forceinline__ int mla_token_of(const int* prefix, int n, int x, int
   return lo;
 }
 
-__device__ __forceinline__ float max_over_groups(float v) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
-  v = fmaxf(v, __shfl_xor(v, 16, kWave));
-  return fmaxf(v, __shfl_xor(v, 32, kWave));
+// Over lanes l, l ^ 16, l ^ 32, l ^ 48: each swap leaves a value and its partner in the two results.
+__device__ __forceinline__ float max_over_groups(float v) {
+  const uint32_t x = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  const uint32_t y = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+  const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float sum_over_groups(float v) {
   v += __shfl_xor(v, 16, kWave);
@@ -240,8 +244,8 @@ __device__ __forceinline__ float sum_over_groups(float v) {
 }
 
 // 16 bytes a lane straight from global memory to LDS, lane l's to base + 16 l: the loads in flight take no
-// registers.  The compiler does not know of these loads; dma_wait waits for the wave's own, and a barrier
-// then shows them to the others.
+// registers.  The compiler does not know of these loads; dma_wait waits for the wave's own but the last N, and
+// a barrier then shows them to the others.
 __device__ __forceinline__ void dma_row(const void* row, uint32_t lane_bytes, uint32_t lds) {  // uniform row
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(lane_bytes), "s"(row)
                : "memory");
@@ -249,38 +253,49 @@ __device__ __forceinline__ void dma_row(const void* row, uint32_t lane_bytes, ui
 __device__ __forceinline__ void dma_lanes(const void* p, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
 }
-__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void dma_wait() {
+  static_assert(N < 64, "the counter's range");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 typedef __attribute__((address_space(3))) s4_t lds_s4;
 
+constexpr int kAttendTile = 32;  // positions a step
+
 // Shape of the attend kernel: HG waves of 16 heads by KS waves of WR positions, RT + PT the padded widths,
-// KV the cache's type.  LDS holds a step's rows in f16: the latents RPI rows to 1024 bytes, with 16 bytes
-// after each 1024 so that 16 rows fall on all banks (RPI > 1: the rows of one 1024 swap their 16-byte chunks
-// by their number instead), then the key parts, whose chunks are swapped the same way.  An f16 cache is
-// loaded straight into one of two such buffers; an f32 cache into a raw buffer, from which each wave turns
-// its rows into a buffer of their upper and one of their lower parts.
-template <int RT, int PT, int HG, int KS, int WR, typename KV>
+// KV the cache's type.  LDS holds a step's rows in f16, the latents and then the key parts, so that neither 8
+// rows' reads of one 16-byte chunk nor a transposing read's 32 bytes of 4 rows meet on a bank: rows of 1024
+// bytes have 16 more after them (one address a lane for all reads), the chunks of shorter ones are swapped by the
+// row's number.  An f16 cache is loaded straight into one of four such buffers; an f32 cache into a raw buffer,
+// from which each wave turns its rows into a buffer of their upper and one of their lower parts.
+template <int RT, int PT, int HG, int KS, typename KV>
 struct AttendShape {
   static constexpr bool kWide = sizeof(KV) == 4;
   static constexpr int kWaves = HG * KS;
-  static constexpr int kTile = WR * KS;  // positions a step
+  static constexpr int kTile = kAttendTile;
+  static constexpr int WR = kTile / KS;
   static constexpr int kRows = kTile / kWaves;  // rows a wave loads
-  static constexpr int RPI = 512 / RT;
-  static constexpr int kLat = kTile / RPI * 1040;
+  static constexpr bool kPad = RT == 512;
+  static constexpr int kPitch = RT * 2 + (kPad ? 16 : 0);
+  static constexpr int kLat = kTile * kPitch;
   static constexpr int kBuf = kLat + kTile * PT * 2;
+  static constexpr int kBufs = kWide ? 2 : 4;
   static constexpr int kRaw = kWide ? kTile * (RT + PT) * 4 : 0;
   static constexpr int kMerge = KS > 1 ? HG * (KS - 1) * 16 * (RT + 4) * 4 : 0;  // over the buffers
-  static constexpr int kLds = 2 * kBuf + kRaw > kMerge ? 2 * kBuf + kRaw : kMerge;
-  static_assert(kTile <= 64 && kRows % RPI == 0 && kLds <= 160 * 1024, "tile shape");
+  static constexpr int kLds = kBufs * kBuf + kRaw > kMerge ? kBufs * kBuf + kRaw : kMerge;
+  // loads of 1024 bytes a wave issues for a step: of the latents, of the key parts
+  static constexpr int kLoadsLat = kRows * RT * int(sizeof(KV)) / 1024;
+  static constexpr int kLoadsKey = (kRows * PT * int(sizeof(KV)) + 1023) / 1024;
+  static constexpr int kLoads = kLoadsLat + kLoadsKey;
+  static_assert(kRows % 8 == 0 && kLds <= 160 * 1024, "tile shape");
+  __device__ static __forceinline__ constexpr int swap8(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+  __device__ static __forceinline__ constexpr int swap_lat(int r) { return kPad ? 0 : swap8(r); }
+  __device__ static __forceinline__ constexpr int swap_key(int r) { return PT == 64 ? swap8(r) : (r >> 1) & 3; }
   // byte of 16-byte chunk k (of the latent, or the key part) of row r
-  __device__ static __forceinline__ int lat(int r, int k) {
-    return r / RPI * 1040 + (r % RPI) * (RT * 2) + 16 * (k ^ ((r % RPI) * (16 / RPI)));
-  }
-  __device__ static __forceinline__ int key(int r, int k) {
-    constexpr int N = PT / 8;
-    return kLat + r * (PT * 2) + 16 * (k ^ ((r / (16 / N)) & (N - 1)));
-  }
+  __device__ static __forceinline__ int lat(int r, int k) { return r * kPitch + 16 * (k ^ swap_lat(r)); }
+  __device__ static __forceinline__ int key(int r, int k) { return kLat + r * (PT * 2) + 16 * (k ^ swap_key(r)); }
 };
 
 // One run of tiles for HG x 16 heads.  Scores S^T[position][head] = K q'^T: A the cache rows from LDS, B
@@ -289,16 +304,19 @@ struct AttendShape {
 // are taken in the order 4g .. 4g + 3, 16 + 4g .. 16 + 4g + 3: numerators never leave the lane, and C^T comes
 // from the same LDS rows by transposing reads.  The accumulators (RT x 16 heads a wave) stay in registers;
 // they are rescaled only where the maximum grew by more than 2^8 (numerators stay below 256, far from f16's
-// end).  The next step's rows are on their way to LDS during this step's products.
-template <int RT, int PT, int HG, int KS, int WR, typename KV, bool TWO>
+// end).
+//
+// Registers allow one wave a SIMD, so a wave covers its own waits: a step's softmax runs between the products
+// of the next step's scores, operands are read from LDS a group of products ahead, and the rows two steps on are
+// on their way from the cache meanwhile (f16 cache; an f32 one has its LDS filled by the parts of one step).
+template <int RT, int PT, int HG, int KS, typename KV, bool TWO>
 __global__ void __launch_bounds__(64 * HG * KS, 1)
     mla_attend_kernel(LatentCache c, const float* __restrict__ qa, int nh, float scale, MlaPlan plan, int runs, int least,
                       float* __restrict__ part_o, float2* __restrict__ part_ml) {
-  using S = AttendShape<RT, PT, HG, KS, WR, KV>;
+  using S = AttendShape<RT, PT, HG, KS, KV>;
   constexpr bool WIDE = S::kWide;
-  constexpr int KT = (RT + PT) / 32, DT = RT / 16, RW = S::kRows, RPI = S::RPI, TR = S::kTile;
+  constexpr int KT = (RT + PT) / 32, DT = RT / 16, RW = S::kRows, TR = S::kTile, WR = S::WR;
   constexpr int NT = WR / 16;  // 16-position tiles a wave
-  constexpr uint64_t FULL = ~0ull >> (64 - TR);
   __shared__ __attribute__((aligned(16))) uint8_t s_raw[S::kLds];
   const uint32_t lds0 = uint32_t(uintptr_t((lds_u8*)s_raw));
 
@@ -309,75 +327,84 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
   const int groups = (nh + 16 * HG - 1) / (16 * HG);
   const int b8 = blockIdx.x >> 3;
   const int run = (b8 / groups) * 8 + (blockIdx.x & 7), h0 = (b8 % groups) * (16 * HG) + hgw * 16;
-  const int tiles = plan.prefix[c.n_tokens];
+  const int n_tok = c.n_tokens;
+  // the plan of up to 64 tokens from t0 on, a token a lane
+  int t0 = 0;
+  int w_prefix = plan.prefix[min(lane, n_tok)], w_seq = plan.seq[min(lane, n_tok - 1)], w_end = plan.end[min(lane, n_tok - 1)];
+  const int tiles = plan.prefix[n_tok];
   const int per = mla_per_run(tiles, runs, least);
   int x = run * per;
   const int x_end = min(x + per, tiles);
   if (x >= x_end) return;
   const int head = min(h0 + col, nh - 1);
 
-  for (int t = mla_token_of(plan.prefix, c.n_tokens, x, lane); x < x_end; t++) {
-    const int first = plan.prefix[t], last = min(plan.prefix[t + 1], x_end);
+  auto window = [&](int t) {
+    t0 = t;
+    w_prefix = plan.prefix[min(t + lane, n_tok)];
+    w_seq = plan.seq[min(t + lane, n_tok - 1)];
+    w_end = plan.end[min(t + lane, n_tok - 1)];
+  };
+  int t = 0;
+  if (n_tok > 63) {
+    t = mla_token_of(plan.prefix, n_tok, x, lane);
+    window(t);
+  } else {
+    t = __popcll(__ballot(lane < n_tok && w_prefix <= x)) - 1;
+  }
+  for (; x < x_end; t++) {
+    if (t - t0 > 62) window(t);
+    const int first = __builtin_amdgcn_readlane(w_prefix, t - t0);
+    const int last = min(__builtin_amdgcn_readlane(w_prefix, t - t0 + 1), x_end);
     if (last <= x) continue;  // a token without positions
-    const int seq = plan.seq[t], end = plan.end[t];
+    const int seq = __builtin_amdgcn_readlane(w_seq, t - t0), end = __builtin_amdgcn_readlane(w_end, t - t0);
     const int32_t* table = c.table + seq * c.table_stride;
+    const int p0 = (x - first) * TR, steps = last - x;
 
-    // lane r looks up row r of the step at p0: its block
-    auto look = [&](int p0) {
-      const int p = p0 + min(lane, TR - 1);
-      return uint32_t(p < end ? table[p >> c.shift] : -1);
+    // block ids of 64 blocks from block b0 on, a block a lane
+    const int blocks = (end - 1) >> c.shift;  // the token's last
+    int b0 = p0 >> c.shift;
+    int ids = table[min(b0 + lane, blocks)];
+    // where the rows of step i are (bytes, row r's in lane r; a row that is not there reads the pool's first
+    // and is cleared once it has come), and which of them there are
+    int64_t at = 0;
+    auto find = [&](int i) {
+      const int p = p0 + i * TR + (lane & (TR - 1));
+      if ((min(p0 + i * TR + TR, end) - 1) >> c.shift >= b0 + 64) {
+        b0 = (p0 + i * TR) >> c.shift;
+        ids = table[min(b0 + lane, blocks)];
+        asm volatile("" : "+v"(ids));  // waited for here, where it was loaded
+      }
+      const uint32_t blk = uint32_t(__shfl(ids, min((p >> c.shift) - b0, 63), kWave));
+      const bool ok = p < end && blk < c.n_blocks;
+      at = ok ? ((int64_t(blk) << c.shift) + (p & ((1 << c.shift) - 1))) * c.width * int(sizeof(KV)) : 0;
+      return uint32_t(__ballot(ok));
     };
-    // loads the wave's rows of that step into buffer buf; returns which rows of the step there are
-    auto fetch = [&](int p0, uint32_t blk, int buf) {
-      const int p = p0 + min(lane, TR - 1);
-      const bool ok = blk < c.n_blocks;
-      // a row that is not there reads the pool's first and is cleared once it has come
-      const int64_t at = ok ? ((int64_t(blk) << c.shift) + (p & ((1 << c.shift) - 1))) * c.width * int(sizeof(KV)) : 0;
-      const uint8_t* rows = static_cast<const uint8_t*>(c.rows);
-      constexpr int CB = 8 * int(sizeof(KV));            // bytes of 8 values
-      constexpr int LB = RT * int(sizeof(KV));           // bytes of a row's latent
-      if constexpr (!WIDE) {
-        const uint32_t dst = lds0 + buf * S::kBuf;
-#pragma unroll
-        for (int i = 0; i < RW / RPI; i++) {
-          const int r = wv * RW + i * RPI;
-          const uint32_t to = dst + r / RPI * 1040;
-          if constexpr (RPI == 1) {
-            const uint32_t lo = __builtin_amdgcn_readlane(int(uint32_t(at)), r), hi = __builtin_amdgcn_readlane(int(at >> 32), r);
-            dma_row(rows + ((int64_t(hi) << 32) | lo), min(16 * lane, 2 * c.rank - 16), to);
-          } else {
-            constexpr int L = 64 / RPI;
-            const int rr = lane / L, k = (lane % L) ^ (rr * (16 / RPI));
-            const int64_t o = __shfl(at, r + rr, kWave);
-            dma_lanes(rows + o + min(16 * k, 2 * c.rank - 16), to);
-          }
-        }
-      } else {
-        // the raw rows of a wave follow each other, latents then key parts
-        const uint32_t dst = lds0 + 2 * S::kBuf + wv * RW * LB;
-#pragma unroll
-        for (int i = 0; i < RW * LB / 1024; i++) {
-          const int b = i * 1024 + 16 * lane;  // byte of the wave's latents
-          const int64_t o = __shfl(at, wv * RW + b / LB, kWave);
-          dma_lanes(rows + o + min(b % LB, 4 * c.rank - 16), dst + i * 1024);
-        }
-      }
-      constexpr int KB = PT * int(sizeof(KV));  // bytes of a row's key part
-#pragma unroll
-      for (int i = 0; i < (RW * KB + 1023) / 1024; i++) {
-        const int b = i * 1024 + 16 * lane;
-        const int r = wv * RW + b / KB;
-        const int64_t o = __shfl(at, min(r, TR - 1), kWave);
-        const int sw = WIDE ? 0 : 16 * ((r / (16 / (PT / 8))) & (PT / 8 - 1));
-        const uint32_t to = WIDE ? lds0 + 2 * S::kBuf + TR * LB + wv * RW * KB + i * 1024
-                                 : lds0 + buf * S::kBuf + S::kLat + wv * RW * KB + i * 1024;
+    // load i of the wave's rows of that step, into buffer buf (or the raw rows)
+    const uint8_t* const rows = static_cast<const uint8_t*>(c.rows);
+    auto load = [&](int i, int buf) {
+      constexpr int LB = RT * int(sizeof(KV)), KB = PT * int(sizeof(KV));  // bytes of a row's parts
+      constexpr int NK = S::kLoadsKey;  // the key parts first: their addresses come through LDS
+      const uint32_t dst = lds0 + (WIDE ? S::kBufs : buf) * S::kBuf;
+      if (i < NK) {
+        const int b = i * 1024 + 16 * lane, r = b / KB;
+        const int64_t o = __shfl(at, min(wv * RW + r, TR - 1), kWave);
+        const int sw = WIDE ? 0 : 16 * S::swap_key(r);
+        const uint32_t to = dst + (WIDE ? TR * LB : S::kLat) + wv * RW * KB + i * 1024;
         if ((RW * KB) % 1024 == 0 || b < RW * KB)
-          dma_lanes(rows + o + c.rank * int(sizeof(KV)) + min((b % KB) ^ sw, (c.rope / 8) * CB - 16), to);
+          dma_lanes(rows + o + c.rank * int(sizeof(KV)) + min((b % KB) ^ sw, c.rope * int(sizeof(KV)) - 16), to);
+      } else if constexpr (LB == 1024 && !WIDE) {
+        const int r = wv * RW + i - NK;
+        const uint32_t lo = __builtin_amdgcn_readlane(int(uint32_t(at)), r), hi = __builtin_amdgcn_readlane(int(at >> 32), r);
+        dma_row(rows + ((int64_t(hi) << 32) | lo), min(16 * lane, 2 * c.rank - 16), dst + r * S::kPitch);
+      } else {
+        const int b = (i - NK) * 1024 + 16 * lane, r = b / LB;
+        const int64_t o = __shfl(at, wv * RW + r, kWave);
+        const int sw = WIDE ? 0 : 16 * S::swap_lat(r);
+        dma_lanes(rows + o + min((b % LB) ^ sw, c.rank * int(sizeof(KV)) - 16), dst + wv * RW * LB + (i - NK) * 1024);
       }
-      return __ballot(ok && lane < TR);
     };
     // clears the wave's rows that are not there
-    auto clear = [&](uint64_t mask, int buf) {
+    auto clear = [&](uint32_t mask, int buf) {
       for (int r = wv * RW; r < wv * RW + RW; r++)
         if (!((mask >> r) & 1)) {
           uint8_t* p = s_raw + buf * S::kBuf;
@@ -387,7 +414,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
         }
     };
     // an f32 cache: the wave's raw rows to their upper and lower parts
-    auto convert = [&](uint64_t mask) {
+    auto convert = [&](uint32_t mask) {
       auto part = [&](const uint8_t* src, int row, int dst) {
         const bool on = (mask >> row) & 1;
         float v[8];
@@ -402,7 +429,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
         *reinterpret_cast<h8_t*>(s_raw + dst) = hi;
         *reinterpret_cast<h8_t*>(s_raw + S::kBuf + dst) = lo;
       };
-      const uint8_t* raw = s_raw + 2 * S::kBuf;
+      const uint8_t* raw = s_raw + S::kBufs * S::kBuf;
 #pragma unroll 4
       for (int i = 0; i < RW * RT / 512; i++) {
         const int b = i * 64 + lane, r = wv * RW + b / (RT / 8), k = b % (RT / 8);
@@ -414,12 +441,16 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
       }
     };
 
-    const int p0 = (x - first) * TR;
-    const int steps = last - x;
-    uint32_t blk = look(p0);
     __syncthreads();  // the buffers are free of the token before
-    uint64_t next = fetch(p0, blk, 0);
-    blk = look(p0 + TR);
+    constexpr int AHEAD = WIDE ? 1 : 3;  // steps whose rows are on their way before the first
+    uint32_t mask[4] = {0, 0, 0, 0};     // which rows of the present step and the next three there are
+#pragma unroll
+    for (int j = 0; j < AHEAD; j++)
+      if (j < steps) {
+        mask[j] = find(j);
+#pragma unroll
+        for (int i = 0; i < S::kLoads; i++) load(i, j);
+      }
 
     // the absorbed queries of the wave's heads: B operands, each head brought near 1 by a power of two so that
     // its parts stay within f16's range, which goes into the score's factor
@@ -427,13 +458,18 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
     float factor;
     {
       const float* qr = qa + (int64_t(t) * nh + head) * c.width;
-      float mx = 0.f;
-      for (int k = 8 * g; k < c.width; k += 32) {
-        float v[8];
-        load8<float>(qr + k, v);
+      float v[KT][8], mx = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[e]));
+      for (int i = 0; i < KT; i++) {
+        const int k = 32 * i + 8 * g;
+        const bool on = k < RT ? k < c.rank : k - RT < c.rope;
+        load8<float>(qr + (on ? (k < RT ? k : c.rank + k - RT) : 0), v[i]);
       }
+      __builtin_amdgcn_sched_barrier(0);  // one round trip for the row
+#pragma unroll
+      for (int i = 0; i < KT; i++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[i][e]));  // a repeated element changes nothing
       mx = max_over_groups(mx);
       int ex = 0;
       if (mx > 0.f && mx < INFINITY) ex = ilogbf(mx);
@@ -442,16 +478,14 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
       for (int i = 0; i < KT; i++) {
         const int k = 32 * i + 8 * g;
         const bool on = k < RT ? k < c.rank : k - RT < c.rope;
-        float v[8];
-        load8<float>(qr + (on ? (k < RT ? k : c.rank + k - RT) : 0), v);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           _Float16 a, b;
-          split2(on ? ldexpf(v[e], -ex) : 0.f, a, b);
+          split2(on ? ldexpf(v[i][e], -ex) : 0.f, a, b);
           qh[i][e] = a;
           if (TWO) ql[i][e] = b;
         }
-        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // few rows in flight: registers
+        __builtin_amdgcn_sched_barrier(0);  // in order: v's registers become the parts'
       }
     }
     f4_t o[DT];
@@ -459,106 +493,233 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
     for (int i = 0; i < DT; i++) o[i] = f4_t{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
 
-    for (int i = 0; i < steps; i++) {
-      const uint64_t here = next;
-      const int buf = WIDE ? 0 : i & 1;
-      dma_wait();
-      if constexpr (WIDE) {
-        __syncthreads();  // the parts of the step before have been read
-        convert(here);
-        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the raw rows have been read
-      } else {
-        if (here != FULL) clear(here, buf);
-      }
-      if constexpr (!WIDE) __syncthreads();
-      if (i + 1 < steps) {
-        next = fetch(p0 + (i + 1) * TR, blk, buf ^ 1);
-        blk = look(p0 + (i + 2) * TR);
-      }
-      if constexpr (WIDE) __syncthreads();
-      const uint8_t* kv = s_raw + buf * S::kBuf;
-      // scores
-      f4_t sa[NT], sb[NT];
+    // where the lane reads in a buffer, for each value of a chunk number's swapped bits; the rest is constant
+    constexpr int NKL = S::kPad ? 1 : 2, NVV = S::kPad ? 1 : 4;
+    int kl[NKL], kk[2], vv[NVV];
+    {
+      const int r = kp * WR + col;
 #pragma unroll
-      for (int j = 0; j < NT; j++) sa[j] = sb[j] = f4_t{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < NKL; i++) kl[i] = S::lat(r, 4 * i + g);
+      kk[0] = S::key(r, g), kk[1] = S::key(r, PT == 64 ? 4 + g : g);
+      // lane l of a transposing read names 4 values of row 4g + col / 4 and gets column col of the 4 rows
+      const int vr = kp * WR + 4 * g + (col >> 2);
 #pragma unroll
-      for (int k = 0; k < KT; k++) {
+      for (int d = 0; d < NVV; d++) vv[d] = S::lat(vr, 2 * d + ((col & 3) >> 1)) + 8 * (col & 1);
+    }
+    f4_t sa[NT], sb[NT];  // the scores of a step, in two sums
+    constexpr int QG = KT % 2 || (TWO && NT == 2) ? 1 : 2, QN = KT / QG;  // k steps a group, groups
+    h8_t ka[2][QG][NT], kb[WIDE ? 2 : 1][QG][NT];
+    auto read_k = [&](int grp, const uint8_t* kv) {
+#pragma unroll
+      for (int i = 0; i < QG; i++)
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-          const int r = kp * WR + 16 * j + col;
-          const int at = k < RT / 32 ? S::lat(r, 4 * k + g) : S::key(r, 4 * k + g - RT / 8);
-          const h8_t a = *reinterpret_cast<const h8_t*>(kv + at);
-          sa[j] = mfma(a, qh[k], sa[j]);
-          if constexpr (TWO) sb[j] = mfma(a, ql[k], sb[j]);
-          if constexpr (WIDE) sb[j] = mfma(*reinterpret_cast<const h8_t*>(kv + S::kBuf + at), qh[k], sb[j]);
+          const int k = grp * QG + i;
+          const uint8_t* p = kv + (k < RT / 32 ? kl[k % NKL] + 64 * (k - k % NKL) + 16 * j * S::kPitch
+                                               : kk[(k - RT / 32) & 1] + 16 * j * PT * 2);
+          ka[grp & 1][i][j] = *reinterpret_cast<const h8_t*>(p);
+          if constexpr (WIDE) kb[grp & 1][i][j] = *reinterpret_cast<const h8_t*>(p + S::kBuf);
         }
+    };
+    // the scores of the step in buffer kv; between the groups of products, between(group)
+    auto scores = [&](const uint8_t* kv, f4_t (&a)[NT], f4_t (&b)[NT], auto between) {
+#pragma unroll
+      for (int j = 0; j < NT; j++) a[j] = b[j] = f4_t{0.f, 0.f, 0.f, 0.f};
+      read_k(0, kv);
+#pragma unroll
+      for (int grp = 0; grp < QN; grp++) {
+        if (grp + 1 < QN) read_k(grp + 1, kv);
+        between(grp);
+#pragma unroll
+        for (int i = 0; i < QG; i++)
+#pragma unroll
+          for (int j = 0; j < NT; j++) {
+            const int k = grp * QG + i;
+            if (!TWO && (k & 1)) b[j] = mfma(ka[grp & 1][i][j], qh[k], b[j]);  // two chains
+            else a[j] = mfma(ka[grp & 1][i][j], qh[k], a[j]);
+            if constexpr (TWO) b[j] = mfma(ka[grp & 1][i][j], ql[k], b[j]);
+            if constexpr (WIDE) b[j] = mfma(kb[grp & 1][i][j], qh[k], b[j]);
+          }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      float sc[4 * NT], mx = -INFINITY;
-      const uint64_t own = here >> (kp * WR);
+    };
+    // the softmax of a step's scores, in three parts
+    float sc[4 * NT], mn = 0.f, alpha = 1.f;
+    bool grew = false;
+    _Float16 ph[4 * NT], pl[4 * NT];
+    auto soft_max = [&](uint32_t here) {
+      const uint32_t own = here >> (kp * WR) >> (4 * g);  // bit 16 j + e: position 4g + e of tile j
+      float mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < NT; j++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) sc[4 * j + e] = (sa[j][e] + sb[j][e]) * factor;
-      if (here != FULL) {
-#pragma unroll
-        for (int j = 0; j < NT; j++)
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            if (!((own >> (16 * j + 4 * g + e)) & 1)) sc[4 * j + e] = -INFINITY;
-      }
-#pragma unroll
-      for (int e = 0; e < 4 * NT; e++) mx = fmaxf(mx, sc[e]);
+        for (int e = 0; e < 4; e++) {
+          const float s = (sa[j][e] + sb[j][e]) * factor;
+          sc[4 * j + e] = own & (1u << (16 * j + e)) ? s : -INFINITY;
+          mx = fmaxf(mx, sc[4 * j + e]);
+        }
       mx = max_over_groups(mx);
-      if (__any(mx > m + 8.f)) {
-        const float mn = fmaxf(m, mx);
-        const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-        l *= a;
-        m = mn;
+      grew = __any(mx > m + 8.f);
+      mn = grew ? fmaxf(m, mx) : m;
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      alpha = __builtin_amdgcn_exp2f(m - ref);  // 0 at first: exp2(-inf)
+      m = mn;
+      mn = ref;
+    };
+    auto soft_exp = [&](int e) {
+      const float p = __builtin_amdgcn_exp2f(sc[e] - mn);
+      split2(p, ph[e], pl[e]);
+      sc[e] = p;
+      asm volatile("" : "+v"(sc[e]));  // here, between the products, and not where they are used
+    };
+    auto soft_sum = [&]() {
+      float s = 0.f;
 #pragma unroll
-        for (int d = 0; d < DT; d++) o[d] *= a;
-      }
-      const float ref = m == -INFINITY ? 0.f : m;
-      _Float16 ph[4 * NT], pl[4 * NT];
-#pragma unroll
-      for (int e = 0; e < 4 * NT; e++) {
-        const float p = __builtin_amdgcn_exp2f(sc[e] - ref);
-        l += p;
-        split2(p, ph[e], pl[e]);
-      }
-      // O^T += C^T p.  Lane l of a transposing read names 4 values of row 4g + col / 4 and gets column col of
-      // the 4 rows.
-      const int vr = kp * WR + 4 * g + (col >> 2), vc = (col & 3) >> 1, vb = 8 * (col & 1);
-      auto tr = [&](int d, int j, int plane) {
-        return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_s4*)(kv + plane * S::kBuf + S::lat(vr + 16 * j, 2 * d + vc) + vb));
-      };
-      if constexpr (NT == 1) {
-        const h4_t bh = {ph[0], ph[1], ph[2], ph[3]}, bl = {pl[0], pl[1], pl[2], pl[3]};
+      for (int e = 0; e < 4 * NT; e++) s += sc[e];
+      l = l * alpha + s;
+    };
+    // O^T += C^T p from buffer kv
+    auto values = [&](const uint8_t* kv) {
+      if (grew) {
 #pragma unroll
         for (int d = 0; d < DT; d++) {
-          const h4_t v = __builtin_bit_cast(h4_t, tr(d, 0, 0));
-          o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(v, bh, o[d], 0, 0, 0);
-          if constexpr (TWO) o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(v, bl, o[d], 0, 0, 0);
+          asm volatile("" : "+a"(o[d]));  // in accumulation registers up to here: else all are copied every step
+          o[d] *= alpha;
+        }
+      }
+      auto tr = [&](int d, int j, int plane) {
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_s4*)(kv + vv[d % NVV] + plane * S::kBuf + 32 * (d - d % NVV) + 16 * j * S::kPitch));
+      };
+      constexpr int VG = 4, VN = DT / VG;  // tiles of 16 latent columns a group
+      if constexpr (NT == 1) {
+        const h4_t bh = {ph[0], ph[1], ph[2], ph[3]}, bl = {pl[0], pl[1], pl[2], pl[3]};
+        h4_t va[2][VG], vl[WIDE ? 2 : 1][VG];
+        auto read_v = [&](int grp) {
+#pragma unroll
+          for (int i = 0; i < VG; i++) {
+            va[grp & 1][i] = __builtin_bit_cast(h4_t, tr(grp * VG + i, 0, 0));
+            if constexpr (WIDE) vl[grp & 1][i] = __builtin_bit_cast(h4_t, tr(grp * VG + i, 0, 1));
+          }
+        };
+        read_v(0);
+#pragma unroll
+        for (int grp = 0; grp < VN; grp++) {
+          if (grp + 1 < VN) read_v(grp + 1);
+#pragma unroll
+          for (int i = 0; i < VG; i++) {
+            f4_t& d = o[grp * VG + i];
+            d = __builtin_amdgcn_mfma_f32_16x16x16f16(va[grp & 1][i], bh, d, 0, 0, 0);
+          }
+          if constexpr (TWO)
+#pragma unroll
+            for (int i = 0; i < VG; i++) {
+              f4_t& d = o[grp * VG + i];
+              d = __builtin_amdgcn_mfma_f32_16x16x16f16(va[grp & 1][i], bl, d, 0, 0, 0);
+            }
           if constexpr (WIDE)
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(h4_t, tr(d, 0, 1)), bh, o[d], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < VG; i++) {
+              f4_t& d = o[grp * VG + i];
+              d = __builtin_amdgcn_mfma_f32_16x16x16f16(vl[grp & 1][i], bh, d, 0, 0, 0);
+            }
+          __builtin_amdgcn_sched_barrier(0);
         }
       } else {
+        h8_t bh, bl;
 #pragma unroll
-        for (int j = 0; j < NT; j += 2) {
-          h8_t bh, bl;
+        for (int e = 0; e < 8; e++) bh[e] = ph[e], bl[e] = pl[e];
+        h8_t va[2][VG], vl[WIDE ? 2 : 1][VG];
+        auto both = [&](int d, int plane) {
+          return __builtin_bit_cast(h8_t, __builtin_shufflevector(tr(d, 0, plane), tr(d, 1, plane), 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        auto read_v = [&](int grp) {
 #pragma unroll
-          for (int e = 0; e < 8; e++) bh[e] = ph[4 * j + e], bl[e] = pl[4 * j + e];
-          auto both = [&](int d, int plane) {
-            return __builtin_bit_cast(h8_t, __builtin_shufflevector(tr(d, j, plane), tr(d, j + 1, plane), 0, 1, 2, 3, 4, 5, 6, 7));
-          };
-#pragma unroll
-          for (int d = 0; d < DT; d++) {
-            const h8_t v = both(d, 0);
-            o[d] = mfma(v, bh, o[d]);
-            if constexpr (TWO) o[d] = mfma(v, bl, o[d]);
-            if constexpr (WIDE) o[d] = mfma(both(d, 1), bh, o[d]);
+          for (int i = 0; i < VG; i++) {
+            va[grp & 1][i] = both(grp * VG + i, 0);
+            if constexpr (WIDE) vl[grp & 1][i] = both(grp * VG + i, 1);
           }
+        };
+        read_v(0);
+#pragma unroll
+        for (int grp = 0; grp < VN; grp++) {
+          if (grp + 1 < VN) read_v(grp + 1);
+#pragma unroll
+          for (int i = 0; i < VG; i++) o[grp * VG + i] = mfma(va[grp & 1][i], bh, o[grp * VG + i]);
+          if constexpr (TWO)
+#pragma unroll
+            for (int i = 0; i < VG; i++) o[grp * VG + i] = mfma(va[grp & 1][i], bl, o[grp * VG + i]);
+          if constexpr (WIDE)
+#pragma unroll
+            for (int i = 0; i < VG; i++) o[grp * VG + i] = mfma(vl[grp & 1][i], bh, o[grp * VG + i]);
+          __builtin_amdgcn_sched_barrier(0);
         }
+      }
+    };
+
+    if constexpr (WIDE) {
+      for (int i = 0; i < steps; i++) {
+        dma_wait<0>();
+        __syncthreads();  // the parts of the step before have been read
+        const uint32_t here = mask[0];
+        convert(here);
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the raw rows have been read
+        const bool more = i + 1 < steps;
+        if (more) {
+          mask[0] = find(i + 1);
+#pragma unroll
+          for (int n = 0; n < S::kLoadsKey; n++) load(n, 0);
+        }
+        __syncthreads();
+        scores(s_raw, sa, sb, [&](int grp) {
+          if (more)  // the next step's loads, a few a group: issued at once they hold the wave up
+#pragma unroll
+            for (int n = grp * S::kLoadsLat / QN; n < (grp + 1) * S::kLoadsLat / QN; n++) load(S::kLoadsKey + n, 0);
+        });
+        soft_max(here);
+#pragma unroll
+        for (int e = 0; e < 4 * NT; e++) soft_exp(e);
+        soft_sum();
+        values(s_raw);
+      }
+    } else {
+      // step i: its scores are there; the next step's rows have come, those of two more are on their way
+      if (steps > 2) dma_wait<2 * S::kLoads>();
+      else if (steps > 1) dma_wait<S::kLoads>();
+      else dma_wait<0>();
+      if (mask[0] != 0xFFFFFFFFu) clear(mask[0], 0);
+      __syncthreads();
+      scores(s_raw, sa, sb, [](int) {});
+      for (int i = 0; i < steps; i++) {
+        // (after the last step the scores are those of some rows still in LDS, and not used: a second copy of
+        // the products for it would cost their registers)
+        const int nb = (i + 1) & 3, fb = (i + 3) & 3;
+        const bool more = i + 3 < steps;
+        if (i + 2 < steps) dma_wait<S::kLoads>();
+        else dma_wait<0>();
+        if (i + 1 < steps && mask[1] != 0xFFFFFFFFu) clear(mask[1], nb);
+        __syncthreads();  // the next step's rows are there, and the step before has been read
+        if (more) {
+          mask[3] = find(i + 3);
+#pragma unroll
+          for (int n = 0; n < S::kLoadsKey; n++) load(n, fb);
+        }
+        f4_t na[NT], nb2[NT];
+        scores(s_raw + nb * S::kBuf, na, nb2, [&](int grp) {
+          if (more)
+#pragma unroll
+            for (int n = grp * S::kLoadsLat / QN; n < (grp + 1) * S::kLoadsLat / QN; n++) load(S::kLoadsKey + n, fb);
+          if (grp == QN / 4) soft_max(mask[0]);
+          constexpr int E0 = QN / 2, EN = QN - E0 - 1;  // groups that take the exponentials
+          if (grp >= E0 && grp < QN - 1)
+#pragma unroll
+            for (int e = (grp - E0) * 4 * NT / EN; e < (grp - E0 + 1) * 4 * NT / EN; e++) soft_exp(e);
+          if (grp == QN - 1) soft_sum();
+        });
+        values(s_raw + (i & 3) * S::kBuf);
+#pragma unroll
+        for (int j = 0; j < NT; j++) sa[j] = na[j], sb[j] = nb2[j];
+        mask[0] = mask[1], mask[1] = mask[2], mask[2] = mask[3];
       }
     }
     l = sum_over_groups(l);
@@ -912,27 +1073,24 @@ static AbsorbedSpace absorbed_space(const jero_latent_cache* c, int64_t n_tokens
   return s;
 }
 
-template <int RT, int PT, int HG, int KS, int WR, typename KV, bool TWO>
+template <int RT, int PT, int HG, int KS, typename KV, bool TWO>
 static void launch_attend(const LatentCache& c, const float* qa, int nh, float scale, const MlaPlan& plan, int runs,
                           int least, float* part_o, float2* part_ml, hipStream_t s) {
   const int groups = (nh + 16 * HG - 1) / (16 * HG);
-  hipLaunchKernelGGL((mla_attend_kernel<RT, PT, HG, KS, WR, KV, TWO>), dim3(unsigned(runs) * groups), dim3(64 * HG * KS),
-                     0, s, c, qa, nh, scale, plan, runs, least, part_o, part_ml);
+  hipLaunchKernelGGL((mla_attend_kernel<RT, PT, HG, KS, KV, TWO>), dim3(unsigned(runs) * groups), dim3(64 * HG * KS), 0, s,
+                     c, qa, nh, scale, plan, runs, least, part_o, part_ml);
 }
 
-// Positions a step: an f16 cache's two buffers hold 64, an f32 cache's parts and raw rows 32.
-constexpr int attend_tile(bool f32_kv) { return f32_kv ? 32 : 64; }
-// Heads a workgroup: 16 by each of its 1, 2 or 4 waves' worth; with fewer than 4 the others share the positions.
+// Heads a workgroup: 16 by each of its 1, 2 or 4 waves' worth; with fewer than 4 others share the positions.
 static int attend_heads(int nh) { return nh <= 16 ? 16 : nh <= 32 ? 32 : 64; }
 
 template <int RT, int PT, typename KV, bool TWO>
 static void launch_attend_heads(const LatentCache& c, const float* qa, int nh, float scale, const MlaPlan& plan, int runs,
                                 int least, float* part_o, float2* part_ml, hipStream_t s) {
-  constexpr int T = attend_tile(sizeof(KV) == 4);
-  if (attend_heads(nh) == 16) launch_attend<RT, PT, 1, 2, T / 2, KV, TWO>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
-  else if (attend_heads(nh) == 32)
-    launch_attend<RT, PT, 2, 2, T / 2, KV, TWO>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
-  else launch_attend<RT, PT, 4, 1, T, KV, TWO>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
+  const int hg = attend_heads(nh);
+  if (hg == 16) launch_attend<RT, PT, 1, 2, KV, TWO>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
+  else if (hg == 32) launch_attend<RT, PT, 2, 2, KV, TWO>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
+  else launch_attend<RT, PT, 4, 1, KV, TWO>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
 }
 
 template <int RT, int PT>
@@ -975,7 +1133,7 @@ extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, i
   plan.end = plan.seq + n_tokens;
   const _Float16 *kb = static_cast<const _Float16*>(k_b_dev), *vb = static_cast<const _Float16*>(v_b_dev);
   const bool f32 = act_dtype == JERO_F32;
-  const int tile = attend_tile(cache->kv_dtype == JERO_KV_F32);
+  const int tile = kAttendTile;
   const int groups = (n_heads + attend_heads(n_heads) - 1) / attend_heads(n_heads);
   const int runs = groups >= kMlaRuns / 8 ? 8 : kMlaRuns / groups / 8 * 8, least = 1;
 
