@@ -74,6 +74,75 @@ __device__ __forceinline__ int64_t mla_row(const LatentCache& c, int seq, int po
   return ((int64_t(b) << c.shift) + (pos & ((1 << c.shift) - 1))) * c.width;
 }
 
+// ---------------------------------------------------------------- matrix cores, LDS
+
+typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef short s4_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f4_t mfma(h8_t a, h8_t b, f4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// x as two f16 parts, hi + lo = x to 22 bits.
+__device__ __forceinline__ void split2(float x, _Float16& hi, _Float16& lo) {
+  hi = _Float16(x);
+  lo = _Float16(x - float(hi));
+}
+
+template <typename X>
+__device__ __forceinline__ void load8(const X* p, float (&v)[8]);
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+template <>
+__device__ __forceinline__ void load8<_Float16>(const _Float16* p, float (&v)[8]) {
+  const h8_t a = *reinterpret_cast<const h8_t*>(p);
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] = float(a[e]);
+}
+
+// Over lanes l, l ^ 16, l ^ 32, l ^ 48: each swap leaves a value and its partner in the two results.
+__device__ __forceinline__ float max_over_groups(float v) {
+  const uint32_t x = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  const uint32_t y = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+  const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum_over_groups(float v) {
+  v += __shfl_xor(v, 16, kWave);
+  return v + __shfl_xor(v, 32, kWave);
+}
+
+// 16 bytes a lane straight from global memory to LDS, lane l's to base + 16 l: the loads in flight take no
+// registers.  The compiler does not know of these loads; dma_wait waits for the wave's own but the last N, and
+// a barrier then shows them to the others.
+__device__ __forceinline__ void dma_row(const void* row, uint32_t lane_bytes, uint32_t lds) {  // uniform row
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(lane_bytes), "s"(row)
+               : "memory");
+}
+__device__ __forceinline__ void dma_lanes(const void* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void dma_wait() {
+  static_assert(N < 64, "the counter's range");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+typedef __attribute__((address_space(3))) s4_t lds_s4;
+
+// The swap of a row's 16-byte chunks in LDS (chunk k of row r sits at k ^ swap8(r)) with which neither 8 rows'
+// reads of one chunk nor a transposing read's 32 bytes of 4 rows meet on a bank, for rows of a multiple of 128 bytes;
+// rows of 64 bytes have 4 chunks to swap.
+__host__ __device__ __forceinline__ constexpr int swap8(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+__host__ __device__ __forceinline__ constexpr int swap4(int r) { return (r >> 1) & 3; }
+
 int mla_check_cache(const jero_latent_cache* cache, int64_t n_tokens, int act_dtype, const char* what);
 LatentCache mla_cache_of(const jero_latent_cache* cache, int64_t n_tokens);
 int mla_rope_of(float theta, int rope_dim, MlaRope* out);

@@ -58,11 +58,6 @@ __global__ void __launch_bounds__(256) mla_append_kernel(LatentCache c, const X*
 // sequences of 900 to 6000 positions leave half the workgroups short.  Run w of token t writes partial
 // w + t: along the runs either w or t grows, so the number names the pair.
 
-typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
-typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
-typedef float f4_t __attribute__((ext_vector_type(4)));
-typedef short s4_t __attribute__((ext_vector_type(4)));
-
 constexpr int kMlaRuns = 256;  // workgroups of the attend kernel: one per CU, its tiles fill the LDS
 
 struct MlaPlan {
@@ -88,30 +83,6 @@ __device__ __forceinline__ bool mla_locate_thread(const LatentCache& c, int t, i
   if (seq < 0 || seq >= c.n_seqs) return false;
   pos = int(int64_t(c.lens[seq]) - c.starts[seq + 1] + t);
   return true;
-}
-
-__device__ __forceinline__ f4_t mfma(h8_t a, h8_t b, f4_t c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
-// x as two f16 parts, hi + lo = x to 22 bits.
-__device__ __forceinline__ void split2(float x, _Float16& hi, _Float16& lo) {
-  hi = _Float16(x);
-  lo = _Float16(x - float(hi));
-}
-
-template <typename X>
-__device__ __forceinline__ void load8(const X* p, float (&v)[8]);
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
-template <>
-__device__ __forceinline__ void load8<_Float16>(const _Float16* p, float (&v)[8]) {
-  const h8_t a = *reinterpret_cast<const h8_t*>(p);
-#pragma unroll
-  for (int e = 0; e < 8; e++) v[e] = float(a[e]);
 }
 
 // Grid (tiles of 64 latent columns, then one for the key part, then one for the plan; heads; tokens by
@@ -230,38 +201,6 @@ __device__ __forceinline__ int mla_token_of(const int* prefix, int n, int x, int
   return lo;
 }
 
-// Over lanes l, l ^ 16, l ^ 32, l ^ 48: each swap leaves a value and its partner in the two results.
-__device__ __forceinline__ float max_over_groups(float v) {
-  const uint32_t x = __float_as_uint(v);
-  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-  const uint32_t y = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
-  const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float sum_over_groups(float v) {
-  v += __shfl_xor(v, 16, kWave);
-  return v + __shfl_xor(v, 32, kWave);
-}
-
-// 16 bytes a lane straight from global memory to LDS, lane l's to base + 16 l: the loads in flight take no
-// registers.  The compiler does not know of these loads; dma_wait waits for the wave's own but the last N, and
-// a barrier then shows them to the others.
-__device__ __forceinline__ void dma_row(const void* row, uint32_t lane_bytes, uint32_t lds) {  // uniform row
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(lane_bytes), "s"(row)
-               : "memory");
-}
-__device__ __forceinline__ void dma_lanes(const void* p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
-}
-template <int N>
-__device__ __forceinline__ void dma_wait() {
-  static_assert(N < 64, "the counter's range");
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-
-typedef __attribute__((address_space(3))) uint8_t lds_u8;
-typedef __attribute__((address_space(3))) s4_t lds_s4;
-
 constexpr int kAttendTile = 32;  // positions a step
 
 // Shape of the attend kernel: HG waves of 16 heads by KS waves of WR positions, RT + PT the padded widths,
@@ -290,9 +229,8 @@ struct AttendShape {
   static constexpr int kLoadsKey = (kRows * PT * int(sizeof(KV)) + 1023) / 1024;
   static constexpr int kLoads = kLoadsLat + kLoadsKey;
   static_assert(kRows % 8 == 0 && kLds <= 160 * 1024, "tile shape");
-  __device__ static __forceinline__ constexpr int swap8(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
   __device__ static __forceinline__ constexpr int swap_lat(int r) { return kPad ? 0 : swap8(r); }
-  __device__ static __forceinline__ constexpr int swap_key(int r) { return PT == 64 ? swap8(r) : (r >> 1) & 3; }
+  __device__ static __forceinline__ constexpr int swap_key(int r) { return PT == 64 ? swap8(r) : swap4(r); }
   // byte of 16-byte chunk k (of the latent, or the key part) of row r
   __device__ static __forceinline__ int lat(int r, int k) { return r * kPitch + 16 * (k ^ swap_lat(r)); }
   __device__ static __forceinline__ int key(int r, int k) { return kLat + r * (PT * 2) + 16 * (k ^ swap_key(r)); }
@@ -944,8 +882,8 @@ int mla_check_cache(const jero_latent_cache* c, int64_t n_tokens, int act_dtype,
                 w + "block_size " + std::to_string(c->block_size) + " is not a power of two up to 2^20");
   if (n_tokens < 1 || c->n_seqs < 1 || c->n_blocks < 1 || c->max_len < 1)
     return fail(JERO_ERR_TENSOR_BOUNDS, w + "no tokens, sequences, blocks or positions");
-  if (n_tokens > (1 << 22) || c->n_seqs > (1 << 22) || c->n_blocks > INT32_MAX)
-    return fail(JERO_ERR_TENSOR_BOUNDS, w + "more than 2^22 tokens or sequences, or 2^31 blocks");
+  if (n_tokens > (1 << 19) || c->n_seqs > (1 << 19) || c->n_blocks > INT32_MAX)
+    return fail(JERO_ERR_TENSOR_BOUNDS, w + "more than 2^19 tokens or sequences, or 2^31 - 1 blocks");
   if (!c->starts_dev && n_tokens != c->n_seqs)
     return fail(JERO_ERR_TENSOR_BOUNDS, w + std::to_string(n_tokens) + " tokens of " + std::to_string(c->n_seqs) +
                                             " sequences without their starts");

@@ -1,101 +1,517 @@
 // mla_prefill.hip -- latent attention over a paged cache: the expanded form, for prompts.
+//
+// For as many heads at a time as the workspace holds: mla_expand_kernel makes every position's keys and
+// values, k = W_uk c and v = W_uv c, as rows of f16 (two parts a value with f32 activations), and copies
+// the shared key parts next to each other; mla_flash_kernel runs the causal attention of 128 tokens of a
+// sequence and a head over them.
 #include "mla.h"
 
 namespace jero {
 
 // Rows of the expanded keys and values: sequence s holds rows base(s) .. base(s) + min(lens[s],
-// max_len) - 1, base the sum of the lengths before it; a sequence that ends past total has none.
+// max_len) - 1, base the sum of the lengths before it that fit; one that would end past total has none.
 __device__ __forceinline__ int mla_len(const LatentCache& c, int s) { return min(max(c.lens[s], 0), c.max_len); }
 
-__device__ __forceinline__ bool mla_base(const LatentCache& c, int seq, int64_t total, int64_t& base) {
-  base = 0;
-  for (int s = 0; s < seq; s++) {
-    const int n = mla_len(c, s);
-    if (base + n <= total) base += n;
-  }
-  return base + mla_len(c, seq) <= total;
-}
-
-// kv[h][row][nope + v] = W[h] c, one workgroup per (position of a sequence, sequence).
-template <typename KV>
-__global__ void __launch_bounds__(256) mla_expand_kernel(LatentCache c, int nh, int wide,
-                                                         const _Float16* __restrict__ w, int64_t total,
-                                                         float* __restrict__ kv) {
-  __shared__ float s_c[kMlaMaxRank];
-  const int j = blockIdx.x, seq = blockIdx.y;
-  int64_t base;
-  if (j >= mla_len(c, seq) || !mla_base(c, seq, total, base)) return;
-  const int64_t at = mla_row(c, seq, j);
-  const KV* row = static_cast<const KV*>(c.rows) + at;
-  for (int r = threadIdx.x; r < c.rank; r += 256) s_c[r] = at < 0 ? 0.f : float(row[r]);
-  __syncthreads();
-  for (int o = threadIdx.x; o < nh * wide; o += 256) {
-    const _Float16* wr = w + int64_t(o) * c.rank;
-    float s = 0.f;
-    for (int r = 0; r < c.rank; r++) s += s_c[r] * float(wr[r]);
-    kv[(int64_t(o / wide) * total + base + j) * wide + o % wide] = s;
-  }
-}
-
-template <typename X, typename KV>
-__global__ void __launch_bounds__(256) mla_prefill_kernel(LatentCache c, const X* __restrict__ q, int64_t q_stride,
-                                                          int h0, int nope, int v_dim, const float* __restrict__ kv,
-                                                          int64_t total, float scale, MlaRope rope, X* __restrict__ out,
-                                                          int64_t out_stride) {
-  __shared__ float s_q[256];
-  __shared__ float s_o[4][256];
-  __shared__ float s_m[4], s_l[4];
-  const int t = blockIdx.x, h = h0 + blockIdx.y;
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  const int wide = nope + v_dim, qw = nope + c.rope;
-  int seq, pos;
-  if (!mla_locate(c, t, lane, seq, pos)) return;
-  int64_t base;
-  const bool fits = mla_base(c, seq, total, base);
-  const X* qr = q + t * q_stride + int64_t(h) * qw;
-  for (int i = threadIdx.x; i < nope; i += 256) s_q[i] = float(qr[i]) * scale;
-  if (int(threadIdx.x) < c.rope / 2) {
-    const int i = threadIdx.x;
-    const float a = float(qr[nope + 2 * i]), b = float(qr[nope + 2 * i + 1]);
-    const float2 cs = rope.on ? mla_cos_sin(rope, i, pos) : make_float2(1.f, 0.f);
-    s_q[nope + 2 * i] = (a * cs.x - b * cs.y) * scale;
-    s_q[nope + 2 * i + 1] = (a * cs.y + b * cs.x) * scale;
-  }
-  __syncthreads();
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
-  const int end = fits ? min(min(pos + 1, c.max_len), mla_len(c, seq)) : 0;
-  for (int j = wv; j < end; j += 4) {
-    const int64_t at = mla_row(c, seq, j);
-    if (at < 0) continue;
-    const KV* row = static_cast<const KV*>(c.rows) + at + c.rank;
-    const float* kr = kv + (int64_t(blockIdx.y) * total + base + j) * wide;
-    float s = 0.f;
-    for (int i = lane; i < qw; i += 64) s += s_q[i] * (i < nope ? kr[i] : float(row[i - nope]));
-    s = wave_sum_dpp(s);
-    const float mn = fmaxf(m, s);
-    const float a = mn == m ? 1.f : expf(m - mn), p = expf(s - mn);
-    l = l * a + p;
-    m = mn;
-#pragma unroll
-    for (int i = 0; i < 4; i++) acc[i] = acc[i] * a + (lane + 64 * i < v_dim ? p * kr[nope + lane + 64 * i] : 0.f);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; i++) s_o[wv][lane + 64 * i] = acc[i];
-  if (lane == 0) s_m[wv] = m, s_l[wv] = l;
-  __syncthreads();
-  for (int v = threadIdx.x; v < v_dim; v += 256) {
-    float M = -INFINITY;
-    for (int w = 0; w < 4; w++) M = s_l[w] > 0.f ? fmaxf(M, s_m[w]) : M;
-    float num = 0.f, den = 0.f;
-    for (int w = 0; w < 4; w++) {
-      if (!(s_l[w] != 0.f)) continue;
-      const float e = expf(s_m[w] - M);
-      num += e * s_o[w][v];
-      den += e * s_l[w];
+// Goes over the sequences, all lanes together: f(s, base, length) until it returns false.
+template <typename F>
+__device__ __forceinline__ void mla_sequences(const LatentCache& c, int64_t total, int lane, F f) {
+  int64_t base = 0;
+  for (int s0 = 0; s0 < c.n_seqs; s0 += kWave) {
+    const int mine = s0 + lane < c.n_seqs ? mla_len(c, s0 + lane) : 0;
+    const int n = min(kWave, c.n_seqs - s0);
+    for (int j = 0; j < n; j++) {
+      const int len = __builtin_amdgcn_readlane(mine, j);
+      const bool fits = base + len <= total;
+      if (!f(s0 + j, base, fits ? len : 0)) return;
+      if (fits) base += len;
     }
-    out[t * out_stride + int64_t(h) * v_dim + v] = X(den != 0.f ? num / den : 0.f);
   }
+}
+
+// The expanded rows: NT, PT, VT the padded widths; each part a plane of f16.
+struct Expanded {
+  _Float16 *k, *v, *p;  // [heads][total][NT], [heads][total][VT], [total][PT]
+  int64_t k_plane, v_plane, p_plane;  // to the lower parts
+  int64_t total;
+};
+
+// The product W C^T of 128 weight rows (of the heads' padded rows, keys before values) and 128 positions, the
+// rank in steps of 64: four waves of 64 x 64, operands through LDS, the next step's loads in registers during
+// this step's products.  A lane ends up with 4 consecutive columns of a position's row.  An f32 cache's latents
+// go in as two f16 parts; TWO: the results come out as two.  One more block in x copies the key parts.
+template <int NT, int PT, int VT, typename KV, bool TWO>
+__global__ void __launch_bounds__(256, (sizeof(KV) == 4 ? 1 : 2)) mla_expand_kernel(LatentCache c, int nh, int nope, int v_dim,
+                                                            const _Float16* __restrict__ w, Expanded x) {
+  constexpr bool WIDE = sizeof(KV) == 4;
+  constexpr int WP = NT + VT, CP = WIDE ? 2 : 1;
+  constexpr int TILE = 128 * 128;  // bytes of 128 rows of 64
+  __shared__ __attribute__((aligned(16))) uint8_t s_t[2][1 + CP][TILE];
+  __shared__ int64_t s_row[128];  // the positions' cache rows: -1 for a block that is none, -2 for no position
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int64_t m0 = int64_t(blockIdx.y) * 128;
+  if (tid < 128) {
+    int seq = -1, pos = 0;
+    mla_sequences(c, x.total, lane, [&](int s, int64_t base, int len) {
+      if (m0 + tid >= base && m0 + tid < base + len) seq = s, pos = int(m0 + tid - base);
+      return base + len <= m0 + 127;
+    });
+    s_row[tid] = seq < 0 ? -2 : mla_row(c, seq, pos);
+  }
+  __syncthreads();
+  if (s_row[0] == -2) return;  // behind the last sequence's rows
+  const KV* rows = static_cast<const KV*>(c.rows);
+
+  if (blockIdx.x == gridDim.x - 1) {
+    for (int i = tid; i < 128 * (PT / 8); i += 256) {
+      const int r = i / (PT / 8), k = 8 * (i % (PT / 8));
+      const int64_t at = s_row[r];
+      if (at == -2) continue;
+      float v[8];
+      if (at >= 0 && k < c.rope) load8<KV>(rows + at + c.rank + k, v);
+      else
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = 0.f;
+      h8_t hi, lo;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        _Float16 a, b;
+        split2(v[e], a, b);
+        hi[e] = a, lo[e] = b;
+      }
+      *reinterpret_cast<h8_t*>(x.p + (m0 + r) * PT + k) = hi;
+      if (TWO) *reinterpret_cast<h8_t*>(x.p + x.p_plane + (m0 + r) * PT + k) = lo;
+    }
+    return;
+  }
+
+  const int w0 = blockIdx.x * 128;
+  // thread's chunks of 8 values: rows tid / 8 + 32 i, columns 8 (tid % 8) of a step
+  const int sr = tid >> 3, sk = 8 * (tid & 7);
+  const _Float16* wp[4];
+  int64_t cr[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int idx = w0 + sr + 32 * i, h = idx / WP, j = idx % WP;
+    const bool on = h < nh && (j < NT ? j < nope : j - NT < v_dim);
+    wp[i] = on ? w + (int64_t(h) * (nope + v_dim) + (j < NT ? j : nope + j - NT)) * c.rank : nullptr;
+    cr[i] = s_row[sr + 32 * i];
+  }
+  const u32x4 zero = {0u, 0u, 0u, 0u};
+  u32x4 rw[4], rc[4][CP];
+  auto fetch = [&](int k0) {
+    const int k = k0 + sk;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      rw[i] = wp[i] && k < c.rank ? *reinterpret_cast<const u32x4*>(wp[i] + k) : zero;
+#pragma unroll
+      for (int e = 0; e < CP; e++)
+        rc[i][e] = cr[i] >= 0 && k < c.rank ? *reinterpret_cast<const u32x4*>(rows + cr[i] + k + 4 * e) : zero;
+    }
+  };
+  auto store = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int r = sr + 32 * i, at = r * 128 + 16 * ((sk >> 3) ^ swap8(r));
+      *reinterpret_cast<u32x4*>(&s_t[buf][0][at]) = rw[i];
+      if constexpr (!WIDE) {
+        *reinterpret_cast<u32x4*>(&s_t[buf][1][at]) = rc[i][0];
+      } else {
+        const uint32_t v[8] = {rc[i][0].x, rc[i][0].y, rc[i][0].z, rc[i][0].w,
+                               rc[i][CP - 1].x, rc[i][CP - 1].y, rc[i][CP - 1].z, rc[i][CP - 1].w};
+        h8_t hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          _Float16 a, b;
+          split2(__uint_as_float(v[e]), a, b);
+          hi[e] = a, lo[e] = b;
+        }
+        *reinterpret_cast<h8_t*>(&s_t[buf][1][at]) = hi;
+        *reinterpret_cast<h8_t*>(&s_t[buf][CP][at]) = lo;
+      }
+    }
+  };
+  const int g = lane >> 4, col = lane & 15;
+  const int wr = 64 * (wv & 1), mr = 64 * (wv >> 1);
+  f4_t acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) acc[i][j] = f4_t{0.f, 0.f, 0.f, 0.f};
+  fetch(0);
+  store(0);
+  __syncthreads();
+  const int steps = (c.rank + 63) / 64;
+  for (int s = 0; s < steps; s++) {
+    if (s + 1 < steps) fetch(64 * (s + 1));
+    const uint8_t(*t)[TILE] = s_t[s & 1];
+#pragma unroll
+    for (int kk = 0; kk < 2; kk++) {
+      const int at = 16 * ((4 * kk + g) ^ swap8(col));
+      h8_t a[4], b[4], bl[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        a[i] = *reinterpret_cast<const h8_t*>(&t[0][(wr + 16 * i + col) * 128 + at]);
+        b[i] = *reinterpret_cast<const h8_t*>(&t[1][(mr + 16 * i + col) * 128 + at]);
+        if (WIDE) bl[i] = *reinterpret_cast<const h8_t*>(&t[CP][(mr + 16 * i + col) * 128 + at]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          acc[i][j] = mfma(a[i], b[j], acc[i][j]);
+          if (WIDE) acc[i][j] = mfma(a[i], bl[j], acc[i][j]);
+        }
+    }
+    if (s + 1 < steps) {
+      store((s + 1) & 1);
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int r = mr + 16 * j + col;
+    if (s_row[r] == -2) continue;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int idx = w0 + wr + 16 * i + 4 * g, h = idx / WP, n = idx % WP;
+      if (h >= nh) continue;
+      h4_t hi, lo;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        _Float16 y, z;
+        split2(acc[i][j][e], y, z);
+        hi[e] = y, lo[e] = z;
+      }
+      const int64_t row = int64_t(h) * x.total + m0 + r;
+      if (n < NT) {
+        *reinterpret_cast<h4_t*>(x.k + row * NT + n) = hi;
+        if (TWO) *reinterpret_cast<h4_t*>(x.k + x.k_plane + row * NT + n) = lo;
+      } else {
+        *reinterpret_cast<h4_t*>(x.v + row * VT + n - NT) = hi;
+        if (TWO) *reinterpret_cast<h4_t*>(x.v + x.v_plane + row * VT + n - NT) = lo;
+      }
+    }
+  }
+}
+
+constexpr int kFlashRows = 128;  // tokens a workgroup: 32 a wave
+
+// Shape of the attention kernel: KR positions a step, in LDS as rows of keys, key parts and values (and of their
+// lower parts), chunks swapped by the row's number; two such buffers, two workgroups a CU.
+template <int NT, int PT, int VT, bool TWO>
+struct FlashShape {
+  static constexpr int kPlanes = TWO ? 2 : 1;
+  static constexpr int KR = NT + PT + VT <= 320 && !TWO ? 64 : 32;
+  static constexpr int kKey = KR * NT * 2, kRope = KR * PT * 2, kVal = KR * VT * 2;
+  static constexpr int kPlane = kKey + kRope + kVal;
+  static constexpr int kBuf = kPlane * kPlanes;
+  static constexpr int kGroups = 4 * kBuf <= 160 * 1024 ? 2 : 1;  // workgroups a CU
+  static_assert(2 * kBuf <= 160 * 1024 && kKey % 1024 == 0 && kRope % 1024 == 0 && kVal % 1024 == 0, "tile shape");
+};
+
+// Causal attention of 128 tokens of a sequence and a head, one pass with a running maximum and sum.  S^T =
+// K q^T (positions x tokens) leaves a token per lane column and, taken in the order 4g .. 4g + 3, 16 + 4g .. of
+// 32 positions, is the B operand of O^T += V^T p, V^T read from LDS transposed: numerators, factors and
+// accumulators of a token stay in its lanes.  Accumulators are rescaled only where a maximum grew by 2^8.
+template <int NT, int PT, int VT, typename X, bool TWO>
+__global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
+    mla_flash_kernel(LatentCache c, const X* __restrict__ q, int64_t q_stride, int nope, int v_dim, int nh, int h0,
+                     Expanded x, float scale, MlaRope rope, X* __restrict__ out, int64_t out_stride, int tiles) {
+  using S = FlashShape<NT, PT, VT, TWO>;
+  constexpr int KR = S::KR, RT = KR / 16, KT = (NT + PT) / 32, DT = VT / 16;
+  __shared__ __attribute__((aligned(16))) uint8_t s_kv[2 * S::kBuf];
+  const uint32_t lds0 = uint32_t(uintptr_t((lds_u8*)s_kv));
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, col = lane & 15;
+  // a head's workgroups on one XCD (blocks go round the 8), so that its keys and values stay in one L2; the late
+  // tiles, which attend to the most, first
+  int h, tile;
+  if (nh % 8 == 0) {
+    const int slot = blockIdx.x >> 3, per = nh / 8;
+    h = (slot % per) * 8 + (blockIdx.x & 7);
+    tile = slot / per;
+  } else {
+    h = blockIdx.x % nh;
+    tile = blockIdx.x / nh;
+  }
+  tile = tiles - 1 - tile;
+  // the tile's sequence: tiles of 128 tokens, sequence after sequence
+  int seq = -1, first = 0, count = 0, len = 0, all = 0;
+  int64_t base = 0;
+  {
+    int before = 0;
+    mla_sequences(c, x.total, lane, [&](int s, int64_t b, int n) {
+      int s0 = s, s1 = s + 1;
+      if (c.starts) s0 = c.starts[s], s1 = c.starts[s + 1];
+      const int mine = max(min(s1, c.n_tokens) - max(s0, 0), 0), nt = (mine + kFlashRows - 1) / kFlashRows;
+      if (tile < before + nt) {
+        seq = s, first = max(s0, 0) + (tile - before) * kFlashRows, count = min(kFlashRows, mine - (tile - before) * kFlashRows);
+        base = b, len = n, all = s1;
+        return false;
+      }
+      before += nt;
+      return true;
+    });
+  }
+  if (seq < 0) return;
+  const int64_t shift = int64_t(c.lens[seq]) - all;  // position of token row t: shift + t
+
+  // the queries: B operands, each token's brought near 1 by a power of two that goes into the scores' factor
+  h8_t qh[2][KT], ql[2][TWO ? KT : 1];
+  float factor[2];
+  int limit[2];  // positions the lane's tokens attend to
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    const int i = wv * 32 + 16 * j + col;
+    const int t = first + min(i, count - 1);
+    const int64_t pos = shift + t;
+    limit[j] = i < count ? int(max(int64_t(0), min(pos + 1, int64_t(len)))) : 0;
+    const X* qr = q + t * q_stride + int64_t(h0 + h) * (nope + c.rope);
+    float v[KT][8], mx = 0.f;
+#pragma unroll
+    for (int k = 0; k < KT; k++) {
+      const int d = 32 * k + 8 * g;
+      const bool on = d < NT ? d < nope : d - NT < c.rope;
+      load8<X>(qr + (on ? (d < NT ? d : nope + d - NT) : 0), v[k]);
+      if (d >= NT && rope.on) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float2 cs = mla_cos_sin(rope, on ? (d - NT + e) / 2 : 0, int(pos));
+          const float a = v[k][e], b = v[k][e + 1];
+          v[k][e] = a * cs.x - b * cs.y;
+          v[k][e + 1] = a * cs.y + b * cs.x;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        v[k][e] = on ? v[k][e] : 0.f;
+        mx = fmaxf(mx, fabsf(v[k][e]));
+      }
+    }
+    mx = max_over_groups(mx);
+    int ex = 0;
+    if (mx > 0.f && mx < INFINITY) ex = ilogbf(mx);
+    factor[j] = ldexpf(scale * 1.44269504088896341f, ex);
+#pragma unroll
+    for (int k = 0; k < KT; k++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        _Float16 a, b;
+        split2(ldexpf(v[k][e], -ex), a, b);
+        qh[j][k][e] = a;
+        if (TWO) ql[j][k][e] = b;
+      }
+  }
+  // the workgroup's positions: up to its last token's; those below its first token's need no mask
+  const int top = int(max(int64_t(0), min(shift + first + count, int64_t(len))));
+  const int low = int(max(int64_t(0), min(shift + first + wv * 32 + 1, int64_t(len))));
+  const int steps = (top + KR - 1) / KR;
+  const int32_t* table = c.table + seq * c.table_stride;
+
+  const uint8_t* const kb = reinterpret_cast<const uint8_t*>(x.k + (int64_t(h) * x.total + base) * NT);
+  const uint8_t* const vb = reinterpret_cast<const uint8_t*>(x.v + (int64_t(h) * x.total + base) * VT);
+  const uint8_t* const pb = reinterpret_cast<const uint8_t*>(x.p + base * PT);
+  // rows of 2 w bytes, swap(r) their chunks' swap: LDS bytes from `at` on of buffer buf, load i of 1024 bytes
+  auto part = [&](int i, int p0, const uint8_t* src, int64_t plane, int w, bool four, uint32_t to) {
+    const int b = i * 1024 + 16 * lane, r = b / (2 * w);
+    const int sw = 16 * (four ? swap4(r) : swap8(r));
+    // (a position behind the last repeats it, and is masked)
+    dma_row(src + plane, uint32_t(min(p0 + r, len - 1)) * uint32_t(2 * w) + uint32_t((b % (2 * w)) ^ sw), to + i * 1024);
+  };
+  auto load = [&](int step, int buf) {
+    const int p0 = step * KR;
+#pragma unroll
+    for (int pl = 0; pl < S::kPlanes; pl++) {
+      const uint32_t to = lds0 + buf * S::kBuf + pl * S::kPlane;
+      constexpr int NK = S::kKey / 1024, NR = S::kRope / 1024, NV = S::kVal / 1024;
+      for (int i = wv; i < NK; i += 4) part(i, p0, kb, pl * x.k_plane * 2, NT, false, to);
+      for (int i = wv; i < NR; i += 4) part(i, p0, pb, pl * x.p_plane * 2, PT, PT == 32, to + S::kKey);
+      for (int i = wv; i < NV; i += 4) part(i, p0, vb, pl * x.v_plane * 2, VT, false, to + S::kKey + S::kRope);
+    }
+  };
+  // which of a step's positions have a block (lane r's, in bit r)
+  auto blocks = [&](int step) {
+    const int p = min(step * KR + (lane & (KR - 1)), len - 1);
+    return uint32_t(table[p >> c.shift]) < c.n_blocks;
+  };
+
+  f4_t o[2][DT];
+#pragma unroll
+  for (int j = 0; j < 2; j++)
+#pragma unroll
+    for (int d = 0; d < DT; d++) o[j][d] = f4_t{0.f, 0.f, 0.f, 0.f};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  const int kat = 16 * (g ^ swap8(col)), kat4 = 16 * ((4 + g) ^ swap8(col));
+  const int rat = 16 * (PT == 64 ? g ^ swap8(col) : g ^ swap4(col)), rat4 = 16 * ((4 + g) ^ swap8(col));
+  const int vr = 4 * g + (col >> 2);
+  int vat[4];
+#pragma unroll
+  for (int d = 0; d < 4; d++) vat[d] = vr * VT * 2 + 16 * ((2 * d + ((col & 3) >> 1)) ^ swap8(vr)) + 8 * (col & 1);
+
+  if (steps > 0) load(0, 0);
+  bool there = steps > 0 ? blocks(0) : true;
+  for (int i = 0; i < steps; i++) {
+    const uint64_t ok = __ballot(there);
+    dma_wait<0>();
+    __syncthreads();
+    if (i + 1 < steps) {
+      load(i + 1, (i + 1) & 1);
+      there = blocks(i + 1);
+    }
+    const uint8_t* kv = s_kv + (i & 1) * S::kBuf;
+    f4_t s[2][RT];
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+      for (int r = 0; r < RT; r++) s[j][r] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KT; k++) {
+#pragma unroll
+      for (int r = 0; r < RT; r++) {
+        const int row = 16 * r + col;
+        const uint8_t* p = k < NT / 32 ? kv + row * NT * 2 + ((k & 1) ? kat4 : kat) + 128 * (k >> 1)
+                                       : kv + S::kKey + row * PT * 2 + (((k - NT / 32) & 1) ? rat4 : rat);
+        const h8_t a = *reinterpret_cast<const h8_t*>(p);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          s[j][r] = mfma(a, qh[j][k], s[j][r]);
+          if constexpr (TWO) s[j][r] = mfma(a, ql[j][k], s[j][r]);
+        }
+        if constexpr (TWO) {
+          const h8_t al = *reinterpret_cast<const h8_t*>(p + S::kPlane);
+#pragma unroll
+          for (int j = 0; j < 2; j++) s[j][r] = mfma(al, qh[j][k], s[j][r]);
+        }
+      }
+    }
+    const int p0 = i * KR;
+    h8_t bh[2][RT / 2], bl[2][RT / 2];
+    bool grew[2];
+    float alpha[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[j][r][e] *= factor[j];
+      if (p0 + KR > low || ok != ~0ull) {
+        const uint64_t mine = ok >> (4 * g);
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (p0 + 16 * r + 4 * g + e >= limit[j] || !(mine & (1ull << (16 * r + e)))) s[j][r][e] = -INFINITY;
+      }
+#pragma unroll
+      for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[j][r][e]);
+      mx = max_over_groups(mx);
+      grew[j] = __any(mx > m[j] + 8.f);
+      const float mn = grew[j] ? fmaxf(m[j], mx) : m[j];
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      alpha[j] = __builtin_amdgcn_exp2f(m[j] - ref);
+      m[j] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float p = __builtin_amdgcn_exp2f(s[j][r][e] - ref);
+          sum += p;
+          _Float16 a, b;
+          split2(p, a, b);
+          bh[j][r / 2][4 * (r & 1) + e] = a;
+          bl[j][r / 2][4 * (r & 1) + e] = b;
+        }
+      l[j] = l[j] * alpha[j] + sum;
+    }
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+      if (grew[j])
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[j][d] *= alpha[j];
+    const uint8_t* vp = kv + S::kKey + S::kRope;
+    auto tr = [&](int d, int r, int plane) {
+      return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_s4*)(vp + plane * S::kPlane + vat[d & 3] + 128 * (d >> 2) + 16 * r * VT * 2));
+    };
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+      for (int r = 0; r < RT / 2; r++) {
+        const h8_t v = __builtin_bit_cast(h8_t, __builtin_shufflevector(tr(d, 2 * r, 0), tr(d, 2 * r + 1, 0), 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          o[j][d] = mfma(v, bh[j][r], o[j][d]);
+          if constexpr (TWO) o[j][d] = mfma(v, bl[j][r], o[j][d]);
+        }
+        if constexpr (TWO) {
+          const h8_t w = __builtin_bit_cast(h8_t, __builtin_shufflevector(tr(d, 2 * r, 1), tr(d, 2 * r + 1, 1), 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+          for (int j = 0; j < 2; j++) o[j][d] = mfma(w, bh[j][r], o[j][d]);
+        }
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    const float sum = sum_over_groups(l[j]);
+    const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+    const int i = wv * 32 + 16 * j + col;
+    if (i >= count) continue;
+    X* dst = out + (first + i) * out_stride + int64_t(h0 + h) * v_dim;
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+      const int v = 16 * d + 4 * g;
+      if (v >= v_dim) continue;
+      if constexpr (sizeof(X) == 4) {
+        *reinterpret_cast<f4_t*>(dst + v) = o[j][d] * inv;
+      } else {
+        h4_t y;
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = _Float16(o[j][d][e] * inv);
+        *reinterpret_cast<h4_t*>(dst + v) = y;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host
+
+// The padded widths that a head's take: the smallest of the three the kernels are built for.
+struct PrefillShape {
+  int nt, pt, vt;
+};
+static PrefillShape prefill_shape(int nope, int rope, int v) {
+  if (nope <= 64 && rope <= 32 && v <= 64) return {64, 32, 64};
+  if (nope <= 128 && v <= 128) return {128, 64, 128};
+  return {256, 64, 256};
+}
+
+static size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
+static size_t prefill_bytes(const PrefillShape& s, int64_t total, size_t heads, int planes) {
+  return up256(size_t(total) * s.pt * 2 * planes) + up256(heads * size_t(total) * s.nt * 2 * planes) +
+         up256(heads * size_t(total) * s.vt * 2 * planes);
+}
+
+// Tiles of a call: a sequence's last may be short, so no more than this.
+static int prefill_tiles(const LatentCache& c) {
+  return c.starts ? c.n_tokens / kFlashRows + (c.n_seqs < c.n_tokens ? c.n_seqs : c.n_tokens) : c.n_seqs;
+}
+
+template <int NT, int PT, int VT, typename X, typename KV, bool TWO>
+static int launch_prefill(const LatentCache& c, const X* q, int64_t q_stride, int nh, int h0, int nope, int v_dim,
+                          const _Float16* w, const Expanded& x, float scale, const MlaRope& rope, X* out,
+                          int64_t out_stride, hipStream_t s) {
+  const dim3 ge{unsigned((nh * (NT + VT) + 127) / 128 + 1), unsigned((x.total + 127) / 128), 1};
+  hipLaunchKernelGGL((mla_expand_kernel<NT, PT, VT, KV, TWO>), ge, dim3(256), 0, s, c, nh, nope, v_dim, w, x);
+  int rc = check_launch("mla expand");
+  if (rc) return rc;
+  const int tiles = prefill_tiles(c);
+  hipLaunchKernelGGL((mla_flash_kernel<NT, PT, VT, X, TWO>), dim3(unsigned(tiles) * nh), dim3(256), 0, s, c, q, q_stride,
+                     nope, v_dim, nh, h0, x, scale, rope, out, out_stride, tiles);
+  return check_launch("mla flash");
 }
 
 }  // namespace jero
@@ -104,11 +520,13 @@ using namespace jero;
 
 extern "C" size_t jero_hip_mla_prefill_workspace_bytes(const jero_latent_cache* cache, int act_dtype, int n_heads,
                                                        int nope_dim, int v_dim, int64_t total_len) {
-  (void)act_dtype;
   if (!cache || n_heads < 1 || nope_dim < 1 || v_dim < 1 || total_len < 1) return 0;
-  const size_t one = size_t(total_len) * (nope_dim + v_dim) * sizeof(float);
-  const size_t most = one > (size_t(1) << 30) ? 1 : (size_t(1) << 30) / one;
-  return one * (size_t(n_heads) < most ? size_t(n_heads) : most);
+  const PrefillShape s = prefill_shape(nope_dim, cache->rope_dim, v_dim);
+  const int planes = act_dtype == JERO_F16 ? 1 : 2;
+  const size_t one = prefill_bytes(s, total_len, 1, planes), head = size_t(total_len) * (s.nt + s.vt) * 2 * planes;
+  size_t heads = 1;
+  if (one < (size_t(1) << 30)) heads += ((size_t(1) << 30) - one) / (head + 512);
+  return prefill_bytes(s, total_len, heads < size_t(n_heads) ? heads : size_t(n_heads), planes);
 }
 
 extern "C" int jero_hip_mla_prefill_attention(const jero_latent_cache* cache, int act_dtype, const void* q_dev,
@@ -122,43 +540,61 @@ extern "C" int jero_hip_mla_prefill_attention(const jero_latent_cache* cache, in
   if (rc) return rc;
   if (nope_dim + cache->rope_dim > 256)
     return fail(JERO_ERR_CAPABILITY_MISMATCH, "mla_prefill_attention: nope_dim + rope_dim above 256");
-  if (total_len < 1 || total_len > INT32_MAX)
-    return fail(JERO_ERR_TENSOR_BOUNDS, "mla_prefill_attention: total_len must be 1 to 2^31 - 1");
+  if (total_len < 1 || total_len > (int64_t(1) << 23))
+    return fail(JERO_ERR_TENSOR_BOUNDS, "mla_prefill_attention: total_len must be 1 to 2^23");
   MlaRope rope;
   if ((rc = mla_rope_of(rope_theta, cache->rope_dim, &rope))) return rc;
-  const size_t one = jero_hip_mla_prefill_workspace_bytes(cache, act_dtype, 1, nope_dim, v_dim, total_len);
+  const PrefillShape shape = prefill_shape(nope_dim, cache->rope_dim, v_dim);
+  const int planes = act_dtype == JERO_F16 ? 1 : 2;
   void* ws = workspace_dev;
   if (!ws) {
     workspace_bytes = jero_hip_mla_prefill_workspace_bytes(cache, act_dtype, n_heads, nope_dim, v_dim, total_len);
     if ((rc = workspace(workspace_bytes, &ws))) return rc;
   }
+  const size_t one = prefill_bytes(shape, total_len, 1, planes);
   if (workspace_bytes < one)
     return fail(JERO_ERR_TENSOR_BOUNDS, "mla_prefill_attention: workspace of " + std::to_string(workspace_bytes) +
                                             " bytes, need " + std::to_string(one));
   if (reinterpret_cast<uintptr_t>(ws) & 255u)
     return fail(JERO_ERR_INVALID_ARGUMENT, "mla_prefill_attention: workspace must be 256-byte aligned");
+  int per = n_heads;
+  while (per > 1 && prefill_bytes(shape, total_len, size_t(per), planes) > workspace_bytes) per--;
   const LatentCache c = mla_cache_of(cache, n_tokens);
+  if (int64_t(prefill_tiles(c)) * n_heads > (int64_t(1) << 23))
+    return fail(JERO_ERR_CAPABILITY_MISMATCH, "mla_prefill_attention: more than 2^23 tiles of 128 tokens over the heads");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int wide = nope_dim + v_dim;
-  const int per = int(workspace_bytes / one < size_t(n_heads) ? workspace_bytes / one : size_t(n_heads));
-  float* kv = static_cast<float*>(ws);
   for (int h0 = 0; h0 < n_heads; h0 += per) {
     const int nh = n_heads - h0 < per ? n_heads - h0 : per;
     const _Float16* w = static_cast<const _Float16*>(kv_b_dev) + int64_t(h0) * wide * c.rank;
-    const dim3 ge{unsigned(c.max_len), unsigned(c.n_seqs), 1}, ga{unsigned(n_tokens), unsigned(nh), 1};
-    if (cache->kv_dtype == JERO_KV_F16)
-      hipLaunchKernelGGL((mla_expand_kernel<_Float16>), ge, dim3(256), 0, s, c, nh, wide, w, total_len, kv);
-    else
-      hipLaunchKernelGGL((mla_expand_kernel<float>), ge, dim3(256), 0, s, c, nh, wide, w, total_len, kv);
-    if ((rc = check_launch("mla expand"))) return rc;
-#define JERO_PREFILL(X, KV)                                                                                           \
-  hipLaunchKernelGGL((mla_prefill_kernel<X, KV>), ga, dim3(256), 0, s, c, static_cast<const X*>(q_dev), q_stride, h0, \
-                     nope_dim, v_dim, kv, total_len, scale, rope, static_cast<X*>(out_dev), out_stride)
-    if (act_dtype == JERO_F16) JERO_PREFILL(_Float16, _Float16);
-    else if (cache->kv_dtype == JERO_KV_F16) JERO_PREFILL(float, _Float16);
-    else JERO_PREFILL(float, float);
+    Expanded x;
+    uint8_t* at = static_cast<uint8_t*>(ws);
+    x.total = total_len;
+    x.p_plane = total_len * shape.pt;
+    x.k_plane = int64_t(per) * total_len * shape.nt;
+    x.v_plane = int64_t(per) * total_len * shape.vt;
+    x.p = reinterpret_cast<_Float16*>(at);
+    at += up256(size_t(x.p_plane) * 2 * planes);
+    x.k = reinterpret_cast<_Float16*>(at);
+    at += up256(size_t(x.k_plane) * 2 * planes);
+    x.v = reinterpret_cast<_Float16*>(at);
+#define JERO_PREFILL(NT, PT, VT, X, KV, TWO)                                                                      \
+  rc = launch_prefill<NT, PT, VT, X, KV, TWO>(c, static_cast<const X*>(q_dev), q_stride, nh, h0, nope_dim, v_dim, w, x, \
+                                              scale, rope, static_cast<X*>(out_dev), out_stride, s)
+#define JERO_PREFILL_TYPES(NT, PT, VT)                                                       \
+  if (act_dtype == JERO_F16) JERO_PREFILL(NT, PT, VT, _Float16, _Float16, false);            \
+  else if (cache->kv_dtype == JERO_KV_F16) JERO_PREFILL(NT, PT, VT, float, _Float16, true);  \
+  else JERO_PREFILL(NT, PT, VT, float, float, true)
+    if (shape.nt == 64) {
+      JERO_PREFILL_TYPES(64, 32, 64);
+    } else if (shape.nt == 128) {
+      JERO_PREFILL_TYPES(128, 64, 128);
+    } else {
+      JERO_PREFILL_TYPES(256, 64, 256);
+    }
+#undef JERO_PREFILL_TYPES
 #undef JERO_PREFILL
-    if ((rc = check_launch("mla prefill"))) return rc;
+    if (rc) return rc;
   }
   return JERO_OK;
 }
