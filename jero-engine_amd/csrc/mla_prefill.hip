@@ -206,7 +206,7 @@ struct FlashShape {
   static constexpr int kPlane = kKey + kRope + kVal;
   static constexpr int kBuf = kPlane * kPlanes;
   static constexpr int kGroups = 4 * kBuf <= 160 * 1024 ? 2 : 1;  // workgroups a CU
-  static_assert(2 * kBuf <= 160 * 1024 && kKey % 1024 == 0 && kRope % 1024 == 0 && kVal % 1024 == 0, "tile shape");
+  static_assert(2 * kBuf <= 160 * 1024 && kKey % 4096 == 0 && kRope % 1024 == 0 && kVal % 4096 == 0, "tile shape");
 };
 
 // Causal attention of 128 tokens of a sequence and a head, one pass with a running maximum and sum.  S^T =
@@ -324,15 +324,19 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
     for (int pl = 0; pl < S::kPlanes; pl++) {
       const uint32_t to = lds0 + buf * S::kBuf + pl * S::kPlane;
       constexpr int NK = S::kKey / 1024, NR = S::kRope / 1024, NV = S::kVal / 1024;
-      for (int i = wv; i < NK; i += 4) part(i, p0, kb, pl * x.k_plane * 2, NT, false, to);
-      for (int i = wv; i < NR; i += 4) part(i, p0, pb, pl * x.p_plane * 2, PT, PT == 32, to + S::kKey);
-      for (int i = wv; i < NV; i += 4) part(i, p0, vb, pl * x.v_plane * 2, VT, false, to + S::kKey + S::kRope);
+#pragma unroll
+      for (int i = 0; i < NK; i += 4) part(i + wv, p0, kb, pl * x.k_plane * 2, NT, false, to);
+#pragma unroll
+      for (int i = 0; i < NR; i += 4)
+        if (NR % 4 == 0 || i + wv < NR) part(i + wv, p0, pb, pl * x.p_plane * 2, PT, PT == 32, to + S::kKey);
+#pragma unroll
+      for (int i = 0; i < NV; i += 4) part(i + wv, p0, vb, pl * x.v_plane * 2, VT, false, to + S::kKey + S::kRope);
     }
   };
-  // which of a step's positions have a block (lane r's, in bit r)
-  auto blocks = [&](int step) {
+  // the block of a step's position lane
+  auto block = [&](int step) {
     const int p = min(step * KR + (lane & (KR - 1)), len - 1);
-    return uint32_t(table[p >> c.shift]) < c.n_blocks;
+    return uint32_t(table[p >> c.shift]);
   };
 
   f4_t o[2][DT];
@@ -349,14 +353,14 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
   for (int d = 0; d < 4; d++) vat[d] = vr * VT * 2 + 16 * ((2 * d + ((col & 3) >> 1)) ^ swap8(vr)) + 8 * (col & 1);
 
   if (steps > 0) load(0, 0);
-  bool there = steps > 0 ? blocks(0) : true;
+  uint32_t ids = steps > 0 ? block(0) : 0;
   for (int i = 0; i < steps; i++) {
-    const uint64_t ok = __ballot(there);
     dma_wait<0>();
+    const uint64_t ok = __ballot(ids < c.n_blocks);  // (its load has come with the others: waited for before)
     __syncthreads();
     if (i + 1 < steps) {
       load(i + 1, (i + 1) & 1);
-      there = blocks(i + 1);
+      ids = block(i + 1);
     }
     const uint8_t* kv = s_kv + (i & 1) * S::kBuf;
     f4_t s[2][RT];
@@ -364,25 +368,38 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
     for (int j = 0; j < 2; j++)
 #pragma unroll
       for (int r = 0; r < RT; r++) s[j][r] = f4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < KT; k++) {
+    // operands are read a group of products ahead
+    constexpr int KP = S::kPlanes;
+    h8_t ka[2][RT][KP];
+    auto read_k = [&](int k) {
 #pragma unroll
       for (int r = 0; r < RT; r++) {
         const int row = 16 * r + col;
         const uint8_t* p = k < NT / 32 ? kv + row * NT * 2 + ((k & 1) ? kat4 : kat) + 128 * (k >> 1)
                                        : kv + S::kKey + row * PT * 2 + (((k - NT / 32) & 1) ? rat4 : rat);
-        const h8_t a = *reinterpret_cast<const h8_t*>(p);
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-          s[j][r] = mfma(a, qh[j][k], s[j][r]);
-          if constexpr (TWO) s[j][r] = mfma(a, ql[j][k], s[j][r]);
-        }
-        if constexpr (TWO) {
-          const h8_t al = *reinterpret_cast<const h8_t*>(p + S::kPlane);
-#pragma unroll
-          for (int j = 0; j < 2; j++) s[j][r] = mfma(al, qh[j][k], s[j][r]);
-        }
+        for (int e = 0; e < KP; e++) ka[k & 1][r][e] = *reinterpret_cast<const h8_t*>(p + e * S::kPlane);
       }
+    };
+    read_k(0);
+#pragma unroll
+    for (int k = 0; k < KT; k++) {
+      if (k + 1 < KT) read_k(k + 1);
+#pragma unroll
+      for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) s[j][r] = mfma(ka[k & 1][r][0], qh[j][k], s[j][r]);
+      if constexpr (TWO) {
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+          for (int j = 0; j < 2; j++) s[j][r] = mfma(ka[k & 1][r][0], ql[j][k], s[j][r]);
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+          for (int j = 0; j < 2; j++) s[j][r] = mfma(ka[k & 1][r][KP - 1], qh[j][k], s[j][r]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
     const int p0 = i * KR;
     h8_t bh[2][RT / 2], bl[2][RT / 2];
@@ -437,22 +454,32 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
       return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           (lds_s4*)(vp + plane * S::kPlane + vat[d & 3] + 128 * (d >> 2) + 16 * r * VT * 2));
     };
+    h8_t va[2][RT / 2][KP];
+    auto read_v = [&](int d) {
 #pragma unroll
-    for (int d = 0; d < DT; d++)
+      for (int r = 0; r < RT / 2; r++)
+#pragma unroll
+        for (int e = 0; e < KP; e++)
+          va[d & 1][r][e] = __builtin_bit_cast(
+              h8_t, __builtin_shufflevector(tr(d, 2 * r, e), tr(d, 2 * r + 1, e), 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    read_v(0);
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+      if (d + 1 < DT) read_v(d + 1);
 #pragma unroll
       for (int r = 0; r < RT / 2; r++) {
-        const h8_t v = __builtin_bit_cast(h8_t, __builtin_shufflevector(tr(d, 2 * r, 0), tr(d, 2 * r + 1, 0), 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-          o[j][d] = mfma(v, bh[j][r], o[j][d]);
-          if constexpr (TWO) o[j][d] = mfma(v, bl[j][r], o[j][d]);
-        }
+        for (int j = 0; j < 2; j++) o[j][d] = mfma(va[d & 1][r][0], bh[j][r], o[j][d]);
         if constexpr (TWO) {
-          const h8_t w = __builtin_bit_cast(h8_t, __builtin_shufflevector(tr(d, 2 * r, 1), tr(d, 2 * r + 1, 1), 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-          for (int j = 0; j < 2; j++) o[j][d] = mfma(w, bh[j][r], o[j][d]);
+          for (int j = 0; j < 2; j++) o[j][d] = mfma(va[d & 1][r][0], bl[j][r], o[j][d]);
+#pragma unroll
+          for (int j = 0; j < 2; j++) o[j][d] = mfma(va[d & 1][r][KP - 1], bh[j][r], o[j][d]);
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 #pragma unroll
   for (int j = 0; j < 2; j++) {
