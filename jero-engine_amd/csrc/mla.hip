@@ -2,6 +2,7 @@
 #include "mla.h"
 
 #include <cmath>
+#include <type_traits>
 
 namespace jero {
 
@@ -85,82 +86,141 @@ __device__ __forceinline__ bool mla_locate_thread(const LatentCache& c, int t, i
   return true;
 }
 
-// Grid (tiles of 64 latent columns, then one for the key part, then one for the plan; heads; tokens by
-// 64).  A wave holds 16 rows of W_uk^T in registers and takes the tokens 16 at a time: one read of the
-// weights for 64 tokens, which is all this kernel costs for a few.  f32 queries go in as two f16 parts.
+// The absorbed queries, as the attend kernel's waves take them: for each token and 16 heads, and each 32 of
+// the padded columns (rt for the latent, then the key part's), the 64 lanes' 8 halves of an MFMA operand (lane
+// 16 g + i: head i, columns 8g ..); the upper parts, and `plane` further on the lower ones.  A head's row is
+// brought near 1 by a power of two, so that its parts stay within f16's range; factor holds what is to be
+// multiplied onto its scores, in log2.
+struct MlaQueries {
+  _Float16* parts;
+  float* factor;  // [T][heads to whole 16s]
+  int64_t plane;
+  int rt, kt;     // padded latent columns, 32s of all columns
+};
+
+// Grid (heads, then one for the plan; tokens by 16).  The 8 waves take the head's rows of W_uk^T by 16; a
+// thread rotates a pair of the key part; the row's largest value is the scale of its parts.
 template <typename X, int NT>
-__global__ void __launch_bounds__(256) mla_absorb_kernel(LatentCache c, const X* __restrict__ q, int64_t q_stride,
+__global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X* __restrict__ q, int64_t q_stride, int nh,
                                                          int nope, const _Float16* __restrict__ k_b, MlaRope rope,
-                                                         float* __restrict__ qa, MlaPlan plan, int tile) {
-  const int h = blockIdx.y, nh = gridDim.y, t0 = blockIdx.z * 64;
+                                                         float scale, MlaQueries qa, MlaPlan plan, int tile, int extra) {
+  const int h = blockIdx.x, t0 = blockIdx.y * 16;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  const int nr = (c.rank + 63) / 64;
-  const int64_t qh = int64_t(h) * (nope + c.rope);
-  if (int(blockIdx.x) < nr) {
+  if (h < nh) {
+    constexpr int NR = kMlaMaxRank / 128;  // 16s of rows a wave
+    __shared__ float s_max[8][16];
+    __shared__ uint32_t s_key[16];
     const int g = lane >> 4, col = lane & 15;
-    const int r0 = blockIdx.x * 64 + wv * 16;
-    if (r0 >= c.rank) return;
-    const int r = min(r0 + col, c.rank - 1);
-    const _Float16* w = k_b + (int64_t(h) * c.rank + r) * nope;
-    h8_t b[NT];
-#pragma unroll
-    for (int i = 0; i < NT; i++) b[i] = *reinterpret_cast<const h8_t*>(w + min(32 * i + 8 * g, nope - 8));
-    for (int t = t0; t < min(t0 + 64, c.n_tokens); t += 16) {
-      const X* qr = q + min(t + col, c.n_tokens - 1) * q_stride + qh;
-      f4_t hi = {0.f, 0.f, 0.f, 0.f}, lo = hi;
-#pragma unroll
-      for (int i = 0; i < NT; i++) {
-        float v[8];
-        load8<X>(qr + min(32 * i + 8 * g, nope - 8), v);
-        h8_t ah, al;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          _Float16 x, y;
-          split2(32 * i + 8 * g < nope ? v[e] : 0.f, x, y);
-          ah[e] = x, al[e] = y;
-        }
-        hi = mfma(ah, b[i], hi);
-        if (sizeof(X) == 4) lo = mfma(al, b[i], lo);
+    const X* qr = q + min(t0 + col, c.n_tokens - 1) * q_stride + int64_t(h) * (nope + c.rope);
+    if (tid < 16) s_key[tid] = 0;
+    // the key part, its pair of the thread's token
+    const int pairs = c.rope / 2, kt_ = tid / pairs, ki = tid % pairs;
+    float ka = 0.f, kb = 0.f;
+    const bool key = kt_ < 16 && t0 + kt_ < c.n_tokens;
+    if (key) {
+      const X* kp = q + (t0 + kt_) * q_stride + int64_t(h) * (nope + c.rope) + nope + 2 * ki;
+      const float x = float(kp[0]), y = float(kp[1]);
+      float2 cs = make_float2(1.f, 0.f);
+      if (rope.on) {
+        int seq, pos;
+        if (!mla_locate_thread(c, t0 + kt_, seq, pos)) pos = 0;
+        cs = mla_cos_sin(rope, ki, pos);
       }
-      if (r0 + col < c.rank)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          if (t + 4 * g + e < c.n_tokens) qa[(int64_t(t + 4 * g + e) * nh + h) * c.width + r0 + col] = hi[e] + lo[e];
+      ka = x * cs.x - y * cs.y;
+      kb = x * cs.y + y * cs.x;
     }
-    return;
-  }
-  if (int(blockIdx.x) == nr) {  // the key part
-    __shared__ int s_pos[64];
-    if (tid < 64) {
-      int seq, pos = -1;
-      if (t0 + tid < c.n_tokens && !mla_locate_thread(c, t0 + tid, seq, pos)) pos = -1;
-      s_pos[tid] = pos;
+    h8_t ah[NT], al[NT];
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+      float v[8];
+      load8<X>(qr + min(32 * i + 8 * g, nope - 8), v);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        _Float16 x, y;
+        split2(32 * i + 8 * g < nope ? v[e] : 0.f, x, y);
+        ah[i][e] = x, al[i][e] = y;
+      }
+    }
+    f4_t v[NR];
+    float mx[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < NR; k++) {
+      const int r0 = 16 * (wv + 8 * k);
+      f4_t hi = {0.f, 0.f, 0.f, 0.f}, lo = hi;
+      if (r0 < c.rank) {
+        const _Float16* w = k_b + (int64_t(h) * c.rank + min(r0 + col, c.rank - 1)) * nope;
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+          const h8_t b = *reinterpret_cast<const h8_t*>(w + min(32 * i + 8 * g, nope - 8));
+          hi = mfma(ah[i], b, hi);
+          if (sizeof(X) == 4) lo = mfma(al[i], b, lo);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        v[k][e] = r0 + col < c.rank ? hi[e] + lo[e] : 0.f;
+        mx[e] = fmaxf(mx[e], fabsf(v[k][e]));
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {  // over the 16 lanes of a row
+      mx[e] = dpp_max<0xB1, 0xF>(mx[e]);
+      mx[e] = dpp_max<0x4E, 0xF>(mx[e]);
+      mx[e] = dpp_max<0x124, 0xF>(mx[e]);
+      mx[e] = dpp_max<0x128, 0xF>(mx[e]);
+      if (col == 0) s_max[wv][4 * g + e] = mx[e];
     }
     __syncthreads();
-    const int pairs = c.rope / 2, n = min(64, c.n_tokens - t0) * pairs;
-    for (int k = tid; k < n; k += 256) {
-      const int t = k / pairs, i = k % pairs;
-      const X* qr = q + (t0 + t) * q_stride + qh + nope + 2 * i;
-      const float x = float(qr[0]), y = float(qr[1]);
-      const float2 cs = rope.on ? mla_cos_sin(rope, i, s_pos[t]) : make_float2(1.f, 0.f);
-      float* o = qa + (int64_t(t0 + t) * nh + h) * c.width + c.rank + 2 * i;
-      o[0] = x * cs.x - y * cs.y;
-      o[1] = x * cs.y + y * cs.x;
+    if (key) atomicMax(&s_key[kt_], __float_as_uint(fmaxf(fabsf(ka), fabsf(kb))));
+    __syncthreads();
+    auto power = [&](int t) {  // of the token's largest value; 0 for a row of zeros, or one that is not finite
+      float x = __uint_as_float(s_key[t]);
+      for (int w = 0; w < 8; w++) x = fmaxf(x, s_max[w][t]);
+      return x > 0.f && x < INFINITY ? ilogbf(x) : 0;
+    };
+    const int groups = (nh + 15) / 16;
+    _Float16* const out = qa.parts + ((int64_t(t0) * groups + h / 16) * qa.kt) * 512 + (h % 16) * 8;
+    auto put = [&](int t, int k, float x) {
+      _Float16 hi, lo;
+      split2(x, hi, lo);
+      _Float16* p = out + (int64_t(t) * groups * qa.kt + k / 32) * 512 + ((k % 32) / 8) * 128 + k % 8;
+      p[0] = hi;
+      if (sizeof(X) == 4) p[qa.plane] = lo;
+    };
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int t = 4 * g + e, ex = power(t);
+      if (t0 + t >= c.n_tokens) continue;
+#pragma unroll
+      for (int k = 0; k < NR; k++) {
+        const int r = 16 * (wv + 8 * k) + col;
+        if (r < qa.rt) put(t, r, ldexpf(v[k][e], -ex));
+      }
     }
+    if (key) {
+      const int ex = power(kt_);
+      put(kt_, qa.rt + 2 * ki, ldexpf(ka, -ex));
+      put(kt_, qa.rt + 2 * ki + 1, ldexpf(kb, -ex));
+      if (ki == 0)
+        qa.factor[int64_t(t0 + kt_) * groups * 16 + h] = ldexpf(scale * 1.44269504088896341f, ex);
+    }
+    const int pad = 32 * qa.kt - qa.rt - c.rope;  // columns of no pair
+    if (tid < 16 * pad && t0 + tid / pad < c.n_tokens) put(tid / pad, qa.rt + c.rope + tid % pad, 0.f);
     return;
   }
-  if (h || t0) return;
-  // the plan: 256 tokens at a time, a scan of their tiles
-  __shared__ int s_scan[4];
+  if (t0) return;
+  // the plan: 512 tokens at a time, a scan of their units (the tiles, and for a token that has any as many as
+  // beginning it takes)
+  __shared__ int s_scan[8];
   int base = 0;
-  for (int first = 0; first < c.n_tokens; first += 256) {
+  for (int first = 0; first < c.n_tokens; first += 512) {
     const int t = first + tid;
     int seq = -1, pos = -1, end = 0;
     if (t < c.n_tokens) {
       if (!mla_locate_thread(c, t, seq, pos)) seq = -1, pos = -1;
-      end = pos < 0 ? 0 : min(int(min(int64_t(pos) + 1, int64_t(c.max_len))), c.max_len);
+      end = pos < 0 ? 0 : int(min(int64_t(pos) + 1, int64_t(c.max_len)));
     }
-    const int mine = (end + tile - 1) / tile;
+    const int mine = end > 0 ? (end + tile - 1) / tile + extra : 0;
     int sum = mine;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -170,21 +230,22 @@ __global__ void __launch_bounds__(256) mla_absorb_kernel(LatentCache c, const X*
     if (lane == 63) s_scan[wv] = sum;
     __syncthreads();
     int before = base;
-    for (int w = 0; w < wv; w++) before += s_scan[w];
-    const int all = s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
+    for (int w = 0; w < 8; w++) {
+      if (w < wv) before += s_scan[w];
+      base += s_scan[w];
+    }
     if (t < c.n_tokens) {
       plan.prefix[t] = before + sum - mine;
       plan.seq[t] = seq;
       plan.end[t] = end;
     }
-    base += all;
     __syncthreads();
   }
   if (tid == 0) plan.prefix[c.n_tokens] = base;
 }
 
-// Tiles of a run: the plan's tiles over the runs, at least `least` each.
-__device__ __forceinline__ int mla_per_run(int tiles, int runs, int least) { return max((tiles + runs - 1) / runs, least); }
+// Units of a run: the plan's over the runs, at least `least` each.
+__device__ __forceinline__ int mla_per_run(int units, int runs, int least) { return max((units + runs - 1) / runs, least); }
 
 // The last token whose prefix is not behind tile x, 64 candidates at a time.
 __device__ __forceinline__ int mla_token_of(const int* prefix, int n, int x, int lane) {
@@ -249,7 +310,7 @@ struct AttendShape {
 // on their way from the cache meanwhile (f16 cache; an f32 one has its LDS filled by the parts of one step).
 template <int RT, int PT, int HG, int KS, typename KV, bool TWO>
 __global__ void __launch_bounds__(64 * HG * KS, 1)
-    mla_attend_kernel(LatentCache c, const float* __restrict__ qa, int nh, float scale, MlaPlan plan, int runs, int least,
+    mla_attend_kernel(LatentCache c, MlaQueries qa, int nh, MlaPlan plan, int runs, int least, int extra,
                       float* __restrict__ part_o, float2* __restrict__ part_ml) {
   using S = AttendShape<RT, PT, HG, KS, KV>;
   constexpr bool WIDE = S::kWide;
@@ -289,11 +350,12 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
   } else {
     t = __popcll(__ballot(lane < n_tok && w_prefix <= x)) - 1;
   }
-  for (; x < x_end; t++) {
+  for (; x < x_end && t < n_tok; t++) {
     if (t - t0 > 62) window(t);
-    const int first = __builtin_amdgcn_readlane(w_prefix, t - t0);
+    const int first = __builtin_amdgcn_readlane(w_prefix, t - t0) + extra;  // unit of the token's first tile
     const int last = min(__builtin_amdgcn_readlane(w_prefix, t - t0 + 1), x_end);
-    if (last <= x) continue;  // a token without positions
+    x = max(x, first);
+    if (last <= x) continue;  // a token without positions, or with none in this run
     const int seq = __builtin_amdgcn_readlane(w_seq, t - t0), end = __builtin_amdgcn_readlane(w_end, t - t0);
     const int32_t* table = c.table + seq * c.table_stride;
     const int p0 = (x - first) * TR, steps = last - x;
@@ -390,41 +452,15 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
         for (int i = 0; i < S::kLoads; i++) load(i, j);
       }
 
-    // the absorbed queries of the wave's heads: B operands, each head brought near 1 by a power of two so that
-    // its parts stay within f16's range, which goes into the score's factor
+    // the absorbed queries of the wave's heads
     h8_t qh[KT], ql[TWO ? KT : 1];
-    float factor;
-    {
-      const float* qr = qa + (int64_t(t) * nh + head) * c.width;
-      float v[KT][8], mx = 0.f;
+    const int g16 = (nh + 15) / 16;
+    const _Float16* const qp = qa.parts + (int64_t(t) * g16 + min(h0 / 16, g16 - 1)) * KT * 512 + 8 * lane;
+    const float factor = qa.factor[int64_t(t) * g16 * 16 + head];
 #pragma unroll
-      for (int i = 0; i < KT; i++) {
-        const int k = 32 * i + 8 * g;
-        const bool on = k < RT ? k < c.rank : k - RT < c.rope;
-        load8<float>(qr + (on ? (k < RT ? k : c.rank + k - RT) : 0), v[i]);
-      }
-      __builtin_amdgcn_sched_barrier(0);  // one round trip for the row
-#pragma unroll
-      for (int i = 0; i < KT; i++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[i][e]));  // a repeated element changes nothing
-      mx = max_over_groups(mx);
-      int ex = 0;
-      if (mx > 0.f && mx < INFINITY) ex = ilogbf(mx);
-      factor = ldexpf(scale * 1.44269504088896341f, ex);
-#pragma unroll
-      for (int i = 0; i < KT; i++) {
-        const int k = 32 * i + 8 * g;
-        const bool on = k < RT ? k < c.rank : k - RT < c.rope;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          _Float16 a, b;
-          split2(on ? ldexpf(v[i][e], -ex) : 0.f, a, b);
-          qh[i][e] = a;
-          if (TWO) ql[i][e] = b;
-        }
-        __builtin_amdgcn_sched_barrier(0);  // in order: v's registers become the parts'
-      }
+    for (int i = 0; i < KT; i++) {
+      qh[i] = *reinterpret_cast<const h8_t*>(qp + 512 * i);
+      if (TWO) ql[i] = *reinterpret_cast<const h8_t*>(qp + qa.plane + 512 * i);
     }
     f4_t o[DT];
 #pragma unroll
@@ -445,39 +481,39 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
       for (int d = 0; d < NVV; d++) vv[d] = S::lat(vr, 2 * d + ((col & 3) >> 1)) + 8 * (col & 1);
     }
     f4_t sa[NT], sb[NT];  // the scores of a step, in two sums
-    constexpr int QG = KT % 2 || (TWO && NT == 2) ? 1 : 2, QN = KT / QG;  // k steps a group, groups
-    h8_t ka[2][QG][NT], kb[WIDE ? 2 : 1][QG][NT];
-    auto read_k = [&](int grp, const uint8_t* kv) {
+    constexpr int QN = KT;                             // groups of products: one k step each
+    constexpr int KD = (NT == 1 ? 8 : 5) / (WIDE ? 2 : 1);  // groups whose operands are on their way
+    h8_t ka[KD + 1][NT], kb[WIDE ? KD + 1 : 1][NT];
+    auto read_k = [&](int k, const uint8_t* kv) {
 #pragma unroll
-      for (int i = 0; i < QG; i++)
-#pragma unroll
-        for (int j = 0; j < NT; j++) {
-          const int k = grp * QG + i;
-          const uint8_t* p = kv + (k < RT / 32 ? kl[k % NKL] + 64 * (k - k % NKL) + 16 * j * S::kPitch
-                                               : kk[(k - RT / 32) & 1] + 16 * j * PT * 2);
-          ka[grp & 1][i][j] = *reinterpret_cast<const h8_t*>(p);
-          if constexpr (WIDE) kb[grp & 1][i][j] = *reinterpret_cast<const h8_t*>(p + S::kBuf);
-        }
+      for (int j = 0; j < NT; j++) {
+        const uint8_t* p = kv + (k < RT / 32 ? kl[k % NKL] + 64 * (k - k % NKL) + 16 * j * S::kPitch
+                                             : kk[(k - RT / 32) & 1] + 16 * j * PT * 2);
+        ka[k % (KD + 1)][j] = *reinterpret_cast<const h8_t*>(p);
+        if constexpr (WIDE) kb[k % (KD + 1)][j] = *reinterpret_cast<const h8_t*>(p + S::kBuf);
+      }
     };
     // the scores of the step in buffer kv; between the groups of products, between(group)
     auto scores = [&](const uint8_t* kv, f4_t (&a)[NT], f4_t (&b)[NT], auto between) {
 #pragma unroll
       for (int j = 0; j < NT; j++) a[j] = b[j] = f4_t{0.f, 0.f, 0.f, 0.f};
-      read_k(0, kv);
 #pragma unroll
-      for (int grp = 0; grp < QN; grp++) {
-        if (grp + 1 < QN) read_k(grp + 1, kv);
-        between(grp);
+      for (int k = 0; k < KD && k < QN; k++) read_k(k, kv);
 #pragma unroll
-        for (int i = 0; i < QG; i++)
+      for (int k = 0; k < QN; k++) {
+        if (k + KD < QN) read_k(k + KD, kv);
+        between(k);
+        constexpr int M = KD + 1;
 #pragma unroll
-          for (int j = 0; j < NT; j++) {
-            const int k = grp * QG + i;
-            if (!TWO && (k & 1)) b[j] = mfma(ka[grp & 1][i][j], qh[k], b[j]);  // two chains
-            else a[j] = mfma(ka[grp & 1][i][j], qh[k], a[j]);
-            if constexpr (TWO) b[j] = mfma(ka[grp & 1][i][j], ql[k], b[j]);
-            if constexpr (WIDE) b[j] = mfma(kb[grp & 1][i][j], qh[k], b[j]);
-          }
+        for (int j = 0; j < NT; j++) {
+          if (!TWO && (k & 1)) b[j] = mfma(ka[k % M][j], qh[k], b[j]);  // two chains
+          else a[j] = mfma(ka[k % M][j], qh[k], a[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+          if constexpr (TWO) b[j] = mfma(ka[k % M][j], ql[k], b[j]);
+          if constexpr (WIDE) b[j] = mfma(kb[k % M][j], qh[k], b[j]);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     };
@@ -529,69 +565,44 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
         return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
             (lds_s4*)(kv + vv[d % NVV] + plane * S::kBuf + 32 * (d - d % NVV) + 16 * j * S::kPitch));
       };
-      constexpr int VG = 4, VN = DT / VG;  // tiles of 16 latent columns a group
-      if constexpr (NT == 1) {
-        const h4_t bh = {ph[0], ph[1], ph[2], ph[3]}, bl = {pl[0], pl[1], pl[2], pl[3]};
-        h4_t va[2][VG], vl[WIDE ? 2 : 1][VG];
-        auto read_v = [&](int grp) {
+      constexpr int VG = 2, VN = DT / VG;               // tiles of 16 latent columns a group
+      constexpr int VD = (NT == 1 ? 6 : 3) / (WIDE ? 2 : 1);  // groups on their way
+      typedef std::conditional_t<NT == 1, h4_t, h8_t> v_t;
+      v_t bh, bl, va[VD + 1][VG], vl[WIDE ? VD + 1 : 1][VG];
 #pragma unroll
-          for (int i = 0; i < VG; i++) {
-            va[grp & 1][i] = __builtin_bit_cast(h4_t, tr(grp * VG + i, 0, 0));
-            if constexpr (WIDE) vl[grp & 1][i] = __builtin_bit_cast(h4_t, tr(grp * VG + i, 0, 1));
-          }
-        };
-        read_v(0);
+      for (int e = 0; e < 4 * NT; e++) bh[e] = ph[e], bl[e] = pl[e];
+      auto operand = [&](int d, int plane) {
+        if constexpr (NT == 1) return __builtin_bit_cast(h4_t, tr(d, 0, plane));
+        else
+          return __builtin_bit_cast(h8_t,
+                                    __builtin_shufflevector(tr(d, 0, plane), tr(d, 1, plane), 0, 1, 2, 3, 4, 5, 6, 7));
+      };
+      auto read_v = [&](int grp) {
 #pragma unroll
-        for (int grp = 0; grp < VN; grp++) {
-          if (grp + 1 < VN) read_v(grp + 1);
-#pragma unroll
-          for (int i = 0; i < VG; i++) {
-            f4_t& d = o[grp * VG + i];
-            d = __builtin_amdgcn_mfma_f32_16x16x16f16(va[grp & 1][i], bh, d, 0, 0, 0);
-          }
-          if constexpr (TWO)
-#pragma unroll
-            for (int i = 0; i < VG; i++) {
-              f4_t& d = o[grp * VG + i];
-              d = __builtin_amdgcn_mfma_f32_16x16x16f16(va[grp & 1][i], bl, d, 0, 0, 0);
-            }
-          if constexpr (WIDE)
-#pragma unroll
-            for (int i = 0; i < VG; i++) {
-              f4_t& d = o[grp * VG + i];
-              d = __builtin_amdgcn_mfma_f32_16x16x16f16(vl[grp & 1][i], bh, d, 0, 0, 0);
-            }
-          __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < VG; i++) {
+          va[grp % (VD + 1)][i] = operand(grp * VG + i, 0);
+          if constexpr (WIDE) vl[grp % (VD + 1)][i] = operand(grp * VG + i, 1);
         }
-      } else {
-        h8_t bh, bl;
+      };
+      auto add = [&](f4_t& d, v_t v, v_t p) {
+        if constexpr (NT == 1) d = __builtin_amdgcn_mfma_f32_16x16x16f16(v, p, d, 0, 0, 0);
+        else d = mfma(v, p, d);
+      };
 #pragma unroll
-        for (int e = 0; e < 8; e++) bh[e] = ph[e], bl[e] = pl[e];
-        h8_t va[2][VG], vl[WIDE ? 2 : 1][VG];
-        auto both = [&](int d, int plane) {
-          return __builtin_bit_cast(h8_t, __builtin_shufflevector(tr(d, 0, plane), tr(d, 1, plane), 0, 1, 2, 3, 4, 5, 6, 7));
-        };
-        auto read_v = [&](int grp) {
+      for (int grp = 0; grp < VD && grp < VN; grp++) read_v(grp);
 #pragma unroll
-          for (int i = 0; i < VG; i++) {
-            va[grp & 1][i] = both(grp * VG + i, 0);
-            if constexpr (WIDE) vl[grp & 1][i] = both(grp * VG + i, 1);
-          }
-        };
-        read_v(0);
+      for (int grp = 0; grp < VN; grp++) {
+        if (grp + VD < VN) read_v(grp + VD);
+        constexpr int M = VD + 1;
 #pragma unroll
-        for (int grp = 0; grp < VN; grp++) {
-          if (grp + 1 < VN) read_v(grp + 1);
+        for (int i = 0; i < VG; i++) add(o[grp * VG + i], va[grp % M][i], bh);
+        if constexpr (TWO)
 #pragma unroll
-          for (int i = 0; i < VG; i++) o[grp * VG + i] = mfma(va[grp & 1][i], bh, o[grp * VG + i]);
-          if constexpr (TWO)
+          for (int i = 0; i < VG; i++) add(o[grp * VG + i], va[grp % M][i], bl);
+        if constexpr (WIDE)
 #pragma unroll
-            for (int i = 0; i < VG; i++) o[grp * VG + i] = mfma(va[grp & 1][i], bl, o[grp * VG + i]);
-          if constexpr (WIDE)
-#pragma unroll
-            for (int i = 0; i < VG; i++) o[grp * VG + i] = mfma(vl[grp & 1][i], bh, o[grp * VG + i]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+          for (int i = 0; i < VG; i++) add(o[grp * VG + i], vl[grp % M][i], bh);
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
 
@@ -712,8 +723,8 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
 template <typename X, int RT>
 __global__ void __launch_bounds__(512) mla_values_kernel(LatentCache c, const float* __restrict__ part_o,
                                                          const float2* __restrict__ part_ml, MlaPlan plan, int runs,
-                                                         int least, const _Float16* __restrict__ v_b, int v_dim,
-                                                         X* __restrict__ out, int64_t out_stride) {
+                                                         int least, int extra, const _Float16* __restrict__ v_b,
+                                                         int v_dim, X* __restrict__ out, int64_t out_stride) {
   constexpr int KT = RT / 32, P = RT + 8, NW = 8, U = 8;
   __shared__ __attribute__((aligned(16))) _Float16 s_hi[16][P], s_lo[16][P];
   __shared__ float s_acc[NW][RT];
@@ -785,7 +796,7 @@ __global__ void __launch_bounds__(512) mla_values_kernel(LatentCache c, const fl
     }
   };
   auto range = [&](int t, int& w0, int& w1) {
-    const int a = plan.prefix[t], e = plan.prefix[t + 1];
+    const int a = plan.prefix[t] + extra, e = plan.prefix[t + 1];
     w0 = a / per;
     w1 = e > a ? (e - 1) / per + 1 : w0;
   };
@@ -997,14 +1008,19 @@ namespace jero {
 
 // Where the parts of the absorbed form's workspace are.
 struct AbsorbedSpace {
-  size_t part_o, part_ml, plan, bytes;
+  size_t factor, part_o, part_ml, plan, bytes;
+  int rt, pt;  // padded widths: the smallest that the attend kernel is built for
 };
 
 static AbsorbedSpace absorbed_space(const jero_latent_cache* c, int64_t n_tokens, int n_heads) {
   auto up = [](size_t n) { return (n + 255) & ~size_t(255); };
-  const size_t rows = size_t(n_tokens) * n_heads, parts = (size_t(n_tokens) + kMlaRuns) * n_heads;
+  const size_t parts = (size_t(n_tokens) + kMlaRuns) * n_heads;
+  const size_t rows16 = size_t(n_tokens) * ((n_heads + 15) / 16 * 16);
   AbsorbedSpace s;
-  s.part_o = up(rows * (size_t(c->rank) + c->rope_dim) * 4);
+  s.rt = c->rank <= 128 && c->rope_dim <= 32 ? 128 : c->rank <= 256 ? 256 : 512;
+  s.pt = s.rt == 128 ? 32 : 64;
+  s.factor = up(rows16 * (s.rt + s.pt) * 4);
+  s.part_o = s.factor + up(rows16 * 4);
   s.part_ml = s.part_o + up(parts * c->rank * 4);
   s.plan = s.part_ml + up(parts * 8);
   s.bytes = s.plan + up((3 * size_t(n_tokens) + 1) * 4);
@@ -1012,31 +1028,31 @@ static AbsorbedSpace absorbed_space(const jero_latent_cache* c, int64_t n_tokens
 }
 
 template <int RT, int PT, int HG, int KS, typename KV, bool TWO>
-static void launch_attend(const LatentCache& c, const float* qa, int nh, float scale, const MlaPlan& plan, int runs,
-                          int least, float* part_o, float2* part_ml, hipStream_t s) {
+static void launch_attend(const LatentCache& c, const MlaQueries& qa, int nh, const MlaPlan& plan, int runs, int least,
+                          int extra, float* part_o, float2* part_ml, hipStream_t s) {
   const int groups = (nh + 16 * HG - 1) / (16 * HG);
   hipLaunchKernelGGL((mla_attend_kernel<RT, PT, HG, KS, KV, TWO>), dim3(unsigned(runs) * groups), dim3(64 * HG * KS), 0, s,
-                     c, qa, nh, scale, plan, runs, least, part_o, part_ml);
+                     c, qa, nh, plan, runs, least, extra, part_o, part_ml);
 }
 
 // Heads a workgroup: 16 by each of its 1, 2 or 4 waves' worth; with fewer than 4 others share the positions.
 static int attend_heads(int nh) { return nh <= 16 ? 16 : nh <= 32 ? 32 : 64; }
 
 template <int RT, int PT, typename KV, bool TWO>
-static void launch_attend_heads(const LatentCache& c, const float* qa, int nh, float scale, const MlaPlan& plan, int runs,
-                                int least, float* part_o, float2* part_ml, hipStream_t s) {
+static void launch_attend_heads(const LatentCache& c, const MlaQueries& qa, int nh, const MlaPlan& plan, int runs,
+                                int least, int extra, float* part_o, float2* part_ml, hipStream_t s) {
   const int hg = attend_heads(nh);
-  if (hg == 16) launch_attend<RT, PT, 1, 2, KV, TWO>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
-  else if (hg == 32) launch_attend<RT, PT, 2, 2, KV, TWO>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
-  else launch_attend<RT, PT, 4, 1, KV, TWO>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
+  if (hg == 16) launch_attend<RT, PT, 1, 2, KV, TWO>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
+  else if (hg == 32) launch_attend<RT, PT, 2, 2, KV, TWO>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
+  else launch_attend<RT, PT, 4, 1, KV, TWO>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
 }
 
 template <int RT, int PT>
-static void launch_attend_types(bool f32_act, bool f32_kv, const LatentCache& c, const float* qa, int nh, float scale,
-                                const MlaPlan& plan, int runs, int least, float* part_o, float2* part_ml, hipStream_t s) {
-  if (f32_kv) launch_attend_heads<RT, PT, float, true>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
-  else if (f32_act) launch_attend_heads<RT, PT, _Float16, true>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
-  else launch_attend_heads<RT, PT, _Float16, false>(c, qa, nh, scale, plan, runs, least, part_o, part_ml, s);
+static void launch_attend_types(bool f32_act, bool f32_kv, const LatentCache& c, const MlaQueries& qa, int nh,
+                                const MlaPlan& plan, int runs, int least, int extra, float* part_o, float2* part_ml, hipStream_t s) {
+  if (f32_kv) launch_attend_heads<RT, PT, float, true>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
+  else if (f32_act) launch_attend_heads<RT, PT, _Float16, true>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
+  else launch_attend_heads<RT, PT, _Float16, false>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
 }
 
 }  // namespace jero
@@ -1063,7 +1079,13 @@ extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, i
   const LatentCache c = mla_cache_of(cache, n_tokens);
   hipStream_t s = static_cast<hipStream_t>(stream);
   uint8_t* const w = static_cast<uint8_t*>(ws);
-  float *qa = reinterpret_cast<float*>(w), *part_o = reinterpret_cast<float*>(w + sp.part_o);
+  MlaQueries qa;
+  qa.parts = reinterpret_cast<_Float16*>(w);
+  qa.factor = reinterpret_cast<float*>(w + sp.factor);
+  qa.plane = n_tokens * ((n_heads + 15) / 16 * 16) * (sp.rt + sp.pt);
+  qa.rt = sp.rt;
+  qa.kt = (sp.rt + sp.pt) / 32;
+  float* part_o = reinterpret_cast<float*>(w + sp.part_o);
   float2* part_ml = reinterpret_cast<float2*>(w + sp.part_ml);
   MlaPlan plan;
   plan.prefix = reinterpret_cast<int*>(w + sp.plan);
@@ -1073,12 +1095,12 @@ extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, i
   const bool f32 = act_dtype == JERO_F32;
   const int tile = kAttendTile;
   const int groups = (n_heads + attend_heads(n_heads) - 1) / attend_heads(n_heads);
-  const int runs = groups >= kMlaRuns / 8 ? 8 : kMlaRuns / groups / 8 * 8, least = 1;
+  const int runs = groups >= kMlaRuns / 8 ? 8 : kMlaRuns / groups / 8 * 8, least = 1, extra = 3;
 
-  const dim3 ga{unsigned((c.rank + 63) / 64 + 2), unsigned(n_heads), unsigned((n_tokens + 63) / 64)};
-#define JERO_ABSORB(X, NT)                                                                                           \
-  hipLaunchKernelGGL((mla_absorb_kernel<X, NT>), ga, dim3(256), 0, s, c, static_cast<const X*>(q_dev), q_stride, nope_dim, \
-                     kb, rope, qa, plan, tile)
+  const dim3 ga{unsigned(n_heads + 1), unsigned((n_tokens + 15) / 16), 1};
+#define JERO_ABSORB(X, NT)                                                                                         \
+  hipLaunchKernelGGL((mla_absorb_kernel<X, NT>), ga, dim3(512), 0, s, c, static_cast<const X*>(q_dev), q_stride, n_heads, \
+                     nope_dim, kb, rope, scale, qa, plan, tile, extra)
   if (nope_dim <= 128) {
     if (f32) JERO_ABSORB(float, 4);
     else JERO_ABSORB(_Float16, 4);
@@ -1090,17 +1112,17 @@ extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, i
   if ((rc = check_launch("mla absorb"))) return rc;
 
   const bool wide = cache->kv_dtype == JERO_KV_F32;
-  if (c.rank <= 128 && c.rope <= 32)
-    launch_attend_types<128, 32>(f32, wide, c, qa, n_heads, scale, plan, runs, least, part_o, part_ml, s);
-  else if (c.rank <= 256)
-    launch_attend_types<256, 64>(f32, wide, c, qa, n_heads, scale, plan, runs, least, part_o, part_ml, s);
+  if (sp.rt == 128)
+    launch_attend_types<128, 32>(f32, wide, c, qa, n_heads, plan, runs, least, extra, part_o, part_ml, s);
+  else if (sp.rt == 256)
+    launch_attend_types<256, 64>(f32, wide, c, qa, n_heads, plan, runs, least, extra, part_o, part_ml, s);
   else
-    launch_attend_types<512, 64>(f32, wide, c, qa, n_heads, scale, plan, runs, least, part_o, part_ml, s);
+    launch_attend_types<512, 64>(f32, wide, c, qa, n_heads, plan, runs, least, extra, part_o, part_ml, s);
   if ((rc = check_launch("mla attend"))) return rc;
 
   const dim3 gv{unsigned(n_heads), unsigned((n_tokens + 15) / 16), 1};
 #define JERO_VALUES(X, RT)                                                                                              \
-  hipLaunchKernelGGL((mla_values_kernel<X, RT>), gv, dim3(512), 0, s, c, part_o, part_ml, plan, runs, least, vb, v_dim, \
+  hipLaunchKernelGGL((mla_values_kernel<X, RT>), gv, dim3(512), 0, s, c, part_o, part_ml, plan, runs, least, extra, vb, v_dim, \
                      static_cast<X*>(out_dev), out_stride)
   if (c.rank <= 128) {
     if (f32) JERO_VALUES(float, 128);
