@@ -98,46 +98,65 @@ struct MlaQueries {
   int rt, kt;     // padded latent columns, 32s of all columns
 };
 
-// Grid (heads, then one for the plan; tokens by 16).  The 8 waves take the head's rows of W_uk^T by 16; a
+// Blocks that read the same head's weights for different tokens, on one XCD (blocks go round the 8) and one
+// after the other, so that all but the first find them in its L2: block b of `per` blocks a head.
+__device__ __forceinline__ bool mla_head_block(int b, int nh, int per, int& h, int& part) {
+  h = (b / (8 * per)) * 8 + (b & 7);
+  part = (b >> 3) % per;
+  return h < nh;
+}
+static unsigned mla_head_blocks(int nh, int per) { return unsigned((nh + 7) / 8 * 8) * unsigned(per); }
+
+// A block per head and 16 tokens, and one more for the plan.  The 8 waves take the head's rows of W_uk^T by 16; a
 // thread rotates a pair of the key part; the row's largest value is the scale of its parts.
 template <typename X, int NT>
 __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X* __restrict__ q, int64_t q_stride, int nh,
                                                          int nope, const _Float16* __restrict__ k_b, MlaRope rope,
                                                          float scale, MlaQueries qa, MlaPlan plan, int tile, int extra) {
-  const int h = blockIdx.x, t0 = blockIdx.y * 16;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  if (h < nh) {
+  if (blockIdx.x + 1 < gridDim.x) {
+    int h, t0;
+    if (!mla_head_block(blockIdx.x, nh, (c.n_tokens + 15) / 16, h, t0)) return;
+    t0 *= 16;
     constexpr int NR = kMlaMaxRank / 128;  // 16s of rows a wave
     __shared__ float s_max[8][16];
     __shared__ uint32_t s_key[16];
     const int g = lane >> 4, col = lane & 15;
+    // everything the wave reads is on its way before anything is waited for
     const X* qr = q + min(t0 + col, c.n_tokens - 1) * q_stride + int64_t(h) * (nope + c.rope);
-    if (tid < 16) s_key[tid] = 0;
+    h8_t b[NR][NT];
+#pragma unroll
+    for (int k = 0; k < NR; k++)
+#pragma unroll
+      for (int i = 0; i < NT; i++)
+        b[k][i] = *reinterpret_cast<const h8_t*>(
+            k_b + (int64_t(h) * c.rank + min(16 * (wv + 8 * k) + col, c.rank - 1)) * nope + min(32 * i + 8 * g, nope - 8));
+    float qv[NT][8];
+#pragma unroll
+    for (int i = 0; i < NT; i++) load8<X>(qr + min(32 * i + 8 * g, nope - 8), qv[i]);
     // the key part, its pair of the thread's token
     const int pairs = c.rope / 2, kt_ = tid / pairs, ki = tid % pairs;
-    float ka = 0.f, kb = 0.f;
     const bool key = kt_ < 16 && t0 + kt_ < c.n_tokens;
-    if (key) {
-      const X* kp = q + (t0 + kt_) * q_stride + int64_t(h) * (nope + c.rope) + nope + 2 * ki;
-      const float x = float(kp[0]), y = float(kp[1]);
-      float2 cs = make_float2(1.f, 0.f);
-      if (rope.on) {
-        int seq, pos;
-        if (!mla_locate_thread(c, t0 + kt_, seq, pos)) pos = 0;
-        cs = mla_cos_sin(rope, ki, pos);
-      }
-      ka = x * cs.x - y * cs.y;
-      kb = x * cs.y + y * cs.x;
+    const int key_t = min(t0 + min(kt_, 15), c.n_tokens - 1);
+    const X* kp = q + key_t * q_stride + int64_t(h) * (nope + c.rope) + nope + 2 * ki;
+    const float kx = float(kp[0]), ky = float(kp[1]);
+    if (tid < 16) s_key[tid] = 0;
+    float ka = kx, kb = ky;
+    if (rope.on) {
+      int seq, pos;
+      if (!mla_locate_thread(c, key_t, seq, pos)) pos = 0;
+      const float2 cs = mla_cos_sin(rope, ki, pos);
+      ka = kx * cs.x - ky * cs.y;
+      kb = kx * cs.y + ky * cs.x;
     }
+    if (!key) ka = kb = 0.f;
     h8_t ah[NT], al[NT];
 #pragma unroll
     for (int i = 0; i < NT; i++) {
-      float v[8];
-      load8<X>(qr + min(32 * i + 8 * g, nope - 8), v);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         _Float16 x, y;
-        split2(32 * i + 8 * g < nope ? v[e] : 0.f, x, y);
+        split2(32 * i + 8 * g < nope ? qv[i][e] : 0.f, x, y);
         ah[i][e] = x, al[i][e] = y;
       }
     }
@@ -147,14 +166,10 @@ __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X*
     for (int k = 0; k < NR; k++) {
       const int r0 = 16 * (wv + 8 * k);
       f4_t hi = {0.f, 0.f, 0.f, 0.f}, lo = hi;
-      if (r0 < c.rank) {
-        const _Float16* w = k_b + (int64_t(h) * c.rank + min(r0 + col, c.rank - 1)) * nope;
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
-          const h8_t b = *reinterpret_cast<const h8_t*>(w + min(32 * i + 8 * g, nope - 8));
-          hi = mfma(ah[i], b, hi);
-          if (sizeof(X) == 4) lo = mfma(al[i], b, lo);
-        }
+      for (int i = 0; i < NT; i++) {
+        hi = mfma(ah[i], b[k][i], hi);
+        if (sizeof(X) == 4) lo = mfma(al[i], b[k][i], lo);
       }
 #pragma unroll
       for (int e = 0; e < 4; e++) {
@@ -178,37 +193,45 @@ __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X*
       for (int w = 0; w < 8; w++) x = fmaxf(x, s_max[w][t]);
       return x > 0.f && x < INFINITY ? ilogbf(x) : 0;
     };
-    const int groups = (nh + 15) / 16;
-    _Float16* const out = qa.parts + ((int64_t(t0) * groups + h / 16) * qa.kt) * 512 + (h % 16) * 8;
+    // the parts by token and column in LDS, from there 16 bytes at a time
+    constexpr int W = kMlaMaxRank + kMlaMaxRope + 8;
+    constexpr bool TWO = sizeof(X) == 4;
+    __shared__ __attribute__((aligned(16))) _Float16 s_part[TWO ? 2 : 1][16][W];
     auto put = [&](int t, int k, float x) {
       _Float16 hi, lo;
       split2(x, hi, lo);
-      _Float16* p = out + (int64_t(t) * groups * qa.kt + k / 32) * 512 + ((k % 32) / 8) * 128 + k % 8;
-      p[0] = hi;
-      if (sizeof(X) == 4) p[qa.plane] = lo;
+      s_part[0][t][k] = hi;
+      if (TWO) s_part[TWO][t][k] = lo;
     };
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const int t = 4 * g + e, ex = power(t);
-      if (t0 + t >= c.n_tokens) continue;
 #pragma unroll
       for (int k = 0; k < NR; k++) {
         const int r = 16 * (wv + 8 * k) + col;
         if (r < qa.rt) put(t, r, ldexpf(v[k][e], -ex));
       }
     }
-    if (key) {
+    const int groups = (nh + 15) / 16;
+    if (kt_ < 16) {
       const int ex = power(kt_);
       put(kt_, qa.rt + 2 * ki, ldexpf(ka, -ex));
       put(kt_, qa.rt + 2 * ki + 1, ldexpf(kb, -ex));
-      if (ki == 0)
+      if (key && ki == 0)
         qa.factor[int64_t(t0 + kt_) * groups * 16 + h] = ldexpf(scale * 1.44269504088896341f, ex);
     }
-    const int pad = 32 * qa.kt - qa.rt - c.rope;  // columns of no pair
-    if (tid < 16 * pad && t0 + tid / pad < c.n_tokens) put(tid / pad, qa.rt + c.rope + tid % pad, 0.f);
+    const int cols = 32 * qa.kt, pad = cols - qa.rt - c.rope;  // columns of no pair
+    for (int i = tid; i < 16 * pad; i += 512) put(i / pad, qa.rt + c.rope + i % pad, 0.f);
+    __syncthreads();
+    for (int i = tid; i < 16 * (cols / 8); i += 512) {
+      const int t = i / (cols / 8), k = i % (cols / 8);  // 8 columns
+      if (t0 + t >= c.n_tokens) break;
+      _Float16* p = qa.parts + ((int64_t(t0 + t) * groups + h / 16) * qa.kt + k / 4) * 512 + (k % 4) * 128 + (h % 16) * 8;
+      *reinterpret_cast<h8_t*>(p) = *reinterpret_cast<const h8_t*>(&s_part[0][t][8 * k]);
+      if (TWO) *reinterpret_cast<h8_t*>(p + qa.plane) = *reinterpret_cast<const h8_t*>(&s_part[TWO][t][8 * k]);
+    }
     return;
   }
-  if (t0) return;
   // the plan: 512 tokens at a time, a scan of their units (the tiles, and for a token that has any as many as
   // beginning it takes)
   __shared__ int s_scan[8];
@@ -514,43 +537,61 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
           if constexpr (TWO) b[j] = mfma(ka[k % M][j], ql[k], b[j]);
           if constexpr (WIDE) b[j] = mfma(kb[k % M][j], qh[k], b[j]);
         }
+        // a product holds the matrix core for 16 cycles and the wave for 4: the softmax goes between
+#pragma unroll
+        for (int n = 0; n < NT * (1 + TWO + WIDE); n++) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product
+          __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // vector instructions
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     };
-    // the softmax of a step's scores, in three parts
-    float sc[4 * NT], mn = 0.f, alpha = 1.f;
+    // the softmax of a step's scores, in 16 pieces to go between products: each result is pinned where it is
+    // made (the compiler would move it to its use)
+    constexpr int PIECES = 16, NS = 4 * NT;
+    float sc[NS], mx = 0.f, ref = 0.f, alpha = 1.f, sum = 0.f;
     bool grew = false;
-    _Float16 ph[4 * NT], pl[4 * NT];
-    auto soft_max = [&](uint32_t here) {
-      const uint32_t own = here >> (kp * WR) >> (4 * g);  // bit 16 j + e: position 4g + e of tile j
-      float mx = -INFINITY;
+    _Float16 ph[NS], pl[NS];
+    auto soft = [&](int piece, uint32_t here) {
+      if (piece < 4) {
+        const uint32_t own = here >> (kp * WR) >> (4 * g);  // bit 16 j + e: position 4g + e of tile j
 #pragma unroll
-      for (int j = 0; j < NT; j++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
+        for (int n = piece * NS / 4; n < (piece + 1) * NS / 4; n++) {
+          const int j = n / 4, e = n % 4;
           const float s = (sa[j][e] + sb[j][e]) * factor;
-          sc[4 * j + e] = own & (1u << (16 * j + e)) ? s : -INFINITY;
-          mx = fmaxf(mx, sc[4 * j + e]);
+          sc[n] = own & (1u << (16 * j + e)) ? s : -INFINITY;
+          asm volatile("" : "+v"(sc[n]));
         }
-      mx = max_over_groups(mx);
-      grew = __any(mx > m + 8.f);
-      mn = grew ? fmaxf(m, mx) : m;
-      const float ref = mn == -INFINITY ? 0.f : mn;
-      alpha = __builtin_amdgcn_exp2f(m - ref);  // 0 at first: exp2(-inf)
-      m = mn;
-      mn = ref;
-    };
-    auto soft_exp = [&](int e) {
-      const float p = __builtin_amdgcn_exp2f(sc[e] - mn);
-      split2(p, ph[e], pl[e]);
-      sc[e] = p;
-      asm volatile("" : "+v"(sc[e]));  // here, between the products, and not where they are used
-    };
-    auto soft_sum = [&]() {
-      float s = 0.f;
+      } else if (piece == 4) {
+        mx = sc[0];
 #pragma unroll
-      for (int e = 0; e < 4 * NT; e++) s += sc[e];
-      l = l * alpha + s;
+        for (int n = 1; n < NS; n++) mx = fmaxf(mx, sc[n]);
+        asm volatile("" : "+v"(mx));
+      } else if (piece == 5) {
+        mx = max_over_groups(mx);
+        asm volatile("" : "+v"(mx));
+      } else if (piece == 6) {
+        grew = __any(mx > m + 8.f);
+        const float mn = grew ? fmaxf(m, mx) : m;
+        ref = mn == -INFINITY ? 0.f : mn;
+        alpha = __builtin_amdgcn_exp2f(m - ref);  // 0 at first: exp2(-inf)
+        m = mn;
+        l *= alpha;
+        asm volatile("" : "+v"(ref), "+v"(alpha), "+v"(m), "+v"(l));
+      } else if (piece < 15) {
+#pragma unroll
+        for (int n = (piece - 7) * NS / 8; n < (piece - 6) * NS / 8; n++) {
+          const float p = __builtin_amdgcn_exp2f(sc[n] - ref);
+          split2(p, ph[n], pl[n]);
+          sc[n] = p;
+          asm volatile("" : "+v"(sc[n]));
+        }
+      } else {
+        sum = sc[0];
+#pragma unroll
+        for (int n = 1; n < NS; n++) sum += sc[n];
+        l += sum;
+      }
     };
     // O^T += C^T p from buffer kv
     auto values = [&](const uint8_t* kv) {
@@ -625,10 +666,8 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
 #pragma unroll
             for (int n = grp * S::kLoadsLat / QN; n < (grp + 1) * S::kLoadsLat / QN; n++) load(S::kLoadsKey + n, 0);
         });
-        soft_max(here);
 #pragma unroll
-        for (int e = 0; e < 4 * NT; e++) soft_exp(e);
-        soft_sum();
+        for (int n = 0; n < PIECES; n++) soft(n, here);
         values(s_raw);
       }
     } else {
@@ -658,12 +697,8 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
           if (more)
 #pragma unroll
             for (int n = grp * S::kLoadsLat / QN; n < (grp + 1) * S::kLoadsLat / QN; n++) load(S::kLoadsKey + n, fb);
-          if (grp == QN / 4) soft_max(mask[0]);
-          constexpr int E0 = QN / 2, EN = QN - E0 - 1;  // groups that take the exponentials
-          if (grp >= E0 && grp < QN - 1)
 #pragma unroll
-            for (int e = (grp - E0) * 4 * NT / EN; e < (grp - E0 + 1) * 4 * NT / EN; e++) soft_exp(e);
-          if (grp == QN - 1) soft_sum();
+          for (int n = grp * PIECES / QN; n < (grp + 1) * PIECES / QN; n++) soft(n, mask[0]);
         });
         values(s_raw + (i & 3) * S::kBuf);
 #pragma unroll
@@ -717,19 +752,21 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
   }
 }
 
-// out[t][h] = W_uv[h] o[t][h], o the merged partials: one workgroup of 8 waves per head and 16 tokens.  The
-// weights' rows (16 of them a wave, its MFMA operand) are on their way while the partials are merged into LDS.
-// With few tokens the waves share a token's partials, else each wave takes tokens of its own.
-template <typename X, int RT>
-__global__ void __launch_bounds__(512) mla_values_kernel(LatentCache c, const float* __restrict__ part_o,
+// out[t][h] = W_uv[h] o[t][h], o the merged partials: a block of 8 waves per head and up to TB tokens.  The
+// weights' rows (16 of them a wave, its MFMA operand) are on their way while the partials are merged, by 8 / TB
+// waves a token (TB 16: a wave, two tokens), into LDS.
+template <typename X, int RT, int TB>
+__global__ void __launch_bounds__(512) mla_values_kernel(LatentCache c, int nh, const float* __restrict__ part_o,
                                                          const float2* __restrict__ part_ml, MlaPlan plan, int runs,
                                                          int least, int extra, const _Float16* __restrict__ v_b,
                                                          int v_dim, X* __restrict__ out, int64_t out_stride) {
-  constexpr int KT = RT / 32, P = RT + 8, NW = 8, U = 8;
+  constexpr int KT = RT / 32, P = RT + 8, NW = 8, U = 4, WPT = TB < 8 ? 8 / TB : 1;
   __shared__ __attribute__((aligned(16))) _Float16 s_hi[16][P], s_lo[16][P];
-  __shared__ float s_acc[NW][RT];
+  __shared__ __attribute__((aligned(16))) float s_acc[WPT > 1 ? NW : 1][RT];
   __shared__ float s_m[NW], s_l[NW];
-  const int h = blockIdx.x, nh = gridDim.x, t0 = blockIdx.y * 16;
+  int h, t0;
+  if (!mla_head_block(blockIdx.x, nh, (c.n_tokens + TB - 1) / TB, h, t0)) return;
+  t0 *= TB;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int g = lane >> 4, col = lane & 15;
   const int vt = (v_dim + 15) / 16;
@@ -740,7 +777,6 @@ __global__ void __launch_bounds__(512) mla_values_kernel(LatentCache c, const fl
     for (int i = 0; i < KT; i++) b[i] = *reinterpret_cast<const h8_t*>(w + min(32 * i + 8 * g, c.rank - 8));
   };
   weights(min(wv, vt - 1));
-  const int nt = min(16, c.n_tokens - t0);
   const int per = mla_per_run(plan.prefix[c.n_tokens], runs, least);
   const int r0 = min(8 * lane, c.rank - 8);
 
@@ -781,8 +817,8 @@ __global__ void __launch_bounds__(512) mla_values_kernel(LatentCache c, const fl
       m = mn;
     }
   };
-  auto keep = [&](int row, float sum) {
-    const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+  auto keep = [&](int row, float total) {
+    const float inv = total != 0.f ? 1.0f / total : 0.f;
     if (8 * lane < RT) {
       h8_t hi, lo;
 #pragma unroll
@@ -795,75 +831,58 @@ __global__ void __launch_bounds__(512) mla_values_kernel(LatentCache c, const fl
       *reinterpret_cast<h8_t*>(&s_lo[row][8 * lane]) = lo;
     }
   };
-  auto range = [&](int t, int& w0, int& w1) {
-    const int a = plan.prefix[t] + extra, e = plan.prefix[t + 1];
-    w0 = a / per;
-    w1 = e > a ? (e - 1) / per + 1 : w0;
-  };
-  int w0, w1;
-  if (nt > 2) {
-    for (int i = wv; i < 16; i += NW) {
-      m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = wv / WPT; i < TB; i += NW / WPT) {
+    const int t = t0 + i;
+    int w0 = 0, w1 = 0;
+    if (t < c.n_tokens) {
+      const int a = plan.prefix[t] + extra, e = plan.prefix[t + 1];
+      w0 = a / per;
+      w1 = e > a ? (e - 1) / per + 1 : w0;
+    }
+    merge(t, w0 + wv % WPT, w1, WPT);
+    if constexpr (WPT == 1) keep(i, l);
+  }
+  if constexpr (WPT > 1) {
+    if (8 * lane < RT) {
+      reinterpret_cast<float4*>(&s_acc[wv][8 * lane])[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      reinterpret_cast<float4*>(&s_acc[wv][8 * lane])[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    }
+    if (lane == 0) s_m[wv] = m, s_l[wv] = l;
+    __syncthreads();
+    if (wv < TB) {
+      float mt = -INFINITY, total = 0.f;
+#pragma unroll
+      for (int w = 0; w < WPT; w++) mt = fmaxf(mt, s_m[wv * WPT + w]);
+      const float ref = mt == -INFINITY ? 0.f : mt;
 #pragma unroll
       for (int e = 0; e < 8; e++) acc[e] = 0.f;
-      if (i < nt) {
-        range(t0 + i, w0, w1);
-        merge(t0 + i, w0, w1, 1);
+#pragma unroll
+      for (int w = 0; w < WPT; w++) {
+        const float f = __builtin_amdgcn_exp2f(s_m[wv * WPT + w] - ref);
+        total += f * s_l[wv * WPT + w];
+#pragma unroll
+        for (int e = 0; e < 8; e++) acc[e] += f * s_acc[wv * WPT + w][min(8 * lane, RT - 8) + e];
       }
-      keep(i, l);
+      keep(wv, total);
     }
-  } else {
-    for (int i = 0; i < nt; i++) {
-      range(t0 + i, w0, w1);
-      merge(t0 + i, w0 + wv, w1, NW);
-      if (8 * lane < RT) {
-        reinterpret_cast<float4*>(&s_acc[wv][8 * lane])[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        reinterpret_cast<float4*>(&s_acc[wv][8 * lane])[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-      }
-      if (lane == 0) s_m[wv] = m, s_l[wv] = l;
-      __syncthreads();
-      if (wv == 0) {
-        float mt = -INFINITY, sum = 0.f;
-        for (int w = 0; w < NW; w++) mt = fmaxf(mt, s_m[w]);
-        const float ref = mt == -INFINITY ? 0.f : mt;
-#pragma unroll
-        for (int e = 0; e < 8; e++) acc[e] = 0.f;
-        for (int w = 0; w < NW; w++) {
-          const float f = __builtin_amdgcn_exp2f(s_m[w] - ref);
-          sum += f * s_l[w];
-#pragma unroll
-          for (int e = 0; e < 8; e++) acc[e] += f * s_acc[w][min(8 * lane, RT - 8) + e];
-        }
-        keep(i, sum);
-      }
-      __syncthreads();
-    }
-    if (wv >= nt)  // the rows of no token
-      for (int i = wv; i < 16; i += NW) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) acc[e] = 0.f;
-        keep(i, 1.f);
-      }
-    if (wv < nt)
-      for (int i = wv + NW; i < 16; i += NW) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) acc[e] = 0.f;
-        keep(i, 1.f);
-      }
   }
   __syncthreads();
+  // (rows from TB on of the product's 16 are those of other tokens, and not stored)
+  const int row = col & (TB - 1);
   for (int tile = wv; tile < vt; tile += NW) {
     if (tile != wv) weights(tile);
     f4_t hi = {0.f, 0.f, 0.f, 0.f}, lo = hi;
 #pragma unroll
     for (int i = 0; i < KT; i++) {
-      hi = mfma(*reinterpret_cast<const h8_t*>(&s_hi[col][32 * i + 8 * g]), b[i], hi);
-      lo = mfma(*reinterpret_cast<const h8_t*>(&s_lo[col][32 * i + 8 * g]), b[i], lo);
+      hi = mfma(*reinterpret_cast<const h8_t*>(&s_hi[row][32 * i + 8 * g]), b[i], hi);
+      lo = mfma(*reinterpret_cast<const h8_t*>(&s_lo[row][32 * i + 8 * g]), b[i], lo);
     }
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const int t = t0 + 4 * g + e, v = 16 * tile + col;
-      if (t < c.n_tokens && v < v_dim && plan.seq[t] >= 0) out[t * out_stride + int64_t(h) * v_dim + v] = X(hi[e] + lo[e]);
+      const int i = 4 * g + e, t = t0 + i, v = 16 * tile + col;
+      if (i < TB && t < c.n_tokens && v < v_dim && plan.seq[t] >= 0)
+        out[t * out_stride + int64_t(h) * v_dim + v] = X(hi[e] + lo[e]);
     }
   }
 }
@@ -1097,7 +1116,7 @@ extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, i
   const int groups = (n_heads + attend_heads(n_heads) - 1) / attend_heads(n_heads);
   const int runs = groups >= kMlaRuns / 8 ? 8 : kMlaRuns / groups / 8 * 8, least = 1, extra = 3;
 
-  const dim3 ga{unsigned(n_heads + 1), unsigned((n_tokens + 15) / 16), 1};
+  const dim3 ga(mla_head_blocks(n_heads, int((n_tokens + 15) / 16)) + 1);
 #define JERO_ABSORB(X, NT)                                                                                         \
   hipLaunchKernelGGL((mla_absorb_kernel<X, NT>), ga, dim3(512), 0, s, c, static_cast<const X*>(q_dev), q_stride, n_heads, \
                      nope_dim, kb, rope, scale, qa, plan, tile, extra)
@@ -1120,20 +1139,34 @@ extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, i
     launch_attend_types<512, 64>(f32, wide, c, qa, n_heads, plan, runs, least, extra, part_o, part_ml, s);
   if ((rc = check_launch("mla attend"))) return rc;
 
-  const dim3 gv{unsigned(n_heads), unsigned((n_tokens + 15) / 16), 1};
-#define JERO_VALUES(X, RT)                                                                                              \
-  hipLaunchKernelGGL((mla_values_kernel<X, RT>), gv, dim3(512), 0, s, c, part_o, part_ml, plan, runs, least, extra, vb, v_dim, \
+  // tokens a block: as many as leave a block for every CU, so that the weights are read seldom
+  const int64_t rows = n_tokens * n_heads;
+#define JERO_VALUES_TB(X, RT, TB)                                                                                    \
+  hipLaunchKernelGGL((mla_values_kernel<X, RT, TB>), dim3(mla_head_blocks(n_heads, int((n_tokens + TB - 1) / TB))), \
+                     dim3(512), 0, s, c, n_heads, part_o, part_ml, plan, runs, least, extra, vb, v_dim,             \
                      static_cast<X*>(out_dev), out_stride)
-  if (c.rank <= 128) {
-    if (f32) JERO_VALUES(float, 128);
-    else JERO_VALUES(_Float16, 128);
-  } else if (c.rank <= 256) {
-    if (f32) JERO_VALUES(float, 256);
-    else JERO_VALUES(_Float16, 256);
+#define JERO_VALUES(X, RT)                                                                                       \
+  if (n_tokens < 2 || rows < 512) JERO_VALUES_TB(X, RT, 1);                                                      \
+  else if (rows < 2048) JERO_VALUES_TB(X, RT, 4);                                                                \
+  else JERO_VALUES_TB(X, RT, 16)
+  if (sp.rt == 128) {
+    if (f32) {
+      JERO_VALUES(float, 128);
+    } else {
+      JERO_VALUES(_Float16, 128);
+    }
+  } else if (sp.rt == 256) {
+    if (f32) {
+      JERO_VALUES(float, 256);
+    } else {
+      JERO_VALUES(_Float16, 256);
+    }
+  } else if (f32) {
+    JERO_VALUES(float, 512);
   } else {
-    if (f32) JERO_VALUES(float, 512);
-    else JERO_VALUES(_Float16, 512);
+    JERO_VALUES(_Float16, 512);
   }
+#undef JERO_VALUES_TB
 #undef JERO_VALUES
   return check_launch("mla values");
 }
