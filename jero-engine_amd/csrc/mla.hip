@@ -106,6 +106,14 @@ __device__ __forceinline__ bool mla_head_block(int b, int nh, int per, int& h, i
   return h < nh;
 }
 static unsigned mla_head_blocks(int nh, int per) { return unsigned((nh + 7) / 8 * 8) * unsigned(per); }
+// The same with 8 heads on one XCD, where what they write shares lines.
+__device__ __forceinline__ bool mla_head8_block(int b, int nh, int per, int& h, int& part) {
+  const int slot = b >> 3, in = slot % (8 * per);
+  h = ((slot / (8 * per)) * 8 + (b & 7)) * 8 + in / per;
+  part = in % per;
+  return h < nh;
+}
+static unsigned mla_head8_blocks(int nh, int per) { return unsigned((nh + 63) / 64 * 64) * unsigned(per); }
 
 // A block per head and 16 tokens, and one more for the plan.  The 8 waves take the head's rows of W_uk^T by 16; a
 // thread rotates a pair of the key part; the row's largest value is the scale of its parts.
@@ -116,11 +124,12 @@ __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X*
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   if (blockIdx.x + 1 < gridDim.x) {
     int h, t0;
-    if (!mla_head_block(blockIdx.x, nh, (c.n_tokens + 15) / 16, h, t0)) return;
+    if (!mla_head8_block(blockIdx.x, nh, (c.n_tokens + 15) / 16, h, t0)) return;
     t0 *= 16;
     constexpr int NR = kMlaMaxRank / 128;  // 16s of rows a wave
     __shared__ float s_max[8][16];
     __shared__ uint32_t s_key[16];
+    __shared__ int s_ex[16];
     const int g = lane >> 4, col = lane & 15;
     // everything the wave reads is on its way before anything is waited for
     const X* qr = q + min(t0 + col, c.n_tokens - 1) * q_stride + int64_t(h) * (nope + c.rope);
@@ -188,11 +197,17 @@ __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X*
     __syncthreads();
     if (key) atomicMax(&s_key[kt_], __float_as_uint(fmaxf(fabsf(ka), fabsf(kb))));
     __syncthreads();
-    auto power = [&](int t) {  // of the token's largest value; 0 for a row of zeros, or one that is not finite
-      float x = __uint_as_float(s_key[t]);
-      for (int w = 0; w < 8; w++) x = fmaxf(x, s_max[w][t]);
-      return x > 0.f && x < INFINITY ? ilogbf(x) : 0;
-    };
+    const int groups = (nh + 15) / 16;
+    if (tid < 16) {  // the power of a token's largest value; 0 for a row of zeros, or one that is not finite
+      float x = __uint_as_float(s_key[tid]);
+#pragma unroll
+      for (int w = 0; w < 8; w++) x = fmaxf(x, s_max[w][tid]);
+      const int ex = x > 0.f && x < INFINITY ? ilogbf(x) : 0;
+      s_ex[tid] = ex;
+      if (t0 + tid < c.n_tokens)
+        qa.factor[int64_t(t0 + tid) * groups * 16 + h] = ldexpf(scale * 1.44269504088896341f, ex);
+    }
+    __syncthreads();
     // the parts by token and column in LDS, from there 16 bytes at a time
     constexpr int W = kMlaMaxRank + kMlaMaxRope + 8;
     constexpr bool TWO = sizeof(X) == 4;
@@ -205,20 +220,17 @@ __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X*
     };
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const int t = 4 * g + e, ex = power(t);
+      const int t = 4 * g + e, ex = s_ex[t];
 #pragma unroll
       for (int k = 0; k < NR; k++) {
         const int r = 16 * (wv + 8 * k) + col;
         if (r < qa.rt) put(t, r, ldexpf(v[k][e], -ex));
       }
     }
-    const int groups = (nh + 15) / 16;
     if (kt_ < 16) {
-      const int ex = power(kt_);
+      const int ex = s_ex[kt_];
       put(kt_, qa.rt + 2 * ki, ldexpf(ka, -ex));
       put(kt_, qa.rt + 2 * ki + 1, ldexpf(kb, -ex));
-      if (key && ki == 0)
-        qa.factor[int64_t(t0 + kt_) * groups * 16 + h] = ldexpf(scale * 1.44269504088896341f, ex);
     }
     const int cols = 32 * qa.kt, pad = cols - qa.rt - c.rope;  // columns of no pair
     for (int i = tid; i < 16 * pad; i += 512) put(i / pad, qa.rt + c.rope + i % pad, 0.f);
@@ -537,13 +549,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
           if constexpr (TWO) b[j] = mfma(ka[k % M][j], ql[k], b[j]);
           if constexpr (WIDE) b[j] = mfma(kb[k % M][j], qh[k], b[j]);
         }
-        // a product holds the matrix core for 16 cycles and the wave for 4: the softmax goes between
-#pragma unroll
-        for (int n = 0; n < NT * (1 + TWO + WIDE); n++) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product
-          __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // vector instructions
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        if (k % 3 == 2) __builtin_amdgcn_sched_barrier(0);  // reads stay ahead, and no further
       }
     };
     // the softmax of a step's scores, in 16 pieces to go between products: each result is pinned where it is
@@ -662,7 +668,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
         }
         __syncthreads();
         scores(s_raw, sa, sb, [&](int grp) {
-          if (more)  // the next step's loads, a few a group: issued at once they hold the wave up
+          if (more)  // the next step's loads, a few a group
 #pragma unroll
             for (int n = grp * S::kLoadsLat / QN; n < (grp + 1) * S::kLoadsLat / QN; n++) load(S::kLoadsKey + n, 0);
         });
@@ -690,13 +696,10 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
         if (more) {
           mask[3] = find(i + 3);
 #pragma unroll
-          for (int n = 0; n < S::kLoadsKey; n++) load(n, fb);
+          for (int n = 0; n < S::kLoads; n++) load(n, fb);
         }
         f4_t na[NT], nb2[NT];
         scores(s_raw + nb * S::kBuf, na, nb2, [&](int grp) {
-          if (more)
-#pragma unroll
-            for (int n = grp * S::kLoadsLat / QN; n < (grp + 1) * S::kLoadsLat / QN; n++) load(S::kLoadsKey + n, fb);
 #pragma unroll
           for (int n = grp * PIECES / QN; n < (grp + 1) * PIECES / QN; n++) soft(n, mask[0]);
         });
@@ -1116,7 +1119,7 @@ extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, i
   const int groups = (n_heads + attend_heads(n_heads) - 1) / attend_heads(n_heads);
   const int runs = groups >= kMlaRuns / 8 ? 8 : kMlaRuns / groups / 8 * 8, least = 1, extra = 3;
 
-  const dim3 ga(mla_head_blocks(n_heads, int((n_tokens + 15) / 16)) + 1);
+  const dim3 ga(mla_head8_blocks(n_heads, int((n_tokens + 15) / 16)) + 1);
 #define JERO_ABSORB(X, NT)                                                                                         \
   hipLaunchKernelGGL((mla_absorb_kernel<X, NT>), ga, dim3(512), 0, s, c, static_cast<const X*>(q_dev), q_stride, n_heads, \
                      nope_dim, kb, rope, scale, qa, plan, tile, extra)
