@@ -205,56 +205,79 @@ struct FlashShape {
   static constexpr int kKey = KR * NT * 2, kRope = KR * PT * 2, kVal = KR * VT * 2;
   static constexpr int kPlane = kKey + kRope + kVal;
   static constexpr int kBuf = kPlane * kPlanes;
-  static constexpr int kGroups = 4 * kBuf <= 160 * 1024 ? 2 : 1;  // workgroups a CU
+  // workgroups a CU: as LDS allows, and the registers of 32 tokens' accumulators
+  static constexpr int kGroups = 4 * kBuf <= 160 * 1024 && VT <= 128 ? 2 : 1;
   static_assert(2 * kBuf <= 160 * 1024 && kKey % 4096 == 0 && kRope % 1024 == 0 && kVal % 4096 == 0, "tile shape");
 };
+
+// What a block of the attention works on: tile of the nh heads' tiles.
+struct FlashTile {
+  int h, seq, first, count, len, steps;  // head, sequence, token rows, the sequence's positions, steps of kr
+  int64_t base, shift;                   // its first expanded row; the position of token row t is shift + t
+};
+__device__ __forceinline__ bool flash_tile(const LatentCache& c, int64_t total, int nh, int tiles, int kr, int lane,
+                                           FlashTile& f) {
+  // a head's blocks on one XCD (blocks go round the 8), so that its keys and values stay in one L2
+  int k;
+  if (nh % 8 == 0) {
+    const int slot = blockIdx.x >> 3, per = nh / 8;
+    f.h = (slot % per) * 8 + (blockIdx.x & 7);
+    k = slot / per;
+  } else {
+    f.h = blockIdx.x % nh;
+    k = blockIdx.x / nh;
+  }
+  // The late tiles, which attend to the most, first; where all blocks run at once, two a CU, the second half
+  // of them in rising order, so that a CU gets a late tile and an early one.
+  const int half = (tiles + 1) / 2;
+  const int tile = tiles * nh <= 2 * 256 + nh && k >= half ? k - half : tiles - 1 - k;
+  // tiles of 128 tokens, sequence after sequence
+  int before = 0, end = 0;
+  f.seq = -1;
+  mla_sequences(c, total, lane, [&](int s, int64_t b, int n) {
+    int s0 = s, s1 = s + 1;
+    if (c.starts) s0 = c.starts[s], s1 = c.starts[s + 1];
+    const int from = max(s0, 0), mine = max(min(s1, c.n_tokens) - from, 0), nt = (mine + kFlashRows - 1) / kFlashRows;
+    if (tile < before + nt) {
+      f.seq = s, f.first = from + (tile - before) * kFlashRows;
+      f.count = min(kFlashRows, mine - (tile - before) * kFlashRows);
+      f.base = b, f.len = n, end = s1;
+      return false;
+    }
+    before += nt;
+    return true;
+  });
+  if (f.seq < 0) return false;
+  f.shift = int64_t(c.lens[f.seq]) - end;
+  const int top = int(max(int64_t(0), min(f.shift + f.first + f.count, int64_t(f.len))));
+  f.steps = (top + kr - 1) / kr;
+  return true;
+}
 
 // Causal attention of 128 tokens of a sequence and a head, one pass with a running maximum and sum.  S^T =
 // K q^T (positions x tokens) leaves a token per lane column and, taken in the order 4g .. 4g + 3, 16 + 4g .. of
 // 32 positions, is the B operand of O^T += V^T p, V^T read from LDS transposed: numerators, factors and
 // accumulators of a token stay in its lanes.  Accumulators are rescaled only where a maximum grew by 2^8.
+// Grid y: runs of `cut` steps; a tile of more than one leaves a partial row a token and run (part_o, part_ml),
+// which mla_flash_merge_kernel joins.
 template <int NT, int PT, int VT, typename X, bool TWO>
 __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
     mla_flash_kernel(LatentCache c, const X* __restrict__ q, int64_t q_stride, int nope, int v_dim, int nh, int h0,
-                     Expanded x, float scale, MlaRope rope, X* __restrict__ out, int64_t out_stride, int tiles) {
+                     Expanded x, float scale, MlaRope rope, X* __restrict__ out, int64_t out_stride, int tiles, int cut,
+                     float* __restrict__ part_o, float2* __restrict__ part_ml) {
   using S = FlashShape<NT, PT, VT, TWO>;
   constexpr int KR = S::KR, RT = KR / 16, KT = (NT + PT) / 32, DT = VT / 16;
   __shared__ __attribute__((aligned(16))) uint8_t s_kv[2 * S::kBuf];
   const uint32_t lds0 = uint32_t(uintptr_t((lds_u8*)s_kv));
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, col = lane & 15;
-  // a head's workgroups on one XCD (blocks go round the 8), so that its keys and values stay in one L2; the late
-  // tiles, which attend to the most, first
-  int h, tile;
-  if (nh % 8 == 0) {
-    const int slot = blockIdx.x >> 3, per = nh / 8;
-    h = (slot % per) * 8 + (blockIdx.x & 7);
-    tile = slot / per;
-  } else {
-    h = blockIdx.x % nh;
-    tile = blockIdx.x / nh;
-  }
-  tile = tiles - 1 - tile;
-  // the tile's sequence: tiles of 128 tokens, sequence after sequence
-  int seq = -1, first = 0, count = 0, len = 0, all = 0;
-  int64_t base = 0;
-  {
-    int before = 0;
-    mla_sequences(c, x.total, lane, [&](int s, int64_t b, int n) {
-      int s0 = s, s1 = s + 1;
-      if (c.starts) s0 = c.starts[s], s1 = c.starts[s + 1];
-      const int mine = max(min(s1, c.n_tokens) - max(s0, 0), 0), nt = (mine + kFlashRows - 1) / kFlashRows;
-      if (tile < before + nt) {
-        seq = s, first = max(s0, 0) + (tile - before) * kFlashRows, count = min(kFlashRows, mine - (tile - before) * kFlashRows);
-        base = b, len = n, all = s1;
-        return false;
-      }
-      before += nt;
-      return true;
-    });
-  }
-  if (seq < 0) return;
-  const int64_t shift = int64_t(c.lens[seq]) - all;  // position of token row t: shift + t
+  FlashTile ft;
+  if (!flash_tile(c, x.total, nh, tiles, KR, lane, ft)) return;
+  const int h = ft.h, seq = ft.seq, first = ft.first, count = ft.count, len = ft.len;
+  const int64_t base = ft.base, shift = ft.shift;
+  const int units = (ft.steps + cut - 1) / cut;
+  const int begin = int(blockIdx.y) * cut, steps = min(ft.steps, begin + cut);
+  if (blockIdx.y > 0 && int(blockIdx.y) >= units) return;
 
   // the queries: B operands, each token's brought near 1 by a power of two that goes into the scores' factor
   h8_t qh[2][KT], ql[2][TWO ? KT : 1];
@@ -291,47 +314,51 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
     mx = max_over_groups(mx);
     int ex = 0;
     if (mx > 0.f && mx < INFINITY) ex = ilogbf(mx);
-    factor[j] = ldexpf(scale * 1.44269504088896341f, ex);
+    factor[j] = ldexpf(fabsf(scale) * 1.44269504088896341f, ex);  // its sign goes into the queries
 #pragma unroll
     for (int k = 0; k < KT; k++)
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         _Float16 a, b;
-        split2(ldexpf(v[k][e], -ex), a, b);
+        split2(ldexpf(scale < 0.f ? -v[k][e] : v[k][e], -ex), a, b);
         qh[j][k][e] = a;
         if (TWO) ql[j][k][e] = b;
       }
   }
-  // the workgroup's positions: up to its last token's; those below its first token's need no mask
-  const int top = int(max(int64_t(0), min(shift + first + count, int64_t(len))));
+  // positions below the wave's first token's need no mask
   const int low = int(max(int64_t(0), min(shift + first + wv * 32 + 1, int64_t(len))));
-  const int steps = (top + KR - 1) / KR;
   const int32_t* table = c.table + seq * c.table_stride;
 
   const uint8_t* const kb = reinterpret_cast<const uint8_t*>(x.k + (int64_t(h) * x.total + base) * NT);
   const uint8_t* const vb = reinterpret_cast<const uint8_t*>(x.v + (int64_t(h) * x.total + base) * VT);
   const uint8_t* const pb = reinterpret_cast<const uint8_t*>(x.p + base * PT);
-  // rows of 2 w bytes, swap(r) their chunks' swap: LDS bytes from `at` on of buffer buf, load i of 1024 bytes
-  auto part = [&](int i, int p0, const uint8_t* src, int64_t plane, int w, bool four, uint32_t to) {
+  // Load i of 1024 bytes of a part with rows of 2 w bytes, into LDS from `to` on: the lane's row, and its byte in
+  // the row (chunks swapped).  Steps that end behind the last position repeat it (and mask it).
+  auto part = [&](int i, int p0, bool whole, const uint8_t* src, int w, bool four, uint32_t to) {
     const int b = i * 1024 + 16 * lane, r = b / (2 * w);
-    const int sw = 16 * (four ? swap4(r) : swap8(r));
-    // (a position behind the last repeats it, and is masked)
-    dma_row(src + plane, uint32_t(min(p0 + r, len - 1)) * uint32_t(2 * w) + uint32_t((b % (2 * w)) ^ sw), to + i * 1024);
+    const uint32_t in = uint32_t((b % (2 * w)) ^ (16 * (four ? swap4(r) : swap8(r))));
+    if (whole) dma_row(src + int64_t(p0) * (2 * w), uint32_t(r * 2 * w) + in, to + i * 1024);
+    else dma_row(src, uint32_t(min(p0 + r, len - 1)) * uint32_t(2 * w) + in, to + i * 1024);
   };
   auto load = [&](int step, int buf) {
     const int p0 = step * KR;
+    auto all = [&](bool whole) {
 #pragma unroll
-    for (int pl = 0; pl < S::kPlanes; pl++) {
-      const uint32_t to = lds0 + buf * S::kBuf + pl * S::kPlane;
-      constexpr int NK = S::kKey / 1024, NR = S::kRope / 1024, NV = S::kVal / 1024;
+      for (int pl = 0; pl < S::kPlanes; pl++) {
+        const uint32_t to = lds0 + buf * S::kBuf + pl * S::kPlane;
+        constexpr int NK = S::kKey / 1024, NR = S::kRope / 1024, NV = S::kVal / 1024;
 #pragma unroll
-      for (int i = 0; i < NK; i += 4) part(i + wv, p0, kb, pl * x.k_plane * 2, NT, false, to);
+        for (int i = 0; i < NK; i += 4) part(i + wv, p0, whole, kb + pl * x.k_plane * 2, NT, false, to);
 #pragma unroll
-      for (int i = 0; i < NR; i += 4)
-        if (NR % 4 == 0 || i + wv < NR) part(i + wv, p0, pb, pl * x.p_plane * 2, PT, PT == 32, to + S::kKey);
+        for (int i = 0; i < NR; i += 4)
+          if (NR % 4 == 0 || i + wv < NR) part(i + wv, p0, whole, pb + pl * x.p_plane * 2, PT, PT == 32, to + S::kKey);
 #pragma unroll
-      for (int i = 0; i < NV; i += 4) part(i + wv, p0, vb, pl * x.v_plane * 2, VT, false, to + S::kKey + S::kRope);
-    }
+        for (int i = 0; i < NV; i += 4)
+          part(i + wv, p0, whole, vb + pl * x.v_plane * 2, VT, false, to + S::kKey + S::kRope);
+      }
+    };
+    if (p0 + KR <= len) all(true);
+    else all(false);
   };
   // the block of a step's position lane
   auto block = [&](int step) {
@@ -344,7 +371,8 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
   for (int j = 0; j < 2; j++)
 #pragma unroll
     for (int d = 0; d < DT; d++) o[j][d] = f4_t{0.f, 0.f, 0.f, 0.f};
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float m[2] = {-INFINITY, -INFINITY};
+  f4_t l[2] = {f4_t{0.f, 0.f, 0.f, 0.f}, f4_t{0.f, 0.f, 0.f, 0.f}};  // (4 times the same)
   const int kat = 16 * (g ^ swap8(col)), kat4 = 16 * ((4 + g) ^ swap8(col));
   const int rat = 16 * (PT == 64 ? g ^ swap8(col) : g ^ swap4(col)), rat4 = 16 * ((4 + g) ^ swap8(col));
   const int vr = 4 * g + (col >> 2);
@@ -352,9 +380,9 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
 #pragma unroll
   for (int d = 0; d < 4; d++) vat[d] = vr * VT * 2 + 16 * ((2 * d + ((col & 3) >> 1)) ^ swap8(vr)) + 8 * (col & 1);
 
-  if (steps > 0) load(0, 0);
-  uint32_t ids = steps > 0 ? block(0) : 0;
-  for (int i = 0; i < steps; i++) {
+  if (steps > begin) load(begin, begin & 1);
+  uint32_t ids = steps > begin ? block(begin) : 0;
+  for (int i = begin; i < steps; i++) {
     dma_wait<0>();
     const uint64_t ok = __ballot(ids < c.n_blocks);  // (its load has come with the others: waited for before)
     __syncthreads();
@@ -364,10 +392,6 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
     }
     const uint8_t* kv = s_kv + (i & 1) * S::kBuf;
     f4_t s[2][RT];
-#pragma unroll
-    for (int j = 0; j < 2; j++)
-#pragma unroll
-      for (int r = 0; r < RT; r++) s[j][r] = f4_t{0.f, 0.f, 0.f, 0.f};
     // operands are read a group of products ahead
     constexpr int KP = S::kPlanes;
     h8_t ka[2][RT][KP];
@@ -388,7 +412,8 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
 #pragma unroll
       for (int r = 0; r < RT; r++)
 #pragma unroll
-        for (int j = 0; j < 2; j++) s[j][r] = mfma(ka[k & 1][r][0], qh[j][k], s[j][r]);
+        for (int j = 0; j < 2; j++)
+          s[j][r] = mfma(ka[k & 1][r][0], qh[j][k], k ? s[j][r] : f4_t{0.f, 0.f, 0.f, 0.f});
       if constexpr (TWO) {
 #pragma unroll
         for (int r = 0; r < RT; r++)
@@ -405,50 +430,65 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
     h8_t bh[2][RT / 2], bl[2][RT / 2];
     bool grew[2];
     float alpha[2];
+    const bool masked = p0 + KR > low || ok != ~0ull;
+    float times[2] = {factor[0], factor[1]};
+    if (masked) {
+      const uint64_t mine = ok >> (4 * g);
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int r = 0; r < RT; r++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) s[j][r][e] *= factor[j];
-      if (p0 + KR > low || ok != ~0ull) {
-        const uint64_t mine = ok >> (4 * g);
+      for (int j = 0; j < 2; j++) {
+        times[j] = 1.f;
 #pragma unroll
         for (int r = 0; r < RT; r++)
 #pragma unroll
           for (int e = 0; e < 4; e++)
-            if (p0 + 16 * r + 4 * g + e >= limit[j] || !(mine & (1ull << (16 * r + e)))) s[j][r][e] = -INFINITY;
+            s[j][r][e] = p0 + 16 * r + 4 * g + e < limit[j] && (mine & (1ull << (16 * r + e))) ? s[j][r][e] * factor[j]
+                                                                                                : -INFINITY;
       }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      float mx = s[j][0][0];
 #pragma unroll
       for (int r = 0; r < RT; r++)
 #pragma unroll
         for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[j][r][e]);
-      mx = max_over_groups(mx);
+      mx = max_over_groups(mx) * times[j];
       grew[j] = __any(mx > m[j] + 8.f);
       const float mn = grew[j] ? fmaxf(m[j], mx) : m[j];
       const float ref = mn == -INFINITY ? 0.f : mn;
       alpha[j] = __builtin_amdgcn_exp2f(m[j] - ref);
       m[j] = mn;
-      float sum = 0.f;
 #pragma unroll
       for (int r = 0; r < RT; r++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float p = __builtin_amdgcn_exp2f(s[j][r][e] - ref);
-          sum += p;
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[j][r][e], times[j], -ref));
           _Float16 a, b;
           split2(p, a, b);
           bh[j][r / 2][4 * (r & 1) + e] = a;
           bl[j][r / 2][4 * (r & 1) + e] = b;
         }
-      l[j] = l[j] * alpha[j] + sum;
     }
 #pragma unroll
     for (int j = 0; j < 2; j++)
-      if (grew[j])
+      if (grew[j]) {
+        l[j] *= alpha[j];
 #pragma unroll
         for (int d = 0; d < DT; d++) o[j][d] *= alpha[j];
+      }
+    // the sums of the numerators, as the product rounds them: a row of ones in place of the values
+    {
+      h8_t one;
+#pragma unroll
+      for (int e = 0; e < 8; e++) one[e] = _Float16(1.f);
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int r = 0; r < RT / 2; r++) {
+          l[j] = mfma(one, bh[j][r], l[j]);
+          if constexpr (TWO) l[j] = mfma(one, bl[j][r], l[j]);
+        }
+    }
     const uint8_t* vp = kv + S::kKey + S::kRope;
     auto tr = [&](int d, int r, int plane) {
       return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -483,10 +523,17 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
   }
 #pragma unroll
   for (int j = 0; j < 2; j++) {
-    const float sum = sum_over_groups(l[j]);
-    const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+    const float sum = l[j][0];
     const int i = wv * 32 + 16 * j + col;
     if (i >= count) continue;
+    if (units > 1) {
+      const int64_t row = (int64_t(blockIdx.x) * gridDim.y + blockIdx.y) * kFlashRows + i;
+#pragma unroll
+      for (int d = 0; d < DT; d++) *reinterpret_cast<f4_t*>(part_o + row * VT + 16 * d + 4 * g) = o[j][d];
+      if (g == 0) part_ml[row] = make_float2(m[j], sum);
+      continue;
+    }
+    const float inv = sum != 0.f ? 1.0f / sum : 0.f;
     X* dst = out + (first + i) * out_stride + int64_t(h0 + h) * v_dim;
 #pragma unroll
     for (int d = 0; d < DT; d++) {
@@ -501,6 +548,39 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
         *reinterpret_cast<h4_t*>(dst + v) = y;
       }
     }
+  }
+}
+
+// Joins the partial rows of a tile's runs: VT / 4 lanes a token.
+template <int VT, typename X>
+__global__ void __launch_bounds__(256) mla_flash_merge_kernel(LatentCache c, int64_t total, int v_dim, int nh, int h0, int kr,
+                                                              X* __restrict__ out, int64_t out_stride, int tiles, int cut,
+                                                              int runs, const float* __restrict__ part_o,
+                                                              const float2* __restrict__ part_ml) {
+  FlashTile f;
+  if (!flash_tile(c, total, nh, tiles, kr, threadIdx.x & 63, f)) return;
+  const int units = (f.steps + cut - 1) / cut;
+  if (units <= 1) return;
+  constexpr int L = VT / 4;
+  const int v = 4 * (threadIdx.x % L);
+  for (int i = blockIdx.y * (256 / L) + threadIdx.x / L; i < f.count; i += gridDim.y * (256 / L)) {
+    const int64_t row = int64_t(blockIdx.x) * runs * kFlashRows + i;
+    float m = -INFINITY, sum = 0.f;
+    for (int u = 0; u < units; u++) m = fmaxf(m, part_ml[row + int64_t(u) * kFlashRows].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+    f4_t acc = {0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < units; u++) {
+      const int64_t at = row + int64_t(u) * kFlashRows;
+      const float2 ml = part_ml[at];
+      const float e = __builtin_amdgcn_exp2f(ml.x - ref);
+      sum += e * ml.y;
+      acc += e * *reinterpret_cast<const f4_t*>(part_o + at * VT + v);
+    }
+    if (v >= v_dim) continue;
+    const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+    X* dst = out + (f.first + i) * out_stride + int64_t(h0 + f.h) * v_dim + v;
+#pragma unroll
+    for (int e = 0; e < 4; e++) dst[e] = X(acc[e] * inv);
   }
 }
 
@@ -527,18 +607,45 @@ static int prefill_tiles(const LatentCache& c) {
   return c.starts ? c.n_tokens / kFlashRows + (c.n_seqs < c.n_tokens ? c.n_seqs : c.n_tokens) : c.n_seqs;
 }
 
+// Runs a tile's positions are cut into.  With fewer blocks than two a CU, cut so that about kFlashUnits
+// runs come out, none below kFlashLeast positions; the partial rows of at most kFlashParts blocks x runs.
+constexpr int kFlashUnits = 768, kFlashLeast = 512, kFlashParts = 1280;
+struct FlashCut {
+  int positions, runs;  // a run's positions, the most runs a tile has
+};
+static FlashCut flash_cut(int64_t blocks, int max_len) {
+  FlashCut f{INT32_MAX / 2, 1};
+  if (blocks >= 2 * 256) return f;
+  int64_t p = (int64_t(max_len) * blocks + kFlashUnits - 1) / kFlashUnits;
+  p = (p < kFlashLeast ? kFlashLeast : p + 63) / 64 * 64;
+  const int64_t runs = (max_len + p - 1) / p;
+  if (runs < 2 || runs * blocks > kFlashParts) return f;
+  return {int(p), int(runs)};
+}
+static size_t flash_part_bytes(int vt) { return size_t(kFlashParts) * kFlashRows * (size_t(vt) * 4 + 8); }
+
 template <int NT, int PT, int VT, typename X, typename KV, bool TWO>
 static int launch_prefill(const LatentCache& c, const X* q, int64_t q_stride, int nh, int h0, int nope, int v_dim,
                           const _Float16* w, const Expanded& x, float scale, const MlaRope& rope, X* out,
-                          int64_t out_stride, hipStream_t s) {
+                          int64_t out_stride, void* parts, hipStream_t s) {
   const dim3 ge{unsigned((nh * (NT + VT) + 127) / 128 + 1), unsigned((x.total + 127) / 128), 1};
   hipLaunchKernelGGL((mla_expand_kernel<NT, PT, VT, KV, TWO>), ge, dim3(256), 0, s, c, nh, nope, v_dim, w, x);
   int rc = check_launch("mla expand");
   if (rc) return rc;
+  constexpr int KR = FlashShape<NT, PT, VT, TWO>::KR;
   const int tiles = prefill_tiles(c);
-  hipLaunchKernelGGL((mla_flash_kernel<NT, PT, VT, X, TWO>), dim3(unsigned(tiles) * nh), dim3(256), 0, s, c, q, q_stride,
-                     nope, v_dim, nh, h0, x, scale, rope, out, out_stride, tiles);
-  return check_launch("mla flash");
+  const unsigned blocks = unsigned(tiles) * nh;
+  const int longest = int(x.total < c.max_len ? x.total : c.max_len);
+  const FlashCut f = parts ? flash_cut(blocks, longest) : FlashCut{INT32_MAX / 2, 1};
+  float* part_o = static_cast<float*>(parts);
+  float2* part_ml = reinterpret_cast<float2*>(part_o + size_t(kFlashParts) * kFlashRows * VT);
+  hipLaunchKernelGGL((mla_flash_kernel<NT, PT, VT, X, TWO>), dim3(blocks, unsigned(f.runs)), dim3(256), 0, s, c, q,
+                     q_stride, nope, v_dim, nh, h0, x, scale, rope, out, out_stride, tiles, f.positions / KR, part_o,
+                     part_ml);
+  if ((rc = check_launch("mla flash")) || f.runs == 1) return rc;
+  hipLaunchKernelGGL((mla_flash_merge_kernel<VT, X>), dim3(blocks, 8), dim3(256), 0, s, c, x.total, v_dim, nh, h0, KR, out,
+                     out_stride, tiles, f.positions / KR, f.runs, part_o, part_ml);
+  return check_launch("mla flash merge");
 }
 
 }  // namespace jero
@@ -553,7 +660,10 @@ extern "C" size_t jero_hip_mla_prefill_workspace_bytes(const jero_latent_cache* 
   const size_t one = prefill_bytes(s, total_len, 1, planes), head = size_t(total_len) * (s.nt + s.vt) * 2 * planes;
   size_t heads = 1;
   if (one < (size_t(1) << 30)) heads += ((size_t(1) << 30) - one) / (head + 512);
-  return prefill_bytes(s, total_len, heads < size_t(n_heads) ? heads : size_t(n_heads), planes);
+  // (a call whose positions may be cut into runs, with room for their partial rows)
+  const int64_t longest = total_len < cache->max_len ? total_len : cache->max_len;
+  return prefill_bytes(s, total_len, heads < size_t(n_heads) ? heads : size_t(n_heads), planes) +
+         (n_heads > 1 && longest > kFlashLeast ? flash_part_bytes(s.vt) : 0);
 }
 
 extern "C" int jero_hip_mla_prefill_attention(const jero_latent_cache* cache, int act_dtype, const void* q_dev,
@@ -586,6 +696,9 @@ extern "C" int jero_hip_mla_prefill_attention(const jero_latent_cache* cache, in
     return fail(JERO_ERR_INVALID_ARGUMENT, "mla_prefill_attention: workspace must be 256-byte aligned");
   int per = n_heads;
   while (per > 1 && prefill_bytes(shape, total_len, size_t(per), planes) > workspace_bytes) per--;
+  const size_t rows_bytes = prefill_bytes(shape, total_len, size_t(per), planes);
+  void* const parts = workspace_bytes - rows_bytes >= flash_part_bytes(shape.vt) ? static_cast<uint8_t*>(ws) + rows_bytes
+                                                                                 : nullptr;
   const LatentCache c = mla_cache_of(cache, n_tokens);
   if (int64_t(prefill_tiles(c)) * n_heads > (int64_t(1) << 23))
     return fail(JERO_ERR_CAPABILITY_MISMATCH, "mla_prefill_attention: more than 2^23 tiles of 128 tokens over the heads");
@@ -607,7 +720,7 @@ extern "C" int jero_hip_mla_prefill_attention(const jero_latent_cache* cache, in
     x.v = reinterpret_cast<_Float16*>(at);
 #define JERO_PREFILL(NT, PT, VT, X, KV, TWO)                                                                      \
   rc = launch_prefill<NT, PT, VT, X, KV, TWO>(c, static_cast<const X*>(q_dev), q_stride, nh, h0, nope_dim, v_dim, w, x, \
-                                              scale, rope, static_cast<X*>(out_dev), out_stride, s)
+                                              scale, rope, static_cast<X*>(out_dev), out_stride, parts, s)
 #define JERO_PREFILL_TYPES(NT, PT, VT)                                                       \
   if (act_dtype == JERO_F16) JERO_PREFILL(NT, PT, VT, _Float16, _Float16, false);            \
   else if (cache->kv_dtype == JERO_KV_F16) JERO_PREFILL(NT, PT, VT, float, _Float16, true);  \
