@@ -35,25 +35,36 @@ struct Expanded {
   int64_t total;
 };
 
-// The product W C^T of 128 weight rows (of the heads' padded rows, keys before values) and 128 positions, the
-// rank in steps of 64: four waves of 64 x 64, operands through LDS, the next step's loads in registers during
-// this step's products.  A lane ends up with 4 consecutive columns of a position's row.  An f32 cache's latents
-// go in as two f16 parts; TWO: the results come out as two.  One more block in x copies the key parts.
+// The product W C^T for 128 positions (64 of an f32 cache, whose latents go in as two f16 parts) and a run of the
+// heads' padded weight rows (keys before values).  The latents stay in LDS for the whole run; a wave takes 64 weight
+// rows at a time, their operands straight from memory (no other wave of the block wants them), so that each 1024
+// bytes read from LDS serve four products.  A lane's rows of the four are chosen so that it ends up with 16
+// consecutive columns of a position's row.  TWO: the results come out as two parts.  The last blocks copy the
+// key parts.
+template <typename KV>
+struct ExpandShape {
+  static constexpr bool kWide = sizeof(KV) == 4;
+  static constexpr int kPos = kWide ? 64 : 128, kPlanes = kWide ? 2 : 1;
+  static constexpr int kPitch = kMlaMaxRank + 8;  // 16 rows fall on all banks
+  static constexpr int kStep = 512;               // weight rows of the 8 waves
+};
 template <int NT, int PT, int VT, typename KV, bool TWO>
-__global__ void __launch_bounds__(256, (sizeof(KV) == 4 ? 1 : 2)) mla_expand_kernel(LatentCache c, int nh, int nope, int v_dim,
-                                                            const _Float16* __restrict__ w, Expanded x) {
-  constexpr bool WIDE = sizeof(KV) == 4;
-  constexpr int WP = NT + VT, CP = WIDE ? 2 : 1;
-  constexpr int TILE = 128 * 128;  // bytes of 128 rows of 64
-  __shared__ __attribute__((aligned(16))) uint8_t s_t[2][1 + CP][TILE];
-  __shared__ int64_t s_row[128];  // the positions' cache rows: -1 for a block that is none, -2 for no position
+__global__ void __launch_bounds__(512) mla_expand_kernel(LatentCache c, int nh, int nope, int v_dim,
+                                                         const _Float16* __restrict__ w, Expanded x, int run) {
+  using S = ExpandShape<KV>;
+  constexpr bool WIDE = S::kWide;
+  constexpr int WP = NT + VT, MP = S::kPos, CP = S::kPlanes, P = S::kPitch, MJ = MP / 16;
+  __shared__ __attribute__((aligned(16))) _Float16 s_c[CP][MP][P];
+  __shared__ int64_t s_row[MP];  // the positions' cache rows: -1 for a block that is none, -2 for no position
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  const int64_t m0 = int64_t(blockIdx.y) * 128;
-  if (tid < 128) {
+  // blocks of one run of weight rows follow each other, over all XCDs; the key parts' come last
+  const int across = int((x.total + MP - 1) / MP), part = blockIdx.x / across;
+  const int64_t m0 = int64_t(blockIdx.x % across) * MP;
+  if (tid < MP) {
     int seq = -1, pos = 0;
     mla_sequences(c, x.total, lane, [&](int s, int64_t base, int len) {
       if (m0 + tid >= base && m0 + tid < base + len) seq = s, pos = int(m0 + tid - base);
-      return base + len <= m0 + 127;
+      return base + len < m0 + MP;
     });
     s_row[tid] = seq < 0 ? -2 : mla_row(c, seq, pos);
   }
@@ -61,8 +72,8 @@ __global__ void __launch_bounds__(256, (sizeof(KV) == 4 ? 1 : 2)) mla_expand_ker
   if (s_row[0] == -2) return;  // behind the last sequence's rows
   const KV* rows = static_cast<const KV*>(c.rows);
 
-  if (blockIdx.x == gridDim.x - 1) {
-    for (int i = tid; i < 128 * (PT / 8); i += 256) {
+  if ((part + 1) * across == int(gridDim.x)) {
+    for (int i = tid; i < MP * (PT / 8); i += 512) {
       const int r = i / (PT / 8), k = 8 * (i % (PT / 8));
       const int64_t at = s_row[r];
       if (at == -2) continue;
@@ -84,111 +95,122 @@ __global__ void __launch_bounds__(256, (sizeof(KV) == 4 ? 1 : 2)) mla_expand_ker
     return;
   }
 
-  const int w0 = blockIdx.x * 128;
-  // thread's chunks of 8 values: rows tid / 8 + 32 i, columns 8 (tid % 8) of a step
-  const int sr = tid >> 3, sk = 8 * (tid & 7);
+  const int g = lane >> 4, col = lane & 15;
+  const int steps = (c.rank + 31) / 32;  // 32s of the rank
+  // weight row of the lane's operand of product i: the result's row 4g + e is column 16g + 4i + e
+  const int all = nh * WP, w_end = min(all, (part + 1) * run);
   const _Float16* wp[4];
-  int64_t cr[4];
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int idx = w0 + sr + 32 * i, h = idx / WP, j = idx % WP;
-    const bool on = h < nh && (j < NT ? j < nope : j - NT < v_dim);
-    wp[i] = on ? w + (int64_t(h) * (nope + v_dim) + (j < NT ? j : nope + j - NT)) * c.rank : nullptr;
-    cr[i] = s_row[sr + 32 * i];
-  }
-  const u32x4 zero = {0u, 0u, 0u, 0u};
-  u32x4 rw[4], rc[4][CP];
-  auto fetch = [&](int k0) {
-    const int k = k0 + sk;
+  auto rows_of = [&](int w0) {  // 64 of them belong to one head and one of its two parts
+    const int h = w0 / WP, j = w0 % WP;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      rw[i] = wp[i] && k < c.rank ? *reinterpret_cast<const u32x4*>(wp[i] + k) : zero;
-#pragma unroll
-      for (int e = 0; e < CP; e++)
-        rc[i][e] = cr[i] >= 0 && k < c.rank ? *reinterpret_cast<const u32x4*>(rows + cr[i] + k + 4 * e) : zero;
+      const int n = (j < NT ? j : j - NT) + 16 * (col >> 2) + 4 * i + (col & 3);
+      const bool on = w0 < w_end && (j < NT ? n < nope : n < v_dim);
+      wp[i] = on ? w + (int64_t(h) * (nope + v_dim) + (j < NT ? n : nope + n)) * c.rank : nullptr;
     }
   };
-  auto store = [&](int buf) {
+  h8_t a[3][4];
+  auto read_w = [&](int k, h8_t (&d)[4]) {
+    const int at = min(32 * k + 8 * g, c.rank - 8);  // (past the rank the latents are zeros)
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const int r = sr + 32 * i, at = r * 128 + 16 * ((sk >> 3) ^ swap8(r));
-      *reinterpret_cast<u32x4*>(&s_t[buf][0][at]) = rw[i];
-      if constexpr (!WIDE) {
-        *reinterpret_cast<u32x4*>(&s_t[buf][1][at]) = rc[i][0];
+      const h8_t z = {};
+      d[i] = wp[i] ? *reinterpret_cast<const h8_t*>(wp[i] + at) : z;
+    }
+  };
+  int w0 = part * run + 64 * wv;
+  rows_of(w0);
+  read_w(0, a[0]);
+  read_w(min(1, steps - 1), a[1]);
+
+  // the latents: a lane 8 values, 8 rows' loads at a time
+  for (int r0 = wv; r0 < MP; r0 += 64) {
+    float v[8][WIDE ? 8 : 1];
+    h8_t hv[8];
+    const int k = 8 * lane;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int64_t at = s_row[r0 + 8 * i];
+      const bool on = at >= 0 && k < c.rank;
+      if constexpr (WIDE) {
+        if (on) load8<float>(rows + at + k, v[i]);
+        else
+#pragma unroll
+          for (int e = 0; e < 8; e++) v[i][e] = 0.f;
       } else {
-        const uint32_t v[8] = {rc[i][0].x, rc[i][0].y, rc[i][0].z, rc[i][0].w,
-                               rc[i][CP - 1].x, rc[i][CP - 1].y, rc[i][CP - 1].z, rc[i][CP - 1].w};
+        const h8_t z = {};
+        hv[i] = on ? *reinterpret_cast<const h8_t*>(rows + at + k) : z;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if constexpr (WIDE) {
         h8_t hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          _Float16 a, b;
-          split2(__uint_as_float(v[e]), a, b);
-          hi[e] = a, lo[e] = b;
+          _Float16 p, q;
+          split2(v[i][e], p, q);
+          hi[e] = p, lo[e] = q;
         }
-        *reinterpret_cast<h8_t*>(&s_t[buf][1][at]) = hi;
-        *reinterpret_cast<h8_t*>(&s_t[buf][CP][at]) = lo;
+        *reinterpret_cast<h8_t*>(&s_c[0][r0 + 8 * i][k]) = hi;
+        *reinterpret_cast<h8_t*>(&s_c[CP - 1][r0 + 8 * i][k]) = lo;
+      } else {
+        *reinterpret_cast<h8_t*>(&s_c[0][r0 + 8 * i][k]) = hv[i];
       }
-    }
-  };
-  const int g = lane >> 4, col = lane & 15;
-  const int wr = 64 * (wv & 1), mr = 64 * (wv >> 1);
-  f4_t acc[4][4];
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) acc[i][j] = f4_t{0.f, 0.f, 0.f, 0.f};
-  fetch(0);
-  store(0);
-  __syncthreads();
-  const int steps = (c.rank + 63) / 64;
-  for (int s = 0; s < steps; s++) {
-    if (s + 1 < steps) fetch(64 * (s + 1));
-    const uint8_t(*t)[TILE] = s_t[s & 1];
-#pragma unroll
-    for (int kk = 0; kk < 2; kk++) {
-      const int at = 16 * ((4 * kk + g) ^ swap8(col));
-      h8_t a[4], b[4], bl[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        a[i] = *reinterpret_cast<const h8_t*>(&t[0][(wr + 16 * i + col) * 128 + at]);
-        b[i] = *reinterpret_cast<const h8_t*>(&t[1][(mr + 16 * i + col) * 128 + at]);
-        if (WIDE) bl[i] = *reinterpret_cast<const h8_t*>(&t[CP][(mr + 16 * i + col) * 128 + at]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          acc[i][j] = mfma(a[i], b[j], acc[i][j]);
-          if (WIDE) acc[i][j] = mfma(a[i], bl[j], acc[i][j]);
-        }
-    }
-    if (s + 1 < steps) {
-      store((s + 1) & 1);
-      __syncthreads();
     }
   }
+  __syncthreads();
+
+  for (; w0 < w_end; w0 += S::kStep) {
+    f4_t acc[4][MJ];
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const int r = mr + 16 * j + col;
-    if (s_row[r] == -2) continue;
+    for (int i = 0; i < 4; i++)
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int idx = w0 + wr + 16 * i + 4 * g, h = idx / WP, n = idx % WP;
-      if (h >= nh) continue;
-      h4_t hi, lo;
+      for (int j = 0; j < MJ; j++) acc[i][j] = f4_t{0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < steps; k0 += 3) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        _Float16 y, z;
-        split2(acc[i][j][e], y, z);
-        hi[e] = y, lo[e] = z;
+      for (int kk = 0; kk < 3; kk++) {
+        const int k = k0 + kk;
+        if (k >= steps) break;
+        if (k + 2 < steps) read_w(k + 2, a[(kk + 2) % 3]);
+        h8_t b[CP][MJ];
+#pragma unroll
+        for (int p = 0; p < CP; p++)
+#pragma unroll
+          for (int j = 0; j < MJ; j++) b[p][j] = *reinterpret_cast<const h8_t*>(&s_c[p][16 * j + col][32 * k + 8 * g]);
+#pragma unroll
+        for (int p = 0; p < CP; p++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < MJ; j++) acc[i][j] = mfma(a[kk][i], b[p][j], acc[i][j]);
       }
-      const int64_t row = int64_t(h) * x.total + m0 + r;
-      if (n < NT) {
-        *reinterpret_cast<h4_t*>(x.k + row * NT + n) = hi;
-        if (TWO) *reinterpret_cast<h4_t*>(x.k + x.k_plane + row * NT + n) = lo;
-      } else {
-        *reinterpret_cast<h4_t*>(x.v + row * VT + n - NT) = hi;
-        if (TWO) *reinterpret_cast<h4_t*>(x.v + x.v_plane + row * VT + n - NT) = lo;
+    }
+    const int h = w0 / WP, n0 = w0 % WP;
+    rows_of(w0 + S::kStep);  // the next rows' first operands are on their way during the stores
+    if (w0 + S::kStep < w_end) {
+      read_w(0, a[0]);
+      read_w(min(1, steps - 1), a[1]);
+    }
+    const bool key = n0 < NT;
+    _Float16* const dst = key ? x.k : x.v;
+    const int64_t plane = key ? x.k_plane : x.v_plane;
+    const int width = key ? NT : VT, n = (key ? n0 : n0 - NT) + 16 * g;
+#pragma unroll
+    for (int j = 0; j < MJ; j++) {
+      if (s_row[16 * j + col] == -2) continue;
+      _Float16* p = dst + (int64_t(h) * x.total + m0 + 16 * j + col) * width + n;
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        h8_t hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          _Float16 y, z;
+          split2(acc[2 * half + e / 4][j][e % 4], y, z);
+          hi[e] = y, lo[e] = z;
+        }
+        *reinterpret_cast<h8_t*>(p + 8 * half) = hi;
+        if (TWO) *reinterpret_cast<h8_t*>(p + plane + 8 * half) = lo;
       }
     }
   }
@@ -628,8 +650,20 @@ template <int NT, int PT, int VT, typename X, typename KV, bool TWO>
 static int launch_prefill(const LatentCache& c, const X* q, int64_t q_stride, int nh, int h0, int nope, int v_dim,
                           const _Float16* w, const Expanded& x, float scale, const MlaRope& rope, X* out,
                           int64_t out_stride, void* parts, hipStream_t s) {
-  const dim3 ge{unsigned((nh * (NT + VT) + 127) / 128 + 1), unsigned((x.total + 127) / 128), 1};
-  hipLaunchKernelGGL((mla_expand_kernel<NT, PT, VT, KV, TWO>), ge, dim3(256), 0, s, c, nh, nope, v_dim, w, x);
+  // Weight rows a block: 512s, so that the rounds of one block a CU, each its 512s and what loading the latents
+  // takes (about half of one), come out shortest.
+  constexpr int kPos = ExpandShape<KV>::kPos, kStep = ExpandShape<KV>::kStep;
+  const int64_t across = (x.total + kPos - 1) / kPos;
+  const int all = (nh * (NT + VT) + kStep - 1) / kStep;
+  int run = all;
+  double best = 0;
+  for (int n = 1; n <= all; n++) {
+    const int each = (all + n - 1) / n;
+    const double cost = double((across * ((all + each - 1) / each) + 255) / 256) * (each + 0.5);
+    if (n == 1 || cost < best) best = cost, run = each;
+  }
+  const dim3 ge(unsigned((all + run - 1) / run + 1) * unsigned(across));
+  hipLaunchKernelGGL((mla_expand_kernel<NT, PT, VT, KV, TWO>), ge, dim3(512), 0, s, c, nh, nope, v_dim, w, x, run * kStep);
   int rc = check_launch("mla expand");
   if (rc) return rc;
   constexpr int KR = FlashShape<NT, PT, VT, TWO>::KR;
