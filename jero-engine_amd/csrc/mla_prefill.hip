@@ -96,7 +96,6 @@ __global__ void __launch_bounds__(512) mla_expand_kernel(LatentCache c, int nh, 
   }
 
   const int g = lane >> 4, col = lane & 15;
-  const int steps = (c.rank + 31) / 32;  // 32s of the rank
   // weight row of the lane's operand of product i: the result's row 4g + e is column 16g + 4i + e
   const int all = nh * WP, w_end = min(all, (part + 1) * run);
   const _Float16* wp[4];
@@ -109,19 +108,24 @@ __global__ void __launch_bounds__(512) mla_expand_kernel(LatentCache c, int nh, 
       wp[i] = on ? w + (int64_t(h) * (nope + v_dim) + (j < NT ? n : nope + n)) * c.rank : nullptr;
     }
   };
-  h8_t a[3][4];
-  auto read_w = [&](int k, h8_t (&d)[4]) {
-    const int at = min(32 * k + 8 * g, c.rank - 8);  // (past the rank the latents are zeros)
+  // Operands of 64 of the rank, two steps: a lane's 16 bytes of both follow each other in its row, so that both
+  // loads want the same lines, whole, at once (taken in the row's order a wave's halves of lines come back to the
+  // cache after eight waves have been through it)
+  h8_t a[2][4][2];
+  const int pairs = (c.rank + 63) / 64;
+  auto read_w = [&](int p, h8_t (&d)[4][2]) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const h8_t z = {};
-      d[i] = wp[i] ? *reinterpret_cast<const h8_t*>(wp[i] + at) : z;
-    }
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int s = 0; s < 2; s++) {
+        const int at = min(64 * p + 16 * g + 8 * s, c.rank - 8);  // (past the rank the latents are zeros)
+        const h8_t z = {};
+        d[i][s] = wp[i] ? *reinterpret_cast<const h8_t*>(wp[i] + at) : z;
+      }
   };
   int w0 = part * run + 64 * wv;
   rows_of(w0);
   read_w(0, a[0]);
-  read_w(min(1, steps - 1), a[1]);
 
   // the latents: a lane 8 values, 8 rows' loads at a time
   for (int r0 = wv; r0 < MP; r0 += 64) {
@@ -167,31 +171,32 @@ __global__ void __launch_bounds__(512) mla_expand_kernel(LatentCache c, int nh, 
     for (int i = 0; i < 4; i++)
 #pragma unroll
       for (int j = 0; j < MJ; j++) acc[i][j] = f4_t{0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 < steps; k0 += 3) {
+    for (int p0 = 0; p0 < pairs; p0 += 2) {
 #pragma unroll
-      for (int kk = 0; kk < 3; kk++) {
-        const int k = k0 + kk;
-        if (k >= steps) break;
-        if (k + 2 < steps) read_w(k + 2, a[(kk + 2) % 3]);
-        h8_t b[CP][MJ];
+      for (int pp = 0; pp < 2; pp++) {
+        const int p = p0 + pp;
+        if (p >= pairs) break;
+        if (p + 1 < pairs) read_w(p + 1, a[pp ^ 1]);
 #pragma unroll
-        for (int p = 0; p < CP; p++)
+        for (int s = 0; s < 2; s++)
 #pragma unroll
-          for (int j = 0; j < MJ; j++) b[p][j] = *reinterpret_cast<const h8_t*>(&s_c[p][16 * j + col][32 * k + 8 * g]);
+          for (int q = 0; q < CP; q++)
 #pragma unroll
-        for (int p = 0; p < CP; p++)
+            for (int j0 = 0; j0 < MJ; j0 += 4) {  // 4 operands at a time: registers
+              h8_t b[4];
 #pragma unroll
-          for (int i = 0; i < 4; i++)
+              for (int j = 0; j < 4; j++)
+                b[j] = *reinterpret_cast<const h8_t*>(&s_c[q][16 * (j0 + j) + col][64 * p + 16 * g + 8 * s]);
 #pragma unroll
-            for (int j = 0; j < MJ; j++) acc[i][j] = mfma(a[kk][i], b[p][j], acc[i][j]);
+              for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[i][j0 + j] = mfma(a[pp][i][s], b[j], acc[i][j0 + j]);
+            }
       }
     }
     const int h = w0 / WP, n0 = w0 % WP;
     rows_of(w0 + S::kStep);  // the next rows' first operands are on their way during the stores
-    if (w0 + S::kStep < w_end) {
-      read_w(0, a[0]);
-      read_w(min(1, steps - 1), a[1]);
-    }
+    if (w0 + S::kStep < w_end) read_w(0, a[0]);
     const bool key = n0 < NT;
     _Float16* const dst = key ? x.k : x.v;
     const int64_t plane = key ? x.k_plane : x.v_plane;
