@@ -10,40 +10,63 @@ namespace jero {
 
 // One wave per token row: lane l holds elements 8l .. 8l + 7 of the latent, the first rope / 2 lanes a
 // pair of the key part each.  The sum of squares is f32; the row is rounded once, to the cache's type.
-template <typename X, typename KV>
+// VEC: the rows of x are 16-byte aligned, and are read so (stores always are: 8-element rows of the pool).  What
+// the row needs is on its way before the row's place is looked up.
+template <typename X, typename KV, bool VEC>
 __global__ void __launch_bounds__(256) mla_append_kernel(LatentCache c, const X* __restrict__ x, int64_t x_stride,
                                                          const float* __restrict__ norm, float eps, MlaRope rope) {
   const int lane = threadIdx.x & 63;
   const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= c.n_tokens) return;
+  const X* xr = x + t * x_stride;
+  const int k = min(8 * lane, c.rank - 8), i = min(lane, c.rope / 2 - 1);
+  float v[8], w[8];
+  if constexpr (VEC) {
+    load8<X>(xr + k, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = float(xr[k + e]);
+  }
+  if (norm) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) w[e] = norm[k + e];
+  }
+  const float a = float(xr[c.rank + 2 * i]), b = float(xr[c.rank + 2 * i + 1]);
   int seq, pos;
   if (!mla_locate(c, t, lane, seq, pos) || pos < 0 || pos >= c.max_len) return;
   const int64_t at = mla_row(c, seq, pos);
   if (at < 0) return;
-  const X* xr = x + t * x_stride;
   KV* row = static_cast<KV*>(const_cast<void*>(c.rows)) + at;
-  float v[8];
-  float ss = 0.f;
   const bool in = 8 * lane < c.rank;
-#pragma unroll
-  for (int e = 0; e < 8; e++) {
-    v[e] = in ? float(xr[8 * lane + e]) : 0.f;
-    ss += v[e] * v[e];
-  }
   if (norm) {
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) ss += in ? v[e] * v[e] : 0.f;
     ss = wave_sum_dpp(ss);
     const float inv = 1.0f / sqrtf(ss / float(c.rank) + eps);
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = in ? v[e] * inv * norm[8 * lane + e] : 0.f;
+    for (int e = 0; e < 8; e++) v[e] = v[e] * inv * w[e];
   }
-  if (in)
+  if (in) {
+    if constexpr (sizeof(KV) == 4) {
+      reinterpret_cast<float4*>(row + k)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(row + k)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      h8_t y;
 #pragma unroll
-    for (int e = 0; e < 8; e++) row[8 * lane + e] = KV(v[e]);
+      for (int e = 0; e < 8; e++) y[e] = _Float16(v[e]);
+      *reinterpret_cast<h8_t*>(row + k) = y;
+    }
+  }
   if (lane < c.rope / 2) {
-    const float a = float(xr[c.rank + 2 * lane]), b = float(xr[c.rank + 2 * lane + 1]);
     const float2 cs = rope.on ? mla_cos_sin(rope, lane, pos) : make_float2(1.f, 0.f);
-    row[c.rank + 2 * lane] = KV(a * cs.x - b * cs.y);
-    row[c.rank + 2 * lane + 1] = KV(a * cs.y + b * cs.x);
+    const float y = a * cs.x - b * cs.y, z = a * cs.y + b * cs.x;
+    if constexpr (sizeof(KV) == 4) {
+      *reinterpret_cast<float2*>(row + c.rank + 2 * lane) = make_float2(y, z);
+    } else {
+      typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+      *reinterpret_cast<h2_t*>(row + c.rank + 2 * lane) = h2_t{_Float16(y), _Float16(z)};
+    }
   }
 }
 
@@ -1013,14 +1036,24 @@ extern "C" int jero_hip_mla_append(const jero_latent_cache* cache, int act_dtype
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool f16 = cache->kv_dtype == JERO_KV_F16;
 #define JERO_APPEND(X, KV)                                                                                          \
-  hipLaunchKernelGGL((mla_append_kernel<X, KV>), grid, dim3(256), 0, s, c, static_cast<const X*>(x_dev), x_stride, \
-                     norm_dev, eps, rope)
+  if (vec)                                                                                                          \
+    hipLaunchKernelGGL((mla_append_kernel<X, KV, true>), grid, dim3(256), 0, s, c, static_cast<const X*>(x_dev),   \
+                       x_stride, norm_dev, eps, rope);                                                              \
+  else                                                                                                              \
+    hipLaunchKernelGGL((mla_append_kernel<X, KV, false>), grid, dim3(256), 0, s, c, static_cast<const X*>(x_dev),  \
+                       x_stride, norm_dev, eps, rope)
+  const int size = act_dtype == JERO_F32 ? 4 : 2;
+  const bool vec = !((reinterpret_cast<uintptr_t>(x_dev) | uintptr_t(x_stride * size)) & 15u);
   if (act_dtype == JERO_F32) {
-    if (f16) JERO_APPEND(float, _Float16);
-    else JERO_APPEND(float, float);
+    if (f16) {
+      JERO_APPEND(float, _Float16);
+    } else {
+      JERO_APPEND(float, float);
+    }
+  } else if (f16) {
+    JERO_APPEND(_Float16, _Float16);
   } else {
-    if (f16) JERO_APPEND(_Float16, _Float16);
-    else JERO_APPEND(_Float16, float);
+    JERO_APPEND(_Float16, float);
   }
 #undef JERO_APPEND
   return check_launch("mla_append");
