@@ -55,7 +55,9 @@ __global__ void __launch_bounds__(512) mla_expand_kernel(LatentCache c, int nh, 
   constexpr bool WIDE = S::kWide;
   constexpr int WP = NT + VT, MP = S::kPos, CP = S::kPlanes, P = S::kPitch, MJ = MP / 16;
   __shared__ __attribute__((aligned(16))) _Float16 s_c[CP][MP][P];
-  __shared__ int64_t s_row[MP];  // the positions' cache rows: -1 for a block that is none, -2 for no position
+  // the positions' cache rows: -1 for a block that is none, -2 for no position; -3, once it is read, for one of
+  // infinities or NaN
+  __shared__ int64_t s_row[MP];
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   // blocks of one run of weight rows follow each other, over all XCDs; the key parts' come last
   const int across = int((x.total + MP - 1) / MP), part = blockIdx.x / across;
@@ -127,7 +129,8 @@ __global__ void __launch_bounds__(512) mla_expand_kernel(LatentCache c, int nh, 
   rows_of(w0);
   read_w(0, a[0]);
 
-  // the latents: a lane 8 values, 8 rows' loads at a time
+  // The latents: a lane 8 values, 8 rows' loads at a time.  A row that is not finite makes keys that are not, so NaN
+  // of every token that attends to it; its values are made zeros, as tokens before it would take 0 * NaN from them.
   for (int r0 = wv; r0 < MP; r0 += 64) {
     float v[8][WIDE ? 8 : 1];
     h8_t hv[8];
@@ -158,9 +161,16 @@ __global__ void __launch_bounds__(512) mla_expand_kernel(LatentCache c, int nh, 
         }
         *reinterpret_cast<h8_t*>(&s_c[0][r0 + 8 * i][k]) = hi;
         *reinterpret_cast<h8_t*>(&s_c[CP - 1][r0 + 8 * i][k]) = lo;
+        hv[i] = hi;
       } else {
         *reinterpret_cast<h8_t*>(&s_c[0][r0 + 8 * i][k]) = hv[i];
       }
+      typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+      float odd = 0.f;  // sum of 0 * value
+#pragma unroll
+      for (int e = 0; e < 8; e += 2)
+        odd = __builtin_amdgcn_fdot2(h2_t{hv[i][e], hv[i][e + 1]}, h2_t{_Float16(0), _Float16(0)}, odd, false);
+      if (__ballot(odd != 0.f) && lane == 0) s_row[r0 + 8 * i] = -3;
     }
   }
   __syncthreads();
@@ -203,7 +213,9 @@ __global__ void __launch_bounds__(512) mla_expand_kernel(LatentCache c, int nh, 
     const int width = key ? NT : VT, n = (key ? n0 : n0 - NT) + 16 * g;
 #pragma unroll
     for (int j = 0; j < MJ; j++) {
-      if (s_row[16 * j + col] == -2) continue;
+      const int64_t row = s_row[16 * j + col];
+      if (row == -2) continue;
+      const bool zero = row == -3 && !key;
       _Float16* p = dst + (int64_t(h) * x.total + m0 + 16 * j + col) * width + n;
 #pragma unroll
       for (int half = 0; half < 2; half++) {
@@ -211,7 +223,7 @@ __global__ void __launch_bounds__(512) mla_expand_kernel(LatentCache c, int nh, 
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           _Float16 y, z;
-          split2(acc[2 * half + e / 4][j][e % 4], y, z);
+          split2(zero ? 0.f : acc[2 * half + e / 4][j][e % 4], y, z);
           hi[e] = y, lo[e] = z;
         }
         *reinterpret_cast<h8_t*>(p + 8 * half) = hi;

@@ -267,6 +267,136 @@ def test_two_streams_at_once(dev, form):
     assert torch.equal(out, want[0])
 
 
+@pytest.mark.parametrize("act,kv", TYPES)
+@pytest.mark.parametrize("form", FORMS)
+def test_later_positions_may_hold_anything(dev, form, act, kv):
+    """Rows and queries of NaN and infinities, of a call's own tokens: the tokens before them do not see them, those
+    that attend to NaN are NaN."""
+    for what, rank in ((np.nan, 64), (np.inf, 128), (-np.inf, 8)):
+        p = Problem(32, [40, 150, 9], [6, 150 if form == "expanded" else 4, 1], heads=3, act=act, kv=kv, rank=rank)
+        hit = []
+        for t, s, pos in p.tokens():
+            if (s, pos) in ((0, 37), (1, 148)):
+                p.rows[p.table[s, pos // p.block], pos % p.block, -3 if s else rank - 1] = what
+                p.q[t] = what
+            if s == 0 and pos >= 37 or s == 1 and pos >= 148:
+                hit.append(t)
+        p.device(dev)
+        out = p.run(form).float().cpu().numpy()
+        if np.isnan(what):
+            assert np.isnan(out[hit]).all()
+        with np.errstate(all="ignore"):
+            exact, far = p.attention()
+        rest = [t for t, _, _ in p.tokens() if t not in hit]
+        far_, rms = off(out[rest].astype(np.float64), exact[rest], far[rest])
+        assert far_ <= 1 and rms <= 1, (what, far_, rms)
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+@pytest.mark.parametrize("form", FORMS)
+def test_other_scales(dev, form, scale):
+    """A negative scale, and 0: the mean of the values."""
+    p = Problem(33, [70, 33], [2, 1], heads=4)
+    p.scale = scale if scale == 0 else float(np.float32(scale))
+    p.device(dev)
+    p.check(p.run(form), what=form)
+
+
+MANY = [(70, [8] * 70, 2), (600, [1] * 600, 16), (130, [i % 7 for i in range(130)], 4)]
+
+
+@pytest.mark.parametrize("n,new,block", MANY, ids=lambda x: str(x) if isinstance(x, int) else "")
+@pytest.mark.parametrize("form", FORMS)
+def test_many_sequences(dev, form, n, new, block):
+    """More sequences, and tokens, than a wave's lanes and than a workgroup's threads."""
+    print(f"mla {form} {n} sequences", flush=True)
+    lens = [(37 * i) % 41 for i in range(n)]
+    p = Problem(34, lens, new, heads=2, block=block, nope=8, v=8, pad_rows=1).device(dev)
+    ref = p.attention()
+    p.check(p.run(form), ref, form)
+    if one_each(p):
+        q = Problem(34, lens, new, heads=2, block=block, nope=8, v=8).device(dev, starts=False)
+        q.check(q.run(form), what="without starts")
+    p.device(dev)
+    J.mla_append(p.cache, p.d["x"], p.d["norm"], EPS, THETA)
+    check_rows(p, p.d["rows"], p.rows, *p.appended())
+
+
+@pytest.mark.parametrize("act,kv", TYPES)
+@pytest.mark.parametrize("block", [1, 2, 16])
+def test_tables_of_many_blocks(dev, block, act, kv):
+    """Long sequences of small blocks: the absorbed form reads their ids 64 at a time, and some are none."""
+    p = Problem(35, [2500 if block == 16 else 333, 130], [1, 2], heads=3, block=block, act=act, kv=kv, rank=128, rope=32)
+    p.table[0, 66:70] = -1
+    p.table[0, 130] = p.n_blocks
+    p.device(dev)
+    ref = p.attention()
+    for form in FORMS:
+        print(f"mla {form} block {block}", flush=True)
+        p.check(p.run(form), ref, form)
+
+
+# lens, new, heads, widths: few blocks of 128 tokens over long sequences, which are cut into runs of 512 positions
+# or more, each a partial row a token
+LONG = [
+    ([1500], [3], 4, {}), ([513], [1], 2, {}), ([1100, 700, 40], [2, 130, 1], 3, dict(rank=128, rope=32, nope=64, v=64)),
+    ([1025, 0, 600], [1, 1, 40], 5, BIG), ([2049], [1], 2, dict(rank=72, rope=24, nope=192, v=200)),
+]
+
+
+@pytest.mark.parametrize("act,kv", TYPES)
+@pytest.mark.parametrize("case", LONG, ids=lambda c: "-".join(map(str, c[0])))
+def test_prompts_cut_into_runs(dev, case, act, kv):
+    """With room for the partial rows and without, and where a whole run's blocks are none."""
+    print(f"mla expanded {act} {kv} {case}", flush=True)
+    lens, new, heads, dims = case
+    p = Problem(36, lens, new, heads=heads, block=64, act=act, kv=kv, pad_rows=2, **dims)
+    for gone in (False, True):
+        if gone:
+            p.table[0, 0:8] = -1
+            p.table[0, 17:25] = -1
+        p.device(dev)
+        ref = p.attention()
+        p.check(p.run("expanded"), ref, "cut")
+        L = J.lib()
+        need = L.jero_hip_mla_prefill_workspace_bytes(p.cache.ref, J.F16 if act == "f16" else J.F32, 1, p.N, p.V, p.total())
+        ws = torch.full((need + 256,), 255, dtype=torch.uint8, device=dev)
+        p.check(p.run("expanded", workspace=ws[:need]), ref, "whole")
+        assert (ws[need:] == 255).all()
+    if gone:  # and nothing but what is masked
+        p.table[0, :] = -1
+        p.device(dev)
+        out = p.run("expanded")
+        p.check(out, what="masked")
+        assert (out[:new[0]] == 0).all()
+
+
+def test_a_captured_long_prompt_follows_its_length(dev):
+    """One graph over lengths on both sides of a run's end."""
+    p = Problem(37, [1400], [2], heads=4, block=64, pad_rows=1, rest=0.0).device(dev)
+    out = torch.full((p.T, p.H, p.V), 7.0, device=dev)
+    need = J.lib().jero_hip_mla_prefill_workspace_bytes(p.cache.ref, J.F32, p.H, p.N, p.V, p.total())
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    kw = dict(workspace=ws, total=1400)
+    s = torch.cuda.Stream(dev)
+    with torch.cuda.stream(s):
+        p.run("expanded", out=out, **kw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        p.run("expanded", out=out, **kw)
+    for n in (1400, 2, 511, 512, 514, 1, 1025, 0, 1399):
+        p.lens = [n]
+        p.d["lens"].copy_(torch.tensor([n], dtype=torch.int32))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        p.check(out, what=f"length {n}")
+        eager = p.run("expanded", total=1400)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, out)
+
+
 # ---------------------------------------------------------------- append
 
 

@@ -90,6 +90,18 @@ def test_bad_weights_and_totals():
     assert prefill(c, nope=248, qs=2 * 264) == 10  # nope + rope above 256
 
 
+def test_largest_calls():
+    """Tokens, sequences, expanded rows and tiles past what the kernels' 32-bit counts are made for."""
+    c = cache(n_seqs=1 << 20, starts_dev=FAKE)
+    for call in (append, absorbed, prefill):
+        assert call(c) == 14
+        assert call(cache(starts_dev=FAKE), tokens=(1 << 19) + 1) == 14
+    assert prefill(cache(), total=(1 << 23) + 1) == 14
+    wide = dict(tokens=1 << 19, heads=1024, qs=1024 * 48, os_=1024 * 40)
+    assert prefill(cache(n_seqs=1 << 19), n=1 << 62, **wide) == 10  # 2^19 tiles of 1024 heads
+    assert absorbed(cache(n_seqs=1 << 19), **wide) == 14  # its workspace
+
+
 def test_workspace_sizes():
     L, c = J.lib(), cache()
     assert L.jero_hip_mla_absorbed_workspace_bytes(None, 1, 1) == 0
