@@ -182,16 +182,30 @@ __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X*
       kb = kx * cs.y + ky * cs.x;
     }
     if (!key) ka = kb = 0.f;
+    // (f32: a token's values are brought near 1 by a power of two, so that their parts keep 22 bits whatever they are)
+    int near = 0;
+    if constexpr (sizeof(X) == 4) {
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) m = fmaxf(m, 32 * i + 8 * g < nope ? fabsf(qv[i][e]) : 0.f);
+      m = max_over_groups(m);
+      near = m > 0.f && m < INFINITY ? ilogbf(m) : 0;
+    }
     h8_t ah[NT], al[NT];
 #pragma unroll
     for (int i = 0; i < NT; i++) {
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         _Float16 x, y;
-        split2(32 * i + 8 * g < nope ? qv[i][e] : 0.f, x, y);
+        split2(32 * i + 8 * g < nope ? ldexpf(qv[i][e], -near) : 0.f, x, y);
         ah[i][e] = x, al[i][e] = y;
       }
     }
+    int back[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) back[e] = sizeof(X) == 4 ? __shfl(near, 4 * g + e, kWave) : 0;
     f4_t v[NR];
     float mx[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -205,7 +219,7 @@ __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X*
       }
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        v[k][e] = r0 + col < c.rank ? hi[e] + lo[e] : 0.f;
+        v[k][e] = r0 + col < c.rank ? ldexpf(hi[e] + lo[e], back[e]) : 0.f;
         mx[e] = fmaxf(mx[e], fabsf(v[k][e]));
       }
     }
@@ -975,9 +989,20 @@ int mla_rope_of(float theta, int rope_dim, MlaRope* out) {
   if (theta == 0.f) return JERO_OK;
   if (!(theta > 0.f) || !std::isfinite(theta))
     return fail(JERO_ERR_INVALID_ARGUMENT, "rope_theta must be positive, or 0 for rotated rows");
-  out->on = 1;
-  for (int i = 0; i < rope_dim / 2; i++)
-    out->turns[i] = std::pow(double(theta), -2.0 * i / rope_dim) / 6.283185307179586476925;
+  // (a model's calls all ask for the same: 32 powers cost the host a launch's time)
+  static thread_local struct {
+    float theta = 0.f;
+    int dim = 0;
+    MlaRope rope{};
+  } last;
+  if (last.theta != theta || last.dim != rope_dim) {
+    last.theta = theta;
+    last.dim = rope_dim;
+    last.rope.on = 1;
+    for (int i = 0; i < rope_dim / 2; i++)
+      last.rope.turns[i] = std::pow(double(theta), -2.0 * i / rope_dim) / 6.283185307179586476925;
+  }
+  *out = last.rope;
   return JERO_OK;
 }
 

@@ -116,6 +116,18 @@ def test_peaked_scores(dev, form, act, kv):
     p.check(p.run(form), what=form)
 
 
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("size", [2.0 ** -70, 1e-7, 1e7, 2.0 ** 70])
+def test_f32_queries_of_any_size(dev, form, size, kv):
+    """Far below and above f16's range, with the scale that brings the scores back."""
+    p = Problem(38, [70, 33], [2, 1], heads=3, kv=kv)
+    p.q = (p.q.astype(np.float64) * size).astype(np.float32)
+    p.scale = float(np.float32(p.scale / size))
+    p.device(dev)
+    p.check(p.run(form), what=f"{form} {size}")
+
+
 def test_long_queries_and_far_positions(dev):
     """Absorbed queries past f16's range (their scores are brought back by the scale), and the rotation at a
     position where 32-bit angles are off by 1e-3."""
