@@ -525,45 +525,48 @@ class LatentCache:
 
     def __init__(self, rows, table, lens, rank, starts=None, max_len=None):
         import torch
-        held = [("rows", rows), ("table", table), ("lens", lens)] + ([("starts", starts)] if starts is not None else [])
-        for name, t in held:
-            _latent_check(t.is_cuda and t.device == rows.device, 21, f"LatentCache: {name} must be on the cache's GPU")
-            _latent_check(t.is_contiguous(), 21, f"LatentCache: {name} must be contiguous")
-            _latent_check(name == "rows" or t.dtype == torch.int32, 21, f"LatentCache: {name} must be int32")
+        device, i32 = rows.device, torch.int32
+        # (a decode step makes one in the time that a kernel takes: names and sentences only for what is refused)
+        for name, t in (("rows", rows), ("table", table), ("lens", lens), ("starts", starts)):
+            if t is None:
+                _latent_check(name == "starts", 21, "LatentCache: rows, table and lens are needed")
+            elif not (t.is_cuda and t.device == device and t.is_contiguous() and (t is rows or t.dtype is i32)):
+                _latent_check(t.is_cuda and t.device == device, 21, f"LatentCache: {name} must be on the cache's GPU")
+                _latent_check(t.is_contiguous(), 21, f"LatentCache: {name} must be contiguous")
+                _latent_check(False, 21, f"LatentCache: {name} must be int32")
         _latent_check(rows.dtype in (torch.float32, torch.float16), 10, "LatentCache: rows must be float32 or float16")
-        _latent_check(rows.dim() == 3 and table.dim() == 2 and lens.dim() == 1, 14,
+        shape, blocks, seqs = rows.shape, table.shape, lens.shape
+        _latent_check(len(shape) == 3 and len(blocks) == 2 and len(seqs) == 1, 14,
                       "LatentCache: rows [blocks, block_size, width], table [seqs, blocks], lens [seqs]")
-        _latent_check(table.shape[0] == lens.shape[0], 14, "LatentCache: table and lens differ in sequences")
-        _latent_check(starts is None or starts.shape == (lens.shape[0] + 1,), 14, "LatentCache: starts must be [seqs + 1]")
-        _latent_check(0 < rank < rows.shape[2], 14, "LatentCache: rank must be below the rows' width")
+        _latent_check(blocks[0] == seqs[0], 14, "LatentCache: table and lens differ in sequences")
+        _latent_check(starts is None or starts.shape == (seqs[0] + 1,), 14, "LatentCache: starts must be [seqs + 1]")
+        _latent_check(0 < rank < shape[2], 14, "LatentCache: rank must be below the rows' width")
         self.rows, self.table, self.lens, self.starts, self.rank = rows, table, lens, starts, rank
         if max_len is None:
-            max_len = table.shape[1] * rows.shape[1]
+            max_len = blocks[1] * shape[1]
         self.c = HipLatentCache(rows.data_ptr(), table.data_ptr(), lens.data_ptr(),
-                                starts.data_ptr() if starts is not None else None, rows.shape[0], table.shape[1],
-                                lens.shape[0], max_len, rows.shape[1], KV_F16 if rows.dtype == torch.float16 else KV_F32,
-                                rank, rows.shape[2] - rank)
+                                None if starts is None else starts.data_ptr(), shape[0], blocks[1], seqs[0], max_len,
+                                shape[1], KV_F16 if rows.dtype is torch.float16 else KV_F32, rank, shape[2] - rank)
         self.ref = C.byref(self.c)
 
 
 def _latent_act(t, cache, what):
     """act_dtype of a device tensor whose last dimensions are packed."""
     import torch
-    _latent_check(t.is_cuda and t.device == cache.rows.device, 21, f"{what} must be on the cache's GPU")
-    if t.dtype == torch.float32:
+    if not (t.is_cuda and t.device == cache.rows.device):
+        _latent_check(False, 21, f"{what} must be on the cache's GPU")
+    if t.dtype is torch.float32:
         return F32
-    _latent_check(t.dtype == torch.float16, 10, f"{what} must be float32 or float16")
+    if t.dtype is not torch.float16:
+        _latent_check(False, 10, f"{what} must be float32 or float16")
     return F16
 
 
 def _latent_stream(cache, stream):
     """The stream's handle; a call runs on the current device, which has to be the cache's."""
-    if stream is None:
-        import torch
-        _latent_check(cache.rows.device.index == torch.cuda.current_device(), 21,
-                      "the cache must be on the current device")
-    else:
-        _latent_check(stream.device == cache.rows.device, 21, "the stream must be of the cache's device")
+    import torch
+    _latent_check(cache.rows.device.index == torch.cuda.current_device(), 21, "the cache must be on the current device")
+    _latent_check(stream is None or stream.device == cache.rows.device, 21, "the stream must be of the cache's device")
     return _stream(stream)
 
 
@@ -572,14 +575,15 @@ def mla_append(cache, x, norm, eps, rope_theta, stream=None):
     may be apart), its latent part RMS-normalised with the f32 weights ``norm`` (None: stored as it is), its key
     part rotated to the token's position (rope_theta 0: stored as it is)."""
     import torch
-    act = _latent_act(x, cache, "mla_append: x")
-    _latent_check(x.dim() == 2 and x.shape[1] == cache.rows.shape[2] and x.stride(1) == 1, 14,
+    act, shape, stride = _latent_act(x, cache, "mla_append: x"), x.shape, x.stride()
+    _latent_check(len(shape) == 2 and shape[1] == cache.c.rank + cache.c.rope_dim and stride[1] == 1, 14,
                   "mla_append: x must be [tokens, rank + rope_dim] with packed rows")
     if norm is not None:
-        _latent_check(norm.dtype == torch.float32 and norm.device == x.device and norm.is_contiguous()
+        _latent_check(norm.dtype is torch.float32 and norm.device == x.device and norm.is_contiguous()
                       and norm.numel() == cache.rank, 14, "mla_append: norm must be rank packed float32 values")
-    check(lib().jero_hip_mla_append(cache.ref, act, x.data_ptr(), x.stride(0) if x.shape[0] > 1 else x.shape[1],
-                                    x.shape[0], _ptr(norm), eps, rope_theta, _latent_stream(cache, stream)))
+        norm = norm.data_ptr()
+    check(lib().jero_hip_mla_append(cache.ref, act, x.data_ptr(), stride[0] if shape[0] > 1 else shape[1], shape[0],
+                                    norm, eps, rope_theta, _latent_stream(cache, stream)))
 
 
 def _latent_args(what, out, q, cache, weights, v_dim):
@@ -597,10 +601,14 @@ def _latent_args(what, out, q, cache, weights, v_dim):
     return act, T, H, q.stride(0) if T > 1 else H * D, out.stride(0) if T > 1 else H * v_dim
 
 
-def _latent_workspace(workspace, need, like):
+def _latent_workspace(workspace, need, like, stream):
     if workspace is None:
         import torch
-        workspace = torch.empty(need, dtype=torch.uint8, device=like.device)
+        if stream is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=like.device)
+        else:  # of the call's own stream: the allocator hands it on to later work of that stream only
+            with torch.cuda.stream(stream):
+                workspace = torch.empty(need, dtype=torch.uint8, device=like.device)
     else:
         _latent_check(workspace.device == like.device and workspace.is_contiguous(), 21,
                       "workspace must be packed, on the cache's GPU")
@@ -620,7 +628,7 @@ def mla_absorbed_attention(out, q, cache, k_b, v_b, scale, rope_theta, workspace
     _latent_check(tuple(k_b.shape) == (H, cache.rank, N) and tuple(v_b.shape) == (H, v_b.shape[1], cache.rank), 14,
                   f"{what}: k_b must be [heads, rank, nope], v_b [heads, v, rank]")
     L, s = lib(), _latent_stream(cache, stream)
-    ws, n = _latent_workspace(workspace, L.jero_hip_mla_absorbed_workspace_bytes(cache.ref, T, H), q)
+    ws, n = _latent_workspace(workspace, L.jero_hip_mla_absorbed_workspace_bytes(cache.ref, T, H), q, stream)
     check(L.jero_hip_mla_absorbed_attention(cache.ref, act, q.data_ptr(), qs, T, H, N, v_b.shape[1], k_b.data_ptr(),
                                             v_b.data_ptr(), scale, rope_theta, out.data_ptr(), os_, ws.data_ptr(), n, s))
     return out
@@ -637,7 +645,8 @@ def mla_prefill_attention(out, q, cache, kv_b, total_len, scale, rope_theta, wor
     N = q.shape[2] - cache.c.rope_dim
     _latent_check(tuple(kv_b.shape) == (H, N + V, cache.rank), 14, f"{what}: kv_b must be [heads, nope + v, rank]")
     L, s = lib(), _latent_stream(cache, stream)
-    ws, n = _latent_workspace(workspace, L.jero_hip_mla_prefill_workspace_bytes(cache.ref, act, H, N, V, total_len), q)
+    ws, n = _latent_workspace(workspace, L.jero_hip_mla_prefill_workspace_bytes(cache.ref, act, H, N, V, total_len), q,
+                              stream)
     check(L.jero_hip_mla_prefill_attention(cache.ref, act, q.data_ptr(), qs, T, H, N, V, kv_b.data_ptr(), total_len,
                                            scale, rope_theta, out.data_ptr(), os_, ws.data_ptr(), n, s))
     return out
