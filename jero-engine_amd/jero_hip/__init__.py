@@ -511,9 +511,9 @@ class HipLatentCache(C.Structure):
                 ("block_size", C.c_int), ("kv_dtype", C.c_int), ("rank", C.c_int), ("rope_dim", C.c_int)]
 
 
-def _latent_check(cond, status, message):
+def _latent_check(cond, status, *words):
     if not cond:
-        raise K3Error(status, message)
+        raise K3Error(status, ": ".join(words))
 
 
 class LatentCache:
@@ -529,7 +529,7 @@ class LatentCache:
         # (a decode step makes one in the time that a kernel takes: names and sentences only for what is refused)
         for name, t in (("rows", rows), ("table", table), ("lens", lens), ("starts", starts)):
             if t is None:
-                _latent_check(name == "starts", 21, "LatentCache: rows, table and lens are needed")
+                _latent_check(name == "starts", 21, "LatentCache: table and lens are needed")
             elif not (t.is_cuda and t.device == device and t.is_contiguous() and (t is rows or t.dtype is i32)):
                 _latent_check(t.is_cuda and t.device == device, 21, f"LatentCache: {name} must be on the cache's GPU")
                 _latent_check(t.is_contiguous(), 21, f"LatentCache: {name} must be contiguous")
@@ -588,17 +588,19 @@ def mla_append(cache, x, norm, eps, rope_theta, stream=None):
 
 def _latent_args(what, out, q, cache, weights, v_dim):
     import torch
-    act = _latent_act(q, cache, f"{what}: q")
-    _latent_check(out.dtype == q.dtype and out.device == q.device, 21, f"{what}: out and q differ in type or device")
-    _latent_check(q.dim() == 3 and out.dim() == 3 and out.shape[:2] == q.shape[:2] and out.shape[2] == v_dim, 14,
-                  f"{what}: q must be [tokens, heads, nope + rope], out [tokens, heads, v]")
-    for t in (q, out):
-        _latent_check(t.stride(2) == 1 and t.stride(1) == t.shape[2], 21, f"{what}: a token's heads must be packed")
+    act, dtype, device = _latent_act(q, cache, "q"), q.dtype, q.device
+    _latent_check(out.dtype is dtype and out.device == device, 21, what, "out and q differ in type or device")
+    shape, to = q.shape, out.shape
+    _latent_check(len(shape) == 3 and len(to) == 3 and to[:2] == shape[:2] and to[2] == v_dim, 14, what,
+                  "q must be [tokens, heads, nope + rope], out [tokens, heads, v]")
+    T, H, D = shape
+    qs, os_ = q.stride(), out.stride()
+    _latent_check(qs[2] == 1 and os_[2] == 1 and (H == 1 or qs[1] == D and os_[1] == v_dim), 21, what,
+                  "a token's heads must be packed")
     for w in weights:
-        _latent_check(w.dtype == torch.float16 and w.device == q.device and w.is_contiguous(), 21,
-                      f"{what}: weights must be packed float16 on the cache's GPU")
-    T, H, D = q.shape
-    return act, T, H, q.stride(0) if T > 1 else H * D, out.stride(0) if T > 1 else H * v_dim
+        _latent_check(w.dtype is torch.float16 and w.device == device and w.is_contiguous(), 21, what,
+                      "weights must be packed float16 on the cache's GPU")
+    return act, T, H, qs[0] if T > 1 else H * D, os_[0] if T > 1 else H * v_dim
 
 
 def _latent_workspace(workspace, need, like, stream):
@@ -622,14 +624,15 @@ def mla_absorbed_attention(out, q, cache, k_b, v_b, scale, rope_theta, workspace
     nope] and v_b [heads, v, rank] f16.  The rows of q and out may be apart.  The tokens' own rows have been
     appended."""
     what = "mla_absorbed_attention"
-    _latent_check(k_b.dim() == 3 and v_b.dim() == 3, 14, f"{what}: k_b must be [heads, rank, nope], v_b [heads, v, rank]")
-    act, T, H, qs, os_ = _latent_args(what, out, q, cache, (k_b, v_b), v_b.shape[1])
+    kb, vb = k_b.shape, v_b.shape
+    V = vb[1] if len(vb) == 3 else 0
+    act, T, H, qs, os_ = _latent_args(what, out, q, cache, (k_b, v_b), V)
     N = q.shape[2] - cache.c.rope_dim
-    _latent_check(tuple(k_b.shape) == (H, cache.rank, N) and tuple(v_b.shape) == (H, v_b.shape[1], cache.rank), 14,
-                  f"{what}: k_b must be [heads, rank, nope], v_b [heads, v, rank]")
+    _latent_check(kb == (H, cache.rank, N) and vb == (H, V, cache.rank), 14, what,
+                  "k_b must be [heads, rank, nope], v_b [heads, v, rank]")
     L, s = lib(), _latent_stream(cache, stream)
     ws, n = _latent_workspace(workspace, L.jero_hip_mla_absorbed_workspace_bytes(cache.ref, T, H), q, stream)
-    check(L.jero_hip_mla_absorbed_attention(cache.ref, act, q.data_ptr(), qs, T, H, N, v_b.shape[1], k_b.data_ptr(),
+    check(L.jero_hip_mla_absorbed_attention(cache.ref, act, q.data_ptr(), qs, T, H, N, V, k_b.data_ptr(),
                                             v_b.data_ptr(), scale, rope_theta, out.data_ptr(), os_, ws.data_ptr(), n, s))
     return out
 
@@ -639,11 +642,10 @@ def mla_prefill_attention(out, q, cache, kv_b, total_len, scale, rope_theta, wor
     (jero_hip_mla_prefill_attention).  As mla_absorbed_attention, with kv_b [heads, nope + v, rank] f16 and
     total_len at least the sum of the sequences' lengths."""
     what = "mla_prefill_attention"
-    _latent_check(kv_b.dim() == 3 and out.dim() == 3, 14, f"{what}: kv_b must be [heads, nope + v, rank]")
-    V = out.shape[2]
+    V = out.shape[2] if out.dim() == 3 else 0
     act, T, H, qs, os_ = _latent_args(what, out, q, cache, (kv_b,), V)
     N = q.shape[2] - cache.c.rope_dim
-    _latent_check(tuple(kv_b.shape) == (H, N + V, cache.rank), 14, f"{what}: kv_b must be [heads, nope + v, rank]")
+    _latent_check(kv_b.shape == (H, N + V, cache.rank), 14, what, "kv_b must be [heads, nope + v, rank]")
     L, s = lib(), _latent_stream(cache, stream)
     ws, n = _latent_workspace(workspace, L.jero_hip_mla_prefill_workspace_bytes(cache.ref, act, H, N, V, total_len), q,
                               stream)
