@@ -334,7 +334,8 @@ __device__ __forceinline__ int mla_token_of(const int* prefix, int n, int x, int
   return lo;
 }
 
-constexpr int kAttendTile = 32;  // positions a step
+// Positions a step: 32, and 32 for each wave where waves of two 16s of heads share the positions.
+static constexpr int attend_tile(int hw, int ks) { return hw > 1 ? 32 * ks : 32; }
 
 // Shape of the attend kernel: HG waves of 16 heads by KS waves of WR positions, RT + PT the padded widths,
 // KV the cache's type.  LDS holds a step's rows in f16, the latents and then the key parts, so that neither 8
@@ -342,20 +343,20 @@ constexpr int kAttendTile = 32;  // positions a step
 // bytes have 16 more after them (one address a lane for all reads), the chunks of shorter ones are swapped by the
 // row's number.  An f16 cache is loaded straight into one of four such buffers; an f32 cache into a raw buffer,
 // from which each wave turns its rows into a buffer of their upper and one of their lower parts.
-template <int RT, int PT, int HG, int KS, typename KV>
+template <int RT, int PT, int HG, int HW, int KS, typename KV>
 struct AttendShape {
   static constexpr bool kWide = sizeof(KV) == 4;
   static constexpr int kWaves = HG * KS;
-  static constexpr int kTile = kAttendTile;
+  static constexpr int kTile = attend_tile(HW, KS);
   static constexpr int WR = kTile / KS;
   static constexpr int kRows = kTile / kWaves;  // rows a wave loads
   static constexpr bool kPad = RT == 512;
   static constexpr int kPitch = RT * 2 + (kPad ? 16 : 0);
   static constexpr int kLat = kTile * kPitch;
   static constexpr int kBuf = kLat + kTile * PT * 2;
-  static constexpr int kBufs = kWide ? 2 : 4;
+  static constexpr int kBufs = kWide ? 2 : HW > 1 ? 4 / KS : 4;
   static constexpr int kRaw = kWide ? kTile * (RT + PT) * 4 : 0;
-  static constexpr int kMerge = KS > 1 ? HG * (KS - 1) * 16 * (RT + 4) * 4 : 0;  // over the buffers
+  static constexpr int kMerge = KS > 1 ? HG * HW * (KS - 1) * 16 * (RT + 4) * 4 : 0;  // over the buffers
   static constexpr int kLds = kBufs * kBuf + kRaw > kMerge ? kBufs * kBuf + kRaw : kMerge;
   // loads of 1024 bytes a wave issues for a step: of the latents, of the key parts
   static constexpr int kLoadsLat = kRows * RT * int(sizeof(KV)) / 1024;
@@ -380,11 +381,13 @@ struct AttendShape {
 // Registers allow one wave a SIMD, so a wave covers its own waits: a step's softmax runs between the products
 // of the next step's scores, operands are read from LDS a group of products ahead, and the rows two steps on are
 // on their way from the cache meanwhile (f16 cache; an f32 one has its LDS filled by the parts of one step).
-template <int RT, int PT, int HG, int KS, typename KV, bool TWO>
+template <int RT, int PT, int HG, int HW, int KS, typename KV, bool TWO>
 __global__ void __launch_bounds__(64 * HG * KS, 1)
     mla_attend_kernel(LatentCache c, MlaQueries qa, int nh, MlaPlan plan, int runs, int least, int extra,
                       float* __restrict__ part_o, float2* __restrict__ part_ml) {
-  using S = AttendShape<RT, PT, HG, KS, KV>;
+  using S = AttendShape<RT, PT, HG, HW, KS, KV>;
+  typedef std::conditional_t<S::kTile == 64, uint64_t, uint32_t> mask_t;
+  constexpr mask_t ALL = ~mask_t(0);
   constexpr bool WIDE = S::kWide;
   constexpr int KT = (RT + PT) / 32, DT = RT / 16, RW = S::kRows, TR = S::kTile, WR = S::WR;
   constexpr int NT = WR / 16;  // 16-position tiles a wave
@@ -395,9 +398,9 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
   const int g = lane >> 4, col = lane & 15;
   const int hgw = wv % HG, kp = wv / HG;  // the wave's heads and positions
   // runs of the same tiles for different heads sit on one XCD (blocks go round the 8)
-  const int groups = (nh + 16 * HG - 1) / (16 * HG);
+  const int groups = (nh + 16 * HW * HG - 1) / (16 * HW * HG);
   const int b8 = blockIdx.x >> 3;
-  const int run = (b8 / groups) * 8 + (blockIdx.x & 7), h0 = (b8 % groups) * (16 * HG) + hgw * 16;
+  const int run = (b8 / groups) * 8 + (blockIdx.x & 7), h0 = ((b8 % groups) * HG + hgw) * (16 * HW);
   const int n_tok = c.n_tokens;
   // the plan of up to 64 tokens from t0 on, a token a lane
   int t0 = 0;
@@ -407,7 +410,6 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
   int x = run * per;
   const int x_end = min(x + per, tiles);
   if (x >= x_end) return;
-  const int head = min(h0 + col, nh - 1);
 
   auto window = [&](int t) {
     t0 = t;
@@ -449,7 +451,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
       const uint32_t blk = uint32_t(__shfl(ids, min((p >> c.shift) - b0, 63), kWave));
       const bool ok = p < end && blk < c.n_blocks;
       at = ok ? ((int64_t(blk) << c.shift) + (p & ((1 << c.shift) - 1))) * c.width * int(sizeof(KV)) : 0;
-      return uint32_t(__ballot(ok));
+      return mask_t(__ballot(ok));
     };
     // load i of the wave's rows of that step, into buffer buf (or the raw rows)
     const uint8_t* const rows = static_cast<const uint8_t*>(c.rows);
@@ -476,7 +478,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
       }
     };
     // clears the wave's rows that are not there
-    auto clear = [&](uint32_t mask, int buf) {
+    auto clear = [&](mask_t mask, int buf) {
       for (int r = wv * RW; r < wv * RW + RW; r++)
         if (!((mask >> r) & 1)) {
           uint8_t* p = s_raw + buf * S::kBuf;
@@ -486,7 +488,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
         }
     };
     // an f32 cache: the wave's raw rows to their upper and lower parts
-    auto convert = [&](uint32_t mask) {
+    auto convert = [&](mask_t mask) {
       auto part = [&](const uint8_t* src, int row, int dst) {
         const bool on = (mask >> row) & 1;
         float v[8];
@@ -514,8 +516,8 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
     };
 
     __syncthreads();  // the buffers are free of the token before
-    constexpr int AHEAD = WIDE ? 1 : 3;  // steps whose rows are on their way before the first
-    uint32_t mask[4] = {0, 0, 0, 0};     // which rows of the present step and the next three there are
+    constexpr int AHEAD = S::kBufs - 1;  // steps whose rows are on their way before the first
+    mask_t mask[4] = {0, 0, 0, 0};     // which rows of the present step and the next three there are
 #pragma unroll
     for (int j = 0; j < AHEAD; j++)
       if (j < steps) {
@@ -525,19 +527,27 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
       }
 
     // the absorbed queries of the wave's heads
-    h8_t qh[KT], ql[TWO ? KT : 1];
+    h8_t qh[HW][KT], ql[TWO ? KT : 1];
     const int g16 = (nh + 15) / 16;
-    const _Float16* const qp = qa.parts + (int64_t(t) * g16 + min(h0 / 16, g16 - 1)) * KT * 512 + 8 * lane;
-    const float factor = qa.factor[int64_t(t) * g16 * 16 + head];
+    float factor[HW];
 #pragma unroll
-    for (int i = 0; i < KT; i++) {
-      qh[i] = *reinterpret_cast<const h8_t*>(qp + 512 * i);
-      if (TWO) ql[i] = *reinterpret_cast<const h8_t*>(qp + qa.plane + 512 * i);
+    for (int w = 0; w < HW; w++) {
+      const _Float16* const qp = qa.parts + (int64_t(t) * g16 + min(h0 / 16 + w, g16 - 1)) * KT * 512 + 8 * lane;
+      factor[w] = qa.factor[int64_t(t) * g16 * 16 + min(h0 + 16 * w + col, nh - 1)];
+#pragma unroll
+      for (int i = 0; i < KT; i++) {
+        qh[w][i] = *reinterpret_cast<const h8_t*>(qp + 512 * i);
+        if constexpr (TWO) ql[i] = *reinterpret_cast<const h8_t*>(qp + qa.plane + 512 * i);
+      }
     }
-    f4_t o[DT];
+    f4_t o[HW][DT];
+    float m[HW], l[HW];
 #pragma unroll
-    for (int i = 0; i < DT; i++) o[i] = f4_t{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
+    for (int w = 0; w < HW; w++) {
+      m[w] = -INFINITY, l[w] = 0.f;
+#pragma unroll
+      for (int i = 0; i < DT; i++) o[w][i] = f4_t{0.f, 0.f, 0.f, 0.f};
+    }
 
     // where the lane reads in a buffer, for each value of a chunk number's swapped bits; the rest is constant
     constexpr int NKL = S::kPad ? 1 : 2, NVV = S::kPad ? 1 : 4;
@@ -554,7 +564,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
     }
     f4_t sa[NT], sb[NT];  // the scores of a step, in two sums
     constexpr int QN = KT;                             // groups of products: one k step each
-    constexpr int KD = (NT == 1 ? 8 : 5) / (WIDE ? 2 : 1);  // groups whose operands are on their way
+    constexpr int KD = HW > 1 ? 2 : (NT == 1 ? 8 : 5) / (WIDE ? 2 : 1);  // groups whose operands are on their way
     h8_t ka[KD + 1][NT], kb[WIDE ? KD + 1 : 1][NT];
     auto read_k = [&](int k, const uint8_t* kv) {
 #pragma unroll
@@ -578,13 +588,13 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
         constexpr int M = KD + 1;
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-          if (!TWO && (k & 1)) b[j] = mfma(ka[k % M][j], qh[k], b[j]);  // two chains
-          else a[j] = mfma(ka[k % M][j], qh[k], a[j]);
+          if (!TWO && (k & 1)) b[j] = mfma(ka[k % M][j], qh[0][k], b[j]);  // two chains
+          else a[j] = mfma(ka[k % M][j], qh[0][k], a[j]);
         }
 #pragma unroll
         for (int j = 0; j < NT; j++) {
           if constexpr (TWO) b[j] = mfma(ka[k % M][j], ql[k], b[j]);
-          if constexpr (WIDE) b[j] = mfma(kb[k % M][j], qh[k], b[j]);
+          if constexpr (WIDE) b[j] = mfma(kb[k % M][j], qh[0][k], b[j]);
         }
         if (k % 3 == 2) __builtin_amdgcn_sched_barrier(0);  // reads stay ahead, and no further
       }
@@ -595,13 +605,13 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
     float sc[NS], mx = 0.f, ref = 0.f, alpha = 1.f, sum = 0.f;
     bool grew = false;
     _Float16 ph[NS], pl[NS];
-    auto soft = [&](int piece, uint32_t here) {
+    auto soft = [&](int piece, mask_t here) {
       if (piece < 4) {
-        const uint32_t own = here >> (kp * WR) >> (4 * g);  // bit 16 j + e: position 4g + e of tile j
+        const uint32_t own = uint32_t(here >> (kp * WR)) >> (4 * g);  // bit 16 j + e: position 4g + e of tile j
 #pragma unroll
         for (int n = piece * NS / 4; n < (piece + 1) * NS / 4; n++) {
           const int j = n / 4, e = n % 4;
-          const float s = (sa[j][e] + sb[j][e]) * factor;
+          const float s = (sa[j][e] + sb[j][e]) * factor[0];
           sc[n] = own & (1u << (16 * j + e)) ? s : -INFINITY;
           asm volatile("" : "+v"(sc[n]));
         }
@@ -614,13 +624,13 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
         mx = max_over_groups(mx);
         asm volatile("" : "+v"(mx));
       } else if (piece == 6) {
-        grew = __any(mx > m + 8.f);
-        const float mn = grew ? fmaxf(m, mx) : m;
+        grew = __any(mx > m[0] + 8.f);
+        const float mn = grew ? fmaxf(m[0], mx) : m[0];
         ref = mn == -INFINITY ? 0.f : mn;
-        alpha = __builtin_amdgcn_exp2f(m - ref);  // 0 at first: exp2(-inf)
-        m = mn;
-        l *= alpha;
-        asm volatile("" : "+v"(ref), "+v"(alpha), "+v"(m), "+v"(l));
+        alpha = __builtin_amdgcn_exp2f(m[0] - ref);  // 0 at first: exp2(-inf)
+        m[0] = mn;
+        l[0] *= alpha;
+        asm volatile("" : "+v"(ref), "+v"(alpha), "+v"(m[0]), "+v"(l[0]));
       } else if (piece < 15) {
 #pragma unroll
         for (int n = (piece - 7) * NS / 8; n < (piece - 6) * NS / 8; n++) {
@@ -633,7 +643,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
         sum = sc[0];
 #pragma unroll
         for (int n = 1; n < NS; n++) sum += sc[n];
-        l += sum;
+        l[0] += sum;
       }
     };
     // O^T += C^T p from buffer kv
@@ -641,8 +651,8 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
       if (grew) {
 #pragma unroll
         for (int d = 0; d < DT; d++) {
-          asm volatile("" : "+a"(o[d]));  // in accumulation registers up to here: else all are copied every step
-          o[d] *= alpha;
+          asm volatile("" : "+a"(o[0][d]));  // in accumulation registers up to here: else all are copied every step
+          o[0][d] *= alpha;
         }
       }
       auto tr = [&](int d, int j, int plane) {
@@ -679,22 +689,113 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
         if (grp + VD < VN) read_v(grp + VD);
         constexpr int M = VD + 1;
 #pragma unroll
-        for (int i = 0; i < VG; i++) add(o[grp * VG + i], va[grp % M][i], bh);
+        for (int i = 0; i < VG; i++) add(o[0][grp * VG + i], va[grp % M][i], bh);
         if constexpr (TWO)
 #pragma unroll
-          for (int i = 0; i < VG; i++) add(o[grp * VG + i], va[grp % M][i], bl);
+          for (int i = 0; i < VG; i++) add(o[0][grp * VG + i], va[grp % M][i], bl);
         if constexpr (WIDE)
 #pragma unroll
-          for (int i = 0; i < VG; i++) add(o[grp * VG + i], vl[grp % M][i], bh);
+          for (int i = 0; i < VG; i++) add(o[0][grp * VG + i], vl[grp % M][i], bh);
         __builtin_amdgcn_sched_barrier(0);
       }
     };
 
-    if constexpr (WIDE) {
+    if constexpr (HW > 1) {
+      // Two 16s of heads a wave, each operand read from LDS for both: products bound a step, not LDS, and the
+      // softmax stands between them (registers hold no second step's scores)
+      static_assert(!WIDE && !TWO && NT == 2);
+      for (int i = 0; i < steps; i++) {
+        if (AHEAD > 1 && i + AHEAD <= steps) dma_wait<(AHEAD - 1) * S::kLoads>();
+        else dma_wait<0>();
+        const mask_t here = mask[0];
+        if (here != ALL) clear(here, i % S::kBufs);
+        __syncthreads();  // the step's rows are there, and the step before has been read
+        if (i + AHEAD < steps) {
+          mask[AHEAD] = find(i + AHEAD);
+#pragma unroll
+          for (int n = 0; n < S::kLoads; n++) load(n, (i + AHEAD) % S::kBufs);
+        }
+        const uint8_t* const kv = s_raw + (i % S::kBufs) * S::kBuf;
+        f4_t sx[HW][NT];
+#pragma unroll
+        for (int w = 0; w < HW; w++)
+#pragma unroll
+          for (int j = 0; j < NT; j++) sx[w][j] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KD && k < QN; k++) read_k(k, kv);
+#pragma unroll
+        for (int k = 0; k < QN; k++) {
+          if (k + KD < QN) read_k(k + KD, kv);
+#pragma unroll
+          for (int w = 0; w < HW; w++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) sx[w][j] = mfma(ka[k % (KD + 1)][j], qh[w][k], sx[w][j]);
+          if (k % 2) __builtin_amdgcn_sched_barrier(0);
+        }
+        h8_t p[HW];
+        float by[HW];
+        bool grown = false;
+        const uint32_t own = uint32_t(here >> (kp * WR)) >> (4 * g);
+#pragma unroll
+        for (int w = 0; w < HW; w++) {
+          float x8[8], top = -INFINITY;
+#pragma unroll
+          for (int n = 0; n < 8; n++) {
+            x8[n] = own & (1u << (16 * (n / 4) + n % 4)) ? sx[w][n / 4][n % 4] * factor[w] : -INFINITY;
+            top = fmaxf(top, x8[n]);
+          }
+          top = max_over_groups(top);
+          const bool up = __any(top > m[w] + 8.f);
+          const float mn = up ? fmaxf(m[w], top) : m[w];
+          const float at0 = mn == -INFINITY ? 0.f : mn;
+          by[w] = __builtin_amdgcn_exp2f(m[w] - at0);
+          m[w] = mn;
+          grown |= up;
+          float add8 = 0.f;
+#pragma unroll
+          for (int n = 0; n < 8; n++) {
+            const float y = __builtin_amdgcn_exp2f(x8[n] - at0);
+            p[w][n] = _Float16(y);
+            add8 += y;
+          }
+          l[w] = l[w] * by[w] + add8;
+        }
+        if (grown) {
+#pragma unroll
+          for (int w = 0; w < HW; w++)
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+              asm volatile("" : "+a"(o[w][d]));
+              o[w][d] *= by[w];
+              asm volatile("" : "+a"(o[w][d]));
+            }
+        }
+        auto operand = [&](int d) {
+          auto tr = [&](int j) {
+            return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s4*)(kv + vv[d % NVV] + 32 * (d - d % NVV) + 16 * j * S::kPitch));
+          };
+          return __builtin_bit_cast(h8_t, __builtin_shufflevector(tr(0), tr(1), 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        constexpr int VD = 4;  // operands on their way
+        h8_t va[VD + 1];
+#pragma unroll
+        for (int d = 0; d < VD; d++) va[d] = operand(d);
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+          if (d + VD < DT) va[(d + VD) % (VD + 1)] = operand(d + VD);
+#pragma unroll
+          for (int w = 0; w < HW; w++) o[w][d] = mfma(va[d % (VD + 1)], p[w], o[w][d]);
+          if (d % 2) __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int n = 0; n < AHEAD; n++) mask[n] = mask[n + 1];
+      }
+    } else if constexpr (WIDE) {
       for (int i = 0; i < steps; i++) {
         dma_wait<0>();
         __syncthreads();  // the parts of the step before have been read
-        const uint32_t here = mask[0];
+        const mask_t here = mask[0];
         convert(here);
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the raw rows have been read
         const bool more = i + 1 < steps;
@@ -718,7 +819,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
       if (steps > 2) dma_wait<2 * S::kLoads>();
       else if (steps > 1) dma_wait<S::kLoads>();
       else dma_wait<0>();
-      if (mask[0] != 0xFFFFFFFFu) clear(mask[0], 0);
+      if (mask[0] != ALL) clear(mask[0], 0);
       __syncthreads();
       scores(s_raw, sa, sb, [](int) {});
       for (int i = 0; i < steps; i++) {
@@ -728,7 +829,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
         const bool more = i + 3 < steps;
         if (i + 2 < steps) dma_wait<S::kLoads>();
         else dma_wait<0>();
-        if (i + 1 < steps && mask[1] != 0xFFFFFFFFu) clear(mask[1], nb);
+        if (i + 1 < steps && mask[1] != ALL) clear(mask[1], nb);
         __syncthreads();  // the next step's rows are there, and the step before has been read
         if (more) {
           mask[3] = find(i + 3);
@@ -746,47 +847,52 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
         mask[0] = mask[1], mask[1] = mask[2], mask[2] = mask[3];
       }
     }
-    l = sum_over_groups(l);
+#pragma unroll
+    for (int w = 0; w < HW; w++) l[w] = sum_over_groups(l[w]);
 
     // waves of the same heads merge through LDS, over the buffers
     const int64_t slot = run + t;
     if constexpr (KS > 1) {
+      static_assert(KS == 2);
       float* const s_o = reinterpret_cast<float*>(s_raw);
       constexpr int W = RT + 4;
+      auto place = [&](int w) { return s_o + (hgw * HW + w) * 16 * W + col * W; };
       __syncthreads();
       if (kp) {
-        float* w = s_o + ((kp - 1) * HG + hgw) * 16 * W + col * W;
 #pragma unroll
-        for (int d = 0; d < DT; d++) *reinterpret_cast<f4_t*>(w + 16 * d + 4 * g) = o[d];
-        if (g == 0) w[RT] = m, w[RT + 1] = l;
+        for (int w = 0; w < HW; w++) {
+          float* to = place(w);
+#pragma unroll
+          for (int d = 0; d < DT; d++) *reinterpret_cast<f4_t*>(to + 16 * d + 4 * g) = o[w][d];
+          if (g == 0) to[RT] = m[w], to[RT + 1] = l[w];
+        }
       }
       __syncthreads();
       if (kp == 0) {
-        float mt = m;
 #pragma unroll
-        for (int k = 0; k < KS - 1; k++) mt = fmaxf(mt, s_o[(k * HG + hgw) * 16 * W + col * W + RT]);
-        const float ref = mt == -INFINITY ? 0.f : mt;
-        const float a = __builtin_amdgcn_exp2f(m - ref);
-        l *= a;
+        for (int w = 0; w < HW; w++) {
+          const float* from = place(w);
+          const float mt = fmaxf(m[w], from[RT]), top = mt == -INFINITY ? 0.f : mt;
+          const float a = __builtin_amdgcn_exp2f(m[w] - top), b = __builtin_amdgcn_exp2f(from[RT] - top);
+          l[w] = a * l[w] + b * from[RT + 1];
 #pragma unroll
-        for (int d = 0; d < DT; d++) o[d] *= a;
-#pragma unroll
-        for (int k = 0; k < KS - 1; k++) {
-          const float* w = s_o + (k * HG + hgw) * 16 * W + col * W;
-          const float b = __builtin_amdgcn_exp2f(w[RT] - ref);
-          l += b * w[RT + 1];
-#pragma unroll
-          for (int d = 0; d < DT; d++) o[d] += b * *reinterpret_cast<const f4_t*>(w + 16 * d + 4 * g);
+          for (int d = 0; d < DT; d++) {
+            o[w][d] = a * o[w][d] + b * *reinterpret_cast<const f4_t*>(from + 16 * d + 4 * g);
+            if (HW > 1) asm volatile("" : "+a"(o[w][d]));
+          }
+          m[w] = mt;
         }
-        m = mt;
       }
     }
-    if (kp == 0 && h0 + col < nh) {
+#pragma unroll
+    for (int w = 0; w < HW; w++) {
+      const int head = h0 + 16 * w + col;
+      if (kp || head >= nh) continue;
       float* po = part_o + (slot * nh + head) * c.rank;
 #pragma unroll
       for (int d = 0; d < DT; d++)
-        if (16 * d + 4 * g < c.rank) *reinterpret_cast<f4_t*>(po + 16 * d + 4 * g) = o[d];
-      if (g == 0) part_ml[slot * nh + head] = make_float2(m, l);
+        if (16 * d + 4 * g < c.rank) *reinterpret_cast<f4_t*>(po + 16 * d + 4 * g) = o[w][d];
+      if (g == 0) part_ml[slot * nh + head] = make_float2(m[w], l[w]);
     }
     x = last;
   }
@@ -1107,24 +1213,35 @@ static AbsorbedSpace absorbed_space(const jero_latent_cache* c, int64_t n_tokens
   return s;
 }
 
-template <int RT, int PT, int HG, int KS, typename KV, bool TWO>
+template <int RT, int PT, int HG, int HW, int KS, typename KV, bool TWO>
 static void launch_attend(const LatentCache& c, const MlaQueries& qa, int nh, const MlaPlan& plan, int runs, int least,
                           int extra, float* part_o, float2* part_ml, hipStream_t s) {
-  const int groups = (nh + 16 * HG - 1) / (16 * HG);
-  hipLaunchKernelGGL((mla_attend_kernel<RT, PT, HG, KS, KV, TWO>), dim3(unsigned(runs) * groups), dim3(64 * HG * KS), 0, s,
-                     c, qa, nh, plan, runs, least, extra, part_o, part_ml);
+  const int groups = (nh + 16 * HW * HG - 1) / (16 * HW * HG);
+  hipLaunchKernelGGL((mla_attend_kernel<RT, PT, HG, HW, KS, KV, TWO>), dim3(unsigned(runs) * groups), dim3(64 * HG * KS),
+                     0, s, c, qa, nh, plan, runs, least, extra, part_o, part_ml);
 }
 
 // Heads a workgroup: 16 by each of its 1, 2 or 4 waves' worth; with fewer than 4 others share the positions.
-static int attend_heads(int nh) { return nh <= 16 ? 16 : nh <= 32 ? 32 : 64; }
+// f16 activations, whose queries are one part, leave the registers for two 16s a wave from 33 heads on.
+struct AttendHeads {
+  int heads, tile;  // a workgroup's, and its positions a step
+};
+static AttendHeads attend_heads(int nh, bool one_part) {
+  if (nh <= 16) return {16, 32};
+  if (nh <= 32) return {32, 32};
+  if (!one_part) return {64, 32};
+  return nh <= 64 ? AttendHeads{64, 32} : AttendHeads{128, 32};
+}
 
 template <int RT, int PT, typename KV, bool TWO>
 static void launch_attend_heads(const LatentCache& c, const MlaQueries& qa, int nh, const MlaPlan& plan, int runs,
                                 int least, int extra, float* part_o, float2* part_ml, hipStream_t s) {
-  const int hg = attend_heads(nh);
-  if (hg == 16) launch_attend<RT, PT, 1, 2, KV, TWO>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
-  else if (hg == 32) launch_attend<RT, PT, 2, 2, KV, TWO>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
-  else launch_attend<RT, PT, 4, 1, KV, TWO>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
+  const int heads = attend_heads(nh, !TWO).heads;
+  if (heads == 16) launch_attend<RT, PT, 1, 1, 2, KV, TWO>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
+  else if (heads == 32) launch_attend<RT, PT, 2, 1, 2, KV, TWO>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
+  else if constexpr (TWO) launch_attend<RT, PT, 4, 1, 1, KV, TWO>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
+  else if (heads == 64) launch_attend<RT, PT, 4, 1, 1, KV, TWO>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
+  else launch_attend<RT, PT, 4, 2, 1, KV, TWO>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
 }
 
 template <int RT, int PT>
@@ -1173,8 +1290,8 @@ extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, i
   plan.end = plan.seq + n_tokens;
   const _Float16 *kb = static_cast<const _Float16*>(k_b_dev), *vb = static_cast<const _Float16*>(v_b_dev);
   const bool f32 = act_dtype == JERO_F32;
-  const int tile = kAttendTile;
-  const int groups = (n_heads + attend_heads(n_heads) - 1) / attend_heads(n_heads);
+  const AttendHeads ah = attend_heads(n_heads, !f32);
+  const int tile = ah.tile, groups = (n_heads + ah.heads - 1) / ah.heads;
   const int runs = groups >= kMlaRuns / 8 ? 8 : kMlaRuns / groups / 8 * 8, least = 1, extra = 3;
 
   const dim3 ga(mla_head8_blocks(n_heads, int((n_tokens + 15) / 16)) + 1);
