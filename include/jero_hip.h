@@ -321,7 +321,11 @@ int jero_hip_gqa_attention(float *out_dev, const float *q_dev, const void *k_dev
  *   - A block id outside [0, n_blocks) is never followed: its positions are not stored, and masked.
  * Two tokens of one call must not share a slot of the pool.  Sums are f32; with f32 activations the
  * products carry 22 bits of each f32 factor (two f16 parts), with f16 activations intermediate
- * queries, expanded keys and values, and softmax numerators are rounded to f16. */
+ * queries, expanded keys and values, and softmax numerators are rounded to f16.  So values of an f32
+ * cache, expanded keys and values have f16's range (to 65504, below 2^-14 to 2^-25 absolute; queries
+ * any f32 range).  A row that is not finite makes NaN of the tokens that attend to it, and of no
+ * others.
+ * At most 2^19 tokens, 2^19 sequences and, in the attentions, 1024 heads a call. */
 typedef struct jero_latent_cache {
   void *rows_dev;            /* [n_blocks][block_size][rank + rope_dim] of kv_dtype, 16-byte aligned */
   const int32_t *table_dev;  /* [n_seqs][table_stride] block ids */
@@ -361,11 +365,13 @@ int jero_hip_mla_absorbed_attention(const jero_latent_cache *cache, int act_dtyp
 /* The expanded form, for prompts and chunks of them: keys and values of every position are made
  * from the latent rows once, into the workspace, and each head attends in nope_dim + rope_dim.  As
  * the absorbed form, with kv_b_dev: [n_heads][nope_dim + v_dim][rank] f16, a head's W_uk rows before
- * its W_uv rows (nope_dim + rope_dim up to 256).  total_len: at least the sum of the lengths (each
- * up to max_len); a sequence whose rows do not fit within total_len after those before it is treated
+ * its W_uv rows (nope_dim + rope_dim up to 256).  total_len, up to 2^23: at least the sum of the
+ * lengths (each up to max_len); a sequence whose rows do not fit within total_len after those before it is treated
  * as empty.  The keys and values of as many heads as the workspace holds are made at a time: it must
  * hold one head's, jero_hip_mla_prefill_workspace_bytes(..., 1, ...), and the entry point's n_heads gives what
- * holds them all up to 1 GiB. */
+ * holds them all up to 1 GiB, and room for the partial rows that let a few long sequences be cut into
+ * runs of positions (without it they are not; the sums' order differs).  The tiles of 128 tokens times
+ * the heads are at most 2^23 (CapabilityMismatch). */
 size_t jero_hip_mla_prefill_workspace_bytes(const jero_latent_cache *cache, int act_dtype, int n_heads, int nope_dim,
                                             int v_dim, int64_t total_len);
 int jero_hip_mla_prefill_attention(const jero_latent_cache *cache, int act_dtype, const void *q_dev, int64_t q_stride,

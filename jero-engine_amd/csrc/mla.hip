@@ -12,6 +12,9 @@ namespace jero {
 // pair of the key part each.  The sum of squares is f32; the row is rounded once, to the cache's type.
 // VEC: the rows of x are 16-byte aligned, and are read so (stores always are: 8-element rows of the pool).  What
 // the row needs is on its way before the row's place is looked up.
+//
+// Bound by its bytes, for a decode step by the launch: 16638 rows of 576 f16 values take 10.0 us (3.8 TB/s; a large
+// copy 4.6), 64 rows 3.9 us; one value a lane and load took 30 us.
 template <typename X, typename KV, bool VEC>
 __global__ void __launch_bounds__(256) mla_append_kernel(LatentCache c, const X* __restrict__ x, int64_t x_stride,
                                                          const float* __restrict__ norm, float eps, MlaRope rope) {
@@ -73,9 +76,9 @@ __global__ void __launch_bounds__(256) mla_append_kernel(LatentCache c, const X*
 // ---------------------------------------------------------------- absorbed attention
 //
 // Three launches.  mla_absorb_kernel makes the absorbed queries q' = [q_n W_uk | rotated q_p] and the
-// plan; mla_attend_kernel reads every cache row once for up to 64 heads, with a running maximum and
-// sum, and leaves one partial row per (run of tiles, token, head); mla_values_kernel merges a token's
-// partials and applies W_uv.
+// plan; mla_attend_kernel reads every cache row once for up to 64 heads (128 with f16 activations), with a
+// running maximum and sum, and leaves one partial row per (run of tiles, token, head); mla_values_kernel
+// merges a token's partials and applies W_uv.
 //
 // The plan cuts the tiles of all tokens, one after the other, into equal runs, one per workgroup and
 // group of heads, so that ragged lengths fill the chip: with splits of equal length per token, 32
@@ -139,7 +142,9 @@ __device__ __forceinline__ bool mla_head8_block(int b, int nh, int per, int& h, 
 static unsigned mla_head8_blocks(int nh, int per) { return unsigned((nh + 63) / 64 * 64) * unsigned(per); }
 
 // A block per head and 16 tokens, and one more for the plan.  The 8 waves take the head's rows of W_uk^T by 16; a
-// thread rotates a pair of the key part; the row's largest value is the scale of its parts.
+// thread rotates a pair of the key part; the row's largest value is the scale of its parts.  Bound by the way of
+// one block's loads, a chain of memory latencies: 9.4 us for one token of 128 heads (16.8 MB of weights), 17 us for 64
+// (f16; the weights come from L2 for 16 tokens each).
 template <typename X, int NT>
 __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X* __restrict__ q, int64_t q_stride, int nh,
                                                          int nope, const _Float16* __restrict__ k_b, MlaRope rope,
@@ -381,6 +386,17 @@ struct AttendShape {
 // Registers allow one wave a SIMD, so a wave covers its own waits: a step's softmax runs between the products
 // of the next step's scores, operands are read from LDS a group of products ahead, and the rows two steps on are
 // on their way from the cache meanwhile (f16 cache; an f32 one has its LDS filled by the parts of one step).
+//
+// HW 2 (f16 activations, more than 64 heads): two 16s of heads a wave, 128 a workgroup, so that each operand read
+// from LDS serves two products, and cache rows go to one workgroup, not two; a step's softmax then stands between
+// its products, as registers hold no second step's scores.  64 sequences of 100 to 4100 positions and 128 heads: 73 us
+// against 84 with one 16 a wave; one of 131073 positions: 62 against 74 (and 5 us more in mla_values_kernel, as there
+// are twice the partial rows).  With 64 heads (two waves sharing positions) it took 99 us and is not used.
+//
+// Measured (512 + 64 wide): one token of 131072 positions, 128 heads, f32 activations: 92 us, 790 TFLOP/s of two-part
+// products; 32 sequences of 900 to 6000, 32 heads: 42 us, 3.0 TB/s.  Two-part products bound the first, the loads' and
+// steps' latencies with one wave a SIMD the second; with f16 activations LDS reads (one 16 a wave: 2300 cycles a step
+// of 32 positions, products 1090) and writing the partial rows (256 KB a workgroup of 128 heads, 14 us).
 template <int RT, int PT, int HG, int HW, int KS, typename KV, bool TWO>
 __global__ void __launch_bounds__(64 * HG * KS, 1)
     mla_attend_kernel(LatentCache c, MlaQueries qa, int nh, MlaPlan plan, int runs, int least, int extra,
@@ -900,7 +916,8 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
 
 // out[t][h] = W_uv[h] o[t][h], o the merged partials: a block of 8 waves per head and up to TB tokens.  The
 // weights' rows (16 of them a wave, its MFMA operand) are on their way while the partials are merged, by 8 / TB
-// waves a token (TB 16: a wave, two tokens), into LDS.
+// waves a token (TB 16: a wave, two tokens), into LDS.  Bound by the partials' bytes and, for a token, latency: one
+// token of 128 heads and 128 runs (33 MB of partials) 12 us, 64 tokens with 256 runs (84 MB) 26 us, 3.2 TB/s.
 template <typename X, int RT, int TB>
 __global__ void __launch_bounds__(512) mla_values_kernel(LatentCache c, int nh, const float* __restrict__ part_o,
                                                          const float2* __restrict__ part_ml, MlaPlan plan, int runs,
@@ -1317,14 +1334,15 @@ extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, i
     launch_attend_types<512, 64>(f32, wide, c, qa, n_heads, plan, runs, least, extra, part_o, part_ml, s);
   if ((rc = check_launch("mla attend"))) return rc;
 
-  // tokens a block: as many as leave a block for every CU, so that the weights are read seldom
+  // tokens a block: as many as leave 64 blocks or more, so that the weights are read seldom (21 tokens of 20 heads:
+  // by 1 14.1 us, by 4 10.5, by 16 16.4; 32 of 32: 26.6, 10.9, 14.3; 16 of 128: 57, 24, 20.6; 64 of 128: 187, 64, 27)
   const int64_t rows = n_tokens * n_heads;
 #define JERO_VALUES_TB(X, RT, TB)                                                                                    \
   hipLaunchKernelGGL((mla_values_kernel<X, RT, TB>), dim3(mla_head_blocks(n_heads, int((n_tokens + TB - 1) / TB))), \
                      dim3(512), 0, s, c, n_heads, part_o, part_ml, plan, runs, least, extra, vb, v_dim,             \
                      static_cast<X*>(out_dev), out_stride)
 #define JERO_VALUES(X, RT)                                                                                       \
-  if (n_tokens < 2 || rows < 512) JERO_VALUES_TB(X, RT, 1);                                                      \
+  if (n_tokens < 2 || rows < 256) JERO_VALUES_TB(X, RT, 1);                                                      \
   else if (rows < 2048) JERO_VALUES_TB(X, RT, 4);                                                                \
   else JERO_VALUES_TB(X, RT, 16)
   if (sp.rt == 128) {
