@@ -355,7 +355,8 @@ int jero_hip_mla_append(const jero_latent_cache *cache, int act_dtype, const voi
  * v_dim multiples of 8 up to 256, strides multiples of 8, all 16-byte aligned; f16 activations need
  * an f16 cache (CapabilityMismatch otherwise).  out may not overlap the inputs.  Workspace:
  * jero_hip_mla_absorbed_workspace_bytes(...) bytes, 256-byte aligned (NULL: library-owned, calls must
- * not overlap on one device). */
+ * not overlap on one device).  n_tokens * max_len at most 2^34, n_tokens * n_heads 2^25
+ * (CapabilityMismatch). */
 size_t jero_hip_mla_absorbed_workspace_bytes(const jero_latent_cache *cache, int64_t n_tokens, int n_heads);
 int jero_hip_mla_absorbed_attention(const jero_latent_cache *cache, int act_dtype, const void *q_dev, int64_t q_stride,
                                     int64_t n_tokens, int n_heads, int nope_dim, int v_dim, const void *k_b_dev,
@@ -370,8 +371,8 @@ int jero_hip_mla_absorbed_attention(const jero_latent_cache *cache, int act_dtyp
  * as empty.  The keys and values of as many heads as the workspace holds are made at a time: it must
  * hold one head's, jero_hip_mla_prefill_workspace_bytes(..., 1, ...), and the entry point's n_heads gives what
  * holds them all up to 1 GiB, and room for the partial rows that let a few long sequences be cut into
- * runs of positions (without it they are not; the sums' order differs).  The tiles of 128 tokens times
- * the heads are at most 2^23 (CapabilityMismatch). */
+ * runs of positions (without it they are not; the sums' order differs).  At most 4096 sequences
+ * (CapabilityMismatch). */
 size_t jero_hip_mla_prefill_workspace_bytes(const jero_latent_cache *cache, int act_dtype, int n_heads, int nope_dim,
                                             int v_dim, int64_t total_len);
 int jero_hip_mla_prefill_attention(const jero_latent_cache *cache, int act_dtype, const void *q_dev, int64_t q_stride,

@@ -44,21 +44,21 @@ __device__ __forceinline__ float2 mla_cos_sin(const MlaRope& rope, int i, int po
 }
 
 // The sequence and position of token row t, found by the whole wave: the sequence is the last whose
-// start is not behind t, and the starts do not decrease, so counting them is enough.  False for rows
-// of no sequence.
+// start is not behind t, and the starts do not decrease, so counting them is enough: 64 spread over those
+// left at a time.  False for rows of no sequence.
 __device__ __forceinline__ bool mla_locate(const LatentCache& c, int t, int lane, int& seq, int& pos) {
   if (!c.starts) {
     seq = t;
     pos = c.lens[t] - 1;
     return true;
   }
-  int count = 0;
-  for (int j0 = 0; j0 <= c.n_seqs; j0 += kWave) {
-    const int j = j0 + lane;
-    const bool below = j <= c.n_seqs && c.starts[min(j, c.n_seqs)] <= t;
-    const int n = __popcll(__ballot(below));
-    count += n;
-    if (n < kWave) break;
+  int count = 0, left = c.n_seqs + 1;  // starts below `count` are not behind t, those from count + left on are
+  while (left > 0) {
+    const int step = (left + kWave - 1) / kWave, j = count + lane * step + step - 1;  // a step's last
+    const int n = __popcll(__ballot(j < count + left && c.starts[min(j, c.n_seqs)] <= t));
+    const int past = n * step;
+    left = min(step - 1, left - past);
+    count += past;
   }
   seq = count - 1;
   if (seq < 0 || seq >= c.n_seqs) return false;

@@ -1287,6 +1287,9 @@ extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, i
   if (rc) return rc;
   MlaRope rope;
   if ((rc = mla_rope_of(rope_theta, cache->rope_dim, &rope))) return rc;
+  // the plan's units (32 positions, and 4 a token more at most) and the grids' work items are 32-bit
+  if (n_tokens * cache->max_len > (int64_t(1) << 34) || n_tokens * n_heads > (int64_t(1) << 25))
+    return fail(JERO_ERR_CAPABILITY_MISMATCH, "mla_absorbed_attention: more than 2^34 tokens x max_len or 2^25 tokens x heads");
   const AbsorbedSpace sp = absorbed_space(cache, n_tokens, n_heads);
   void* ws = workspace_dev;
   if ((rc = absorbed_workspace(sp.bytes, &ws, workspace_bytes, kName))) return rc;

@@ -12,7 +12,9 @@ namespace jero {
 // max_len) - 1, base the sum of the lengths before it that fit; one that would end past total has none.
 __device__ __forceinline__ int mla_len(const LatentCache& c, int s) { return min(max(c.lens[s], 0), c.max_len); }
 
-// Goes over the sequences, all lanes together: f(s, base, length) until it returns false.
+// Goes over the sequences, all lanes together: f(s, base, length) until it returns false.  Every workgroup does, so a
+// call takes no more than kPrefillSeqs of them (2^19 tokens are then 2^13 tiles at most, 2^23 of 1024 heads).
+constexpr int kPrefillSeqs = 4096;
 template <typename F>
 __device__ __forceinline__ void mla_sequences(const LatentCache& c, int64_t total, int lane, F f) {
   int64_t base = 0;
@@ -739,6 +741,8 @@ extern "C" int jero_hip_mla_prefill_attention(const jero_latent_cache* cache, in
   if (rc) return rc;
   if (nope_dim + cache->rope_dim > 256)
     return fail(JERO_ERR_CAPABILITY_MISMATCH, "mla_prefill_attention: nope_dim + rope_dim above 256");
+  if (cache->n_seqs > kPrefillSeqs)
+    return fail(JERO_ERR_CAPABILITY_MISMATCH, "mla_prefill_attention: more than " + std::to_string(kPrefillSeqs) + " sequences");
   if (total_len < 1 || total_len > (int64_t(1) << 23))
     return fail(JERO_ERR_TENSOR_BOUNDS, "mla_prefill_attention: total_len must be 1 to 2^23");
   MlaRope rope;
@@ -762,8 +766,6 @@ extern "C" int jero_hip_mla_prefill_attention(const jero_latent_cache* cache, in
   void* const parts = workspace_bytes - rows_bytes >= flash_part_bytes(shape.vt) ? static_cast<uint8_t*>(ws) + rows_bytes
                                                                                  : nullptr;
   const LatentCache c = mla_cache_of(cache, n_tokens);
-  if (int64_t(prefill_tiles(c)) * n_heads > (int64_t(1) << 23))
-    return fail(JERO_ERR_CAPABILITY_MISMATCH, "mla_prefill_attention: more than 2^23 tiles of 128 tokens over the heads");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int wide = nope_dim + v_dim;
   for (int h0 = 0; h0 < n_heads; h0 += per) {

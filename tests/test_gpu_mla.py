@@ -314,6 +314,32 @@ def test_other_scales(dev, form, scale):
     p.check(p.run(form), what=form)
 
 
+@pytest.mark.parametrize("form", FORMS)
+def test_rows_before_the_first_start(dev, form):
+    """The first sequence's rows begin at 3: those before it belong to none."""
+    p = Problem(39, [50, 0, 21], [4, 0, 2], heads=3, pad_rows=3, rest=0.25)
+    p.starts += 3
+    p.device(dev)
+    p.check(p.run(form), what=form)
+    J.mla_append(p.cache, p.d["x"], p.d["norm"], EPS, THETA)
+    check_rows(p, p.d["rows"], p.rows, *p.appended())
+
+
+# more than 64 heads, which f16 activations take two 16s a wave: each padded width, part 16s, steps on both sides
+# of the buffers' number
+@pytest.mark.parametrize("act,kv", TYPES)
+@pytest.mark.parametrize("heads,dims", [(66, {}), (81, dict(rank=72, rope=24)), (97, dict(rank=256, rope=64)),
+                                        (130, dict(rank=200, rope=40)), (113, dict(rank=504, rope=64)), (257, {})],
+                         ids=str)
+def test_many_heads(dev, heads, dims, act, kv):
+    print(f"mla absorbed {act} {kv} {heads} {dims}", flush=True)
+    p = Problem(40, [1, 31, 32, 95, 97, 130, 161, 3], [1, 1, 2, 1, 1, 3, 1, 1], heads=heads, nope=16, v=24, act=act, kv=kv,
+                pad_rows=1, **dims)
+    p.table[4, 2] = -1
+    p.device(dev)
+    p.check(p.run("absorbed"), what="many heads")
+
+
 MANY = [(70, [8] * 70, 2), (600, [1] * 600, 16), (130, [i % 7 for i in range(130)], 4)]
 
 

@@ -99,7 +99,11 @@ def test_largest_calls():
     assert prefill(cache(), total=(1 << 23) + 1) == 14
     wide = dict(tokens=1 << 19, heads=1024, qs=1024 * 48, os_=1024 * 40)
     assert prefill(cache(n_seqs=1 << 19), n=1 << 62, **wide) == 10  # 2^19 tiles of 1024 heads
-    assert absorbed(cache(n_seqs=1 << 19), **wide) == 14  # its workspace
+    assert absorbed(cache(n_seqs=1 << 19), **wide) == 10  # 2^29 rows
+    assert prefill(cache(n_seqs=4097, starts_dev=FAKE)) == 10
+    long = dict(max_len=1 << 22, table_stride=1 << 18)
+    assert absorbed(cache(n_seqs=4097, **long), tokens=4097, n=0) == 10
+    assert absorbed(cache(n_seqs=4096, **long), tokens=4096, n=0) == 14  # its workspace
 
 
 def test_workspace_sizes():
