@@ -1,6 +1,7 @@
 // mla.hip -- latent attention over a paged cache: appending rows, and the absorbed form.
 #include "mla.h"
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -90,8 +91,20 @@ constexpr int kMlaRuns = 256;  // workgroups of the attend kernel: one per CU, i
 struct MlaPlan {
   int* prefix;  // [T + 1] tiles before each token
   int* seq;     // [T] sequence, -1 for a row of none
-  int* end;     // [T] positions attended to
+  int* end;     // [T] positions attended to, an item's by its last token
+  int* item;    // [T] the item's first token
 };
+
+// An item: up to `share` tokens of a sequence, one after the other, whose heads attend to its rows together, token
+// after token (so that drafted tokens read them once; 1: each token by itself).  Its units are its first token's.
+// Number of an item, no two alike and growing: along a sequence first / share grows, from one to the next seq does.
+__device__ __forceinline__ int mla_item(int share, int seq, int first) { return share > 1 ? seq + first / share : first; }
+__device__ __forceinline__ int mla_item_first(const LatentCache& c, int share, int seq, int t) {
+  return share > 1 ? t - (t - max(c.starts[seq], 0)) % share : t;
+}
+__device__ __forceinline__ int mla_item_tokens(const LatentCache& c, int share, int seq, int first) {
+  return share > 1 ? min(share, min(c.starts[seq + 1], c.n_tokens) - first) : 1;
+}
 
 // Sequence and position of token t by one thread (mla_locate is a wave's).
 __device__ __forceinline__ bool mla_locate_thread(const LatentCache& c, int t, int& seq, int& pos) {
@@ -148,7 +161,8 @@ static unsigned mla_head8_blocks(int nh, int per) { return unsigned((nh + 63) / 
 template <typename X, int NT>
 __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X* __restrict__ q, int64_t q_stride, int nh,
                                                          int nope, const _Float16* __restrict__ k_b, MlaRope rope,
-                                                         float scale, MlaQueries qa, MlaPlan plan, int tile, int extra) {
+                                                         float scale, MlaQueries qa, MlaPlan plan, int tile, int extra,
+                                                         int share) {
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   if (blockIdx.x + 1 < gridDim.x) {
     int h, t0;
@@ -157,7 +171,7 @@ __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X*
     constexpr int NR = kMlaMaxRank / 128;  // 16s of rows a wave
     __shared__ float s_max[8][16];
     __shared__ uint32_t s_key[16];
-    __shared__ int s_ex[16];
+    __shared__ int s_ex[16], s_first[16];
     const int g = lane >> 4, col = lane & 15;
     // everything the wave reads is on its way before anything is waited for
     const X* qr = q + min(t0 + col, c.n_tokens - 1) * q_stride + int64_t(h) * (nope + c.rope);
@@ -177,7 +191,13 @@ __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X*
     const int key_t = min(t0 + min(kt_, 15), c.n_tokens - 1);
     const X* kp = q + key_t * q_stride + int64_t(h) * (nope + c.rope) + nope + 2 * ki;
     const float kx = float(kp[0]), ky = float(kp[1]);
-    if (tid < 16) s_key[tid] = 0;
+    if (tid < 16) {
+      s_key[tid] = 0;
+      int first = t0 + tid, seq, pos;
+      if (share > 1 && first < c.n_tokens && mla_locate_thread(c, first, seq, pos))
+        first = mla_item_first(c, share, seq, first);
+      s_first[tid] = first;
+    }
     float ka = kx, kb = ky;
     if (rope.on) {
       int seq, pos;
@@ -247,7 +267,7 @@ __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X*
       const int ex = x > 0.f && x < INFINITY ? ilogbf(x) : 0;
       s_ex[tid] = ex;
       if (t0 + tid < c.n_tokens)
-        qa.factor[int64_t(t0 + tid) * groups * 16 + h] = ldexpf(scale * 1.44269504088896341f, ex);
+        qa.factor[int64_t(s_first[tid]) * groups * 16 + (t0 + tid - s_first[tid]) * nh + h] = ldexpf(scale * 1.44269504088896341f, ex);
     }
     __syncthreads();
     // the parts by token and column in LDS, from there 16 bytes at a time
@@ -280,7 +300,8 @@ __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X*
     for (int i = tid; i < 16 * (cols / 8); i += 512) {
       const int t = i / (cols / 8), k = i % (cols / 8);  // 8 columns
       if (t0 + t >= c.n_tokens) break;
-      _Float16* p = qa.parts + ((int64_t(t0 + t) * groups + h / 16) * qa.kt + k / 4) * 512 + (k % 4) * 128 + (h % 16) * 8;
+      const int first = s_first[t], row = (t0 + t - first) * nh + h;
+      _Float16* p = qa.parts + ((int64_t(first) * groups + row / 16) * qa.kt + k / 4) * 512 + (k % 4) * 128 + (row % 16) * 8;
       *reinterpret_cast<h8_t*>(p) = *reinterpret_cast<const h8_t*>(&s_part[0][t][8 * k]);
       if (TWO) *reinterpret_cast<h8_t*>(p + qa.plane) = *reinterpret_cast<const h8_t*>(&s_part[TWO][t][8 * k]);
     }
@@ -292,12 +313,16 @@ __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X*
   int base = 0;
   for (int first = 0; first < c.n_tokens; first += 512) {
     const int t = first + tid;
-    int seq = -1, pos = -1, end = 0;
+    int seq = -1, pos = -1, end = 0, item = t;
     if (t < c.n_tokens) {
-      if (!mla_locate_thread(c, t, seq, pos)) seq = -1, pos = -1;
-      end = pos < 0 ? 0 : int(min(int64_t(pos) + 1, int64_t(c.max_len)));
+      if (mla_locate_thread(c, t, seq, pos)) {
+        item = mla_item_first(c, share, seq, t);
+        end = int(max(int64_t(0), min(int64_t(pos) + mla_item_tokens(c, share, seq, t), int64_t(c.max_len))));
+      } else {
+        seq = -1;
+      }
     }
-    const int mine = end > 0 ? (end + tile - 1) / tile + extra : 0;
+    const int mine = end > 0 && item == t ? (end + tile - 1) / tile + extra : 0;
     int sum = mine;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -315,6 +340,7 @@ __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X*
       plan.prefix[t] = before + sum - mine;
       plan.seq[t] = seq;
       plan.end[t] = end;
+      plan.item[t] = item;
     }
     __syncthreads();
   }
@@ -399,7 +425,7 @@ struct AttendShape {
 // of 32 positions, products 1090) and writing the partial rows (256 KB a workgroup of 128 heads, 14 us).
 template <int RT, int PT, int HG, int HW, int KS, typename KV, bool TWO>
 __global__ void __launch_bounds__(64 * HG * KS, 1)
-    mla_attend_kernel(LatentCache c, MlaQueries qa, int nh, MlaPlan plan, int runs, int least, int extra,
+    mla_attend_kernel(LatentCache c, MlaQueries qa, int nh, int share, MlaPlan plan, int runs, int least, int extra,
                       float* __restrict__ part_o, float2* __restrict__ part_ml) {
   using S = AttendShape<RT, PT, HG, HW, KS, KV>;
   typedef std::conditional_t<S::kTile == 64, uint64_t, uint32_t> mask_t;
@@ -414,7 +440,8 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
   const int g = lane >> 4, col = lane & 15;
   const int hgw = wv % HG, kp = wv / HG;  // the wave's heads and positions
   // runs of the same tiles for different heads sit on one XCD (blocks go round the 8)
-  const int groups = (nh + 16 * HW * HG - 1) / (16 * HW * HG);
+  const int rows_all = share * nh;  // of an item: its tokens' heads
+  const int groups = (rows_all + 16 * HW * HG - 1) / (16 * HW * HG);
   const int b8 = blockIdx.x >> 3;
   const int run = (b8 / groups) * 8 + (blockIdx.x & 7), h0 = ((b8 % groups) * HG + hgw) * (16 * HW);
   const int n_tok = c.n_tokens;
@@ -449,6 +476,19 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
     const int seq = __builtin_amdgcn_readlane(w_seq, t - t0), end = __builtin_amdgcn_readlane(w_end, t - t0);
     const int32_t* table = c.table + seq * c.table_stride;
     const int p0 = (x - first) * TR, steps = last - x;
+    const int rows_in = nh * mla_item_tokens(c, share, seq, t);
+    int lim = end, top = end;  // positions that the lane's token attends to, and the item's first
+    if (HW == 1 && share > 1) {
+      const int64_t n = int64_t(c.lens[seq]) - c.starts[seq + 1] + t + 1;
+      top = int(min(max(n, int64_t(0)), int64_t(end)));
+      lim = int(min(max(n + min(h0 + col, rows_in - 1) / nh, int64_t(0)), int64_t(end)));
+    }
+    // of a step's rows that are there, those that the lane's token attends to
+    auto seen = [&](mask_t here, int i) {
+      if (HW > 1 || share == 1) return here;
+      const int n = lim - (p0 + i * TR);
+      return n >= TR ? here : n > 0 ? here & ((mask_t(1) << n) - 1) : mask_t(0);
+    };
 
     // block ids of 64 blocks from block b0 on, a block a lane
     const int blocks = (end - 1) >> c.shift;  // the token's last
@@ -503,6 +543,27 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
           if (lane < PT / 8) *reinterpret_cast<u32x4*>(p + S::key(r, lane)) = z;
         }
     };
+    // Rows that some of the item's tokens do not attend to: where the latent is not finite it is made zeros, as
+    // those would take 0 * NaN from it, and the key part NaN for the others.
+    auto scrub = [&](mask_t mask, int i, int buf) {
+      if (HW > 1 || share == 1 || p0 + i * TR + TR <= top) return;
+      for (int r = wv * RW; r < wv * RW + RW; r++) {
+        if (!((mask >> r) & 1) || p0 + i * TR + r < top) continue;
+        uint8_t* p = s_raw + buf * S::kBuf;
+        bool odd = false;
+        if (lane < RT / 8) {
+          const u32x4 v = *reinterpret_cast<const u32x4*>(p + S::lat(r, lane));
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            odd |= (v[e] & 0x7C00u) == 0x7C00u || (v[e] & 0x7C000000u) == 0x7C000000u;
+        }
+        if (!__any(odd)) continue;
+        const u32x4 z = {0u, 0u, 0u, 0u}, nan = {0x7E007E00u, 0x7E007E00u, 0x7E007E00u, 0x7E007E00u};
+        if (lane < RT / 8) *reinterpret_cast<u32x4*>(p + S::lat(r, lane)) = z;
+        if (WIDE && lane < RT / 8) *reinterpret_cast<u32x4*>(p + S::kBuf + S::lat(r, lane)) = z;
+        if (lane < PT / 8) *reinterpret_cast<u32x4*>(p + S::key(r, lane)) = nan;
+      }
+    };
     // an f32 cache: the wave's raw rows to their upper and lower parts
     auto convert = [&](mask_t mask) {
       auto part = [&](const uint8_t* src, int row, int dst) {
@@ -548,8 +609,9 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
     float factor[HW];
 #pragma unroll
     for (int w = 0; w < HW; w++) {
-      const _Float16* const qp = qa.parts + (int64_t(t) * g16 + min(h0 / 16 + w, g16 - 1)) * KT * 512 + 8 * lane;
-      factor[w] = qa.factor[int64_t(t) * g16 * 16 + min(h0 + 16 * w + col, nh - 1)];
+      const _Float16* const qp =
+          qa.parts + (int64_t(t) * g16 + min(h0 / 16 + w, (rows_in + 15) / 16 - 1)) * KT * 512 + 8 * lane;
+      factor[w] = qa.factor[int64_t(t) * g16 * 16 + min(h0 + 16 * w + col, rows_in - 1)];
 #pragma unroll
       for (int i = 0; i < KT; i++) {
         qh[w][i] = *reinterpret_cast<const h8_t*>(qp + 512 * i);
@@ -813,6 +875,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
         __syncthreads();  // the parts of the step before have been read
         const mask_t here = mask[0];
         convert(here);
+        scrub(here, i, 0);
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the raw rows have been read
         const bool more = i + 1 < steps;
         if (more) {
@@ -827,7 +890,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
             for (int n = grp * S::kLoadsLat / QN; n < (grp + 1) * S::kLoadsLat / QN; n++) load(S::kLoadsKey + n, 0);
         });
 #pragma unroll
-        for (int n = 0; n < PIECES; n++) soft(n, here);
+        for (int n = 0; n < PIECES; n++) soft(n, seen(here, i));
         values(s_raw);
       }
     } else {
@@ -836,6 +899,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
       else if (steps > 1) dma_wait<S::kLoads>();
       else dma_wait<0>();
       if (mask[0] != ALL) clear(mask[0], 0);
+      scrub(mask[0], 0, 0);
       __syncthreads();
       scores(s_raw, sa, sb, [](int) {});
       for (int i = 0; i < steps; i++) {
@@ -846,16 +910,18 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
         if (i + 2 < steps) dma_wait<S::kLoads>();
         else dma_wait<0>();
         if (i + 1 < steps && mask[1] != ALL) clear(mask[1], nb);
+        if (i + 1 < steps) scrub(mask[1], i + 1, nb);
         __syncthreads();  // the next step's rows are there, and the step before has been read
         if (more) {
           mask[3] = find(i + 3);
 #pragma unroll
           for (int n = 0; n < S::kLoads; n++) load(n, fb);
         }
+        const mask_t here = seen(mask[0], i);
         f4_t na[NT], nb2[NT];
         scores(s_raw + nb * S::kBuf, na, nb2, [&](int grp) {
 #pragma unroll
-          for (int n = grp * PIECES / QN; n < (grp + 1) * PIECES / QN; n++) soft(n, mask[0]);
+          for (int n = grp * PIECES / QN; n < (grp + 1) * PIECES / QN; n++) soft(n, here);
         });
         values(s_raw + (i & 3) * S::kBuf);
 #pragma unroll
@@ -867,7 +933,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
     for (int w = 0; w < HW; w++) l[w] = sum_over_groups(l[w]);
 
     // waves of the same heads merge through LDS, over the buffers
-    const int64_t slot = run + t;
+    const int64_t slot = run + mla_item(share, seq, t);
     if constexpr (KS > 1) {
       static_assert(KS == 2);
       float* const s_o = reinterpret_cast<float*>(s_raw);
@@ -903,12 +969,12 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
 #pragma unroll
     for (int w = 0; w < HW; w++) {
       const int head = h0 + 16 * w + col;
-      if (kp || head >= nh) continue;
-      float* po = part_o + (slot * nh + head) * c.rank;
+      if (kp || head >= rows_in) continue;
+      float* po = part_o + (slot * rows_all + head) * c.rank;
 #pragma unroll
       for (int d = 0; d < DT; d++)
         if (16 * d + 4 * g < c.rank) *reinterpret_cast<f4_t*>(po + 16 * d + 4 * g) = o[w][d];
-      if (g == 0) part_ml[slot * nh + head] = make_float2(m[w], l[w]);
+      if (g == 0) part_ml[slot * rows_all + head] = make_float2(m[w], l[w]);
     }
     x = last;
   }
@@ -921,8 +987,8 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
 template <typename X, int RT, int TB>
 __global__ void __launch_bounds__(512) mla_values_kernel(LatentCache c, int nh, const float* __restrict__ part_o,
                                                          const float2* __restrict__ part_ml, MlaPlan plan, int runs,
-                                                         int least, int extra, const _Float16* __restrict__ v_b,
-                                                         int v_dim, X* __restrict__ out, int64_t out_stride) {
+                                                         int least, int extra, int share,
+                                                         const _Float16* __restrict__ v_b, int v_dim, X* __restrict__ out, int64_t out_stride) {
   constexpr int KT = RT / 32, P = RT + 8, NW = 8, U = 4, WPT = TB < 8 ? 8 / TB : 1;
   __shared__ __attribute__((aligned(16))) _Float16 s_hi[16][P], s_lo[16][P];
   __shared__ __attribute__((aligned(16))) float s_acc[WPT > 1 ? NW : 1][RT];
@@ -943,9 +1009,10 @@ __global__ void __launch_bounds__(512) mla_values_kernel(LatentCache c, int nh, 
   const int per = mla_per_run(plan.prefix[c.n_tokens], runs, least);
   const int r0 = min(8 * lane, c.rank - 8);
 
-  // partials w0, w0 + by, ... below w1 of token t, of which lane l holds elements 8l ..: sum, maximum, total
+  // partials w0, w0 + by, ... below w1 of row `row` of item `item`, of which lane l holds elements 8l ..: sum,
+  // maximum, total
   float acc[8], m, l;
-  auto merge = [&](int t, int w0, int w1, int by) {
+  auto merge = [&](int item, int row, int w0, int w1, int by) {
 #pragma unroll
     for (int e = 0; e < 8; e++) acc[e] = 0.f;
     m = -INFINITY, l = 0.f;
@@ -954,7 +1021,7 @@ __global__ void __launch_bounds__(512) mla_values_kernel(LatentCache c, int nh, 
       float2 ml[U];
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const int64_t at = int64_t(min(w + u * by, w1 - 1) + t) * nh + h;
+        const int64_t at = int64_t(min(w + u * by, w1 - 1) + item) * (share * nh) + row;
         const float* p = part_o + at * c.rank + r0;
         lo[u] = *reinterpret_cast<const float4*>(p);
         hi[u] = *reinterpret_cast<const float4*>(p + 4);
@@ -997,13 +1064,14 @@ __global__ void __launch_bounds__(512) mla_values_kernel(LatentCache c, int nh, 
 #pragma unroll
   for (int i = wv / WPT; i < TB; i += NW / WPT) {
     const int t = t0 + i;
-    int w0 = 0, w1 = 0;
+    int w0 = 0, w1 = 0, first = t, item = t;
     if (t < c.n_tokens) {
-      const int a = plan.prefix[t] + extra, e = plan.prefix[t + 1];
+      if (share > 1) first = plan.item[t], item = mla_item(share, plan.seq[t], first);
+      const int a = plan.prefix[first] + extra, e = plan.prefix[first + 1];
       w0 = a / per;
       w1 = e > a ? (e - 1) / per + 1 : w0;
     }
-    merge(t, w0 + wv % WPT, w1, WPT);
+    merge(item, (t - first) * nh + h, w0 + wv % WPT, w1, WPT);
     if constexpr (WPT == 1) keep(i, l);
   }
   if constexpr (WPT > 1) {
@@ -1215,9 +1283,20 @@ struct AbsorbedSpace {
   int rt, pt;  // padded widths: the smallest that the attend kernel is built for
 };
 
+// Tokens an item: as many as sequences have on average, and 64 rows of heads hold.  Only n_tokens and n_seqs are
+// known here: where most sequences have one token, each is by itself.  Measured, attend and value product, tokens by
+// themselves and together: 7 sequences x 2-4 tokens, 20 heads, 40-2500 positions of f32 31 + 10 and 24 + 12 us; 16
+// sequences of 2000-6000, 32 heads 126 + 17 and 88 + 20; 16 heads, f16 53 + 10 and 37 + 12.
+static int absorbed_share(const jero_latent_cache* c, int64_t n_tokens, int n_heads) {
+  if (!c->starts_dev || n_tokens <= c->n_seqs || n_heads > 32) return 1;
+  return int(std::min<int64_t>(64 / n_heads, (n_tokens + c->n_seqs - 1) / c->n_seqs));
+}
+
 static AbsorbedSpace absorbed_space(const jero_latent_cache* c, int64_t n_tokens, int n_heads) {
   auto up = [](size_t n) { return (n + 255) & ~size_t(255); };
-  const size_t parts = (size_t(n_tokens) + kMlaRuns) * n_heads;
+  const int share = absorbed_share(c, n_tokens, n_heads);
+  const size_t items = size_t(share > 1 ? n_tokens / share + c->n_seqs : n_tokens);
+  const size_t parts = (items + kMlaRuns) * share * n_heads;
   const size_t rows16 = size_t(n_tokens) * ((n_heads + 15) / 16 * 16);
   AbsorbedSpace s;
   s.rt = c->rank <= 128 && c->rope_dim <= 32 ? 128 : c->rank <= 256 ? 256 : 512;
@@ -1226,16 +1305,16 @@ static AbsorbedSpace absorbed_space(const jero_latent_cache* c, int64_t n_tokens
   s.part_o = s.factor + up(rows16 * 4);
   s.part_ml = s.part_o + up(parts * c->rank * 4);
   s.plan = s.part_ml + up(parts * 8);
-  s.bytes = s.plan + up((3 * size_t(n_tokens) + 1) * 4);
+  s.bytes = s.plan + up((4 * size_t(n_tokens) + 1) * 4);
   return s;
 }
 
 template <int RT, int PT, int HG, int HW, int KS, typename KV, bool TWO>
-static void launch_attend(const LatentCache& c, const MlaQueries& qa, int nh, const MlaPlan& plan, int runs, int least,
+static void launch_attend(const LatentCache& c, const MlaQueries& qa, int nh, int share, const MlaPlan& plan, int runs, int least,
                           int extra, float* part_o, float2* part_ml, hipStream_t s) {
-  const int groups = (nh + 16 * HW * HG - 1) / (16 * HW * HG);
+  const int groups = (share * nh + 16 * HW * HG - 1) / (16 * HW * HG);
   hipLaunchKernelGGL((mla_attend_kernel<RT, PT, HG, HW, KS, KV, TWO>), dim3(unsigned(runs) * groups), dim3(64 * HG * KS),
-                     0, s, c, qa, nh, plan, runs, least, extra, part_o, part_ml);
+                     0, s, c, qa, nh, share, plan, runs, least, extra, part_o, part_ml);
 }
 
 // Heads a workgroup: 16 by each of its 1, 2 or 4 waves' worth; with fewer than 4 others share the positions.
@@ -1251,28 +1330,28 @@ static AttendHeads attend_heads(int nh, bool one_part) {
 }
 
 template <int RT, int PT, typename KV, bool TWO>
-static void launch_attend_heads(const LatentCache& c, const MlaQueries& qa, int nh, const MlaPlan& plan, int runs,
+static void launch_attend_heads(const LatentCache& c, const MlaQueries& qa, int nh, int share, const MlaPlan& plan, int runs,
                                 int least, int extra, float* part_o, float2* part_ml, hipStream_t s) {
-  const int heads = attend_heads(nh, !TWO).heads;
-  if (heads == 16) launch_attend<RT, PT, 1, 1, 2, KV, TWO>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
-  else if (heads == 32) launch_attend<RT, PT, 2, 1, 2, KV, TWO>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
-  else if constexpr (TWO) launch_attend<RT, PT, 4, 1, 1, KV, TWO>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
-  else if (heads == 64) launch_attend<RT, PT, 4, 1, 1, KV, TWO>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
-  else launch_attend<RT, PT, 4, 2, 1, KV, TWO>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
+  const int heads = attend_heads(share * nh, !TWO).heads;
+  if (heads == 16) launch_attend<RT, PT, 1, 1, 2, KV, TWO>(c, qa, nh, share, plan, runs, least, extra, part_o, part_ml, s);
+  else if (heads == 32) launch_attend<RT, PT, 2, 1, 2, KV, TWO>(c, qa, nh, share, plan, runs, least, extra, part_o, part_ml, s);
+  else if constexpr (TWO) launch_attend<RT, PT, 4, 1, 1, KV, TWO>(c, qa, nh, share, plan, runs, least, extra, part_o, part_ml, s);
+  else if (heads == 64) launch_attend<RT, PT, 4, 1, 1, KV, TWO>(c, qa, nh, share, plan, runs, least, extra, part_o, part_ml, s);
+  else launch_attend<RT, PT, 4, 2, 1, KV, TWO>(c, qa, nh, share, plan, runs, least, extra, part_o, part_ml, s);
 }
 
 template <int RT, int PT>
 static void launch_attend_types(bool f32_act, bool f32_kv, const LatentCache& c, const MlaQueries& qa, int nh,
-                                const MlaPlan& plan, int runs, int least, int extra, float* part_o, float2* part_ml, hipStream_t s) {
-  if (f32_kv) launch_attend_heads<RT, PT, float, true>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
-  else if (f32_act) launch_attend_heads<RT, PT, _Float16, true>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
-  else launch_attend_heads<RT, PT, _Float16, false>(c, qa, nh, plan, runs, least, extra, part_o, part_ml, s);
+                                int share, const MlaPlan& plan, int runs, int least, int extra, float* part_o, float2* part_ml, hipStream_t s) {
+  if (f32_kv) launch_attend_heads<RT, PT, float, true>(c, qa, nh, share, plan, runs, least, extra, part_o, part_ml, s);
+  else if (f32_act) launch_attend_heads<RT, PT, _Float16, true>(c, qa, nh, share, plan, runs, least, extra, part_o, part_ml, s);
+  else launch_attend_heads<RT, PT, _Float16, false>(c, qa, nh, share, plan, runs, least, extra, part_o, part_ml, s);
 }
 
 }  // namespace jero
 
 extern "C" size_t jero_hip_mla_absorbed_workspace_bytes(const jero_latent_cache* cache, int64_t n_tokens, int n_heads) {
-  if (!cache || n_tokens < 1 || n_heads < 1 || cache->rank < 1 || cache->rope_dim < 1) return 0;
+  if (!cache || n_tokens < 1 || n_heads < 1 || cache->rank < 1 || cache->rope_dim < 1 || cache->n_seqs < 1) return 0;
   return absorbed_space(cache, n_tokens, n_heads).bytes;
 }
 
@@ -1308,16 +1387,18 @@ extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, i
   plan.prefix = reinterpret_cast<int*>(w + sp.plan);
   plan.seq = plan.prefix + n_tokens + 1;
   plan.end = plan.seq + n_tokens;
+  plan.item = plan.end + n_tokens;
   const _Float16 *kb = static_cast<const _Float16*>(k_b_dev), *vb = static_cast<const _Float16*>(v_b_dev);
   const bool f32 = act_dtype == JERO_F32;
-  const AttendHeads ah = attend_heads(n_heads, !f32);
-  const int tile = ah.tile, groups = (n_heads + ah.heads - 1) / ah.heads;
+  const int share = absorbed_share(cache, n_tokens, n_heads);
+  const AttendHeads ah = attend_heads(share * n_heads, !f32);
+  const int tile = ah.tile, groups = (share * n_heads + ah.heads - 1) / ah.heads;
   const int runs = groups >= kMlaRuns / 8 ? 8 : kMlaRuns / groups / 8 * 8, least = 1, extra = 3;
 
   const dim3 ga(mla_head8_blocks(n_heads, int((n_tokens + 15) / 16)) + 1);
 #define JERO_ABSORB(X, NT)                                                                                         \
   hipLaunchKernelGGL((mla_absorb_kernel<X, NT>), ga, dim3(512), 0, s, c, static_cast<const X*>(q_dev), q_stride, n_heads, \
-                     nope_dim, kb, rope, scale, qa, plan, tile, extra)
+                     nope_dim, kb, rope, scale, qa, plan, tile, extra, share)
   if (nope_dim <= 128) {
     if (f32) JERO_ABSORB(float, 4);
     else JERO_ABSORB(_Float16, 4);
@@ -1330,11 +1411,11 @@ extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, i
 
   const bool wide = cache->kv_dtype == JERO_KV_F32;
   if (sp.rt == 128)
-    launch_attend_types<128, 32>(f32, wide, c, qa, n_heads, plan, runs, least, extra, part_o, part_ml, s);
+    launch_attend_types<128, 32>(f32, wide, c, qa, n_heads, share, plan, runs, least, extra, part_o, part_ml, s);
   else if (sp.rt == 256)
-    launch_attend_types<256, 64>(f32, wide, c, qa, n_heads, plan, runs, least, extra, part_o, part_ml, s);
+    launch_attend_types<256, 64>(f32, wide, c, qa, n_heads, share, plan, runs, least, extra, part_o, part_ml, s);
   else
-    launch_attend_types<512, 64>(f32, wide, c, qa, n_heads, plan, runs, least, extra, part_o, part_ml, s);
+    launch_attend_types<512, 64>(f32, wide, c, qa, n_heads, share, plan, runs, least, extra, part_o, part_ml, s);
   if ((rc = check_launch("mla attend"))) return rc;
 
   // tokens a block: as many as leave 64 blocks or more, so that the weights are read seldom (21 tokens of 20 heads:
@@ -1342,7 +1423,7 @@ extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, i
   const int64_t rows = n_tokens * n_heads;
 #define JERO_VALUES_TB(X, RT, TB)                                                                                    \
   hipLaunchKernelGGL((mla_values_kernel<X, RT, TB>), dim3(mla_head_blocks(n_heads, int((n_tokens + TB - 1) / TB))), \
-                     dim3(512), 0, s, c, n_heads, part_o, part_ml, plan, runs, least, extra, vb, v_dim,             \
+                     dim3(512), 0, s, c, n_heads, part_o, part_ml, plan, runs, least, extra, share, vb, v_dim,             \
                      static_cast<X*>(out_dev), out_stride)
 #define JERO_VALUES(X, RT)                                                                                       \
   if (n_tokens < 2 || rows < 256) JERO_VALUES_TB(X, RT, 1);                                                      \

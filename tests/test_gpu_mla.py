@@ -340,6 +340,33 @@ def test_many_heads(dev, heads, dims, act, kv):
     p.check(p.run("absorbed"), what="many heads")
 
 
+# tokens of a sequence that read its rows together: few heads, sequences of more and of fewer tokens than an item,
+# ends within a step, at its edges and past max_len, tokens below position 0, and rows that are not finite
+SHARED = [(20, [3, 3, 3, 3], [32, 33, 34, 65], None), (8, [9, 1, 17, 0, 2], [40, 1, 100, 7, 64], None),
+          (1, [70, 3, 5], [129, 40, 4], None), (32, [2, 2, 3], [31, 96, 200], 128), (13, [4, 4], [3, 5], None),
+          (16, [1, 1, 1, 12], [50, 20, 70, 161], 150)]
+
+
+@pytest.mark.parametrize("act,kv", TYPES)
+@pytest.mark.parametrize("dims", [{}, dict(rank=200, rope=40), dict(rank=512, rope=64)], ids=["128", "256", "512"])
+@pytest.mark.parametrize("heads,new,lens,max_len", SHARED, ids=lambda x: str(x))
+def test_tokens_that_share_rows(dev, heads, new, lens, max_len, dims, act, kv):
+    print(f"mla absorbed {act} {kv} {heads} {new} {dims}", flush=True)
+    p = Problem(41, lens, new, heads=heads, nope=16, v=24, act=act, kv=kv, max_len=max_len, block=8, pad_rows=1, **dims)
+    p.table[0, 1 if lens[0] > 8 else 0] = -1 if max_len is None else p.table[0, 0]
+    p.device(dev)
+    ref = p.attention()
+    p.check(p.run("absorbed"), ref, "shared")
+    # the last token's own row of NaN: no other sees it
+    s = int(np.argmax(p.new))
+    t, pos = int(p.starts[s + 1]) - 1, p.lens[s] - 1
+    if pos < p.max_len and p.table[s, pos // 8] >= 0:  # (a row of no block is not attended to)
+        p.d["rows"][int(p.table[s, pos // 8]), pos % 8, 0] = float("nan")
+        out = p.run("absorbed").float().cpu().numpy().astype(np.float64)
+        rest = [i for i, _, _ in p.tokens() if i != t]
+        assert np.isnan(out[t]).all() and off(out[rest], ref[0][rest], ref[1][rest])[0] <= 1
+
+
 MANY = [(70, [8] * 70, 2), (600, [1] * 600, 16), (130, [i % 7 for i in range(130)], 4)]
 
 
