@@ -258,6 +258,35 @@ def test_a_captured_call_follows_lengths_and_tables(dev, form):
         assert torch.equal(eager, out)
 
 
+def test_two_graphs_by_turns(dev):
+    """Both forms captured, each with the workspace it made for itself, replayed by turns with eager calls in
+    between."""
+    p = Problem(42, [700, 90, 33], [3, 1, 2], heads=6, rank=128, rope=32, nope=64, v=64, pad_rows=1).device(dev)
+    ref = p.attention()
+    outs, graphs = [], []
+    side = torch.cuda.Stream(dev)
+    for form in FORMS:
+        out = torch.full((p.T, p.H, p.V), 7.0, device=dev)
+        with torch.cuda.stream(side):
+            p.run(form, out=out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            p.run(form, out=out)
+        outs.append(out)
+        graphs.append(graph)
+    for turn in range(4):
+        for out in outs:
+            out[:-1].zero_()
+        for graph in graphs if turn % 2 else graphs[::-1]:
+            graph.replay()
+        eager = [p.run(form) for form in FORMS]
+        torch.cuda.synchronize()
+        for form, out, e in zip(FORMS, outs, eager):
+            p.check(out, ref, f"{form} turn {turn}")
+            assert torch.equal(out, e)
+
+
 @pytest.mark.parametrize("form", FORMS)
 def test_two_streams_at_once(dev, form):
     """Two calls that overlap, each with a workspace of its own."""
