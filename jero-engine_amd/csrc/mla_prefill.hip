@@ -50,16 +50,16 @@ struct Expanded {
 template <typename KV>
 struct ExpandShape {
   static constexpr bool kWide = sizeof(KV) == 4;
-  static constexpr int kPos = kWide ? 64 : 128, kPlanes = kWide ? 2 : 1;
+  static constexpr int kPos = kWide ? 64 : 128, kShort = 32, kPlanes = kWide ? 2 : 1;
   static constexpr int kPitch = kMlaMaxRank + 8;  // 16 rows fall on all banks
-  static constexpr int kStep = 512;               // weight rows of the 8 waves
 };
-template <int NT, int PT, int VT, typename KV, bool TWO>
-__global__ void __launch_bounds__(512) mla_expand_kernel(LatentCache c, int nh, int nope, int v_dim,
+template <int NT, int PT, int VT, typename KV, bool TWO, int MP, int NW>
+__global__ void __launch_bounds__(64 * NW) mla_expand_kernel(LatentCache c, int nh, int nope, int v_dim,
                                                          const _Float16* __restrict__ w, Expanded x, int run) {
   using S = ExpandShape<KV>;
   constexpr bool WIDE = S::kWide;
-  constexpr int WP = NT + VT, MP = S::kPos, CP = S::kPlanes, P = S::kPitch, MJ = MP / 16;
+  constexpr int WP = NT + VT, CP = S::kPlanes, P = S::kPitch, MJ = MP / 16, JB = MJ < 4 ? MJ : 4;
+  constexpr int STEP = 64 * NW;  // threads, and weight rows of the waves
   __shared__ __attribute__((aligned(16))) _Float16 s_c[CP][MP][P];
   // the positions' cache rows: -1 for a block that is none, -2 for no position; -3, once it is read, for one of
   // infinities or NaN
@@ -68,20 +68,20 @@ __global__ void __launch_bounds__(512) mla_expand_kernel(LatentCache c, int nh, 
   // blocks of one run of weight rows follow each other, over all XCDs; the key parts' come last
   const int across = int((x.total + MP - 1) / MP), part = blockIdx.x / across;
   const int64_t m0 = int64_t(blockIdx.x % across) * MP;
-  if (tid < MP) {
+  if (tid < (MP > kWave ? MP : kWave)) {  // (whole waves)
     int seq = -1, pos = 0;
     mla_sequences(c, x.total, lane, [&](int s, int64_t base, int len) {
       if (m0 + tid >= base && m0 + tid < base + len) seq = s, pos = int(m0 + tid - base);
       return base + len < m0 + MP;
     });
-    s_row[tid] = seq < 0 ? -2 : mla_row(c, seq, pos);
+    if (tid < MP) s_row[tid] = seq < 0 ? -2 : mla_row(c, seq, pos);
   }
   __syncthreads();
   if (s_row[0] == -2) return;  // behind the last sequence's rows
   const KV* rows = static_cast<const KV*>(c.rows);
 
   if ((part + 1) * across == int(gridDim.x)) {
-    for (int i = tid; i < MP * (PT / 8); i += 512) {
+    for (int i = tid; i < MP * (PT / 8); i += STEP) {
       const int r = i / (PT / 8), k = 8 * (i % (PT / 8));
       const int64_t at = s_row[r];
       if (at == -2) continue;
@@ -135,15 +135,16 @@ __global__ void __launch_bounds__(512) mla_expand_kernel(LatentCache c, int nh, 
   rows_of(w0);
   read_w(0, a[0]);
 
-  // The latents: a lane 8 values, 8 rows' loads at a time.  A row that is not finite makes keys that are not, so NaN
+  // The latents: a lane 8 values, up to 8 rows' loads at a time.  A row that is not finite makes keys that are not, so NaN
   // of every token that attends to it; its values are made zeros, as tokens before it would take 0 * NaN from them.
-  for (int r0 = wv; r0 < MP; r0 += 64) {
-    float v[8][WIDE ? 8 : 1];
-    h8_t hv[8];
+  constexpr int RB = MP < 8 * NW ? MP / NW : 8;
+  for (int r0 = wv; r0 < MP; r0 += NW * RB) {
+    float v[RB][WIDE ? 8 : 1];
+    h8_t hv[RB];
     const int k = 8 * lane;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const int64_t at = s_row[r0 + 8 * i];
+    for (int i = 0; i < RB; i++) {
+      const int64_t at = s_row[r0 + NW * i];
       const bool on = at >= 0 && k < c.rank;
       if constexpr (WIDE) {
         if (on) load8<float>(rows + at + k, v[i]);
@@ -156,7 +157,7 @@ __global__ void __launch_bounds__(512) mla_expand_kernel(LatentCache c, int nh, 
       }
     }
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < RB; i++) {
       if constexpr (WIDE) {
         h8_t hi, lo;
 #pragma unroll
@@ -165,23 +166,23 @@ __global__ void __launch_bounds__(512) mla_expand_kernel(LatentCache c, int nh, 
           split2(v[i][e], p, q);
           hi[e] = p, lo[e] = q;
         }
-        *reinterpret_cast<h8_t*>(&s_c[0][r0 + 8 * i][k]) = hi;
-        *reinterpret_cast<h8_t*>(&s_c[CP - 1][r0 + 8 * i][k]) = lo;
+        *reinterpret_cast<h8_t*>(&s_c[0][r0 + NW * i][k]) = hi;
+        *reinterpret_cast<h8_t*>(&s_c[CP - 1][r0 + NW * i][k]) = lo;
         hv[i] = hi;
       } else {
-        *reinterpret_cast<h8_t*>(&s_c[0][r0 + 8 * i][k]) = hv[i];
+        *reinterpret_cast<h8_t*>(&s_c[0][r0 + NW * i][k]) = hv[i];
       }
       typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
       float odd = 0.f;  // sum of 0 * value
 #pragma unroll
       for (int e = 0; e < 8; e += 2)
         odd = __builtin_amdgcn_fdot2(h2_t{hv[i][e], hv[i][e + 1]}, h2_t{_Float16(0), _Float16(0)}, odd, false);
-      if (__ballot(odd != 0.f) && lane == 0) s_row[r0 + 8 * i] = -3;
+      if (__ballot(odd != 0.f) && lane == 0) s_row[r0 + NW * i] = -3;
     }
   }
   __syncthreads();
 
-  for (; w0 < w_end; w0 += S::kStep) {
+  for (; w0 < w_end; w0 += STEP) {
     f4_t acc[4][MJ];
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -198,21 +199,21 @@ __global__ void __launch_bounds__(512) mla_expand_kernel(LatentCache c, int nh, 
 #pragma unroll
           for (int q = 0; q < CP; q++)
 #pragma unroll
-            for (int j0 = 0; j0 < MJ; j0 += 4) {  // 4 operands at a time: registers
-              h8_t b[4];
+            for (int j0 = 0; j0 < MJ; j0 += JB) {  // 4 operands at a time: registers
+              h8_t b[JB];
 #pragma unroll
-              for (int j = 0; j < 4; j++)
+              for (int j = 0; j < JB; j++)
                 b[j] = *reinterpret_cast<const h8_t*>(&s_c[q][16 * (j0 + j) + col][64 * p + 16 * g + 8 * s]);
 #pragma unroll
               for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j0 + j] = mfma(a[pp][i][s], b[j], acc[i][j0 + j]);
+                for (int j = 0; j < JB; j++) acc[i][j0 + j] = mfma(a[pp][i][s], b[j], acc[i][j0 + j]);
             }
       }
     }
     const int h = w0 / WP, n0 = w0 % WP;
-    rows_of(w0 + S::kStep);  // the next rows' first operands are on their way during the stores
-    if (w0 + S::kStep < w_end) read_w(0, a[0]);
+    rows_of(w0 + STEP);  // the next rows' first operands are on their way during the stores
+    if (w0 + STEP < w_end) read_w(0, a[0]);
     const bool key = n0 < NT;
     _Float16* const dst = key ? x.k : x.v;
     const int64_t plane = key ? x.k_plane : x.v_plane;
@@ -680,20 +681,32 @@ template <int NT, int PT, int VT, typename X, typename KV, bool TWO>
 static int launch_prefill(const LatentCache& c, const X* q, int64_t q_stride, int nh, int h0, int nope, int v_dim,
                           const _Float16* w, const Expanded& x, float scale, const MlaRope& rope, X* out,
                           int64_t out_stride, void* parts, hipStream_t s) {
-  // Weight rows a block: 512s, so that the rounds of one block a CU, each its 512s and what loading the latents
-  // takes (about half of one), come out shortest.
-  constexpr int kPos = ExpandShape<KV>::kPos, kStep = ExpandShape<KV>::kStep;
-  const int64_t across = (x.total + kPos - 1) / kPos;
-  const int all = (nh * (NT + VT) + kStep - 1) / kStep;
-  int run = all;
-  double best = 0;
-  for (int n = 1; n <= all; n++) {
-    const int each = (all + n - 1) / n;
-    const double cost = double((across * ((all + each - 1) / each) + 255) / 256) * (each + 0.5);
-    if (n == 1 || cost < best) best = cost, run = each;
+  // Where 512 weight rows and the larger tile of positions a block leave more than half the CUs without one: 128 rows
+  // and 32 positions a block.  A CU takes as long to draw 512 rows from memory whatever the positions: 23 positions of
+  // 20 heads 11 us, with the larger blocks 21; 250 15 and 28; 500 19 and 30; 700 23 and 28.  With 400 positions of 128
+  // heads, blocks for 192 CUs, 32 positions a block would read the weights twelve times (69 us and 32).
+  // Otherwise weight rows a block: 512s, so that the rounds of one block a CU, each its 512s and what loading the
+  // latents takes (about half of one), come out shortest.
+  using S = ExpandShape<KV>;
+  const int rows = nh * (NT + VT), all = (rows + 511) / 512;
+  int64_t across = (x.total + S::kPos - 1) / S::kPos;
+  if (across * all < 128) {
+    across = (x.total + S::kShort - 1) / S::kShort;
+    const dim3 ge(unsigned((rows + 127) / 128 + 1) * unsigned(across));
+    hipLaunchKernelGGL((mla_expand_kernel<NT, PT, VT, KV, TWO, S::kShort, 2>), ge, dim3(128), 0, s, c, nh, nope, v_dim, w,
+                       x, 128);
+  } else {
+    int run = all;
+    double best = 0;
+    for (int n = 1; n <= all; n++) {
+      const int each = (all + n - 1) / n;
+      const double cost = double((across * ((all + each - 1) / each) + 255) / 256) * (each + 0.5);
+      if (n == 1 || cost < best) best = cost, run = each;
+    }
+    const dim3 ge(unsigned((all + run - 1) / run + 1) * unsigned(across));
+    hipLaunchKernelGGL((mla_expand_kernel<NT, PT, VT, KV, TWO, S::kPos, 8>), ge, dim3(512), 0, s, c, nh, nope, v_dim, w,
+                       x, run * 512);
   }
-  const dim3 ge(unsigned((all + run - 1) / run + 1) * unsigned(across));
-  hipLaunchKernelGGL((mla_expand_kernel<NT, PT, VT, KV, TWO>), ge, dim3(512), 0, s, c, nh, nope, v_dim, w, x, run * kStep);
   int rc = check_launch("mla expand");
   if (rc) return rc;
   constexpr int KR = FlashShape<NT, PT, VT, TWO>::KR;

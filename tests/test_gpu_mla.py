@@ -430,6 +430,24 @@ def test_tables_of_many_blocks(dev, block, act, kv):
         p.check(p.run(form), ref, form)
 
 
+@pytest.mark.parametrize("act,kv", TYPES)
+@pytest.mark.parametrize("dims", [{}, dict(rank=72, rope=24), dict(rank=512, rope=64, nope=104, v=128),
+                                  dict(rank=328, rope=64, nope=136, v=72), dict(rank=8, rope=8, nope=192, v=256)], ids=str)
+def test_positions_of_many_heads(dev, dims, act, kv):
+    """Enough heads for the expansion's large tiles: positions that end inside one, a block that is none, and a NaN
+    row, which the tokens before it do not see."""
+    print(f"mla expanded {act} {kv} {dims}", flush=True)
+    p = Problem(43, [200, 0, 131, 1, 190], [3, 1, 0, 1, 2], heads=131, act=act, kv=kv, pad_rows=1, **dims)
+    p.table[0, 3] = -1
+    p.device(dev)
+    ref = p.attention()
+    p.check(p.run("expanded"), ref, "many heads")
+    p.d["rows"][int(p.table[4, 189 // 16]), 189 % 16, 1] = float("nan")
+    out = p.run("expanded").float().cpu().numpy().astype(np.float64)
+    rest = [t for t, _, _ in p.tokens() if t != 6]
+    assert np.isnan(out[6]).all() and off(out[rest], ref[0][rest], ref[1][rest])[0] <= 1
+
+
 # lens, new, heads, widths: few blocks of 128 tokens over long sequences, which are cut into runs of 512 positions
 # or more, each a partial row a token
 LONG = [
