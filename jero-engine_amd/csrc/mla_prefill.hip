@@ -661,8 +661,10 @@ static int prefill_tiles(const LatentCache& c) {
 
 // Runs a tile's positions are cut into.  With fewer blocks than two a CU, cut so that about kFlashUnits
 // runs come out, none below kFlashLeast positions; the partial rows of at most kFlashParts blocks x runs.  Six chunks of
-// 17 to 600 tokens at the end of up to 2100 positions, 20 heads: 125 to 136 us and 13 for the merge, uncut 181.
-constexpr int kFlashUnits = 768, kFlashLeast = 512, kFlashParts = 1280;
+// 17 to 600 tokens at the end of up to 2100 positions, 20 heads: 125 to 136 us and 13 for the merge, uncut 181; a
+// prompt of 500, 20 heads: 28 and 6, uncut 40 (runs of 512 the same as uncut, of 192 25 and 7; a prompt of 700 32 and 8,
+// by 512s 42 and 6, by 192s 34 and 9).
+constexpr int kFlashUnits = 768, kFlashLeast = 256, kFlashParts = 1280;
 struct FlashCut {
   int positions, runs;  // a run's positions, the most runs a tile has
 };

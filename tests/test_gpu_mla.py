@@ -448,10 +448,10 @@ def test_positions_of_many_heads(dev, dims, act, kv):
     assert np.isnan(out[6]).all() and off(out[rest], ref[0][rest], ref[1][rest])[0] <= 1
 
 
-# lens, new, heads, widths: few blocks of 128 tokens over long sequences, which are cut into runs of 512 positions
+# lens, new, heads, widths: few blocks of 128 tokens over long sequences, which are cut into runs of 256 positions
 # or more, each a partial row a token
 LONG = [
-    ([1500], [3], 4, {}), ([513], [1], 2, {}), ([1100, 700, 40], [2, 130, 1], 3, dict(rank=128, rope=32, nope=64, v=64)),
+    ([1500], [3], 4, {}), ([513], [1], 2, {}), ([257], [257], 2, {}), ([300, 20, 256], [40, 20, 1], 3, {}), ([1100, 700, 40], [2, 130, 1], 3, dict(rank=128, rope=32, nope=64, v=64)),
     ([1025, 0, 600], [1, 1, 40], 5, BIG), ([2049], [1], 2, dict(rank=72, rope=24, nope=192, v=200)),
 ]
 
@@ -497,7 +497,7 @@ def test_a_captured_long_prompt_follows_its_length(dev):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         p.run("expanded", out=out, **kw)
-    for n in (1400, 2, 511, 512, 514, 1, 1025, 0, 1399):
+    for n in (1400, 2, 511, 512, 514, 255, 256, 257, 1, 1025, 0, 1399):
         p.lens = [n]
         p.d["lens"].copy_(torch.tensor([n], dtype=torch.int32))
         torch.cuda.synchronize()
