@@ -135,8 +135,8 @@ __global__ void __launch_bounds__(64 * NW) mla_expand_kernel(LatentCache c, int 
   rows_of(w0);
   read_w(0, a[0]);
 
-  // The latents: a lane 8 values, up to 8 rows' loads at a time.  A row that is not finite makes keys that are not, so NaN
-  // of every token that attends to it; its values are made zeros, as tokens before it would take 0 * NaN from them.
+  // The latents: a lane 8 values, up to 8 rows' loads at a time.  A row that is not finite gets keys of NaN, which make
+  // NaN of every token that attends to it, and values of zeros, as tokens before it would take 0 * NaN from them.
   constexpr int RB = MP < 8 * NW ? MP / NW : 8;
   for (int r0 = wv; r0 < MP; r0 += NW * RB) {
     float v[RB][WIDE ? 8 : 1];
@@ -222,7 +222,8 @@ __global__ void __launch_bounds__(64 * NW) mla_expand_kernel(LatentCache c, int 
     for (int j = 0; j < MJ; j++) {
       const int64_t row = s_row[16 * j + col];
       if (row == -2) continue;
-      const bool zero = row == -3 && !key;
+      const bool odd = row == -3;
+      const float instead = key ? NAN : 0.f;
       _Float16* p = dst + (int64_t(h) * x.total + m0 + 16 * j + col) * width + n;
 #pragma unroll
       for (int half = 0; half < 2; half++) {
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(64 * NW) mla_expand_kernel(LatentCache c, int 
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           _Float16 y, z;
-          split2(zero ? 0.f : acc[2 * half + e / 4][j][e % 4], y, z);
+          split2(odd ? instead : acc[2 * half + e / 4][j][e % 4], y, z);
           hi[e] = y, lo[e] = z;
         }
         *reinterpret_cast<h8_t*>(p + 8 * half) = hi;

@@ -333,6 +333,23 @@ def test_later_positions_may_hold_anything(dev, form, act, kv):
         assert far_ <= 1 and rms <= 1, (what, far_, rms)
 
 
+@pytest.mark.parametrize("act,kv", TYPES)
+@pytest.mark.parametrize("form", FORMS)
+def test_infinite_latents_with_scores_of_minus_infinity(dev, form, act, kv):
+    """A score of minus infinity weighs nothing, but the values beside it are not finite: NaN, as 0 * inf."""
+    p = Problem(44, [60, 40], [3, 1], heads=2, nope=8, act=act, kv=kv)
+    p.rows[p.table[0, 2], 32 % 16, 0] = np.inf
+    first = range(3)
+    for h in range(2):
+        p.q[:3, h, :8] = -np.sign(p.wk[h, :, 0]) * np.abs(p.q[:3, h, :8])
+    p.device(dev)
+    out = p.run(form).float().cpu().numpy().astype(np.float64)
+    with np.errstate(all="ignore"):
+        exact, far = p.attention()
+    assert np.isnan(out[list(first)]).all()
+    assert off(out[3:4], exact[3:4], far[3:4])[0] <= 1
+
+
 @pytest.mark.parametrize("scale", [-0.3, 0.0])
 @pytest.mark.parametrize("form", FORMS)
 def test_other_scales(dev, form, scale):
