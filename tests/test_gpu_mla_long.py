@@ -1,0 +1,108 @@
+"""Latent attention over long caches on the GPU: what only runs of many steps reach.
+
+A workgroup of the absorbed form takes a run of 32-position steps, and all CUs get one: a run has several
+steps only where the call's sequences hold some 70000 positions together.  Here the sequences share one
+set of blocks, so that the oracle works on one set of rows, all tokens at a time.
+"""
+import math
+
+import numpy as np
+import pytest
+
+from mla_oracle import Problem, THETA, off, rotate
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [("f32", "f16"), ("f16", "f16"), ("f32", "f32")]
+
+
+class Shared(Problem):
+    """Sequences of `lens` positions, all over the blocks of the longest.  `stairs` nats are added to the scores of
+    every second head at three places (by the key part, whose queries come rotated: theta 0)."""
+
+    def __init__(self, seed, lens, new, stairs=0.0, **kw):
+        super().__init__(seed, [max(lens)], [1], max_len=max(lens), **kw)
+        g = np.random.default_rng(seed + 1)
+        self.theta = 0.0 if stairs else THETA
+        self.lens, self.new = list(lens), list(new)
+        self.c = self.visible(0, max(lens) - 1)
+        self.table = np.repeat(self.table, len(lens), 0)
+        self.starts = np.cumsum([0] + self.new).astype(np.int32)
+        self.T = int(self.starts[-1])
+        q = g.standard_normal((self.T, self.H, self.N + self.P)) * 1.5
+        if stairs:
+            self.c[:, self.R] = np.searchsorted([3300, 3860, 4420], np.arange(max(lens)), side="right")
+            for j in range(max(lens)):
+                self.rows[self.table[0, j // self.block], j % self.block, self.R] = self.c[j, self.R]
+            q[:, :, self.N] = 0
+            q[:, ::2, self.N] = stairs / self.scale
+        self.q = q.astype(self.q.dtype)
+
+    def attention(self, theta=None):
+        """Problem.attention and Problem.bound for all tokens of a head at once; a score's own error weighs its own
+        position, so that positions far below the maximum do not widen the bounds."""
+        theta = self.theta if theta is None else theta
+        half = self.act == "f16"
+        u, f = 2.0 ** (-11 if half else -22) / math.sqrt(3), 2.0 ** -24
+        n, c, c2, s, R, N = self.R + self.P + self.N, self.c, self.c ** 2, self.scale, self.R, self.N
+        out, far = np.zeros((self.T, self.H, self.V)), np.zeros((self.T, self.H, 2))
+        pos = np.array([p for _, _, p in self.tokens()])
+        hidden = np.arange(len(c))[None, :] > pos[:, None]
+        for h in range(self.H):
+            wk, wv, q = self.wk[h].astype(np.float64), self.wv[h].astype(np.float64), self.q[:, h].astype(np.float64)
+            qp = np.stack([rotate(x, p, theta) for x, p in zip(q[:, N:], pos)]) if theta else q[:, N:]
+            q = np.concatenate([q[:, :N], qp], 1)
+            qa = np.concatenate([q[:, :N] @ wk, qp], 1)
+            k, v = c[:, :R] @ wk.T, c[:, :R] @ wv.T
+            a = np.where(hidden, -np.inf, s * (qa @ c.T))
+            under = a.max(1, keepdims=True) - a
+            p = np.exp(-under)
+            p /= p.sum(1, keepdims=True)
+            o = p @ v
+            prod = np.sqrt(np.maximum((qa ** 2 @ c2.T).max(1), (q ** 2 @ np.concatenate([k ** 2, c2[:, R:]], 1).T).max(1)))
+            inner = np.sqrt((q[:, :N] ** 2 @ wk ** 2).max(1) * c2.sum(1).max())
+            ds = s * (math.sqrt(2) * u * prod + f * math.sqrt(n) * (prod + inner))[:, None] + \
+                np.where(hidden, 0, under) * 2.0 ** -22
+            w = (p * ds) ** 2
+            apart = w @ v ** 2 - 2 * o * (w @ v) + o ** 2 * w.sum(1, keepdims=True)
+            lat = ((p ** 2) @ c2[:, :R] + (p @ c[:, :R]) ** 2) @ (wv ** 2).T
+            each = np.maximum(apart, 0) + (2 * u * u + f * f * (n + len(c))) * ((p ** 2) @ v ** 2 + lat + o * o)
+            each = each + (2.0 ** -11 / math.sqrt(3) * o if half else f * o) ** 2
+            out[:, h], far[:, h, 0], far[:, h, 1] = o, 8 * np.sqrt(each.max(1)), np.sqrt(each.mean(1))
+        return out, far
+
+    def steps(self):
+        """Steps of the longest run, by the plan's rule: equal runs of the items' units (steps, and 3 an item)."""
+        share = min(64 // self.H, -(-self.T // len(self.lens))) if self.T > len(self.lens) and self.H <= 32 else 1
+        rows = share * self.H
+        at = 16 if rows <= 16 else 32 if rows <= 32 else 128 if rows > 64 and self.act == "f16" else 64
+        groups = -(-rows // at)
+        runs = 8 if groups >= 32 else 256 // groups // 8 * 8
+        items = []
+        for n, L in zip(self.new, self.lens):
+            items += [-(-min(L, L - n + i + share) // 32) + 3 for i in range(0, n, share)]
+        return -(-sum(items) // runs) - 3
+
+
+# sixteen sequences of odd lengths; one token each and several
+LENS = [4700 - 13 * i for i in range(16)]
+ONE, TWO_ = [1] * 16, [2] * 16
+BIG = dict(rank=512, rope=64, nope=16, v=24)
+LONG = [(h, new, t, BIG) for t in TYPES for h, new in ((5, ONE), (20, ONE), (40, ONE), (5, TWO_), (20, TWO_))]
+LONG += [(66, ONE, ("f16", "f16"), BIG), (128, ONE, ("f16", "f16"), BIG), (66, ONE, ("f32", "f32"), BIG)]
+LONG += [(h, ONE, t, d) for d in (dict(rank=120, rope=24), dict(rank=248, rope=40)) for t in TYPES for h in (5, 40, 66)
+         if h < 66 or t[0] == "f16"]
+
+
+@pytest.mark.parametrize("stairs", [0.0, 6.5], ids=["level", "stairs"])
+@pytest.mark.parametrize("heads,new,types,dims", LONG, ids=lambda x: "-".join(map(str, x.values() if isinstance(x, dict) else x))
+                         if not isinstance(x, int) else f"h{x}")
+def test_runs_of_many_steps(dev, heads, new, types, dims, stairs):
+    """Every ring buffer is used again, maxima grow by 2^9 within runs (stairs), and block ids are read anew."""
+    act, kv = types
+    print(f"mla absorbed {act} {kv} {heads} heads, {new[0]} tokens, {dims}, stairs {stairs}", flush=True)
+    p = Shared(50, LENS, new, heads=heads, act=act, kv=kv, block=2 if heads in (5, 66) else 64, stairs=stairs,
+               **{**dict(nope=16, v=24), **dims})
+    assert p.steps() >= 5
+    p.device(dev, starts=new != ONE)
+    print("  off by", p.check(p.run("absorbed", theta=p.theta), what="long"), flush=True)
