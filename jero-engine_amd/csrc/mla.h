@@ -12,6 +12,14 @@ namespace jero {
 constexpr int kMlaMaxRank = 512;
 constexpr int kMlaMaxRope = 64;
 
+// Softmax numerators go into the f16 products (and the totals) 2^Lift above 2^(score - maximum), and a row's
+// accumulators are rescaled once its maximum grew by more than 2^Grow: none is above 2^15, and f16's last place,
+// 2^-24, is at most 2^(-24 - Lift) of the row's largest.  Not lifted, 6 % are lost of 8192 positions 16 nats below a
+// peak (9e-4 of the row), and all of them at 17.4 nats.  The absorbed form's runs are short and rescaling 16 heads'
+// 512 columns is dear: one token of 131072 positions takes 107 us in all with Grow 6, 109 with 5, 111 with 4 (106
+// with 8), 64 f16 sequences 116, 119, 123 (115).  The expanded form's time is the same.
+constexpr float kAttendLift = 9.f, kAttendGrow = 6.f, kFlashLift = 11.f, kFlashGrow = 4.f;
+
 // A jero_latent_cache as the kernels take it.
 struct LatentCache {
   const void* rows;

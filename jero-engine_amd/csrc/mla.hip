@@ -406,8 +406,8 @@ struct AttendShape {
 // 4g + e (g = lane / 16) of each 16, which is the B layout of the product O^T[r][head] += C^T p if 32 positions
 // are taken in the order 4g .. 4g + 3, 16 + 4g .. 16 + 4g + 3: numerators never leave the lane, and C^T comes
 // from the same LDS rows by transposing reads.  The accumulators (RT x 16 heads a wave) stay in registers;
-// they are rescaled only where the maximum grew by more than 2^8 (numerators stay below 256, far from f16's
-// end).
+// they are rescaled only where the maximum grew by more than 2^kAttendGrow.  With one part, the totals sum
+// the numerators as the product rounds them.
 //
 // Registers allow one wave a SIMD, so a wave covers its own waits: a step's softmax runs between the products
 // of the next step's scores, operands are read from LDS a group of products ahead, and the rows two steps on are
@@ -702,10 +702,11 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
         mx = max_over_groups(mx);
         asm volatile("" : "+v"(mx));
       } else if (piece == 6) {
-        grew = __any(mx > m[0] + 8.f);
+        grew = __any(mx > m[0] + kAttendGrow);
         const float mn = grew ? fmaxf(m[0], mx) : m[0];
         ref = mn == -INFINITY ? 0.f : mn;
         alpha = __builtin_amdgcn_exp2f(m[0] - ref);  // 0 at first: exp2(-inf)
+        ref -= kAttendLift;
         m[0] = mn;
         l[0] *= alpha;
         asm volatile("" : "+v"(ref), "+v"(alpha), "+v"(m[0]), "+v"(l[0]));
@@ -714,7 +715,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
         for (int n = (piece - 7) * NS / 8; n < (piece - 6) * NS / 8; n++) {
           const float p = __builtin_amdgcn_exp2f(sc[n] - ref);
           split2(p, ph[n], pl[n]);
-          sc[n] = p;
+          sc[n] = TWO ? p : float(ph[n]);
           asm volatile("" : "+v"(sc[n]));
         }
       } else {
@@ -823,7 +824,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
             top = fmaxf(top, x8[n]);
           }
           top = max_over_groups(top);
-          const bool up = __any(top > m[w] + 8.f);
+          const bool up = __any(top > m[w] + kAttendGrow);
           const float mn = up ? fmaxf(m[w], top) : m[w];
           const float at0 = mn == -INFINITY ? 0.f : mn;
           by[w] = __builtin_amdgcn_exp2f(m[w] - at0);
@@ -832,9 +833,8 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
           float add8 = 0.f;
 #pragma unroll
           for (int n = 0; n < 8; n++) {
-            const float y = __builtin_amdgcn_exp2f(x8[n] - at0);
-            p[w][n] = _Float16(y);
-            add8 += y;
+            p[w][n] = _Float16(__builtin_amdgcn_exp2f(x8[n] - (at0 - kAttendLift)));
+            add8 += float(p[w][n]);
           }
           l[w] = l[w] * by[w] + add8;
         }

@@ -305,7 +305,7 @@ __device__ __forceinline__ bool flash_tile(const LatentCache& c, int64_t total, 
 // Causal attention of 128 tokens of a sequence and a head, one pass with a running maximum and sum.  S^T =
 // K q^T (positions x tokens) leaves a token per lane column and, taken in the order 4g .. 4g + 3, 16 + 4g .. of
 // 32 positions, is the B operand of O^T += V^T p, V^T read from LDS transposed: numerators, factors and
-// accumulators of a token stay in its lanes.  Accumulators are rescaled only where a maximum grew by 2^8.
+// accumulators of a token stay in its lanes.  Accumulators are rescaled only where a maximum grew by 2^kFlashGrow.
 // Grid y: runs of `cut` steps; a tile of more than one leaves a partial row a token and run (part_o, part_ml),
 // which mla_flash_merge_kernel joins.
 //
@@ -506,16 +506,16 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
 #pragma unroll
         for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[j][r][e]);
       mx = max_over_groups(mx) * times[j];
-      grew[j] = __any(mx > m[j] + 8.f);
+      grew[j] = __any(mx > m[j] + kFlashGrow);
       const float mn = grew[j] ? fmaxf(m[j], mx) : m[j];
-      const float ref = mn == -INFINITY ? 0.f : mn;
+      const float ref = mn == -INFINITY ? 0.f : mn, from = ref - kFlashLift;
       alpha[j] = __builtin_amdgcn_exp2f(m[j] - ref);
       m[j] = mn;
 #pragma unroll
       for (int r = 0; r < RT; r++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[j][r][e], times[j], -ref));
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[j][r][e], times[j], -from));
           _Float16 a, b;
           split2(p, a, b);
           bh[j][r / 2][4 * (r & 1) + e] = a;

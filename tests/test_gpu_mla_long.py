@@ -4,12 +4,15 @@ A workgroup of the absorbed form takes a run of 32-position steps, and all CUs g
 steps only where the call's sequences hold some 70000 positions together.  Here the sequences share one
 set of blocks, so that the oracle works on one set of rows, all tokens at a time.
 """
+import ctypes as C
 import math
 
 import numpy as np
 import pytest
+import torch
 
-from mla_oracle import Problem, THETA, off, rotate
+import jero_hip as J
+from mla_oracle import Problem, THETA, rotate
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +109,54 @@ def test_runs_of_many_steps(dev, heads, new, types, dims, stairs):
     assert p.steps() >= 5
     p.device(dev, starts=new != ONE)
     print("  off by", p.check(p.run("absorbed", theta=p.theta), what="long"), flush=True)
+
+
+# ---------------------------------------------------------------- one peak over a long tail
+
+
+@pytest.mark.parametrize("act,kv", TYPES)
+@pytest.mark.parametrize("peak", [0, 5000, 8192])
+@pytest.mark.parametrize("nats", [10.0, 13.0, 16.0, 17.375])
+@pytest.mark.parametrize("form", ["absorbed", "expanded"])
+def test_a_peak_over_thousands_of_small_numerators(dev, form, nats, peak, act, kv):
+    """One position of value 0, and 8192 of value 1 with scores `nats` below it, in one run: their small
+    numerators add up to what is seen of them.
+
+    Scores and values are exact.  A numerator's relative error: the exponent's three f32 roundings and its
+    exponential's (nats 3 2^-24 + 2^-23), its parts' (2^-22, with f16 activations 2^-11), and, as f16 holds
+    numerators 2^9 (expanded: 2^11) above their value, half its last place: 2^-34 (2^-36) of the peak.  The f32 sums
+    of equal terms: 2^-24 a step of 32, for numerators and total."""
+    print(f"mla {form} {act} {kv}: peak at {peak}, {nats} nats", flush=True)
+    n, T = 8192, 512 if form == "absorbed" else 1
+    p = Problem(51, [1], [1], heads=1, rank=64, rope=16, nope=8, v=8, act=act, kv=kv, block=256)
+    p.lens, p.new, p.T, p.max_len = [n + 1] * T, [1] * T, T, n + 1
+    p.n_blocks = 33
+    rows = np.zeros((33 * 256, 80), p.rows.dtype)
+    rows[:, 1] = 1
+    rows[peak] = 0
+    rows[peak, 0] = nats
+    p.rows = rows.reshape(33, 256, 80)
+    p.table = np.repeat(np.arange(33, dtype=np.int32)[None], T, 0)
+    p.starts = np.arange(T + 1, dtype=np.int32)
+    p.wk[:], p.wv[:] = 0, 0
+    p.wk[0, 0, 0] = 1
+    p.wv[0, :, 1] = 1
+    p.q = np.zeros((T, 1, 24), p.q.dtype)
+    p.q[..., 0] = 1
+    p.scale = 1.0
+    p.device(dev, starts=False)
+    kw = {}
+    if form == "expanded":  # a workspace without room for partial rows: the positions stay in one run
+        c = J.HipLatentCache.from_buffer_copy(p.cache.c)
+        c.max_len = 1
+        need = J.lib().jero_hip_mla_prefill_workspace_bytes(C.byref(c), J.F16 if act == "f16" else J.F32, 1, 8, 8, n + 1)
+        kw = dict(workspace=torch.empty(need, dtype=torch.uint8, device=dev))
+    got = p.run(form, theta=0.0, **kw).double().cpu().numpy()
+    small = math.exp(-nats)
+    exact = n * small / (1 + n * small)
+    half = act == "f16"
+    each = nats * 3 * 2.0 ** -24 + 2.0 ** -23 + (2.0 ** -11 if half else 2.0 ** -22) + \
+        2.0 ** (-34 if form == "absorbed" else -36) / small
+    far = exact * each + 2 * exact * (n / 32 + 64) * 2.0 ** -24 + exact * (2.0 ** -11 if half else 2.0 ** -22)
+    print(f"  {np.abs(got - exact).max() / far:.3g} of {far / exact:.3g}", flush=True)
+    assert (np.abs(got - exact) <= far).all()
