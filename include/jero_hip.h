@@ -313,8 +313,8 @@ int jero_hip_gqa_attention(float *out_dev, const float *q_dev, const void *k_dev
  * them, and its tokens are rows starts[s] .. starts[s + 1] - 1 of x / q / out (starts NULL: row s,
  * one token each, and n_tokens = n_seqs).  lens, starts and the table are read on the device, so a
  * captured graph follows them from replay to replay.
- *   - Token rows from starts[n_seqs] on belong to no sequence: they are not read, their outputs not
- *     written.
+ *   - Token rows before starts[0] and from starts[n_seqs] on belong to no sequence: they are not read
+ *     (a call of more n_tokens than x or q has rows may be captured), their outputs not written.
  *   - A position below 0 (a sequence with more tokens than positions) is not stored and attends to
  *     nothing; a token that attends to nothing gets zeros.
  *   - Positions from max_len on are neither stored nor attended to.

@@ -51,6 +51,12 @@ __device__ __forceinline__ float2 mla_cos_sin(const MlaRope& rope, int i, int po
   return make_float2(c, s);
 }
 
+// The call's token rows that belong to a sequence, [lo, hi): the others' memory need not be there.
+__device__ __forceinline__ void mla_owned(const LatentCache& c, int& lo, int& hi) {
+  lo = c.starts ? max(c.starts[0], 0) : 0;
+  hi = c.starts ? min(c.starts[c.n_seqs], c.n_tokens) : c.n_tokens;
+}
+
 // The sequence and position of token row t, found by the whole wave: the sequence is the last whose
 // start is not behind t, and the starts do not decrease, so counting them is enough: 64 spread over those
 // left at a time.  False for rows of no sequence.

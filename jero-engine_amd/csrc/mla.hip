@@ -12,7 +12,7 @@ namespace jero {
 // One wave per token row: lane l holds elements 8l .. 8l + 7 of the latent, the first rope / 2 lanes a
 // pair of the key part each.  The sum of squares is f32; the row is rounded once, to the cache's type.
 // VEC: the rows of x are 16-byte aligned, and are read so (stores always are: 8-element rows of the pool).  What
-// the row needs is on its way before the row's place is looked up.
+// a row of some sequence needs is on its way before its place is looked up.
 //
 // Bound by its bytes, for a decode step by the launch: 16638 rows of 576 f16 values take 10.0 us (3.8 TB/s; a large
 // copy 4.6), 64 rows 3.9 us; one value a lane and load took 30 us.
@@ -21,7 +21,9 @@ __global__ void __launch_bounds__(256) mla_append_kernel(LatentCache c, const X*
                                                          const float* __restrict__ norm, float eps, MlaRope rope) {
   const int lane = threadIdx.x & 63;
   const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (t >= c.n_tokens) return;
+  int lo, hi;
+  mla_owned(c, lo, hi);
+  if (t < lo || t >= hi) return;
   const X* xr = x + t * x_stride;
   const int k = min(8 * lane, c.rank - 8), i = min(lane, c.rope / 2 - 1);
   float v[8], w[8];
@@ -168,13 +170,14 @@ __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X*
     int h, t0;
     if (!mla_head8_block(blockIdx.x, nh, (c.n_tokens + 15) / 16, h, t0)) return;
     t0 *= 16;
+    int lo, hi;
+    mla_owned(c, lo, hi);
     constexpr int NR = kMlaMaxRank / 128;  // 16s of rows a wave
     __shared__ float s_max[8][16];
     __shared__ uint32_t s_key[16];
     __shared__ int s_ex[16], s_first[16];
     const int g = lane >> 4, col = lane & 15;
     // everything the wave reads is on its way before anything is waited for
-    const X* qr = q + min(t0 + col, c.n_tokens - 1) * q_stride + int64_t(h) * (nope + c.rope);
     h8_t b[NR][NT];
 #pragma unroll
     for (int k = 0; k < NR; k++)
@@ -182,13 +185,16 @@ __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X*
       for (int i = 0; i < NT; i++)
         b[k][i] = *reinterpret_cast<const h8_t*>(
             k_b + (int64_t(h) * c.rank + min(16 * (wv + 8 * k) + col, c.rank - 1)) * nope + min(32 * i + 8 * g, nope - 8));
+    // (the parts of rows of no sequence are not used, nor made where all 16 are such)
+    if (lo >= hi || t0 >= hi || t0 + 16 <= lo) return;
+    const X* qr = q + min(max(t0 + col, lo), hi - 1) * q_stride + int64_t(h) * (nope + c.rope);
     float qv[NT][8];
 #pragma unroll
     for (int i = 0; i < NT; i++) load8<X>(qr + min(32 * i + 8 * g, nope - 8), qv[i]);
     // the key part, its pair of the thread's token
     const int pairs = c.rope / 2, kt_ = tid / pairs, ki = tid % pairs;
     const bool key = kt_ < 16 && t0 + kt_ < c.n_tokens;
-    const int key_t = min(t0 + min(kt_, 15), c.n_tokens - 1);
+    const int key_t = min(max(t0 + min(kt_, 15), lo), hi - 1);
     const X* kp = q + key_t * q_stride + int64_t(h) * (nope + c.rope) + nope + 2 * ki;
     const float kx = float(kp[0]), ky = float(kp[1]);
     if (tid < 16) {
