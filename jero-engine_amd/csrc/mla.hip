@@ -617,7 +617,9 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
     for (int w = 0; w < HW; w++) {
       const _Float16* const qp =
           qa.parts + (int64_t(t) * g16 + min(h0 / 16 + w, (rows_in + 15) / 16 - 1)) * KT * 512 + 8 * lane;
-      factor[w] = qa.factor[int64_t(t) * g16 * 16 + min(h0 + 16 * w + col, rows_in - 1)];
+      // (columns past the item's rows hold what the workspace held: scores of 0 or NaN, which no maximum grows by)
+      const int row = h0 + 16 * w + col;
+      factor[w] = row < rows_in ? qa.factor[int64_t(t) * g16 * 16 + row] : 0.f;
 #pragma unroll
       for (int i = 0; i < KT; i++) {
         qh[w][i] = *reinterpret_cast<const h8_t*>(qp + 512 * i);

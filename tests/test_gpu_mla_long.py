@@ -111,6 +111,22 @@ def test_runs_of_many_steps(dev, heads, new, types, dims, stairs):
     print("  off by", p.check(p.run("absorbed", theta=p.theta), what="long"), flush=True)
 
 
+@pytest.mark.parametrize("act,kv", TYPES)
+@pytest.mark.parametrize("heads,new", [(5, ONE), (20, ONE), (7, TWO_), (35, ONE), (70, ONE)], ids=lambda x: str(x) if isinstance(x, int) else f"new{x[0]}")
+def test_bits_do_not_hang_on_what_the_workspace_held(dev, heads, new, act, kv):
+    """Heads that do not fill 16s: the same bits over workspaces of zeros, of NaN, and of any values."""
+    print(f"mla absorbed {act} {kv} {heads} heads, {new[0]} tokens", flush=True)
+    p = Shared(52, LENS, new, heads=heads, act=act, kv=kv, block=64, rank=64, rope=16, nope=16, v=24).device(dev, starts=new != ONE)
+    need = J.lib().jero_hip_mla_absorbed_workspace_bytes(p.cache.ref, p.T, heads)
+    want = p.run("absorbed", workspace=torch.zeros(need, dtype=torch.uint8, device=dev))
+    g = torch.Generator(device=dev).manual_seed(1)
+    for ws in [torch.full((need,), 255, dtype=torch.uint8, device=dev)] + \
+            [torch.randint(0, 256, (need,), dtype=torch.uint8, device=dev, generator=g) for _ in range(4)]:
+        got = p.run("absorbed", workspace=ws)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), (got != want).sum().item()
+
+
 # ---------------------------------------------------------------- one peak over a long tail
 
 
