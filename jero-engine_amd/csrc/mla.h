@@ -57,13 +57,18 @@ __device__ __forceinline__ void mla_owned(const LatentCache& c, int& lo, int& hi
   hi = c.starts ? min(c.starts[c.n_seqs], c.n_tokens) : c.n_tokens;
 }
 
+// Position of token row t of a sequence that ends before row `end` with `len` positions; far below 0 it stays there.
+__device__ __forceinline__ int mla_position(int len, int end, int t) {
+  return int(max(int64_t(len) - end + t, int64_t(-(1 << 30))));
+}
+
 // The sequence and position of token row t, found by the whole wave: the sequence is the last whose
 // start is not behind t, and the starts do not decrease, so counting them is enough: 64 spread over those
 // left at a time.  False for rows of no sequence.
 __device__ __forceinline__ bool mla_locate(const LatentCache& c, int t, int lane, int& seq, int& pos) {
   if (!c.starts) {
     seq = t;
-    pos = c.lens[t] - 1;
+    pos = mla_position(c.lens[t], 1, 0);
     return true;
   }
   int count = 0, left = c.n_seqs + 1;  // starts below `count` are not behind t, those from count + left on are
@@ -77,7 +82,7 @@ __device__ __forceinline__ bool mla_locate(const LatentCache& c, int t, int lane
   seq = count - 1;
   if (seq < 0 || seq >= c.n_seqs) return false;
   const int first = c.starts[seq], end = c.starts[seq + 1];
-  pos = int(int64_t(c.lens[seq]) - end + t);
+  pos = mla_position(c.lens[seq], end, t);
   return t >= first;
 }
 

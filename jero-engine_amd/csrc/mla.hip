@@ -112,7 +112,7 @@ __device__ __forceinline__ int mla_item_tokens(const LatentCache& c, int share, 
 __device__ __forceinline__ bool mla_locate_thread(const LatentCache& c, int t, int& seq, int& pos) {
   if (!c.starts) {
     seq = t;
-    pos = c.lens[t] - 1;
+    pos = mla_position(c.lens[t], 1, 0);
     return true;
   }
   int lo = 0, hi = c.n_seqs + 1;  // starts below lo are <= t, those from hi on are not
@@ -123,7 +123,7 @@ __device__ __forceinline__ bool mla_locate_thread(const LatentCache& c, int t, i
   }
   seq = lo - 1;
   if (seq < 0 || seq >= c.n_seqs) return false;
-  pos = int(int64_t(c.lens[seq]) - c.starts[seq + 1] + t);
+  pos = mla_position(c.lens[seq], c.starts[seq + 1], t);
   return true;
 }
 

@@ -65,3 +65,20 @@ def test_a_call_of_more_rows_than_there_are(dev, act, new, heads, tokens, first)
     assert np.array_equal(got[~hit], p.rows[~hit].astype(np.float64))
     # half a step of f16 and of the f32 arithmetic before it (at most 16 roundings of values up to 8)
     assert (np.abs(got[hit] - rows[hit]) <= 2.0 ** -11 * np.abs(rows[hit]) + 2.0 ** -17).all()
+
+
+@pytest.mark.parametrize("one", [True, False], ids=["no starts", "starts"])
+def test_lengths_far_below_zero(dev, one):
+    """A length at the end of 32 bits: the sequence's tokens are at positions below 0, stored nowhere, zeros out."""
+    p = Problem(61, [50, 60, 40, 64], [1] * 4 if one else [1, 3, 2, 2], heads=3, rest=0.25)
+    p.lens[1], p.lens[2] = -(2 ** 31), -(2 ** 31) + 1
+    p.device(dev, starts=not one)
+    for form in ("absorbed", "expanded"):
+        print(f"mla {form}, lengths far below 0", flush=True)
+        out = p.run(form)
+        p.check(out, what=form)
+        assert (out[1:2 if one else 6] == 0).all()
+    J.mla_append(p.cache, p.d["x"], p.d["norm"], EPS, THETA)
+    _, hit = p.appended()
+    got = p.d["rows"].double().cpu().numpy()
+    assert np.array_equal(got[~hit], p.rows[~hit].astype(np.float64)) and hit.sum() == (2 if one else 3)
