@@ -136,7 +136,9 @@ __global__ void __launch_bounds__(64 * NW) mla_expand_kernel(LatentCache c, int 
   read_w(0, a[0]);
 
   // The latents: a lane 8 values, up to 8 rows' loads at a time.  A row that is not finite gets keys of NaN, which make
-  // NaN of every token that attends to it, and values of zeros, as tokens before it would take 0 * NaN from them.
+  // NaN of every token that attends to it, and values of zeros, as tokens before it would take 0 * NaN from them.  A key
+  // past f16's range is NaN too (minus infinity would drop its position; two parts, infinities of both signs, do not);
+  // such a value stays infinite.
   constexpr int RB = MP < 8 * NW ? MP / NW : 8;
   for (int r0 = wv; r0 < MP; r0 += NW * RB) {
     float v[RB][WIDE ? 8 : 1];
@@ -231,7 +233,8 @@ __global__ void __launch_bounds__(64 * NW) mla_expand_kernel(LatentCache c, int 
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           _Float16 y, z;
-          split2(odd ? instead : acc[2 * half + e / 4][j][e % 4], y, z);
+          const float sum = acc[2 * half + e / 4][j][e % 4];
+          split2(odd || (!TWO && key && !(fabsf(sum) < 65520.f)) ? instead : sum, y, z);
           hi[e] = y, lo[e] = z;
         }
         *reinterpret_cast<h8_t*>(p + 8 * half) = hi;
@@ -380,6 +383,8 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
   }
   // positions below the wave's first token's need no mask
   const int low = int(max(int64_t(0), min(shift + first + wv * 32 + 1, int64_t(len))));
+  // below the first token's, all tokens of the block attend to a position
+  const int common = int(max(int64_t(0), min(shift + first + 1, int64_t(len))));
   const int32_t* table = c.table + seq * c.table_stride;
 
   const uint8_t* const kb = reinterpret_cast<const uint8_t*>(x.k + (int64_t(h) * x.total + base) * NT);
@@ -444,6 +449,42 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
       ids = block(i + 1);
     }
     const uint8_t* kv = s_kv + (i & 1) * S::kBuf;
+    const int p0 = i * KR;
+    // Rows of values past f16's range, of which a token that does not attend to them would take 0 * infinity, are made
+    // zeros, and their key parts NaN.  Every wave looks through all rows and finds the same (LDS is full: no word for it).
+    // 2048 f32 tokens of 32 heads take 175 us with this (expansion too) and 172.5 without, 4097 f16 of 128 1020 and 1006.
+    if (p0 + KR > common) {
+      constexpr int L = VT / 8, PER = 64 / L;  // lanes a row, rows a read
+      uint8_t* const rows = s_kv + (i & 1) * S::kBuf;
+      uint64_t odd = 0;
+      int id = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));  // the lane
+      asm volatile("" : "+v"(id));  // (what hangs on it is made here, not kept in registers over the loop)
+#pragma unroll 4
+      for (int k = 0; k < KR / PER; k++) {
+        typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+        const h8_t v = *reinterpret_cast<const h8_t*>(rows + S::kKey + S::kRope + k * 1024 + 16 * id);
+        float sum = 0.f;  // of 0 * value
+#pragma unroll
+        for (int e = 0; e < 8; e += 2)
+          sum = __builtin_amdgcn_fdot2(h2_t{v[e], v[e + 1]}, h2_t{_Float16(0), _Float16(0)}, sum, false);
+        const uint64_t any = __ballot(sum != 0.f);
+        for (int r = 0; any && r < PER; r++)
+          if ((any >> (r * L)) & ((1ull << L) - 1)) odd |= 1ull << (k * PER + r);
+      }
+      if (odd) {
+        __syncthreads();
+        for (int r = wv; r < KR; r += 4)
+          if ((odd >> r) & 1) {
+            uint32_t z1 = 0u, nan1 = 0x7E007E00u;
+            asm volatile("" : "+v"(z1), "+v"(nan1));
+            const u32x4 z = {z1, z1, z1, z1}, nan = {nan1, nan1, nan1, nan1};
+            if (id < L * S::kPlanes)
+              *reinterpret_cast<u32x4*>(rows + S::kKey + S::kRope + (id / L) * S::kPlane + r * VT * 2 + 16 * (id % L)) = z;
+            if (id < PT / 8) *reinterpret_cast<u32x4*>(rows + S::kKey + r * PT * 2 + 16 * id) = nan;
+          }
+        __syncthreads();
+      }
+    }
     f4_t s[2][RT];
     // operands are read a group of products ahead
     constexpr int KP = S::kPlanes;
@@ -479,7 +520,6 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    const int p0 = i * KR;
     h8_t bh[2][RT / 2], bl[2][RT / 2];
     bool grew[2];
     float alpha[2];
