@@ -371,7 +371,7 @@ int jero_hip_mla_absorbed_attention(const jero_latent_cache *cache, int act_dtyp
  * its W_uv rows (nope_dim + rope_dim up to 256).  total_len, up to 2^23: at least the sum of the
  * lengths (each up to max_len); a sequence whose rows do not fit within total_len after those before it is treated
  * as empty.  The keys and values of as many heads as the workspace holds are made at a time: it must
- * hold one head's, jero_hip_mla_prefill_workspace_bytes(..., 1, ...), and the entry point's n_heads gives what
+ * hold one head's, jero_hip_mla_prefill_workspace_bytes(..., 0, ...), and the entry point's n_heads gives what
  * holds them all up to 1 GiB, and room for the partial rows that let a few long sequences be cut into
  * runs of positions (without it they are not; the sums' order differs).  At most 4096 sequences
  * (CapabilityMismatch). */

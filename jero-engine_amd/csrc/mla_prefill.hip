@@ -774,16 +774,17 @@ using namespace jero;
 
 extern "C" size_t jero_hip_mla_prefill_workspace_bytes(const jero_latent_cache* cache, int act_dtype, int n_heads,
                                                        int nope_dim, int v_dim, int64_t total_len) {
-  if (!cache || n_heads < 1 || nope_dim < 1 || v_dim < 1 || total_len < 1) return 0;
+  if (!cache || n_heads < 0 || nope_dim < 1 || v_dim < 1 || total_len < 1) return 0;
   const PrefillShape s = prefill_shape(nope_dim, cache->rope_dim, v_dim);
   const int planes = act_dtype == JERO_F16 ? 1 : 2;
   const size_t one = prefill_bytes(s, total_len, 1, planes), head = size_t(total_len) * (s.nt + s.vt) * 2 * planes;
+  if (n_heads == 0) return one;
   size_t heads = 1;
   if (one < (size_t(1) << 30)) heads += ((size_t(1) << 30) - one) / (head + 512);
   // (a call whose positions may be cut into runs, with room for their partial rows)
   const int64_t longest = total_len < cache->max_len ? total_len : cache->max_len;
   return prefill_bytes(s, total_len, heads < size_t(n_heads) ? heads : size_t(n_heads), planes) +
-         (n_heads > 1 && longest > kFlashLeast ? flash_part_bytes(s.vt) : 0);
+         (longest > kFlashLeast ? flash_part_bytes(s.vt) : 0);
 }
 
 extern "C" int jero_hip_mla_prefill_attention(const jero_latent_cache* cache, int act_dtype, const void* q_dev,
