@@ -817,12 +817,19 @@ extern "C" int jero_hip_mla_prefill_attention(const jero_latent_cache* cache, in
                                             " bytes, need " + std::to_string(one));
   if (reinterpret_cast<uintptr_t>(ws) & 255u)
     return fail(JERO_ERR_INVALID_ARGUMENT, "mla_prefill_attention: workspace must be 256-byte aligned");
-  int per = n_heads;
-  while (per > 1 && prefill_bytes(shape, total_len, size_t(per), planes) > workspace_bytes) per--;
-  const size_t rows_bytes = prefill_bytes(shape, total_len, size_t(per), planes);
-  void* const parts = workspace_bytes - rows_bytes >= flash_part_bytes(shape.vt) ? static_cast<uint8_t*>(ws) + rows_bytes
-                                                                                 : nullptr;
   const LatentCache c = mla_cache_of(cache, n_tokens);
+  auto heads_in = [&](size_t bytes) {
+    int n = n_heads;
+    while (n > 1 && prefill_bytes(shape, total_len, size_t(n), planes) > bytes) n--;
+    return n;
+  };
+  // heads at a time: those that fit beside the partial rows where such a call is cut into runs, else all that fit
+  const size_t part_bytes = flash_part_bytes(shape.vt);
+  const int longest = int(total_len < cache->max_len ? total_len : cache->max_len);
+  int per = heads_in(workspace_bytes >= one + part_bytes ? workspace_bytes - part_bytes : workspace_bytes);
+  if (flash_cut(int64_t(prefill_tiles(c)) * per, longest).runs == 1) per = heads_in(workspace_bytes);
+  const size_t rows_bytes = prefill_bytes(shape, total_len, size_t(per), planes);
+  void* const parts = workspace_bytes - rows_bytes >= part_bytes ? static_cast<uint8_t*>(ws) + rows_bytes : nullptr;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int wide = nope_dim + v_dim;
   for (int h0 = 0; h0 < n_heads; h0 += per) {

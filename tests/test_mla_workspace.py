@@ -40,3 +40,21 @@ def test_one_head_is_cut_into_runs_as_two_are(dev, act):
     assert torch.equal(got, both[:, :1])
     if act == "f32":  # (f16's rounding hides the order of the sums)
         assert not torch.equal(whole, both)
+
+
+@pytest.mark.gpu
+def test_heads_that_do_not_fit_at_once_leave_the_partial_rows_their_room(dev):
+    """A workspace of two heads' rows and of partial rows, for six heads: two at a time and cut, not all six in the
+    partial rows' place and not cut."""
+    p = Problem(81, [3000], [1], heads=6, block=64).device(dev)
+    want = p.run("expanded")
+    c = J.HipLatentCache.from_buffer_copy(p.cache.c)
+    L = J.lib()
+    two = L.jero_hip_mla_prefill_workspace_bytes(p.cache.ref, J.F32, 2, p.N, p.V, p.total())
+    got = p.run("expanded", workspace=torch.empty(two, dtype=torch.uint8, device=dev))
+    c.max_len = 1  # without partial rows
+    rows = L.jero_hip_mla_prefill_workspace_bytes(C.byref(c), J.F32, 6, p.N, p.V, p.total())
+    whole = p.run("expanded", workspace=torch.empty(rows, dtype=torch.uint8, device=dev))
+    torch.cuda.synchronize()
+    p.check(got)
+    assert torch.equal(got, want) and not torch.equal(whole, want)
