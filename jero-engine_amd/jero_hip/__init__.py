@@ -646,6 +646,7 @@ def mla_prefill_attention(out, q, cache, kv_b, total_len, scale, rope_theta, wor
     act, T, H, qs, os_ = _latent_args(what, out, q, cache, (kv_b,), V)
     N = q.shape[2] - cache.c.rope_dim
     _latent_check(kv_b.shape == (H, N + V, cache.rank), 14, what, "kv_b must be [heads, nope + v, rank]")
+    _latent_check(0 < total_len <= 1 << 23, 14, what, "total_len must be 1 to 2^23")  # (before its workspace is made)
     L, s = lib(), _latent_stream(cache, stream)
     ws, n = _latent_workspace(workspace, L.jero_hip_mla_prefill_workspace_bytes(cache.ref, act, H, N, V, total_len), q,
                               stream)

@@ -58,3 +58,12 @@ def test_heads_that_do_not_fit_at_once_leave_the_partial_rows_their_room(dev):
     torch.cuda.synchronize()
     p.check(got)
     assert torch.equal(got, want) and not torch.equal(whole, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("total", [-1, 0, (1 << 23) + 1, 1 << 40])
+def test_totals_are_refused_before_their_workspace_is_made(dev, total):
+    p = Problem(82, [20], [2]).device(dev)
+    with pytest.raises(J.K3Error) as ei:
+        p.run("expanded", total=total)
+    assert ei.value.variant == "TensorBoundsError"
