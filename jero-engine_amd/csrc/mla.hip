@@ -89,6 +89,8 @@ __global__ void __launch_bounds__(256) mla_append_kernel(LatentCache c, const X*
 // w + t: along the runs either w or t grows, so the number names the pair.
 
 constexpr int kMlaRuns = 256;  // workgroups of the attend kernel: one per CU, its tiles fill the LDS
+constexpr int kMlaTile = 32;   // positions a step
+constexpr int kMlaBegin = 3;   // what beginning an item takes, in steps
 
 struct MlaPlan {
   int* prefix;  // [T + 1] tiles before each token
@@ -163,8 +165,7 @@ static unsigned mla_head8_blocks(int nh, int per) { return unsigned((nh + 63) / 
 template <typename X, int NT>
 __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X* __restrict__ q, int64_t q_stride, int nh,
                                                          int nope, const _Float16* __restrict__ k_b, MlaRope rope,
-                                                         float scale, MlaQueries qa, MlaPlan plan, int tile, int extra,
-                                                         int share) {
+                                                         float scale, MlaQueries qa, MlaPlan plan, int share) {
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   if (blockIdx.x + 1 < gridDim.x) {
     int h, t0;
@@ -328,7 +329,7 @@ __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X*
         seq = -1;
       }
     }
-    const int mine = end > 0 && item == t ? (end + tile - 1) / tile + extra : 0;
+    const int mine = end > 0 && item == t ? (end + kMlaTile - 1) / kMlaTile + kMlaBegin : 0;
     int sum = mine;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -353,8 +354,8 @@ __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X*
   if (tid == 0) plan.prefix[c.n_tokens] = base;
 }
 
-// Units of a run: the plan's over the runs, at least `least` each.
-__device__ __forceinline__ int mla_per_run(int units, int runs, int least) { return max((units + runs - 1) / runs, least); }
+// Units of a run: the plan's over the runs.
+__device__ __forceinline__ int mla_per_run(int units, int runs) { return max((units + runs - 1) / runs, 1); }
 
 // The last token whose prefix is not behind tile x, 64 candidates at a time.
 __device__ __forceinline__ int mla_token_of(const int* prefix, int n, int x, int lane) {
@@ -371,9 +372,6 @@ __device__ __forceinline__ int mla_token_of(const int* prefix, int n, int x, int
   return lo;
 }
 
-// Positions a step: 32, and 32 for each wave where waves of two 16s of heads share the positions.
-static constexpr int attend_tile(int hw, int ks) { return hw > 1 ? 32 * ks : 32; }
-
 // Shape of the attend kernel: HG waves of 16 heads by KS waves of WR positions, RT + PT the padded widths,
 // KV the cache's type.  LDS holds a step's rows in f16, the latents and then the key parts, so that neither 8
 // rows' reads of one 16-byte chunk nor a transposing read's 32 bytes of 4 rows meet on a bank: rows of 1024
@@ -384,22 +382,23 @@ template <int RT, int PT, int HG, int HW, int KS, typename KV>
 struct AttendShape {
   static constexpr bool kWide = sizeof(KV) == 4;
   static constexpr int kWaves = HG * KS;
-  static constexpr int kTile = attend_tile(HW, KS);
+  static constexpr int kTile = kMlaTile;
   static constexpr int WR = kTile / KS;
   static constexpr int kRows = kTile / kWaves;  // rows a wave loads
   static constexpr bool kPad = RT == 512;
   static constexpr int kPitch = RT * 2 + (kPad ? 16 : 0);
   static constexpr int kLat = kTile * kPitch;
   static constexpr int kBuf = kLat + kTile * PT * 2;
-  static constexpr int kBufs = kWide ? 2 : HW > 1 ? 4 / KS : 4;
+  static constexpr int kBufs = kWide ? 2 : 4;
   static constexpr int kRaw = kWide ? kTile * (RT + PT) * 4 : 0;
-  static constexpr int kMerge = KS > 1 ? HG * HW * (KS - 1) * 16 * (RT + 4) * 4 : 0;  // over the buffers
+  static constexpr int kMerge = KS > 1 ? HG * (KS - 1) * 16 * (RT + 4) * 4 : 0;  // over the buffers
   static constexpr int kLds = kBufs * kBuf + kRaw > kMerge ? kBufs * kBuf + kRaw : kMerge;
   // loads of 1024 bytes a wave issues for a step: of the latents, of the key parts
   static constexpr int kLoadsLat = kRows * RT * int(sizeof(KV)) / 1024;
   static constexpr int kLoadsKey = (kRows * PT * int(sizeof(KV)) + 1023) / 1024;
   static constexpr int kLoads = kLoadsLat + kLoadsKey;
   static_assert(kRows % 8 == 0 && kLds <= 160 * 1024, "tile shape");
+  static_assert(HW == 1 || (KS == 1 && !kWide), "two 16s a wave have all positions of a step, and one part");
   __device__ static __forceinline__ constexpr int swap_lat(int r) { return kPad ? 0 : swap8(r); }
   __device__ static __forceinline__ constexpr int swap_key(int r) { return PT == 64 ? swap8(r) : swap4(r); }
   // byte of 16-byte chunk k (of the latent, or the key part) of row r
@@ -431,10 +430,10 @@ struct AttendShape {
 // of 32 positions, products 1090) and writing the partial rows (256 KB a workgroup of 128 heads, 14 us).
 template <int RT, int PT, int HG, int HW, int KS, typename KV, bool TWO>
 __global__ void __launch_bounds__(64 * HG * KS, 1)
-    mla_attend_kernel(LatentCache c, MlaQueries qa, int nh, int share, MlaPlan plan, int runs, int least, int extra,
+    mla_attend_kernel(LatentCache c, MlaQueries qa, int nh, int share, MlaPlan plan, int runs,
                       float* __restrict__ part_o, float2* __restrict__ part_ml) {
   using S = AttendShape<RT, PT, HG, HW, KS, KV>;
-  typedef std::conditional_t<S::kTile == 64, uint64_t, uint32_t> mask_t;
+  typedef uint32_t mask_t;  // a bit a position of a step
   constexpr mask_t ALL = ~mask_t(0);
   constexpr bool WIDE = S::kWide;
   constexpr int KT = (RT + PT) / 32, DT = RT / 16, RW = S::kRows, TR = S::kTile, WR = S::WR;
@@ -455,7 +454,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
   int t0 = 0;
   int w_prefix = plan.prefix[min(lane, n_tok)], w_seq = plan.seq[min(lane, n_tok - 1)], w_end = plan.end[min(lane, n_tok - 1)];
   const int tiles = plan.prefix[n_tok];
-  const int per = mla_per_run(tiles, runs, least);
+  const int per = mla_per_run(tiles, runs);
   int x = run * per;
   const int x_end = min(x + per, tiles);
   if (x >= x_end) return;
@@ -475,7 +474,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
   }
   for (; x < x_end && t < n_tok; t++) {
     if (t - t0 > 62) window(t);
-    const int first = __builtin_amdgcn_readlane(w_prefix, t - t0) + extra;  // unit of the token's first tile
+    const int first = __builtin_amdgcn_readlane(w_prefix, t - t0) + kMlaBegin;  // unit of the token's first tile
     const int last = min(__builtin_amdgcn_readlane(w_prefix, t - t0 + 1), x_end);
     x = max(x, first);
     if (last <= x) continue;  // a token without positions, or with none in this run
@@ -790,7 +789,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
     if constexpr (HW > 1) {
       // Two 16s of heads a wave, each operand read from LDS for both: products bound a step, not LDS, and the
       // softmax stands between them (registers hold no second step's scores)
-      static_assert(!WIDE && !TWO && NT == 2);
+      static_assert(!TWO && NT == 2);
       for (int i = 0; i < steps; i++) {
         if (AHEAD > 1 && i + AHEAD <= steps) dma_wait<(AHEAD - 1) * S::kLoads>();
         else dma_wait<0>();
@@ -944,34 +943,22 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
     const int64_t slot = run + mla_item(share, seq, t);
     if constexpr (KS > 1) {
       static_assert(KS == 2);
-      float* const s_o = reinterpret_cast<float*>(s_raw);
       constexpr int W = RT + 4;
-      auto place = [&](int w) { return s_o + (hgw * HW + w) * 16 * W + col * W; };
+      float* const at = reinterpret_cast<float*>(s_raw) + hgw * 16 * W + col * W;
       __syncthreads();
       if (kp) {
 #pragma unroll
-        for (int w = 0; w < HW; w++) {
-          float* to = place(w);
-#pragma unroll
-          for (int d = 0; d < DT; d++) *reinterpret_cast<f4_t*>(to + 16 * d + 4 * g) = o[w][d];
-          if (g == 0) to[RT] = m[w], to[RT + 1] = l[w];
-        }
+        for (int d = 0; d < DT; d++) *reinterpret_cast<f4_t*>(at + 16 * d + 4 * g) = o[0][d];
+        if (g == 0) at[RT] = m[0], at[RT + 1] = l[0];
       }
       __syncthreads();
       if (kp == 0) {
+        const float mt = fmaxf(m[0], at[RT]), top = mt == -INFINITY ? 0.f : mt;
+        const float a = __builtin_amdgcn_exp2f(m[0] - top), b = __builtin_amdgcn_exp2f(at[RT] - top);
+        l[0] = a * l[0] + b * at[RT + 1];
 #pragma unroll
-        for (int w = 0; w < HW; w++) {
-          const float* from = place(w);
-          const float mt = fmaxf(m[w], from[RT]), top = mt == -INFINITY ? 0.f : mt;
-          const float a = __builtin_amdgcn_exp2f(m[w] - top), b = __builtin_amdgcn_exp2f(from[RT] - top);
-          l[w] = a * l[w] + b * from[RT + 1];
-#pragma unroll
-          for (int d = 0; d < DT; d++) {
-            o[w][d] = a * o[w][d] + b * *reinterpret_cast<const f4_t*>(from + 16 * d + 4 * g);
-            if (HW > 1) asm volatile("" : "+a"(o[w][d]));
-          }
-          m[w] = mt;
-        }
+        for (int d = 0; d < DT; d++) o[0][d] = a * o[0][d] + b * *reinterpret_cast<const f4_t*>(at + 16 * d + 4 * g);
+        m[0] = mt;
       }
     }
 #pragma unroll
@@ -995,7 +982,7 @@ __global__ void __launch_bounds__(64 * HG * KS, 1)
 template <typename X, int RT, int TB>
 __global__ void __launch_bounds__(512) mla_values_kernel(LatentCache c, int nh, const float* __restrict__ part_o,
                                                          const float2* __restrict__ part_ml, MlaPlan plan, int runs,
-                                                         int least, int extra, int share,
+                                                         int share,
                                                          const _Float16* __restrict__ v_b, int v_dim, X* __restrict__ out, int64_t out_stride) {
   constexpr int KT = RT / 32, P = RT + 8, NW = 8, U = 4, WPT = TB < 8 ? 8 / TB : 1;
   __shared__ __attribute__((aligned(16))) _Float16 s_hi[16][P], s_lo[16][P];
@@ -1014,7 +1001,7 @@ __global__ void __launch_bounds__(512) mla_values_kernel(LatentCache c, int nh, 
     for (int i = 0; i < KT; i++) b[i] = *reinterpret_cast<const h8_t*>(w + min(32 * i + 8 * g, c.rank - 8));
   };
   weights(min(wv, vt - 1));
-  const int per = mla_per_run(plan.prefix[c.n_tokens], runs, least);
+  const int per = mla_per_run(plan.prefix[c.n_tokens], runs);
   const int r0 = min(8 * lane, c.rank - 8);
 
   // partials w0, w0 + by, ... below w1 of row `row` of item `item`, of which lane l holds elements 8l ..: sum,
@@ -1075,7 +1062,7 @@ __global__ void __launch_bounds__(512) mla_values_kernel(LatentCache c, int nh, 
     int w0 = 0, w1 = 0, first = t, item = t;
     if (t < c.n_tokens) {
       if (share > 1) first = plan.item[t], item = mla_item(share, plan.seq[t], first);
-      const int a = plan.prefix[first] + extra, e = plan.prefix[first + 1];
+      const int a = plan.prefix[first] + kMlaBegin, e = plan.prefix[first + 1];
       w0 = a / per;
       w1 = e > a ? (e - 1) / per + 1 : w0;
     }
@@ -1318,42 +1305,33 @@ static AbsorbedSpace absorbed_space(const jero_latent_cache* c, int64_t n_tokens
 }
 
 template <int RT, int PT, int HG, int HW, int KS, typename KV, bool TWO>
-static void launch_attend(const LatentCache& c, const MlaQueries& qa, int nh, int share, const MlaPlan& plan, int runs, int least,
-                          int extra, float* part_o, float2* part_ml, hipStream_t s) {
+static void launch_attend(const LatentCache& c, const MlaQueries& qa, int nh, int share, const MlaPlan& plan, int runs,
+                          float* part_o, float2* part_ml, hipStream_t s) {
   const int groups = (share * nh + 16 * HW * HG - 1) / (16 * HW * HG);
   hipLaunchKernelGGL((mla_attend_kernel<RT, PT, HG, HW, KS, KV, TWO>), dim3(unsigned(runs) * groups), dim3(64 * HG * KS),
-                     0, s, c, qa, nh, share, plan, runs, least, extra, part_o, part_ml);
+                     0, s, c, qa, nh, share, plan, runs, part_o, part_ml);
 }
 
 // Heads a workgroup: 16 by each of its 1, 2 or 4 waves' worth; with fewer than 4 others share the positions.
-// f16 activations, whose queries are one part, leave the registers for two 16s a wave from 33 heads on.
-struct AttendHeads {
-  int heads, tile;  // a workgroup's, and its positions a step
-};
-static AttendHeads attend_heads(int nh, bool one_part) {
-  if (nh <= 16) return {16, 32};
-  if (nh <= 32) return {32, 32};
-  if (!one_part) return {64, 32};
-  return nh <= 64 ? AttendHeads{64, 32} : AttendHeads{128, 32};
-}
+// f16 activations, whose queries are one part, leave the registers for two 16s a wave from 65 heads on.
+static int attend_heads(int nh, bool one_part) { return nh <= 16 ? 16 : nh <= 32 ? 32 : nh <= 64 || !one_part ? 64 : 128; }
 
 template <int RT, int PT, typename KV, bool TWO>
 static void launch_attend_heads(const LatentCache& c, const MlaQueries& qa, int nh, int share, const MlaPlan& plan, int runs,
-                                int least, int extra, float* part_o, float2* part_ml, hipStream_t s) {
-  const int heads = attend_heads(share * nh, !TWO).heads;
-  if (heads == 16) launch_attend<RT, PT, 1, 1, 2, KV, TWO>(c, qa, nh, share, plan, runs, least, extra, part_o, part_ml, s);
-  else if (heads == 32) launch_attend<RT, PT, 2, 1, 2, KV, TWO>(c, qa, nh, share, plan, runs, least, extra, part_o, part_ml, s);
-  else if constexpr (TWO) launch_attend<RT, PT, 4, 1, 1, KV, TWO>(c, qa, nh, share, plan, runs, least, extra, part_o, part_ml, s);
-  else if (heads == 64) launch_attend<RT, PT, 4, 1, 1, KV, TWO>(c, qa, nh, share, plan, runs, least, extra, part_o, part_ml, s);
-  else launch_attend<RT, PT, 4, 2, 1, KV, TWO>(c, qa, nh, share, plan, runs, least, extra, part_o, part_ml, s);
+                                float* part_o, float2* part_ml, hipStream_t s) {
+  const int heads = attend_heads(share * nh, !TWO);
+  if (heads == 16) launch_attend<RT, PT, 1, 1, 2, KV, TWO>(c, qa, nh, share, plan, runs, part_o, part_ml, s);
+  else if (heads == 32) launch_attend<RT, PT, 2, 1, 2, KV, TWO>(c, qa, nh, share, plan, runs, part_o, part_ml, s);
+  else if (heads == 64) launch_attend<RT, PT, 4, 1, 1, KV, TWO>(c, qa, nh, share, plan, runs, part_o, part_ml, s);
+  else if constexpr (!TWO) launch_attend<RT, PT, 4, 2, 1, KV, TWO>(c, qa, nh, share, plan, runs, part_o, part_ml, s);
 }
 
 template <int RT, int PT>
 static void launch_attend_types(bool f32_act, bool f32_kv, const LatentCache& c, const MlaQueries& qa, int nh,
-                                int share, const MlaPlan& plan, int runs, int least, int extra, float* part_o, float2* part_ml, hipStream_t s) {
-  if (f32_kv) launch_attend_heads<RT, PT, float, true>(c, qa, nh, share, plan, runs, least, extra, part_o, part_ml, s);
-  else if (f32_act) launch_attend_heads<RT, PT, _Float16, true>(c, qa, nh, share, plan, runs, least, extra, part_o, part_ml, s);
-  else launch_attend_heads<RT, PT, _Float16, false>(c, qa, nh, share, plan, runs, least, extra, part_o, part_ml, s);
+                                int share, const MlaPlan& plan, int runs, float* part_o, float2* part_ml, hipStream_t s) {
+  if (f32_kv) launch_attend_heads<RT, PT, float, true>(c, qa, nh, share, plan, runs, part_o, part_ml, s);
+  else if (f32_act) launch_attend_heads<RT, PT, _Float16, true>(c, qa, nh, share, plan, runs, part_o, part_ml, s);
+  else launch_attend_heads<RT, PT, _Float16, false>(c, qa, nh, share, plan, runs, part_o, part_ml, s);
 }
 
 }  // namespace jero
@@ -1399,14 +1377,13 @@ extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, i
   const _Float16 *kb = static_cast<const _Float16*>(k_b_dev), *vb = static_cast<const _Float16*>(v_b_dev);
   const bool f32 = act_dtype == JERO_F32;
   const int share = absorbed_share(cache, n_tokens, n_heads);
-  const AttendHeads ah = attend_heads(share * n_heads, !f32);
-  const int tile = ah.tile, groups = (share * n_heads + ah.heads - 1) / ah.heads;
-  const int runs = groups >= kMlaRuns / 8 ? 8 : kMlaRuns / groups / 8 * 8, least = 1, extra = 3;
+  const int heads = attend_heads(share * n_heads, !f32), groups = (share * n_heads + heads - 1) / heads;
+  const int runs = kMlaRuns / groups / 8 * 8;  // (groups: 16 at most)
 
   const dim3 ga(mla_head8_blocks(n_heads, int((n_tokens + 15) / 16)) + 1);
 #define JERO_ABSORB(X, NT)                                                                                         \
   hipLaunchKernelGGL((mla_absorb_kernel<X, NT>), ga, dim3(512), 0, s, c, static_cast<const X*>(q_dev), q_stride, n_heads, \
-                     nope_dim, kb, rope, scale, qa, plan, tile, extra, share)
+                     nope_dim, kb, rope, scale, qa, plan, share)
   if (nope_dim <= 128) {
     if (f32) JERO_ABSORB(float, 4);
     else JERO_ABSORB(_Float16, 4);
@@ -1419,11 +1396,11 @@ extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, i
 
   const bool wide = cache->kv_dtype == JERO_KV_F32;
   if (sp.rt == 128)
-    launch_attend_types<128, 32>(f32, wide, c, qa, n_heads, share, plan, runs, least, extra, part_o, part_ml, s);
+    launch_attend_types<128, 32>(f32, wide, c, qa, n_heads, share, plan, runs, part_o, part_ml, s);
   else if (sp.rt == 256)
-    launch_attend_types<256, 64>(f32, wide, c, qa, n_heads, share, plan, runs, least, extra, part_o, part_ml, s);
+    launch_attend_types<256, 64>(f32, wide, c, qa, n_heads, share, plan, runs, part_o, part_ml, s);
   else
-    launch_attend_types<512, 64>(f32, wide, c, qa, n_heads, share, plan, runs, least, extra, part_o, part_ml, s);
+    launch_attend_types<512, 64>(f32, wide, c, qa, n_heads, share, plan, runs, part_o, part_ml, s);
   if ((rc = check_launch("mla attend"))) return rc;
 
   // tokens a block: as many as leave 64 blocks or more, so that the weights are read seldom (21 tokens of 20 heads:
@@ -1431,7 +1408,7 @@ extern "C" int jero_hip_mla_absorbed_attention(const jero_latent_cache* cache, i
   const int64_t rows = n_tokens * n_heads;
 #define JERO_VALUES_TB(X, RT, TB)                                                                                    \
   hipLaunchKernelGGL((mla_values_kernel<X, RT, TB>), dim3(mla_head_blocks(n_heads, int((n_tokens + TB - 1) / TB))), \
-                     dim3(512), 0, s, c, n_heads, part_o, part_ml, plan, runs, least, extra, share, vb, v_dim,             \
+                     dim3(512), 0, s, c, n_heads, part_o, part_ml, plan, runs, share, vb, v_dim,                           \
                      static_cast<X*>(out_dev), out_stride)
 #define JERO_VALUES(X, RT)                                                                                       \
   if (n_tokens < 2 || rows < 256) JERO_VALUES_TB(X, RT, 1);                                                      \
