@@ -325,8 +325,8 @@ int jero_hip_gqa_attention(float *out_dev, const float *q_dev, const void *k_dev
  * cache, expanded keys and values have f16's range (to 65504, below 2^-14 to 2^-25 absolute; queries
  * any f32 range).  A numerator far below its row's largest is off by up to 2^-34 of that (2^-36 in
  * the expanded form): 2^20 such positions by 2^-14 of the row.  What attends to a row whose latent is
- * not finite, or in the expanded form one whose keys or values pass f16's range, is not finite; no
- * other token sees it.
+ * not finite, or in the expanded form one whose keys or values pass f16's range, is not finite; a key
+ * part that is not finite makes scores that are not.  No other token sees either.
  * At most 2^19 tokens, 2^19 sequences and, in the attentions, 1024 heads a call. */
 typedef struct jero_latent_cache {
   void *rows_dev;            /* [n_blocks][block_size][rank + rope_dim] of kv_dtype, 16-byte aligned */

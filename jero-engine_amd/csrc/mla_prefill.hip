@@ -6,6 +6,8 @@
 // sequence and a head over them.
 #include "mla.h"
 
+#include <type_traits>
+
 namespace jero {
 
 // Rows of the expanded keys and values: sequence s holds rows base(s) .. base(s) + min(lens[s],
@@ -33,6 +35,7 @@ __device__ __forceinline__ void mla_sequences(const LatentCache& c, int64_t tota
 // The expanded rows: NT, PT, VT the padded widths; each part a plane of f16.
 struct Expanded {
   _Float16 *k, *v, *p;  // [heads][total][NT], [heads][total][VT], [total][PT]
+  uint8_t* odd;                       // [heads][total][VT / 64]: 64 values with one past f16's range
   int64_t k_plane, v_plane, p_plane;  // to the lower parts
   int64_t total;
 };
@@ -138,7 +141,7 @@ __global__ void __launch_bounds__(64 * NW) mla_expand_kernel(LatentCache c, int 
   // The latents: a lane 8 values, up to 8 rows' loads at a time.  A row that is not finite gets keys of NaN, which make
   // NaN of every token that attends to it, and values of zeros, as tokens before it would take 0 * NaN from them.  A key
   // past f16's range is NaN too (minus infinity would drop its position; two parts, infinities of both signs, do not);
-  // such a value stays infinite.
+  // such a value stays infinite, and its 64 are marked.
   constexpr int RB = MP < 8 * NW ? MP / NW : 8;
   for (int r0 = wv; r0 < MP; r0 += NW * RB) {
     float v[RB][WIDE ? 8 : 1];
@@ -226,6 +229,15 @@ __global__ void __launch_bounds__(64 * NW) mla_expand_kernel(LatentCache c, int 
       if (row == -2) continue;
       const bool odd = row == -3;
       const float instead = key ? NAN : 0.f;
+      if (!key) {
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(acc[e / 4][j][e % 4]));
+        const uint64_t past = __ballot(!odd && !(top < 65520.f));
+        if (g == 0)
+          x.odd[(int64_t(h) * x.total + m0 + 16 * j + col) * (VT / 64) + (n0 - NT) / 64] =
+              ((past >> col) & 0x0001000100010001ull) != 0;
+      }
       _Float16* p = dst + (int64_t(h) * x.total + m0 + 16 * j + col) * width + n;
 #pragma unroll
       for (int half = 0; half < 2; half++) {
@@ -418,10 +430,14 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
     if (p0 + KR <= len) all(true);
     else all(false);
   };
-  // the block of a step's position lane
-  auto block = [&](int step) {
+  // the block of a step's position lane, and whether its values are marked
+  const uint8_t* const ob = x.odd + (int64_t(h) * x.total + base) * (VT / 64);
+  uint32_t ids = 0, marks = 0;
+  auto find = [&](int step) {
+    typedef std::conditional_t<VT == 64, uint8_t, std::conditional_t<VT == 128, uint16_t, uint32_t>> mark_t;
     const int p = min(step * KR + (lane & (KR - 1)), len - 1);
-    return uint32_t(table[p >> c.shift]);
+    ids = uint32_t(table[p >> c.shift]);
+    marks = reinterpret_cast<const mark_t*>(ob)[p];
   };
 
   f4_t o[2][DT];
@@ -439,51 +455,34 @@ __global__ void __launch_bounds__(256, (FlashShape<NT, PT, VT, TWO>::kGroups))
   for (int d = 0; d < 4; d++) vat[d] = vr * VT * 2 + 16 * ((2 * d + ((col & 3) >> 1)) ^ swap8(vr)) + 8 * (col & 1);
 
   if (steps > begin) load(begin, begin & 1);
-  uint32_t ids = steps > begin ? block(begin) : 0;
+  if (steps > begin) find(begin);
   for (int i = begin; i < steps; i++) {
     dma_wait<0>();
-    const uint64_t ok = __ballot(ids < c.n_blocks);  // (its load has come with the others: waited for before)
+    const uint64_t ok = __ballot(ids < c.n_blocks);  // (their loads have come with the others: waited for before)
+    const uint64_t odd = __ballot(marks != 0);
     __syncthreads();
     if (i + 1 < steps) {
       load(i + 1, (i + 1) & 1);
-      ids = block(i + 1);
+      find(i + 1);
     }
     const uint8_t* kv = s_kv + (i & 1) * S::kBuf;
     const int p0 = i * KR;
     // Rows of values past f16's range, of which a token that does not attend to them would take 0 * infinity, are made
-    // zeros, and their key parts NaN.  Every wave looks through all rows and finds the same (LDS is full: no word for it).
-    // 2048 f32 tokens of 32 heads take 175 us with this (expansion too) and 172.5 without, 4097 f16 of 128 1020 and 1006.
-    if (p0 + KR > common) {
-      constexpr int L = VT / 8, PER = 64 / L;  // lanes a row, rows a read
+    // zeros, and their key parts NaN.  (Looked for here, not marked when they were made: 1 to 2 % more.)
+    if (odd && p0 + KR > common) {
+      constexpr int L = VT / 8;  // lanes a row
       uint8_t* const rows = s_kv + (i & 1) * S::kBuf;
-      uint64_t odd = 0;
-      int id = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));  // the lane
-      asm volatile("" : "+v"(id));  // (what hangs on it is made here, not kept in registers over the loop)
-#pragma unroll 4
-      for (int k = 0; k < KR / PER; k++) {
-        typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
-        const h8_t v = *reinterpret_cast<const h8_t*>(rows + S::kKey + S::kRope + k * 1024 + 16 * id);
-        float sum = 0.f;  // of 0 * value
-#pragma unroll
-        for (int e = 0; e < 8; e += 2)
-          sum = __builtin_amdgcn_fdot2(h2_t{v[e], v[e + 1]}, h2_t{_Float16(0), _Float16(0)}, sum, false);
-        const uint64_t any = __ballot(sum != 0.f);
-        for (int r = 0; any && r < PER; r++)
-          if ((any >> (r * L)) & ((1ull << L) - 1)) odd |= 1ull << (k * PER + r);
-      }
-      if (odd) {
-        __syncthreads();
-        for (int r = wv; r < KR; r += 4)
-          if ((odd >> r) & 1) {
-            uint32_t z1 = 0u, nan1 = 0x7E007E00u;
-            asm volatile("" : "+v"(z1), "+v"(nan1));
-            const u32x4 z = {z1, z1, z1, z1}, nan = {nan1, nan1, nan1, nan1};
-            if (id < L * S::kPlanes)
-              *reinterpret_cast<u32x4*>(rows + S::kKey + S::kRope + (id / L) * S::kPlane + r * VT * 2 + 16 * (id % L)) = z;
-            if (id < PT / 8) *reinterpret_cast<u32x4*>(rows + S::kKey + r * PT * 2 + 16 * id) = nan;
-          }
-        __syncthreads();
-      }
+      uint32_t z1 = 0u, nan1 = 0x7E007E00u;
+      int id = lane;
+      asm volatile("" : "+v"(z1), "+v"(nan1), "+v"(id));  // (what hangs on these stays in here, out of the loop's registers)
+      const u32x4 z = {z1, z1, z1, z1}, nan = {nan1, nan1, nan1, nan1};
+      for (int r = wv; r < KR; r += 4)
+        if ((odd >> r) & 1) {
+          if (id < L * S::kPlanes)
+            *reinterpret_cast<u32x4*>(rows + S::kKey + S::kRope + (id / L) * S::kPlane + r * VT * 2 + 16 * (id % L)) = z;
+          if (id < PT / 8) *reinterpret_cast<u32x4*>(rows + S::kKey + r * PT * 2 + 16 * id) = nan;
+        }
+      __syncthreads();
     }
     f4_t s[2][RT];
     // operands are read a group of products ahead
@@ -692,7 +691,7 @@ static PrefillShape prefill_shape(int nope, int rope, int v) {
 static size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 static size_t prefill_bytes(const PrefillShape& s, int64_t total, size_t heads, int planes) {
   return up256(size_t(total) * s.pt * 2 * planes) + up256(heads * size_t(total) * s.nt * 2 * planes) +
-         up256(heads * size_t(total) * s.vt * 2 * planes);
+         up256(heads * size_t(total) * s.vt * 2 * planes) + up256(heads * size_t(total) * (s.vt / 64));
 }
 
 // Tiles of a call: a sequence's last may be short, so no more than this.
@@ -777,10 +776,10 @@ extern "C" size_t jero_hip_mla_prefill_workspace_bytes(const jero_latent_cache* 
   if (!cache || n_heads < 0 || nope_dim < 1 || v_dim < 1 || total_len < 1) return 0;
   const PrefillShape s = prefill_shape(nope_dim, cache->rope_dim, v_dim);
   const int planes = act_dtype == JERO_F16 ? 1 : 2;
-  const size_t one = prefill_bytes(s, total_len, 1, planes), head = size_t(total_len) * (s.nt + s.vt) * 2 * planes;
+  const size_t one = prefill_bytes(s, total_len, 1, planes), head = size_t(total_len) * ((s.nt + s.vt) * 2 * planes + s.vt / 64);
   if (n_heads == 0) return one;
   size_t heads = 1;
-  if (one < (size_t(1) << 30)) heads += ((size_t(1) << 30) - one) / (head + 512);
+  if (one < (size_t(1) << 30)) heads += ((size_t(1) << 30) - one) / (head + 768);
   // (a call whose positions may be cut into runs, with room for their partial rows)
   const int64_t longest = total_len < cache->max_len ? total_len : cache->max_len;
   return prefill_bytes(s, total_len, heads < size_t(n_heads) ? heads : size_t(n_heads), planes) +
@@ -846,6 +845,7 @@ extern "C" int jero_hip_mla_prefill_attention(const jero_latent_cache* cache, in
     x.k = reinterpret_cast<_Float16*>(at);
     at += up256(size_t(x.k_plane) * 2 * planes);
     x.v = reinterpret_cast<_Float16*>(at);
+    x.odd = at + up256(size_t(x.v_plane) * 2 * planes);
 #define JERO_PREFILL(NT, PT, VT, X, KV, TWO)                                                                      \
   rc = launch_prefill<NT, PT, VT, X, KV, TWO>(c, static_cast<const X*>(q_dev), q_stride, nh, h0, nope_dim, v_dim, w, x, \
                                               scale, rope, static_cast<X*>(out_dev), out_stride, parts, s)
