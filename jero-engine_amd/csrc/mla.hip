@@ -14,8 +14,8 @@ namespace jero {
 // VEC: the rows of x are 16-byte aligned, and are read so (stores always are: 8-element rows of the pool).  What
 // a row of some sequence needs is on its way before its place is looked up.
 //
-// Bound by its bytes, for a decode step by the launch: 16638 rows of 576 f16 values take 10.0 us (3.8 TB/s; a large
-// copy 4.6), 64 rows 3.9 us; one value a lane and load took 30 us.
+// Bound by its bytes, for a decode step by the launch: 16638 rows of 576 f16 values take 11.0 us (3.5 TB/s; a large
+// copy 4.6), 64 rows 3.3 us; one value a lane and load took 30 us.
 template <typename X, typename KV, bool VEC>
 __global__ void __launch_bounds__(256) mla_append_kernel(LatentCache c, const X* __restrict__ x, int64_t x_stride,
                                                          const float* __restrict__ norm, float eps, MlaRope rope) {
@@ -160,7 +160,7 @@ static unsigned mla_head8_blocks(int nh, int per) { return unsigned((nh + 63) / 
 
 // A block per head and 16 tokens, and one more for the plan.  The 8 waves take the head's rows of W_uk^T by 16; a
 // thread rotates a pair of the key part; the row's largest value is the scale of its parts.  Bound by the way of
-// one block's loads, a chain of memory latencies: 9.4 us for one token of 128 heads (16.8 MB of weights), 17 us for 64
+// one block's loads, a chain of memory latencies: 9.5 us for one token of 128 heads (16.8 MB of weights), 18 us for 64
 // (f16; the weights come from L2 for 16 tokens each).
 template <typename X, int NT>
 __global__ void __launch_bounds__(512) mla_absorb_kernel(LatentCache c, const X* __restrict__ q, int64_t q_stride, int nh,
@@ -420,12 +420,12 @@ struct AttendShape {
 //
 // HW 2 (f16 activations, more than 64 heads): two 16s of heads a wave, 128 a workgroup, so that each operand read
 // from LDS serves two products, and cache rows go to one workgroup, not two; a step's softmax then stands between
-// its products, as registers hold no second step's scores.  64 sequences of 100 to 4100 positions and 128 heads: 73 us
-// against 84 with one 16 a wave; one of 131073 positions: 62 against 74 (and 5 us more in mla_values_kernel, as there
+// its products, as registers hold no second step's scores.  64 sequences of 100 to 4100 positions and 128 heads: 78 us
+// against 86 with one 16 a wave; one of 131072 positions: 66 against 78 (and 4 to 5 us more in mla_values_kernel, as there
 // are twice the partial rows).  With 64 heads (two waves sharing positions) it took 99 us and is not used.
 //
-// Measured (512 + 64 wide): one token of 131072 positions, 128 heads, f32 activations: 92 us, 790 TFLOP/s of two-part
-// products; 32 sequences of 900 to 6000, 32 heads: 42 us, 3.0 TB/s.  Two-part products bound the first, the loads' and
+// Measured (512 + 64 wide): one token of 131072 positions, 128 heads, f32 activations: 98 us, 740 TFLOP/s of two-part
+// products; 32 sequences of 900 to 6000, 32 heads: 44 us, 2.9 TB/s.  Two-part products bound the first, the loads' and
 // steps' latencies with one wave a SIMD the second; with f16 activations LDS reads (one 16 a wave: 2300 cycles a step
 // of 32 positions, products 1090) and writing the partial rows (256 KB a workgroup of 128 heads, 14 us).
 template <int RT, int PT, int HG, int HW, int KS, typename KV, bool TWO>

@@ -47,8 +47,8 @@ struct Expanded {
 // consecutive columns of a position's row.  TWO: the results come out as two parts.  The last blocks copy the
 // key parts.
 //
-// Measured: 4097 positions of 512 for 128 heads of 128 + 128 (f16): 204 us, 674 TFLOP/s and 270 MB written; 2048 for
-// 32 heads, two parts: 37 us.  Bound by the products' issue and, with two parts, the rows written.  Steps before it:
+// Measured: 4097 positions of 512 for 128 heads of 128 + 128 (f16): 214 us, 640 TFLOP/s and 270 MB written; 2048 for
+// 32 heads, two parts: 41 us.  Bound by the products' issue and, with two parts, the rows written.  Steps before it:
 // tiles of both operands in LDS 300 us, latents kept 225, weights' lines read whole 204.
 template <typename KV>
 struct ExpandShape {
@@ -263,7 +263,7 @@ constexpr int kFlashRows = 128;  // tokens a workgroup: 32 a wave
 template <int NT, int PT, int VT, bool TWO>
 struct FlashShape {
   static constexpr int kPlanes = TWO ? 2 : 1;
-  // (64 positions where two workgroups' LDS holds them: 852 us for 4097 f16 tokens of 128 heads, by 32s 894)
+  // (64 positions where two workgroups' LDS holds them: 901 us for 4097 f16 tokens of 128 heads, by 32s 952)
   static constexpr int KR = NT + PT + VT <= 320 && !TWO ? 64 : 32;
   static constexpr int kKey = KR * NT * 2, kRope = KR * PT * 2, kVal = KR * VT * 2;
   static constexpr int kPlane = kKey + kRope + kVal;
@@ -324,8 +324,8 @@ __device__ __forceinline__ bool flash_tile(const LatentCache& c, int64_t total, 
 // Grid y: runs of `cut` steps; a tile of more than one leaves a partial row a token and run (part_o, part_ml),
 // which mla_flash_merge_kernel joins.
 //
-// Measured: 4097 tokens of 128 heads of 192 and 128 (f16): 857 us, 802 TFLOP/s of what the mask leaves; 2048 tokens of
-// 32 heads with two-part products (three for each): 148 us, 870 TFLOP/s of products.  Bound by the products and, half
+// Measured: 4097 tokens of 128 heads of 192 and 128 (f16): 850 to 900 us, 760 to 810 TFLOP/s of what the mask leaves;
+// 2048 tokens of 32 heads with two-part products (three for each): 162 us, 800 TFLOP/s of products.  Bound by the products and, half
 // as long, the softmax between them: 32 tokens a wave and two workgroups a CU let one's products run under the
 // other's softmax.
 template <int NT, int PT, int VT, typename X, bool TWO>
@@ -701,7 +701,7 @@ static int prefill_tiles(const LatentCache& c) {
 
 // Runs a tile's positions are cut into.  With fewer blocks than two a CU, cut so that about kFlashUnits
 // runs come out, none below kFlashLeast positions; the partial rows of at most kFlashParts blocks x runs.  Six chunks of
-// 17 to 600 tokens at the end of up to 2100 positions, 20 heads: 125 to 136 us and 13 for the merge, uncut 181; a
+// 17 to 600 tokens at the end of up to 2100 positions, 20 heads: 125 to 140 us and 13 for the merge, uncut 181; a
 // prompt of 500, 20 heads: 28 and 6, uncut 40 (runs of 512 the same as uncut, of 192 25 and 7; a prompt of 700 32 and 8,
 // by 512s 42 and 6, by 192s 34 and 9).
 constexpr int kFlashUnits = 768, kFlashLeast = 256, kFlashParts = 1280;
