@@ -321,6 +321,8 @@ __device__ __forceinline__ bool flash_tile(const LatentCache& c, int64_t total, 
 // K q^T (positions x tokens) leaves a token per lane column and, taken in the order 4g .. 4g + 3, 16 + 4g .. of
 // 32 positions, is the B operand of O^T += V^T p, V^T read from LDS transposed: numerators, factors and
 // accumulators of a token stay in its lanes.  Accumulators are rescaled only where a maximum grew by 2^kFlashGrow.
+// f16 activations: queries, keys, values and numerators are one part, and an output is off by 0.0004 of its size, its
+// own rounding 0.0002; as two parts (f32 activations have them) 4097 tokens of 128 heads take 2.3 ms in all against 1.1.
 // Grid y: runs of `cut` steps; a tile of more than one leaves a partial row a token and run (part_o, part_ml),
 // which mla_flash_merge_kernel joins.
 //
