@@ -133,8 +133,8 @@ def test_bits_do_not_hang_on_what_the_workspace_held(dev, heads, new, act, kv):
 @pytest.mark.parametrize("act,kv", TYPES)
 @pytest.mark.parametrize("peak", [0, 5000, 8192])
 @pytest.mark.parametrize("nats", [10.0, 13.0, 16.0, 17.375])
-@pytest.mark.parametrize("form", ["absorbed", "expanded"])
-def test_a_peak_over_thousands_of_small_numerators(dev, form, nats, peak, act, kv):
+@pytest.mark.parametrize("form,heads", [("absorbed", 1), ("absorbed", 20), ("absorbed", 40), ("absorbed", 70), ("expanded", 1)])
+def test_a_peak_over_thousands_of_small_numerators(dev, form, heads, nats, peak, act, kv):
     """One position of value 0, and 8192 of value 1 with scores `nats` below it, in one run: their small
     numerators add up to what is seen of them.
 
@@ -142,9 +142,9 @@ def test_a_peak_over_thousands_of_small_numerators(dev, form, nats, peak, act, k
     exponential's (nats 3 2^-24 + 2^-23), its parts' (2^-22, with f16 activations 2^-11), and, as f16 holds
     numerators 2^9 (expanded: 2^11) above their value, half its last place: 2^-34 (2^-36) of the peak.  The f32 sums
     of equal terms: 2^-24 a step of 32, for numerators and total."""
-    print(f"mla {form} {act} {kv}: peak at {peak}, {nats} nats", flush=True)
+    print(f"mla {form} {act} {kv} {heads} heads: peak at {peak}, {nats} nats", flush=True)
     n, T = 8192, 512 if form == "absorbed" else 1
-    p = Problem(51, [1], [1], heads=1, rank=64, rope=16, nope=8, v=8, act=act, kv=kv, block=256)
+    p = Problem(51, [1], [1], heads=heads, rank=64, rope=16, nope=8, v=8, act=act, kv=kv, block=256)
     p.lens, p.new, p.T, p.max_len = [n + 1] * T, [1] * T, T, n + 1
     p.n_blocks = 33
     rows = np.zeros((33 * 256, 80), p.rows.dtype)
@@ -155,9 +155,9 @@ def test_a_peak_over_thousands_of_small_numerators(dev, form, nats, peak, act, k
     p.table = np.repeat(np.arange(33, dtype=np.int32)[None], T, 0)
     p.starts = np.arange(T + 1, dtype=np.int32)
     p.wk[:], p.wv[:] = 0, 0
-    p.wk[0, 0, 0] = 1
-    p.wv[0, :, 1] = 1
-    p.q = np.zeros((T, 1, 24), p.q.dtype)
+    p.wk[:, 0, 0] = 1
+    p.wv[:, :, 1] = 1
+    p.q = np.zeros((T, heads, 24), p.q.dtype)
     p.q[..., 0] = 1
     p.scale = 1.0
     p.device(dev, starts=False)
@@ -176,3 +176,57 @@ def test_a_peak_over_thousands_of_small_numerators(dev, form, nats, peak, act, k
     far = exact * each + 2 * exact * (n / 32 + 64) * 2.0 ** -24 + exact * (2.0 ** -11 if half else 2.0 ** -22)
     print(f"  {np.abs(got - exact).max() / far:.3g} of {far / exact:.3g}", flush=True)
     assert (np.abs(got - exact) <= far).all()
+
+
+# ---------------------------------------------------------------- the largest calls
+
+
+@pytest.mark.parametrize("act,kv", TYPES)
+def test_the_most_heads(dev, act, kv):
+    print(f"mla {act} {kv} 1024 heads", flush=True)
+    p = Problem(53, [70, 33], [1, 2], heads=1024, nope=8, v=8, act=act, kv=kv, pad_rows=1).device(dev)
+    ref = p.attention()
+    for form in ("absorbed", "expanded"):
+        p.check(p.run(form), ref, form)
+
+
+@pytest.mark.parametrize("starts", [False, True])
+def test_the_most_tokens(dev, starts):
+    """2^19 sequences of a token each, of 0 to 2 positions over one block, whose 192 different rows repeat."""
+    print(f"mla append and absorbed, 2^19 sequences, starts {starts}", flush=True)
+    n, few = 1 << 19, 192
+    p = Problem(54, [2], [1], heads=1, nope=8, v=8, rank=8, rope=8)
+    p.lens, p.new, p.T = [i % 3 for i in range(few)], [1] * few, few
+    p.table = np.repeat(p.table, few, 0)
+    p.starts = np.arange(few + 1, dtype=np.int32)
+    p.q = np.random.default_rng(1).standard_normal((few, 1, 16)).astype(np.float32)
+    ref = p.attention()
+    p.device(dev, starts=starts)
+    p.check(p.run("absorbed"), ref, "few")
+    d = p.d
+    again = lambda t: t.repeat((n + few - 1) // few, *[1] * (t.dim() - 1))[:n].contiguous()  # noqa: E731
+    cache = J.LatentCache(d["rows"], again(d["table"]), again(d["lens"]), 8, max_len=p.max_len,
+                          starts=torch.arange(n + 1, dtype=torch.int32, device=dev) if starts else None)
+    out = torch.full((n, 1, 8), 7.0, device=dev)
+    J.mla_absorbed_attention(out, again(d["q"]), cache, d["k_b"], d["v_b"], p.scale, THETA)
+    torch.cuda.synchronize()
+    p.check(out[:few], ref, "first")
+    whole = out[:n // few * few].view(-1, few, 8)
+    assert torch.equal(whole, whole[:1].expand_as(whole)) and torch.equal(out[n // few * few:, 0], whole[0, :n % few])
+    # each token into a row of its own
+    rows = torch.zeros((n // 16, 16, 16), dtype=torch.float16, device=dev)
+    table = torch.arange(n, dtype=torch.int32, device=dev).view(-1, 1) // 16
+    lens = torch.arange(n, dtype=torch.int32, device=dev) % 16 + 1
+    x = torch.randn((n, 16), device=dev)
+    J.mla_append(J.LatentCache(rows, table, lens, 8, starts=cache.starts), x, None, 0.0, 0.0)
+    torch.cuda.synchronize()
+    assert torch.equal(rows.view(n, 16), x.half())
+
+
+def test_the_most_sequences_of_the_expanded_form(dev):
+    print("mla expanded, 4096 sequences", flush=True)
+    n = 4096
+    lens = [(37 * i) % 19 for i in range(n)]
+    p = Problem(55, lens, [min(L, 1 + i % 3) for i, L in enumerate(lens)], heads=1, nope=8, v=8, rank=8, rope=8, block=4,
+                pad_rows=1).device(dev)
+    p.check(p.run("expanded"), what="expanded")
