@@ -142,10 +142,10 @@ __device__ __forceinline__ float sum_over_groups(float v) {
 // a barrier then shows them to the others.
 __device__ __forceinline__ void dma_row(const void* row, uint32_t lane_bytes, uint32_t lds) {  // uniform row
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(lane_bytes), "s"(row)
-               : "memory", "m0");
+               : "memory");
 }
 __device__ __forceinline__ void dma_lanes(const void* p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
 }
 template <int N>
 __device__ __forceinline__ void dma_wait() {
