@@ -418,9 +418,10 @@ struct AttendShape {
 // of the next step's scores, operands are read from LDS a group of products ahead, and the rows two steps on are
 // on their way from the cache meanwhile (f16 cache; an f32 one has its LDS filled by the parts of one step).
 //
-// f16 activations: the queries and the numerators go in as one part.  An output is then off by 0.0004 of its size, where
-// its own rounding is 0.0002; as two parts (f32 activations have them) 64 sequences of 128 heads take 156 us in all
-// against 124.
+// f16 activations: the queries and the numerators go in as one part.  An output is then off by 0.00038 of its size, of
+// which its own rounding is 0.00021; 64 sequences of 128 heads take 122 us in all.  With queries of two parts (which
+// leave no registers for two 16s of heads a wave) it is 0.00026 and 144 us, with numerators of two parts as well
+// 0.00021 and 151; f32 activations are there for who needs them.
 //
 // HW 2 (f16 activations, more than 64 heads): two 16s of heads a wave, 128 a workgroup, so that each operand read
 // from LDS serves two products, and cache rows go to one workgroup, not two; a step's softmax then stands between
