@@ -382,6 +382,112 @@ int jero_hip_mla_prefill_attention(const jero_latent_cache *cache, int act_dtype
                                    int64_t total_len, float scale, float rope_theta, void *out_dev, int64_t out_stride,
                                    void *workspace_dev, size_t workspace_bytes, void *stream);
 
+/* ---- a serving step over a paged key/value cache ----
+ * What a program that serves many requests of a grouped-query model does beside its products: blocks
+ * for the step's tokens (jero_hip_paged_extend), their queries and keys rotated and stored
+ * (jero_hip_paged_append), attention (jero_hip_paged_attention), and, where a small model drafts
+ * tokens, which of them stand (jero_hip_verify_drafts).  Everything that changes from step to step is
+ * read on the device, so that a captured graph follows it from replay to replay.
+ *
+ * The cache is two pools, keys and values, of blocks of block_size positions, a position's row
+ * [n_heads_kv][head_dim]; a slot is a row's place in a pool, block * block_size + offset.  Sequence s
+ * has lens[s] positions with the call's tokens, the last of them, among them; its tokens are rows
+ * starts[s] .. starts[s + 1] - 1 of the call's (starts NULL: row s, one token each).
+ */
+
+/* Block tables and slots.  A request that asks for n = new[s] >= 0 tokens holds L = lens[s] - drop[s]
+ * positions (drop: tokens taken back, as verify_drafts refuses them) in the first owned[s] blocks of
+ * its table row, which stay its own; it needs max(0, ceil((L + n) / block_size) - owned[s]) more
+ * (none where n is 0).  A request with new[s] < 0 ends: its blocks from column shared_blocks on go
+ * back, in the order of requests and columns, onto the stack of free ids before any is taken, and its
+ * lens and owned become 0.  Blocks are then taken from the stack's top, in that order too.  A request
+ * is granted what it needs if the needs of all requests up to it are no more than what is free, and
+ * L + n positions fit its table row; another (granted 0) keeps L and its blocks, and its tokens'
+ * positions and slots are -1.
+ *   starts[s]     sum of max(new, 0) before s, granted or not (n_seqs + 1 of them)
+ *   positions[t]  L + t - starts[s] of token row t;  slots[t]: block * block_size + offset there, or -1
+ *                 for a block id outside [0, n_blocks)
+ *   rows from starts[n_seqs] on: -1, -1.  Rows from n_tokens on are not written.
+ * drop and granted may be NULL.  lens_out, owned_out and n_free_out may be NULL: in place.  Table
+ * entries and free ids that the call does not name stay.  Values out of range (owned beyond the row,
+ * n_free beyond the stack, drop beyond the length) count as the range's end.  Workspace:
+ * jero_hip_paged_extend_workspace_bytes(n_seqs), 16-byte aligned (NULL: library-owned, calls must not
+ * overlap on one device).  At most 2^19 sequences and 2^24 tokens; n_seqs * table_stride below 2^31. */
+typedef struct jero_block_pool {
+  int32_t *table_dev;       /* [n_seqs][table_stride] */
+  int32_t *lens_dev;        /* [n_seqs] */
+  int32_t *owned_dev;       /* [n_seqs] */
+  int32_t *free_dev;        /* [free_capacity], the first n_free[0] the free ids */
+  int32_t *n_free_dev;      /* [1] */
+  int32_t *lens_out_dev, *owned_out_dev, *n_free_out_dev; /* as the three they follow, or NULL */
+  int64_t n_seqs, table_stride, n_blocks, free_capacity, shared_blocks;
+  int block_size; /* a power of two up to 2^20 */
+} jero_block_pool;
+size_t jero_hip_paged_extend_workspace_bytes(int64_t n_seqs);
+int jero_hip_paged_extend(const jero_block_pool *pool, const int32_t *new_dev, const int32_t *drop_dev, int64_t n_tokens,
+                          int32_t *starts_dev, int32_t *granted_dev, int32_t *positions_dev, int64_t *slots_dev,
+                          void *workspace_dev, size_t workspace_bytes, void *stream);
+
+/* Rotary positions: pair i of a head's first rot_dim elements is turned by position * f_i, and scaled
+ * by magnitude.  f_i = theta^(-2i / rot_dim), for positions beyond those a model was trained on:
+ *   JERO_ROPE_LINEAR      f_i / factor
+ *   JERO_ROPE_NTK         theta * factor^(rot_dim / (rot_dim - 2)) in theta's place
+ *   JERO_ROPE_YARN        f_i / factor * r + f_i * (1 - r), r = (i - lo) / (hi - lo) within [0, 1], lo and hi the
+ *                         pairs (rounded down and up, within [0, rot_dim - 1]) that turn `high` and `low` times over
+ *                         original_len positions: rot_dim ln(original_len / (2 pi turns)) / (2 ln theta);
+ *                         magnitude 0.1 ln(factor) + 1
+ *   JERO_ROPE_WAVELENGTH  f_i / factor * (1 - r) + f_i * r, r = (original_len f_i / 2 pi - low) / (high - low) within
+ *                         [0, 1]
+ * low, high 0: 1 and 32 (YARN), 1 and 4 (WAVELENGTH).  Pairs are (i, i + rot_dim / 2) or (2i, 2i + 1).  rot_dim: a
+ * multiple of 8 up to 256.  The angle is computed in 64 bits.  A host call: the struct goes into others by value. */
+typedef enum jero_rope_layout { JERO_ROPE_HALF = 0, JERO_ROPE_INTERLEAVED = 1 } jero_rope_layout;
+typedef enum jero_rope_scaling {
+  JERO_ROPE_NONE = 0, JERO_ROPE_LINEAR = 1, JERO_ROPE_NTK = 2, JERO_ROPE_YARN = 3, JERO_ROPE_WAVELENGTH = 4
+} jero_rope_scaling;
+typedef struct jero_rope {
+  double turns[128]; /* f_i / 2 pi */
+  float magnitude;
+  int rot_dim, layout;
+} jero_rope;
+int jero_hip_rope_init(jero_rope *rope, int rot_dim, int layout, double theta, int scaling, double factor,
+                       double original_len, double low, double high);
+
+/* Rotates n_tokens tokens' queries into q_out (q itself, or memory apart from it) and their keys into the key pool, and
+ * stores their values: token row t, rows apart by the strides, [heads][head_dim] packed; positions[t] below 0: the token
+ * is left out; slots[t] outside [0, n_slots): its key and value are not stored.  No two tokens' slots may be the same.  q_norm /
+ * k_norm (f32 [head_dim], or NULL): heads are first RMS-normalised (f32, eps) with these weights.  rope NULL: not
+ * rotated.  q (n_heads 0) or keys and values (n_heads_kv 0) may be left out.  act_dtype JERO_F32 or JERO_F16, the pools'
+ * kv_dtype any of both; sums and rotations are f32, each result is rounded once.  head_dim: a multiple of 8 up to 256,
+ * at least rot_dim; strides multiples of 8 elements, pointers 16-byte aligned (positions 4, slots 8).  At most 2^24 tokens,
+ * 1024 heads. */
+int jero_hip_paged_append(int act_dtype, const void *q_dev, int64_t q_stride, const void *k_dev, int64_t k_stride,
+                          const void *v_dev, int64_t v_stride, int64_t n_tokens, int n_heads, int n_heads_kv, int head_dim,
+                          const int32_t *positions_dev, const int64_t *slots_dev, const jero_rope *rope,
+                          const float *q_norm_dev, const float *k_norm_dev, float eps, void *q_out_dev, int64_t q_out_stride,
+                          void *k_rows_dev, void *v_rows_dev, int kv_dtype, int64_t n_slots, void *stream);
+
+/* Drafted tokens against the target's probabilities, from given random numbers.  Sequence s has rows
+ * starts[s] .. starts[s + 1] - 1 of tokens_dev: the last token that stands, then n = rows - 1 drafted
+ * ones.  target_dev row t (f32, vocab of them, target_stride apart) holds the probabilities of the
+ * token after row t; draft_dev (f32, draft_stride apart) the draft's of each drafted token, those of
+ * sequence after sequence packed, as u_dev (f32, in [0, 1)) is.  Drafted token x stands if those before
+ * it do and u * draft[x] < target[x]; draft NULL: the draft gave it all of its probability, u <
+ * target[x].  The token after the last that stands is drawn with u_last[s]: the first whose running sum
+ * of weights w passes u_last * sum(w), w = max(target - draft, 0) where a drafted token was refused
+ * (target itself where that leaves nothing), else target; weights that are not finite count as 0, and
+ * a draw from none gives -1.  Products and sums are 64-bit.
+ *   out[t]       rows of s: the drafted tokens that stand, the token drawn, then -1
+ *   accepted[s]  drafted tokens that stand;  dropped[s] (or NULL): n less those, paged_extend's drop
+ * A sequence without rows gets 0, 0.  Rows outside [starts[0], starts[n_seqs]) stay.  A drafted token outside
+ * [0, vocab) is refused.  Workspace: jero_hip_verify_drafts_workspace_bytes(n_seqs, vocab), 16-byte aligned (NULL:
+ * library-owned, calls must not overlap on one device).  At most 65535 sequences, 2^22 tokens, a vocabulary of 2^24. */
+size_t jero_hip_verify_drafts_workspace_bytes(int64_t n_seqs, int64_t vocab);
+int jero_hip_verify_drafts(const float *target_dev, int64_t target_stride, const float *draft_dev, int64_t draft_stride,
+                           const int32_t *tokens_dev, const int32_t *starts_dev, const float *u_dev,
+                           const float *u_last_dev, int64_t n_seqs, int64_t n_tokens, int64_t n_drafts, int64_t vocab,
+                           int32_t *out_dev, int32_t *accepted_dev, int32_t *dropped_dev, void *workspace_dev,
+                           size_t workspace_bytes, void *stream);
+
 /* ---- routed experts ----
  * dispatch_qwen3_moe_ffn (src/qwen_deepseek.rs:847-951) from router logits, with
  * select_top_k_experts(logits, top_k, normalize = true) (src/gemma.rs:362-442) and

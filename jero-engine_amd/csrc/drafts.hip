@@ -1,0 +1,250 @@
+// drafts.hip -- drafted tokens accepted or replaced by given random numbers.
+#include "jero_common.h"
+#include "runtime.h"
+
+namespace jero {
+
+constexpr int kDraftChunk = 4096;  // of the vocabulary, a workgroup
+
+struct Drafts {
+  const float *target, *draft, *u, *u_last;
+  const int32_t *tokens, *starts;
+  int64_t target_stride, draft_stride;
+  int n_seqs, n_tokens, n_drafts, vocab, chunks;
+  int32_t *out, *accepted, *dropped;
+  double2* sums;  // [n_seqs][chunks]: of the weights, and of the target alone
+};
+
+// Where a sequence's next token is drawn from.
+struct Verdict {
+  int first, rows, accepted;
+  int row;       // of the target's probabilities; -1: no rows
+  int less;      // the draft's row taken off, or -1
+  int without;   // a token that gets no weight, or -1
+};
+
+// By a whole workgroup of whole waves; s_n: one int of LDS.  Each wave finds the same.
+__device__ __forceinline__ Verdict verdict_of(const Drafts& d, int s, int* s_n) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  Verdict v;
+  v.first = min(max(d.starts[s], 0), d.n_tokens);
+  v.rows = min(max(d.starts[s + 1], v.first), d.n_tokens) - v.first;
+  v.accepted = 0, v.row = v.less = v.without = -1;
+  // the drafted tokens of the sequences before
+  if (tid == 0) *s_n = 0;
+  __syncthreads();
+  int n = 0;
+  for (int i = tid; i < s; i += blockDim.x) n += max(d.starts[i + 1] - d.starts[i] - 1, 0);
+  n = group_sum_i<64>(n);
+  if (lane == 0 && n) atomicAdd(s_n, n);
+  __syncthreads();
+  const int before = *s_n;
+  if (v.rows < 1) return v;
+  const int drafted = max(min(v.rows - 1, d.n_drafts - before), 0);
+  int at = drafted;  // the first that is refused
+  for (int j0 = 0; j0 < drafted && at == drafted; j0 += kWave) {
+    const int j = j0 + lane;
+    bool good = true;
+    if (j < drafted) {
+      const int x = d.tokens[v.first + j + 1];
+      good = false;
+      if (x >= 0 && x < d.vocab) {
+        const double p = d.target[(v.first + j) * d.target_stride + x];
+        const double q = d.draft ? double(d.draft[(before + j) * d.draft_stride + x]) : 1.0;
+        good = double(d.u[before + j]) * q < p;
+      }
+    }
+    const uint64_t bad = __ballot(!good);
+    if (bad) at = j0 + __builtin_ctzll(bad);
+  }
+  v.accepted = at;
+  v.row = v.first + at;
+  if (at < drafted) {
+    if (d.draft) v.less = before + at;
+    else v.without = d.tokens[v.row + 1];
+  }
+  return v;
+}
+
+__device__ __forceinline__ double finite_weight(double w) { return w > 0.0 && w < 1e300 ? w : 0.0; }
+
+// The weight of token i: the target's probability less the draft's.
+__device__ __forceinline__ double weight_of(const Verdict& v, const float* p, const float* q, int i) {
+  const double w = p[i];
+  if (q) return finite_weight(w - double(q[i]));
+  return i == v.without ? 0.0 : finite_weight(w);
+}
+
+// Workgroup (chunk, sequence): the sums of its chunk's weights.
+__global__ void __launch_bounds__(256) draft_sums_kernel(Drafts d) {
+  __shared__ int s_n;
+  __shared__ double2 s_sum[4];
+  const int s = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const Verdict v = verdict_of(d, s, &s_n);
+  if (v.row < 0) return;
+  const int lo = blockIdx.x * kDraftChunk, hi = min(lo + kDraftChunk, d.vocab);
+  const float* p = d.target + v.row * d.target_stride;
+  const float* q = v.less >= 0 ? d.draft + v.less * d.draft_stride : nullptr;
+  double2 sum = {0.0, 0.0};
+#pragma unroll 4
+  for (int i = lo + tid; i < hi; i += 256) {
+    sum.x += weight_of(v, p, q, i);
+    sum.y += finite_weight(p[i]);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) sum.x += __shfl_xor(sum.x, off, kWave), sum.y += __shfl_xor(sum.y, off, kWave);
+  if (lane == 0) s_sum[tid >> 6] = sum;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < 4; w++) sum.x += s_sum[w].x, sum.y += s_sum[w].y;
+    d.sums[int64_t(s) * d.chunks + blockIdx.x] = sum;
+  }
+}
+
+// Inclusive sums over 1024 threads; s: 16 of LDS.
+__device__ __forceinline__ double scan1024(double v, double* s, int tid) {
+  const int lane = tid & 63;
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const double o = __shfl_up(v, off, kWave);
+    if (lane >= off) v += o;
+  }
+  __syncthreads();
+  if (lane == 63) s[tid >> 6] = v;
+  __syncthreads();
+  for (int w = 0; w < (tid >> 6); w++) v += s[w];
+  return v;
+}
+
+// Workgroup a sequence: finds the chunk, then the token in it, and writes the sequence's rows.
+__global__ void __launch_bounds__(1024) draft_pick_kernel(Drafts d) {
+  __shared__ int s_n, s_at, s_last;
+  __shared__ double s_scan[16], s_before, s_total;
+  const int s = blockIdx.x, tid = threadIdx.x;
+  Verdict v = verdict_of(d, s, &s_n);
+  if (tid == 0) {
+    d.accepted[s] = v.accepted;
+    if (d.dropped) d.dropped[s] = max(v.rows - 1, 0) - v.accepted;
+  }
+  if (v.row < 0) return;
+  const double2* sums = d.sums + int64_t(s) * d.chunks;
+  const float* p = d.target + v.row * d.target_stride;
+  const float* q = v.less >= 0 ? d.draft + v.less * d.draft_stride : nullptr;
+  bool alone = false;
+  double total = 0.0;
+  for (;;) {
+    double mine = 0.0;
+    for (int c = tid; c < d.chunks; c += 1024) mine += alone ? sums[c].y : sums[c].x;
+    mine = scan1024(mine, s_scan, tid);
+    if (tid == 1023) s_total = mine;
+    __syncthreads();
+    total = s_total;
+    if (total > 0.0 || alone) break;
+    alone = true, q = nullptr, v.without = -1;  // the draft takes off all there is
+  }
+  const double passes = double(d.u_last[s]) * total;
+  // the first chunk whose running sum passes, or the last of any weight
+  if (tid == 0) s_at = INT32_MAX, s_last = -1;
+  __syncthreads();
+  double carry = 0.0;
+  for (int c0 = 0; c0 < d.chunks; c0 += 1024) {
+    const int c = c0 + tid;
+    const double w = c < d.chunks ? (alone ? sums[c].y : sums[c].x) : 0.0;
+    const double run = carry + scan1024(w, s_scan, tid);
+    if (w > 0.0) {
+      if (run > passes) atomicMin(&s_at, c);
+      atomicMax(&s_last, c);
+    }
+    if (tid == 1023) s_total = run;
+    __syncthreads();
+    if (s_at == c || (s_at == INT32_MAX && s_last == c)) s_before = run - w;
+    carry = s_total;
+    if (s_at != INT32_MAX) break;
+    __syncthreads();
+  }
+  __syncthreads();
+  const int chunk = s_at != INT32_MAX ? s_at : s_last;
+  const double before = s_before;
+  __syncthreads();
+  int drawn = -1;
+  if (chunk >= 0) {
+    if (tid == 0) s_at = INT32_MAX, s_last = -1;
+    const int lo = chunk * kDraftChunk + 4 * tid, hi = min(min(lo + 4, (chunk + 1) * kDraftChunk), d.vocab);
+    double w[4] = {};
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      if (lo + e < hi) w[e] = weight_of(v, p, q, lo + e);
+    double run = scan1024(w[0] + w[1] + w[2] + w[3], s_scan, tid) - (w[0] + w[1] + w[2] + w[3]) + before;
+#pragma unroll
+    for (int e = 3; e >= 0; e--)
+      if (w[e] > 0.0) {
+        atomicMax(&s_last, lo + e);
+        break;
+      }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      run += w[e];
+      if (w[e] > 0.0 && run > passes) {
+        atomicMin(&s_at, lo + e);
+        break;
+      }
+    }
+    __syncthreads();
+    drawn = s_at != INT32_MAX ? s_at : s_last;
+  }
+  for (int i = tid; i < v.rows; i += 1024)
+    d.out[v.first + i] = i < v.accepted ? d.tokens[v.first + i + 1] : i == v.accepted ? drawn : -1;
+}
+
+}  // namespace jero
+
+using namespace jero;
+
+extern "C" size_t jero_hip_verify_drafts_workspace_bytes(int64_t n_seqs, int64_t vocab) {
+  if (n_seqs < 1 || n_seqs > 65535 || vocab < 1 || vocab > (1 << 24)) return 0;
+  return size_t(n_seqs) * size_t((vocab + kDraftChunk - 1) / kDraftChunk) * sizeof(double2);
+}
+
+extern "C" int jero_hip_verify_drafts(const float* target_dev, int64_t target_stride, const float* draft_dev,
+                                      int64_t draft_stride, const int32_t* tokens_dev, const int32_t* starts_dev,
+                                      const float* u_dev, const float* u_last_dev, int64_t n_seqs, int64_t n_tokens,
+                                      int64_t n_drafts, int64_t vocab, int32_t* out_dev, int32_t* accepted_dev,
+                                      int32_t* dropped_dev, void* workspace_dev, size_t workspace_bytes, void* stream) {
+  auto bad = [](int status, const char* what) { return fail(status, std::string("verify_drafts: ") + what); };
+  if (!target_dev || !tokens_dev || !starts_dev || !u_last_dev || !out_dev || !accepted_dev || (n_drafts > 0 && !u_dev))
+    return bad(JERO_ERR_INVALID_ARGUMENT, "null pointer");
+  for (const void* p : {static_cast<const void*>(target_dev), static_cast<const void*>(draft_dev),
+                        static_cast<const void*>(tokens_dev), static_cast<const void*>(starts_dev),
+                        static_cast<const void*>(u_dev), static_cast<const void*>(u_last_dev),
+                        static_cast<const void*>(out_dev), static_cast<const void*>(accepted_dev),
+                        static_cast<const void*>(dropped_dev)})
+    if (!aligned4(p)) return bad(JERO_ERR_INVALID_ARGUMENT, "arrays must be 4-byte aligned");
+  if (n_seqs < 1 || n_tokens < 1 || vocab < 1 || n_drafts < 0 || n_drafts >= n_tokens)
+    return bad(JERO_ERR_TENSOR_BOUNDS, "no sequences, tokens or vocabulary, or as many drafts as tokens");
+  if (n_seqs > 65535 || n_tokens > (1 << 22) || vocab > (1 << 24))
+    return bad(JERO_ERR_TENSOR_BOUNDS, "more than 65535 sequences, 2^22 tokens or a vocabulary of 2^24");
+  if (target_stride < vocab || (draft_dev && draft_stride < vocab))
+    return bad(JERO_ERR_TENSOR_BOUNDS, "rows overlap: a stride is below the vocabulary");
+  const size_t need = jero_hip_verify_drafts_workspace_bytes(n_seqs, vocab);
+  if (!workspace_dev) {
+    if (int rc = workspace(need, &workspace_dev)) return rc;
+  } else if (workspace_bytes < need) {
+    return bad(JERO_ERR_TENSOR_BOUNDS, "the workspace is too small");
+  } else if (reinterpret_cast<uintptr_t>(workspace_dev) & 15u) {
+    return bad(JERO_ERR_INVALID_ARGUMENT, "the workspace must be 16-byte aligned");
+  }
+  Drafts d{};
+  d.target = target_dev, d.draft = draft_dev, d.u = u_dev, d.u_last = u_last_dev;
+  d.tokens = tokens_dev, d.starts = starts_dev;
+  d.target_stride = target_stride, d.draft_stride = draft_stride;
+  d.n_seqs = int(n_seqs), d.n_tokens = int(n_tokens), d.n_drafts = int(n_drafts), d.vocab = int(vocab);
+  d.chunks = (d.vocab + kDraftChunk - 1) / kDraftChunk;
+  d.out = out_dev, d.accepted = accepted_dev, d.dropped = dropped_dev;
+  d.sums = static_cast<double2*>(workspace_dev);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid = {unsigned(d.chunks), unsigned(n_seqs), 1};
+  hipLaunchKernelGGL(draft_sums_kernel, grid, dim3(256), 0, s, d);
+  if (int rc = check_launch("verify_drafts sums")) return rc;
+  hipLaunchKernelGGL(draft_pick_kernel, dim3(unsigned(n_seqs)), dim3(1024), 0, s, d);
+  return check_launch("verify_drafts");
+}

@@ -82,6 +82,14 @@ _SIGS = {
     "jero_hip_mla_prefill_workspace_bytes": (_SZ, [_P, _I32, _I32, _I32, _I32, _I64]),
     "jero_hip_mla_prefill_attention": (_I32, [_P, _I32, _P, _I64, _I64, _I32, _I32, _I32, _P, _I64, _F, _F, _P, _I64, _P,
                                               _SZ, _P]),
+    "jero_hip_paged_extend_workspace_bytes": (_SZ, [_I64]),
+    "jero_hip_paged_extend": (_I32, [_P, _P, _P, _I64, _P, _P, _P, _P, _P, _SZ, _P]),
+    "jero_hip_rope_init": (_I32, [_P, _I32, _I32, C.c_double, _I32, C.c_double, C.c_double, C.c_double, C.c_double]),
+    "jero_hip_paged_append": (_I32, [_I32, _P, _I64, _P, _I64, _P, _I64, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P, _F,
+                                     _P, _I64, _P, _P, _I32, _I64, _P]),
+    "jero_hip_verify_drafts_workspace_bytes": (_SZ, [_I64, _I64]),
+    "jero_hip_verify_drafts": (_I32, [_P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _SZ,
+                                      _P]),
     "jero_hip_moe_ffn": (_I32, [_P, _P, _I64, _I64, _I32, _I32, _P, _SZ, _I32, _P, _SZ, _I32, _P, _SZ, _I64, _I64,
                                 _P, _P, _P, _P, _SZ, _P]),
     "jero_hip_moe_workspace_bytes": (_SZ, [_I64, _I64, _I32, _I64, _I64]),
@@ -653,6 +661,204 @@ def mla_prefill_attention(out, q, cache, kv_b, total_len, scale, rope_theta, wor
     check(L.jero_hip_mla_prefill_attention(cache.ref, act, q.data_ptr(), qs, T, H, N, V, kv_b.data_ptr(), total_len,
                                            scale, rope_theta, out.data_ptr(), os_, ws.data_ptr(), n, s))
     return out
+
+
+class HipBlockPool(C.Structure):
+    """jero_block_pool."""
+    _fields_ = [(n, C.c_void_p) for n in ("table_dev", "lens_dev", "owned_dev", "free_dev", "n_free_dev", "lens_out_dev",
+                                          "owned_out_dev", "n_free_out_dev")] + \
+               [(n, C.c_int64) for n in ("n_seqs", "table_stride", "n_blocks", "free_capacity", "shared_blocks")] + \
+               [("block_size", C.c_int)]
+
+
+def _paged_stream(device, stream):
+    """The stream's handle; a call runs on the current device, which has to be the tensors'."""
+    import torch
+    _latent_check(device.index == torch.cuda.current_device(), 21, "the tensors must be on the current device")
+    _latent_check(stream is None or stream.device == device, 21, "the stream must be of the tensors' device")
+    return _stream(stream)
+
+
+def _paged_ints(what, name, t, device, count=None, dtype=None):
+    """Address of a packed integer array of `count` elements (None: any) on the device."""
+    import torch
+    dtype = dtype or torch.int32
+    if t.dtype is not dtype or t.device != device or not t.is_contiguous() or (count is not None and t.numel() != count):
+        _latent_check(t.device == device, 21, f"{what}: {name} must be on the same GPU as the others")
+        _latent_check(t.dtype is dtype and t.is_contiguous(), 21, f"{what}: {name} must be packed {dtype}")
+        _latent_check(False, 14, f"{what}: {name} must have {count} elements")
+    return t.data_ptr()
+
+
+class BlockPool:
+    """What a server keeps of its requests' blocks from step to step (jero_block_pool): ``table`` [n_seqs, blocks]
+    int32 block ids, ``lens`` and ``owned`` [n_seqs] int32 positions and blocks of each request, ``free`` int32, a
+    stack of free ids of which the first ``n_free`` [1] int32 are there; n_blocks, the pool's blocks, of block_size
+    positions.  The first shared_blocks blocks of a request are shared with others and not given back.  Device
+    tensors, held; a request is admitted by writing its owned, lens and shared blocks."""
+
+    def __init__(self, table, lens, owned, free, n_free, n_blocks, block_size, shared_blocks=0):
+        _latent_check(table.is_cuda and table.dim() == 2, 21, "BlockPool: table must be [n_seqs, blocks], on a GPU")
+        (n, cols), device = table.shape, table.device
+        ints = _paged_ints
+        self.table, self.lens, self.owned, self.free, self.n_free = table, lens, owned, free, n_free
+        self.c = HipBlockPool(ints("BlockPool", "table", table, device), ints("BlockPool", "lens", lens, device, n),
+                              ints("BlockPool", "owned", owned, device, n), ints("BlockPool", "free", free, device),
+                              ints("BlockPool", "n_free", n_free, device, 1), None, None, None, n, cols, n_blocks,
+                              free.numel(), shared_blocks, block_size)
+
+
+def paged_extend(pool, new, positions, slots, starts, drop=None, granted=None, into=None, workspace=None, stream=None):
+    """Blocks, positions and slots of a step's tokens (jero_hip_paged_extend): ``new`` [n_seqs] int32 tokens of each
+    request (below 0: it ends), ``drop`` [n_seqs] int32 positions taken back first, or None.  Writes the pool's
+    table and free ids, ``starts`` [n_seqs + 1] int32, ``positions`` int32 and ``slots`` int64 of the call's token
+    rows (-1 behind the last), ``granted`` [n_seqs] int32 or None, and lens, owned and n_free in place, or
+    ``into`` three tensors like them."""
+    import torch
+    what, c, device = "paged_extend", pool.c, pool.table.device
+    n, T = c.n_seqs, positions.numel()
+    ints = _paged_ints
+    if into is not None:
+        d = HipBlockPool()
+        C.memmove(C.byref(d), C.byref(c), C.sizeof(d))
+        d.lens_out_dev = ints(what, "lens", into[0], device, n)
+        d.owned_out_dev = ints(what, "owned", into[1], device, n)
+        d.n_free_out_dev = ints(what, "n_free", into[2], device, 1)
+        c = d
+    s = _paged_stream(device, stream)
+    L = lib()
+    ws, size = _latent_workspace(workspace, L.jero_hip_paged_extend_workspace_bytes(n), positions, stream) \
+        if workspace is not None or n > 1024 or T > 4096 else (None, 0)
+    check(L.jero_hip_paged_extend(C.byref(c), ints(what, "new", new, device, n),
+                                  None if drop is None else ints(what, "drop", drop, device, n), T,
+                                  ints(what, "starts", starts, device, n + 1),
+                                  None if granted is None else ints(what, "granted", granted, device, n),
+                                  ints(what, "positions", positions, device), ints(what, "slots", slots, device, T, torch.int64),
+                                  None if ws is None else ws.data_ptr(), size, s))
+
+
+class HipRope(C.Structure):
+    """jero_rope."""
+    _fields_ = [("turns", C.c_double * 128), ("magnitude", C.c_float), ("rot_dim", C.c_int), ("layout", C.c_int)]
+
+
+class Rope:
+    """A model's rotation (jero_hip_rope_init): pairs of a head's first rot_dim elements, ``layout`` "half" (i, i +
+    rot_dim / 2) or "interleaved" (2i, 2i + 1), turned by position * theta^(-2i / rot_dim), scaled for contexts
+    beyond ``original`` positions as ``scaling`` says: "none", "linear", "ntk", "yarn" or "wavelength"."""
+    LAYOUTS = {"half": 0, "interleaved": 1}
+    SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "wavelength": 4}
+
+    def __init__(self, rot_dim, theta, layout="half", scaling="none", factor=1.0, original=0, low=0.0, high=0.0):
+        _latent_check(layout in self.LAYOUTS, 10, f"Rope: unknown layout {layout!r}")
+        _latent_check(scaling in self.SCALINGS, 10, f"Rope: unknown scaling {scaling!r}")
+        self.c = HipRope()
+        check(lib().jero_hip_rope_init(C.byref(self.c), rot_dim, self.LAYOUTS[layout], theta, self.SCALINGS[scaling], factor,
+                                       original, low, high))
+        self.ref = C.byref(self.c)
+
+
+def _paged_rows(what, name, t, like, heads_dim=None):
+    """Stride of a [tokens, heads, head_dim] tensor whose tokens' heads are packed."""
+    shape, stride = t.shape, t.stride()
+    _latent_check(t.dtype is like.dtype and t.device == like.device, 21, what, f"{name} differs in type or device")
+    _latent_check(len(shape) == 3 and shape[0] == like.shape[0] and shape[2] == like.shape[2], 14, what,
+                  f"{name} must be [tokens, heads, head_dim]")
+    T, H, D = shape
+    _latent_check((D == 1 or stride[2] == 1) and (H == 1 or stride[1] == D), 21, what, f"{name}: a token's heads must be packed")
+    return stride[0] if T > 1 else H * D
+
+
+def _paged_act(what, t):
+    import torch
+    _latent_check(t.is_cuda, 21, what, "the tensors must be on a GPU")
+    if t.dtype is torch.float32:
+        return F32
+    _latent_check(t.dtype is torch.float16, 10, what, "activations must be float32 or float16")
+    return F16
+
+
+def _paged_norm(what, name, w, like):
+    import torch
+    if w is None:
+        return None
+    _latent_check(w.dtype is torch.float32 and w.device == like.device and w.is_contiguous()
+                  and w.numel() == like.shape[2], 14, what, f"{name} must be head_dim packed float32 values")
+    return w.data_ptr()
+
+
+def paged_append(k_rows, v_rows, q_out, q, k, v, positions, slots, rope, q_norm=None, k_norm=None, eps=1e-6, stream=None):
+    """Rotates a step's queries and keys to their positions and stores keys and values (jero_hip_paged_append): q
+    [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim] f32 or f16 (tokens may be apart) into q_out
+    (q itself, or apart from it) and the pools k_rows, v_rows [..., kv_heads, head_dim] f32 or f16, whose rows
+    ``slots`` [tokens] int64 counts; ``positions`` [tokens] int32.  A token of a position below 0 is left out, one
+    of a slot that is none is not stored.  ``q_norm``, ``k_norm`` [head_dim] f32: heads are RMS-normalised first."""
+    import torch
+    what, device = "paged_append", k.device
+    act = _paged_act(what, k)
+    T, KV, D = k.shape if k.dim() == 3 else (0, 0, 0)
+    _latent_check(q.shape[1:2] != (0,), 14, what, "q has no heads")
+    ks, vs = _paged_rows(what, "k", k, k), _paged_rows(what, "v", v, k)
+    qs, qo = _paged_rows(what, "q", q, k), _paged_rows(what, "q_out", q_out, k)
+    _latent_check(v.shape == k.shape and q_out.shape == q.shape, 14, what, "k and v, or q and q_out, differ in shape")
+    kd = k_rows.dtype
+    _latent_check(kd in (torch.float32, torch.float16), 10, what, "the pools must be float32 or float16")
+    for rows in (k_rows, v_rows):
+        _latent_check(rows.dtype is kd and rows.device == device and rows.is_contiguous() and rows.shape == k_rows.shape
+                      and rows.dim() >= 3 and rows.shape[-2:] == (KV, D), 14, what,
+                      "the pools must be packed [..., kv_heads, head_dim], of one type, on the tokens' GPU")
+    s = _paged_stream(device, stream)
+    check(lib().jero_hip_paged_append(
+        act, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, T, q.shape[1], KV, D,
+        _paged_ints(what, "positions", positions, device, T), _paged_ints(what, "slots", slots, device, T, torch.int64),
+        None if rope is None else rope.ref, _paged_norm(what, "q_norm", q_norm, k), _paged_norm(what, "k_norm", k_norm, k),
+        eps, q_out.data_ptr(), qo, k_rows.data_ptr(), v_rows.data_ptr(), KV_F16 if kd is torch.float16 else KV_F32,
+        k_rows.numel() // (KV * D), s))
+
+
+def rope(out, x, positions, rope, norm=None, eps=1e-6, stream=None):
+    """The rotation alone: x [tokens, heads, head_dim] f32 or f16 into out (x itself, or apart from it), as
+    paged_append rotates queries."""
+    what = "rope"
+    act = _paged_act(what, x)
+    xs, os_ = _paged_rows(what, "x", x, x), _paged_rows(what, "out", out, x)
+    _latent_check(out.shape == x.shape, 14, what, "x and out differ in shape")
+    T, H, D = x.shape
+    s = _paged_stream(x.device, stream)
+    check(lib().jero_hip_paged_append(act, x.data_ptr(), xs, None, 0, None, 0, T, H, 0, D,
+                                      _paged_ints(what, "positions", positions, x.device, T), None, rope.ref,
+                                      _paged_norm(what, "norm", norm, x), None, eps, out.data_ptr(), os_, None, None, KV_F16,
+                                      0, s))
+    return out
+
+
+def verify_drafts(out, accepted, target, draft, tokens, starts, u, u_last, dropped=None, workspace=None, stream=None):
+    """Which drafted tokens stand, and the token that follows (jero_hip_verify_drafts): ``tokens`` [tokens] int32, a
+    sequence's last token and its drafted ones in rows starts[s] .. starts[s + 1] - 1 (``starts`` [n_seqs + 1]
+    int32); ``target`` [tokens, vocab] f32 probabilities after each row, ``draft`` [drafts, vocab] f32 the draft's of
+    each drafted token, sequence after sequence (None: it was sure of each); ``u`` [drafts] and ``u_last``
+    [n_seqs] f32 numbers from [0, 1).  Writes ``out`` [tokens] int32, the tokens that stand, the one drawn, -1s;
+    ``accepted`` and ``dropped`` (or None) [n_seqs] int32."""
+    import torch
+    what, device = "verify_drafts", target.device
+    n, T, f32 = starts.numel() - 1, tokens.numel(), torch.float32
+    _latent_check(target.is_cuda and target.dtype is f32 and target.dim() == 2 and target.shape[0] == T
+                  and target.stride(1) == 1, 14, what, "target must be [tokens, vocab] float32 with packed rows, on a GPU")
+    V, N = target.shape[1], u.numel()
+    if draft is not None:
+        _latent_check(draft.device == device and draft.dtype is f32 and draft.shape == (N, V)
+                      and (N == 0 or draft.stride(1) == 1), 14, what, "draft must be [drafts, vocab] float32 with packed rows")
+    ints = _paged_ints
+    s = _paged_stream(device, stream)
+    L = lib()
+    ws, size = _latent_workspace(workspace, L.jero_hip_verify_drafts_workspace_bytes(n, V), target, stream)
+    check(L.jero_hip_verify_drafts(
+        target.data_ptr(), target.stride(0) if T > 1 else V, None if draft is None or N == 0 else draft.data_ptr(),
+        V if draft is None or N < 2 else draft.stride(0), ints(what, "tokens", tokens, device, T),
+        ints(what, "starts", starts, device, n + 1), ints(what, "u", u, device, N, f32) if N else None,
+        ints(what, "u_last", u_last, device, n, f32), n, T, N, V, ints(what, "out", out, device, T),
+        ints(what, "accepted", accepted, device, n), None if dropped is None else ints(what, "dropped", dropped, device, n),
+        ws.data_ptr(), size, s))
 
 
 def dispatch_qwen3_moe_ffn(out, norm_ffn_in, router_logits, top_k, gate, up, down, workspace=None, stream=None,
