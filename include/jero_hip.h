@@ -466,6 +466,42 @@ int jero_hip_paged_append(int act_dtype, const void *q_dev, int64_t q_stride, co
                           const float *q_norm_dev, const float *k_norm_dev, float eps, void *q_out_dev, int64_t q_out_stride,
                           void *k_rows_dev, void *v_rows_dev, int kv_dtype, int64_t n_slots, void *stream);
 
+/* Attention of a batch that may share its first positions: token row t of sequence s attends causally,
+ * out = sum_j softmax_j(scale * q . k_j) v_j over positions j up to its own, queries and keys rotated
+ * before (paged_append).  The first shared_blocks blocks of every sequence are those of shared_dev: rows of all
+ * sequences go over them together, so that they are read once for many; table rows hold the blocks behind them at
+ * their columns (columns below shared_blocks are not read).
+ *   - Token rows before starts[0] and from starts[n_seqs] on belong to no sequence: not read, not written.
+ *   - A token whose position is below 0 (a sequence of more tokens than positions) gets zeros, as one gets that
+ *     sees no block.
+ *   - Positions from max_len on, and those of a block id outside [0, n_blocks), are not attended to.
+ * q_dev: [n_tokens][n_heads][head_dim] of act_dtype JERO_F32 or JERO_F16 (f16 needs an f16 cache), rows q_stride
+ * apart; out_dev like it, apart from the inputs.  head_dim: a multiple of 8 up to 256; n_heads a multiple of n_heads_kv;
+ * strides multiples of 8 elements, 16-byte aligned.  Sums are f32; with f32 activations the products carry 22 bits of each
+ * f32 factor (two f16 parts), with f16 activations softmax numerators are rounded to f16.  So keys and values of an f32
+ * cache have f16's range (to 65504, below 2^-14 to 2^-25 absolute); queries any f32 range.  A numerator far below its row's
+ * largest is off by up to 2^-36 of that.  What attends to a value that is not finite is not finite, which others do not see.
+ * Workspace: jero_hip_paged_attention_workspace_bytes(...), 256-byte aligned (NULL: library-owned, calls must not
+ * overlap on one device).  At most 2^19 tokens, 2^19 sequences, 1024 heads and n_tokens * n_heads 2^25. */
+typedef struct jero_paged_cache {
+  const void *k_dev, *v_dev;  /* [n_blocks][block_size][n_heads_kv][head_dim] of kv_dtype, 16-byte aligned */
+  const int32_t *table_dev;   /* [n_seqs][table_stride] block ids */
+  const int32_t *lens_dev;    /* [n_seqs] */
+  const int32_t *starts_dev;  /* [n_seqs + 1], not decreasing, or NULL */
+  const int32_t *shared_dev;  /* [shared_blocks] block ids, or NULL */
+  int64_t n_blocks, table_stride, n_seqs;
+  int64_t max_len; /* at least 1, at most table_stride * block_size and JERO_MAX_PAGED_POSITIONS */
+  int64_t shared_blocks;
+  int block_size; /* a power of two up to 2^20 */
+  int kv_dtype;   /* JERO_KV_F32 or JERO_KV_F16 */
+  int n_heads_kv, head_dim;
+} jero_paged_cache;
+#define JERO_MAX_PAGED_POSITIONS 4194304
+size_t jero_hip_paged_attention_workspace_bytes(const jero_paged_cache *cache, int64_t n_tokens, int n_heads);
+int jero_hip_paged_attention(const jero_paged_cache *cache, int act_dtype, const void *q_dev, int64_t q_stride,
+                             int64_t n_tokens, int n_heads, float scale, void *out_dev, int64_t out_stride,
+                             void *workspace_dev, size_t workspace_bytes, void *stream);
+
 /* Drafted tokens against the target's probabilities, from given random numbers.  Sequence s has rows
  * starts[s] .. starts[s + 1] - 1 of tokens_dev: the last token that stands, then n = rows - 1 drafted
  * ones.  target_dev row t (f32, vocab of them, target_stride apart) holds the probabilities of the

@@ -1,0 +1,695 @@
+// paged_attend.h -- attention over a paged key/value cache whose sequences may share their first positions:
+// the kernel, built for one head_dim a translation unit.
+#pragma once
+
+#include "mla.h"
+#include "paged.h"
+
+namespace jero {
+
+// What places that hold nothing are read from: 8 values of either type.
+__device__ __constant__ const uint32_t kPagedZeros[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+
+// ---------------------------------------------------------------- what a workgroup works on
+
+// Position below which token row t of the call attends (t's own and max_len within it), by every lane on its own.
+__device__ __forceinline__ int paged_visible(const PagedCall& c, int t) {
+  int seq = t, end = t + 1;
+  if (c.starts) {
+    int lo = 0, left = c.n_seqs + 1;  // starts from 0 .. lo - 1 are not behind t
+    while (left > 0) {
+      const int half = left >> 1;
+      if (c.starts[lo + half] <= t) lo += half + 1, left -= half + 1;
+      else left = half;
+    }
+    seq = lo - 1;
+    if (seq < 0 || seq >= c.n_seqs) return -1;  // no sequence's
+    end = c.starts[seq + 1];
+  }
+  const int64_t pos = int64_t(c.lens[seq]) - end + t;
+  return int(max(min(pos + 1, int64_t(c.max_len)), int64_t(0)));
+}
+
+// Rows (token row * group + head of the group) first .. first + count - 1 of the kv head, the positions lo .. hi - 1,
+// and the sequence whose table holds those that are not shared.
+struct PagedItem {
+  int first, count, lo, hi, seq, head, part;
+};
+
+__device__ __forceinline__ bool paged_item(const PagedCall& c, const PagedPlan& p, int lane, PagedItem& it, bool& wide) {
+  // the two phases' blocks by turns, 256 of each: a CU gets one that computes and one that reads
+  const int k = blockIdx.x >> 8, in = blockIdx.x & 255;
+  const int np = (p.pre_blocks + 255) >> 8, no = (p.own_blocks + 255) >> 8, both = min(np, no);
+  const bool pre = k < 2 * both ? (k & 1) == 0 : np > no;
+  const int i = (k < 2 * both ? k >> 1 : k - both) * 256 + in;
+  if (i >= (pre ? p.pre_blocks : p.own_blocks)) return false;
+  it.head = i % c.kv_heads;
+  const int rest = i / c.kv_heads;
+  if (pre) {
+    const int tile = rest % p.pre_tiles, chunk = rest / p.pre_tiles;
+    const int rows = p.pre_wide ? p.wide_rows : p.narrow_rows;
+    wide = p.pre_wide;
+    it.first = tile * rows;
+    it.count = min(rows, c.n_tokens * c.group - it.first);
+    it.lo = chunk * p.pre_len;
+    it.hi = min(it.lo + p.pre_len, c.shared_len);
+    it.seq = 0, it.part = chunk;
+    return true;
+  }
+  wide = p.own_wide;
+  const int rows = wide ? p.wide_rows : p.narrow_rows;
+  const int chunk = rest / p.own_tiles, tile = p.own_tiles - 1 - rest % p.own_tiles;
+  int end, from, skip = 0;
+  if (!c.starts) {
+    // a token's tiles
+    const int each = (c.group + rows - 1) / rows;
+    it.seq = tile / each, skip = tile % each * rows;
+    from = it.seq, end = it.seq + 1;
+  } else {
+    // sequence s holds tiles floor(starts[s] group / rows) + s on: enough for its rows, and they do not fall with s
+    int count = 0, left = c.n_seqs;  // sequences 0 .. count - 1 begin at no later tile
+    while (left > 0) {
+      const int step = (left + kWave - 1) / kWave, j = count + lane * step + step - 1;
+      const int s = min(j, c.n_seqs - 1);
+      const int64_t at = int64_t(min(max(c.starts[s], 0), c.n_tokens)) * c.group / rows + s;
+      const int n = __popcll(__ballot(j < count + left && at <= tile));
+      const int past = n * step;
+      left = min(step - 1, left - past);
+      count += past;
+    }
+    it.seq = count - 1;
+    if (it.seq < 0) return false;
+    from = min(max(c.starts[it.seq], 0), c.n_tokens);
+    end = c.starts[it.seq + 1];
+    skip = int(tile - (int64_t(from) * c.group / rows + it.seq)) * rows;
+  }
+  const int mine = max(min(end, c.n_tokens) - from, 0) * c.group;
+  if (skip >= mine) return false;
+  it.first = from * c.group + skip;
+  it.count = min(rows, mine - skip);
+  it.lo = p.own_lo + chunk * p.own_len;
+  // the last row sees the most
+  const int last = (it.first + it.count - 1) / c.group;
+  const int64_t top = min(int64_t(c.lens[it.seq]) - end + last + 1, int64_t(c.max_len));
+  it.hi = int(max(min(top, int64_t(it.lo) + p.own_len), int64_t(it.lo)));
+  it.part = p.pre_chunks + chunk;
+  return p.parts == 1 || it.hi > it.lo;  // (the only part of a row writes it whatever it sees)
+}
+
+// ---------------------------------------------------------------- a wave's step
+
+template <int HD, int NJ, bool TWOQ>
+struct AttendState {
+  static constexpr int KT = HD / 32, DT = HD / 16;
+  h8_t qh[NJ][KT], ql[NJ][TWOQ ? KT : 1];
+  f4_t o[NJ][DT], l[NJ];
+  float factor[NJ], m[NJ];
+  int limit[NJ];  // positions below it are seen by the lane's row
+};
+
+constexpr float kPagedLift = 11.f, kPagedGrow = 4.f;
+
+// KR positions from p0 on: S^T = K q^T leaves a row per lane column and, taken in the order 4g .. 4g + 3, 16 + 4g .. of
+// 32 positions, is the B operand of O^T += V^T p, V^T read from LDS transposed.  ok: positions that are there; bad:
+// those whose values are not finite and have been made zeros.
+template <int HD, int NJ, int KR, bool TWOQ, bool TWOK, typename KRead>
+__device__ __forceinline__ void attend_step(AttendState<HD, NJ, TWOQ>& st, KRead kread, const uint8_t* vp, int vplane,
+                                            const int (&vat)[4], int p0, bool masked, uint64_t ok, uint64_t bad, int g) {
+  constexpr int RT = KR / 16, KT = HD / 32, DT = HD / 16, KP = TWOK ? 2 : 1;
+  f4_t s[NJ][RT];
+  h8_t ka[2][RT][KP];
+  auto read_k = [&](int k) {
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+      for (int e = 0; e < KP; e++) ka[k & 1][r][e] = kread(k, r, e);
+  };
+  read_k(0);
+#pragma unroll
+  for (int k = 0; k < KT; k++) {
+    if (k + 1 < KT) read_k(k + 1);
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+      for (int j = 0; j < NJ; j++)
+        s[j][r] = mfma(ka[k & 1][r][0], st.qh[j][k], k ? s[j][r] : f4_t{0.f, 0.f, 0.f, 0.f});
+    if constexpr (TWOQ) {
+#pragma unroll
+      for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int j = 0; j < NJ; j++) s[j][r] = mfma(ka[k & 1][r][0], st.ql[j][k], s[j][r]);
+    }
+    if constexpr (TWOK) {
+#pragma unroll
+      for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int j = 0; j < NJ; j++) s[j][r] = mfma(ka[k & 1][r][KP - 1], st.qh[j][k], s[j][r]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  h8_t bh[NJ][RT / 2], bl[NJ][RT / 2];
+  bool grew[NJ];
+  float alpha[NJ], times[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; j++) times[j] = st.factor[j];
+  if (masked) {
+    const uint64_t mine = ok >> (4 * g), odd = bad >> (4 * g);
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      times[j] = 1.f;
+#pragma unroll
+      for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const uint64_t bit = 1ull << (16 * r + e);
+          const float y = (odd & bit) ? NAN : s[j][r][e] * st.factor[j];
+          s[j][r][e] = p0 + 16 * r + 4 * g + e < st.limit[j] && (mine & bit) ? y : -INFINITY;
+        }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NJ; j++) {
+    float mx = s[j][0][0];
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[j][r][e]);
+    mx = max_over_groups(mx) * times[j];
+    grew[j] = __any(mx > st.m[j] + kPagedGrow);
+    const float mn = grew[j] ? fmaxf(st.m[j], mx) : st.m[j];
+    const float ref = mn == -INFINITY ? 0.f : mn, from = ref - kPagedLift;
+    alpha[j] = __builtin_amdgcn_exp2f(st.m[j] - ref);
+    st.m[j] = mn;
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[j][r][e], times[j], -from));
+        _Float16 a, b;
+        split2(p, a, b);
+        bh[j][r / 2][4 * (r & 1) + e] = a;
+        bl[j][r / 2][4 * (r & 1) + e] = b;
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < NJ; j++)
+    if (grew[j]) {
+      st.l[j] *= alpha[j];
+#pragma unroll
+      for (int d = 0; d < DT; d++) st.o[j][d] *= alpha[j];
+    }
+  // the sums of the numerators, as the product rounds them: a row of ones in place of the values
+  {
+    h8_t one;
+#pragma unroll
+    for (int e = 0; e < 8; e++) one[e] = _Float16(1.f);
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+#pragma unroll
+      for (int r = 0; r < RT / 2; r++) {
+        st.l[j] = mfma(one, bh[j][r], st.l[j]);
+        if constexpr (TWOQ) st.l[j] = mfma(one, bl[j][r], st.l[j]);
+      }
+  }
+  auto tr = [&](int d, int r, int plane) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(vp + plane * vplane + vat[d & 3] + 128 * (d >> 2) + 16 * r * HD * 2));
+  };
+  h8_t va[2][RT / 2][KP];
+  auto read_v = [&](int d) {
+#pragma unroll
+    for (int r = 0; r < RT / 2; r++)
+#pragma unroll
+      for (int e = 0; e < KP; e++)
+        va[d & 1][r][e] = __builtin_bit_cast(
+            h8_t, __builtin_shufflevector(tr(d, 2 * r, e), tr(d, 2 * r + 1, e), 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  read_v(0);
+#pragma unroll
+  for (int d = 0; d < DT; d++) {
+    if (d + 1 < DT) read_v(d + 1);
+#pragma unroll
+    for (int r = 0; r < RT / 2; r++) {
+#pragma unroll
+      for (int j = 0; j < NJ; j++) st.o[j][d] = mfma(va[d & 1][r][0], bh[j][r], st.o[j][d]);
+      if constexpr (TWOQ) {
+#pragma unroll
+        for (int j = 0; j < NJ; j++) st.o[j][d] = mfma(va[d & 1][r][0], bl[j][r], st.o[j][d]);
+      }
+      if constexpr (TWOK) {
+#pragma unroll
+        for (int j = 0; j < NJ; j++) st.o[j][d] = mfma(va[d & 1][r][KP - 1], bh[j][r], st.o[j][d]);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// ---------------------------------------------------------------- the kernel
+
+// F ("wide"): four waves share KR positions in LDS and hold 16 NJ rows each.  D ("narrow"): four waves share 16 NB rows and
+// hold 32 positions each, keys in registers, values in their own part of LDS; they are joined at the end.
+template <int HD, typename X, typename KV>
+struct PagedShape {
+  static constexpr bool TWOQ = sizeof(X) == 4, TWOK = sizeof(KV) == 4;
+  static constexpr int NJ = HD <= 128 ? 2 : 1, KR = TWOQ || HD == 256 ? 32 : 64;
+  static constexpr int kRows = 64 * NJ;
+  static constexpr int kPlanes = TWOK ? 2 : 1, kBufs = TWOK ? 1 : 2;
+  static constexpr int kPlane = KR * HD * 2, kBuf = 2 * kPlanes * kPlane;  // keys, then values
+  static constexpr int kNarrow = 32 * HD * 2;                              // a wave's values
+  static constexpr int kWaveLds = kNarrow * (TWOK ? 2 : 2);                // two buffers, or two parts
+  static constexpr int kJoin = 4 * 16 * (HD + 4) * 4;
+  static constexpr int kMost = kBufs * kBuf > 4 * kWaveLds ? kBufs * kBuf : 4 * kWaveLds;
+  static constexpr int kLds = kMost > kJoin ? kMost : kJoin;
+  static constexpr int kGroups = TWOK || HD == 256 ? 1 : 2;
+};
+
+// Infinities or NaN among 8 f16: their exponent's bits all set.
+__device__ __forceinline__ bool odd8(u32x4 v) {
+  auto one = [](uint32_t w) {
+    const uint32_t e = w & 0x7C007C00u;
+    return (e & 0xFFFFu) == 0x7C00u || (e >> 16) == 0x7C00u;
+  };
+  return one(v.x) || one(v.y) || one(v.z) || one(v.w);
+}
+
+template <int HD, typename X, typename KV, int NB>
+__global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
+    paged_attend_kernel(PagedCall c, PagedPlan plan, const X* __restrict__ q, X* __restrict__ out,
+                        float* __restrict__ part_o, float2* __restrict__ part_ml) {
+  using S = PagedShape<HD, X, KV>;
+  constexpr bool TWOQ = S::TWOQ, TWOK = S::TWOK;
+  constexpr int KT = HD / 32, DT = HD / 16;
+  __shared__ __attribute__((aligned(16))) uint8_t s_kv[S::kLds];
+  __shared__ float s_m[4][16], s_l[4][16];
+  __shared__ int s_low;
+  __shared__ unsigned long long s_bad;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, col = lane & 15;
+  PagedItem it;
+  bool wide;
+  if (!paged_item(c, plan, lane, it, wide)) return;
+  const uint32_t lds0 = uint32_t(uintptr_t((lds_u8*)s_kv));
+  const int D = c.dim;
+  const int64_t row_len = int64_t(c.kv_heads) * D;
+  const KV* const kb = static_cast<const KV*>(c.k) + int64_t(it.head) * D;
+  const KV* const vb = static_cast<const KV*>(c.v) + int64_t(it.head) * D;
+  const int32_t* const table = c.table + it.seq * c.table_stride;
+  const void* const zeros = kPagedZeros;
+
+  // The block of a position; ~0: none, or not the item's.
+  auto block_of = [&](int pos) -> uint32_t {
+    if (pos >= it.hi) return ~0u;
+    const int b = pos >> c.shift;
+    const uint32_t id = uint32_t(pos < c.shared_len ? c.shared[b] : table[b]);
+    return id < c.n_blocks ? id : ~0u;
+  };
+  auto row_of = [&](const KV* base, uint32_t id, int pos) -> const uint8_t* {
+    return reinterpret_cast<const uint8_t*>(base + ((int64_t(id) << c.shift) + (pos & ((1 << c.shift) - 1))) * row_len);
+  };
+  int vat[4];
+  {
+    const int vr = 4 * g + (col >> 2);
+#pragma unroll
+    for (int d = 0; d < 4; d++) vat[d] = vr * HD * 2 + 16 * ((2 * d + ((col & 3) >> 1)) ^ swap8(vr)) + 8 * (col & 1);
+  }
+
+  // Loads the queries of the lane's columns; `row0`: of the wave's first.
+  auto queries = [&](auto& st, int row0) {
+    constexpr int NJ = sizeof(st.m) / sizeof(float);
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      const int i = row0 + 16 * j + col;
+      const bool mine = i < it.count;
+      const int r = it.first + (mine ? i : 0), t = r / c.group, h = it.head * c.group + r % c.group;
+      const int seen = mine ? paged_visible(c, t) : 0;
+      st.limit[j] = seen;
+      const X* qr = q + t * c.q_stride + int64_t(h) * D;
+      float v[KT][8], mx = 0.f;
+#pragma unroll
+      for (int k = 0; k < KT; k++) {
+        const int d = 32 * k + 8 * g;
+        const bool on = d < D && seen > 0;
+        if (on) load8<X>(qr + d, v[k]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          v[k][e] = on ? v[k][e] : 0.f;
+          mx = fmaxf(mx, fabsf(v[k][e]));
+        }
+      }
+      // each row's brought near 1 by a power of two that goes into the scores' factor
+      mx = max_over_groups(mx);
+      int ex = 0;
+      if (TWOQ && mx > 0.f && mx < INFINITY) ex = ilogbf(mx);
+      st.factor[j] = ldexpf(fabsf(c.scale) * 1.44269504088896341f, ex);  // its sign goes into the queries
+#pragma unroll
+      for (int k = 0; k < KT; k++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          _Float16 a, b;
+          split2(ldexpf(c.scale < 0.f ? -v[k][e] : v[k][e], -ex), a, b);
+          st.qh[j][k][e] = a;
+          if (TWOQ) st.ql[j][k][e] = b;
+        }
+      st.m[j] = -INFINITY;
+      st.l[j] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int d = 0; d < DT; d++) st.o[j][d] = f4_t{0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  // Lowest limit of the wave's rows that see anything (those that do not are put right at the end).
+  auto lowest = [&](const auto& st) {
+    constexpr int NJ = sizeof(st.m) / sizeof(float);
+    int low = INT32_MAX;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) low = min(low, st.limit[j] > 0 ? st.limit[j] : INT32_MAX);
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) low = min(low, __shfl_xor(low, off, kWave));
+    return low;
+  };
+  // Row i of the item, 4 of its results.
+  auto store = [&](int i, int d, f4_t v, float m, float l, bool first) {
+    const int r = it.first + i, t = r / c.group, h = it.head * c.group + r % c.group;
+    if (plan.parts > 1) {
+      const int64_t at = (int64_t(it.part) * c.n_tokens + t) * c.heads + h;
+      if (d < D) *reinterpret_cast<f4_t*>(part_o + at * D + d) = v;
+      if (first) part_ml[at] = make_float2(m, l);
+      return;
+    }
+    if (d >= D) return;
+    const float inv = l != 0.f ? 1.0f / l : 0.f;
+    X* dst = out + t * c.out_stride + int64_t(h) * D + d;
+    if constexpr (sizeof(X) == 4) {
+      *reinterpret_cast<f4_t*>(dst) = v * inv;
+    } else {
+      h4_t y;
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[e] = _Float16(v[e] * inv);
+      *reinterpret_cast<h4_t*>(dst) = y;
+    }
+  };
+
+  if (wide) {
+    // ------------------------------------------------------------ F
+    constexpr int KR = S::KR, NJ = S::NJ;
+    AttendState<HD, NJ, TWOQ> st;
+    if (tid == 0) s_low = INT32_MAX, s_bad = 0;
+    queries(st, wv * 16 * NJ);
+    const int low = lowest(st);
+    __syncthreads();
+    if (lane == 0) atomicMin(&s_low, low);
+    __syncthreads();
+    const int common = s_low;  // below it, all rows of the workgroup see a position
+    const int steps = (it.hi - it.lo + KR - 1) / KR;
+    auto find = [&](int step) { return block_of(it.lo + step * KR + (lane & (KR - 1))); };
+    constexpr int NI = S::kPlane / 1024 / 4;  // 1024-byte pieces a wave, of keys and of values
+    auto load = [&](int step, int buf, uint32_t ids) {  // f16: straight to LDS
+      const int p0 = it.lo + step * KR;
+#pragma unroll
+      for (int n = 0; n < NI; n++) {
+        const int i = 4 * n + wv, b = i * 1024 + 16 * lane, r = b / (2 * HD);
+        const int at = (b % (2 * HD)) ^ (16 * swap8(r));
+        const uint32_t id = __shfl(ids, r, kWave);
+        const bool on = id != ~0u && at < 2 * D;
+        const uint32_t to = lds0 + buf * S::kBuf + i * 1024;
+        dma_lanes(on ? row_of(kb, id, p0 + r) + at : zeros, to);
+        dma_lanes(on ? row_of(vb, id, p0 + r) + at : zeros, to + S::kPlane);
+      }
+    };
+    // f32: through registers, a lane 8 values of a row
+    constexpr int NR = TWOK ? KR * HD / 8 / 256 : 1;
+    float raw[TWOK ? 2 : 1][NR][8];
+    auto fetch = [&](int step, uint32_t ids) {
+      const int p0 = it.lo + step * KR;
+#pragma unroll
+      for (int n = 0; n < NR; n++) {
+        const int i = n * 256 + tid, r = i / (HD / 8), d = 8 * (i % (HD / 8));
+        const uint32_t id = __shfl(ids, r, kWave);
+        const bool on = id != ~0u && d < D;
+        load8<float>(static_cast<const float*>(on ? static_cast<const void*>(row_of(kb, id, p0 + r) + 4 * d) : zeros), raw[0][n]);
+        load8<float>(static_cast<const float*>(on ? static_cast<const void*>(row_of(vb, id, p0 + r) + 4 * d) : zeros),
+                     raw[TWOK ? 1 : 0][n]);
+      }
+    };
+    auto put = [&]() {
+#pragma unroll
+      for (int w = 0; w < (TWOK ? 2 : 1); w++)
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+          const int i = n * 256 + tid, r = i / (HD / 8), d = i % (HD / 8);
+          h8_t hi, lo;
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            _Float16 a, b;
+            split2(raw[w][n][e], a, b);
+            hi[e] = a, lo[e] = b;
+          }
+          uint8_t* to = s_kv + w * S::kPlanes * S::kPlane + r * HD * 2 + 16 * (d ^ swap8(r));
+          *reinterpret_cast<h8_t*>(to) = hi;
+          *reinterpret_cast<h8_t*>(to + S::kPlane) = lo;
+        }
+    };
+    const int kat = 16 * (g ^ swap8(col)), kat4 = 16 * ((4 + g) ^ swap8(col));
+    uint32_t ids = find(0), next = ids;
+    if (steps > 0) {
+      if constexpr (TWOK) fetch(0, ids);
+      else load(0, 0, ids);
+      next = find(1);
+    }
+    for (int i = 0; i < steps; i++) {
+      const int buf = TWOK ? 0 : i & 1, p0 = it.lo + i * KR;
+      uint64_t ok = __ballot(ids != ~0u);
+      if constexpr (TWOK) {
+        __syncthreads();  // the last step's reads
+        put();
+        __syncthreads();
+        ids = next;
+        if (i + 1 < steps) fetch(i + 1, ids), next = find(i + 2);
+      } else {
+        dma_wait<0>();
+        __syncthreads();
+        ids = next;
+        if (i + 1 < steps) load(i + 1, buf ^ 1, ids), next = find(i + 2);
+      }
+      uint8_t* const kv = s_kv + buf * S::kBuf;
+      uint64_t bad = 0;
+      if (min(p0 + KR, it.hi) > common) {
+        // Values that are not finite, of which a row that does not see them would take 0 * infinity, are made zeros, and
+        // their positions' scores NaN.
+        constexpr int L = HD / 8;
+        uint8_t* const rows = kv + S::kPlanes * S::kPlane;
+        for (int n = tid; n < KR * L; n += 256)
+          if (odd8(*reinterpret_cast<const u32x4*>(rows + 16 * n))) atomicOr(&s_bad, 1ull << (n / L));
+        __syncthreads();
+        bad = s_bad;
+        if (bad) {
+          const u32x4 z = {0u, 0u, 0u, 0u};
+          for (int n = tid; n < KR * L; n += 256)
+            if ((bad >> (n / L)) & 1) {
+              *reinterpret_cast<u32x4*>(rows + 16 * n) = z;
+              if (TWOK) *reinterpret_cast<u32x4*>(rows + S::kPlane + 16 * n) = z;
+            }
+        }
+        __syncthreads();
+        if (tid == 0) s_bad = 0;  // (the next step's barriers come before its next use)
+      }
+      auto kread = [&](int k, int r, int e) {
+        return *reinterpret_cast<const h8_t*>(kv + e * S::kPlane + (16 * r + col) * HD * 2 + ((k & 1) ? kat4 : kat) +
+                                              128 * (k >> 1));
+      };
+      const bool masked = p0 + KR > low || ok != ~0ull || p0 + KR > it.hi;
+      attend_step<HD, NJ, KR, TWOQ, TWOK>(st, kread, kv + S::kPlanes * S::kPlane, S::kPlane, vat, p0, masked, ok, bad, g);
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      const int i = wv * 16 * NJ + 16 * j + col;
+      if (i >= it.count || st.limit[j] < 0) continue;
+      const bool sees = st.limit[j] > it.lo;
+      const f4_t z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+        store(i, 16 * d + 4 * g, sees ? st.o[j][d] : z, sees ? st.m[j] : -INFINITY, sees ? st.l[j][0] : 0.f, d == 0 && g == 0);
+    }
+    return;
+  }
+
+  // -------------------------------------------------------------- D
+  constexpr int KR = 32;
+  AttendState<HD, NB, TWOQ> st;
+  queries(st, 0);
+  const int low = lowest(st);
+  const int steps = (it.hi - it.lo + KR - 1) / KR;
+  uint8_t* const mine = s_kv + wv * S::kWaveLds;
+  const uint32_t mine0 = lds0 + wv * S::kWaveLds;
+  auto find = [&](int step) { return block_of(it.lo + step * KR + (lane & (KR - 1))); };
+  constexpr bool AHEAD = !(TWOK && HD == 256);  // (its registers hold one step)
+  constexpr int KRAW = TWOK ? 2 : 1;            // 16-byte pieces for 8 values
+  u32x4 kraw[2][KT][KRAW];                      // keys: row 16 r + col, values 32 k + 8 g ..
+  constexpr int NV = TWOK ? 32 * HD / 8 / 64 : 1;
+  u32x4 vraw[NV][2];
+  auto fetch = [&](int step, int buf, uint32_t ids) {
+    const int p0 = it.lo + step * KR;
+    if constexpr (!TWOK) {
+#pragma unroll
+      for (int i = 0; i < S::kNarrow / 1024; i++) {
+        const int b = i * 1024 + 16 * lane, r = b / (2 * HD), at = (b % (2 * HD)) ^ (16 * swap8(r));
+        const uint32_t id = __shfl(ids, r, kWave);
+        dma_lanes(id != ~0u && at < 2 * D ? row_of(vb, id, p0 + r) + at : zeros, mine0 + buf * S::kNarrow + i * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NV; n++) {
+        const int i = n * 64 + lane, r = i / (HD / 8), d = 8 * (i % (HD / 8));
+        const uint32_t id = __shfl(ids, r, kWave);
+        const bool on = id != ~0u && d < D;
+        const uint8_t* p = static_cast<const uint8_t*>(on ? static_cast<const void*>(row_of(vb, id, p0 + r) + 4 * d) : zeros);
+        vraw[n][0] = *reinterpret_cast<const u32x4*>(p);
+        vraw[n][1] = *reinterpret_cast<const u32x4*>(p + (on ? 16 : 0));
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+      const uint32_t id = __shfl(ids, 16 * r + col, kWave);
+      const uint8_t* row = id != ~0u ? row_of(kb, id, p0 + 16 * r + col) : nullptr;
+#pragma unroll
+      for (int k = 0; k < KT; k++) {
+        const int d = 32 * k + 8 * g;
+        const bool on = row && d < D;
+        const uint8_t* p = on ? row + d * int(sizeof(KV)) : static_cast<const uint8_t*>(zeros);
+#pragma unroll
+        for (int e = 0; e < KRAW; e++) kraw[r][k][e] = *reinterpret_cast<const u32x4*>(p + (on ? 16 * e : 0));
+      }
+    }
+  };
+  uint32_t ids = find(wv), next = ids;
+  if (AHEAD && wv < steps) {
+    fetch(wv, 0, ids);
+    next = find(wv + 4);
+  }
+  int buf = 0;
+  for (int i = wv; i < steps; i += 4) {
+    const int p0 = it.lo + i * KR;
+    const uint64_t ok = __ballot(ids != ~0u);
+    if constexpr (!AHEAD) fetch(i, 0, ids), next = find(i + 4);
+    dma_wait<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last step's reads of the buffer that is loaded next
+    uint8_t* const vp = mine + (TWOK ? 0 : buf * S::kNarrow);
+    h8_t kc[2][KT][TWOK ? 2 : 1];
+#pragma unroll
+    for (int r = 0; r < 2; r++)
+#pragma unroll
+      for (int k = 0; k < KT; k++) {
+        if constexpr (!TWOK) {
+          kc[r][k][0] = __builtin_bit_cast(h8_t, kraw[r][k][0]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            _Float16 a, b;
+            split2(__uint_as_float(kraw[r][k][(KRAW - 1) * (e >> 2)][e & 3]), a, b);
+            kc[r][k][0][e] = a, kc[r][k][TWOK ? 1 : 0][e] = b;
+          }
+        }
+      }
+    if constexpr (TWOK) {
+#pragma unroll
+      for (int n = 0; n < NV; n++) {
+        const int b = n * 64 + lane, r = b / (HD / 8), d = b % (HD / 8);
+        h8_t hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          _Float16 x, y;
+          split2(__uint_as_float(vraw[n][e >> 2][e & 3]), x, y);
+          hi[e] = x, lo[e] = y;
+        }
+        uint8_t* to = vp + r * HD * 2 + 16 * (d ^ swap8(r));
+        *reinterpret_cast<h8_t*>(to) = hi;
+        *reinterpret_cast<h8_t*>(to + S::kNarrow) = lo;
+      }
+    }
+    ids = next;
+    if (AHEAD && i + 4 < steps) {
+      fetch(i + 4, buf ^ 1, ids);
+      next = find(i + 8);
+    }
+    uint64_t bad = 0;
+    if (min(p0 + KR, it.hi) > low) {
+      constexpr int L = HD / 8;
+      for (int n = lane; n < KR * L; n += 64) {
+        const bool odd = odd8(*reinterpret_cast<const u32x4*>(vp + 16 * n));
+        const uint64_t b = __ballot(odd);
+#pragma unroll
+        for (int x = 0; x < 64; x += L)
+          if ((b >> x) & (L == 64 ? ~0ull : (1ull << (L & 63)) - 1)) bad |= 1ull << ((n - lane + x) / L);
+      }
+      if (bad) {
+        const u32x4 z = {0u, 0u, 0u, 0u};
+        for (int n = lane; n < KR * L; n += 64)
+          if ((bad >> (n / L)) & 1) {
+            *reinterpret_cast<u32x4*>(vp + 16 * n) = z;
+            if (TWOK) *reinterpret_cast<u32x4*>(vp + S::kNarrow + 16 * n) = z;
+          }
+      }
+    }
+    const bool masked = p0 + KR > low || ok != ~0ull || p0 + KR > it.hi;
+    auto kread = [&](int k, int r, int e) { return kc[r][k][e]; };
+    attend_step<HD, NB, KR, TWOQ, TWOK>(st, kread, vp, S::kNarrow, vat, p0, masked, ok, bad, g);
+    buf ^= 1;
+  }
+  // the four waves' rows joined, 16 at a time
+  float* const rows = reinterpret_cast<float*>(s_kv);
+#pragma unroll
+  for (int j = 0; j < NB; j++) {
+    __syncthreads();
+    if (g == 0) s_m[wv][col] = st.m[j], s_l[wv][col] = st.l[j][0];
+    __syncthreads();
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; w++) m = fmaxf(m, s_m[w][col]);
+    const float ref = m == -INFINITY ? 0.f : m, f = __builtin_amdgcn_exp2f(st.m[j] - ref);
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+      *reinterpret_cast<f4_t*>(rows + (wv * 16 + col) * (HD + 4) + 16 * d + 4 * g) = st.o[j][d] * f;
+    __syncthreads();
+    for (int n = tid; n < 16 * HD / 4; n += 256) {
+      const int r = n / (HD / 4), d = 4 * (n % (HD / 4)), i = 16 * j + r;
+      if (i >= it.count) continue;
+      const int seen = paged_visible(c, (it.first + i) / c.group);
+      if (seen < 0) continue;
+      const bool sees = seen > it.lo;
+      float mm = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; w++) mm = fmaxf(mm, s_m[w][r]);
+      const float at = mm == -INFINITY ? 0.f : mm;
+      f4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        l += s_l[w][r] * __builtin_amdgcn_exp2f(s_m[w][r] - at);
+        v += *reinterpret_cast<const f4_t*>(rows + (w * 16 + r) * (HD + 4) + d);
+      }
+      const f4_t z = {0.f, 0.f, 0.f, 0.f};
+      store(i, d, sees ? v : z, sees ? mm : -INFINITY, sees ? l : 0.f, d == 0);
+    }
+  }
+}
+
+template <int HD, typename X, typename KV>
+static int launch_paged(const PagedCall& c, const PagedPlan& p, const void* q, void* out, float* part_o, float2* part_ml,
+                        hipStream_t s) {
+  const unsigned blocks = unsigned(((p.pre_blocks + 255) / 256 + (p.own_blocks + 255) / 256) * 256);
+  if (HD < 256 && p.narrow_rows == 32)
+    hipLaunchKernelGGL((paged_attend_kernel<HD, X, KV, HD < 256 ? 2 : 1>), dim3(blocks), dim3(256), 0, s, c, p,
+                       static_cast<const X*>(q), static_cast<X*>(out), part_o, part_ml);
+  else
+    hipLaunchKernelGGL((paged_attend_kernel<HD, X, KV, 1>), dim3(blocks), dim3(256), 0, s, c, p, static_cast<const X*>(q),
+                       static_cast<X*>(out), part_o, part_ml);
+  return check_launch("paged_attention");
+}
+
+template <int HD>
+static int launch_paged_types(const PagedCall& c, const PagedPlan& p, bool x16, bool kv16, const void* q, void* out,
+                              float* part_o, float2* part_ml, hipStream_t s) {
+  if (x16) return launch_paged<HD, _Float16, _Float16>(c, p, q, out, part_o, part_ml, s);
+  if (kv16) return launch_paged<HD, float, _Float16>(c, p, q, out, part_o, part_ml, s);
+  return launch_paged<HD, float, float>(c, p, q, out, part_o, part_ml, s);
+}
+
+}  // namespace jero

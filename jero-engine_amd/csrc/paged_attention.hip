@@ -1,0 +1,185 @@
+// paged_attention.hip -- attention over a paged key/value cache whose sequences may share their first positions:
+// how a call is cut, the joining of its parts, and the entry point.
+#include <algorithm>
+#include <cmath>
+
+#include "paged_attend.h"
+#include "runtime.h"
+
+namespace jero {
+
+// Joins a row's parts: the chunks of the shared positions, then those of its own.  Workgroup (token, 1024 of its
+// results), a thread four of them.
+template <typename X>
+__global__ void __launch_bounds__(256) paged_merge_kernel(PagedCall c, PagedPlan p, X* __restrict__ out,
+                                                          const float* __restrict__ part_o,
+                                                          const float2* __restrict__ part_ml) {
+  const int t = blockIdx.x, i = 4 * (blockIdx.y * 256 + threadIdx.x);
+  const int seen = paged_visible(c, t);
+  if (seen < 0 || i >= c.heads * c.dim) return;
+  const int h = i / c.dim;
+  const int shared = min(seen, c.shared_len);
+  const int pre = p.pre_chunks ? (shared + p.pre_len - 1) / p.pre_len : 0;
+  const int own = seen > p.own_lo ? (seen - p.own_lo + p.own_len - 1) / p.own_len : 0;
+  const int64_t step = int64_t(c.n_tokens) * c.heads, row = int64_t(t) * c.heads + h;
+  float m = -INFINITY;
+  for (int k = 0; k < pre + own; k++) m = fmaxf(m, part_ml[row + step * (k < pre ? k : p.pre_chunks + k - pre)].x);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  f4_t v = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < pre + own; k++) {
+    const int64_t at = row + step * (k < pre ? k : p.pre_chunks + k - pre);
+    const float2 ml = part_ml[at];
+    const float e = __builtin_amdgcn_exp2f(ml.x - ref);
+    l += e * ml.y;
+    v += e * *reinterpret_cast<const f4_t*>(part_o + at * c.dim + (i - h * c.dim));
+  }
+  const float inv = l != 0.f ? 1.0f / l : 0.f;
+  X* dst = out + t * c.out_stride + i;
+#pragma unroll
+  for (int e = 0; e < 4; e++) dst[e] = X(v[e] * inv);
+}
+
+static int head_width(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+static PagedPlan paged_plan(const jero_paged_cache* k, int64_t n_tokens, int n_heads) {
+  PagedPlan p{};
+  const int group = n_heads / k->n_heads_kv, hd = head_width(k->head_dim), kv = k->n_heads_kv;
+  const int64_t shared = std::min<int64_t>(k->shared_blocks * k->block_size, k->max_len);
+  const int64_t rows = n_tokens * group, each = (n_tokens + k->n_seqs - 1) / k->n_seqs * group;
+  p.wide_rows = hd <= 128 ? 128 : 64;
+  // rows of all sequences over the shared positions, where there is more than one and they do not fill tiles themselves
+  const bool apart = shared > 0 && k->n_seqs > 1 && each < p.wide_rows;
+  p.narrow_rows = hd < 256 && (each > 16 || (apart && rows > 16 && rows <= 32)) ? 32 : 16;
+  p.own_wide = each > p.narrow_rows;
+  p.own_lo = apart ? int(shared) : 0;
+  const int own_rows = p.own_wide ? p.wide_rows : p.narrow_rows;
+  const int64_t tiles = k->starts_dev ? rows / own_rows + k->n_seqs : n_tokens * ((group + own_rows - 1) / own_rows);
+  p.own_tiles = int(tiles);
+  const int64_t span = std::max<int64_t>(k->max_len - p.own_lo, 1);
+  auto chunks = [&](int64_t blocks, int64_t span, int64_t want, int64_t least) {
+    return std::max<int64_t>(1, std::min((want + blocks - 1) / blocks, (span + least - 1) / least));
+  };
+  auto length = [](int64_t span, int64_t n) { return int(((span + n - 1) / n + 127) / 128 * 128); };
+  p.own_len = length(span, chunks(tiles * kv, span, 1024, 256));
+  p.own_chunks = int((span + p.own_len - 1) / p.own_len);
+  p.own_blocks = int(tiles * kv * p.own_chunks);
+  if (apart) {
+    p.pre_wide = rows > 32;
+    const int pre_rows = p.pre_wide ? p.wide_rows : p.narrow_rows;
+    p.pre_tiles = int((rows + pre_rows - 1) / pre_rows);
+    p.pre_len = length(shared, chunks(int64_t(p.pre_tiles) * kv, shared, 256, 256));
+    p.pre_chunks = int((shared + p.pre_len - 1) / p.pre_len);
+    p.pre_blocks = p.pre_tiles * kv * p.pre_chunks;
+  }
+  p.parts = p.pre_chunks + p.own_chunks;
+  return p;
+}
+
+static size_t part_bytes(const PagedPlan& p, int64_t n_tokens, int n_heads, int dim, size_t* ml) {
+  if (p.parts == 1) return 0;
+  const size_t rows = size_t(p.parts) * n_tokens * n_heads, o = (rows * dim * 4 + 255) & ~size_t(255);
+  if (ml) *ml = o;
+  return o + rows * 8;
+}
+
+static int check_paged(const jero_paged_cache* c, int64_t n_tokens, int n_heads) {
+  auto bad = [](int status, const std::string& what) { return fail(status, "paged_attention: " + what); };
+  auto aligned = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+  if (!c || !c->k_dev || !c->v_dev || !c->table_dev || !c->lens_dev) return bad(JERO_ERR_INVALID_ARGUMENT, "null pointer");
+  if (!aligned(c->k_dev, 16) || !aligned(c->v_dev, 16))
+    return bad(JERO_ERR_INVALID_ARGUMENT, "the cache must be 16-byte aligned");
+  if (!aligned(c->table_dev, 4) || !aligned(c->lens_dev, 4) || !aligned(c->starts_dev, 4) || !aligned(c->shared_dev, 4))
+    return bad(JERO_ERR_INVALID_ARGUMENT, "table, lens, starts and shared must be 4-byte aligned");
+  if (c->kv_dtype != JERO_KV_F32 && c->kv_dtype != JERO_KV_F16)
+    return bad(JERO_ERR_CAPABILITY_MISMATCH, "kv_dtype must be JERO_KV_F32 or JERO_KV_F16");
+  if (c->head_dim < 8 || c->head_dim % 8 || c->head_dim > 256)
+    return bad(JERO_ERR_CAPABILITY_MISMATCH, "head_dim " + std::to_string(c->head_dim) + " is not a multiple of 8 up to 256");
+  if (c->block_size < 1 || c->block_size > (1 << 20) || (c->block_size & (c->block_size - 1)))
+    return bad(JERO_ERR_CAPABILITY_MISMATCH, "block_size " + std::to_string(c->block_size) + " is not a power of two up to 2^20");
+  if (n_tokens < 1 || c->n_seqs < 1 || c->n_blocks < 1 || c->max_len < 1 || n_heads < 1 || c->n_heads_kv < 1)
+    return bad(JERO_ERR_TENSOR_BOUNDS, "no tokens, sequences, blocks, positions or heads");
+  if (n_heads > 1024) return bad(JERO_ERR_CAPABILITY_MISMATCH, "more than 1024 heads");
+  if (n_heads % c->n_heads_kv) return bad(JERO_ERR_TENSOR_BOUNDS, "n_heads is not a multiple of n_heads_kv");
+  if (n_tokens > (1 << 19) || c->n_seqs > (1 << 19) || c->n_blocks > INT32_MAX)
+    return bad(JERO_ERR_TENSOR_BOUNDS, "more than 2^19 tokens or sequences, or 2^31 - 1 blocks");
+  if (!c->starts_dev && n_tokens != c->n_seqs)
+    return bad(JERO_ERR_TENSOR_BOUNDS, std::to_string(n_tokens) + " tokens of " + std::to_string(c->n_seqs) +
+                                           " sequences without their starts");
+  if (c->max_len > JERO_MAX_PAGED_POSITIONS)
+    return bad(JERO_ERR_CONTEXT_LENGTH_EXCEEDED, "more than " + std::to_string(JERO_MAX_PAGED_POSITIONS) + " positions");
+  if (c->table_stride < 1 || c->table_stride > INT32_MAX || c->max_len > c->table_stride * c->block_size)
+    return bad(JERO_ERR_TENSOR_BOUNDS, std::to_string(c->table_stride) + " blocks a sequence do not hold " +
+                                           std::to_string(c->max_len) + " positions");
+  if (c->shared_blocks < 0 || (c->shared_blocks > 0 && !c->shared_dev) || c->shared_blocks > c->table_stride)
+    return bad(JERO_ERR_TENSOR_BOUNDS, "shared_blocks without their ids, or more than a table row");
+  if (n_tokens * n_heads > (1 << 25)) return bad(JERO_ERR_CAPABILITY_MISMATCH, "more than 2^25 rows of heads");
+  return JERO_OK;
+}
+
+}  // namespace jero
+
+using namespace jero;
+
+extern "C" size_t jero_hip_paged_attention_workspace_bytes(const jero_paged_cache* cache, int64_t n_tokens, int n_heads) {
+  if (check_paged(cache, n_tokens, n_heads)) return 0;
+  return part_bytes(paged_plan(cache, n_tokens, n_heads), n_tokens, n_heads, cache->head_dim, nullptr);
+}
+
+extern "C" int jero_hip_paged_attention(const jero_paged_cache* cache, int act_dtype, const void* q_dev, int64_t q_stride,
+                                        int64_t n_tokens, int n_heads, float scale, void* out_dev, int64_t out_stride,
+                                        void* workspace_dev, size_t workspace_bytes, void* stream) {
+  auto bad = [](int status, const char* what) { return fail(status, std::string("paged_attention: ") + what); };
+  int rc = check_paged(cache, n_tokens, n_heads);
+  if (rc) return rc;
+  if (act_dtype != JERO_F32 && act_dtype != JERO_F16)
+    return bad(JERO_ERR_CAPABILITY_MISMATCH, "activations must be JERO_F32 or JERO_F16");
+  if (act_dtype == JERO_F16 && cache->kv_dtype != JERO_KV_F16)
+    return bad(JERO_ERR_CAPABILITY_MISMATCH, "f16 activations need an f16 cache");
+  if (!q_dev || !out_dev) return bad(JERO_ERR_INVALID_ARGUMENT, "null pointer");
+  if ((reinterpret_cast<uintptr_t>(q_dev) | reinterpret_cast<uintptr_t>(out_dev)) & 15u)
+    return bad(JERO_ERR_INVALID_ARGUMENT, "q and out must be 16-byte aligned");
+  if (q_stride < int64_t(n_heads) * cache->head_dim || out_stride < int64_t(n_heads) * cache->head_dim)
+    return bad(JERO_ERR_TENSOR_BOUNDS, "rows overlap: a stride is below its row's length");
+  if (q_stride % 8 || out_stride % 8) return bad(JERO_ERR_INVALID_ARGUMENT, "strides must be multiples of 8 elements");
+  if (!std::isfinite(scale)) return bad(JERO_ERR_INVALID_ARGUMENT, "scale must be finite");
+  const PagedPlan p = paged_plan(cache, n_tokens, n_heads);
+  size_t ml = 0;
+  const size_t need = part_bytes(p, n_tokens, n_heads, cache->head_dim, &ml);
+  if (need) {
+    if (!workspace_dev) {
+      if ((rc = workspace(need, &workspace_dev))) return rc;
+    } else if (workspace_bytes < need) {
+      return fail(JERO_ERR_TENSOR_BOUNDS, "paged_attention: workspace of " + std::to_string(workspace_bytes) +
+                                              " bytes, need " + std::to_string(need));
+    } else if (reinterpret_cast<uintptr_t>(workspace_dev) & 255u) {
+      return bad(JERO_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+    }
+  }
+  PagedCall c{};
+  c.k = cache->k_dev, c.v = cache->v_dev;
+  c.table = cache->table_dev, c.lens = cache->lens_dev, c.starts = cache->starts_dev, c.shared = cache->shared_dev;
+  c.table_stride = cache->table_stride;
+  c.q_stride = q_stride, c.out_stride = out_stride;
+  c.n_blocks = uint32_t(cache->n_blocks);
+  c.n_seqs = int(cache->n_seqs), c.n_tokens = int(n_tokens), c.max_len = int(cache->max_len);
+  c.shared_len = int(std::min<int64_t>(cache->shared_blocks * cache->block_size, cache->max_len));
+  c.shift = __builtin_ctz(unsigned(cache->block_size));
+  c.heads = n_heads, c.kv_heads = cache->n_heads_kv, c.group = n_heads / cache->n_heads_kv, c.dim = cache->head_dim;
+  c.scale = scale;
+  float* part_o = static_cast<float*>(workspace_dev);
+  float2* part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace_dev) + ml);
+  const bool x16 = act_dtype == JERO_F16, kv16 = cache->kv_dtype == JERO_KV_F16;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int hd = head_width(c.dim);
+  rc = (hd == 64 ? paged_attend_64 : hd == 128 ? paged_attend_128 : paged_attend_256)(c, p, x16, kv16, q_dev, out_dev, part_o,
+                                                                                    part_ml, s);
+  if (rc || p.parts == 1) return rc;
+  const dim3 grid = {unsigned(n_tokens), unsigned((c.heads * c.dim + 1023) / 1024), 1};
+  if (x16)
+    hipLaunchKernelGGL((paged_merge_kernel<_Float16>), grid, dim3(256), 0, s, c, p, static_cast<_Float16*>(out_dev), part_o,
+                       part_ml);
+  else
+    hipLaunchKernelGGL((paged_merge_kernel<float>), grid, dim3(256), 0, s, c, p, static_cast<float*>(out_dev), part_o, part_ml);
+  return check_launch("paged_attention merge");
+}

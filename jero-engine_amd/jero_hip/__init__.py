@@ -87,6 +87,8 @@ _SIGS = {
     "jero_hip_rope_init": (_I32, [_P, _I32, _I32, C.c_double, _I32, C.c_double, C.c_double, C.c_double, C.c_double]),
     "jero_hip_paged_append": (_I32, [_I32, _P, _I64, _P, _I64, _P, _I64, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P, _F,
                                      _P, _I64, _P, _P, _I32, _I64, _P]),
+    "jero_hip_paged_attention_workspace_bytes": (_SZ, [_P, _I64, _I32]),
+    "jero_hip_paged_attention": (_I32, [_P, _I32, _P, _I64, _I64, _I32, _F, _P, _I64, _P, _SZ, _P]),
     "jero_hip_verify_drafts_workspace_bytes": (_SZ, [_I64, _I64]),
     "jero_hip_verify_drafts": (_I32, [_P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _SZ,
                                       _P]),
@@ -829,6 +831,64 @@ def rope(out, x, positions, rope, norm=None, eps=1e-6, stream=None):
                                       _paged_ints(what, "positions", positions, x.device, T), None, rope.ref,
                                       _paged_norm(what, "norm", norm, x), None, eps, out.data_ptr(), os_, None, None, KV_F16,
                                       0, s))
+    return out
+
+
+class HipPagedCache(C.Structure):
+    """jero_paged_cache."""
+    _fields_ = [(n, C.c_void_p) for n in ("k_dev", "v_dev", "table_dev", "lens_dev", "starts_dev", "shared_dev")] + \
+               [(n, C.c_int64) for n in ("n_blocks", "table_stride", "n_seqs", "max_len", "shared_blocks")] + \
+               [(n, C.c_int) for n in ("block_size", "kv_dtype", "n_heads_kv", "head_dim")]
+
+
+class PagedCache:
+    """A paged key/value cache and a call's sequences (jero_paged_cache): ``k`` and ``v`` [n_blocks, block_size,
+    kv_heads, head_dim] f32 or f16, ``table`` [n_seqs, blocks] int32 block ids, ``lens`` [n_seqs] int32 positions of
+    each sequence with the call's tokens among them, ``starts`` [n_seqs + 1] int32 first token row of each sequence
+    (None: one token each), ``shared`` int32 ids of the blocks that all sequences begin with (None: none).  Device
+    tensors, held and read as they are when a call runs; max_len (default: all a table row holds) bounds the
+    positions looked at."""
+
+    def __init__(self, k, v, table, lens, starts=None, max_len=None, shared=None):
+        import torch
+        device, dtype = k.device, k.dtype
+        ints, what = _paged_ints, "PagedCache"
+        if not (k.is_cuda and dtype in (torch.float16, torch.float32) and v.dtype is dtype and v.device == device
+                and k.dim() == 4 and v.shape == k.shape and k.is_contiguous() and v.is_contiguous() and table.dim() == 2):
+            _latent_check(k.is_cuda and v.device == device, 21, "PagedCache: k and v must be on one GPU")
+            _latent_check(dtype in (torch.float16, torch.float32) and v.dtype is dtype, 10,
+                          "PagedCache: k and v must both be float32 or float16")
+            _latent_check(k.dim() == 4 and v.shape == k.shape and table.dim() == 2, 14,
+                          "PagedCache: k and v [blocks, block_size, kv_heads, head_dim], table [seqs, blocks]")
+            _latent_check(False, 21, "PagedCache: k and v must be contiguous")
+        shape, (n, cols) = k.shape, table.shape
+        self.k, self.v, self.table, self.lens, self.starts, self.shared = k, v, table, lens, starts, shared
+        shared_blocks = 0 if shared is None else shared.numel()
+        self.c = HipPagedCache(k.data_ptr(), v.data_ptr(), ints(what, "table", table, device),
+                               ints(what, "lens", lens, device, n),
+                               None if starts is None else ints(what, "starts", starts, device, n + 1),
+                               ints(what, "shared", shared, device) if shared_blocks else None, shape[0], cols, n,
+                               cols * shape[1] if max_len is None else max_len, shared_blocks, shape[1],
+                               KV_F16 if dtype is torch.float16 else KV_F32, shape[2], shape[3])
+        self.ref = C.byref(self.c)
+
+
+def paged_attention(out, q, cache, scale, workspace=None, stream=None):
+    """Causal attention of a batch over a paged cache, positions that all sequences share read once for many
+    (jero_hip_paged_attention): q [tokens, heads, head_dim] f32 or f16, rotated, out like it (tokens may be apart).
+    The tokens' own rows have been stored."""
+    what = "paged_attention"
+    act = _paged_act(what, q)
+    _latent_check(q.device == cache.k.device, 21, what, "q must be on the cache's GPU")
+    qs, os_ = _paged_rows(what, "q", q, q), _paged_rows(what, "out", out, q)
+    _latent_check(out.shape == q.shape and q.shape[2] == cache.c.head_dim, 14, what,
+                  "q and out must be [tokens, heads, head_dim] of the cache's head_dim")
+    T, H = q.shape[:2]
+    L, s = lib(), _paged_stream(q.device, stream)
+    need = L.jero_hip_paged_attention_workspace_bytes(cache.ref, T, H)
+    ws, n = _latent_workspace(workspace, need, q, stream) if need else (None, 0)
+    check(L.jero_hip_paged_attention(cache.ref, act, q.data_ptr(), qs, T, H, scale, out.data_ptr(), os_,
+                                     None if ws is None else ws.data_ptr(), n, s))
     return out
 
 

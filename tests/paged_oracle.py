@@ -89,32 +89,35 @@ def rotated(x, positions, freq, magnitude, layout, norm=None, eps=0.0):
 
 
 def attend(q, k, v, table, lens, starts, scale, block, n_blocks, shared=(), max_len=None):
-    """q [T][H][D], pools [n_blocks][block][KV][D]; rows of no sequence come back as NaN."""
+    """q [T][H][D], pools [n_blocks][block][KV][D].  Returns the outputs, the same sums of |v| in v's place, the largest
+    scale * sum |q k| of each row's scores, and the positions it sees; rows of no sequence are NaN."""
     T, H, D = q.shape
-    KV = k.shape[2]
-    G = H // KV
-    out = np.full((T, H, v.shape[3]), np.nan)
+    G = H // k.shape[2]
+    out, size = np.full((T, H, D), np.nan), np.zeros((T, H, D))
+    most, seen = np.zeros((T, H)), np.zeros(T, np.int64)
     S, M = table.shape
     max_len = M * block if max_len is None else max_len
     for s in range(S):
         lo, hi = (s, s + 1) if starts is None else (int(starts[s]), int(starts[s + 1]))
         for t in range(max(lo, 0), min(hi, T)):
-            pos = int(lens[s]) - hi + t
-            seen = []
-            for p in range(min(pos + 1, max_len)):
-                b = int(shared[p // block]) if p < len(shared) * block else int(table[s, p // block])
-                if 0 <= b < n_blocks:
-                    seen.append((b, p % block))
-            if not seen:
+            p = np.arange(max(min(int(lens[s]) - hi + t + 1, max_len), 0))
+            ids = np.concatenate([np.asarray(shared, np.int64), table[s, len(shared):].astype(np.int64)])[p // block]
+            there = (ids >= 0) & (ids < n_blocks)
+            p, ids = p[there], ids[there]
+            seen[t] = len(p)
+            if not len(p):
                 out[t] = 0.0
                 continue
-            bi, oi = np.array(seen).T
-            for h in range(H):
-                kk, vv = k[bi, oi, h // G].astype(np.float64), v[bi, oi, h // G].astype(np.float64)
-                a = kk @ q[t, h].astype(np.float64) * scale
-                e = np.exp(a - a.max())
-                out[t, h] = (e @ vv) / e.sum()
-    return out
+            for j in range(H // G):
+                kk, vv = k[ids, p % block, j].astype(np.float64), v[ids, p % block, j].astype(np.float64)
+                qq = q[t, j * G:(j + 1) * G].astype(np.float64)
+                a = qq @ kk.T * scale
+                e = np.exp(a - a.max(1, keepdims=True))
+                e /= e.sum(1, keepdims=True)
+                out[t, j * G:(j + 1) * G] = e @ vv
+                size[t, j * G:(j + 1) * G] = e @ np.abs(vv)
+                most[t, j * G:(j + 1) * G] = (np.abs(qq) @ np.abs(kk).T).max(1) * abs(scale)
+    return out, size, most, seen
 
 
 def verify(target, draft, tokens, starts, u, u_last):

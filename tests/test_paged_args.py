@@ -130,3 +130,48 @@ def test_bad_verify():
     size = J.lib().jero_hip_verify_drafts_workspace_bytes
     assert size(0, 100) == size(65536, 100) == size(2, 0) == size(2, (1 << 24) + 1) == 0
     assert size(2, 100) == 32 and size(2, 4097) == 64
+
+
+def cache(**kw):
+    d = dict(k_dev=FAKE, v_dev=FAKE, table_dev=FAKE, lens_dev=FAKE, starts_dev=None, shared_dev=None, n_blocks=8,
+             table_stride=4, n_seqs=2, max_len=64, shared_blocks=0, block_size=16, kv_dtype=J.KV_F16, n_heads_kv=2, head_dim=64)
+    d.update(kw)
+    return J.HipPagedCache(**d)
+
+
+def attention(c, act=J.F32, q=FAKE, qs=256, tokens=2, heads=4, scale=0.1, out=FAKE, os_=256, ws=FAKE, n=1 << 30):
+    return J.lib().jero_hip_paged_attention(C.byref(c) if c else None, act, q, qs, tokens, heads, scale, out, os_, ws, n, None)
+
+
+BAD_CACHES = [
+    (dict(k_dev=None), 21), (dict(v_dev=None), 21), (dict(table_dev=None), 21), (dict(lens_dev=None), 21),
+    (dict(k_dev=FAKE + 8), 21), (dict(v_dev=FAKE + 4), 21), (dict(table_dev=FAKE + 2), 21), (dict(lens_dev=FAKE + 1), 21),
+    (dict(starts_dev=FAKE + 2), 21), (dict(shared_dev=FAKE + 2), 21), (dict(kv_dtype=2), 10), (dict(head_dim=0), 10),
+    (dict(head_dim=60), 10), (dict(head_dim=264), 10), (dict(block_size=0), 10), (dict(block_size=24), 10),
+    (dict(block_size=1 << 21), 10), (dict(n_blocks=0), 14), (dict(n_blocks=1 << 31), 14), (dict(n_seqs=0), 14),
+    (dict(n_seqs=1), 14), (dict(n_seqs=3), 14), (dict(n_heads_kv=0), 14), (dict(n_heads_kv=3), 14), (dict(max_len=0), 14),
+    (dict(max_len=65), 14), (dict(table_stride=0), 14), (dict(shared_blocks=1), 14), (dict(shared_blocks=-1), 14),
+    (dict(shared_blocks=5, shared_dev=FAKE), 14), (dict(max_len=4194305), 12),
+]
+
+
+def test_bad_attention():
+    assert attention(None) == 21
+    size = J.lib().jero_hip_paged_attention_workspace_bytes
+    for kw, status in BAD_CACHES:
+        assert attention(cache(**kw)) == status, kw
+        assert size(C.byref(cache(**kw)), 2, 4) == 0, kw
+    c = cache()
+    assert attention(c, act=J.BF16) == 10 and attention(cache(kv_dtype=J.KV_F32), act=J.F16) == 10
+    for kw in (dict(q=None), dict(out=None), dict(q=FAKE + 8), dict(out=FAKE + 4), dict(qs=260), dict(os_=260),
+               dict(scale=float("nan")), dict(scale=float("inf"))):
+        assert attention(c, **kw) == 21, kw
+    for kw in (dict(heads=0), dict(heads=3), dict(tokens=0), dict(tokens=1 << 23), dict(qs=248), dict(os_=248)):
+        assert attention(c, **kw) == 14, kw
+    assert attention(c, heads=1026) == 10
+    # a call whose positions are cut wants room for its parts
+    long = cache(table_stride=1 << 10, max_len=1 << 14)
+    need = size(C.byref(long), 2, 4)
+    assert need > 0
+    assert attention(long, n=need - 1) == 14 and attention(long, ws=FAKE + 16, n=need) == 21
+    assert size(C.byref(cache()), 2, 4) == 0
