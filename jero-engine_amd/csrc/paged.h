@@ -14,7 +14,7 @@ struct PagedCall {
   const int32_t *table, *lens, *starts, *shared;
   int64_t table_stride, q_stride, out_stride;
   uint32_t n_blocks;
-  int n_seqs, n_tokens, max_len, shared_len;
+  int n_seqs, n_tokens, max_len, shared_len, shared_blocks;
   int shift;  // log2 of the block size
   int heads, kv_heads, group, dim;
   float scale;

@@ -253,8 +253,9 @@ struct PagedShape {
   static constexpr bool TWOQ = sizeof(X) == 4, TWOK = sizeof(KV) == 4;
   static constexpr int NJ = HD <= 128 ? 2 : 1, KR = TWOQ || HD == 256 ? 32 : 64;
   static constexpr int kRows = 64 * NJ;
-  static constexpr int kPlanes = TWOK ? 2 : 1, kBufs = TWOK ? 1 : 2;
+  static constexpr int kPlanes = TWOK ? 2 : 1;
   static constexpr int kPlane = KR * HD * 2, kBuf = 2 * kPlanes * kPlane;  // keys, then values
+  static constexpr int kBufs = TWOK ? 1 : HD == 256 ? 4 : 64 * 1024 / kBuf > 4 ? 4 : 64 * 1024 / kBuf;
   static constexpr int kNarrow = 32 * HD * 2;                              // a wave's values
   static constexpr int kWaveLds = kNarrow * (TWOK ? 2 : 2);                // two buffers, or two parts
   static constexpr int kJoin = 4 * 16 * (HD + 4) * 4;
@@ -295,13 +296,34 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
   const KV* const vb = static_cast<const KV*>(c.v) + int64_t(it.head) * D;
   const int32_t* const table = c.table + it.seq * c.table_stride;
   const void* const zeros = kPagedZeros;
+  // A load to LDS of 1024 bytes holds RPI rows.  Where all positions of a step are there and blocks hold that many, its
+  // rows follow each other from one address for the whole wave (values behind head_dim are then the row's first: no
+  // query's, and not stored).
+  constexpr int RPI = 1024 / (2 * HD);
+  const int shift_mask = (1 << c.shift) - 1;
+  const int64_t row_bytes = row_len * int64_t(sizeof(KV)), block_bytes = row_bytes << c.shift;
+  auto offset_of = [&](uint32_t ids, int r, int p0) -> int64_t {  // of row r of a step, the wave's
+    const uint32_t id = __builtin_amdgcn_readlane(ids, r);
+    return int64_t(id) * block_bytes + int64_t((p0 + r) & shift_mask) * row_bytes;
+  };
 
-  // The block of a position; ~0: none, or not the item's.
-  auto block_of = [&](int pos) -> uint32_t {
-    if (pos >= it.hi) return ~0u;
-    const int b = pos >> c.shift;
-    const uint32_t id = uint32_t(pos < c.shared_len ? c.shared[b] : table[b]);
-    return id < c.n_blocks ? id : ~0u;
+  // The block of the lane's position of a step from p0 on; ~0: none, or not the item's.  64 blocks' ids are kept, a lane
+  // each, and the load that renews them is waited for where it is made: a wait further on would be for all loads in flight.
+  uint32_t window = ~0u;
+  int window0 = INT32_MIN / 2;
+  auto blocks_of = [&](int p0, int kr) -> uint32_t {
+    const int b0 = p0 >> c.shift;
+    if (b0 - window0 >= kWave) {
+      window0 = b0;
+      const int b = b0 + lane;
+      window = ~0u;
+      if (int64_t(b) << c.shift < it.hi) window = uint32_t(b < c.shared_blocks ? c.shared[b] : table[b]);
+      asm volatile("" : "+v"(window));
+      window = window < c.n_blocks ? window : ~0u;
+    }
+    const int pos = p0 + (lane & (kr - 1));
+    const uint32_t id = __shfl(window, (pos >> c.shift) - window0, kWave);
+    return pos < it.hi ? id : ~0u;
   };
   auto row_of = [&](const KV* base, uint32_t id, int pos) -> const uint8_t* {
     return reinterpret_cast<const uint8_t*>(base + ((int64_t(id) << c.shift) + (pos & ((1 << c.shift) - 1))) * row_len);
@@ -400,10 +422,23 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
     __syncthreads();
     const int common = s_low;  // below it, all rows of the workgroup see a position
     const int steps = (it.hi - it.lo + KR - 1) / KR;
-    auto find = [&](int step) { return block_of(it.lo + step * KR + (lane & (KR - 1))); };
     constexpr int NI = S::kPlane / 1024 / 4;  // 1024-byte pieces a wave, of keys and of values
+    const int lane_row = lane / (HD / 8);
+    const int lane_at = (16 * lane) % (2 * HD) ^ (16 * swap8(wv * RPI + lane_row));  // (4 pieces further on: 16 rows)
+    const uint32_t lane_bytes = uint32_t(lane_row * row_bytes) + (lane_at < 2 * D ? lane_at : 0);
     auto load = [&](int step, int buf, uint32_t ids) {  // f16: straight to LDS
       const int p0 = it.lo + step * KR;
+      if (__ballot(ids != ~0u) == ~0ull && (1 << c.shift) >= RPI) {
+#pragma unroll
+        for (int n = 0; n < NI; n++) {
+          const int i = 4 * n + wv;
+          const int64_t at = offset_of(ids, i * RPI, p0);
+          const uint32_t to = lds0 + buf * S::kBuf + i * 1024;
+          dma_row(reinterpret_cast<const uint8_t*>(kb) + at, lane_bytes, to);
+          dma_row(reinterpret_cast<const uint8_t*>(vb) + at, lane_bytes, to + S::kPlane);
+        }
+        return;
+      }
 #pragma unroll
       for (int n = 0; n < NI; n++) {
         const int i = 4 * n + wv, b = i * 1024 + 16 * lane, r = b / (2 * HD);
@@ -449,26 +484,34 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
         }
     };
     const int kat = 16 * (g ^ swap8(col)), kat4 = 16 * ((4 + g) ^ swap8(col));
-    uint32_t ids = find(0), next = ids;
-    if (steps > 0) {
-      if constexpr (TWOK) fetch(0, ids);
-      else load(0, 0, ids);
-      next = find(1);
-    }
+    // tiles on their way: A of them, each kLoads loads a wave; and which of their positions are there
+    constexpr int A = TWOK ? 1 : S::kBufs - 1, kLoads = 2 * NI;
+    uint64_t there[A];
+    auto ask = [&](int i, int to) -> uint64_t {
+      if (i >= steps) return 0;
+      const uint32_t ids = blocks_of(it.lo + i * KR, KR);
+      if constexpr (TWOK) fetch(i, ids);
+      else load(i, to, ids);
+      return __ballot(ids != ~0u);
+    };
+#pragma unroll
+    for (int i = 0; i < A; i++) there[i] = ask(i, i);
+    int buf = 0;
     for (int i = 0; i < steps; i++) {
-      const int buf = TWOK ? 0 : i & 1, p0 = it.lo + i * KR;
-      uint64_t ok = __ballot(ids != ~0u);
+      const int p0 = it.lo + i * KR;
+      const uint64_t ok = there[0];
+#pragma unroll
+      for (int n = 0; n + 1 < A; n++) there[n] = there[n + 1];
       if constexpr (TWOK) {
         __syncthreads();  // the last step's reads
         put();
         __syncthreads();
-        ids = next;
-        if (i + 1 < steps) fetch(i + 1, ids), next = find(i + 2);
+        there[0] = ask(i + 1, 0);
       } else {
-        dma_wait<0>();
-        __syncthreads();
-        ids = next;
-        if (i + 1 < steps) load(i + 1, buf ^ 1, ids), next = find(i + 2);
+        if (i + A <= steps) dma_wait<(A - 1) * kLoads>();
+        else dma_wait<0>();
+        __syncthreads();  // (and the last step's reads are done: its buffer is the next to be filled)
+        there[A - 1] = ask(i + A, buf == 0 ? A : buf - 1);
       }
       uint8_t* const kv = s_kv + buf * S::kBuf;
       uint64_t bad = 0;
@@ -498,6 +541,7 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
       };
       const bool masked = p0 + KR > low || ok != ~0ull || p0 + KR > it.hi;
       attend_step<HD, NJ, KR, TWOQ, TWOK>(st, kread, kv + S::kPlanes * S::kPlane, S::kPlane, vat, p0, masked, ok, bad, g);
+      if (!TWOK) buf = buf == S::kBufs - 1 ? 0 : buf + 1;
     }
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
@@ -515,20 +559,31 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
   // -------------------------------------------------------------- D
   constexpr int KR = 32;
   AttendState<HD, NB, TWOQ> st;
-  queries(st, 0);
-  const int low = lowest(st);
   const int steps = (it.hi - it.lo + KR - 1) / KR;
   uint8_t* const mine = s_kv + wv * S::kWaveLds;
   const uint32_t mine0 = lds0 + wv * S::kWaveLds;
-  auto find = [&](int step) { return block_of(it.lo + step * KR + (lane & (KR - 1))); };
   constexpr bool AHEAD = !(TWOK && HD == 256);  // (its registers hold one step)
   constexpr int KRAW = TWOK ? 2 : 1;            // 16-byte pieces for 8 values
   u32x4 kraw[2][KT][KRAW];                      // keys: row 16 r + col, values 32 k + 8 g ..
   constexpr int NV = TWOK ? 32 * HD / 8 / 64 : 1;
   u32x4 vraw[NV][2];
+  // (a piece's rows are swapped by their number's last three bits: with 2 or 4 rows a piece, 4 or 2 patterns)
+  constexpr int PAT = RPI < 8 ? 8 / RPI : 1;
+  uint32_t lane_bytes[PAT];
+#pragma unroll
+  for (int i = 0; i < PAT; i++) {
+    const int r = i * RPI + lane / (HD / 8), at = (16 * lane) % (2 * HD) ^ (16 * swap8(r));
+    lane_bytes[i] = uint32_t(lane / (HD / 8) * row_bytes) + (at < 2 * D ? at : 0);
+  }
   auto fetch = [&](int step, int buf, uint32_t ids) {
     const int p0 = it.lo + step * KR;
-    if constexpr (!TWOK) {
+    const bool whole = __ballot(ids != ~0u) == ~0ull;
+    if (!TWOK && whole && (1 << c.shift) >= RPI) {
+#pragma unroll
+      for (int i = 0; i < S::kNarrow / 1024; i++)
+        dma_row(reinterpret_cast<const uint8_t*>(vb) + offset_of(ids, i * RPI, p0), lane_bytes[i % PAT],
+                mine0 + buf * S::kNarrow + i * 1024);
+    } else if constexpr (!TWOK) {
 #pragma unroll
       for (int i = 0; i < S::kNarrow / 1024; i++) {
         const int b = i * 1024 + 16 * lane, r = b / (2 * HD), at = (b % (2 * HD)) ^ (16 * swap8(r));
@@ -546,6 +601,20 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
         vraw[n][1] = *reinterpret_cast<const u32x4*>(p + (on ? 16 : 0));
       }
     }
+    if (whole && c.shift >= 4) {
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const uint8_t* row = reinterpret_cast<const uint8_t*>(kb) + offset_of(ids, 16 * r, p0);
+#pragma unroll
+        for (int k = 0; k < KT; k++) {
+          const int d = 32 * k + 8 * g;
+          const uint32_t at = uint32_t(col * row_bytes) + (d < D ? d : 0) * int(sizeof(KV));
+#pragma unroll
+          for (int e = 0; e < KRAW; e++) kraw[r][k][e] = *reinterpret_cast<const u32x4*>(row + at + 16 * e);
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int r = 0; r < 2; r++) {
       const uint32_t id = __shfl(ids, 16 * r + col, kWave);
@@ -560,16 +629,21 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
       }
     }
   };
-  uint32_t ids = find(wv), next = ids;
-  if (AHEAD && wv < steps) {
-    fetch(wv, 0, ids);
-    next = find(wv + 4);
-  }
+  uint64_t there = 0;
+  auto ask = [&](int i, int to) {
+    if (i >= steps) return;
+    const uint32_t ids = blocks_of(it.lo + i * KR, KR);
+    there = __ballot(ids != ~0u);
+    fetch(i, to, ids);
+  };
+  if (AHEAD) ask(wv, 0);  // (before the queries: both are on their way at once)
+  queries(st, 0);
+  const int low = lowest(st);
   int buf = 0;
   for (int i = wv; i < steps; i += 4) {
     const int p0 = it.lo + i * KR;
-    const uint64_t ok = __ballot(ids != ~0u);
-    if constexpr (!AHEAD) fetch(i, 0, ids), next = find(i + 4);
+    if constexpr (!AHEAD) ask(i, 0);
+    const uint64_t ok = there;
     dma_wait<0>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last step's reads of the buffer that is loaded next
     uint8_t* const vp = mine + (TWOK ? 0 : buf * S::kNarrow);
@@ -605,11 +679,7 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
         *reinterpret_cast<h8_t*>(to + S::kNarrow) = lo;
       }
     }
-    ids = next;
-    if (AHEAD && i + 4 < steps) {
-      fetch(i + 4, buf ^ 1, ids);
-      next = find(i + 8);
-    }
+    if (AHEAD) ask(i + 4, buf ^ 1);
     uint64_t bad = 0;
     if (min(p0 + KR, it.hi) > low) {
       constexpr int L = HD / 8;

@@ -8,36 +8,70 @@
 
 namespace jero {
 
-// Joins a row's parts: the chunks of the shared positions, then those of its own.  Workgroup (token, 1024 of its
-// results), a thread four of them.
-template <typename X>
+// Joins a row's (a token's head's) parts: the chunks of the shared positions, then those of its own.  DL lanes a part, four
+// results each, PL parts of a row at a time.
+template <typename X, int DL, int PL>
 __global__ void __launch_bounds__(256) paged_merge_kernel(PagedCall c, PagedPlan p, X* __restrict__ out,
                                                           const float* __restrict__ part_o,
                                                           const float2* __restrict__ part_ml) {
-  const int t = blockIdx.x, i = 4 * (blockIdx.y * 256 + threadIdx.x);
-  const int seen = paged_visible(c, t);
-  if (seen < 0 || i >= c.heads * c.dim) return;
-  const int h = i / c.dim;
+  constexpr int R = 256 / (DL * PL);
+  __shared__ f4_t s_v[R][PL][DL];
+  __shared__ float s_l[R][PL];
+  const int tid = threadIdx.x, d = 4 * (tid % DL), k0 = tid / DL % PL, r = tid / (DL * PL);
+  const int64_t row = int64_t(blockIdx.x) * R + r;
+  const int t = int(row / c.heads), h = int(row % c.heads);
+  const int seen = t < c.n_tokens ? paged_visible(c, t) : -1;
   const int shared = min(seen, c.shared_len);
-  const int pre = p.pre_chunks ? (shared + p.pre_len - 1) / p.pre_len : 0;
+  const int pre = p.pre_chunks && seen > 0 ? (shared + p.pre_len - 1) / p.pre_len : 0;
   const int own = seen > p.own_lo ? (seen - p.own_lo + p.own_len - 1) / p.own_len : 0;
-  const int64_t step = int64_t(c.n_tokens) * c.heads, row = int64_t(t) * c.heads + h;
+  const int64_t step = int64_t(c.n_tokens) * c.heads;
+  auto at = [&](int k) { return row + step * (k < pre ? k : p.pre_chunks + k - pre); };
   float m = -INFINITY;
-  for (int k = 0; k < pre + own; k++) m = fmaxf(m, part_ml[row + step * (k < pre ? k : p.pre_chunks + k - pre)].x);
+  for (int k = tid % DL; k < pre + own; k += DL) m = fmaxf(m, part_ml[at(k)].x);
+#pragma unroll
+  for (int off = 1; off < DL; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
   const float ref = m == -INFINITY ? 0.f : m;
   float l = 0.f;
   f4_t v = {0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < pre + own; k++) {
-    const int64_t at = row + step * (k < pre ? k : p.pre_chunks + k - pre);
-    const float2 ml = part_ml[at];
+  for (int k = k0; k < pre + own; k += PL) {
+    const float2 ml = part_ml[at(k)];
     const float e = __builtin_amdgcn_exp2f(ml.x - ref);
     l += e * ml.y;
-    v += e * *reinterpret_cast<const f4_t*>(part_o + at * c.dim + (i - h * c.dim));
+    if (d < c.dim) v += e * *reinterpret_cast<const f4_t*>(part_o + at(k) * c.dim + d);
   }
+  if constexpr (PL > 1) {
+    s_v[r][k0][tid % DL] = v;
+    if (tid % DL == 0) s_l[r][k0] = l;
+    __syncthreads();
+  }
+  if (k0 || d >= c.dim || seen < 0) return;
+#pragma unroll
+  for (int k = 1; k < PL; k++) v += s_v[r][k][tid % DL], l += s_l[r][k];
   const float inv = l != 0.f ? 1.0f / l : 0.f;
-  X* dst = out + t * c.out_stride + i;
+  X* dst = out + t * c.out_stride + int64_t(h) * c.dim + d;
 #pragma unroll
   for (int e = 0; e < 4; e++) dst[e] = X(v[e] * inv);
+}
+
+template <typename X>
+static void launch_merge(const PagedCall& c, const PagedPlan& p, void* out, const float* part_o, const float2* part_ml,
+                         hipStream_t s) {
+  const int64_t rows = int64_t(c.n_tokens) * c.heads;
+#define JERO_MERGE(DL, PL)                                                                                            \
+  hipLaunchKernelGGL((paged_merge_kernel<X, DL, PL>), dim3(unsigned((rows * DL * PL + 255) / 256)), dim3(256), 0, s, c, p, \
+                     static_cast<X*>(out), part_o, part_ml)
+  const bool few = p.parts <= 4;
+  if (c.dim <= 64) {
+    if (few) JERO_MERGE(16, 1);
+    else JERO_MERGE(16, 8);
+  } else if (c.dim <= 128) {
+    if (few) JERO_MERGE(32, 1);
+    else JERO_MERGE(32, 8);
+  } else {
+    if (few) JERO_MERGE(64, 1);
+    else JERO_MERGE(64, 4);
+  }
+#undef JERO_MERGE
 }
 
 static int head_width(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
@@ -164,6 +198,7 @@ extern "C" int jero_hip_paged_attention(const jero_paged_cache* cache, int act_d
   c.n_blocks = uint32_t(cache->n_blocks);
   c.n_seqs = int(cache->n_seqs), c.n_tokens = int(n_tokens), c.max_len = int(cache->max_len);
   c.shared_len = int(std::min<int64_t>(cache->shared_blocks * cache->block_size, cache->max_len));
+  c.shared_blocks = int(cache->shared_blocks);
   c.shift = __builtin_ctz(unsigned(cache->block_size));
   c.heads = n_heads, c.kv_heads = cache->n_heads_kv, c.group = n_heads / cache->n_heads_kv, c.dim = cache->head_dim;
   c.scale = scale;
@@ -175,11 +210,7 @@ extern "C" int jero_hip_paged_attention(const jero_paged_cache* cache, int act_d
   rc = (hd == 64 ? paged_attend_64 : hd == 128 ? paged_attend_128 : paged_attend_256)(c, p, x16, kv16, q_dev, out_dev, part_o,
                                                                                     part_ml, s);
   if (rc || p.parts == 1) return rc;
-  const dim3 grid = {unsigned(n_tokens), unsigned((c.heads * c.dim + 1023) / 1024), 1};
-  if (x16)
-    hipLaunchKernelGGL((paged_merge_kernel<_Float16>), grid, dim3(256), 0, s, c, p, static_cast<_Float16*>(out_dev), part_o,
-                       part_ml);
-  else
-    hipLaunchKernelGGL((paged_merge_kernel<float>), grid, dim3(256), 0, s, c, p, static_cast<float*>(out_dev), part_o, part_ml);
+  if (x16) launch_merge<_Float16>(c, p, out_dev, part_o, part_ml, s);
+  else launch_merge<float>(c, p, out_dev, part_o, part_ml, s);
   return check_launch("paged_attention merge");
 }
