@@ -497,7 +497,7 @@ typedef struct jero_paged_cache {
   int n_heads_kv, head_dim;
 } jero_paged_cache;
 #define JERO_MAX_PAGED_POSITIONS 4194304
-size_t jero_hip_paged_attention_workspace_bytes(const jero_paged_cache *cache, int64_t n_tokens, int n_heads);
+size_t jero_hip_paged_attention_workspace_bytes(const jero_paged_cache *cache, int act_dtype, int64_t n_tokens, int n_heads);
 int jero_hip_paged_attention(const jero_paged_cache *cache, int act_dtype, const void *q_dev, int64_t q_stride,
                              int64_t n_tokens, int n_heads, float scale, void *out_dev, int64_t out_stride,
                              void *workspace_dev, size_t workspace_bytes, void *stream);

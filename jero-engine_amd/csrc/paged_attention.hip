@@ -76,14 +76,18 @@ static void launch_merge(const PagedCall& c, const PagedPlan& p, void* out, cons
 
 static int head_width(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-static PagedPlan paged_plan(const jero_paged_cache* k, int64_t n_tokens, int n_heads) {
+static PagedPlan paged_plan(const jero_paged_cache* k, bool f16, int64_t n_tokens, int n_heads) {
   PagedPlan p{};
   const int group = n_heads / k->n_heads_kv, hd = head_width(k->head_dim), kv = k->n_heads_kv;
   const int64_t shared = std::min<int64_t>(k->shared_blocks * k->block_size, k->max_len);
   const int64_t rows = n_tokens * group, each = (n_tokens + k->n_seqs - 1) / k->n_seqs * group;
   p.wide_rows = hd <= 128 ? 128 : 64;
-  // rows of all sequences over the shared positions, where there is more than one and they do not fill tiles themselves
-  const bool apart = shared > 0 && k->n_seqs > 1 && each < p.wide_rows;
+  // Rows of all sequences go over the shared positions together where sequences do not fill tiles themselves and more than
+  // 48 MB are spared: 32 sequences x 256 shared positions x 8 heads of 128 (f16, 33 MB) 26 us and 30 apart and not, 8 x
+  // 1024 (29 MB) 24 and 19, 128 x 64 (33 MB) 60 and 55, 128 x 256 (133 MB) 59 and 61, 8 x 4096 (117 MB) 30 and 32,
+  // 128 x 4096 69 and 192.
+  const double pair = 2.0 * kv * k->head_dim * (k->kv_dtype == JERO_KV_F16 ? 2 : 4);  // bytes of a position
+  const bool apart = k->n_seqs > 1 && each < p.wide_rows && double(k->n_seqs - 1) * shared * pair >= 48e6;
   p.narrow_rows = hd < 256 && (each > 16 || (apart && rows > 16 && rows <= 32)) ? 32 : 16;
   p.own_wide = each > p.narrow_rows;
   p.own_lo = apart ? int(shared) : 0;
@@ -102,7 +106,14 @@ static PagedPlan paged_plan(const jero_paged_cache* k, int64_t n_tokens, int n_h
     p.pre_wide = rows > 32;
     const int pre_rows = p.pre_wide ? p.wide_rows : p.narrow_rows;
     p.pre_tiles = int((rows + pre_rows - 1) / pre_rows);
-    p.pre_len = length(shared, chunks(int64_t(p.pre_tiles) * kv, shared, 256, 256));
+    // Chunks that take no longer than the call: with the cards' rates of a workgroup over the shared positions (us a position)
+    // and of memory, four fifths of both phases' times one after the other.  64 f32 sequences, 8192 shared positions,
+    // up to 1500 own: chunks of 1024 positions 67 us, of 512 73, of 256 79; 256 f16 sequences, 32768 and 700: chunks of
+    // 8192 372 us, of 16384 430, of 4096 383.
+    const double rate = p.pre_wide ? (f16 ? 0.04 : 0.06) * (hd / 128.0) : 0.01, memory = 5e6;
+    const double both = double(p.pre_tiles) * kv * shared * rate / 512 + double(k->n_seqs) * span * 0.6 * pair / memory;
+    const int64_t least = int64_t(std::max(256.0, 0.8 * both / rate));
+    p.pre_len = length(shared, std::max<int64_t>(1, (shared + least - 1) / least));
     p.pre_chunks = int((shared + p.pre_len - 1) / p.pre_len);
     p.pre_blocks = p.pre_tiles * kv * p.pre_chunks;
   }
@@ -155,9 +166,10 @@ static int check_paged(const jero_paged_cache* c, int64_t n_tokens, int n_heads)
 
 using namespace jero;
 
-extern "C" size_t jero_hip_paged_attention_workspace_bytes(const jero_paged_cache* cache, int64_t n_tokens, int n_heads) {
+extern "C" size_t jero_hip_paged_attention_workspace_bytes(const jero_paged_cache* cache, int act_dtype, int64_t n_tokens,
+                                                           int n_heads) {
   if (check_paged(cache, n_tokens, n_heads)) return 0;
-  return part_bytes(paged_plan(cache, n_tokens, n_heads), n_tokens, n_heads, cache->head_dim, nullptr);
+  return part_bytes(paged_plan(cache, act_dtype == JERO_F16, n_tokens, n_heads), n_tokens, n_heads, cache->head_dim, nullptr);
 }
 
 extern "C" int jero_hip_paged_attention(const jero_paged_cache* cache, int act_dtype, const void* q_dev, int64_t q_stride,
@@ -177,7 +189,7 @@ extern "C" int jero_hip_paged_attention(const jero_paged_cache* cache, int act_d
     return bad(JERO_ERR_TENSOR_BOUNDS, "rows overlap: a stride is below its row's length");
   if (q_stride % 8 || out_stride % 8) return bad(JERO_ERR_INVALID_ARGUMENT, "strides must be multiples of 8 elements");
   if (!std::isfinite(scale)) return bad(JERO_ERR_INVALID_ARGUMENT, "scale must be finite");
-  const PagedPlan p = paged_plan(cache, n_tokens, n_heads);
+  const PagedPlan p = paged_plan(cache, act_dtype == JERO_F16, n_tokens, n_heads);
   size_t ml = 0;
   const size_t need = part_bytes(p, n_tokens, n_heads, cache->head_dim, &ml);
   if (need) {

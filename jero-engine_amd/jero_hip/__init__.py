@@ -87,7 +87,7 @@ _SIGS = {
     "jero_hip_rope_init": (_I32, [_P, _I32, _I32, C.c_double, _I32, C.c_double, C.c_double, C.c_double, C.c_double]),
     "jero_hip_paged_append": (_I32, [_I32, _P, _I64, _P, _I64, _P, _I64, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P, _F,
                                      _P, _I64, _P, _P, _I32, _I64, _P]),
-    "jero_hip_paged_attention_workspace_bytes": (_SZ, [_P, _I64, _I32]),
+    "jero_hip_paged_attention_workspace_bytes": (_SZ, [_P, _I32, _I64, _I32]),
     "jero_hip_paged_attention": (_I32, [_P, _I32, _P, _I64, _I64, _I32, _F, _P, _I64, _P, _SZ, _P]),
     "jero_hip_verify_drafts_workspace_bytes": (_SZ, [_I64, _I64]),
     "jero_hip_verify_drafts": (_I32, [_P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _SZ,
@@ -673,23 +673,61 @@ class HipBlockPool(C.Structure):
                [("block_size", C.c_int)]
 
 
-def _paged_stream(device, stream):
-    """The stream's handle; a call runs on the current device, which has to be the tensors'."""
-    import torch
-    _latent_check(device.index == torch.cuda.current_device(), 21, "the tensors must be on the current device")
-    _latent_check(stream is None or stream.device == device, 21, "the stream must be of the tensors' device")
-    return _stream(stream)
+# A step's calls are as short as a launch: torch's types, and its current device and stream as numbers, are found once, and
+# what a tensor must be is asked in one expression, whose parts are told apart only for what is refused.
+_paged = None
 
 
-def _paged_ints(what, name, t, device, count=None, dtype=None):
-    """Address of a packed integer array of `count` elements (None: any) on the device."""
-    import torch
-    dtype = dtype or torch.int32
-    if t.dtype is not dtype or t.device != device or not t.is_contiguous() or (count is not None and t.numel() != count):
-        _latent_check(t.device == device, 21, f"{what}: {name} must be on the same GPU as the others")
-        _latent_check(t.dtype is dtype and t.is_contiguous(), 21, f"{what}: {name} must be packed {dtype}")
-        _latent_check(False, 14, f"{what}: {name} must have {count} elements")
-    return t.data_ptr()
+class _Paged:
+    def __init__(self):
+        import torch
+        self.f32, self.f16, self.i32, self.i64, self.empty, self.u8 = (torch.float32, torch.float16, torch.int32, torch.int64,
+                                                                       torch.empty, torch.uint8)
+        self.stream_guard = torch.cuda.stream
+        torch.cuda.current_stream()  # the first use initializes torch's GPU state
+        get, device = (getattr(torch._C, n, None) for n in ("_cuda_getCurrentRawStream", "_cuda_getDevice"))
+        self.device = device or torch.cuda.current_device
+        self.raw = get or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+        self.lib = lib()
+
+
+def _paged_state():
+    global _paged
+    if _paged is None:
+        _paged = _Paged()
+    return _paged
+
+
+def _paged_stream(P, device, stream):
+    """The stream's handle; a call runs on the current device, which has to be the tensors' (its number)."""
+    _latent_check(device == P.device(), 21, "the tensors must be on the current device")
+    if stream is None:
+        return P.raw(device)
+    _latent_check(stream.device.index == device, 21, "the stream must be of the tensors' device")
+    return stream.cuda_stream
+
+
+def _paged_ints(what, name, t, device, dtype, count=None):
+    """Address of a packed array of `count` numbers (None: any) on the device."""
+    if t.dtype is dtype and t.get_device() == device and t.is_contiguous() and (count is None or t.numel() == count):
+        return t.data_ptr()
+    _latent_check(t.get_device() == device and device >= 0, 21, f"{what}: {name} must be on the same GPU as the others")
+    _latent_check(t.dtype is dtype and t.is_contiguous(), 21, f"{what}: {name} must be packed {dtype}")
+    _latent_check(False, 14, f"{what}: {name} must have {count} elements")
+
+
+def _paged_workspace(P, workspace, need, device, stream):
+    """(address, bytes) of the call's workspace, and what holds it."""
+    if workspace is None:
+        if stream is None:
+            workspace = P.empty(need, dtype=P.u8, device=device)
+        else:  # of the call's own stream: the allocator hands it on to later work of that stream only
+            with P.stream_guard(stream):
+                workspace = P.empty(need, dtype=P.u8, device=device)
+    else:
+        _latent_check(workspace.get_device() == device and workspace.is_contiguous(), 21,
+                      "workspace must be packed, on the tensors' GPU")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
 class BlockPool:
@@ -701,12 +739,12 @@ class BlockPool:
 
     def __init__(self, table, lens, owned, free, n_free, n_blocks, block_size, shared_blocks=0):
         _latent_check(table.is_cuda and table.dim() == 2, 21, "BlockPool: table must be [n_seqs, blocks], on a GPU")
-        (n, cols), device = table.shape, table.device
-        ints = _paged_ints
-        self.table, self.lens, self.owned, self.free, self.n_free = table, lens, owned, free, n_free
-        self.c = HipBlockPool(ints("BlockPool", "table", table, device), ints("BlockPool", "lens", lens, device, n),
-                              ints("BlockPool", "owned", owned, device, n), ints("BlockPool", "free", free, device),
-                              ints("BlockPool", "n_free", n_free, device, 1), None, None, None, n, cols, n_blocks,
+        (n, cols), device = table.shape, table.get_device()
+        i32, ints, what = _paged_state().i32, _paged_ints, "BlockPool"
+        self.table, self.lens, self.owned, self.free, self.n_free, self.device = table, lens, owned, free, n_free, device
+        self.c = HipBlockPool(ints(what, "table", table, device, i32), ints(what, "lens", lens, device, i32, n),
+                              ints(what, "owned", owned, device, i32, n), ints(what, "free", free, device, i32),
+                              ints(what, "n_free", n_free, device, i32, 1), None, None, None, n, cols, n_blocks,
                               free.numel(), shared_blocks, block_size)
 
 
@@ -716,27 +754,23 @@ def paged_extend(pool, new, positions, slots, starts, drop=None, granted=None, i
     table and free ids, ``starts`` [n_seqs + 1] int32, ``positions`` int32 and ``slots`` int64 of the call's token
     rows (-1 behind the last), ``granted`` [n_seqs] int32 or None, and lens, owned and n_free in place, or
     ``into`` three tensors like them."""
-    import torch
-    what, c, device = "paged_extend", pool.c, pool.table.device
+    P = _paged_state()
+    what, c, device, i32, ints = "paged_extend", pool.c, pool.device, P.i32, _paged_ints
     n, T = c.n_seqs, positions.numel()
-    ints = _paged_ints
     if into is not None:
-        d = HipBlockPool()
-        C.memmove(C.byref(d), C.byref(c), C.sizeof(d))
-        d.lens_out_dev = ints(what, "lens", into[0], device, n)
-        d.owned_out_dev = ints(what, "owned", into[1], device, n)
-        d.n_free_out_dev = ints(what, "n_free", into[2], device, 1)
-        c = d
-    s = _paged_stream(device, stream)
-    L = lib()
-    ws, size = _latent_workspace(workspace, L.jero_hip_paged_extend_workspace_bytes(n), positions, stream) \
-        if workspace is not None or n > 1024 or T > 4096 else (None, 0)
-    check(L.jero_hip_paged_extend(C.byref(c), ints(what, "new", new, device, n),
-                                  None if drop is None else ints(what, "drop", drop, device, n), T,
-                                  ints(what, "starts", starts, device, n + 1),
-                                  None if granted is None else ints(what, "granted", granted, device, n),
-                                  ints(what, "positions", positions, device), ints(what, "slots", slots, device, T, torch.int64),
-                                  None if ws is None else ws.data_ptr(), size, s))
+        c = HipBlockPool(c.table_dev, c.lens_dev, c.owned_dev, c.free_dev, c.n_free_dev, ints(what, "lens", into[0], device, i32, n),
+                         ints(what, "owned", into[1], device, i32, n), ints(what, "n_free", into[2], device, i32, 1), n,
+                         c.table_stride, c.n_blocks, c.free_capacity, c.shared_blocks, c.block_size)
+    s = _paged_stream(P, device, stream)
+    ws = size = hold = None
+    if workspace is not None or n > 1024 or T > 4096:  # (smaller calls need none)
+        ws, size, hold = _paged_workspace(P, workspace, P.lib.jero_hip_paged_extend_workspace_bytes(n), device, stream)
+    check(P.lib.jero_hip_paged_extend(C.byref(c), ints(what, "new", new, device, i32, n),
+                                      None if drop is None else ints(what, "drop", drop, device, i32, n), T,
+                                      ints(what, "starts", starts, device, i32, n + 1),
+                                      None if granted is None else ints(what, "granted", granted, device, i32, n),
+                                      ints(what, "positions", positions, device, i32),
+                                      ints(what, "slots", slots, device, P.i64, T), ws, size or 0, s))
 
 
 class HipRope(C.Structure):
@@ -760,33 +794,23 @@ class Rope:
         self.ref = C.byref(self.c)
 
 
-def _paged_rows(what, name, t, like, heads_dim=None):
-    """Stride of a [tokens, heads, head_dim] tensor whose tokens' heads are packed."""
+def _paged_rows(what, name, t, dtype, device, T, D):
+    """(heads, stride) of a [tokens, heads, head_dim] tensor whose tokens' heads are packed."""
     shape, stride = t.shape, t.stride()
-    _latent_check(t.dtype is like.dtype and t.device == like.device, 21, what, f"{name} differs in type or device")
-    _latent_check(len(shape) == 3 and shape[0] == like.shape[0] and shape[2] == like.shape[2], 14, what,
-                  f"{name} must be [tokens, heads, head_dim]")
-    T, H, D = shape
-    _latent_check((D == 1 or stride[2] == 1) and (H == 1 or stride[1] == D), 21, what, f"{name}: a token's heads must be packed")
-    return stride[0] if T > 1 else H * D
+    if t.dtype is dtype and t.get_device() == device and len(shape) == 3 and shape[0] == T and shape[2] == D \
+            and stride[2] == 1 and (shape[1] == 1 or stride[1] == D):
+        return shape[1], stride[0] if T > 1 else shape[1] * D
+    _latent_check(t.get_device() == device and device >= 0, 21, what, f"{name} must be on the others' GPU")
+    _latent_check(t.dtype is dtype, 21, what, f"{name} differs in type")
+    _latent_check(len(shape) == 3 and shape[0] == T and shape[2] == D, 14, what, f"{name} must be [tokens, heads, head_dim]")
+    _latent_check(False, 21, what, f"{name}: a token's heads must be packed")
 
 
-def _paged_act(what, t):
-    import torch
-    _latent_check(t.is_cuda, 21, what, "the tensors must be on a GPU")
-    if t.dtype is torch.float32:
+def _paged_act(P, what, t):
+    if t.dtype is P.f32:
         return F32
-    _latent_check(t.dtype is torch.float16, 10, what, "activations must be float32 or float16")
+    _latent_check(t.dtype is P.f16, 10, what, "activations must be float32 or float16")
     return F16
-
-
-def _paged_norm(what, name, w, like):
-    import torch
-    if w is None:
-        return None
-    _latent_check(w.dtype is torch.float32 and w.device == like.device and w.is_contiguous()
-                  and w.numel() == like.shape[2], 14, what, f"{name} must be head_dim packed float32 values")
-    return w.data_ptr()
 
 
 def paged_append(k_rows, v_rows, q_out, q, k, v, positions, slots, rope, q_norm=None, k_norm=None, eps=1e-6, stream=None):
@@ -795,42 +819,44 @@ def paged_append(k_rows, v_rows, q_out, q, k, v, positions, slots, rope, q_norm=
     (q itself, or apart from it) and the pools k_rows, v_rows [..., kv_heads, head_dim] f32 or f16, whose rows
     ``slots`` [tokens] int64 counts; ``positions`` [tokens] int32.  A token of a position below 0 is left out, one
     of a slot that is none is not stored.  ``q_norm``, ``k_norm`` [head_dim] f32: heads are RMS-normalised first."""
-    import torch
-    what, device = "paged_append", k.device
-    act = _paged_act(what, k)
-    T, KV, D = k.shape if k.dim() == 3 else (0, 0, 0)
-    _latent_check(q.shape[1:2] != (0,), 14, what, "q has no heads")
-    ks, vs = _paged_rows(what, "k", k, k), _paged_rows(what, "v", v, k)
-    qs, qo = _paged_rows(what, "q", q, k), _paged_rows(what, "q_out", q_out, k)
-    _latent_check(v.shape == k.shape and q_out.shape == q.shape, 14, what, "k and v, or q and q_out, differ in shape")
-    kd = k_rows.dtype
-    _latent_check(kd in (torch.float32, torch.float16), 10, what, "the pools must be float32 or float16")
-    for rows in (k_rows, v_rows):
-        _latent_check(rows.dtype is kd and rows.device == device and rows.is_contiguous() and rows.shape == k_rows.shape
-                      and rows.dim() >= 3 and rows.shape[-2:] == (KV, D), 14, what,
-                      "the pools must be packed [..., kv_heads, head_dim], of one type, on the tokens' GPU")
-    s = _paged_stream(device, stream)
-    check(lib().jero_hip_paged_append(
-        act, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, T, q.shape[1], KV, D,
-        _paged_ints(what, "positions", positions, device, T), _paged_ints(what, "slots", slots, device, T, torch.int64),
-        None if rope is None else rope.ref, _paged_norm(what, "q_norm", q_norm, k), _paged_norm(what, "k_norm", k_norm, k),
-        eps, q_out.data_ptr(), qo, k_rows.data_ptr(), v_rows.data_ptr(), KV_F16 if kd is torch.float16 else KV_F32,
-        k_rows.numel() // (KV * D), s))
+    P = _paged_state()
+    what, device, dtype, rows, ints = "paged_append", k.get_device(), k.dtype, _paged_rows, _paged_ints
+    act = _paged_act(P, what, k)
+    _latent_check(k.dim() == 3, 14, what, "k must be [tokens, heads, head_dim]")
+    T, KV, D = k.shape
+    (_, ks), (vh, vs) = rows(what, "k", k, dtype, device, T, D), rows(what, "v", v, dtype, device, T, D)
+    (H, qs), (oh, qo) = rows(what, "q", q, dtype, device, T, D), rows(what, "q_out", q_out, dtype, device, T, D)
+    _latent_check(vh == KV and oh == H, 14, what, "k and v, or q and q_out, differ in shape")
+    kd, shape = k_rows.dtype, k_rows.shape
+    if not (kd is P.f16 or kd is P.f32):
+        _latent_check(False, 10, what, "the pools must be float32 or float16")
+    _latent_check(v_rows.dtype is kd and k_rows.get_device() == device == v_rows.get_device() and k_rows.is_contiguous()
+                  and v_rows.is_contiguous() and v_rows.shape == shape and len(shape) >= 3 and shape[-2] == KV
+                  and shape[-1] == D, 14, what,
+                  "the pools must be packed [..., kv_heads, head_dim], of one type, on the tokens' GPU")
+    check(P.lib.jero_hip_paged_append(
+        act, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, T, H, KV, D,
+        ints(what, "positions", positions, device, P.i32, T), ints(what, "slots", slots, device, P.i64, T),
+        None if rope is None else rope.ref, None if q_norm is None else ints(what, "q_norm", q_norm, device, P.f32, D),
+        None if k_norm is None else ints(what, "k_norm", k_norm, device, P.f32, D), eps, q_out.data_ptr(), qo,
+        k_rows.data_ptr(), v_rows.data_ptr(), KV_F16 if kd is P.f16 else KV_F32, k_rows.numel() // (KV * D),
+        _paged_stream(P, device, stream)))
 
 
 def rope(out, x, positions, rope, norm=None, eps=1e-6, stream=None):
     """The rotation alone: x [tokens, heads, head_dim] f32 or f16 into out (x itself, or apart from it), as
     paged_append rotates queries."""
-    what = "rope"
-    act = _paged_act(what, x)
-    xs, os_ = _paged_rows(what, "x", x, x), _paged_rows(what, "out", out, x)
-    _latent_check(out.shape == x.shape, 14, what, "x and out differ in shape")
+    P = _paged_state()
+    what, device = "rope", x.get_device()
+    act = _paged_act(P, what, x)
+    _latent_check(x.dim() == 3, 14, what, "x must be [tokens, heads, head_dim]")
     T, H, D = x.shape
-    s = _paged_stream(x.device, stream)
-    check(lib().jero_hip_paged_append(act, x.data_ptr(), xs, None, 0, None, 0, T, H, 0, D,
-                                      _paged_ints(what, "positions", positions, x.device, T), None, rope.ref,
-                                      _paged_norm(what, "norm", norm, x), None, eps, out.data_ptr(), os_, None, None, KV_F16,
-                                      0, s))
+    (_, xs), (oh, os_) = _paged_rows(what, "x", x, x.dtype, device, T, D), _paged_rows(what, "out", out, x.dtype, device, T, D)
+    _latent_check(oh == H, 14, what, "x and out differ in shape")
+    check(P.lib.jero_hip_paged_append(act, x.data_ptr(), xs, None, 0, None, 0, T, H, 0, D,
+                                      _paged_ints(what, "positions", positions, device, P.i32, T), None, rope.ref,
+                                      None if norm is None else _paged_ints(what, "norm", norm, device, P.f32, D), None, eps,
+                                      out.data_ptr(), os_, None, None, KV_F16, 0, _paged_stream(P, device, stream)))
     return out
 
 
@@ -850,45 +876,46 @@ class PagedCache:
     positions looked at."""
 
     def __init__(self, k, v, table, lens, starts=None, max_len=None, shared=None):
-        import torch
-        device, dtype = k.device, k.dtype
-        ints, what = _paged_ints, "PagedCache"
-        if not (k.is_cuda and dtype in (torch.float16, torch.float32) and v.dtype is dtype and v.device == device
-                and k.dim() == 4 and v.shape == k.shape and k.is_contiguous() and v.is_contiguous() and table.dim() == 2):
-            _latent_check(k.is_cuda and v.device == device, 21, "PagedCache: k and v must be on one GPU")
-            _latent_check(dtype in (torch.float16, torch.float32) and v.dtype is dtype, 10,
+        P = _paged_state()
+        device, dtype, i32, ints, what = k.get_device(), k.dtype, P.i32, _paged_ints, "PagedCache"
+        shape, blocks = k.shape, table.shape
+        if not (device >= 0 and (dtype is P.f16 or dtype is P.f32) and v.dtype is dtype and v.get_device() == device
+                and len(shape) == 4 and v.shape == shape and k.is_contiguous() and v.is_contiguous() and len(blocks) == 2):
+            _latent_check(device >= 0 and v.get_device() == device, 21, "PagedCache: k and v must be on one GPU")
+            _latent_check((dtype is P.f16 or dtype is P.f32) and v.dtype is dtype, 10,
                           "PagedCache: k and v must both be float32 or float16")
-            _latent_check(k.dim() == 4 and v.shape == k.shape and table.dim() == 2, 14,
+            _latent_check(len(shape) == 4 and v.shape == shape and len(blocks) == 2, 14,
                           "PagedCache: k and v [blocks, block_size, kv_heads, head_dim], table [seqs, blocks]")
             _latent_check(False, 21, "PagedCache: k and v must be contiguous")
-        shape, (n, cols) = k.shape, table.shape
+        n, cols = blocks
         self.k, self.v, self.table, self.lens, self.starts, self.shared = k, v, table, lens, starts, shared
         shared_blocks = 0 if shared is None else shared.numel()
-        self.c = HipPagedCache(k.data_ptr(), v.data_ptr(), ints(what, "table", table, device),
-                               ints(what, "lens", lens, device, n),
-                               None if starts is None else ints(what, "starts", starts, device, n + 1),
-                               ints(what, "shared", shared, device) if shared_blocks else None, shape[0], cols, n,
+        self.c = HipPagedCache(k.data_ptr(), v.data_ptr(), ints(what, "table", table, device, i32),
+                               ints(what, "lens", lens, device, i32, n),
+                               None if starts is None else ints(what, "starts", starts, device, i32, n + 1),
+                               ints(what, "shared", shared, device, i32) if shared_blocks else None, shape[0], cols, n,
                                cols * shape[1] if max_len is None else max_len, shared_blocks, shape[1],
-                               KV_F16 if dtype is torch.float16 else KV_F32, shape[2], shape[3])
-        self.ref = C.byref(self.c)
+                               KV_F16 if dtype is P.f16 else KV_F32, shape[2], shape[3])
+        self.ref, self.device, self.dim = C.byref(self.c), device, shape[3]
 
 
 def paged_attention(out, q, cache, scale, workspace=None, stream=None):
     """Causal attention of a batch over a paged cache, positions that all sequences share read once for many
     (jero_hip_paged_attention): q [tokens, heads, head_dim] f32 or f16, rotated, out like it (tokens may be apart).
     The tokens' own rows have been stored."""
-    what = "paged_attention"
-    act = _paged_act(what, q)
-    _latent_check(q.device == cache.k.device, 21, what, "q must be on the cache's GPU")
-    qs, os_ = _paged_rows(what, "q", q, q), _paged_rows(what, "out", out, q)
-    _latent_check(out.shape == q.shape and q.shape[2] == cache.c.head_dim, 14, what,
-                  "q and out must be [tokens, heads, head_dim] of the cache's head_dim")
-    T, H = q.shape[:2]
-    L, s = lib(), _paged_stream(q.device, stream)
-    need = L.jero_hip_paged_attention_workspace_bytes(cache.ref, T, H)
-    ws, n = _latent_workspace(workspace, need, q, stream) if need else (None, 0)
-    check(L.jero_hip_paged_attention(cache.ref, act, q.data_ptr(), qs, T, H, scale, out.data_ptr(), os_,
-                                     None if ws is None else ws.data_ptr(), n, s))
+    P = _paged_state()
+    what, device, L = "paged_attention", cache.device, P.lib
+    act = _paged_act(P, what, q)
+    T = q.shape[0] if q.dim() == 3 else 0
+    (H, qs), (oh, os_) = _paged_rows(what, "q", q, q.dtype, device, T, cache.dim), \
+        _paged_rows(what, "out", out, q.dtype, device, T, cache.dim)
+    _latent_check(oh == H, 14, what, "q and out differ in heads")
+    s = _paged_stream(P, device, stream)
+    need = L.jero_hip_paged_attention_workspace_bytes(cache.ref, act, T, H)
+    ws = size = hold = None
+    if need:
+        ws, size, hold = _paged_workspace(P, workspace, need, device, stream)
+    check(L.jero_hip_paged_attention(cache.ref, act, q.data_ptr(), qs, T, H, scale, out.data_ptr(), os_, ws, size or 0, s))
     return out
 
 
@@ -899,26 +926,24 @@ def verify_drafts(out, accepted, target, draft, tokens, starts, u, u_last, dropp
     each drafted token, sequence after sequence (None: it was sure of each); ``u`` [drafts] and ``u_last``
     [n_seqs] f32 numbers from [0, 1).  Writes ``out`` [tokens] int32, the tokens that stand, the one drawn, -1s;
     ``accepted`` and ``dropped`` (or None) [n_seqs] int32."""
-    import torch
-    what, device = "verify_drafts", target.device
-    n, T, f32 = starts.numel() - 1, tokens.numel(), torch.float32
-    _latent_check(target.is_cuda and target.dtype is f32 and target.dim() == 2 and target.shape[0] == T
+    P = _paged_state()
+    what, device, i32, f32, ints, L = "verify_drafts", target.get_device(), P.i32, P.f32, _paged_ints, P.lib
+    n, T = starts.numel() - 1, tokens.numel()
+    _latent_check(device >= 0 and target.dtype is f32 and target.dim() == 2 and target.shape[0] == T
                   and target.stride(1) == 1, 14, what, "target must be [tokens, vocab] float32 with packed rows, on a GPU")
     V, N = target.shape[1], u.numel()
     if draft is not None:
-        _latent_check(draft.device == device and draft.dtype is f32 and draft.shape == (N, V)
+        _latent_check(draft.get_device() == device and draft.dtype is f32 and draft.shape == (N, V)
                       and (N == 0 or draft.stride(1) == 1), 14, what, "draft must be [drafts, vocab] float32 with packed rows")
-    ints = _paged_ints
-    s = _paged_stream(device, stream)
-    L = lib()
-    ws, size = _latent_workspace(workspace, L.jero_hip_verify_drafts_workspace_bytes(n, V), target, stream)
+    s = _paged_stream(P, device, stream)
+    ws, size, hold = _paged_workspace(P, workspace, L.jero_hip_verify_drafts_workspace_bytes(n, V), device, stream)
     check(L.jero_hip_verify_drafts(
         target.data_ptr(), target.stride(0) if T > 1 else V, None if draft is None or N == 0 else draft.data_ptr(),
-        V if draft is None or N < 2 else draft.stride(0), ints(what, "tokens", tokens, device, T),
-        ints(what, "starts", starts, device, n + 1), ints(what, "u", u, device, N, f32) if N else None,
-        ints(what, "u_last", u_last, device, n, f32), n, T, N, V, ints(what, "out", out, device, T),
-        ints(what, "accepted", accepted, device, n), None if dropped is None else ints(what, "dropped", dropped, device, n),
-        ws.data_ptr(), size, s))
+        V if draft is None or N < 2 else draft.stride(0), ints(what, "tokens", tokens, device, i32, T),
+        ints(what, "starts", starts, device, i32), ints(what, "u", u, device, f32, N) if N else None,
+        ints(what, "u_last", u_last, device, f32, n), n, T, N, V, ints(what, "out", out, device, i32, T),
+        ints(what, "accepted", accepted, device, i32, n),
+        None if dropped is None else ints(what, "dropped", dropped, device, i32, n), ws, size, s))
 
 
 def dispatch_qwen3_moe_ffn(out, norm_ffn_in, router_logits, top_k, gate, up, down, workspace=None, stream=None,

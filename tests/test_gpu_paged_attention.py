@@ -153,6 +153,81 @@ def test_against_the_oracle(dev, case, act, kv):
     q.check(q.run(), what="with starts")
 
 
+# Batches that go over their shared positions together (which pays from 48 MB spared on): few rows, 17 to 32 of them, more
+# than a tile of 128; one and several tiles of a sequence's own rows, narrow and wide ones
+SHARED = [
+    ([780] + [770] * 8, [1] * 9, 16, 16, 128, 16, 48),
+    ([1600] * 12, [1] * 12, 32, 16, 64, 64, 24),
+    ([850, 834, 833, 840] * 6, [1] * 24, 16, 16, 80, 32, 26),
+    ([515, 600, 513] * 14, [1] * 42, 32, 8, 128, 16, 32),
+    ([530, 514, 513, 640] * 5, [1, 2, 0, 5] * 5, 40, 8, 256, 64, 8),
+    ([800, 705, 720] * 8, [4, 5, 1] * 8, 64, 8, 96, 64, 11),
+    ([1100, 1054] * 14, [12, 14] * 14, 16, 4, 128, 16, 65),
+]
+
+
+@pytest.mark.parametrize("act,kv", TYPES)
+@pytest.mark.parametrize("case", SHARED, ids=ids)
+def test_shared_positions(dev, case, act, kv):
+    print(f"paged_attention {act} {kv} {case}", flush=True)
+    p = problem(case, act, kv, pad_rows=0 if case[1] == [1] * len(case[1]) else 2).device(dev)
+    print("  off by", p.check(p.run()), flush=True)
+
+
+@pytest.mark.parametrize("act,kv", TYPES)
+def test_shared_positions_that_not_all_see(dev, act, kv):
+    """Empty sequences, the first among them, sequences that end within the shared positions, ids that are none, positions
+    from max_len on; values that are not finite are for those who see them."""
+    lens = [0, 600, 513, 100, 1, 530, 0, 512, 511] * 5
+    p = Problem(21, lens, [1] * 45, 16, 8, 128, 32, 16, act, kv, max_len=520)
+    p.shared[3] = -5
+    p.shared[9] = p.n_blocks
+    p.table[1, 16] = p.n_blocks
+    ref = p.oracle()
+    b = p.shared[512 // 32 - 1]
+    p.v[b, 30, 2, 7] = np.inf  # position 510: for the sequences of 511 positions and more
+    p.k[b, 29, 5, 1] = np.nan  # position 509
+    p.device(dev)
+    out = p.run()
+    sees = torch.tensor([n >= 511 for n in lens], device=dev)
+    assert not torch.isfinite(out[sees][:, 4:6, 7]).any() and not torch.isfinite(out[sees][:, 10:12]).any()
+    good = torch.from_numpy(ref[0]).to(out)
+    out[sees, 4:6] = good[sees, 4:6]
+    out[sees, 10:12] = good[sees, 10:12]
+    p.check(out, ref)
+    assert (out[0] == 0).all() and (out[6] == 0).all()
+
+
+def test_shared_positions_captured(dev):
+    """Replays over other lengths, tables and queries, with eager calls between; two graphs that share a workspace."""
+    p = Problem(22, [600] * 40, [1] * 40, 16, 8, 128, 16, 32).device(dev)
+    n = J.lib().jero_hip_paged_attention_workspace_bytes(p.cache.ref, J.F32, p.T, p.H)
+    assert n > 0
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    outs = [torch.zeros_like(p.d["q"]) for _ in range(2)]
+    graphs = []
+    for out in outs:
+        J.paged_attention(out, p.d["q"], p.cache, p.scale, workspace=ws)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            J.paged_attention(out, p.d["q"], p.cache, p.scale, workspace=ws)
+        graphs.append(g)
+    r = np.random.default_rng(3)
+    for i in range(4):
+        p.lens = r.integers(0, 601, 40).astype(np.int32)
+        p.q = np.roll(p.q, 1, 0)
+        p.d["lens"].copy_(torch.from_numpy(p.lens))
+        p.d["q"].copy_(torch.from_numpy(p.q))
+        for g, out in zip(graphs, outs):
+            out.fill_(5)
+            g.replay()
+        torch.cuda.synchronize()
+        eager = p.run(workspace=ws)
+        assert torch.equal(outs[0], eager) and torch.equal(outs[1], eager)
+    p.check(eager)
+
+
 @pytest.mark.parametrize("shared", [0, 2])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_rows_that_see_nothing_get_zeros(dev, shared, dim):
@@ -246,7 +321,7 @@ def test_tensors_apart_and_a_workspace_of_ones_own(dev):
     wide = torch.full((p.T, 2, p.H, p.D), 3.0, device=dev)
     wide[:, 1] = p.d["q"]
     out = torch.full((p.T, p.H + 1, p.D), 7.0, device=dev)
-    n = J.lib().jero_hip_paged_attention_workspace_bytes(p.cache.ref, p.T, p.H)
+    n = J.lib().jero_hip_paged_attention_workspace_bytes(p.cache.ref, J.F32, p.T, p.H)
     assert n > 0
     ws = torch.full((n,), 255, dtype=torch.uint8, device=dev)
     s = torch.cuda.Stream(dev)
@@ -262,7 +337,7 @@ def test_captured(dev):
     """One step captured, replayed over other lengths, tables and queries, with eager calls between."""
     p = Problem(13, [300, 200, 260], [1, 1, 1], 8, 2, 64, 16, 8).device(dev)
     out = torch.zeros_like(p.d["q"])
-    ws = torch.empty(J.lib().jero_hip_paged_attention_workspace_bytes(p.cache.ref, p.T, p.H), dtype=torch.uint8, device=dev)
+    ws = torch.empty(J.lib().jero_hip_paged_attention_workspace_bytes(p.cache.ref, J.F32, p.T, p.H), dtype=torch.uint8, device=dev)
     J.paged_attention(out, p.d["q"], p.cache, p.scale, workspace=ws)
     torch.cuda.synchronize()
     g = torch.cuda.CUDAGraph()
@@ -283,7 +358,7 @@ def test_captured(dev):
 
 def test_runs_repeat(dev):
     """The same bits each time, whatever the workspace held."""
-    for case in (CASES[15], PROMPTS[5], PROMPTS[6]):
+    for case in (CASES[15], PROMPTS[5], PROMPTS[6], SHARED[0], SHARED[4]):
         p = problem(case).device(dev)
         a = p.run()
         for _ in range(3):

@@ -160,7 +160,7 @@ def test_bad_attention():
     size = J.lib().jero_hip_paged_attention_workspace_bytes
     for kw, status in BAD_CACHES:
         assert attention(cache(**kw)) == status, kw
-        assert size(C.byref(cache(**kw)), 2, 4) == 0, kw
+        assert size(C.byref(cache(**kw)), J.F32, 2, 4) == 0, kw
     c = cache()
     assert attention(c, act=J.BF16) == 10 and attention(cache(kv_dtype=J.KV_F32), act=J.F16) == 10
     for kw in (dict(q=None), dict(out=None), dict(q=FAKE + 8), dict(out=FAKE + 4), dict(qs=260), dict(os_=260),
@@ -171,7 +171,7 @@ def test_bad_attention():
     assert attention(c, heads=1026) == 10
     # a call whose positions are cut wants room for its parts
     long = cache(table_stride=1 << 10, max_len=1 << 14)
-    need = size(C.byref(long), 2, 4)
+    need = size(C.byref(long), J.F32, 2, 4)
     assert need > 0
     assert attention(long, n=need - 1) == 14 and attention(long, ws=FAKE + 16, n=need) == 21
-    assert size(C.byref(cache()), 2, 4) == 0
+    assert size(C.byref(cache()), J.F32, 2, 4) == 0
