@@ -6,21 +6,22 @@ namespace jero {
 
 constexpr int kDraftChunk = 4096;  // of the vocabulary, a workgroup
 
-struct Drafts {
-  const float *target, *draft, *u, *u_last;
-  const int32_t *tokens, *starts;
-  int64_t target_stride, draft_stride;
-  int n_seqs, n_tokens, n_drafts, vocab, chunks;
-  int32_t *out, *accepted, *dropped;
-  double2* sums;  // [n_seqs][chunks]: of the weights, and of the target alone
-};
-
 // Where a sequence's next token is drawn from.
 struct Verdict {
   int first, rows, accepted;
   int row;       // of the target's probabilities; -1: no rows
   int less;      // the draft's row taken off, or -1
   int without;   // a token that gets no weight, or -1
+};
+
+struct Drafts {
+  const float *target, *draft, *u, *u_last;
+  const int32_t *tokens, *starts;
+  int64_t target_stride, draft_stride;
+  int n_seqs, n_tokens, n_drafts, vocab, chunks;
+  int32_t *out, *accepted, *dropped;
+  double* sums;       // [n_seqs][chunks]: of the weights
+  Verdict* verdicts;  // [n_seqs]
 };
 
 // By a whole workgroup of whole waves; s_n: one int of LDS.  Each wave finds the same.
@@ -75,34 +76,74 @@ __device__ __forceinline__ double weight_of(const Verdict& v, const float* p, co
   return i == v.without ? 0.0 : finite_weight(w);
 }
 
-// Workgroup (chunk, sequence): the sums of its chunk's weights.
-__global__ void __launch_bounds__(256) draft_sums_kernel(Drafts d) {
-  __shared__ int s_n;
-  __shared__ double2 s_sum[4];
-  const int s = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
-  const Verdict v = verdict_of(d, s, &s_n);
-  if (v.row < 0) return;
-  const int lo = blockIdx.x * kDraftChunk, hi = min(lo + kDraftChunk, d.vocab);
-  const float* p = d.target + v.row * d.target_stride;
-  const float* q = v.less >= 0 ? d.draft + v.less * d.draft_stride : nullptr;
-  double2 sum = {0.0, 0.0};
-#pragma unroll 4
-  for (int i = lo + tid; i < hi; i += 256) {
-    sum.x += weight_of(v, p, q, i);
-    sum.y += finite_weight(p[i]);
-  }
+// The weights of tokens [lo, lo + 4 n), four a lane and step: all loads before the sum.
+template <int N, typename L>
+__device__ __forceinline__ double sum_weights(const Verdict& v, const float* p, const float* q, int lo, int step, L load) {
+  float4 a[N], b[N];
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) sum.x += __shfl_xor(sum.x, off, kWave), sum.y += __shfl_xor(sum.y, off, kWave);
-  if (lane == 0) s_sum[tid >> 6] = sum;
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < 4; w++) sum.x += s_sum[w].x, sum.y += s_sum[w].y;
-    d.sums[int64_t(s) * d.chunks + blockIdx.x] = sum;
+  for (int n = 0; n < N; n++) a[n] = load(p + lo + n * step);
+  if (q)
+#pragma unroll
+    for (int n = 0; n < N; n++) b[n] = load(q + lo + n * step);
+  double sum = 0.0;
+#pragma unroll
+  for (int n = 0; n < N; n++) {
+    const float x[4] = {a[n].x, a[n].y, a[n].z, a[n].w}, y[4] = {b[n].x, b[n].y, b[n].z, b[n].w};
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const double w = q ? double(x[e]) - double(y[e]) : double(x[e]);
+      sum += lo + n * step + e == v.without ? 0.0 : finite_weight(w);
+    }
   }
+  return sum;
 }
 
-// Inclusive sums over 1024 threads; s: 16 of LDS.
-__device__ __forceinline__ double scan1024(double v, double* s, int tid) {
+// The sum of a chunk's weights, by 256 threads; s: 4 of LDS.  Thread 0 has it.
+__device__ __forceinline__ double chunk_sum(const Drafts& d, const Verdict& v, const float* p, const float* q, int chunk,
+                                            double* s, int tid) {
+  const int lo = chunk * kDraftChunk, hi = min(lo + kDraftChunk, d.vocab);
+  double sum = 0.0;
+  if (hi - lo == kDraftChunk) {
+    constexpr int N = kDraftChunk / 1024;
+    if (((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q)) & 15u) == 0) {
+      sum = sum_weights<N>(v, p, q, lo + 4 * tid, 1024, [](const float* x) { return *reinterpret_cast<const float4*>(x); });
+    } else {  // (rows of an odd vocabulary)
+      sum = sum_weights<N>(v, p, q, lo + 4 * tid, 1024, [](const float* x) { return make_float4(x[0], x[1], x[2], x[3]); });
+    }
+  } else {
+    for (int i = lo + tid; i < hi; i += 256) sum += weight_of(v, p, q, i);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
+  __syncthreads();
+  if ((tid & 63) == 0) s[tid >> 6] = sum;
+  __syncthreads();
+  return s[0] + s[1] + s[2] + s[3];
+}
+
+// Workgroup (chunk, sequence): the sum of its chunk's weights; the first chunk's writes what is known of the sequence.
+__global__ void __launch_bounds__(256) draft_sums_kernel(Drafts d) {
+  __shared__ int s_n;
+  __shared__ double s_sum[4];
+  const int s = blockIdx.y, tid = threadIdx.x;
+  const Verdict v = verdict_of(d, s, &s_n);
+  if (blockIdx.x == 0) {
+    if (tid == 0) {
+      d.verdicts[s] = v;
+      d.accepted[s] = v.accepted;
+      if (d.dropped) d.dropped[s] = max(v.rows - 1, 0) - v.accepted;
+    }
+    for (int i = tid; i < v.rows; i += 256)
+      if (i != v.accepted) d.out[v.first + i] = i < v.accepted ? d.tokens[v.first + i + 1] : -1;
+  }
+  if (v.row < 0) return;
+  const double sum = chunk_sum(d, v, d.target + v.row * d.target_stride,
+                               v.less >= 0 ? d.draft + v.less * d.draft_stride : nullptr, blockIdx.x, s_sum, tid);
+  if (tid == 0) d.sums[int64_t(s) * d.chunks + blockIdx.x] = sum;
+}
+
+// Inclusive sums over the workgroup's 256 threads; s: 4 of LDS.
+__device__ __forceinline__ double scan256(double v, double* s, int tid) {
   const int lane = tid & 63;
 #pragma unroll
   for (int off = 1; off < kWave; off <<= 1) {
@@ -112,88 +153,88 @@ __device__ __forceinline__ double scan1024(double v, double* s, int tid) {
   __syncthreads();
   if (lane == 63) s[tid >> 6] = v;
   __syncthreads();
-  for (int w = 0; w < (tid >> 6); w++) v += s[w];
+#pragma unroll
+  for (int w = 0; w < 3; w++)
+    if (w < (tid >> 6)) v += s[w];
   return v;
 }
 
-// Workgroup a sequence: finds the chunk, then the token in it, and writes the sequence's rows.
-__global__ void __launch_bounds__(1024) draft_pick_kernel(Drafts d) {
-  __shared__ int s_n, s_at, s_last;
-  __shared__ double s_scan[16], s_before, s_total;
+// Workgroup a sequence: finds the chunk, then the token in it.
+__global__ void __launch_bounds__(256) draft_pick_kernel(Drafts d) {
+  __shared__ int s_at, s_last;
+  __shared__ double s_scan[4], s_before, s_total;
   const int s = blockIdx.x, tid = threadIdx.x;
-  Verdict v = verdict_of(d, s, &s_n);
-  if (tid == 0) {
-    d.accepted[s] = v.accepted;
-    if (d.dropped) d.dropped[s] = max(v.rows - 1, 0) - v.accepted;
-  }
+  double* const sums = d.sums + int64_t(s) * d.chunks;
+  Verdict v = d.verdicts[s];
+  const float u = d.u_last[s];
+  const double first = tid < d.chunks ? sums[tid] : 0.0;  // (on its way with the verdict)
   if (v.row < 0) return;
-  const double2* sums = d.sums + int64_t(s) * d.chunks;
   const float* p = d.target + v.row * d.target_stride;
   const float* q = v.less >= 0 ? d.draft + v.less * d.draft_stride : nullptr;
-  bool alone = false;
-  double total = 0.0;
-  for (;;) {
-    double mine = 0.0;
-    for (int c = tid; c < d.chunks; c += 1024) mine += alone ? sums[c].y : sums[c].x;
-    mine = scan1024(mine, s_scan, tid);
-    if (tid == 1023) s_total = mine;
-    __syncthreads();
-    total = s_total;
-    if (total > 0.0 || alone) break;
-    alone = true, q = nullptr, v.without = -1;  // the draft takes off all there is
-  }
-  const double passes = double(d.u_last[s]) * total;
-  // the first chunk whose running sum passes, or the last of any weight
   if (tid == 0) s_at = INT32_MAX, s_last = -1;
-  __syncthreads();
+  bool again = false;
+  for (;;) {
+    double mine = again ? (tid < d.chunks ? sums[tid] : 0.0) : first;
+    for (int c = tid + 256; c < d.chunks; c += 256) mine += sums[c];
+    mine = scan256(mine, s_scan, tid);
+    if (tid == 255) s_total = mine;
+    __syncthreads();
+    if (s_total > 0.0 || again || (!q && v.without < 0)) break;
+    // the draft takes off all there is: the target's own sums
+    again = true, q = nullptr, v.without = -1;
+    for (int c = 0; c < d.chunks; c++) {
+      const double sum = chunk_sum(d, v, p, nullptr, c, s_scan, tid);
+      if (tid == 0) sums[c] = sum;
+    }
+    __syncthreads();
+  }
+  const double passes = double(u) * s_total;
+  // the first chunk whose running sum passes, or the last of any weight
   double carry = 0.0;
-  for (int c0 = 0; c0 < d.chunks; c0 += 1024) {
+  for (int c0 = 0; c0 < d.chunks; c0 += 256) {
     const int c = c0 + tid;
-    const double w = c < d.chunks ? (alone ? sums[c].y : sums[c].x) : 0.0;
-    const double run = carry + scan1024(w, s_scan, tid);
+    const double w = c0 == 0 && !again ? first : c < d.chunks ? sums[c] : 0.0;
+    const double run = carry + scan256(w, s_scan, tid);
     if (w > 0.0) {
       if (run > passes) atomicMin(&s_at, c);
       atomicMax(&s_last, c);
     }
-    if (tid == 1023) s_total = run;
     __syncthreads();
+    if (tid == 255) s_total = run;
     if (s_at == c || (s_at == INT32_MAX && s_last == c)) s_before = run - w;
+    __syncthreads();
     carry = s_total;
     if (s_at != INT32_MAX) break;
-    __syncthreads();
   }
-  __syncthreads();
   const int chunk = s_at != INT32_MAX ? s_at : s_last;
   const double before = s_before;
   __syncthreads();
   int drawn = -1;
   if (chunk >= 0) {
     if (tid == 0) s_at = INT32_MAX, s_last = -1;
-    const int lo = chunk * kDraftChunk + 4 * tid, hi = min(min(lo + 4, (chunk + 1) * kDraftChunk), d.vocab);
-    double w[4] = {};
+    constexpr int N = kDraftChunk / 256;
+    const int lo = chunk * kDraftChunk + N * tid;
+    double w[N], sum = 0.0;
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-      if (lo + e < hi) w[e] = weight_of(v, p, q, lo + e);
-    double run = scan1024(w[0] + w[1] + w[2] + w[3], s_scan, tid) - (w[0] + w[1] + w[2] + w[3]) + before;
+    for (int e = 0; e < N; e++) w[e] = lo + e < d.vocab ? weight_of(v, p, q, lo + e) : 0.0;
 #pragma unroll
-    for (int e = 3; e >= 0; e--)
-      if (w[e] > 0.0) {
-        atomicMax(&s_last, lo + e);
-        break;
-      }
+    for (int e = 0; e < N; e++) sum += w[e];
+    double run = scan256(sum, s_scan, tid) - sum + before;
+    int at = INT32_MAX, last = -1;
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
+    for (int e = 0; e < N; e++) {
       run += w[e];
-      if (w[e] > 0.0 && run > passes) {
-        atomicMin(&s_at, lo + e);
-        break;
+      if (w[e] > 0.0) {
+        if (run > passes) at = min(at, lo + e);
+        last = lo + e;
       }
     }
+    if (at != INT32_MAX) atomicMin(&s_at, at);
+    if (last >= 0) atomicMax(&s_last, last);
     __syncthreads();
     drawn = s_at != INT32_MAX ? s_at : s_last;
   }
-  for (int i = tid; i < v.rows; i += 1024)
-    d.out[v.first + i] = i < v.accepted ? d.tokens[v.first + i + 1] : i == v.accepted ? drawn : -1;
+  if (tid == 0) d.out[v.first + v.accepted] = drawn;
 }
 
 }  // namespace jero
@@ -202,7 +243,7 @@ using namespace jero;
 
 extern "C" size_t jero_hip_verify_drafts_workspace_bytes(int64_t n_seqs, int64_t vocab) {
   if (n_seqs < 1 || n_seqs > 65535 || vocab < 1 || vocab > (1 << 24)) return 0;
-  return size_t(n_seqs) * size_t((vocab + kDraftChunk - 1) / kDraftChunk) * sizeof(double2);
+  return size_t(n_seqs) * (size_t((vocab + kDraftChunk - 1) / kDraftChunk) * sizeof(double) + sizeof(Verdict));
 }
 
 extern "C" int jero_hip_verify_drafts(const float* target_dev, int64_t target_stride, const float* draft_dev,
@@ -240,11 +281,12 @@ extern "C" int jero_hip_verify_drafts(const float* target_dev, int64_t target_st
   d.n_seqs = int(n_seqs), d.n_tokens = int(n_tokens), d.n_drafts = int(n_drafts), d.vocab = int(vocab);
   d.chunks = (d.vocab + kDraftChunk - 1) / kDraftChunk;
   d.out = out_dev, d.accepted = accepted_dev, d.dropped = dropped_dev;
-  d.sums = static_cast<double2*>(workspace_dev);
+  d.sums = static_cast<double*>(workspace_dev);
+  d.verdicts = reinterpret_cast<Verdict*>(d.sums + n_seqs * d.chunks);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid = {unsigned(d.chunks), unsigned(n_seqs), 1};
   hipLaunchKernelGGL(draft_sums_kernel, grid, dim3(256), 0, s, d);
   if (int rc = check_launch("verify_drafts sums")) return rc;
-  hipLaunchKernelGGL(draft_pick_kernel, dim3(unsigned(n_seqs)), dim3(1024), 0, s, d);
+  hipLaunchKernelGGL(draft_pick_kernel, dim3(unsigned(n_seqs)), dim3(256), 0, s, d);
   return check_launch("verify_drafts");
 }

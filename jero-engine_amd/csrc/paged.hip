@@ -18,46 +18,31 @@ struct BlockPool {
   int n_seqs, capacity, shared, shift, n_tokens;
 };
 
-// What the second part wants of a request: its positions and blocks before, and the sums before it.
+// What the second part wants of a request: its positions and blocks before the call, and the blocks taken before it.
 struct Request {
-  int len, owned, taken, back;  // len -1: not granted; taken, back: blocks taken and given back before it
+  int len, owned, taken;  // len -1: not granted
 };
 // The stack: ids before, and with those given back; then how many are taken and given back in all.
 struct Stack {
   int before, top, taken, back;
 };
+// The workspace's arrays: a request's, and the sums of blocks given back before each.
+struct ExtendSpace {
+  Request* r;
+  int32_t* back;
+  Stack* st;
+};
 
-constexpr int kExtendThreads = 1024;
+constexpr int kExtendThreads = 1024, kExtendWaves = kExtendThreads / kWave;
+constexpr int kExtendMost = 1 << 24;  // tokens of a request that are counted: a call has no more
 
-__device__ __forceinline__ int64_t scan_add(int64_t v, int lane) {
+__device__ __forceinline__ int wave_scan(int v, int lane) {
 #pragma unroll
   for (int off = 1; off < kWave; off <<= 1) {
-    const int64_t o = __shfl_up(v, off, kWave);
+    const int o = __shfl_up(v, off, kWave);
     if (lane >= off) v += o;
   }
   return v;
-}
-
-// Inclusive sums over the workgroup of three values at once; total: of all.  s: 16 of each.
-__device__ __forceinline__ void scan3(int64_t (&v)[3], int64_t (&total)[3], int64_t (*s)[kExtendThreads / kWave], int tid) {
-  const int lane = tid & 63, wv = tid >> 6;
-#pragma unroll
-  for (int i = 0; i < 3; i++) v[i] = scan_add(v[i], lane);
-  __syncthreads();
-  if (lane == 63)
-#pragma unroll
-    for (int i = 0; i < 3; i++) s[i][wv] = v[i];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 3; i++) {
-    total[i] = 0;
-    int64_t before = 0;
-    for (int w = 0; w < kExtendThreads / kWave; w++) {
-      if (w < wv) before += s[i][w];
-      total[i] += s[i][w];
-    }
-    v[i] += before;
-  }
 }
 
 struct Held {
@@ -91,99 +76,143 @@ __device__ __forceinline__ int last_not_above(const int32_t* v, int n, int strid
   return lo;
 }
 
+// Id e of those given back, in order.
+__device__ __forceinline__ int returned_id(const BlockPool& p, const int32_t* back, int e) {
+  const int s = last_not_above(back, p.n_seqs, 1, e);
+  return p.table[int64_t(s) * p.table_stride + p.shared + (e - back[s])];
+}
 // Block i (of all that the call takes, in order): the ids given back stand above those that were there.
-__device__ __forceinline__ int taken_id(const BlockPool& p, const Request* r, const Stack& st, int i) {
+__device__ __forceinline__ int taken_id(const BlockPool& p, const int32_t* back, const Stack& st, int i) {
   const int j = st.top - 1 - i;
-  if (j < st.before) return p.free_ids[j];
-  const int e = j - st.before, s = last_not_above(&r[0].back, p.n_seqs, sizeof(Request) / 4, e);
-  return p.table[int64_t(s) * p.table_stride + p.shared + (e - r[s].back)];
+  return j < st.before ? p.free_ids[j] : returned_id(p, back, j - st.before);
 }
 
-// First part: the sums over the requests, by one workgroup, and what follows from them for each.
-__device__ void extend_sums(const BlockPool& p, Request* r, Stack* st, int tid) {
-  __shared__ int64_t s_sum[3][kExtendThreads / kWave];
-  // all that is given back is there before the first block is taken
-  int64_t back = 0;
-  for (int s = tid; s < p.n_seqs; s += kExtendThreads) back += held_by(p, s).back;
-  int64_t v[3] = {back, 0, 0}, total[3];
-  scan3(v, total, s_sum, tid);
+// First part: the sums over the requests, by one workgroup, a request a thread and round.  All that is given back is
+// there before the first block is taken, so its sum comes first, from the requests of the first round as they are kept.
+__device__ void extend_sums(const BlockPool& p, const ExtendSpace& to, int tid) {
+  __shared__ int s_sum[2][3][kExtendWaves], s_got;
+  __shared__ int64_t s_back[kExtendWaves];
+  const int lane = tid & 63, wv = tid >> 6;
+  Held h = {};
+  if (tid < p.n_seqs) h = held_by(p, tid);
+  int64_t back = h.back;
+  for (int s = tid + kExtendThreads; s < p.n_seqs; s += kExtendThreads) back += held_by(p, s).back;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) back += __shfl_xor(back, off, kWave);
+  if (lane == 0) s_back[wv] = back;
+  if (tid == 0) s_got = 0;
   const int before = min(max(p.n_free[0], 0), p.capacity);
-  const int top = int(min(int64_t(before) + total[0], int64_t(p.capacity)));
-  int64_t carry[3] = {0, 0, 0}, got = 0;
-  for (int s0 = 0; s0 < p.n_seqs; s0 += kExtendThreads) {
+  int top = 0;
+  int64_t carry[3] = {0, 0, 0};
+  for (int s0 = 0, round = 0; s0 < p.n_seqs; s0 += kExtendThreads, round ^= 1) {
     const int s = s0 + tid;
     const bool on = s < p.n_seqs;
-    Held h = {};
-    if (on) h = held_by(p, s);
-    int64_t w[3] = {h.tokens, h.need, h.back};
-    scan3(w, total, s_sum, tid);
+    if (s0) {
+      h = Held{};
+      if (on) h = held_by(p, s);
+    }
+    const int mine[3] = {min(h.tokens, kExtendMost), h.need, h.back};
+    int w[3];
 #pragma unroll
-    for (int i = 0; i < 3; i++) w[i] += carry[i], carry[i] += total[i];
-    const bool granted = h.fits && (h.need == 0 || w[1] <= top);
+    for (int i = 0; i < 3; i++) {
+      w[i] = wave_scan(mine[i], lane);
+      if (lane == 63) s_sum[round][i][wv] = w[i];
+    }
+    __syncthreads();
+    if (s0 == 0) {
+      int64_t all = before;
+#pragma unroll
+      for (int i = 0; i < kExtendWaves; i++) all += s_back[i];
+      top = int(min(all, int64_t(p.capacity)));
+    }
+    int64_t sum[3];
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+      // (16 waves' sums, a lane each)
+      const int64_t v = s_sum[round][i][lane & (kExtendWaves - 1)];
+      int64_t below = (lane & (kExtendWaves - 1)) < wv ? v : 0, all = v;
+#pragma unroll
+      for (int off = 1; off < kExtendWaves; off <<= 1) below += __shfl_xor(below, off, kWave), all += __shfl_xor(all, off, kWave);
+      sum[i] = carry[i] + below + w[i];
+      carry[i] += all;
+    }
+    const bool granted = h.fits && (h.need == 0 || sum[1] <= top);
     if (on) {
-      p.starts[s] = int(min(w[0] - h.tokens, int64_t(INT32_MAX)));
-      r[s] = Request{granted ? h.len : -1, h.owned, int(w[1] - h.need), int(w[2] - h.back)};
+      p.starts[s] = int(min(sum[0] - mine[0], int64_t(INT32_MAX)));
+      to.r[s] = Request{granted ? h.len : -1, h.owned, int(sum[1] - h.need)};
+      to.back[s] = int(sum[2] - h.back);
       p.lens_out[s] = h.ends ? 0 : granted ? h.len + h.tokens : h.len;
       p.owned_out[s] = h.ends ? 0 : granted ? h.owned + h.need : h.owned;
       if (p.granted) p.granted[s] = granted;
     }
-    // (the needs' sums do not fall: those granted any are the first)
-    v[0] = granted && on ? h.need : 0, v[1] = v[2] = 0;
-    scan3(v, total, s_sum, tid);
-    got += total[0];
+    // the needs' sums do not fall, so what is taken is the last granted one's
+    const uint64_t some = __ballot(on && granted && h.need > 0);
+    if (some && lane == 63 - __builtin_clzll(some)) atomicMax(&s_got, int(sum[1]));
   }
+  __syncthreads();
   if (tid == 0) {
     p.starts[p.n_seqs] = int(min(carry[0], int64_t(INT32_MAX)));
-    *st = Stack{before, top, int(got), int(carry[2])};
-    p.n_free_out[0] = top - int(got);
+    *to.st = Stack{before, top, s_got, int(carry[2])};
+    p.n_free_out[0] = top - s_got;
   }
 }
 
-// Second part: each token's position and slot, the blocks given back, and those taken.
-__device__ void extend_rows(const BlockPool& p, const Request* r, const Stack& st, int at, int step) {
-  const int total = p.starts[p.n_seqs], mask = (1 << p.shift) - 1;
+// Second part: each token's position and slot, the blocks given back, and those taken.  starts and back may be copies.
+__device__ void extend_rows(const BlockPool& p, const Request* r, const int32_t* starts, const int32_t* back, const Stack& st,
+                            int at, int step) {
+  const int total = starts[p.n_seqs], mask = (1 << p.shift) - 1;
   for (int t = at; t < p.n_tokens; t += step) {
     int pos = -1;
     int64_t slot = -1;
     if (t < total) {
-      const int s = last_not_above(p.starts, p.n_seqs, 1, t);
+      const int s = last_not_above(starts, p.n_seqs, 1, t);
       const Request q = r[s];
       if (q.len >= 0) {
-        pos = q.len + (t - p.starts[s]);
+        pos = q.len + (t - starts[s]);
         const int c = pos >> p.shift;
-        const int id = c < q.owned ? p.table[int64_t(s) * p.table_stride + c] : taken_id(p, r, st, q.taken + c - q.owned);
+        const int id = c < q.owned ? p.table[int64_t(s) * p.table_stride + c] : taken_id(p, back, st, q.taken + c - q.owned);
         if (uint32_t(id) < uint64_t(p.n_blocks)) slot = (int64_t(id) << p.shift) + (pos & mask);
       }
     }
     p.positions[t] = pos;
     p.slots[t] = slot;
   }
-  for (int e = at; e < st.back; e += step) {
-    const int s = last_not_above(&r[0].back, p.n_seqs, sizeof(Request) / 4, e);
-    if (st.before + e < p.capacity)
-      p.free_ids[st.before + e] = p.table[int64_t(s) * p.table_stride + p.shared + (e - r[s].back)];
-  }
+  for (int e = at; e < st.back; e += step)
+    if (st.before + e < p.capacity) p.free_ids[st.before + e] = returned_id(p, back, e);
   for (int i = at; i < st.taken; i += step) {
     const int s = last_not_above(&r[0].taken, p.n_seqs, sizeof(Request) / 4, i);
-    p.table[int64_t(s) * p.table_stride + r[s].owned + (i - r[s].taken)] = taken_id(p, r, st, i);
+    p.table[int64_t(s) * p.table_stride + r[s].owned + (i - r[s].taken)] = taken_id(p, back, st, i);
   }
 }
 
-// The requests of the second part are kept in LDS up to this many.
+// One launch, its arrays in LDS, up to this many requests and tokens (64 requests of one token: 10 us in two launches).
 constexpr int kExtendSeqs = 1024, kExtendTokens = 4096;
+// Requests whose starts and sums of blocks given back the second launch's workgroups copy to LDS: 11 steps of a search
+// there for 1500 requests, 11 times the memory's latency otherwise.
+constexpr int kExtendCopied = 4096;
 
 __global__ void __launch_bounds__(kExtendThreads) extend_small_kernel(BlockPool p) {
   __shared__ Request s_r[kExtendSeqs];
+  __shared__ int32_t s_back[kExtendSeqs];
   __shared__ Stack s_st;
-  extend_sums(p, s_r, &s_st, threadIdx.x);
+  extend_sums(p, ExtendSpace{s_r, s_back, &s_st}, threadIdx.x);
   __syncthreads();
-  extend_rows(p, s_r, s_st, threadIdx.x, kExtendThreads);
+  extend_rows(p, s_r, p.starts, s_back, s_st, threadIdx.x, kExtendThreads);
 }
-__global__ void __launch_bounds__(kExtendThreads) extend_sums_kernel(BlockPool p, Request* r, Stack* st) {
-  extend_sums(p, r, st, threadIdx.x);
+__global__ void __launch_bounds__(kExtendThreads) extend_sums_kernel(BlockPool p, ExtendSpace to) {
+  extend_sums(p, to, threadIdx.x);
 }
-__global__ void __launch_bounds__(256) extend_rows_kernel(BlockPool p, const Request* r, const Stack* st) {
-  extend_rows(p, r, *st, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+template <bool COPIED>
+__global__ void __launch_bounds__(256) extend_rows_kernel(BlockPool p, ExtendSpace from) {
+  if constexpr (COPIED) {
+    __shared__ int32_t s_starts[kExtendCopied + 1], s_back[kExtendCopied];
+    for (int i = threadIdx.x; i <= p.n_seqs; i += 256) s_starts[i] = p.starts[i];
+    for (int i = threadIdx.x; i < p.n_seqs; i += 256) s_back[i] = from.back[i];
+    __syncthreads();
+    extend_rows(p, from.r, s_starts, s_back, *from.st, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+  } else {
+    extend_rows(p, from.r, p.starts, from.back, *from.st, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+  }
 }
 
 // ---------------------------------------------------------------- rotation and storing
@@ -330,7 +359,7 @@ static void launch_append(const void* q, const void* k, const void* v, const App
 using namespace jero;
 
 extern "C" size_t jero_hip_paged_extend_workspace_bytes(int64_t n_seqs) {
-  return n_seqs < 1 || n_seqs > (1 << 19) ? 0 : size_t(n_seqs + 1) * sizeof(Request);
+  return n_seqs < 1 || n_seqs > (1 << 19) ? 0 : sizeof(Stack) + size_t(n_seqs) * (sizeof(Request) + 4);
 }
 
 extern "C" int jero_hip_paged_extend(const jero_block_pool* pool, const int32_t* new_dev, const int32_t* drop_dev,
@@ -396,12 +425,16 @@ extern "C" int jero_hip_paged_extend(const jero_block_pool* pool, const int32_t*
   } else if (!aligned(workspace_dev, 16)) {
     return bad(JERO_ERR_INVALID_ARGUMENT, "the workspace must be 16-byte aligned");
   }
-  Request* r = static_cast<Request*>(workspace_dev);
-  Stack* st = reinterpret_cast<Stack*>(r + p.n_seqs);
-  hipLaunchKernelGGL(extend_sums_kernel, dim3(1), dim3(kExtendThreads), 0, s, p, r, st);
+  uint8_t* const at = static_cast<uint8_t*>(workspace_dev);
+  const ExtendSpace space{reinterpret_cast<Request*>(at + sizeof(Stack)),
+                          reinterpret_cast<int32_t*>(at + sizeof(Stack) + size_t(p.n_seqs) * sizeof(Request)),
+                          reinterpret_cast<Stack*>(at)};
+  hipLaunchKernelGGL(extend_sums_kernel, dim3(1), dim3(kExtendThreads), 0, s, p, space);
   if ((rc = check_launch("paged_extend"))) return rc;
   const int64_t items = n_tokens > p.n_seqs ? n_tokens : p.n_seqs, blocks = (items + 255) / 256;
-  hipLaunchKernelGGL(extend_rows_kernel, dim3(unsigned(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, p, r, st);
+  const dim3 grid = {unsigned(blocks < 1024 ? blocks : 1024), 1, 1};
+  if (p.n_seqs <= kExtendCopied) hipLaunchKernelGGL((extend_rows_kernel<true>), grid, dim3(256), 0, s, p, space);
+  else hipLaunchKernelGGL((extend_rows_kernel<false>), grid, dim3(256), 0, s, p, space);
   return check_launch("paged_extend rows");
 }
 
