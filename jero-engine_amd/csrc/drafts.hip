@@ -142,8 +142,8 @@ __global__ void __launch_bounds__(256) draft_sums_kernel(Drafts d) {
   if (tid == 0) d.sums[int64_t(s) * d.chunks + blockIdx.x] = sum;
 }
 
-// Inclusive sums over the workgroup's 256 threads; s: 4 of LDS.
-__device__ __forceinline__ double scan256(double v, double* s, int tid) {
+// Inclusive sums over the workgroup's 1024 threads; s: 16 of LDS.
+__device__ __forceinline__ double scan1024(double v, double* s, int tid) {
   const int lane = tid & 63;
 #pragma unroll
   for (int off = 1; off < kWave; off <<= 1) {
@@ -154,83 +154,103 @@ __device__ __forceinline__ double scan256(double v, double* s, int tid) {
   if (lane == 63) s[tid >> 6] = v;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 3; w++)
-    if (w < (tid >> 6)) v += s[w];
+  for (int w = 0; w < 15; w++) {
+    const double o = s[w];
+    if (w < (tid >> 6)) v += o;
+  }
   return v;
 }
 
+// The lowest of the workgroup's `at` and the highest of its `last` (both rise with the thread): one lane a wave asks, as
+// 64 lanes' operations on one word go one after another.
+__device__ __forceinline__ void lowest_and_highest(int at, int last, int* s_at, int* s_last, int lane) {
+  const uint64_t found = __ballot(at != INT32_MAX), any = __ballot(last >= 0);
+  if (found && lane == __builtin_ctzll(found)) atomicMin(s_at, at);
+  if (any && lane == 63 - __builtin_clzll(any)) atomicMax(s_last, last);
+}
+
 // Workgroup a sequence: finds the chunk, then the token in it.
-__global__ void __launch_bounds__(256) draft_pick_kernel(Drafts d) {
+constexpr int kPickThreads = 1024, kPickChunks = (1 << 24) / kDraftChunk / kPickThreads;  // a thread, at most
+__global__ void __launch_bounds__(kPickThreads) draft_pick_kernel(Drafts d) {
   __shared__ int s_at, s_last;
-  __shared__ double s_scan[4], s_before, s_total;
+  __shared__ double s_scan[16], s_before, s_total;
   const int s = blockIdx.x, tid = threadIdx.x;
   double* const sums = d.sums + int64_t(s) * d.chunks;
   Verdict v = d.verdicts[s];
   const float u = d.u_last[s];
-  const double first = tid < d.chunks ? sums[tid] : 0.0;  // (on its way with the verdict)
+  const int each = (d.chunks + kPickThreads - 1) / kPickThreads, c0 = tid * each;  // chunks of a thread
+  double w[kPickChunks];
+  auto read = [&]() {
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPickChunks; i++) sum += w[i] = i < each && c0 + i < d.chunks ? sums[c0 + i] : 0.0;
+    return sum;
+  };
+  double mine = read();  // (on their way with the verdict)
   if (v.row < 0) return;
   const float* p = d.target + v.row * d.target_stride;
   const float* q = v.less >= 0 ? d.draft + v.less * d.draft_stride : nullptr;
   if (tid == 0) s_at = INT32_MAX, s_last = -1;
-  bool again = false;
-  for (;;) {
-    double mine = again ? (tid < d.chunks ? sums[tid] : 0.0) : first;
-    for (int c = tid + 256; c < d.chunks; c += 256) mine += sums[c];
-    mine = scan256(mine, s_scan, tid);
-    if (tid == 255) s_total = mine;
-    __syncthreads();
-    if (s_total > 0.0 || again || (!q && v.without < 0)) break;
+  double run = scan1024(mine, s_scan, tid);
+  if (tid == kPickThreads - 1) s_total = run;
+  __syncthreads();
+  if (!(s_total > 0.0) && (q || v.without >= 0)) {
     // the draft takes off all there is: the target's own sums
-    again = true, q = nullptr, v.without = -1;
-    for (int c = 0; c < d.chunks; c++) {
-      const double sum = chunk_sum(d, v, p, nullptr, c, s_scan, tid);
-      if (tid == 0) sums[c] = sum;
+    q = nullptr, v.without = -1;
+    for (int c = tid >> 6; c < d.chunks; c += kPickThreads / kWave) {
+      double sum = 0.0;
+      for (int i = c * kDraftChunk + (tid & 63); i < min((c + 1) * kDraftChunk, d.vocab); i += kWave)
+        sum += weight_of(v, p, nullptr, i);
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
+      if ((tid & 63) == 0) sums[c] = sum;
     }
+    __syncthreads();
+    mine = read();
+    run = scan1024(mine, s_scan, tid);
+    if (tid == kPickThreads - 1) s_total = run;
     __syncthreads();
   }
   const double passes = double(u) * s_total;
   // the first chunk whose running sum passes, or the last of any weight
-  double carry = 0.0;
-  for (int c0 = 0; c0 < d.chunks; c0 += 256) {
-    const int c = c0 + tid;
-    const double w = c0 == 0 && !again ? first : c < d.chunks ? sums[c] : 0.0;
-    const double run = carry + scan256(w, s_scan, tid);
-    if (w > 0.0) {
-      if (run > passes) atomicMin(&s_at, c);
-      atomicMax(&s_last, c);
+  run -= mine;
+  double before[kPickChunks];
+  int at = INT32_MAX, last = -1;
+#pragma unroll
+  for (int i = 0; i < kPickChunks; i++) {
+    before[i] = run;
+    run += w[i];
+    if (w[i] > 0.0) {
+      if (run > passes) at = min(at, c0 + i);
+      last = c0 + i;
     }
-    __syncthreads();
-    if (tid == 255) s_total = run;
-    if (s_at == c || (s_at == INT32_MAX && s_last == c)) s_before = run - w;
-    __syncthreads();
-    carry = s_total;
-    if (s_at != INT32_MAX) break;
   }
+  lowest_and_highest(at, last, &s_at, &s_last, tid & 63);
+  __syncthreads();
   const int chunk = s_at != INT32_MAX ? s_at : s_last;
-  const double before = s_before;
+#pragma unroll
+  for (int i = 0; i < kPickChunks; i++)
+    if (i < each && c0 + i == chunk) s_before = before[i];
   __syncthreads();
   int drawn = -1;
   if (chunk >= 0) {
     if (tid == 0) s_at = INT32_MAX, s_last = -1;
-    constexpr int N = kDraftChunk / 256;
+    constexpr int N = kDraftChunk / kPickThreads;
     const int lo = chunk * kDraftChunk + N * tid;
-    double w[N], sum = 0.0;
+    double x[N], sum = 0.0;
 #pragma unroll
-    for (int e = 0; e < N; e++) w[e] = lo + e < d.vocab ? weight_of(v, p, q, lo + e) : 0.0;
-#pragma unroll
-    for (int e = 0; e < N; e++) sum += w[e];
-    double run = scan256(sum, s_scan, tid) - sum + before;
-    int at = INT32_MAX, last = -1;
+    for (int e = 0; e < N; e++) sum += x[e] = lo + e < d.vocab ? weight_of(v, p, q, lo + e) : 0.0;
+    run = scan1024(sum, s_scan, tid) - sum + s_before;
+    at = INT32_MAX, last = -1;
 #pragma unroll
     for (int e = 0; e < N; e++) {
-      run += w[e];
-      if (w[e] > 0.0) {
+      run += x[e];
+      if (x[e] > 0.0) {
         if (run > passes) at = min(at, lo + e);
         last = lo + e;
       }
     }
-    if (at != INT32_MAX) atomicMin(&s_at, at);
-    if (last >= 0) atomicMax(&s_last, last);
+    lowest_and_highest(at, last, &s_at, &s_last, tid & 63);
     __syncthreads();
     drawn = s_at != INT32_MAX ? s_at : s_last;
   }
@@ -287,6 +307,6 @@ extern "C" int jero_hip_verify_drafts(const float* target_dev, int64_t target_st
   const dim3 grid = {unsigned(d.chunks), unsigned(n_seqs), 1};
   hipLaunchKernelGGL(draft_sums_kernel, grid, dim3(256), 0, s, d);
   if (int rc = check_launch("verify_drafts sums")) return rc;
-  hipLaunchKernelGGL(draft_pick_kernel, dim3(unsigned(n_seqs)), dim3(256), 0, s, d);
+  hipLaunchKernelGGL(draft_pick_kernel, dim3(unsigned(n_seqs)), dim3(kPickThreads), 0, s, d);
   return check_launch("verify_drafts");
 }

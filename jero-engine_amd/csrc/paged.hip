@@ -161,27 +161,29 @@ __device__ void extend_sums(const BlockPool& p, const ExtendSpace& to, int tid) 
 __device__ void extend_rows(const BlockPool& p, const Request* r, const int32_t* starts, const int32_t* back, const Stack& st,
                             int at, int step) {
   const int total = starts[p.n_seqs], mask = (1 << p.shift) - 1;
-  for (int t = at; t < p.n_tokens; t += step) {
-    int pos = -1;
-    int64_t slot = -1;
-    if (t < total) {
-      const int s = last_not_above(starts, p.n_seqs, 1, t);
-      const Request q = r[s];
-      if (q.len >= 0) {
-        pos = q.len + (t - starts[s]);
-        const int c = pos >> p.shift;
-        const int id = c < q.owned ? p.table[int64_t(s) * p.table_stride + c] : taken_id(p, back, st, q.taken + c - q.owned);
-        if (uint32_t(id) < uint64_t(p.n_blocks)) slot = (int64_t(id) << p.shift) + (pos & mask);
+  for (int i = at; i < p.n_tokens + st.back + st.taken; i += step) {
+    if (i < p.n_tokens) {
+      int pos = -1;
+      int64_t slot = -1;
+      if (i < total) {
+        const int s = last_not_above(starts, p.n_seqs, 1, i);
+        const Request q = r[s];
+        if (q.len >= 0) {
+          pos = q.len + (i - starts[s]);
+          const int c = pos >> p.shift;
+          const int id = c < q.owned ? p.table[int64_t(s) * p.table_stride + c] : taken_id(p, back, st, q.taken + c - q.owned);
+          if (uint32_t(id) < uint64_t(p.n_blocks)) slot = (int64_t(id) << p.shift) + (pos & mask);
+        }
       }
+      p.positions[i] = pos;
+      p.slots[i] = slot;
+    } else if (i < p.n_tokens + st.back) {
+      const int e = i - p.n_tokens;
+      if (st.before + e < p.capacity) p.free_ids[st.before + e] = returned_id(p, back, e);
+    } else {
+      const int k = i - p.n_tokens - st.back, s = last_not_above(&r[0].taken, p.n_seqs, sizeof(Request) / 4, k);
+      p.table[int64_t(s) * p.table_stride + r[s].owned + (k - r[s].taken)] = taken_id(p, back, st, k);
     }
-    p.positions[t] = pos;
-    p.slots[t] = slot;
-  }
-  for (int e = at; e < st.back; e += step)
-    if (st.before + e < p.capacity) p.free_ids[st.before + e] = returned_id(p, back, e);
-  for (int i = at; i < st.taken; i += step) {
-    const int s = last_not_above(&r[0].taken, p.n_seqs, sizeof(Request) / 4, i);
-    p.table[int64_t(s) * p.table_stride + r[s].owned + (i - r[s].taken)] = taken_id(p, back, st, i);
   }
 }
 
@@ -432,7 +434,7 @@ extern "C" int jero_hip_paged_extend(const jero_block_pool* pool, const int32_t*
   hipLaunchKernelGGL(extend_sums_kernel, dim3(1), dim3(kExtendThreads), 0, s, p, space);
   if ((rc = check_launch("paged_extend"))) return rc;
   const int64_t items = n_tokens > p.n_seqs ? n_tokens : p.n_seqs, blocks = (items + 255) / 256;
-  const dim3 grid = {unsigned(blocks < 1024 ? blocks : 1024), 1, 1};
+  const dim3 grid = {unsigned(blocks < 2048 ? blocks : 2048), 1, 1};
   if (p.n_seqs <= kExtendCopied) hipLaunchKernelGGL((extend_rows_kernel<true>), grid, dim3(256), 0, s, p, space);
   else hipLaunchKernelGGL((extend_rows_kernel<false>), grid, dim3(256), 0, s, p, space);
   return check_launch("paged_extend rows");
