@@ -4,7 +4,7 @@
 
 namespace jero {
 
-constexpr int kDraftChunk = 4096;  // of the vocabulary, a workgroup
+constexpr int kDraftChunk = 2048;  // of the vocabulary, a workgroup
 
 // Where a sequence's next token is drawn from.
 struct Verdict {
