@@ -34,6 +34,7 @@ __device__ __forceinline__ int paged_visible(const PagedCall& c, int t) {
 // and the sequence whose table holds those that are not shared.
 struct PagedItem {
   int first, count, lo, hi, seq, head, part;
+  int end;  // own positions: the token row behind the sequence's last, by which hi is still to be bounded; or -1
 };
 
 __device__ __forceinline__ bool paged_item(const PagedCall& c, const PagedPlan& p, int lane, PagedItem& it, bool& wide) {
@@ -53,7 +54,7 @@ __device__ __forceinline__ bool paged_item(const PagedCall& c, const PagedPlan& 
     it.count = min(rows, c.n_tokens * c.group - it.first);
     it.lo = chunk * p.pre_len;
     it.hi = min(it.lo + p.pre_len, c.shared_len);
-    it.seq = 0, it.part = chunk;
+    it.seq = 0, it.part = chunk, it.end = -1;
     return true;
   }
   wide = p.own_wide;
@@ -88,11 +89,18 @@ __device__ __forceinline__ bool paged_item(const PagedCall& c, const PagedPlan& 
   it.first = from * c.group + skip;
   it.count = min(rows, mine - skip);
   it.lo = p.own_lo + chunk * p.own_len;
-  // the last row sees the most
-  const int last = (it.first + it.count - 1) / c.group;
-  const int64_t top = min(int64_t(c.lens[it.seq]) - end + last + 1, int64_t(c.max_len));
-  it.hi = int(max(min(top, int64_t(it.lo) + p.own_len), int64_t(it.lo)));
+  it.hi = it.lo + p.own_len;
+  it.end = end;
   it.part = p.pre_chunks + chunk;
+  return true;
+}
+
+// Bounds hi by what the last row sees; false: no position is left, and no one else waits for the rows.
+__device__ __forceinline__ bool paged_bound(const PagedCall& c, const PagedPlan& p, PagedItem& it) {
+  if (it.end < 0) return true;
+  const int last = (it.first + it.count - 1) / c.group;
+  const int64_t top = min(int64_t(c.lens[it.seq]) - it.end + last + 1, int64_t(c.max_len));
+  it.hi = int(max(min(top, int64_t(it.hi)), int64_t(it.lo)));
   return p.parts == 1 || it.hi > it.lo;  // (the only part of a row writes it whatever it sees)
 }
 
@@ -117,36 +125,54 @@ __device__ __forceinline__ void attend_step(AttendState<HD, NJ, TWOQ>& st, KRead
                                             const int (&vat)[4], int p0, bool masked, uint64_t ok, uint64_t bad, int g) {
   constexpr int RT = KR / 16, KT = HD / 32, DT = HD / 16, KP = TWOK ? 2 : 1;
   f4_t s[NJ][RT];
-  h8_t ka[2][RT][KP];
+  constexpr int KD = RT == 2 ? 3 : 2;  // (registers)
+  h8_t ka[KD][RT][KP];
   auto read_k = [&](int k) {
 #pragma unroll
     for (int r = 0; r < RT; r++)
 #pragma unroll
-      for (int e = 0; e < KP; e++) ka[k & 1][r][e] = kread(k, r, e);
+      for (int e = 0; e < KP; e++) ka[k % KD][r][e] = kread(k, r, e);
   };
-  read_k(0);
+#pragma unroll
+  for (int k = 0; k < KD - 1; k++) read_k(k);
 #pragma unroll
   for (int k = 0; k < KT; k++) {
-    if (k + 1 < KT) read_k(k + 1);
+    if (k + KD - 1 < KT) read_k(k + KD - 1);
 #pragma unroll
     for (int r = 0; r < RT; r++)
 #pragma unroll
       for (int j = 0; j < NJ; j++)
-        s[j][r] = mfma(ka[k & 1][r][0], st.qh[j][k], k ? s[j][r] : f4_t{0.f, 0.f, 0.f, 0.f});
+        s[j][r] = mfma(ka[k % KD][r][0], st.qh[j][k], k ? s[j][r] : f4_t{0.f, 0.f, 0.f, 0.f});
     if constexpr (TWOQ) {
 #pragma unroll
       for (int r = 0; r < RT; r++)
 #pragma unroll
-        for (int j = 0; j < NJ; j++) s[j][r] = mfma(ka[k & 1][r][0], st.ql[j][k], s[j][r]);
+        for (int j = 0; j < NJ; j++) s[j][r] = mfma(ka[k % KD][r][0], st.ql[j][k], s[j][r]);
     }
     if constexpr (TWOK) {
 #pragma unroll
       for (int r = 0; r < RT; r++)
 #pragma unroll
-        for (int j = 0; j < NJ; j++) s[j][r] = mfma(ka[k & 1][r][KP - 1], st.qh[j][k], s[j][r]);
+        for (int j = 0; j < NJ; j++) s[j][r] = mfma(ka[k % KD][r][KP - 1], st.qh[j][k], s[j][r]);
     }
     __builtin_amdgcn_sched_barrier(0);
   }
+  // the values' first operands are on their way during the softmax
+  constexpr int VD = 3;
+  h8_t va[VD][RT / 2][KP];
+  auto tr = [&](int d, int r, int plane) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(vp + plane * vplane + vat[d & 3] + 128 * (d >> 2) + 16 * r * HD * 2));
+  };
+  auto read_v = [&](int d) {
+#pragma unroll
+    for (int r = 0; r < RT / 2; r++)
+#pragma unroll
+      for (int e = 0; e < KP; e++)
+        va[d % VD][r][e] = __builtin_bit_cast(
+            h8_t, __builtin_shufflevector(tr(d, 2 * r, e), tr(d, 2 * r + 1, e), 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+#pragma unroll
+  for (int d = 0; d < VD - 1; d++) read_v(d);
   h8_t bh[NJ][RT / 2], bl[NJ][RT / 2];
   bool grew[NJ];
   float alpha[NJ], times[NJ];
@@ -211,33 +237,20 @@ __device__ __forceinline__ void attend_step(AttendState<HD, NJ, TWOQ>& st, KRead
         if constexpr (TWOQ) st.l[j] = mfma(one, bl[j][r], st.l[j]);
       }
   }
-  auto tr = [&](int d, int r, int plane) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(vp + plane * vplane + vat[d & 3] + 128 * (d >> 2) + 16 * r * HD * 2));
-  };
-  h8_t va[2][RT / 2][KP];
-  auto read_v = [&](int d) {
-#pragma unroll
-    for (int r = 0; r < RT / 2; r++)
-#pragma unroll
-      for (int e = 0; e < KP; e++)
-        va[d & 1][r][e] = __builtin_bit_cast(
-            h8_t, __builtin_shufflevector(tr(d, 2 * r, e), tr(d, 2 * r + 1, e), 0, 1, 2, 3, 4, 5, 6, 7));
-  };
-  read_v(0);
 #pragma unroll
   for (int d = 0; d < DT; d++) {
-    if (d + 1 < DT) read_v(d + 1);
+    if (d + VD - 1 < DT) read_v(d + VD - 1);
 #pragma unroll
     for (int r = 0; r < RT / 2; r++) {
 #pragma unroll
-      for (int j = 0; j < NJ; j++) st.o[j][d] = mfma(va[d & 1][r][0], bh[j][r], st.o[j][d]);
+      for (int j = 0; j < NJ; j++) st.o[j][d] = mfma(va[d % VD][r][0], bh[j][r], st.o[j][d]);
       if constexpr (TWOQ) {
 #pragma unroll
-        for (int j = 0; j < NJ; j++) st.o[j][d] = mfma(va[d & 1][r][0], bl[j][r], st.o[j][d]);
+        for (int j = 0; j < NJ; j++) st.o[j][d] = mfma(va[d % VD][r][0], bl[j][r], st.o[j][d]);
       }
       if constexpr (TWOK) {
 #pragma unroll
-        for (int j = 0; j < NJ; j++) st.o[j][d] = mfma(va[d & 1][r][KP - 1], bh[j][r], st.o[j][d]);
+        for (int j = 0; j < NJ; j++) st.o[j][d] = mfma(va[d % VD][r][KP - 1], bh[j][r], st.o[j][d]);
       }
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -311,13 +324,16 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
   // each, and the load that renews them is waited for where it is made: a wait further on would be for all loads in flight.
   uint32_t window = ~0u;
   int window0 = INT32_MIN / 2;
+  auto open_window = [&](int b0) {
+    window0 = b0;
+    const int b = b0 + lane;
+    window = ~0u;
+    if (b < c.table_stride) window = uint32_t(b < c.shared_blocks ? c.shared[b] : table[b]);
+  };
   auto blocks_of = [&](int p0, int kr) -> uint32_t {
     const int b0 = p0 >> c.shift;
     if (b0 - window0 >= kWave) {
-      window0 = b0;
-      const int b = b0 + lane;
-      window = ~0u;
-      if (int64_t(b) << c.shift < it.hi) window = uint32_t(b < c.shared_blocks ? c.shared[b] : table[b]);
+      open_window(b0);
       asm volatile("" : "+v"(window));
       window = window < c.n_blocks ? window : ~0u;
     }
@@ -335,29 +351,46 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
     for (int d = 0; d < 4; d++) vat[d] = vr * HD * 2 + 16 * ((2 * d + ((col & 3) >> 1)) ^ swap8(vr)) + 8 * (col & 1);
   }
 
-  // Loads the queries of the lane's columns; `row0`: of the wave's first.
-  auto queries = [&](auto& st, int row0) {
+  // The queries of the lane's columns, from the wave's row `row0` on: their loads, which hang on no length (rows of no
+  // sequence are not read), then what is made of them.
+  int owned_lo = 0, owned_hi = c.n_tokens;
+  if (c.starts && it.end < 0) owned_lo = c.starts[0], owned_hi = c.starts[c.n_seqs];
+  constexpr int QW = TWOQ ? 2 : 1;
+  auto load_queries = [&](auto& raw, int row0) {
+    constexpr int NJ = sizeof(raw) / (KT * QW * 16);
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      const int i = row0 + 16 * j + col, r = it.first + (i < it.count ? i : 0), t = r / c.group;
+      const X* qr = q + t * c.q_stride + int64_t(it.head * c.group + r % c.group) * D;
+#pragma unroll
+      for (int k = 0; k < KT; k++) {
+        const int d = 32 * k + 8 * g;
+        const bool on = d < D && t >= owned_lo && t < owned_hi;
+        const uint8_t* p = on ? reinterpret_cast<const uint8_t*>(qr + d) : static_cast<const uint8_t*>(zeros);
+#pragma unroll
+        for (int e = 0; e < QW; e++) raw[j][k][e] = *reinterpret_cast<const u32x4*>(p + 16 * e);
+      }
+    }
+  };
+  auto queries = [&](auto& st, const auto& raw, int row0) {
     constexpr int NJ = sizeof(st.m) / sizeof(float);
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
       const int i = row0 + 16 * j + col;
       const bool mine = i < it.count;
-      const int r = it.first + (mine ? i : 0), t = r / c.group, h = it.head * c.group + r % c.group;
-      const int seen = mine ? paged_visible(c, t) : 0;
+      const int seen = mine ? paged_visible(c, (it.first + i) / c.group) : 0;
       st.limit[j] = seen;
-      const X* qr = q + t * c.q_stride + int64_t(h) * D;
       float v[KT][8], mx = 0.f;
 #pragma unroll
-      for (int k = 0; k < KT; k++) {
-        const int d = 32 * k + 8 * g;
-        const bool on = d < D && seen > 0;
-        if (on) load8<X>(qr + d, v[k]);
+      for (int k = 0; k < KT; k++)
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          v[k][e] = on ? v[k][e] : 0.f;
+          float x;
+          if constexpr (TWOQ) x = __uint_as_float(raw[j][k][e >> 2][e & 3]);
+          else x = float(__builtin_bit_cast(h8_t, raw[j][k][0])[e]);
+          v[k][e] = seen > 0 ? x : 0.f;
           mx = fmaxf(mx, fabsf(v[k][e]));
         }
-      }
       // each row's brought near 1 by a power of two that goes into the scores' factor
       mx = max_over_groups(mx);
       int ex = 0;
@@ -415,7 +448,12 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
     constexpr int KR = S::KR, NJ = S::NJ;
     AttendState<HD, NJ, TWOQ> st;
     if (tid == 0) s_low = INT32_MAX, s_bad = 0;
-    queries(st, wv * 16 * NJ);
+    open_window(it.lo >> c.shift);
+    u32x4 qraw[NJ][KT][QW];
+    load_queries(qraw, wv * 16 * NJ);
+    if (!paged_bound(c, plan, it)) return;
+    window = window < c.n_blocks ? window : ~0u;
+    queries(st, qraw, wv * 16 * NJ);
     const int low = lowest(st);
     __syncthreads();
     if (lane == 0) atomicMin(&s_low, low);
@@ -559,6 +597,11 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
   // -------------------------------------------------------------- D
   constexpr int KR = 32;
   AttendState<HD, NB, TWOQ> st;
+  open_window(it.lo >> c.shift);
+  u32x4 qraw[NB][KT][QW];
+  load_queries(qraw, 0);
+  if (!paged_bound(c, plan, it)) return;
+  window = window < c.n_blocks ? window : ~0u;
   const int steps = (it.hi - it.lo + KR - 1) / KR;
   uint8_t* const mine = s_kv + wv * S::kWaveLds;
   const uint32_t mine0 = lds0 + wv * S::kWaveLds;
@@ -636,8 +679,8 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
     there = __ballot(ids != ~0u);
     fetch(i, to, ids);
   };
-  if (AHEAD) ask(wv, 0);  // (before the queries: both are on their way at once)
-  queries(st, 0);
+  if (AHEAD) ask(wv, 0);
+  queries(st, qraw, 0);
   const int low = lowest(st);
   int buf = 0;
   for (int i = wv; i < steps; i += 4) {

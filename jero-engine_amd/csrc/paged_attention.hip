@@ -99,7 +99,7 @@ static PagedPlan paged_plan(const jero_paged_cache* k, bool f16, int64_t n_token
     return std::max<int64_t>(1, std::min((want + blocks - 1) / blocks, (span + least - 1) / least));
   };
   auto length = [](int64_t span, int64_t n) { return int(((span + n - 1) / n + 127) / 128 * 128); };
-  p.own_len = length(span, chunks(tiles * kv, span, 1024, 256));
+  p.own_len = length(span, chunks(tiles * kv, span, 512, 256));
   p.own_chunks = int((span + p.own_len - 1) / p.own_len);
   p.own_blocks = int(tiles * kv * p.own_chunks);
   if (apart) {
@@ -109,10 +109,10 @@ static PagedPlan paged_plan(const jero_paged_cache* k, bool f16, int64_t n_token
     // Chunks that take no longer than the call: with the cards' rates of a workgroup over the shared positions (us a position)
     // and of memory, four fifths of both phases' times one after the other.  64 f32 sequences, 8192 shared positions,
     // up to 1500 own: chunks of 1024 positions 67 us, of 512 73, of 256 79; 256 f16 sequences, 32768 and 700: chunks of
-    // 8192 372 us, of 16384 430, of 4096 383.
+    // 8192 372 us, of 16384 430, of 4096 383; 7 sequences, 2048 (f32 cache): of 128 21, of 256 25.
     const double rate = p.pre_wide ? (f16 ? 0.04 : 0.06) * (hd / 128.0) : 0.01, memory = 5e6;
     const double both = double(p.pre_tiles) * kv * shared * rate / 512 + double(k->n_seqs) * span * 0.6 * pair / memory;
-    const int64_t least = int64_t(std::max(256.0, 0.8 * both / rate));
+    const int64_t least = int64_t(std::max(128.0, 0.8 * both / rate));
     p.pre_len = length(shared, std::max<int64_t>(1, (shared + least - 1) / least));
     p.pre_chunks = int((shared + p.pre_len - 1) / p.pre_len);
     p.pre_blocks = p.pre_tiles * kv * p.pre_chunks;
