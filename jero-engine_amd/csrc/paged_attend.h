@@ -119,13 +119,15 @@ constexpr float kPagedLift = 11.f, kPagedGrow = 4.f;
 
 // KR positions from p0 on: S^T = K q^T leaves a row per lane column and, taken in the order 4g .. 4g + 3, 16 + 4g .. of
 // 32 positions, is the B operand of O^T += V^T p, V^T read from LDS transposed.  ok: positions that are there; bad:
-// those whose values are not finite and have been made zeros.
-template <int HD, int NJ, int KR, bool TWOQ, bool TWOK, typename KRead>
-__device__ __forceinline__ void attend_step(AttendState<HD, NJ, TWOQ>& st, KRead kread, const uint8_t* vp, int vplane,
-                                            const int (&vat)[4], int p0, bool masked, uint64_t ok, uint64_t bad, int g) {
+// those whose values are not finite and have been made zeros.  kread and vread give the products' operands; after_keys and
+// before_values are done in between.  EARLY: the values are in LDS from the start.
+template <int HD, int NJ, int KR, bool TWOQ, bool TWOK, bool EARLY, typename KRead, typename VRead, typename AfterKeys,
+          typename BeforeValues>
+__device__ __forceinline__ void attend_step(AttendState<HD, NJ, TWOQ>& st, KRead kread, VRead vread, AfterKeys after_keys,
+                                            BeforeValues before_values, int p0, bool masked, uint64_t ok, uint64_t bad, int g) {
   constexpr int RT = KR / 16, KT = HD / 32, DT = HD / 16, KP = TWOK ? 2 : 1;
   f4_t s[NJ][RT];
-  constexpr int KD = RT == 2 ? 3 : 2;  // (registers)
+  constexpr int KD = !EARLY ? 1 : RT == 2 ? 3 : 2;  // (registers; where values come late, keys are in them)
   h8_t ka[KD][RT][KP];
   auto read_k = [&](int k) {
 #pragma unroll
@@ -137,7 +139,8 @@ __device__ __forceinline__ void attend_step(AttendState<HD, NJ, TWOQ>& st, KRead
   for (int k = 0; k < KD - 1; k++) read_k(k);
 #pragma unroll
   for (int k = 0; k < KT; k++) {
-    if (k + KD - 1 < KT) read_k(k + KD - 1);
+    if (KD == 1) read_k(k);
+    else if (k + KD - 1 < KT) read_k(k + KD - 1);
 #pragma unroll
     for (int r = 0; r < RT; r++)
 #pragma unroll
@@ -157,22 +160,14 @@ __device__ __forceinline__ void attend_step(AttendState<HD, NJ, TWOQ>& st, KRead
     }
     __builtin_amdgcn_sched_barrier(0);
   }
+  after_keys();
   // the values' first operands are on their way during the softmax
   constexpr int VD = 3;
   h8_t va[VD][RT / 2][KP];
-  auto tr = [&](int d, int r, int plane) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(vp + plane * vplane + vat[d & 3] + 128 * (d >> 2) + 16 * r * HD * 2));
-  };
-  auto read_v = [&](int d) {
+  auto read_v = [&](int d) { vread(d, va[d % VD]); };
+  if constexpr (EARLY)
 #pragma unroll
-    for (int r = 0; r < RT / 2; r++)
-#pragma unroll
-      for (int e = 0; e < KP; e++)
-        va[d % VD][r][e] = __builtin_bit_cast(
-            h8_t, __builtin_shufflevector(tr(d, 2 * r, e), tr(d, 2 * r + 1, e), 0, 1, 2, 3, 4, 5, 6, 7));
-  };
-#pragma unroll
-  for (int d = 0; d < VD - 1; d++) read_v(d);
+    for (int d = 0; d < VD - 1; d++) read_v(d);
   h8_t bh[NJ][RT / 2], bl[NJ][RT / 2];
   bool grew[NJ];
   float alpha[NJ], times[NJ];
@@ -237,6 +232,11 @@ __device__ __forceinline__ void attend_step(AttendState<HD, NJ, TWOQ>& st, KRead
         if constexpr (TWOQ) st.l[j] = mfma(one, bl[j][r], st.l[j]);
       }
   }
+  if constexpr (!EARLY) {
+    before_values();
+#pragma unroll
+    for (int d = 0; d < VD - 1; d++) read_v(d);
+  }
 #pragma unroll
   for (int d = 0; d < DT; d++) {
     if (d + VD - 1 < DT) read_v(d + VD - 1);
@@ -257,6 +257,20 @@ __device__ __forceinline__ void attend_step(AttendState<HD, NJ, TWOQ>& st, KRead
   }
 }
 
+// Columns 16 d + col of the values of 32 N positions, as A operands: rows of f16 (in PARTS planes) read transposed.
+template <int HD, int N, int PARTS>
+__device__ __forceinline__ void read_transposed(const uint8_t* vp, int plane, const int (&vat)[4], int d, h8_t (&to)[N][PARTS]) {
+#pragma unroll
+  for (int r = 0; r < N; r++)
+#pragma unroll
+    for (int e = 0; e < PARTS; e++) {
+      const uint8_t* p = vp + e * plane + vat[d & 3] + 128 * (d >> 2) + 32 * r * HD * 2;
+      const s4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p);
+      const s4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 16 * HD * 2));
+      to[r][e] = __builtin_bit_cast(h8_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+}
+
 // ---------------------------------------------------------------- the kernel
 
 // F ("wide"): four waves share KR positions in LDS and hold 16 NJ rows each.  D ("narrow"): four waves share 16 NB rows and
@@ -264,26 +278,31 @@ __device__ __forceinline__ void attend_step(AttendState<HD, NJ, TWOQ>& st, KRead
 template <int HD, typename X, typename KV>
 struct PagedShape {
   static constexpr bool TWOQ = sizeof(X) == 4, TWOK = sizeof(KV) == 4;
-  static constexpr int NJ = HD <= 128 ? 2 : 1, KR = TWOQ || HD == 256 ? 32 : 64;
+  static constexpr int NJ = HD <= 128 && !TWOK ? 2 : 1, KR = TWOQ || HD == 256 ? 32 : 64;
   static constexpr int kRows = 64 * NJ;
   static constexpr int kPlanes = TWOK ? 2 : 1;
   static constexpr int kPlane = KR * HD * 2, kBuf = 2 * kPlanes * kPlane;  // keys, then values
   static constexpr int kBufs = TWOK ? 1 : HD == 256 ? 4 : 64 * 1024 / kBuf > 4 ? 4 : 64 * 1024 / kBuf;
-  static constexpr int kNarrow = 32 * HD * 2;                              // a wave's values
-  static constexpr int kWaveLds = kNarrow * (TWOK ? 2 : 2);                // two buffers, or two parts
+  static constexpr int kNarrow = 32 * HD * int(sizeof(KV));                // a wave's values
+  static constexpr int kValueBufs = TWOK && HD > 64 ? 1 : 2;
+  static constexpr int kWaveLds = kNarrow * kValueBufs;
   static constexpr int kJoin = 4 * 16 * (HD + 4) * 4;
   static constexpr int kMost = kBufs * kBuf > 4 * kWaveLds ? kBufs * kBuf : 4 * kWaveLds;
   static constexpr int kLds = kMost > kJoin ? kMost : kJoin;
-  static constexpr int kGroups = TWOK || HD == 256 ? 1 : 2;
+  static constexpr int kGroups = HD == 256 ? 1 : 2;
 };
 
-// Infinities or NaN among 8 f16: their exponent's bits all set.
-__device__ __forceinline__ bool odd8(u32x4 v) {
-  auto one = [](uint32_t w) {
-    const uint32_t e = w & 0x7C007C00u;
-    return (e & 0xFFFFu) == 0x7C00u || (e >> 16) == 0x7C00u;
-  };
-  return one(v.x) || one(v.y) || one(v.z) || one(v.w);
+// Whether 16 bytes of values have one that is not finite as f16: the exponent's bits all set, or an f32 that rounds past 65504.
+template <typename KV>
+__device__ __forceinline__ bool odd_piece(u32x4 v) {
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint32_t w = v[i];
+    if constexpr (sizeof(KV) == 4) odd |= !(fabsf(__uint_as_float(w)) < 65520.f);
+    else odd |= (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
+  }
+  return odd;
 }
 
 template <int HD, typename X, typename KV, int NB>
@@ -559,7 +578,7 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
         constexpr int L = HD / 8;
         uint8_t* const rows = kv + S::kPlanes * S::kPlane;
         for (int n = tid; n < KR * L; n += 256)
-          if (odd8(*reinterpret_cast<const u32x4*>(rows + 16 * n))) atomicOr(&s_bad, 1ull << (n / L));
+          if (odd_piece<_Float16>(*reinterpret_cast<const u32x4*>(rows + 16 * n))) atomicOr(&s_bad, 1ull << (n / L));
         __syncthreads();
         bad = s_bad;
         if (bad) {
@@ -578,7 +597,9 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
                                               128 * (k >> 1));
       };
       const bool masked = p0 + KR > low || ok != ~0ull || p0 + KR > it.hi;
-      attend_step<HD, NJ, KR, TWOQ, TWOK>(st, kread, kv + S::kPlanes * S::kPlane, S::kPlane, vat, p0, masked, ok, bad, g);
+      auto vread = [&](int d, auto& to) { read_transposed<HD, KR / 32, S::kPlanes>(kv + S::kPlanes * S::kPlane, S::kPlane, vat, d, to); };
+      auto none = [] {};
+      attend_step<HD, NJ, KR, TWOQ, TWOK, true>(st, kread, vread, none, none, p0, masked, ok, bad, g);
       if (!TWOK) buf = buf == S::kBufs - 1 ? 0 : buf + 1;
     }
 #pragma unroll
@@ -605,46 +626,45 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
   const int steps = (it.hi - it.lo + KR - 1) / KR;
   uint8_t* const mine = s_kv + wv * S::kWaveLds;
   const uint32_t mine0 = lds0 + wv * S::kWaveLds;
-  constexpr bool AHEAD = !(TWOK && HD == 256);  // (its registers hold one step)
-  constexpr int KRAW = TWOK ? 2 : 1;            // 16-byte pieces for 8 values
-  u32x4 kraw[2][KT][KRAW];                      // keys: row 16 r + col, values 32 k + 8 g ..
-  constexpr int NV = TWOK ? 32 * HD / 8 / 64 : 1;
-  u32x4 vraw[NV][2];
-  // (a piece's rows are swapped by their number's last three bits: with 2 or 4 rows a piece, 4 or 2 patterns)
-  constexpr int PAT = RPI < 8 ? 8 / RPI : 1;
-  uint32_t lane_bytes[PAT];
+  constexpr int KRAW = TWOK ? 2 : 1;  // 16-byte pieces for 8 values
+  u32x4 kraw[2][KT][KRAW];            // keys: row 16 r + col, values 32 k + 8 g ..
+  // Values go straight to LDS, pieces of 1024 bytes.  f16 rows are swapped by their number's last three bits: with 2 or 4
+  // rows a piece, 4 or 2 patterns.  f32 rows by 64 bytes, by (r >> 2) & 3: the four rows that a read wants at once, 4 apart,
+  // are then on banks of their own.
+  constexpr int VR = 1024 / (HD * int(sizeof(KV))), PIECES = 32 / VR;
+  constexpr int PAT = TWOK ? 1 : VR < 8 ? 8 / VR : 1;
+  const int lane_row = lane / (64 / VR);
+  int lane_at[PAT];
 #pragma unroll
-  for (int i = 0; i < PAT; i++) {
-    const int r = i * RPI + lane / (HD / 8), at = (16 * lane) % (2 * HD) ^ (16 * swap8(r));
-    lane_bytes[i] = uint32_t(lane / (HD / 8) * row_bytes) + (at < 2 * D ? at : 0);
-  }
-  auto fetch = [&](int step, int buf, uint32_t ids) {
-    const int p0 = it.lo + step * KR;
-    const bool whole = __ballot(ids != ~0u) == ~0ull;
-    if (!TWOK && whole && (1 << c.shift) >= RPI) {
+  for (int i = 0; i < PAT; i++)
+    lane_at[i] = 16 * lane % (1024 / VR) ^ (TWOK ? 0 : 16 * swap8(i * VR + lane_row));
+  auto value_at = [&](int i) {  // byte of the row that the lane loads of piece i
+    if constexpr (TWOK) return lane_at[0] ^ (64 * ((i * VR >> 2) & 3));
+    else return lane_at[i % PAT];
+  };
+  constexpr int kKeyLoads = 2 * KT * KRAW;
+  auto fetch_values = [&](int step, int buf, uint32_t ids) {
+    const int p0 = it.lo + step * KR, bytes = D * int(sizeof(KV));
+    const uint32_t to = mine0 + buf * S::kNarrow;
+    if (__ballot(ids != ~0u) == ~0ull && (1 << c.shift) >= VR) {
 #pragma unroll
-      for (int i = 0; i < S::kNarrow / 1024; i++)
-        dma_row(reinterpret_cast<const uint8_t*>(vb) + offset_of(ids, i * RPI, p0), lane_bytes[i % PAT],
-                mine0 + buf * S::kNarrow + i * 1024);
-    } else if constexpr (!TWOK) {
-#pragma unroll
-      for (int i = 0; i < S::kNarrow / 1024; i++) {
-        const int b = i * 1024 + 16 * lane, r = b / (2 * HD), at = (b % (2 * HD)) ^ (16 * swap8(r));
-        const uint32_t id = __shfl(ids, r, kWave);
-        dma_lanes(id != ~0u && at < 2 * D ? row_of(vb, id, p0 + r) + at : zeros, mine0 + buf * S::kNarrow + i * 1024);
+      for (int i = 0; i < PIECES; i++) {
+        const int at = value_at(i);
+        dma_row(reinterpret_cast<const uint8_t*>(vb) + offset_of(ids, i * VR, p0),
+                uint32_t(lane_row * row_bytes) + (at < bytes ? at : 0), to + i * 1024);
       }
-    } else {
-#pragma unroll
-      for (int n = 0; n < NV; n++) {
-        const int i = n * 64 + lane, r = i / (HD / 8), d = 8 * (i % (HD / 8));
-        const uint32_t id = __shfl(ids, r, kWave);
-        const bool on = id != ~0u && d < D;
-        const uint8_t* p = static_cast<const uint8_t*>(on ? static_cast<const void*>(row_of(vb, id, p0 + r) + 4 * d) : zeros);
-        vraw[n][0] = *reinterpret_cast<const u32x4*>(p);
-        vraw[n][1] = *reinterpret_cast<const u32x4*>(p + (on ? 16 : 0));
-      }
+      return;
     }
-    if (whole && c.shift >= 4) {
+#pragma unroll
+    for (int i = 0; i < PIECES; i++) {
+      const int r = i * VR + lane_row, at = value_at(i);
+      const uint32_t id = __shfl(ids, r, kWave);
+      dma_lanes(id != ~0u && at < bytes ? row_of(vb, id, p0 + r) + at : zeros, to + i * 1024);
+    }
+  };
+  auto fetch_keys = [&](int step, uint32_t ids) {
+    const int p0 = it.lo + step * KR;
+    if (__ballot(ids != ~0u) == ~0ull && c.shift >= 4) {
 #pragma unroll
       for (int r = 0; r < 2; r++) {
         const uint8_t* row = reinterpret_cast<const uint8_t*>(kb) + offset_of(ids, 16 * r, p0);
@@ -672,63 +692,44 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
       }
     }
   };
-  uint64_t there = 0;
-  auto ask = [&](int i, int to) {
-    if (i >= steps) return;
-    const uint32_t ids = blocks_of(it.lo + i * KR, KR);
-    there = __ballot(ids != ~0u);
-    fetch(i, to, ids);
-  };
-  if (AHEAD) ask(wv, 0);
+  uint32_t ids = ~0u;
+  if (wv < steps) {
+    ids = blocks_of(it.lo + wv * KR, KR);
+    fetch_values(wv, 0, ids);
+    fetch_keys(wv, ids);
+  }
   queries(st, qraw, 0);
   const int low = lowest(st);
+  // Where LDS and registers hold two steps' values and keys, the next step's are asked for at a step's start; otherwise
+  // when its own are used up.
+  constexpr bool TWO_V = S::kValueBufs == 2, TWO_K = HD == 64 || (!TWOK && NB == 1);
   int buf = 0;
   for (int i = wv; i < steps; i += 4) {
     const int p0 = it.lo + i * KR;
-    if constexpr (!AHEAD) ask(i, 0);
-    const uint64_t ok = there;
-    dma_wait<0>();
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last step's reads of the buffer that is loaded next
-    uint8_t* const vp = mine + (TWOK ? 0 : buf * S::kNarrow);
-    h8_t kc[2][KT][TWOK ? 2 : 1];
+    const uint64_t ok = __ballot(ids != ~0u);
+    const bool more = i + 4 < steps;
+    uint8_t* const vp = mine + (TWO_V ? buf * S::kNarrow : 0);
+    if (more) ids = blocks_of(p0 + 4 * KR, KR);
+    if constexpr (TWO_V) {
+      dma_wait<0>();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last step's reads of the buffer that is loaded next
+    }
+    u32x4 kc[2][KT][KRAW];
 #pragma unroll
     for (int r = 0; r < 2; r++)
 #pragma unroll
-      for (int k = 0; k < KT; k++) {
-        if constexpr (!TWOK) {
-          kc[r][k][0] = __builtin_bit_cast(h8_t, kraw[r][k][0]);
-        } else {
+      for (int k = 0; k < KT; k++)
 #pragma unroll
-          for (int e = 0; e < 8; e++) {
-            _Float16 a, b;
-            split2(__uint_as_float(kraw[r][k][(KRAW - 1) * (e >> 2)][e & 3]), a, b);
-            kc[r][k][0][e] = a, kc[r][k][TWOK ? 1 : 0][e] = b;
-          }
-        }
-      }
-    if constexpr (TWOK) {
-#pragma unroll
-      for (int n = 0; n < NV; n++) {
-        const int b = n * 64 + lane, r = b / (HD / 8), d = b % (HD / 8);
-        h8_t hi, lo;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          _Float16 x, y;
-          split2(__uint_as_float(vraw[n][e >> 2][e & 3]), x, y);
-          hi[e] = x, lo[e] = y;
-        }
-        uint8_t* to = vp + r * HD * 2 + 16 * (d ^ swap8(r));
-        *reinterpret_cast<h8_t*>(to) = hi;
-        *reinterpret_cast<h8_t*>(to + S::kNarrow) = lo;
-      }
-    }
-    if (AHEAD) ask(i + 4, buf ^ 1);
+        for (int e = 0; e < KRAW; e++) kc[r][k][e] = kraw[r][k][e];
+    if (TWO_K && more) fetch_keys(i + 4, ids);
+    if (TWO_V && more) fetch_values(i + 4, buf ^ 1, ids);
+    const bool check = min(p0 + KR, it.hi) > low;
+    if (!TWO_V && check) dma_wait<0>();
     uint64_t bad = 0;
-    if (min(p0 + KR, it.hi) > low) {
-      constexpr int L = HD / 8;
+    if (check) {
+      constexpr int L = HD * int(sizeof(KV)) / 16;  // pieces of 16 bytes a row
       for (int n = lane; n < KR * L; n += 64) {
-        const bool odd = odd8(*reinterpret_cast<const u32x4*>(vp + 16 * n));
-        const uint64_t b = __ballot(odd);
+        const uint64_t b = __ballot(odd_piece<KV>(*reinterpret_cast<const u32x4*>(vp + 16 * n)));
 #pragma unroll
         for (int x = 0; x < 64; x += L)
           if ((b >> x) & (L == 64 ? ~0ull : (1ull << (L & 63)) - 1)) bad |= 1ull << ((n - lane + x) / L);
@@ -736,15 +737,51 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
       if (bad) {
         const u32x4 z = {0u, 0u, 0u, 0u};
         for (int n = lane; n < KR * L; n += 64)
-          if ((bad >> (n / L)) & 1) {
-            *reinterpret_cast<u32x4*>(vp + 16 * n) = z;
-            if (TWOK) *reinterpret_cast<u32x4*>(vp + S::kNarrow + 16 * n) = z;
-          }
+          if ((bad >> (n / L)) & 1) *reinterpret_cast<u32x4*>(vp + 16 * n) = z;
       }
     }
     const bool masked = p0 + KR > low || ok != ~0ull || p0 + KR > it.hi;
-    auto kread = [&](int k, int r, int e) { return kc[r][k][e]; };
-    attend_step<HD, NB, KR, TWOQ, TWOK>(st, kread, vp, S::kNarrow, vat, p0, masked, ok, bad, g);
+    auto kread = [&](int k, int r, int e) {
+      if constexpr (!TWOK) {
+        return __builtin_bit_cast(h8_t, kc[r][k][0]);
+      } else {
+        h8_t part;
+#pragma unroll
+        for (int x = 0; x < 8; x++) {
+          _Float16 a, b;
+          split2(__uint_as_float(kc[r][k][(KRAW - 1) * (x >> 2)][x & 3]), a, b);
+          part[x] = e ? b : a;
+        }
+        return part;
+      }
+    };
+    auto after_keys = [&] {
+      if (!TWO_K && more) fetch_keys(i + 4, ids);
+    };
+    auto before_values = [&] {  // (the next keys' loads, behind the values', stay on their way)
+      if (more) dma_wait<kKeyLoads>();
+      else dma_wait<0>();
+    };
+    auto vread = [&](int d, auto& to) {
+      if constexpr (!TWOK) {
+        read_transposed<HD, 1, 1>(vp, 0, vat, d, to);
+      } else {
+        const uint8_t* p = vp + 4 * g * HD * 4 + ((64 * g) ^ (64 * (d & 3))) + 256 * (d >> 2) + 4 * col;
+        h8_t hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          _Float16 x, y;
+          split2(*reinterpret_cast<const float*>(p + ((e & 3) + 16 * (e >> 2)) * HD * 4), x, y);
+          hi[e] = x, lo[e] = y;
+        }
+        to[0][0] = hi, to[0][TWOK ? 1 : 0] = lo;
+      }
+    };
+    attend_step<HD, NB, KR, TWOQ, TWOK, TWO_V>(st, kread, vread, after_keys, before_values, p0, masked, ok, bad, g);
+    if (!TWO_V && more) {  // (the one buffer is free when its reads are done)
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      fetch_values(i + 4, 0, ids);
+    }
     buf ^= 1;
   }
   // the four waves' rows joined, 16 at a time

@@ -81,13 +81,13 @@ static PagedPlan paged_plan(const jero_paged_cache* k, bool f16, int64_t n_token
   const int group = n_heads / k->n_heads_kv, hd = head_width(k->head_dim), kv = k->n_heads_kv;
   const int64_t shared = std::min<int64_t>(k->shared_blocks * k->block_size, k->max_len);
   const int64_t rows = n_tokens * group, each = (n_tokens + k->n_seqs - 1) / k->n_seqs * group;
-  p.wide_rows = hd <= 128 ? 128 : 64;
+  p.wide_rows = hd <= 128 && k->kv_dtype == JERO_KV_F16 ? 128 : 64;
   // Rows of all sequences go over the shared positions together where sequences do not fill tiles themselves and more than
-  // 48 MB are spared: 32 sequences x 256 shared positions x 8 heads of 128 (f16, 33 MB) 26 us and 30 apart and not, 8 x
+  // 48 MB (24 of f32, whose rows cost more than their bytes) are spared: 32 sequences x 256 shared positions x 8 heads of 128 (f16, 33 MB) 26 us and 30 apart and not, 8 x
   // 1024 (29 MB) 24 and 19, 128 x 64 (33 MB) 60 and 55, 128 x 256 (133 MB) 59 and 61, 8 x 4096 (117 MB) 30 and 32,
   // 128 x 4096 69 and 192.
   const double pair = 2.0 * kv * k->head_dim * (k->kv_dtype == JERO_KV_F16 ? 2 : 4);  // bytes of a position
-  const bool apart = k->n_seqs > 1 && each < p.wide_rows && double(k->n_seqs - 1) * shared * pair >= 48e6;
+  const bool apart = k->n_seqs > 1 && each < p.wide_rows && double(k->n_seqs - 1) * shared * pair >= (k->kv_dtype == JERO_KV_F16 ? 48e6 : 24e6);
   p.narrow_rows = hd < 256 && (each > 16 || (apart && rows > 16 && rows <= 32)) ? 32 : 16;
   p.own_wide = each > p.narrow_rows;
   p.own_lo = apart ? int(shared) : 0;
