@@ -23,11 +23,12 @@ struct PagedCall {
 // How a call's work is cut.  Its two phases, the shared positions for the rows of all sequences and each sequence's
 // own from own_lo on, are cut into tiles of rows and chunks of positions; each chunk of a row is a part, joined
 // by paged_merge_kernel where there are more than one.
+constexpr int kNarrowRows = 16;
 struct PagedPlan {
   int pre_blocks, pre_tiles, pre_chunks, pre_len;
   int own_blocks, own_tiles, own_chunks, own_len, own_lo;
   int parts;
-  int wide_rows, narrow_rows;
+  int wide_rows;
   int pre_wide, own_wide;
 };
 

@@ -10,6 +10,18 @@ namespace jero {
 // What places that hold nothing are read from: 8 values of either type.
 __device__ __constant__ const uint32_t kPagedZeros[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
 
+// The swap of a row's 16-byte chunks in LDS, chunk k of row r at k ^ swap(r): f16 rows of HD.  LDS has 64 banks of 4 bytes.  A
+// read of 16 bytes a lane goes by 16 lanes: those of 8 rows at one chunk and of the 8 others at the next (lanes 0 - 3,
+// 12 - 15 and 20 - 27, then 4 - 11, 16 - 19 and 28 - 31); a transposing read by 32, two chunks of 8 rows.  Neither meets on
+// a bank: rows of 256 bytes and more have 16 chunks to swap, rows of 128 two to a round of the banks.  (Swaps within 128
+// bytes: 2 ways, and chunks of nine prompts took 635 us.)  It is linear in the row's bits, so that a swap by a constant is
+// one more exclusive or.
+template <int HD>
+__host__ __device__ __forceinline__ constexpr int swap_of(int r) {
+  const int x = HD == 64 ? r >> 1 : r;
+  return HD == 64 ? ((x & 3) << 1) ^ ((x & 4) ? 5 : 0) : ((x & 7) << 1) ^ ((x & 8) ? 9 : 0);
+}
+
 // ---------------------------------------------------------------- what a workgroup works on
 
 // Position below which token row t of the call attends (t's own and max_len within it), by every lane on its own.
@@ -48,7 +60,7 @@ __device__ __forceinline__ bool paged_item(const PagedCall& c, const PagedPlan& 
   const int rest = i / c.kv_heads;
   if (pre) {
     const int tile = rest % p.pre_tiles, chunk = rest / p.pre_tiles;
-    const int rows = p.pre_wide ? p.wide_rows : p.narrow_rows;
+    const int rows = p.pre_wide ? p.wide_rows : kNarrowRows;
     wide = p.pre_wide;
     it.first = tile * rows;
     it.count = min(rows, c.n_tokens * c.group - it.first);
@@ -58,7 +70,7 @@ __device__ __forceinline__ bool paged_item(const PagedCall& c, const PagedPlan& 
     return true;
   }
   wide = p.own_wide;
-  const int rows = wide ? p.wide_rows : p.narrow_rows;
+  const int rows = wide ? p.wide_rows : kNarrowRows;
   const int chunk = rest / p.own_tiles, tile = p.own_tiles - 1 - rest % p.own_tiles;
   int end, from, skip = 0;
   if (!c.starts) {
@@ -257,23 +269,37 @@ __device__ __forceinline__ void attend_step(AttendState<HD, NJ, TWOQ>& st, KRead
   }
 }
 
+typedef __attribute__((address_space(3))) h8_t lds_h8;
+
+// Where a lane reads: keys' rows 16 r + col from chunk g on, values' rows 4 g + (col >> 2) transposed; then 64 bytes of the row
+// further for each k, 32 for each d, within 256 by an exclusive or.
+template <int HD>
+__device__ __forceinline__ uint32_t key_lane(int g, int col) {
+  return uint32_t(col * HD * 2 + 16 * (g ^ swap_of<HD>(col)));
+}
+template <int HD>
+__device__ __forceinline__ uint32_t value_lane(int g, int col) {
+  const int r = 4 * g + (col >> 2);
+  return uint32_t(r * HD * 2 + 16 * (((col & 3) >> 1) ^ swap_of<HD>(r)) + 8 * (col & 1));
+}
 // Columns 16 d + col of the values of 32 N positions, as A operands: rows of f16 (in PARTS planes) read transposed.
 template <int HD, int N, int PARTS>
-__device__ __forceinline__ void read_transposed(const uint8_t* vp, int plane, const int (&vat)[4], int d, h8_t (&to)[N][PARTS]) {
+__device__ __forceinline__ void read_transposed(uint32_t at, int plane, int d, h8_t (&to)[N][PARTS]) {
+  const uint32_t p = (at ^ (32 * (d & 7))) + 256 * (d >> 3);
 #pragma unroll
   for (int r = 0; r < N; r++)
 #pragma unroll
     for (int e = 0; e < PARTS; e++) {
-      const uint8_t* p = vp + e * plane + vat[d & 3] + 128 * (d >> 2) + 32 * r * HD * 2;
-      const s4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p);
-      const s4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 16 * HD * 2));
+      const uint32_t q = p + e * plane + 32 * r * HD * 2;
+      const s4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)uintptr_t(q));
+      const s4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)uintptr_t(q + 16 * HD * 2));
       to[r][e] = __builtin_bit_cast(h8_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 }
 
 // ---------------------------------------------------------------- the kernel
 
-// F ("wide"): four waves share KR positions in LDS and hold 16 NJ rows each.  D ("narrow"): four waves share 16 NB rows and
+// F ("wide"): four waves share KR positions in LDS and hold 16 NJ rows each.  D ("narrow"): four waves share 16 rows and
 // hold 32 positions each, keys in registers, values in their own part of LDS; they are joined at the end.
 template <int HD, typename X, typename KV>
 struct PagedShape {
@@ -305,14 +331,14 @@ __device__ __forceinline__ bool odd_piece(u32x4 v) {
   return odd;
 }
 
-template <int HD, typename X, typename KV, int NB>
+template <int HD, typename X, typename KV>
 __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
     paged_attend_kernel(PagedCall c, PagedPlan plan, const X* __restrict__ q, X* __restrict__ out,
                         float* __restrict__ part_o, float2* __restrict__ part_ml) {
   using S = PagedShape<HD, X, KV>;
   constexpr bool TWOQ = S::TWOQ, TWOK = S::TWOK;
   constexpr int KT = HD / 32, DT = HD / 16;
-  __shared__ __attribute__((aligned(16))) uint8_t s_kv[S::kLds];
+  __shared__ __attribute__((aligned(256))) uint8_t s_kv[S::kLds];
   __shared__ float s_m[4][16], s_l[4][16];
   __shared__ int s_low;
   __shared__ unsigned long long s_bad;
@@ -363,12 +389,7 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
   auto row_of = [&](const KV* base, uint32_t id, int pos) -> const uint8_t* {
     return reinterpret_cast<const uint8_t*>(base + ((int64_t(id) << c.shift) + (pos & ((1 << c.shift) - 1))) * row_len);
   };
-  int vat[4];
-  {
-    const int vr = 4 * g + (col >> 2);
-#pragma unroll
-    for (int d = 0; d < 4; d++) vat[d] = vr * HD * 2 + 16 * ((2 * d + ((col & 3) >> 1)) ^ swap8(vr)) + 8 * (col & 1);
-  }
+  const uint32_t value0 = value_lane<HD>(g, col);
 
   // The queries of the lane's columns, from the wave's row `row0` on: their loads, which hang on no length (rows of no
   // sequence are not read), then what is made of them.
@@ -481,8 +502,8 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
     const int steps = (it.hi - it.lo + KR - 1) / KR;
     constexpr int NI = S::kPlane / 1024 / 4;  // 1024-byte pieces a wave, of keys and of values
     const int lane_row = lane / (HD / 8);
-    const int lane_at = (16 * lane) % (2 * HD) ^ (16 * swap8(wv * RPI + lane_row));  // (4 pieces further on: 16 rows)
-    const uint32_t lane_bytes = uint32_t(lane_row * row_bytes) + (lane_at < 2 * D ? lane_at : 0);
+    const int lane_at = (16 * lane) % (2 * HD) ^ (16 * swap_of<HD>(wv * RPI + lane_row));
+    auto piece_at = [&](int n) { return lane_at ^ (16 * swap_of<HD>(4 * n * RPI)); };  // piece 4 n + wv
     auto load = [&](int step, int buf, uint32_t ids) {  // f16: straight to LDS
       const int p0 = it.lo + step * KR;
       if (__ballot(ids != ~0u) == ~0ull && (1 << c.shift) >= RPI) {
@@ -491,6 +512,7 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
           const int i = 4 * n + wv;
           const int64_t at = offset_of(ids, i * RPI, p0);
           const uint32_t to = lds0 + buf * S::kBuf + i * 1024;
+          const uint32_t lane_bytes = uint32_t(lane_row * row_bytes) + (piece_at(n) < 2 * D ? piece_at(n) : 0);
           dma_row(reinterpret_cast<const uint8_t*>(kb) + at, lane_bytes, to);
           dma_row(reinterpret_cast<const uint8_t*>(vb) + at, lane_bytes, to + S::kPlane);
         }
@@ -498,8 +520,7 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
       }
 #pragma unroll
       for (int n = 0; n < NI; n++) {
-        const int i = 4 * n + wv, b = i * 1024 + 16 * lane, r = b / (2 * HD);
-        const int at = (b % (2 * HD)) ^ (16 * swap8(r));
+        const int i = 4 * n + wv, r = i * RPI + lane_row, at = piece_at(n);
         const uint32_t id = __shfl(ids, r, kWave);
         const bool on = id != ~0u && at < 2 * D;
         const uint32_t to = lds0 + buf * S::kBuf + i * 1024;
@@ -535,12 +556,12 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
             split2(raw[w][n][e], a, b);
             hi[e] = a, lo[e] = b;
           }
-          uint8_t* to = s_kv + w * S::kPlanes * S::kPlane + r * HD * 2 + 16 * (d ^ swap8(r));
+          uint8_t* to = s_kv + w * S::kPlanes * S::kPlane + r * HD * 2 + 16 * (d ^ swap_of<HD>(r));
           *reinterpret_cast<h8_t*>(to) = hi;
           *reinterpret_cast<h8_t*>(to + S::kPlane) = lo;
         }
     };
-    const int kat = 16 * (g ^ swap8(col)), kat4 = 16 * ((4 + g) ^ swap8(col));
+    const uint32_t key0 = key_lane<HD>(g, col);
     // tiles on their way: A of them, each kLoads loads a wave; and which of their positions are there
     constexpr int A = TWOK ? 1 : S::kBufs - 1, kLoads = 2 * NI;
     uint64_t there[A];
@@ -592,12 +613,15 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
         __syncthreads();
         if (tid == 0) s_bad = 0;  // (the next step's barriers come before its next use)
       }
+      const uint32_t at = lds0 + buf * S::kBuf;
       auto kread = [&](int k, int r, int e) {
-        return *reinterpret_cast<const h8_t*>(kv + e * S::kPlane + (16 * r + col) * HD * 2 + ((k & 1) ? kat4 : kat) +
-                                              128 * (k >> 1));
+        const uint32_t p = ((at + key0) ^ (64 * (k & 3))) + 256 * (k >> 2);
+        return *(lds_h8*)uintptr_t(p + e * S::kPlane + 16 * r * HD * 2);
+      };
+      auto vread = [&](int d, auto& to) {
+        read_transposed<HD, KR / 32, S::kPlanes>(at + S::kPlanes * S::kPlane + value0, S::kPlane, d, to);
       };
       const bool masked = p0 + KR > low || ok != ~0ull || p0 + KR > it.hi;
-      auto vread = [&](int d, auto& to) { read_transposed<HD, KR / 32, S::kPlanes>(kv + S::kPlanes * S::kPlane, S::kPlane, vat, d, to); };
       auto none = [] {};
       attend_step<HD, NJ, KR, TWOQ, TWOK, true>(st, kread, vread, none, none, p0, masked, ok, bad, g);
       if (!TWOK) buf = buf == S::kBufs - 1 ? 0 : buf + 1;
@@ -617,9 +641,9 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
 
   // -------------------------------------------------------------- D
   constexpr int KR = 32;
-  AttendState<HD, NB, TWOQ> st;
+  AttendState<HD, 1, TWOQ> st;
   open_window(it.lo >> c.shift);
-  u32x4 qraw[NB][KT][QW];
+  u32x4 qraw[1][KT][QW];
   load_queries(qraw, 0);
   if (!paged_bound(c, plan, it)) return;
   window = window < c.n_blocks ? window : ~0u;
@@ -628,19 +652,13 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
   const uint32_t mine0 = lds0 + wv * S::kWaveLds;
   constexpr int KRAW = TWOK ? 2 : 1;  // 16-byte pieces for 8 values
   u32x4 kraw[2][KT][KRAW];            // keys: row 16 r + col, values 32 k + 8 g ..
-  // Values go straight to LDS, pieces of 1024 bytes.  f16 rows are swapped by their number's last three bits: with 2 or 4
-  // rows a piece, 4 or 2 patterns.  f32 rows by 64 bytes, by (r >> 2) & 3: the four rows that a read wants at once, 4 apart,
-  // are then on banks of their own.
+  // Values go straight to LDS, pieces of 1024 bytes.  f32 rows are swapped by 64 bytes, by (r >> 2) & 3: the four rows that a
+  // read wants at once, 4 apart, are then on banks of their own.
   constexpr int VR = 1024 / (HD * int(sizeof(KV))), PIECES = 32 / VR;
-  constexpr int PAT = TWOK ? 1 : VR < 8 ? 8 / VR : 1;
   const int lane_row = lane / (64 / VR);
-  int lane_at[PAT];
-#pragma unroll
-  for (int i = 0; i < PAT; i++)
-    lane_at[i] = 16 * lane % (1024 / VR) ^ (TWOK ? 0 : 16 * swap8(i * VR + lane_row));
+  const int lane_at = 16 * lane % (1024 / VR) ^ (TWOK ? 0 : 16 * swap_of<HD>(lane_row));
   auto value_at = [&](int i) {  // byte of the row that the lane loads of piece i
-    if constexpr (TWOK) return lane_at[0] ^ (64 * ((i * VR >> 2) & 3));
-    else return lane_at[i % PAT];
+    return lane_at ^ (TWOK ? 64 * ((i * VR >> 2) & 3) : 16 * swap_of<HD>(i * VR));
   };
   constexpr int kKeyLoads = 2 * KT * KRAW;
   auto fetch_values = [&](int step, int buf, uint32_t ids) {
@@ -702,7 +720,7 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
   const int low = lowest(st);
   // Where LDS and registers hold two steps' values and keys, the next step's are asked for at a step's start; otherwise
   // when its own are used up.
-  constexpr bool TWO_V = S::kValueBufs == 2, TWO_K = HD == 64 || (!TWOK && NB == 1);
+  constexpr bool TWO_V = S::kValueBufs == 2, TWO_K = HD == 64 || !TWOK;
   int buf = 0;
   for (int i = wv; i < steps; i += 4) {
     const int p0 = it.lo + i * KR;
@@ -764,7 +782,7 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
     };
     auto vread = [&](int d, auto& to) {
       if constexpr (!TWOK) {
-        read_transposed<HD, 1, 1>(vp, 0, vat, d, to);
+        read_transposed<HD, 1, 1>(mine0 + uint32_t(vp - mine) + value0, 0, d, to);
       } else {
         const uint8_t* p = vp + 4 * g * HD * 4 + ((64 * g) ^ (64 * (d & 3))) + 256 * (d >> 2) + 4 * col;
         h8_t hi, lo;
@@ -777,47 +795,43 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
         to[0][0] = hi, to[0][TWOK ? 1 : 0] = lo;
       }
     };
-    attend_step<HD, NB, KR, TWOQ, TWOK, TWO_V>(st, kread, vread, after_keys, before_values, p0, masked, ok, bad, g);
+    attend_step<HD, 1, KR, TWOQ, TWOK, TWO_V>(st, kread, vread, after_keys, before_values, p0, masked, ok, bad, g);
     if (!TWO_V && more) {  // (the one buffer is free when its reads are done)
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       fetch_values(i + 4, 0, ids);
     }
     buf ^= 1;
   }
-  // the four waves' rows joined, 16 at a time
+  // the four waves' rows joined
   float* const rows = reinterpret_cast<float*>(s_kv);
+  if (g == 0) s_m[wv][col] = st.m[0], s_l[wv][col] = st.l[0][0];
+  __syncthreads();
+  float m = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < NB; j++) {
-    __syncthreads();
-    if (g == 0) s_m[wv][col] = st.m[j], s_l[wv][col] = st.l[j][0];
-    __syncthreads();
-    float m = -INFINITY;
+  for (int w = 0; w < 4; w++) m = fmaxf(m, s_m[w][col]);
+  const float ref = m == -INFINITY ? 0.f : m, f = __builtin_amdgcn_exp2f(st.m[0] - ref);
 #pragma unroll
-    for (int w = 0; w < 4; w++) m = fmaxf(m, s_m[w][col]);
-    const float ref = m == -INFINITY ? 0.f : m, f = __builtin_amdgcn_exp2f(st.m[j] - ref);
+  for (int d = 0; d < DT; d++)
+    *reinterpret_cast<f4_t*>(rows + (wv * 16 + col) * (HD + 4) + 16 * d + 4 * g) = st.o[0][d] * f;
+  __syncthreads();
+  for (int n = tid; n < 16 * HD / 4; n += 256) {
+    const int r = n / (HD / 4), d = 4 * (n % (HD / 4));
+    if (r >= it.count) continue;
+    const int seen = paged_visible(c, (it.first + r) / c.group);
+    if (seen < 0) continue;
+    const bool sees = seen > it.lo;
+    float mm = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int d = 0; d < DT; d++)
-      *reinterpret_cast<f4_t*>(rows + (wv * 16 + col) * (HD + 4) + 16 * d + 4 * g) = st.o[j][d] * f;
-    __syncthreads();
-    for (int n = tid; n < 16 * HD / 4; n += 256) {
-      const int r = n / (HD / 4), d = 4 * (n % (HD / 4)), i = 16 * j + r;
-      if (i >= it.count) continue;
-      const int seen = paged_visible(c, (it.first + i) / c.group);
-      if (seen < 0) continue;
-      const bool sees = seen > it.lo;
-      float mm = -INFINITY, l = 0.f;
+    for (int w = 0; w < 4; w++) mm = fmaxf(mm, s_m[w][r]);
+    const float at = mm == -INFINITY ? 0.f : mm;
+    f4_t v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < 4; w++) mm = fmaxf(mm, s_m[w][r]);
-      const float at = mm == -INFINITY ? 0.f : mm;
-      f4_t v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < 4; w++) {
-        l += s_l[w][r] * __builtin_amdgcn_exp2f(s_m[w][r] - at);
-        v += *reinterpret_cast<const f4_t*>(rows + (w * 16 + r) * (HD + 4) + d);
-      }
-      const f4_t z = {0.f, 0.f, 0.f, 0.f};
-      store(i, d, sees ? v : z, sees ? mm : -INFINITY, sees ? l : 0.f, d == 0);
+    for (int w = 0; w < 4; w++) {
+      l += s_l[w][r] * __builtin_amdgcn_exp2f(s_m[w][r] - at);
+      v += *reinterpret_cast<const f4_t*>(rows + (w * 16 + r) * (HD + 4) + d);
     }
+    const f4_t z = {0.f, 0.f, 0.f, 0.f};
+    store(r, d, sees ? v : z, sees ? mm : -INFINITY, sees ? l : 0.f, d == 0);
   }
 }
 
@@ -825,12 +839,8 @@ template <int HD, typename X, typename KV>
 static int launch_paged(const PagedCall& c, const PagedPlan& p, const void* q, void* out, float* part_o, float2* part_ml,
                         hipStream_t s) {
   const unsigned blocks = unsigned(((p.pre_blocks + 255) / 256 + (p.own_blocks + 255) / 256) * 256);
-  if (HD < 256 && p.narrow_rows == 32)
-    hipLaunchKernelGGL((paged_attend_kernel<HD, X, KV, HD < 256 ? 2 : 1>), dim3(blocks), dim3(256), 0, s, c, p,
-                       static_cast<const X*>(q), static_cast<X*>(out), part_o, part_ml);
-  else
-    hipLaunchKernelGGL((paged_attend_kernel<HD, X, KV, 1>), dim3(blocks), dim3(256), 0, s, c, p, static_cast<const X*>(q),
-                       static_cast<X*>(out), part_o, part_ml);
+  hipLaunchKernelGGL((paged_attend_kernel<HD, X, KV>), dim3(blocks), dim3(256), 0, s, c, p, static_cast<const X*>(q),
+                     static_cast<X*>(out), part_o, part_ml);
   return check_launch("paged_attention");
 }
 

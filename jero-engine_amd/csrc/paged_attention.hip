@@ -88,10 +88,12 @@ static PagedPlan paged_plan(const jero_paged_cache* k, bool f16, int64_t n_token
   // 128 x 4096 69 and 192.
   const double pair = 2.0 * kv * k->head_dim * (k->kv_dtype == JERO_KV_F16 ? 2 : 4);  // bytes of a position
   const bool apart = k->n_seqs > 1 && each < p.wide_rows && double(k->n_seqs - 1) * shared * pair >= (k->kv_dtype == JERO_KV_F16 ? 48e6 : 24e6);
-  p.narrow_rows = hd < 256 && (each > 16 || (apart && rows > 16 && rows <= 32)) ? 32 : 16;
-  p.own_wide = each > p.narrow_rows;
+  // Rows a sequence from which its own positions go by wide tiles, not by 16 rows at a time: 16 sequences of up to 2000, 8 heads
+  // of 128, 32, 48, 64 and 96 rows each: f16 36, 41, 43 and 44 us wide, 37, 41, 46 and 65 by 16; f32 over f16 48, 56, 61 and
+  // 64, and 39, 42, 48 and 66; f32 68, 68, 85 and 85, and 74, 91, 98 and 132.
+  p.own_wide = each > (f16 ? 48 : k->kv_dtype == JERO_KV_F16 ? 95 : 31);
   p.own_lo = apart ? int(shared) : 0;
-  const int own_rows = p.own_wide ? p.wide_rows : p.narrow_rows;
+  const int own_rows = p.own_wide ? p.wide_rows : kNarrowRows;
   const int64_t tiles = k->starts_dev ? rows / own_rows + k->n_seqs : n_tokens * ((group + own_rows - 1) / own_rows);
   p.own_tiles = int(tiles);
   const int64_t span = std::max<int64_t>(k->max_len - p.own_lo, 1);
@@ -103,8 +105,9 @@ static PagedPlan paged_plan(const jero_paged_cache* k, bool f16, int64_t n_token
   p.own_chunks = int((span + p.own_len - 1) / p.own_len);
   p.own_blocks = int(tiles * kv * p.own_chunks);
   if (apart) {
+    // (8192 shared positions, 32, 64 and 128 rows: f16 31, 24 and 32 us wide, 21, 31 and 43 by 16)
     p.pre_wide = rows > 32;
-    const int pre_rows = p.pre_wide ? p.wide_rows : p.narrow_rows;
+    const int pre_rows = p.pre_wide ? p.wide_rows : kNarrowRows;
     p.pre_tiles = int((rows + pre_rows - 1) / pre_rows);
     // Chunks that take no longer than the call: with the cards' rates of a workgroup over the shared positions (us a position)
     // and of memory, four fifths of both phases' times one after the other.  64 f32 sequences, 8192 shared positions,
