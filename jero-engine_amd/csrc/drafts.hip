@@ -121,6 +121,32 @@ __device__ __forceinline__ double chunk_sum(const Drafts& d, const Verdict& v, c
   return s[0] + s[1] + s[2] + s[3];
 }
 
+// What is known of a sequence is written by one workgroup of it.
+__device__ __forceinline__ void write_verdict(const Drafts& d, const Verdict& v, int s, int tid, int threads) {
+  if (tid == 0) {
+    d.accepted[s] = v.accepted;
+    if (d.dropped) d.dropped[s] = max(v.rows - 1, 0) - v.accepted;
+  }
+  for (int i = tid; i < v.rows; i += threads)
+    if (i != v.accepted) d.out[v.first + i] = i < v.accepted ? d.tokens[v.first + i + 1] : -1;
+}
+
+// The sums of a sequence's chunks by the waves of one workgroup, a chunk each.
+__device__ __forceinline__ void wave_sums(const Drafts& d, const Verdict& v, const float* p, const float* q, double* sums,
+                                          int tid, int waves) {
+  for (int c = tid >> 6; c < d.chunks; c += waves) {
+    double sum = 0.0;
+    const int lo = c * kDraftChunk, hi = min(lo + kDraftChunk, d.vocab), lane = tid & 63;
+    if (hi - lo == kDraftChunk && ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q)) & 15u) == 0)
+      sum = sum_weights<kDraftChunk / 256>(v, p, q, lo + 4 * lane, 256, [](const float* x) { return *reinterpret_cast<const float4*>(x); });
+    else
+      for (int i = lo + lane; i < hi; i += kWave) sum += weight_of(v, p, q, i);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
+    if ((tid & 63) == 0) sums[c] = sum;
+  }
+}
+
 // Workgroup (chunk, sequence): the sum of its chunk's weights; the first chunk's writes what is known of the sequence.
 __global__ void __launch_bounds__(256) draft_sums_kernel(Drafts d) {
   __shared__ int s_n;
@@ -128,13 +154,8 @@ __global__ void __launch_bounds__(256) draft_sums_kernel(Drafts d) {
   const int s = blockIdx.y, tid = threadIdx.x;
   const Verdict v = verdict_of(d, s, &s_n);
   if (blockIdx.x == 0) {
-    if (tid == 0) {
-      d.verdicts[s] = v;
-      d.accepted[s] = v.accepted;
-      if (d.dropped) d.dropped[s] = max(v.rows - 1, 0) - v.accepted;
-    }
-    for (int i = tid; i < v.rows; i += 256)
-      if (i != v.accepted) d.out[v.first + i] = i < v.accepted ? d.tokens[v.first + i + 1] : -1;
+    if (tid == 0) d.verdicts[s] = v;
+    write_verdict(d, v, s, tid, 256);
   }
   if (v.row < 0) return;
   const double sum = chunk_sum(d, v, d.target + v.row * d.target_stride,
@@ -169,15 +190,27 @@ __device__ __forceinline__ void lowest_and_highest(int at, int last, int* s_at, 
   if (any && lane == 63 - __builtin_clzll(any)) atomicMax(s_last, last);
 }
 
-// Workgroup a sequence: finds the chunk, then the token in it.
+// Workgroup a sequence: finds the chunk, then the token in it.  WHOLE: the sums are its own work too.
 constexpr int kPickThreads = 1024, kPickChunks = (1 << 24) / kDraftChunk / kPickThreads;  // a thread, at most
+constexpr int kWholeChunks = 32;
+template <bool WHOLE>
 __global__ void __launch_bounds__(kPickThreads) draft_pick_kernel(Drafts d) {
-  __shared__ int s_at, s_last;
-  __shared__ double s_scan[16], s_before, s_total;
+  __shared__ int s_at, s_last, s_n;
+  __shared__ double s_scan[16], s_before, s_total, s_sums[WHOLE ? kWholeChunks : 1];
   const int s = blockIdx.x, tid = threadIdx.x;
-  double* const sums = d.sums + int64_t(s) * d.chunks;
-  Verdict v = d.verdicts[s];
+  double* const sums = WHOLE ? s_sums : d.sums + int64_t(s) * d.chunks;
   const float u = d.u_last[s];
+  Verdict v;
+  if constexpr (WHOLE) {
+    v = verdict_of(d, s, &s_n);
+    write_verdict(d, v, s, tid, kPickThreads);
+    if (v.row < 0) return;
+    wave_sums(d, v, d.target + v.row * d.target_stride, v.less >= 0 ? d.draft + v.less * d.draft_stride : nullptr, s_sums, tid,
+              kPickThreads / kWave);
+    __syncthreads();
+  } else {
+    v = d.verdicts[s];
+  }
   const int each = (d.chunks + kPickThreads - 1) / kPickThreads, c0 = tid * each;  // chunks of a thread
   double w[kPickChunks];
   auto read = [&]() {
@@ -197,14 +230,7 @@ __global__ void __launch_bounds__(kPickThreads) draft_pick_kernel(Drafts d) {
   if (!(s_total > 0.0) && (q || v.without >= 0)) {
     // the draft takes off all there is: the target's own sums
     q = nullptr, v.without = -1;
-    for (int c = tid >> 6; c < d.chunks; c += kPickThreads / kWave) {
-      double sum = 0.0;
-      for (int i = c * kDraftChunk + (tid & 63); i < min((c + 1) * kDraftChunk, d.vocab); i += kWave)
-        sum += weight_of(v, p, nullptr, i);
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
-      if ((tid & 63) == 0) sums[c] = sum;
-    }
+    wave_sums(d, v, p, nullptr, sums, tid, kPickThreads / kWave);
     __syncthreads();
     mine = read();
     run = scan1024(mine, s_scan, tid);
@@ -263,7 +289,8 @@ using namespace jero;
 
 extern "C" size_t jero_hip_verify_drafts_workspace_bytes(int64_t n_seqs, int64_t vocab) {
   if (n_seqs < 1 || n_seqs > 65535 || vocab < 1 || vocab > (1 << 24)) return 0;
-  return size_t(n_seqs) * (size_t((vocab + kDraftChunk - 1) / kDraftChunk) * sizeof(double) + sizeof(Verdict));
+  const size_t chunks = size_t((vocab + kDraftChunk - 1) / kDraftChunk);
+  return chunks <= kWholeChunks ? 0 : size_t(n_seqs) * (chunks * sizeof(double) + sizeof(Verdict));
 }
 
 extern "C" int jero_hip_verify_drafts(const float* target_dev, int64_t target_stride, const float* draft_dev,
@@ -286,8 +313,12 @@ extern "C" int jero_hip_verify_drafts(const float* target_dev, int64_t target_st
     return bad(JERO_ERR_TENSOR_BOUNDS, "more than 65535 sequences, 2^22 tokens or a vocabulary of 2^24");
   if (target_stride < vocab || (draft_dev && draft_stride < vocab))
     return bad(JERO_ERR_TENSOR_BOUNDS, "rows overlap: a stride is below the vocabulary");
+  // One launch, and no workspace, where a workgroup's reading of a whole row takes no longer than a second launch.
+  const int64_t chunks = (vocab + kDraftChunk - 1) / kDraftChunk;
+  const bool whole = chunks <= kWholeChunks;
   const size_t need = jero_hip_verify_drafts_workspace_bytes(n_seqs, vocab);
-  if (!workspace_dev) {
+  if (whole) {
+  } else if (!workspace_dev) {
     if (int rc = workspace(need, &workspace_dev)) return rc;
   } else if (workspace_bytes < need) {
     return bad(JERO_ERR_TENSOR_BOUNDS, "the workspace is too small");
@@ -299,14 +330,18 @@ extern "C" int jero_hip_verify_drafts(const float* target_dev, int64_t target_st
   d.tokens = tokens_dev, d.starts = starts_dev;
   d.target_stride = target_stride, d.draft_stride = draft_stride;
   d.n_seqs = int(n_seqs), d.n_tokens = int(n_tokens), d.n_drafts = int(n_drafts), d.vocab = int(vocab);
-  d.chunks = (d.vocab + kDraftChunk - 1) / kDraftChunk;
+  d.chunks = int(chunks);
   d.out = out_dev, d.accepted = accepted_dev, d.dropped = dropped_dev;
   d.sums = static_cast<double*>(workspace_dev);
   d.verdicts = reinterpret_cast<Verdict*>(d.sums + n_seqs * d.chunks);
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (whole) {
+    hipLaunchKernelGGL((draft_pick_kernel<true>), dim3(unsigned(n_seqs)), dim3(kPickThreads), 0, s, d);
+    return check_launch("verify_drafts");
+  }
   const dim3 grid = {unsigned(d.chunks), unsigned(n_seqs), 1};
   hipLaunchKernelGGL(draft_sums_kernel, grid, dim3(256), 0, s, d);
   if (int rc = check_launch("verify_drafts sums")) return rc;
-  hipLaunchKernelGGL(draft_pick_kernel, dim3(unsigned(n_seqs)), dim3(kPickThreads), 0, s, d);
+  hipLaunchKernelGGL((draft_pick_kernel<false>), dim3(unsigned(n_seqs)), dim3(kPickThreads), 0, s, d);
   return check_launch("verify_drafts");
 }

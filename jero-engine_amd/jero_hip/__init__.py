@@ -936,14 +936,17 @@ def verify_drafts(out, accepted, target, draft, tokens, starts, u, u_last, dropp
         _latent_check(draft.get_device() == device and draft.dtype is f32 and draft.shape == (N, V)
                       and (N == 0 or draft.stride(1) == 1), 14, what, "draft must be [drafts, vocab] float32 with packed rows")
     s = _paged_stream(P, device, stream)
-    ws, size, hold = _paged_workspace(P, workspace, L.jero_hip_verify_drafts_workspace_bytes(n, V), device, stream)
+    need = L.jero_hip_verify_drafts_workspace_bytes(n, V)
+    ws = size = hold = None
+    if need:
+        ws, size, hold = _paged_workspace(P, workspace, need, device, stream)
     check(L.jero_hip_verify_drafts(
         target.data_ptr(), target.stride(0) if T > 1 else V, None if draft is None or N == 0 else draft.data_ptr(),
         V if draft is None or N < 2 else draft.stride(0), ints(what, "tokens", tokens, device, i32, T),
         ints(what, "starts", starts, device, i32), ints(what, "u", u, device, f32, N) if N else None,
         ints(what, "u_last", u_last, device, f32, n), n, T, N, V, ints(what, "out", out, device, i32, T),
         ints(what, "accepted", accepted, device, i32, n),
-        None if dropped is None else ints(what, "dropped", dropped, device, i32, n), ws, size, s))
+        None if dropped is None else ints(what, "dropped", dropped, device, i32, n), ws, size or 0, s))
 
 
 def dispatch_qwen3_moe_ffn(out, norm_ffn_in, router_logits, top_k, gate, up, down, workspace=None, stream=None,

@@ -112,7 +112,7 @@ def test_bad_append():
         assert append(**kw) == 14, kw
 
 
-def verify(target=FAKE, ts=100, draft=FAKE, ds=100, tokens=FAKE, starts=FAKE, u=FAKE, ul=FAKE, n=2, T=6, N=4, V=100, out=FAKE,
+def verify(target=FAKE, ts=100000, draft=FAKE, ds=100000, tokens=FAKE, starts=FAKE, u=FAKE, ul=FAKE, n=2, T=6, N=4, V=100000, out=FAKE,
            acc=FAKE, dropped=None, ws=FAKE, size=1 << 20):
     return J.lib().jero_hip_verify_drafts(target, ts, draft, ds, tokens, starts, u, ul, n, T, N, V, out, acc, dropped, ws, size,
                                           None)
@@ -125,12 +125,12 @@ def test_bad_verify():
                dict(ws=FAKE + 8)):
         assert verify(**kw) == 21, kw
     for kw in (dict(n=0), dict(n=65536), dict(T=0), dict(T=(1 << 22) + 1), dict(N=-1), dict(N=6), dict(V=0),
-               dict(V=(1 << 24) + 1), dict(ts=99), dict(ds=99), dict(size=31)):
+               dict(V=(1 << 24) + 1), dict(ts=99999), dict(ds=99999), dict(size=31)):
         assert verify(**kw) == 14, kw
     size = J.lib().jero_hip_verify_drafts_workspace_bytes
     assert size(0, 100) == size(65536, 100) == size(2, 0) == size(2, (1 << 24) + 1) == 0
-    need = size(2, 100)
-    assert 0 < need < size(2, 4097) and verify(size=need - 1) == 14
+    need = size(2, 100000)
+    assert size(2, 100) == 0 < need < size(2, 200000) and verify(size=need - 1) == 14
 
 
 def cache(**kw):
