@@ -482,7 +482,8 @@ int jero_hip_paged_append(int act_dtype, const void *q_dev, int64_t q_stride, co
  * cache have f16's range (to 65504, below 2^-14 to 2^-25 absolute); queries any f32 range.  A numerator far below its row's
  * largest is off by up to 2^-36 of that.  What attends to a value that is not finite is not finite, which others do not see.
  * Workspace: jero_hip_paged_attention_workspace_bytes(...), 256-byte aligned (NULL: library-owned, calls must not
- * overlap on one device).  At most 2^19 tokens, 2^19 sequences, 1024 heads and n_tokens * n_heads 2^25. */
+ * overlap on one device).  At most 2^19 tokens, 2^19 sequences, 1024 heads, n_tokens * n_heads 2^25 and
+ * n_seqs * n_heads_kv 2^22. */
 typedef struct jero_paged_cache {
   const void *k_dev, *v_dev;  /* [n_blocks][block_size][n_heads_kv][head_dim] of kv_dtype, 16-byte aligned */
   const int32_t *table_dev;   /* [n_seqs][table_stride] block ids */

@@ -161,8 +161,9 @@ __device__ void extend_sums(const BlockPool& p, const ExtendSpace& to, int tid) 
 __device__ void extend_rows(const BlockPool& p, const Request* r, const int32_t* starts, const int32_t* back, const Stack& st,
                             int at, int step) {
   const int total = starts[p.n_seqs], mask = (1 << p.shift) - 1;
-  for (int i = at; i < p.n_tokens + st.back + st.taken; i += step) {
-    if (i < p.n_tokens) {
+  for (int64_t item = at; item < int64_t(p.n_tokens) + st.back + st.taken; item += step) {
+    if (item < p.n_tokens) {
+      const int i = int(item);
       int pos = -1;
       int64_t slot = -1;
       if (i < total) {
@@ -177,11 +178,11 @@ __device__ void extend_rows(const BlockPool& p, const Request* r, const int32_t*
       }
       p.positions[i] = pos;
       p.slots[i] = slot;
-    } else if (i < p.n_tokens + st.back) {
-      const int e = i - p.n_tokens;
-      if (st.before + e < p.capacity) p.free_ids[st.before + e] = returned_id(p, back, e);
+    } else if (item < int64_t(p.n_tokens) + st.back) {
+      const int e = int(item - p.n_tokens);
+      if (e < p.capacity - st.before) p.free_ids[st.before + e] = returned_id(p, back, e);
     } else {
-      const int k = i - p.n_tokens - st.back, s = last_not_above(&r[0].taken, p.n_seqs, sizeof(Request) / 4, k);
+      const int k = int(item - p.n_tokens - st.back), s = last_not_above(&r[0].taken, p.n_seqs, sizeof(Request) / 4, k);
       p.table[int64_t(s) * p.table_stride + r[s].owned + (k - r[s].taken)] = taken_id(p, back, st, k);
     }
   }
@@ -256,9 +257,8 @@ struct AppendArgs {
 // halves' layout 4 + 4 elements rot / 2 apart), or 8 behind it.  A lane keeps its pairs from row to row, so their
 // angles are found once.
 template <typename X, typename KV, int LP>
-__global__ void __launch_bounds__(256) append_kernel(const X* __restrict__ q, const X* __restrict__ k,
-                                                     const X* __restrict__ v, AppendArgs a, jero_rope rope,
-                                                     X* q_out, KV* __restrict__ k_rows,
+__global__ void __launch_bounds__(256) append_kernel(const X* q, const X* __restrict__ k, const X* __restrict__ v,
+                                                     AppendArgs a, jero_rope rope, X* q_out, KV* __restrict__ k_rows,
                                                      KV* __restrict__ v_rows) {
   const int64_t t = blockIdx.x;
   const int u = threadIdx.x % LP, sub = threadIdx.x / LP;

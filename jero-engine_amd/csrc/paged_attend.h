@@ -97,7 +97,7 @@ __device__ __forceinline__ bool paged_item(const PagedCall& c, const PagedPlan& 
     skip = int(tile - (int64_t(from) * c.group / rows + it.seq)) * rows;
   }
   const int mine = max(min(end, c.n_tokens) - from, 0) * c.group;
-  if (skip >= mine) return false;
+  if (skip < 0 || skip >= mine) return false;
   it.first = from * c.group + skip;
   it.count = min(rows, mine - skip);
   it.lo = p.own_lo + chunk * p.own_len;

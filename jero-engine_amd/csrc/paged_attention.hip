@@ -87,7 +87,8 @@ static PagedPlan paged_plan(const jero_paged_cache* k, bool f16, int64_t n_token
   // 1024 (29 MB) 24 and 19, 128 x 64 (33 MB) 60 and 55, 128 x 256 (133 MB) 59 and 61, 8 x 4096 (117 MB) 30 and 32,
   // 128 x 4096 69 and 192.
   const double pair = 2.0 * kv * k->head_dim * (k->kv_dtype == JERO_KV_F16 ? 2 : 4);  // bytes of a position
-  const bool apart = k->n_seqs > 1 && each < p.wide_rows && double(k->n_seqs - 1) * shared * pair >= (k->kv_dtype == JERO_KV_F16 ? 48e6 : 24e6);
+  // (Not where the two parts of all rows would take more than 4 GiB.)
+  const bool apart = k->n_seqs > 1 && each < p.wide_rows && n_tokens * n_heads * k->head_dim <= (int64_t(1) << 29) && double(k->n_seqs - 1) * shared * pair >= (k->kv_dtype == JERO_KV_F16 ? 48e6 : 24e6);
   // Rows a sequence from which its own positions go by wide tiles, not by 16 rows at a time: 16 sequences of up to 2000, 8 heads
   // of 128, 32, 48, 64 and 96 rows each: f16 36, 41, 43 and 44 us wide, 37, 41, 46 and 65 by 16; f32 over f16 48, 56, 61 and
   // 64, and 39, 42, 48 and 66; f32 68, 68, 85 and 85, and 74, 91, 98 and 132.
@@ -162,6 +163,8 @@ static int check_paged(const jero_paged_cache* c, int64_t n_tokens, int n_heads)
   if (c->shared_blocks < 0 || (c->shared_blocks > 0 && !c->shared_dev) || c->shared_blocks > c->table_stride)
     return bad(JERO_ERR_TENSOR_BOUNDS, "shared_blocks without their ids, or more than a table row");
   if (n_tokens * n_heads > (1 << 25)) return bad(JERO_ERR_CAPABILITY_MISMATCH, "more than 2^25 rows of heads");
+  if (c->n_seqs * c->n_heads_kv > (1 << 22))  // (each a workgroup, if only to see that it has no rows)
+    return bad(JERO_ERR_CAPABILITY_MISMATCH, "more than 2^22 sequences times key heads");
   return JERO_OK;
 }
 

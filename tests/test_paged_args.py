@@ -170,6 +170,9 @@ def test_bad_attention():
     for kw in (dict(heads=0), dict(heads=3), dict(tokens=0), dict(tokens=1 << 23), dict(qs=248), dict(os_=248)):
         assert attention(c, **kw) == 14, kw
     assert attention(c, heads=1026) == 10
+    many = cache(n_seqs=1 << 19, n_heads_kv=16, starts_dev=FAKE)
+    assert attention(many, tokens=4, heads=16, qs=1024, os_=1024) == 10
+    assert attention(cache(n_seqs=1 << 16, n_heads_kv=1), tokens=1 << 16, heads=1024, qs=65536, os_=65536) == 10
     # a call whose positions are cut wants room for its parts
     long = cache(table_stride=1 << 10, max_len=1 << 14)
     need = size(C.byref(long), J.F32, 2, 4)
