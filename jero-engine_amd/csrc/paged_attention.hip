@@ -20,7 +20,9 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedCall c, PagedPlan
   const int tid = threadIdx.x, d = 4 * (tid % DL), k0 = tid / DL % PL, r = tid / (DL * PL);
   const int64_t row = int64_t(blockIdx.x) * R + r;
   const int t = int(row / c.heads), h = int(row % c.heads);
-  const int seen = t < c.n_tokens ? paged_visible(c, t) : -1;
+  __shared__ int32_t s_starts[kSearchSeqs + 1];
+  const int32_t* const starts = paged_starts(c, s_starts, tid);
+  const int seen = t < c.n_tokens ? paged_visible(c, starts, t) : -1;
   const int shared = min(seen, c.shared_len);
   const int pre = p.pre_chunks && seen > 0 ? (shared + p.pre_len - 1) / p.pre_len : 0;
   const int own = seen > p.own_lo ? (seen - p.own_lo + p.own_len - 1) / p.own_len : 0;
@@ -33,11 +35,27 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedCall c, PagedPlan
   const float ref = m == -INFINITY ? 0.f : m;
   float l = 0.f;
   f4_t v = {0.f, 0.f, 0.f, 0.f};
-  for (int k = k0; k < pre + own; k += PL) {
-    const float2 ml = part_ml[at(k)];
-    const float e = __builtin_amdgcn_exp2f(ml.x - ref);
-    l += e * ml.y;
-    if (d < c.dim) v += e * *reinterpret_cast<const f4_t*>(part_o + at(k) * c.dim + d);
+  // (eight parts' loads at a time)
+  const int parts = pre + own;
+  for (int k1 = k0; k1 < parts; k1 += 8 * PL) {
+    float2 ml[8];
+    f4_t o[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int k = k1 + i * PL;
+      ml[i] = make_float2(-INFINITY, 0.f);
+      o[i] = f4_t{0.f, 0.f, 0.f, 0.f};
+      if (k < parts) {
+        ml[i] = part_ml[at(k)];
+        if (d < c.dim) o[i] = *reinterpret_cast<const f4_t*>(part_o + at(k) * c.dim + d);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float e = __builtin_amdgcn_exp2f(ml[i].x - ref);
+      l += e * ml[i].y;
+      v += e * o[i];
+    }
   }
   if constexpr (PL > 1) {
     s_v[r][k0][tid % DL] = v;
