@@ -78,15 +78,20 @@ static void launch_merge(const PagedCall& c, const PagedPlan& p, void* out, cons
 #define JERO_MERGE(DL, PL)                                                                                            \
   hipLaunchKernelGGL((paged_merge_kernel<X, DL, PL>), dim3(unsigned((rows * DL * PL + 255) / 256)), dim3(256), 0, s, c, p, \
                      static_cast<X*>(out), part_o, part_ml)
-  const bool few = p.parts <= 4;
+  // a row's lanes read eight parts at a time: more of them only where there are more parts (5 parts of 16384 rows of 128: 34 us
+  // by eight, 11 by one)
+  const int by = p.parts <= 8 ? 1 : p.parts <= 32 ? 2 : 8;
   if (c.dim <= 64) {
-    if (few) JERO_MERGE(16, 1);
+    if (by == 1) JERO_MERGE(16, 1);
+    else if (by == 2) JERO_MERGE(16, 2);
     else JERO_MERGE(16, 8);
   } else if (c.dim <= 128) {
-    if (few) JERO_MERGE(32, 1);
+    if (by == 1) JERO_MERGE(32, 1);
+    else if (by == 2) JERO_MERGE(32, 2);
     else JERO_MERGE(32, 8);
   } else {
-    if (few) JERO_MERGE(64, 1);
+    if (by == 1) JERO_MERGE(64, 1);
+    else if (by == 2) JERO_MERGE(64, 2);
     else JERO_MERGE(64, 4);
   }
 #undef JERO_MERGE
@@ -101,21 +106,29 @@ static PagedPlan paged_plan(const jero_paged_cache* k, bool f16, int64_t n_token
   const int64_t rows = n_tokens * group, each = (n_tokens + k->n_seqs - 1) / k->n_seqs * group;
   p.wide_rows = hd <= 128 && k->kv_dtype == JERO_KV_F16 ? 128 : 64;
   // Rows of all sequences go over the shared positions together where sequences do not fill tiles themselves and more than
-  // 48 MB (24 of f32, whose rows cost more than their bytes) are spared: 32 sequences x 256 shared positions x 8 heads of 128 (f16, 33 MB) 26 us and 30 apart and not, 8 x
-  // 1024 (29 MB) 24 and 19, 128 x 64 (33 MB) 60 and 55, 128 x 256 (133 MB) 59 and 61, 8 x 4096 (117 MB) 30 and 32,
-  // 128 x 4096 69 and 192.
+  // 48 MB (24 of f32, whose rows cost more than their bytes) are spared: 32 sequences x 256 shared positions x 8 heads of
+  // 128 (f16, 33 MB) 26 us and 30 apart and not, 8 x 1024 (29 MB) 24 and 19, 128 x 64 (33 MB) 60 and 55, 128 x 256
+  // (133 MB) 59 and 61, 8 x 4096 (117 MB) 30 and 32, 128 x 4096 69 and 192; f32: 16 x 256 (31 MB) the same, 16 x 1024
+  // 34 and 58.  Not where the two parts of all rows would take more than 4 GiB.
   const double pair = 2.0 * kv * k->head_dim * (k->kv_dtype == JERO_KV_F16 ? 2 : 4);  // bytes of a position
-  // (Not where the two parts of all rows would take more than 4 GiB.)
-  const bool apart = k->n_seqs > 1 && each < p.wide_rows && n_tokens * n_heads * k->head_dim <= (int64_t(1) << 29) && double(k->n_seqs - 1) * shared * pair >= (k->kv_dtype == JERO_KV_F16 ? 48e6 : 24e6);
+  const double spared = double(k->n_seqs - 1) * shared * pair;
+  const bool apart = k->n_seqs > 1 && each < p.wide_rows && spared >= (k->kv_dtype == JERO_KV_F16 ? 48e6 : 24e6) &&
+                     n_tokens * n_heads * k->head_dim <= (int64_t(1) << 29);
   // Rows a sequence from which its own positions go by wide tiles, not by 16 rows at a time: 16 sequences of up to 2000, 8 heads
   // of 128, 32, 48, 64 and 96 rows each: f16 36, 41, 43 and 44 us wide, 37, 41, 46 and 65 by 16; f32 over f16 48, 56, 61 and
-  // 64, and 39, 42, 48 and 66; f32 68, 68, 85 and 85, and 74, 91, 98 and 132.
-  p.own_wide = each > (f16 ? 48 : k->kv_dtype == JERO_KV_F16 ? 95 : 31);
+  // 64, and 39, 42, 48 and 66; f32 68, 68, 85 and 85, and 74, 91, 98 and 132.  Heads of 256, whose narrow tiles are one a CU,
+  // 24 and 48 rows: f32 over f16 43 and 50 wide, 49 and 59 by 16; heads of 64, 48 and 80: 28 and 31, and 16 and 22.
+  // Where wide tiles alone are two workgroups a CU they pay from 17 rows on (74 sequences, 8 heads of 80, 24, 40 and 80 rows
+  // over 128 positions behind 736 shared: f32 over f16 43, 60 and 83 us wide, 49, 71 and 123 by 16).
+  const bool many = k->n_seqs * kv >= 512;
+  p.own_wide = each > (many || hd == 256 ? kNarrowRows : hd == 64 ? 80 : f16 ? 48 : k->kv_dtype == JERO_KV_F16 ? 95 : 31);
   p.own_lo = apart ? int(shared) : 0;
   const int own_rows = p.own_wide ? p.wide_rows : kNarrowRows;
   const int64_t tiles = k->starts_dev ? rows / own_rows + k->n_seqs : n_tokens * ((group + own_rows - 1) / own_rows);
   p.own_tiles = int(tiles);
   const int64_t span = std::max<int64_t>(k->max_len - p.own_lo, 1);
+  // Own positions in chunks where 512 workgroups, two a CU, would not come out otherwise (64 sequences of up to 1500, 8 heads:
+  // one chunk 69 us, two 73; 32 of up to 800: one 20, four 27; one of 131072: 64 chunks 110, 128 119), of 256 and more.
   auto chunks = [&](int64_t blocks, int64_t span, int64_t want, int64_t least) {
     return std::max<int64_t>(1, std::min((want + blocks - 1) / blocks, (span + least - 1) / least));
   };
