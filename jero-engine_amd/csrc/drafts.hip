@@ -4,6 +4,12 @@
 
 namespace jero {
 
+// A drafted token stands where u q < p; the next is the first token whose running sum of weights passes u times their
+// total, weights max(p - q, 0) or p.  Two launches: the sums of 2048 weights a workgroup, then the search, by chunks and
+// within one; for small vocabularies one workgroup a sequence does both.  Only the row that a token is drawn from is read.
+// Bound by its bytes and, before them, three latencies (starts, tokens, probabilities): 64 chats of up to four drafts over
+// 151936 tokens, 78 MB: 18.3 + 6.3 us, 4.3 TB/s; one chat, 32000: 11.6 us.  Chunks of 1024, 4096 and 8192: 21, 17.5 and 22 us
+// and 7, 7 and 13.  64-bit sums of 32-bit values: no order of theirs moves a border by more than 2^-47 of the total.
 constexpr int kDraftChunk = 2048;  // of the vocabulary, a workgroup
 
 // Where a sequence's next token is drawn from.
@@ -138,7 +144,8 @@ __device__ __forceinline__ void wave_sums(const Drafts& d, const Verdict& v, con
     double sum = 0.0;
     const int lo = c * kDraftChunk, hi = min(lo + kDraftChunk, d.vocab), lane = tid & 63;
     if (hi - lo == kDraftChunk && ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q)) & 15u) == 0)
-      sum = sum_weights<kDraftChunk / 256>(v, p, q, lo + 4 * lane, 256, [](const float* x) { return *reinterpret_cast<const float4*>(x); });
+      sum = sum_weights<kDraftChunk / 256>(v, p, q, lo + 4 * lane, 256,
+                                           [](const float* x) { return *reinterpret_cast<const float4*>(x); });
     else
       for (int i = lo + lane; i < hi; i += kWave) sum += weight_of(v, p, q, i);
 #pragma unroll

@@ -87,6 +87,11 @@ __device__ __forceinline__ int taken_id(const BlockPool& p, const int32_t* back,
   return j < st.before ? p.free_ids[j] : returned_id(p, back, j - st.before);
 }
 
+// Three sums over the requests (tokens, blocks needed, blocks given back), then each token's place by a search in them.  The
+// bytes are few; what bounds it is latencies one after another: a request's counts, the sums, the search, the block's id.
+// 64 requests of one token: one launch, 6.2 us; 1500 requests, 302000 tokens, 5000 blocks: 9.6 and 10.9 us (64-bit sums in
+// three passes and searches in memory 22.6 and 11.7).
+
 // First part: the sums over the requests, by one workgroup, a request a thread and round.  All that is given back is
 // there before the first block is taken, so its sum comes first, from the requests of the first round as they are kept.
 __device__ void extend_sums(const BlockPool& p, const ExtendSpace& to, int tid) {
@@ -188,7 +193,7 @@ __device__ void extend_rows(const BlockPool& p, const Request* r, const int32_t*
   }
 }
 
-// One launch, its arrays in LDS, up to this many requests and tokens (64 requests of one token: 10 us in two launches).
+// One launch, its arrays in LDS, up to this many requests and tokens.
 constexpr int kExtendSeqs = 1024, kExtendTokens = 4096;
 // Requests whose starts and sums of blocks given back the second launch's workgroups copy to LDS: 11 steps of a search
 // there for 1500 requests, 11 times the memory's latency otherwise.
@@ -253,6 +258,9 @@ struct AppendArgs {
   int heads, kv_heads, dim;
 };
 
+// y_a = m (x_a cos - x_b sin), y_b = m (x_a sin + x_b cos) of a pair (a, b) at position * f.  Bound by the bytes: 12001 tokens
+// of 32 + 8 + 8 heads of 128, f16: 295 MB in 50.6 us, 5.8 TB/s; 64 tokens, f32 into f16, both norms: 4.6 us, of which most is
+// the chain positions, rows, stores.
 // Workgroup (token, run of its rows): LP lanes a row, 8 elements a lane: four pairs of the rotated part (with the
 // halves' layout 4 + 4 elements rot / 2 apart), or 8 behind it.  A lane keeps its pairs from row to row, so their
 // angles are found once.
