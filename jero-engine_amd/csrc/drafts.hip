@@ -8,7 +8,7 @@ namespace jero {
 // total, weights max(p - q, 0) or p.  Two launches: the sums of 2048 weights a workgroup, then the search, by chunks and
 // within one; for small vocabularies one workgroup a sequence does both.  Only the row that a token is drawn from is read.
 // Bound by its bytes and, before them, three latencies (starts, tokens, probabilities): 64 chats of up to four drafts over
-// 151936 tokens, 78 MB: 18.3 + 6.3 us, 4.3 TB/s; one chat, 32000: 11.6 us.  Chunks of 1024, 4096 and 8192: 21, 17.5 and 22 us
+// 151936 tokens, 78 MB: 17.7 + 6.2 us, 4.4 TB/s; one chat, 32000: 11.7 us.  Chunks of 1024, 4096 and 8192: 21, 17.5 and 22 us
 // and 7, 7 and 13.  64-bit sums of 32-bit values: no order of theirs moves a border by more than 2^-47 of the total.
 constexpr int kDraftChunk = 2048;  // of the vocabulary, a workgroup
 
@@ -37,12 +37,14 @@ __device__ __forceinline__ Verdict verdict_of(const Drafts& d, int s, int* s_n) 
   v.first = min(max(d.starts[s], 0), d.n_tokens);
   v.rows = min(max(d.starts[s + 1], v.first), d.n_tokens) - v.first;
   v.accepted = 0, v.row = v.less = v.without = -1;
-  // the drafted tokens of the sequences before
+  // The drafted tokens of the sequences before.  Each sum stops at all there are, behind which none is this sequence's:
+  // whatever the starts are, it does not wrap (16 waves of at most 2^22).
   if (tid == 0) *s_n = 0;
   __syncthreads();
   int n = 0;
-  for (int i = tid; i < s; i += blockDim.x) n += max(d.starts[i + 1] - d.starts[i] - 1, 0);
-  n = group_sum_i<64>(n);
+  auto start = [&](int i) { return min(max(d.starts[i], 0), d.n_tokens); };
+  for (int i = tid; i < s; i += blockDim.x) n = min(n + max(start(i + 1) - start(i) - 1, 0), d.n_drafts);
+  n = min(group_sum_i<64>(n), d.n_drafts);
   if (lane == 0 && n) atomicAdd(s_n, n);
   __syncthreads();
   const int before = *s_n;

@@ -356,6 +356,20 @@ def test_verify_borders(dev):
     check_verify(dev, d)
 
 
+@pytest.mark.parametrize("V", [50, 70000])
+def test_verify_starts_out_of_order(dev, V):
+    """Starts that fall and whose counts of drafts add up to 2^32 - 4: no number is read before the first, so the
+    sequence behind them has no drafts of its own, and stands on its last token alone."""
+    d = drafts(5, [4], V)
+    top = (1 << 31) - 1
+    starts = torch.tensor([0, top, 0, top, 0, 4], dtype=torch.int32, device=dev)
+    out, acc, dropped = (torch.full((n,), 9, dtype=torch.int32, device=dev) for n in (4, 5, 5))
+    J.verify_drafts(out, acc, put(dev, d["target"], torch.float32), put(dev, d["draft"], torch.float32), put(dev, d["tokens"]),
+                    starts, put(dev, d["u"], torch.float32), torch.full((5,), 0.5, device=dev), dropped=dropped)
+    torch.cuda.synchronize()
+    assert acc.tolist()[1::2] == [0, 0] and acc[4] == 0 and dropped.tolist()[1::2] == [0, 0] and dropped[4] == 3
+
+
 def test_verify_is_the_targets_distribution(dev):
     """What stands or is drawn for the first place is distributed as the target's row, whatever the draft: over 20000
     chats of one drafted token, each of 8 tokens' counts within 5 standard deviations."""
