@@ -458,8 +458,8 @@ int jero_hip_rope_init(jero_rope *rope, int rot_dim, int layout, double theta, i
  * k_norm (f32 [head_dim], or NULL): heads are first RMS-normalised (f32, eps) with these weights.  rope NULL: not
  * rotated.  q (n_heads 0) or keys and values (n_heads_kv 0) may be left out.  act_dtype JERO_F32 or JERO_F16, the pools'
  * kv_dtype any of both; sums and rotations are f32, each result is rounded once.  head_dim: a multiple of 8 up to 256,
- * at least rot_dim; strides multiples of 8 elements, pointers 16-byte aligned (positions 4, slots 8).  At most 2^24 tokens,
- * 1024 heads. */
+ * at least rot_dim; strides multiples of 8 elements, pointers 16-byte aligned (positions 4, slots 8).  At most 2^24 - 1
+ * tokens, 1024 heads. */
 int jero_hip_paged_append(int act_dtype, const void *q_dev, int64_t q_stride, const void *k_dev, int64_t k_stride,
                           const void *v_dev, int64_t v_stride, int64_t n_tokens, int n_heads, int n_heads_kv, int head_dim,
                           const int32_t *positions_dev, const int64_t *slots_dev, const jero_rope *rope,

@@ -513,7 +513,8 @@ extern "C" int jero_hip_paged_append(int act_dtype, const void* q_dev, int64_t q
   if (n_heads > 1024 || n_heads_kv > 1024) return bad(JERO_ERR_CAPABILITY_MISMATCH, "more than 1024 heads");
   if (head_dim < 8 || head_dim % 8 || head_dim > 256)
     return bad(JERO_ERR_CAPABILITY_MISMATCH, "head_dim is not a multiple of 8 up to 256");
-  if (n_tokens < 1 || n_tokens > (1 << 24)) return bad(JERO_ERR_TENSOR_BOUNDS, "tokens must be 1 to 2^24");
+  if (n_tokens < 1 || n_tokens >= (1 << 24))  // (256 threads each, and a launch has fewer than 2^32)
+    return bad(JERO_ERR_TENSOR_BOUNDS, "tokens must be 1 to 2^24 - 1");
   if (n_heads && (!q_dev || !q_out_dev)) return bad(JERO_ERR_INVALID_ARGUMENT, "null pointer");
   if (n_heads_kv && (!k_dev || !v_dev || !k_rows_dev || !v_rows_dev || !slots_dev))
     return bad(JERO_ERR_INVALID_ARGUMENT, "null pointer");

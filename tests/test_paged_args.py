@@ -112,6 +112,12 @@ def test_bad_append():
         assert append(**kw) == 14, kw
 
 
+def test_append_tokens_that_a_launch_holds():
+    """256 threads a token, and a launch has fewer than 2^32 threads."""
+    for tokens in (1 << 24, (1 << 24) + 1):
+        assert append(tokens=tokens) == 14
+
+
 def verify(target=FAKE, ts=100000, draft=FAKE, ds=100000, tokens=FAKE, starts=FAKE, u=FAKE, ul=FAKE, n=2, T=6, N=4, V=100000, out=FAKE,
            acc=FAKE, dropped=None, ws=FAKE, size=1 << 20):
     return J.lib().jero_hip_verify_drafts(target, ts, draft, ds, tokens, starts, u, ul, n, T, N, V, out, acc, dropped, ws, size,
