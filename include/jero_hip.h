@@ -452,8 +452,8 @@ typedef struct jero_rope {
 int jero_hip_rope_init(jero_rope *rope, int rot_dim, int layout, double theta, int scaling, double factor,
                        double original_len, double low, double high);
 
-/* Rotates n_tokens tokens' queries into q_out (q itself, or memory apart from it) and their keys into the key pool, and
- * stores their values: token row t, rows apart by the strides, [heads][head_dim] packed; positions[t] below 0: the token
+/* Rotates n_tokens tokens' queries into q_out (q itself, of its stride, or memory apart from it) and their keys into the
+ * key pool, and stores their values: token row t, rows apart by the strides, [heads][head_dim] packed; positions[t] below 0: the token
  * is left out; slots[t] outside [0, n_slots): its key and value are not stored.  No two tokens' slots may be the same.  q_norm /
  * k_norm (f32 [head_dim], or NULL): heads are first RMS-normalised (f32, eps) with these weights.  rope NULL: not
  * rotated.  q (n_heads 0) or keys and values (n_heads_kv 0) may be left out.  act_dtype JERO_F32 or JERO_F16, the pools'

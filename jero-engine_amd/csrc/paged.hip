@@ -530,6 +530,8 @@ extern "C" int jero_hip_paged_append(int act_dtype, const void* q_dev, int64_t q
     return bad(JERO_ERR_TENSOR_BOUNDS, "rows overlap: a stride is below its row's length");
   if ((n_heads && (q_stride % 8 || q_out_stride % 8)) || (n_heads_kv && (k_stride % 8 || v_stride % 8)))
     return bad(JERO_ERR_INVALID_ARGUMENT, "strides must be multiples of 8 elements");
+  if (n_heads && q_out_dev == q_dev && n_tokens > 1 && q_out_stride != q_stride)
+    return bad(JERO_ERR_INVALID_ARGUMENT, "queries rotated in place need one stride");
   if (n_heads_kv && n_slots < 1) return bad(JERO_ERR_TENSOR_BOUNDS, "no slots");
   if ((q_norm_dev || k_norm_dev) && !(eps >= 0.f && std::isfinite(eps)))
     return bad(JERO_ERR_INVALID_ARGUMENT, "eps must be finite and not negative");

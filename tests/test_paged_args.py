@@ -118,6 +118,13 @@ def test_append_tokens_that_a_launch_holds():
         assert append(tokens=tokens) == 14
 
 
+def test_append_in_place_at_another_stride():
+    """A token's results would fall on another's queries."""
+    for other in (dict(qos=512), dict(qs=512)):
+        assert append(qo=FAKE, q=FAKE, **other) == 21
+        assert "one stride" in J.lib().jero_hip_last_error().decode()
+
+
 def verify(target=FAKE, ts=100000, draft=FAKE, ds=100000, tokens=FAKE, starts=FAKE, u=FAKE, ul=FAKE, n=2, T=6, N=4, V=100000, out=FAKE,
            acc=FAKE, dropped=None, ws=FAKE, size=1 << 20):
     return J.lib().jero_hip_verify_drafts(target, ts, draft, ds, tokens, starts, u, ul, n, T, N, V, out, acc, dropped, ws, size,
