@@ -8,7 +8,7 @@ namespace jero {
 // total, weights max(p - q, 0) or p.  Two launches: the sums of 2048 weights a workgroup, then the search, by chunks and
 // within one; for small vocabularies one workgroup a sequence does both.  Only the row that a token is drawn from is read.
 // Bound by its bytes and, before them, three latencies (starts, tokens, probabilities): 64 chats of up to four drafts over
-// 151936 tokens, 78 MB: 17.7 + 6.2 us, 4.4 TB/s; one chat, 32000: 11.7 us.  Chunks of 1024, 4096 and 8192: 21, 17.5 and 22 us
+// 151936 tokens, 78 MB: 17.7 + 6.2 us, 4.4 TB/s; one chat, 32000: 11.5 us.  Chunks of 1024, 4096 and 8192: 21, 17.5 and 22 us
 // and 7, 7 and 13.  64-bit sums of 32-bit values: no order of theirs moves a border by more than 2^-47 of the total.
 constexpr int kDraftChunk = 2048;  // of the vocabulary, a workgroup
 

@@ -315,8 +315,8 @@ __device__ __forceinline__ void read_transposed(uint32_t at, int plane, int d, h
 // out = sum_j softmax_j(scale q . k_j) v_j in one pass with a running maximum and sum, for two kinds of tiles.
 //
 // F ("wide"): many rows over the same positions.  Four waves share KR positions in LDS, up to three steps of them on their
-// way, and hold 16 NJ rows each.  Bound by the products and the softmax between them: 2.04 GHz, products busy 42 % and other
-// vector instructions 40 % of the cycles.  Chunks of nine prompts, 5000 tokens behind 4096 shared positions, 32 heads of 128
+// way, and hold 16 NJ rows each.  Bound by the products and the softmax between them: products busy 43 % and other vector
+// instructions 40 % of the cycles.  Chunks of nine prompts, 6823 tokens behind 4096 shared positions, 32 heads of 128
 // over 4, f16: 626 to 680 us over cards, 840 to 910 TFLOP/s of what the mask leaves; f32 activations, two products for one,
 // 1080; over an f32 cache, three and the parts made in registers, 2260.  64 positions a step and two buffers: 32 and four
 // 14 % more; the softmax of one half under the products of the other, with its maxima taken twice, 8 % more; wave priorities
