@@ -656,7 +656,8 @@ __global__ void __launch_bounds__(256, (PagedShape<HD, X, KV>::kGroups))
       auto vread = [&](int d, auto& to) {
         read_transposed<HD, KR / 32, S::kPlanes>(at + S::kPlanes * S::kPlane + value0, S::kPlane, d, to);
       };
-      const bool masked = p0 + KR > low || ok != ~0ull || p0 + KR > it.hi;
+      // (bad: a wave whose rows all see the step has been given zeros for its values too)
+      const bool masked = bad || p0 + KR > low || ok != ~0ull || p0 + KR > it.hi;
       auto none = [] {};
       attend_step<HD, NJ, KR, TWOQ, TWOK, true>(st, kread, vread, none, none, p0, masked, ok, bad, g);
       if (!TWOK) buf = buf == S::kBufs - 1 ? 0 : buf + 1;
