@@ -403,7 +403,8 @@ int jero_hip_mla_prefill_attention(const jero_latent_cache *cache, int act_dtype
  * lens and owned become 0.  Blocks are then taken from the stack's top, in that order too.  A request
  * is granted what it needs if the needs of all requests up to it are no more than what is free, and
  * L + n positions fit its table row; another (granted 0) keeps L and its blocks, and its tokens'
- * positions and slots are -1.
+ * positions and slots are -1: nothing of them is to be dropped by a later call
+ * (jero_hip_verify_drafts_granted).
  *   starts[s]     sum of max(new, 0) before s, granted or not (n_seqs + 1 of them)
  *   positions[t]  L + t - starts[s] of token row t;  slots[t]: block * block_size + offset there, or -1
  *                 for a block id outside [0, n_blocks)
@@ -515,7 +516,9 @@ int jero_hip_paged_attention(const jero_paged_cache *cache, int act_dtype, const
  * a draw from none gives -1.  Products and sums are 64-bit.
  *   out[t]       rows of s: the drafted tokens that stand, the token drawn, then -1
  *   accepted[s]  drafted tokens that stand;  dropped[s] (or NULL): n less those, paged_extend's drop
- * A sequence without rows gets 0, 0.  Rows outside [starts[0], starts[n_seqs]) stay.  A drafted token outside
+ * A sequence without rows gets 0, 0.  _granted: paged_extend's granted (or NULL: all were); a sequence that
+ * was refused holds no position of its rows and their probabilities mean nothing, so its rows get -1 and it 0, 0:
+ * a 0 that paged_extend may take as its drop, and its tokens are asked for again.  Rows outside [starts[0], starts[n_seqs]) stay.  A drafted token outside
  * [0, vocab) is refused.  Workspace: jero_hip_verify_drafts_workspace_bytes(n_seqs, vocab), 16-byte aligned (NULL:
  * library-owned, calls must not overlap on one device).  At most 65535 sequences, 2^22 tokens, a vocabulary of 2^24. */
 size_t jero_hip_verify_drafts_workspace_bytes(int64_t n_seqs, int64_t vocab);
@@ -524,6 +527,12 @@ int jero_hip_verify_drafts(const float *target_dev, int64_t target_stride, const
                            const float *u_last_dev, int64_t n_seqs, int64_t n_tokens, int64_t n_drafts, int64_t vocab,
                            int32_t *out_dev, int32_t *accepted_dev, int32_t *dropped_dev, void *workspace_dev,
                            size_t workspace_bytes, void *stream);
+int jero_hip_verify_drafts_granted(const float *target_dev, int64_t target_stride, const float *draft_dev,
+                                   int64_t draft_stride, const int32_t *tokens_dev, const int32_t *starts_dev,
+                                   const int32_t *granted_dev, const float *u_dev, const float *u_last_dev, int64_t n_seqs,
+                                   int64_t n_tokens, int64_t n_drafts, int64_t vocab, int32_t *out_dev,
+                                   int32_t *accepted_dev, int32_t *dropped_dev, void *workspace_dev,
+                                   size_t workspace_bytes, void *stream);
 
 /* ---- routed experts ----
  * dispatch_qwen3_moe_ffn (src/qwen_deepseek.rs:847-951) from router logits, with

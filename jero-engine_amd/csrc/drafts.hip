@@ -14,7 +14,8 @@ constexpr int kDraftChunk = 2048;  // of the vocabulary, a workgroup
 
 // Where a sequence's next token is drawn from.
 struct Verdict {
-  int first, rows, accepted;
+  int first, rows;
+  int accepted;  // -1: the sequence was not granted its rows
   int row;       // of the target's probabilities; -1: no rows
   int less;      // the draft's row taken off, or -1
   int without;   // a token that gets no weight, or -1
@@ -22,7 +23,7 @@ struct Verdict {
 
 struct Drafts {
   const float *target, *draft, *u, *u_last;
-  const int32_t *tokens, *starts;
+  const int32_t *tokens, *starts, *granted;
   int64_t target_stride, draft_stride;
   int n_seqs, n_tokens, n_drafts, vocab, chunks;
   int32_t *out, *accepted, *dropped;
@@ -36,7 +37,7 @@ __device__ __forceinline__ Verdict verdict_of(const Drafts& d, int s, int* s_n) 
   Verdict v;
   v.first = min(max(d.starts[s], 0), d.n_tokens);
   v.rows = min(max(d.starts[s + 1], v.first), d.n_tokens) - v.first;
-  v.accepted = 0, v.row = v.less = v.without = -1;
+  v.accepted = d.granted && !d.granted[s] ? -1 : 0, v.row = v.less = v.without = -1;
   // The drafted tokens of the sequences before.  Each sum stops at all there are, behind which none is this sequence's:
   // whatever the starts are, it does not wrap (16 waves of at most 2^22).
   if (tid == 0) *s_n = 0;
@@ -48,7 +49,7 @@ __device__ __forceinline__ Verdict verdict_of(const Drafts& d, int s, int* s_n) 
   if (lane == 0 && n) atomicAdd(s_n, n);
   __syncthreads();
   const int before = *s_n;
-  if (v.rows < 1) return v;
+  if (v.rows < 1 || v.accepted < 0) return v;
   const int drafted = max(min(v.rows - 1, d.n_drafts - before), 0);
   int at = drafted;  // the first that is refused
   for (int j0 = 0; j0 < drafted && at == drafted; j0 += kWave) {
@@ -129,11 +130,12 @@ __device__ __forceinline__ double chunk_sum(const Drafts& d, const Verdict& v, c
   return s[0] + s[1] + s[2] + s[3];
 }
 
-// What is known of a sequence is written by one workgroup of it.
+// What is known of a sequence is written by one workgroup of it.  One that was not granted its rows holds none of their
+// positions, so that none is to be taken back.
 __device__ __forceinline__ void write_verdict(const Drafts& d, const Verdict& v, int s, int tid, int threads) {
   if (tid == 0) {
-    d.accepted[s] = v.accepted;
-    if (d.dropped) d.dropped[s] = max(v.rows - 1, 0) - v.accepted;
+    d.accepted[s] = max(v.accepted, 0);
+    if (d.dropped) d.dropped[s] = v.accepted < 0 ? 0 : max(v.rows - 1, 0) - v.accepted;
   }
   for (int i = tid; i < v.rows; i += threads)
     if (i != v.accepted) d.out[v.first + i] = i < v.accepted ? d.tokens[v.first + i + 1] : -1;
@@ -302,19 +304,20 @@ extern "C" size_t jero_hip_verify_drafts_workspace_bytes(int64_t n_seqs, int64_t
   return chunks <= kWholeChunks ? 0 : size_t(n_seqs) * (chunks * sizeof(double) + sizeof(Verdict));
 }
 
-extern "C" int jero_hip_verify_drafts(const float* target_dev, int64_t target_stride, const float* draft_dev,
-                                      int64_t draft_stride, const int32_t* tokens_dev, const int32_t* starts_dev,
-                                      const float* u_dev, const float* u_last_dev, int64_t n_seqs, int64_t n_tokens,
-                                      int64_t n_drafts, int64_t vocab, int32_t* out_dev, int32_t* accepted_dev,
-                                      int32_t* dropped_dev, void* workspace_dev, size_t workspace_bytes, void* stream) {
+extern "C" int jero_hip_verify_drafts_granted(const float* target_dev, int64_t target_stride, const float* draft_dev,
+                                              int64_t draft_stride, const int32_t* tokens_dev, const int32_t* starts_dev,
+                                              const int32_t* granted_dev, const float* u_dev, const float* u_last_dev,
+                                              int64_t n_seqs, int64_t n_tokens, int64_t n_drafts, int64_t vocab,
+                                              int32_t* out_dev, int32_t* accepted_dev, int32_t* dropped_dev,
+                                              void* workspace_dev, size_t workspace_bytes, void* stream) {
   auto bad = [](int status, const char* what) { return fail(status, std::string("verify_drafts: ") + what); };
   if (!target_dev || !tokens_dev || !starts_dev || !u_last_dev || !out_dev || !accepted_dev || (n_drafts > 0 && !u_dev))
     return bad(JERO_ERR_INVALID_ARGUMENT, "null pointer");
   for (const void* p : {static_cast<const void*>(target_dev), static_cast<const void*>(draft_dev),
                         static_cast<const void*>(tokens_dev), static_cast<const void*>(starts_dev),
-                        static_cast<const void*>(u_dev), static_cast<const void*>(u_last_dev),
-                        static_cast<const void*>(out_dev), static_cast<const void*>(accepted_dev),
-                        static_cast<const void*>(dropped_dev)})
+                        static_cast<const void*>(granted_dev), static_cast<const void*>(u_dev),
+                        static_cast<const void*>(u_last_dev), static_cast<const void*>(out_dev),
+                        static_cast<const void*>(accepted_dev), static_cast<const void*>(dropped_dev)})
     if (!aligned4(p)) return bad(JERO_ERR_INVALID_ARGUMENT, "arrays must be 4-byte aligned");
   if (n_seqs < 1 || n_tokens < 1 || vocab < 1 || n_drafts < 0 || n_drafts >= n_tokens)
     return bad(JERO_ERR_TENSOR_BOUNDS, "no sequences, tokens or vocabulary, or as many drafts as tokens");
@@ -336,7 +339,7 @@ extern "C" int jero_hip_verify_drafts(const float* target_dev, int64_t target_st
   }
   Drafts d{};
   d.target = target_dev, d.draft = draft_dev, d.u = u_dev, d.u_last = u_last_dev;
-  d.tokens = tokens_dev, d.starts = starts_dev;
+  d.tokens = tokens_dev, d.starts = starts_dev, d.granted = granted_dev;
   d.target_stride = target_stride, d.draft_stride = draft_stride;
   d.n_seqs = int(n_seqs), d.n_tokens = int(n_tokens), d.n_drafts = int(n_drafts), d.vocab = int(vocab);
   d.chunks = int(chunks);
@@ -353,4 +356,14 @@ extern "C" int jero_hip_verify_drafts(const float* target_dev, int64_t target_st
   if (int rc = check_launch("verify_drafts sums")) return rc;
   hipLaunchKernelGGL((draft_pick_kernel<false>), dim3(unsigned(n_seqs)), dim3(kPickThreads), 0, s, d);
   return check_launch("verify_drafts");
+}
+
+extern "C" int jero_hip_verify_drafts(const float* target_dev, int64_t target_stride, const float* draft_dev,
+                                      int64_t draft_stride, const int32_t* tokens_dev, const int32_t* starts_dev,
+                                      const float* u_dev, const float* u_last_dev, int64_t n_seqs, int64_t n_tokens,
+                                      int64_t n_drafts, int64_t vocab, int32_t* out_dev, int32_t* accepted_dev,
+                                      int32_t* dropped_dev, void* workspace_dev, size_t workspace_bytes, void* stream) {
+  return jero_hip_verify_drafts_granted(target_dev, target_stride, draft_dev, draft_stride, tokens_dev, starts_dev, nullptr,
+                                        u_dev, u_last_dev, n_seqs, n_tokens, n_drafts, vocab, out_dev, accepted_dev,
+                                        dropped_dev, workspace_dev, workspace_bytes, stream);
 }

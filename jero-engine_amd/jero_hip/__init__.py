@@ -92,6 +92,8 @@ _SIGS = {
     "jero_hip_verify_drafts_workspace_bytes": (_SZ, [_I64, _I64]),
     "jero_hip_verify_drafts": (_I32, [_P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _SZ,
                                       _P]),
+    "jero_hip_verify_drafts_granted": (_I32, [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P,
+                                              _P, _SZ, _P]),
     "jero_hip_moe_ffn": (_I32, [_P, _P, _I64, _I64, _I32, _I32, _P, _SZ, _I32, _P, _SZ, _I32, _P, _SZ, _I64, _I64,
                                 _P, _P, _P, _P, _SZ, _P]),
     "jero_hip_moe_workspace_bytes": (_SZ, [_I64, _I64, _I32, _I64, _I64]),
@@ -919,13 +921,15 @@ def paged_attention(out, q, cache, scale, workspace=None, stream=None):
     return out
 
 
-def verify_drafts(out, accepted, target, draft, tokens, starts, u, u_last, dropped=None, workspace=None, stream=None):
+def verify_drafts(out, accepted, target, draft, tokens, starts, u, u_last, dropped=None, workspace=None, stream=None,
+                  granted=None):
     """Which drafted tokens stand, and the token that follows (jero_hip_verify_drafts): ``tokens`` [tokens] int32, a
     sequence's last token and its drafted ones in rows starts[s] .. starts[s + 1] - 1 (``starts`` [n_seqs + 1]
     int32); ``target`` [tokens, vocab] f32 probabilities after each row, ``draft`` [drafts, vocab] f32 the draft's of
     each drafted token, sequence after sequence (None: it was sure of each); ``u`` [drafts] and ``u_last``
     [n_seqs] f32 numbers from [0, 1).  Writes ``out`` [tokens] int32, the tokens that stand, the one drawn, -1s;
-    ``accepted`` and ``dropped`` (or None) [n_seqs] int32."""
+    ``accepted`` and ``dropped`` (or None) [n_seqs] int32.  ``granted`` [n_seqs] int32, as paged_extend wrote it (None: all
+    were): a sequence that was refused gets 0, 0 and rows of -1 (jero_hip_verify_drafts_granted)."""
     P = _paged_state()
     what, device, i32, f32, ints, L = "verify_drafts", target.get_device(), P.i32, P.f32, _paged_ints, P.lib
     n, T = starts.numel() - 1, tokens.numel()
@@ -940,10 +944,11 @@ def verify_drafts(out, accepted, target, draft, tokens, starts, u, u_last, dropp
     ws = size = hold = None
     if need:
         ws, size, hold = _paged_workspace(P, workspace, need, device, stream)
-    check(L.jero_hip_verify_drafts(
+    check(L.jero_hip_verify_drafts_granted(
         target.data_ptr(), target.stride(0) if T > 1 else V, None if draft is None or N == 0 else draft.data_ptr(),
         V if draft is None or N < 2 else draft.stride(0), ints(what, "tokens", tokens, device, i32, T),
-        ints(what, "starts", starts, device, i32), ints(what, "u", u, device, f32, N) if N else None,
+        ints(what, "starts", starts, device, i32), None if granted is None else ints(what, "granted", granted, device, i32, n),
+        ints(what, "u", u, device, f32, N) if N else None,
         ints(what, "u_last", u_last, device, f32, n), n, T, N, V, ints(what, "out", out, device, i32, T),
         ints(what, "accepted", accepted, device, i32, n),
         None if dropped is None else ints(what, "dropped", dropped, device, i32, n), ws, size or 0, s))
