@@ -516,10 +516,11 @@ int jero_hip_paged_attention(const jero_paged_cache *cache, int act_dtype, const
  * a draw from none gives -1.  Products and sums are 64-bit.
  *   out[t]       rows of s: the drafted tokens that stand, the token drawn, then -1
  *   accepted[s]  drafted tokens that stand;  dropped[s] (or NULL): n less those, paged_extend's drop
- * A sequence without rows gets 0, 0.  _granted: paged_extend's granted (or NULL: all were); a sequence that
- * was refused holds no position of its rows and their probabilities mean nothing, so its rows get -1 and it 0, 0:
- * a 0 that paged_extend may take as its drop, and its tokens are asked for again.  Rows outside [starts[0], starts[n_seqs]) stay.  A drafted token outside
- * [0, vocab) is refused.  Workspace: jero_hip_verify_drafts_workspace_bytes(n_seqs, vocab), 16-byte aligned (NULL:
+ * A sequence without rows gets 0, 0.  _granted: paged_extend's granted (or NULL: all were); a sequence that was
+ * refused holds no position of its rows and their probabilities mean nothing, so its rows get -1 and it 0, 0: a 0
+ * that paged_extend may take as its drop, and its tokens are asked for again.  Rows outside [starts[0],
+ * starts[n_seqs]) stay.  A drafted token outside [0, vocab) does not stand.  The outputs lie apart from the inputs: out
+ * is not tokens.  Workspace: jero_hip_verify_drafts_workspace_bytes(n_seqs, vocab), 16-byte aligned (NULL:
  * library-owned, calls must not overlap on one device).  At most 65535 sequences, 2^22 tokens, a vocabulary of 2^24. */
 size_t jero_hip_verify_drafts_workspace_bytes(int64_t n_seqs, int64_t vocab);
 int jero_hip_verify_drafts(const float *target_dev, int64_t target_stride, const float *draft_dev, int64_t draft_stride,

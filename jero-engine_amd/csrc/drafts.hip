@@ -329,14 +329,27 @@ extern "C" int jero_hip_verify_drafts_granted(const float* target_dev, int64_t t
   const int64_t chunks = (vocab + kDraftChunk - 1) / kDraftChunk;
   const bool whole = chunks <= kWholeChunks;
   const size_t need = jero_hip_verify_drafts_workspace_bytes(n_seqs, vocab);
-  if (whole) {
-  } else if (!workspace_dev) {
-    if (int rc = workspace(need, &workspace_dev)) return rc;
-  } else if (workspace_bytes < need) {
-    return bad(JERO_ERR_TENSOR_BOUNDS, "the workspace is too small");
-  } else if (reinterpret_cast<uintptr_t>(workspace_dev) & 15u) {
-    return bad(JERO_ERR_INVALID_ARGUMENT, "the workspace must be 16-byte aligned");
+  if (!whole && workspace_dev) {
+    if (workspace_bytes < need) return bad(JERO_ERR_TENSOR_BOUNDS, "the workspace is too small");
+    if (reinterpret_cast<uintptr_t>(workspace_dev) & 15u)
+      return bad(JERO_ERR_INVALID_ARGUMENT, "the workspace must be 16-byte aligned");
   }
+  // A sequence's inputs are read by several workgroups and waves, with no order between them and what one of them writes.
+  struct Array {
+    const void* p;
+    int64_t n;
+  };
+  const Array ins[] = {{tokens_dev, n_tokens}, {starts_dev, n_seqs + 1}, {granted_dev, n_seqs}, {u_dev, n_drafts},
+                       {u_last_dev, n_seqs}},
+              outs[] = {{out_dev, n_tokens}, {accepted_dev, n_seqs}, {dropped_dev, n_seqs}};
+  for (const Array& o : outs)
+    for (const Array& i : ins) {
+      const uintptr_t a = reinterpret_cast<uintptr_t>(o.p), b = reinterpret_cast<uintptr_t>(i.p);
+      if (a && b && a < b + 4 * uintptr_t(i.n) && b < a + 4 * uintptr_t(o.n))
+        return bad(JERO_ERR_INVALID_ARGUMENT, "an output overlaps an input");
+    }
+  if (!whole && !workspace_dev)
+    if (int rc = workspace(need, &workspace_dev)) return rc;
   Drafts d{};
   d.target = target_dev, d.draft = draft_dev, d.u = u_dev, d.u_last = u_last_dev;
   d.tokens = tokens_dev, d.starts = starts_dev, d.granted = granted_dev;

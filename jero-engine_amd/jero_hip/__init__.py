@@ -927,7 +927,7 @@ def verify_drafts(out, accepted, target, draft, tokens, starts, u, u_last, dropp
     sequence's last token and its drafted ones in rows starts[s] .. starts[s + 1] - 1 (``starts`` [n_seqs + 1]
     int32); ``target`` [tokens, vocab] f32 probabilities after each row, ``draft`` [drafts, vocab] f32 the draft's of
     each drafted token, sequence after sequence (None: it was sure of each); ``u`` [drafts] and ``u_last``
-    [n_seqs] f32 numbers from [0, 1).  Writes ``out`` [tokens] int32, the tokens that stand, the one drawn, -1s;
+    [n_seqs] f32 numbers from [0, 1).  Writes ``out`` [tokens] int32 (not ``tokens`` itself), the tokens that stand, the one drawn, -1s;
     ``accepted`` and ``dropped`` (or None) [n_seqs] int32.  ``granted`` [n_seqs] int32, as paged_extend wrote it (None: all
     were): a sequence that was refused gets 0, 0 and rows of -1 (jero_hip_verify_drafts_granted)."""
     P = _paged_state()

@@ -16,3 +16,17 @@ def test_granted():
         assert verify(granted=granted) == 14
         assert "workspace" in J.lib().jero_hip_last_error().decode()
     assert verify(out=None) == 21 and verify(n=0) == 14
+
+
+def test_outputs_apart_from_inputs():
+    """The last refusal: in place, or overlapping by an element, in both forms."""
+    need = J.lib().jero_hip_verify_drafts_workspace_bytes(2, 100000)
+    a = dict(target=FAKE, draft=FAKE, tokens=0x20000, starts=0x21000, granted=0x22000, u=0x23000, ul=0x24000, out=0x25000,
+             acc=0x26000, dropped=0x27000, size=need)
+    lengths = dict(tokens=6, starts=3, granted=2, u=4, ul=2)
+    for V in (100, 100000):
+        for o, n in (("out", 6), ("acc", 2), ("dropped", 2)):
+            for i, m in lengths.items():
+                for at in (a[i], a[i] + 4 * (m - 1), a[i] - 4 * (n - 1)):
+                    assert verify(**dict(a, V=V, **{o: at})) == 21, (o, i, at)
+                    assert "overlaps" in J.lib().jero_hip_last_error().decode()
