@@ -405,7 +405,7 @@ int jero_hip_mla_prefill_attention(const jero_latent_cache *cache, int act_dtype
  * L + n positions fit its table row; another (granted 0) keeps L and its blocks, and its tokens'
  * positions and slots are -1: nothing of them is to be dropped by a later call
  * (jero_hip_verify_drafts_granted).
- *   starts[s]     sum of max(new, 0) before s, granted or not (n_seqs + 1 of them)
+ *   starts[s]     sum of max(new, 0) before s, granted or not (n_seqs + 1 of them), at most 2^31 - 1
  *   positions[t]  L + t - starts[s] of token row t;  slots[t]: block * block_size + offset there, or -1
  *                 for a block id outside [0, n_blocks)
  *   rows from starts[n_seqs] on: -1, -1.  Rows from n_tokens on are not written.

@@ -34,12 +34,12 @@ struct ExtendSpace {
 };
 
 constexpr int kExtendThreads = 1024, kExtendWaves = kExtendThreads / kWave;
-constexpr int kExtendMost = 1 << 24;  // tokens of a request that are counted: a call has no more
 
-__device__ __forceinline__ int wave_scan(int v, int lane) {
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v, int lane) {
 #pragma unroll
   for (int off = 1; off < kWave; off <<= 1) {
-    const int o = __shfl_up(v, off, kWave);
+    const T o = __shfl_up(v, off, kWave);
     if (lane >= off) v += o;
   }
   return v;
@@ -95,8 +95,8 @@ __device__ __forceinline__ int taken_id(const BlockPool& p, const int32_t* back,
 // First part: the sums over the requests, by one workgroup, a request a thread and round.  All that is given back is
 // there before the first block is taken, so its sum comes first, from the requests of the first round as they are kept.
 __device__ void extend_sums(const BlockPool& p, const ExtendSpace& to, int tid) {
-  __shared__ int s_sum[2][3][kExtendWaves], s_got;
-  __shared__ int64_t s_back[kExtendWaves];
+  __shared__ int s_got;
+  __shared__ int64_t s_sum[2][3][kExtendWaves], s_back[kExtendWaves];
   const int lane = tid & 63, wv = tid >> 6;
   Held h = {};
   if (tid < p.n_seqs) h = held_by(p, tid);
@@ -116,13 +116,11 @@ __device__ void extend_sums(const BlockPool& p, const ExtendSpace& to, int tid) 
       h = Held{};
       if (on) h = held_by(p, s);
     }
-    const int mine[3] = {min(h.tokens, kExtendMost), h.need, h.back};
-    int w[3];
+    // (tokens in 64 bits: a request may ask for any number; the table's entries, so its blocks, are below 2^31 in all)
+    const int64_t w[3] = {wave_scan(int64_t(h.tokens), lane), wave_scan(h.need, lane), wave_scan(h.back, lane)};
 #pragma unroll
-    for (int i = 0; i < 3; i++) {
-      w[i] = wave_scan(mine[i], lane);
+    for (int i = 0; i < 3; i++)
       if (lane == 63) s_sum[round][i][wv] = w[i];
-    }
     __syncthreads();
     if (s0 == 0) {
       int64_t all = before;
@@ -143,7 +141,7 @@ __device__ void extend_sums(const BlockPool& p, const ExtendSpace& to, int tid) 
     }
     const bool granted = h.fits && (h.need == 0 || sum[1] <= top);
     if (on) {
-      p.starts[s] = int(min(sum[0] - mine[0], int64_t(INT32_MAX)));
+      p.starts[s] = int(min(sum[0] - h.tokens, int64_t(INT32_MAX)));
       to.r[s] = Request{granted ? h.len : -1, h.owned, int(sum[1] - h.need)};
       to.back[s] = int(sum[2] - h.back);
       p.lens_out[s] = h.ends ? 0 : granted ? h.len + h.tokens : h.len;
