@@ -820,7 +820,8 @@ def paged_append(k_rows, v_rows, q_out, q, k, v, positions, slots, rope, q_norm=
     [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim] f32 or f16 (tokens may be apart) into q_out
     (q itself, or apart from it) and the pools k_rows, v_rows [..., kv_heads, head_dim] f32 or f16, whose rows
     ``slots`` [tokens] int64 counts; ``positions`` [tokens] int32.  A token of a position below 0 is left out, one
-    of a slot that is none is not stored.  ``q_norm``, ``k_norm`` [head_dim] f32: heads are RMS-normalised first."""
+    of a slot that is none is not stored.  ``q_norm``, ``k_norm`` [head_dim] f32: heads are RMS-normalised first.  q, or k
+    and v with their pools, may have no heads."""
     P = _paged_state()
     what, device, dtype, rows, ints = "paged_append", k.get_device(), k.dtype, _paged_rows, _paged_ints
     act = _paged_act(P, what, k)
@@ -841,7 +842,7 @@ def paged_append(k_rows, v_rows, q_out, q, k, v, positions, slots, rope, q_norm=
         ints(what, "positions", positions, device, P.i32, T), ints(what, "slots", slots, device, P.i64, T),
         None if rope is None else rope.ref, None if q_norm is None else ints(what, "q_norm", q_norm, device, P.f32, D),
         None if k_norm is None else ints(what, "k_norm", k_norm, device, P.f32, D), eps, q_out.data_ptr(), qo,
-        k_rows.data_ptr(), v_rows.data_ptr(), KV_F16 if kd is P.f16 else KV_F32, k_rows.numel() // (KV * D),
+        k_rows.data_ptr(), v_rows.data_ptr(), KV_F16 if kd is P.f16 else KV_F32, k_rows.numel() // max(KV * D, 1),
         _paged_stream(P, device, stream)))
 
 
