@@ -25,7 +25,7 @@ struct Drafts {
   const float *target, *draft, *u, *u_last;
   const int32_t *tokens, *starts, *granted;
   int64_t target_stride, draft_stride;
-  int n_seqs, n_tokens, n_drafts, vocab, chunks;
+  int n_tokens, n_drafts, vocab, chunks;
   int32_t *out, *accepted, *dropped;
   double* sums;       // [n_seqs][chunks]: of the weights
   Verdict* verdicts;  // [n_seqs]
@@ -354,7 +354,7 @@ extern "C" int jero_hip_verify_drafts_granted(const float* target_dev, int64_t t
   d.target = target_dev, d.draft = draft_dev, d.u = u_dev, d.u_last = u_last_dev;
   d.tokens = tokens_dev, d.starts = starts_dev, d.granted = granted_dev;
   d.target_stride = target_stride, d.draft_stride = draft_stride;
-  d.n_seqs = int(n_seqs), d.n_tokens = int(n_tokens), d.n_drafts = int(n_drafts), d.vocab = int(vocab);
+  d.n_tokens = int(n_tokens), d.n_drafts = int(n_drafts), d.vocab = int(vocab);
   d.chunks = int(chunks);
   d.out = out_dev, d.accepted = accepted_dev, d.dropped = dropped_dev;
   d.sums = static_cast<double*>(workspace_dev);
