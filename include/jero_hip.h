@@ -481,7 +481,9 @@ int jero_hip_paged_append(int act_dtype, const void *q_dev, int64_t q_stride, co
  * strides multiples of 8 elements, 16-byte aligned.  Sums are f32; with f32 activations the products carry 22 bits of each
  * f32 factor (two f16 parts), with f16 activations softmax numerators are rounded to f16.  So keys and values of an f32
  * cache have f16's range (to 65504, below 2^-14 to 2^-25 absolute); queries any f32 range.  A numerator far below its row's
- * largest is off by up to 2^-36 of that.  What attends to a value that is not finite is not finite, which others do not see.
+ * largest is off by up to 2^-36 of that.  A token that attends to a value that is not finite gets nothing finite in that
+ * value's column, and maybe in its head's others; one that attends to a key that is not finite nothing in its whole head,
+ * unless the score is minus infinity, which may leave the key out.  Tokens that do not attend to it do not see it.
  * Workspace: jero_hip_paged_attention_workspace_bytes(...), 256-byte aligned (NULL: library-owned, calls must not
  * overlap on one device).  At most 2^19 tokens, 2^19 sequences, 1024 heads, n_tokens * n_heads 2^25 and
  * n_seqs * n_heads_kv 2^22. */

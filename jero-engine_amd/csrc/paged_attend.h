@@ -327,8 +327,14 @@ __device__ __forceinline__ void read_transposed(uint32_t at, int plane, int d, h
 // 64 sequences of 6144 positions, 8 heads of 128, f16: 285 us, 5.65 TB/s; of 1536 79 us, 5.1 TB/s; one of 131072 110 us, 4.9.
 // 32 rows a tile: registers spill, 16 sequences of 5 to 8 tokens and 4 heads 47 us against 36.
 //
-// Both are one launch: a CU gets a workgroup of each, one that computes and one that reads (64 chats of 30 to 1500 positions
-// behind 8192: shared positions alone 31 us, own alone 49, together 54).
+// Both are one launch, 256 workgroups of each by turns: where the shared positions make no more than 256, a CU gets one that
+// computes and one that reads (64 f32 chats of 30 to 1500 positions behind 8192: shared positions alone 45 us, own alone 47,
+// the call 61).  More of them fill both places of a CU, and most own positions come after (256 f16 chats of 10 to 700
+// behind 32768, 512 workgroups: 297 and 100, the call 362).
+//
+// f16 activations: numerators are one f16 part, where everything else is as exact as the f16 inputs.  Results are off by 2.5e-4
+// to 2.8e-4 of their size, of which their own rounding is 2.1e-4.  A second part for them leaves that rounding alone and takes
+// 30 to 36 % more: those 256 chats 455 us for 350, the chunks of nine prompts 851 for 628.
 template <int HD, typename X, typename KV>
 struct PagedShape {
   static constexpr bool TWOQ = sizeof(X) == 4, TWOK = sizeof(KV) == 4;

@@ -106,10 +106,13 @@ static PagedPlan paged_plan(const jero_paged_cache* k, bool f16, int64_t n_token
   const int64_t rows = n_tokens * group, each = (n_tokens + k->n_seqs - 1) / k->n_seqs * group;
   p.wide_rows = hd <= 128 && k->kv_dtype == JERO_KV_F16 ? 128 : 64;
   // Rows of all sequences go over the shared positions together where sequences do not fill tiles themselves and more than
-  // 48 MB (24 of f32, whose rows cost more than their bytes) are spared: 32 sequences x 256 shared positions x 8 heads of
-  // 128 (f16, 33 MB) 26 us and 30 apart and not, 8 x 1024 (29 MB) 24 and 19, 128 x 64 (33 MB) 60 and 55, 128 x 256
-  // (133 MB) 59 and 61, 8 x 4096 (117 MB) 30 and 32, 128 x 4096 69 and 192; f32: 16 x 256 (31 MB) the same, 16 x 1024
-  // 34 and 58.  Not where the two parts of all rows would take more than 4 GiB.
+  // 48 MB (24 of f32, whose rows cost more than their bytes) are spared.  Single tokens of 8, 32 and 128 sequences, 50 to 300
+  // positions of their own, 8 heads of 128, f16, us apart and not: at 24 MB 15 and 14, 16 and 16, (33 MB) 29 and 25; at 48
+  // MB 15 and 16, 16 and 18, (67) 30 and 28; at 160 MB 18 and 25, 18 and 26, 31 and 33.  Heads of 64 are even later, at 50 to
+  // 160 MB.  An f32 cache: 25 and 20 (26 MB), 25 and 28 (33 MB), 55 and 53 (67 MB); at 160 MB 27 and 38, 28 and 40, (133) 57
+  // and 62; of 45 calls drawn over all sizes the time not apart is 0.95 of that apart on average below 24 MB (0.59 to 1.21), 1.02
+  // from 24 to 48 (0.69 to 1.23), 1.21 above (0.97 to 1.67).  128 x 4096 shared positions: 69 and 192.  Not where the two
+  // parts of all rows would take more than 4 GiB.
   const double pair = 2.0 * kv * k->head_dim * (k->kv_dtype == JERO_KV_F16 ? 2 : 4);  // bytes of a position
   const double spared = double(k->n_seqs - 1) * shared * pair;
   const bool apart = k->n_seqs > 1 && each < p.wide_rows && spared >= (k->kv_dtype == JERO_KV_F16 ? 48e6 : 24e6) &&
@@ -118,8 +121,12 @@ static PagedPlan paged_plan(const jero_paged_cache* k, bool f16, int64_t n_token
   // of 128, 32, 48, 64 and 96 rows each: f16 36, 41, 43 and 44 us wide, 37, 41, 46 and 65 by 16; f32 over f16 48, 56, 61 and
   // 64, and 39, 42, 48 and 66; f32 68, 68, 85 and 85, and 74, 91, 98 and 132.  Heads of 256, whose narrow tiles are one a CU,
   // 24 and 48 rows: f32 over f16 43 and 50 wide, 49 and 59 by 16; heads of 64, 48 and 80: 28 and 31, and 16 and 22.
-  // Where wide tiles alone are two workgroups a CU they pay from 17 rows on (74 sequences, 8 heads of 80, 24, 40 and 80 rows
-  // over 128 positions behind 736 shared: f32 over f16 43, 60 and 83 us wide, 49, 71 and 123 by 16).
+  // Where wide tiles alone are two workgroups a CU they are taken from 17 rows on (74 sequences, 8 heads of 80, 24, 40 and 80
+  // rows over 128 positions behind 736 shared: f32 over f16 43, 60 and 83 us wide, 49, 71 and 123 by 16).  74 sequences of 50
+  // to 700, 8 heads, 20, 32 and 48 rows, wide and by 16: heads of 64 f16 31, 35, 36 and 29, 32, 49, f32 over f32 41, 45, 45
+  // and 40, 47, 72; of 128 f16 44, 45, 47 and 42, 48, 77, f32 70, 75, 73 and 91, 102, 161; of 256 f16 79, 80, 88 and 96, 112,
+  // 194.  f32 over f16 would want narrow tiles up to 32 rows there: heads of 64 40, 45, 45 and 26, 27, 41, of 128 67, 64, 63
+  // and 45, 49, 77 (200 sequences 124, 128, 123 and 115, 124, 200); only heads of 256 have 100, 95, 88 and 116, 128, 209.
   const bool many = k->n_seqs * kv >= 512;
   p.own_wide = each > (many || hd == 256 ? kNarrowRows : hd == 64 ? 80 : f16 ? 48 : k->kv_dtype == JERO_KV_F16 ? 95 : 31);
   p.own_lo = apart ? int(shared) : 0;
